@@ -1,0 +1,261 @@
+// Host side of the output projection with softmax cross entropy: argument checks, the plan of the backward (pieces of the
+// vocabulary, splits), workspaces, and the autograd node.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+
+#include "host_common.h"
+#include "linear_loss.h"
+#include "train_ops.h"
+
+namespace sep {
+
+namespace {
+
+int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// One dz buffer holds at most about this much.  Larger pieces mean fewer passes over the fp32 sums of dx.
+constexpr int64_t kPieceBytes = 128ll << 20;
+constexpr int64_t kBandBytes = 48ll << 20;       // rows of x that a band of units shares in L2
+
+void plan_backward(LossParams& p, int sms) {
+  const int64_t T = p.T, H = p.H, V = p.V, pairs = sms / 2;
+  p.row_units = static_cast<int>(ceil_of(T, kLossUnit));
+  p.h_units = static_cast<int>(ceil_of(H, kLossUnit));
+  // Short calls keep dz to 16 bits of mantissa, as a sum of two bf16 numbers: rounding errors of many tokens average out in dW,
+  // those of a few do not (one token, target at p = 0.5: dW 0.4 % off where the result's own rounding is 0.2 %).  The remainders sit
+  // where the second CTA's rows of a unit would be empty, so they cost no further products.
+  p.split2 = T <= kLossPart ? 1 : 0;
+  const int64_t row_bytes = T * 2 * (p.split2 ? 2 : 1);
+  // at least four pieces where they have a few tiles each, so that products of one piece overlap the dz of the next
+  const int64_t want = std::max(ceil_of(V * row_bytes, kPieceBytes), std::min<int64_t>(4, ceil_of(V, 2048)));
+  p.piece = static_cast<int>(ceil_of(ceil_of(V, want), kLossUnit) * kLossUnit);
+  p.pieces = static_cast<int>(ceil_of(V, p.piece));
+  p.last_cols = static_cast<int>(V - static_cast<int64_t>(p.pieces - 1) * p.piece);
+  p.ahead = std::min(1, p.pieces);
+  p.buffers = std::min(p.ahead + 1, p.pieces);
+  // dx units of one place follow each other piece by piece: a chain of V / 64 / splits k-blocks, which is to stay within half of the
+  // time that the whole work takes on all pairs.
+  const int64_t v_blocks = ceil_of(V, 64), tiles = ceil_of(V, kLossUnit);
+  const int64_t all = (p.row_units * tiles * ceil_of(H, 64) + (p.want_dx ? p.row_units * p.h_units * v_blocks : 0) +
+                       (p.want_dw ? tiles * p.h_units * ceil_of(T, 64) : 0)) / pairs + 1;
+  const int64_t piece_blocks = ceil_of(std::min<int64_t>(V, p.piece), 64);
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min({ceil_of(2 * v_blocks, all), piece_blocks / 4, static_cast<int64_t>(64)})));
+  p.split_blocks = static_cast<int>(ceil_of(piece_blocks, p.splits));
+  p.splits = static_cast<int>(ceil_of(piece_blocks, p.split_blocks));
+}
+void plan_band(LossParams& p) {
+  const int64_t rows = std::max<int64_t>(kBandBytes / (2 * static_cast<int64_t>(p.H)), kLossUnit);
+  p.row_units = static_cast<int>(ceil_of(p.T, kLossUnit));
+  // bands of equal height
+  const int64_t bands = ceil_of(p.row_units, std::max<int64_t>(rows / kLossUnit, 1));
+  p.band = static_cast<int>(ceil_of(p.row_units, bands));
+}
+
+// [rows, cols] bf16 with rows 16 bytes apart at least, as TMA reads them; a copy where they are not.
+at::Tensor readable(const at::Tensor& t) {
+  const bool fits = t.stride(1) == 1 && is_aligned(t) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1)));
+  if (fits) return t;
+  return aligned_rows(t.contiguous());
+}
+int64_t pitch(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+// Places in one workspace, 256 bytes apart.
+struct Carver {
+  int64_t bytes = 0;
+  int64_t take(int64_t n) { const int64_t at = bytes; bytes += ceil_of(std::max<int64_t>(n, 1), 256) * 256; return at; }
+};
+
+struct LossCall : torch::CustomClassHolder {
+  ContextFn context;
+  int64_t ignore_index;
+  int reduction;
+};
+
+struct Forward { at::Tensor loss, lse, inv_count; };
+
+Forward loss_forward(const LossCall& call, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets) {
+  const int64_t T = x.size(0), H = x.size(1), V = w.size(0);
+  const auto f32 = x.options().dtype(at::kFloat);
+  const bool reduced = call.reduction != kLossNone;
+  Forward out;
+  out.lse = at::empty({T}, f32);
+  out.inv_count = at::empty({1}, f32);
+  if (T == 0) {
+    out.loss = reduced ? at::full({}, call.reduction == kLossMean ? std::numeric_limits<float>::quiet_NaN() : 0.0, f32) : at::empty({0}, f32);
+    out.inv_count.zero_();
+    return out;
+  }
+  out.loss = reduced ? at::empty({}, f32) : at::empty({T}, f32);
+  const int64_t parts = ceil_of(V, kLossPart);
+  Carver c;
+  const int64_t counters = c.take(64), part_at = c.take(parts * T * 8), logit_at = c.take(T * 4), each_at = reduced ? c.take(T * 4) : 0;
+  const at::Tensor space = at::empty({c.bytes}, x.options().dtype(at::kByte));
+  char* base = static_cast<char*>(space.data_ptr());
+  const LaunchContext ctx = call.context(2);
+
+  LossParams p{};
+  p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
+  plan_band(p);
+  p.parts = reinterpret_cast<float2*>(base + part_at);
+  p.target_logit = reinterpret_cast<float*>(base + logit_at);
+  p.targets = reinterpret_cast<const long long*>(targets.data_ptr<int64_t>());
+  p.ignore_index = call.ignore_index;
+  p.claim = reinterpret_cast<int*>(base + counters);
+  p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
+  LossMaps m{};
+  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, 128);
+  m.w_k = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 128);
+  SEP_CUDA_CHECK(cudaMemsetAsync(base + counters, 0, 64, ctx.stream));
+  SEP_CUDA_CHECK(launch_loss_forward(p, m, ctx.sms, ctx.stream));
+
+  LossFinalParams f{};
+  f.T = p.T; f.V = p.V; f.num_parts = static_cast<int>(parts);
+  f.parts = p.parts; f.target_logit = p.target_logit; f.targets = p.targets; f.ignore_index = p.ignore_index;
+  f.mean = call.reduction == kLossMean; f.sum = call.reduction == kLossSum;
+  f.each = reduced ? reinterpret_cast<float*>(base + each_at) : out.loss.data_ptr<float>();
+  f.lse = out.lse.data_ptr<float>();
+  f.loss = reduced ? out.loss.data_ptr<float>() : nullptr;
+  f.inv_count = out.inv_count.data_ptr<float>();
+  f.ticket = p.claim + 1;
+  f.status = ctx.status; f.rank = ctx.rank;
+  SEP_CUDA_CHECK(launch_loss_final(f, ctx.stream));
+  return out;
+}
+
+std::pair<at::Tensor, at::Tensor> loss_backward(const LossCall& call, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
+                                                const at::Tensor& lse, const at::Tensor& inv_count, const at::Tensor& upstream,
+                                                bool want_dx, bool want_dw) {
+  const int64_t T = x.size(0), H = x.size(1), V = w.size(0);
+  at::Tensor dx, dw;
+  if (T == 0) {
+    if (want_dx) dx = at::empty({0, H}, x.options());
+    if (want_dw) dw = at::zeros({V, H}, w.options());
+    return {dx, dw};
+  }
+  if (want_dx) dx = at::empty({T, H}, x.options());
+  if (want_dw) dw = at::empty({V, H}, w.options());
+  const LaunchContext ctx = call.context(want_dx ? 2 : 1);
+  const at::Tensor up = upstream.to(at::kFloat).contiguous();
+
+  LossParams p{};
+  p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
+  p.want_dx = want_dx; p.want_dw = want_dw;
+  plan_backward(p, ctx.sms);
+  plan_band(p);
+  SEP_ASSERT(loss_backward_units(p) < (1ll << 30), "this loss has too many tiles for one call: split the tokens");
+  const int64_t z_layers = p.split2 ? 2 : 1, slots = static_cast<int64_t>(p.splits) * z_layers;
+  const int64_t counters = 4 * (4 + 3 * static_cast<int64_t>(p.pieces));
+  Carver c;
+  const int64_t count_at = c.take(counters), z_at = c.take(p.buffers * z_layers * T * p.piece * 2);
+  const int64_t dx_at = want_dx ? c.take(slots * T * H * 4) : 0;
+  const at::Tensor space = at::empty({c.bytes}, x.options().dtype(at::kByte));
+  char* base = static_cast<char*>(space.data_ptr());
+  p.targets = reinterpret_cast<const long long*>(targets.data_ptr<int64_t>());
+  p.ignore_index = call.ignore_index;
+  p.lse = lse.data_ptr<float>();
+  if (call.reduction == kLossNone) p.row_scale = up.data_ptr<float>();
+  else p.scale = up.data_ptr<float>();
+  if (call.reduction == kLossMean) p.scale2 = inv_count.data_ptr<float>();
+  p.claim = reinterpret_cast<int*>(base + count_at);
+  p.done = p.claim + 4;
+  p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
+
+  LossMaps m{};
+  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, 128);
+  m.x_mn = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, 64);
+  m.w_k = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 128);
+  m.w_mn = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 64);
+  for (int i = 0; i < 2; ++i) {
+    // of the last piece only the columns that exist (up to whole 16 bytes, zeros in between) are stored and read back
+    const int64_t cols = i == 0 ? p.piece : ceil_of(p.last_cols, 8) * 8, layers = p.buffers * z_layers;
+    m.z_k[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, 128);
+    m.z_mn[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, 64);
+    m.z_out[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, 32);
+  }
+  if (want_dw) m.dw = make_tmap(dw.data_ptr(), H, V, 1, H, H * V, 64, 32);
+  if (want_dx) m.dx = make_tmap(base + dx_at, H, T, slots, H, T * H, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
+  SEP_CUDA_CHECK(cudaMemsetAsync(base + count_at, 0, counters, ctx.stream));
+  SEP_CUDA_CHECK(launch_loss_backward(p, m, ctx.sms, ctx.stream));
+  if (want_dx) {
+    LossDxParams d{};
+    d.T = p.T; d.H = p.H; d.slots = static_cast<int>(slots);
+    d.parts = reinterpret_cast<const float*>(base + dx_at);
+    d.scale = p.scale; d.scale2 = p.scale2;
+    d.dx = dx.data_ptr();
+    SEP_CUDA_CHECK(launch_loss_dx(d, ctx.stream));
+  }
+  return {dx, dw};
+}
+
+class LinearLoss : public torch::autograd::Function<LinearLoss> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets,
+                            const c10::intrusive_ptr<LossCall>& call) {
+    const at::Tensor xr = readable(x), wr = readable(weight), y = targets.contiguous();
+    Forward f = loss_forward(*call, xr, wr, y);
+    ctx->save_for_backward({x, weight, targets, f.lse, f.inv_count});
+    ctx->saved_data["call"] = c10::IValue::make_capsule(call);
+    return f.loss;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    SEP_ASSERT(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative: its backward was asked for a graph");
+    auto call = c10::static_intrusive_pointer_cast<LossCall>(ctx->saved_data["call"].toCapsule());
+    const auto saved = ctx->get_saved_variables();
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    const c10::cuda::CUDAGuard guard(saved[0].device());
+    // A thread of the autograd engine may not have made a call of the CUDA runtime yet, and the driver encodes tensor maps only
+    // with a context bound to the thread.
+    SEP_CUDA_CHECK(cudaSetDevice(saved[0].get_device()));
+    auto g = loss_backward(*call, readable(saved[0]), readable(saved[1]), saved[2].contiguous(), saved[3], saved[4], grads[0],
+                           ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    return {g.first, g.second, at::Tensor(), at::Tensor()};
+  }
+};
+
+}  // namespace
+
+at::Tensor linear_loss(const ContextFn& context, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets,
+                       int64_t ignore_index, int reduction) {
+  SEP_ASSERT(x.is_cuda() && x.dim() == 2 && x.scalar_type() == at::kBFloat16, "x must be a [..., H] bf16 CUDA tensor");
+  SEP_ASSERT(weight.dim() == 2 && weight.scalar_type() == at::kBFloat16 && weight.device() == x.device() && weight.size(1) == x.size(1),
+             "weight must be a [V, H] bf16 tensor on the device of x");
+  SEP_ASSERT(targets.dim() == 1 && targets.scalar_type() == at::kLong && targets.device() == x.device() && targets.size(0) == x.size(0),
+             "targets must be int64, one for each row of x, on its device");
+  SEP_ASSERT(x.size(1) > 0 && x.size(1) % 8 == 0, "hidden must be a positive multiple of 8");
+  SEP_ASSERT(weight.size(0) >= 1, "the vocabulary is empty");
+  SEP_ASSERT(x.size(0) < (1ll << 30) && weight.size(0) < (1ll << 30) && x.size(1) < (1ll << 30) &&
+                 ceil_of(x.size(0), kLossUnit) * ceil_of(weight.size(0), kLossUnit) < (1ll << 30),
+             "this loss has too many tiles for one call: split the tokens");
+  SEP_ASSERT(reduction >= kLossNone && reduction <= kLossSum, "unknown reduction");
+  SEP_ASSERT(!x._fw_grad(0).defined() && !weight._fw_grad(0).defined(), "linear_cross_entropy has no forward-mode derivative");
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto call = c10::make_intrusive<LossCall>();
+  call->context = context;
+  call->ignore_index = ignore_index;
+  call->reduction = reduction;
+  SEP_ASSERT(context(0).device == x.get_device(), "x is not on the device of the buffer that this call reports into");
+  if (!(at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad())))
+    return loss_forward(*call, readable(x), readable(weight), targets.contiguous()).loss;
+  return LinearLoss::apply(x, weight, targets, call);
+}
+
+std::vector<std::vector<int>> linear_loss_schedule(int64_t tokens, int64_t hidden, int64_t vocab, int sms, bool want_dx, bool want_dw) {
+  LossParams p{};
+  p.T = static_cast<int>(tokens); p.H = static_cast<int>(hidden); p.V = static_cast<int>(vocab);
+  p.want_dx = want_dx; p.want_dw = want_dw;
+  plan_backward(p, sms);
+  plan_band(p);
+  std::vector<std::vector<int>> out = {{p.pieces, p.piece, p.splits, p.ahead, p.buffers, p.row_units, p.split2}};
+  const long long units = loss_backward_units(p);
+  for (long long i = 0; i < units; ++i) {
+    int v[7];
+    loss_backward_unit(p, static_cast<int>(i), v);
+    out.emplace_back(v, v + 7);
+  }
+  return out;
+}
+
+}  // namespace sep

@@ -1,0 +1,85 @@
+// Host <-> kernel interface of the output projection with softmax cross entropy (linear_loss_kernels.cu).
+#pragma once
+
+#include <cuda.h>
+
+#include "api.h"
+
+namespace sep {
+
+constexpr int kLossUnit = 256;        // rows and columns of a unit of work: one tile of a CTA pair
+constexpr int kLossPart = 128;        // columns that one thread reduces: the softmax statistics come in parts of this many
+
+// Kinds of work.  Forward: kLossStats.  Backward, for each piece of the vocabulary: kLossDz, then kLossDx and kLossDw.
+enum LossKind : int { kLossStats = 0, kLossDz = 1, kLossDx = 2, kLossDw = 3 };
+
+struct LossParams {
+  int T, H, V;
+  int num_pairs;                 // CTA pairs of the launch
+  int row_units;                 // ceil(T / 256)
+  int band;                      // row units that are walked together (see unit_of)
+  // --- forward ---
+  float2* parts;                 // [ceil(V / 128)][T] running maximum and sum of exp(z - maximum) of 128 columns
+  float* target_logit;           // [T]
+  const long long* targets;      // [T]
+  long long ignore_index;
+  // --- backward ---
+  const float* lse;              // [T] log of the softmax denominator
+  const float* row_scale;        // [T] upstream gradient of each token's loss, or null: 1
+  const float* scale;            // [1] factor of every gradient, or null: 1 ...
+  const float* scale2;           // [1] ... and another (1 / counted tokens)
+  int piece;                     // columns of a piece, a multiple of 256
+  int pieces, last_cols;         // how many, and the columns of the last
+  int ahead;                     // pieces whose dz is computed before the first product is taken from one
+  int buffers;                   // dz buffers in rotation, > ahead
+  int split2;                    // 1: dz is kept as the sum of two bf16 numbers (short calls)
+  int want_dx, want_dw;
+  int splits;                    // reductions over a piece of the vocabulary into which a dx unit is split
+  int split_blocks;              // k-blocks of each but the last
+  int h_units;                   // ceil(H / 256)
+  int* claim;                    // next unit; zero on entry
+  int* done;                     // [3][pieces] epilogue warps that have finished dz / dx / dw units; zero on entry
+  StatusBlock* status;
+  int rank;
+  unsigned long long wait_budget_ns;
+};
+
+struct LossMaps {                // CUtensorMap each: loads in boxes of 64 columns by 128 (k: K-major) or 64 (mn) rows
+  CUtensorMap x_k, x_mn, w_k, w_mn;
+  CUtensorMap z_k[2], z_mn[2], z_out[2];    // [0] full pieces, [1] the last one
+  CUtensorMap dw, dx;
+};
+
+cudaError_t launch_loss_forward(const LossParams& p, const LossMaps& m, int sms, cudaStream_t stream);
+cudaError_t launch_loss_backward(const LossParams& p, const LossMaps& m, int sms, cudaStream_t stream);
+long long loss_backward_units(const LossParams& p);
+// {kind, piece, unit row, unit column, split, first k-block, k-blocks} of backward unit `lin`
+void loss_backward_unit(const LossParams& p, int lin, int (&out)[7]);
+
+struct LossFinalParams {
+  int T, V, num_parts;
+  const float2* parts;
+  const float* target_logit;
+  const long long* targets;
+  long long ignore_index;
+  int mean, sum;                 // reduction (neither: per token)
+  float* each;                   // [T] losses (scratch where they are reduced)
+  float* lse;                    // [T]
+  float* loss;                   // [1] where they are reduced
+  float* inv_count;              // [1] 1 / counted tokens (mean; 0 without any)
+  int* ticket;                   // [1], zero on entry
+  StatusBlock* status;
+  int rank;
+};
+cudaError_t launch_loss_final(const LossFinalParams& p, cudaStream_t stream);
+
+struct LossDxParams {
+  int T, H, slots;
+  const float* parts;            // [slots][T][H]
+  const float* scale;            // as in LossParams
+  const float* scale2;
+  void* dx;                      // [T, H] bf16
+};
+cudaError_t launch_loss_dx(const LossDxParams& p, cudaStream_t stream);
+
+}  // namespace sep

@@ -24,72 +24,14 @@
 
 #include "api.h"
 #include "arena.h"
+#include "host_common.h"
+#include "train_ops.h"
 
 namespace py = pybind11;
 
 namespace sep {
 
-#define SEP_CUDA_CHECK(expr)                                                                        \
-  do {                                                                                              \
-    cudaError_t e__ = (expr);                                                                       \
-    if (e__ != cudaSuccess) {                                                                       \
-      std::ostringstream os__;                                                                      \
-      os__ << "CUDA error " << cudaGetErrorName(e__) << " (" << cudaGetErrorString(e__) << ") at "  \
-           << __FILE__ << ":" << __LINE__ << " in " #expr;                                          \
-      throw std::runtime_error(os__.str());                                                         \
-    }                                                                                               \
-  } while (0)
-
-#define SEP_ASSERT(cond, msg)                                                         \
-  do {                                                                                \
-    if (!(cond)) {                                                                    \
-      std::ostringstream os__;                                                        \
-      os__ << "streamep_b200: " << msg << " (" #cond ") at " << __FILE__ << ":" << __LINE__; \
-      throw std::invalid_argument(os__.str());                                        \
-    }                                                                                 \
-  } while (0)
-
-// ---------------------------------------------------------------------------------------------
-// Driver entry points fetched at run time (the extension does not link libcuda).
-// ---------------------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 using StreamWaitValue32Fn = CUresult (*)(CUstream, CUdeviceptr, cuuint32_t, unsigned int);
-
-template <class Fn>
-static Fn driver_fn(const char* name) {
-  void* fn = nullptr;
-  cudaDriverEntryPointQueryResult q;
-  SEP_CUDA_CHECK(cudaGetDriverEntryPoint(name, &fn, cudaEnableDefault, &q));
-  if (q != cudaDriverEntryPointSuccess || fn == nullptr)
-    throw std::runtime_error(std::string("streamep_b200: driver entry point not found: ") + name);
-  return reinterpret_cast<Fn>(fn);
-}
-
-// 3-D bf16 tensor map, 128-byte swizzle, OOB reads return zero.  dims/box are innermost-first.
-static CUtensorMap make_tmap(const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1_elems,
-                             uint64_t stride2_elems, uint32_t b0, uint32_t b1,
-                             CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
-  static EncodeTiledFn encode = driver_fn<EncodeTiledFn>("cuTensorMapEncodeTiled");
-  CUtensorMap m;
-  cuuint64_t dims[3] = {d0, d1, d2};
-  cuuint64_t strides[2] = {stride1_elems * 2, stride2_elems * 2};
-  cuuint32_t box[3] = {b0, b1, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  SEP_ASSERT(reinterpret_cast<uintptr_t>(base) % 16 == 0, "TMA base address must be 16-byte aligned");
-  SEP_ASSERT(strides[0] % 16 == 0 && strides[1] % 16 == 0, "TMA row pitch must be a multiple of 16 bytes");
-  CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) throw std::runtime_error("streamep_b200: cuTensorMapEncodeTiled failed with code " + std::to_string(r));
-  return m;
-}
-
-// Rows are read 16 bytes at a time.  A contiguous tensor may still start anywhere (a view of a flat buffer at an odd element,
-// the gradient of an output that was concatenated behind something): such rows are copied to an aligned place first.
-static bool is_aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
-static at::Tensor aligned_rows(const at::Tensor& t) { return !t.is_contiguous() || is_aligned(t) ? t : t.clone(); }
 
 // ---------------------------------------------------------------------------------------------
 // Peer-shareable device memory through the virtual-memory-management driver API: cuMemCreate with a POSIX file
@@ -791,9 +733,10 @@ class Runtime : public std::enable_shared_from_this<Runtime> {
     static const char* names[] = {"ok", "barrier timeout", "buffer-record timeout", "tile gate timeout",
                                   "token gate timeout", "GEMM pipeline timeout", "tail wait timeout", "bad index",
                                   "capacity overflow (where = region, expected = tile capacity, observed = tiles needed; the dispatch was run as an empty one)",
-                                  "ranks disagree on the capacity-mode region of a dispatch"};
+                                  "ranks disagree on the capacity-mode region of a dispatch",
+                                  "target outside the vocabulary (where = token, expected = vocabulary, observed = target; its loss and the gradients are NaN)"};
     std::ostringstream os;
-    os << names[(h.code >= 0 && h.code < 10) ? h.code : 0] << " (code " << h.code << ") in kernel " << h.kernel_id
+    os << names[(h.code >= 0 && h.code < 11) ? h.code : 0] << " (code " << h.code << ") in kernel " << h.kernel_id
        << " role " << h.role << " on rank " << h.rank << ": where=" << h.where << " expected=" << h.expected
        << " observed=" << h.observed;
     return os.str();
@@ -1946,6 +1889,12 @@ class Runtime : public std::enable_shared_from_this<Runtime> {
     SEP_CUDA_CHECK(cudaGetLastError());
     return {idx, w, in_rank, probs};
   }
+  // What the operators around the layer need for a launch into the current stream.
+  LaunchContext launch_context(int launches) {
+    check_alive();
+    launches_ += launches;
+    return {status_, budget_ns_, rank_, num_sms(), device_, stream()};
+  }
   // {tokens per tile, CTAs that share the hidden dimension, pipeline stages} of the tensor-core router for a shape
   std::vector<int> router_plan(int tokens, int hidden, int experts) {
     RouterParams p{};
@@ -2288,5 +2237,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
            py::arg("dw_src") = std::nullopt, py::arg("dw_dst") = std::nullopt, py::arg("sizes") = std::nullopt)
       .def("pool_compress", &Runtime::pool_compress)
       .def("pool_expand", &Runtime::pool_expand)
-      .def("router", &Runtime::router);
+      .def("router", &Runtime::router)
+      .def("linear_loss", [](const std::shared_ptr<Runtime>& r, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets,
+                             int64_t ignore_index, int reduction) {
+        return linear_loss([r](int launches) { return r->launch_context(launches); }, x, weight, targets, ignore_index, reduction);
+      });
+  m.def("linear_loss_schedule", &linear_loss_schedule);
 }

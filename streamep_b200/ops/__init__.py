@@ -1,13 +1,16 @@
 """Python entry points of the native kernels (lazy: importing the package does not load the extension)."""
 import importlib
 
+_MODULES = ("grouped_gemm", "linear_loss")
+
 
 def __getattr__(name):
     if name.startswith("__"):
         raise AttributeError(name)
-    mod = importlib.import_module(__name__ + ".grouped_gemm")
-    if name == "grouped_gemm":
-        return mod
-    if hasattr(mod, name):
-        return getattr(mod, name)
+    if name in _MODULES:
+        return importlib.import_module(f"{__name__}.{name}")
+    for module in _MODULES:
+        mod = importlib.import_module(f"{__name__}.{module}")
+        if hasattr(mod, name):
+            return getattr(mod, name)
     raise AttributeError(name)
