@@ -2243,4 +2243,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return linear_loss([r](int launches) { return r->launch_context(launches); }, x, weight, targets, ignore_index, reduction);
       });
   m.def("linear_loss_schedule", &linear_loss_schedule);
+  m.def("list_norm", &list_norm);
+  m.def("list_clip", &list_clip);
+  m.def("list_scale", &list_scale);
+  m.def("list_adamw", [](const TensorList& params, const TensorList& grads, const TensorList& exp_avgs, const TensorList& exp_avg_sqs, const TensorList& masters,
+                         const std::optional<at::Tensor>& norm, int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
+                         double max_norm, bool skip_nonfinite) {
+    list_adamw(params, grads, exp_avgs, exp_avg_sqs, masters, norm, AdamOptions{step, lr, beta1, beta2, eps, weight_decay, max_norm, skip_nonfinite});
+  });
 }

@@ -1,8 +1,11 @@
-// Operators of a training step around the MoE layer, host side: the loss over the vocabulary (linear_loss.cpp).
+// Operators of a training step around the MoE layer, host side: the loss over the vocabulary (linear_loss.cpp), and lists
+// of tensors (list_ops.cpp): gradients' norm and clipping, AdamW.
 #pragma once
 
 #include <functional>
+#include <optional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include <cuda_runtime.h>
@@ -28,5 +31,19 @@ at::Tensor linear_loss(const ContextFn& context, const at::Tensor& x, const at::
 // The backward's units in order, for the schedule's test: each {kind, piece, unit row, unit column, split, first k-block, k-blocks};
 // first of all {pieces, columns of a piece, splits, ahead, buffers, row units, split2}.
 std::vector<std::vector<int>> linear_loss_schedule(int64_t tokens, int64_t hidden, int64_t vocab, int sms, bool want_dx, bool want_dw);
+
+using TensorList = std::vector<at::Tensor>;
+// {norm (fp32), sum of squares (fp64)}, 0-dim
+std::pair<at::Tensor, at::Tensor> list_norm(const TensorList& tensors);
+at::Tensor list_clip(const TensorList& tensors, double max_norm);
+void list_scale(const TensorList& tensors, const at::Tensor& norm, double max_norm);
+struct AdamOptions {
+  int64_t step;
+  double lr, beta1, beta2, eps, weight_decay;
+  double max_norm;               // < 0: no clipping
+  bool skip_nonfinite;
+};
+void list_adamw(const TensorList& params, const TensorList& grads, const TensorList& exp_avgs, const TensorList& exp_avg_sqs,
+                const TensorList& masters, const std::optional<at::Tensor>& norm, const AdamOptions& o);
 
 }  // namespace sep
