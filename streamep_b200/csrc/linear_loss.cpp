@@ -18,6 +18,7 @@ int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // One dz buffer holds at most about this much.  Larger pieces mean fewer passes over the fp32 sums of dx.
 constexpr int64_t kPieceBytes = 128ll << 20;
+constexpr int64_t kSplitTokens = 64;             // calls whose dz is kept as a sum of two bf16 numbers: one k-block of tokens
 constexpr int64_t kBandBytes = 48ll << 20;       // rows of x that a band of units shares in L2
 
 void plan_backward(LossParams& p, int sms) {
@@ -27,28 +28,42 @@ void plan_backward(LossParams& p, int sms) {
   // Short calls keep dz to 16 bits of mantissa, as a sum of two bf16 numbers: rounding errors of many tokens average out in dW,
   // those of a few do not (one token, target at p = 0.5: dW 0.4 % off where the result's own rounding is 0.2 %).  The remainders sit
   // where the second CTA's rows of a unit would be empty, so they cost no further products.
-  p.split2 = T <= kLossPart ? 1 : 0;
+  p.split2 = T <= kSplitTokens ? 1 : 0;
   const int64_t row_bytes = T * 2 * (p.split2 ? 2 : 1);
-  // at least four pieces where they have a few tiles each, so that products of one piece overlap the dz of the next
-  const int64_t want = std::max(ceil_of(V * row_bytes, kPieceBytes), std::min<int64_t>(4, ceil_of(V, 2048)));
+  const int64_t want = ceil_of(V * row_bytes, kPieceBytes);
   p.piece = static_cast<int>(ceil_of(ceil_of(V, want), kLossUnit) * kLossUnit);
   p.pieces = static_cast<int>(ceil_of(V, p.piece));
   p.last_cols = static_cast<int>(V - static_cast<int64_t>(p.pieces - 1) * p.piece);
   p.ahead = std::min(1, p.pieces);
   p.buffers = std::min(p.ahead + 1, p.pieces);
-  // dx units of one place follow each other piece by piece: a chain of V / 64 / splits k-blocks, which is to stay within half of the
-  // time that the whole work takes on all pairs.
-  const int64_t v_blocks = ceil_of(V, 64), tiles = ceil_of(V, kLossUnit);
+  // A single piece: nothing but its dz stands before its products, and dw units can begin on the first finished column tiles.
+  p.dw_first = p.pieces == 1 ? 1 : 0;
+  const int64_t v_blocks = ceil_of(V, 64), t_blocks = ceil_of(T, 64) * (p.split2 ? 2 : 1), tiles = ceil_of(V, kLossUnit);
+  // k-blocks of all the work, for each pair
   const int64_t all = (p.row_units * tiles * ceil_of(H, 64) + (p.want_dx ? p.row_units * p.h_units * v_blocks : 0) +
-                       (p.want_dw ? tiles * p.h_units * ceil_of(T, 64) : 0)) / pairs + 1;
+                       (p.want_dw ? tiles * p.h_units * t_blocks : 0)) / pairs + 1;
+  // dx units of one place follow each other piece by piece: a chain of v_blocks / splits k-blocks, which is to stay within half of the
+  // time that the whole takes; and a unit within an eighth of it, so that pairs end together.
   const int64_t piece_blocks = ceil_of(std::min<int64_t>(V, p.piece), 64);
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min({ceil_of(2 * v_blocks, all), piece_blocks / 4, static_cast<int64_t>(64)})));
+  // But no more than keep the traffic of the partial sums (4 bytes, written and read) within an eighth of reading the projection.
+  const int64_t chain = ceil_of(2 * v_blocks, all), even = std::min(ceil_of(8 * piece_blocks, all), V / (32 * T * (p.split2 ? 2 : 1)));
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min({std::max(chain, even), piece_blocks / 4, static_cast<int64_t>(64)})));
   p.split_blocks = static_cast<int>(ceil_of(piece_blocks, p.splits));
   p.splits = static_cast<int>(ceil_of(piece_blocks, p.split_blocks));
+  // dw units of few k-blocks take several column tiles, as long as there are a few units for every pair: claiming one and asking
+  // whether its dz is there takes longer than its products.
+  const int64_t per_pair = tiles * p.h_units / pairs;
+  p.dw_group = static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(p.h_units), 24 / t_blocks, per_pair / 4})));
+}
+// Units of few k-blocks are claimed further ahead: a claim takes about as long as the operands of four k-blocks.
+int claim_lead(const LossParams& p, bool backward) {
+  const int64_t shortest = std::min<int64_t>(ceil_of(p.H, 64), backward ? ceil_of(p.T, 64) : 1 << 20);
+  return shortest <= 8 ? 2 : 0;
 }
 void plan_band(LossParams& p) {
   const int64_t rows = std::max<int64_t>(kBandBytes / (2 * static_cast<int64_t>(p.H)), kLossUnit);
   p.row_units = static_cast<int>(ceil_of(p.T, kLossUnit));
+  p.x_rows = static_cast<int>(std::min<int64_t>(128, ceil_of(p.T, 8) * 8));
   // bands of equal height
   const int64_t bands = ceil_of(p.row_units, std::max<int64_t>(rows / kLossUnit, 1));
   p.band = static_cast<int>(ceil_of(p.row_units, bands));
@@ -72,43 +87,68 @@ struct LossCall : torch::CustomClassHolder {
   ContextFn context;
   int64_t ignore_index;
   int reduction;
+  bool want_dx = false, want_dw = false;
+  at::Tensor counters;           // of the backward's kernel, cleared by the forward's
+  bool counters_used = false;    // a backward has run (with retain_graph another may follow)
 };
 
-struct Forward { at::Tensor loss, lse, inv_count; };
+// the loss; and [T] log-denominators followed by 1 / counted tokens
+struct Forward { at::Tensor loss, stats; };
 
-Forward loss_forward(const LossCall& call, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets) {
+LossParams plan(int64_t T, int64_t H, int64_t V, bool want_dx, bool want_dw, int sms) {
+  LossParams p{};
+  p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
+  p.want_dx = want_dx; p.want_dw = want_dw;
+  plan_backward(p, sms);
+  plan_band(p);
+  p.claim_lead = claim_lead(p, true);
+  return p;
+}
+int64_t counter_ints(const LossParams& p) { return 4 + (3 + p.piece / kLossUnit) * static_cast<int64_t>(p.pieces); }
+
+Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets) {
   const int64_t T = x.size(0), H = x.size(1), V = w.size(0);
   const auto f32 = x.options().dtype(at::kFloat);
   const bool reduced = call.reduction != kLossNone;
   Forward out;
-  out.lse = at::empty({T}, f32);
-  out.inv_count = at::empty({1}, f32);
+  out.stats = at::empty({T + 1}, f32);
   if (T == 0) {
     out.loss = reduced ? at::full({}, call.reduction == kLossMean ? std::numeric_limits<float>::quiet_NaN() : 0.0, f32) : at::empty({0}, f32);
-    out.inv_count.zero_();
     return out;
   }
   out.loss = reduced ? at::empty({}, f32) : at::empty({T}, f32);
+  const LaunchContext ctx = call.context(2);
   const int64_t parts = ceil_of(V, kLossPart);
   Carver c;
   const int64_t counters = c.take(64), part_at = c.take(parts * T * 8), logit_at = c.take(T * 4), each_at = reduced ? c.take(T * 4) : 0;
   const at::Tensor space = at::empty({c.bytes}, x.options().dtype(at::kByte));
   char* base = static_cast<char*>(space.data_ptr());
-  const LaunchContext ctx = call.context(2);
 
   LossParams p{};
   p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
   plan_band(p);
+  p.claim_lead = claim_lead(p, false);
   p.parts = reinterpret_cast<float2*>(base + part_at);
   p.target_logit = reinterpret_cast<float*>(base + logit_at);
   p.targets = reinterpret_cast<const long long*>(targets.data_ptr<int64_t>());
   p.ignore_index = call.ignore_index;
-  p.claim = reinterpret_cast<int*>(base + counters);
+  int* ticket = reinterpret_cast<int*>(base + counters) + 1;
+  p.zero = ticket; p.zero_ints = 1;
+  if (call.want_dx || call.want_dw) {
+    // the ticket stands in front of the backward's counters, to be cleared with them
+    const int64_t ints = counter_ints(plan(T, H, V, call.want_dx, call.want_dw, ctx.sms));
+    call.counters = at::empty({ints + 1}, x.options().dtype(at::kInt));
+    ticket = call.counters.data_ptr<int>() + ints;
+    p.zero = call.counters.data_ptr<int>(); p.zero_ints = static_cast<int>(ints + 1);
+  }
   p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
   LossMaps m{};
-  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, 128);
+  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, p.x_rows);
   m.w_k = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 128);
-  SEP_CUDA_CHECK(cudaMemsetAsync(base + counters, 0, 64, ctx.stream));
+  if (static_cast<int64_t>(p.row_units) * ceil_of(V, kLossUnit) > ctx.sms / 2) {      // (else every pair has one unit at most)
+    p.claim = reinterpret_cast<int*>(base + counters);
+    SEP_CUDA_CHECK(cudaMemsetAsync(p.claim, 0, sizeof(int), ctx.stream));
+  }
   SEP_CUDA_CHECK(launch_loss_forward(p, m, ctx.sms, ctx.stream));
 
   LossFinalParams f{};
@@ -116,18 +156,17 @@ Forward loss_forward(const LossCall& call, const at::Tensor& x, const at::Tensor
   f.parts = p.parts; f.target_logit = p.target_logit; f.targets = p.targets; f.ignore_index = p.ignore_index;
   f.mean = call.reduction == kLossMean; f.sum = call.reduction == kLossSum;
   f.each = reduced ? reinterpret_cast<float*>(base + each_at) : out.loss.data_ptr<float>();
-  f.lse = out.lse.data_ptr<float>();
+  f.lse = out.stats.data_ptr<float>();
   f.loss = reduced ? out.loss.data_ptr<float>() : nullptr;
-  f.inv_count = out.inv_count.data_ptr<float>();
-  f.ticket = p.claim + 1;
+  f.inv_count = f.lse + T;
+  f.ticket = ticket;
   f.status = ctx.status; f.rank = ctx.rank;
   SEP_CUDA_CHECK(launch_loss_final(f, ctx.stream));
   return out;
 }
 
-std::pair<at::Tensor, at::Tensor> loss_backward(const LossCall& call, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
-                                                const at::Tensor& lse, const at::Tensor& inv_count, const at::Tensor& upstream,
-                                                bool want_dx, bool want_dw) {
+std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
+                                                const at::Tensor& stats, const at::Tensor& upstream, bool want_dx, bool want_dw) {
   const int64_t T = x.size(0), H = x.size(1), V = w.size(0);
   at::Tensor dx, dw;
   if (T == 0) {
@@ -140,44 +179,39 @@ std::pair<at::Tensor, at::Tensor> loss_backward(const LossCall& call, const at::
   const LaunchContext ctx = call.context(want_dx ? 2 : 1);
   const at::Tensor up = upstream.to(at::kFloat).contiguous();
 
-  LossParams p{};
-  p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
-  p.want_dx = want_dx; p.want_dw = want_dw;
-  plan_backward(p, ctx.sms);
-  plan_band(p);
+  LossParams p = plan(T, H, V, want_dx, want_dw, ctx.sms);
   SEP_ASSERT(loss_backward_units(p) < (1ll << 30), "this loss has too many tiles for one call: split the tokens");
   const int64_t z_layers = p.split2 ? 2 : 1, slots = static_cast<int64_t>(p.splits) * z_layers;
-  const int64_t counters = 4 * (4 + 3 * static_cast<int64_t>(p.pieces));
   Carver c;
-  const int64_t count_at = c.take(counters), z_at = c.take(p.buffers * z_layers * T * p.piece * 2);
-  const int64_t dx_at = want_dx ? c.take(slots * T * H * 4) : 0;
+  const int64_t z_at = c.take(p.buffers * z_layers * T * p.piece * 2), dx_at = want_dx ? c.take(slots * T * H * 4) : 0;
   const at::Tensor space = at::empty({c.bytes}, x.options().dtype(at::kByte));
   char* base = static_cast<char*>(space.data_ptr());
   p.targets = reinterpret_cast<const long long*>(targets.data_ptr<int64_t>());
   p.ignore_index = call.ignore_index;
-  p.lse = lse.data_ptr<float>();
+  p.lse = stats.data_ptr<float>();
   if (call.reduction == kLossNone) p.row_scale = up.data_ptr<float>();
   else p.scale = up.data_ptr<float>();
-  if (call.reduction == kLossMean) p.scale2 = inv_count.data_ptr<float>();
-  p.claim = reinterpret_cast<int*>(base + count_at);
+  if (call.reduction == kLossMean) p.scale2 = p.lse + T;
+  p.claim = call.counters.data_ptr<int>();
   p.done = p.claim + 4;
   p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
 
   LossMaps m{};
-  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, 128);
-  m.x_mn = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, 64);
+  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, p.x_rows);
   m.w_k = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 128);
-  m.w_mn = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 64);
-  for (int i = 0; i < 2; ++i) {
+  if (want_dw) m.x_mn = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, 64);
+  if (want_dx) m.w_mn = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 64);
+  for (int i = p.pieces > 1 ? 0 : 1; i < 2; ++i) {
     // of the last piece only the columns that exist (up to whole 16 bytes, zeros in between) are stored and read back
     const int64_t cols = i == 0 ? p.piece : ceil_of(p.last_cols, 8) * 8, layers = p.buffers * z_layers;
-    m.z_k[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, 128);
-    m.z_mn[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, 64);
+    if (want_dx) m.z_k[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, p.x_rows);
+    if (want_dw) m.z_mn[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, 64);
     m.z_out[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, 32);
   }
   if (want_dw) m.dw = make_tmap(dw.data_ptr(), H, V, 1, H, H * V, 64, 32);
   if (want_dx) m.dx = make_tmap(base + dx_at, H, T, slots, H, T * H, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
-  SEP_CUDA_CHECK(cudaMemsetAsync(base + count_at, 0, counters, ctx.stream));
+  if (call.counters_used) SEP_CUDA_CHECK(cudaMemsetAsync(p.claim, 0, counter_ints(p) * sizeof(int), ctx.stream));
+  call.counters_used = true;
   SEP_CUDA_CHECK(launch_loss_backward(p, m, ctx.sms, ctx.stream));
   if (want_dx) {
     LossDxParams d{};
@@ -196,7 +230,7 @@ class LinearLoss : public torch::autograd::Function<LinearLoss> {
                             const c10::intrusive_ptr<LossCall>& call) {
     const at::Tensor xr = readable(x), wr = readable(weight), y = targets.contiguous();
     Forward f = loss_forward(*call, xr, wr, y);
-    ctx->save_for_backward({x, weight, targets, f.lse, f.inv_count});
+    ctx->save_for_backward({x, weight, targets, f.stats});
     ctx->saved_data["call"] = c10::IValue::make_capsule(call);
     return f.loss;
   }
@@ -209,8 +243,8 @@ class LinearLoss : public torch::autograd::Function<LinearLoss> {
     // A thread of the autograd engine may not have made a call of the CUDA runtime yet, and the driver encodes tensor maps only
     // with a context bound to the thread.
     SEP_CUDA_CHECK(cudaSetDevice(saved[0].get_device()));
-    auto g = loss_backward(*call, readable(saved[0]), readable(saved[1]), saved[2].contiguous(), saved[3], saved[4], grads[0],
-                           ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    auto g = loss_backward(*call, readable(saved[0]), readable(saved[1]), saved[2].contiguous(), saved[3], grads[0],
+                           call->want_dx && ctx->needs_input_grad(0), call->want_dw && ctx->needs_input_grad(1));
     return {g.first, g.second, at::Tensor(), at::Tensor()};
   }
 };
@@ -239,16 +273,14 @@ at::Tensor linear_loss(const ContextFn& context, const at::Tensor& x, const at::
   SEP_ASSERT(context(0).device == x.get_device(), "x is not on the device of the buffer that this call reports into");
   if (!(at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad())))
     return loss_forward(*call, readable(x), readable(weight), targets.contiguous()).loss;
+  call->want_dx = x.requires_grad();
+  call->want_dw = weight.requires_grad();
   return LinearLoss::apply(x, weight, targets, call);
 }
 
 std::vector<std::vector<int>> linear_loss_schedule(int64_t tokens, int64_t hidden, int64_t vocab, int sms, bool want_dx, bool want_dw) {
-  LossParams p{};
-  p.T = static_cast<int>(tokens); p.H = static_cast<int>(hidden); p.V = static_cast<int>(vocab);
-  p.want_dx = want_dx; p.want_dw = want_dw;
-  plan_backward(p, sms);
-  plan_band(p);
-  std::vector<std::vector<int>> out = {{p.pieces, p.piece, p.splits, p.ahead, p.buffers, p.row_units, p.split2}};
+  const LossParams p = plan(tokens, hidden, vocab, want_dx, want_dw, sms);
+  std::vector<std::vector<int>> out = {{p.pieces, p.piece, p.splits, p.ahead, p.buffers, p.row_units, p.split2, p.dw_group}};
   const long long units = loss_backward_units(p);
   for (long long i = 0; i < units; ++i) {
     int v[7];

@@ -15,7 +15,7 @@ enum LossKind : int { kLossStats = 0, kLossDz = 1, kLossDx = 2, kLossDw = 3 };
 
 struct LossParams {
   int T, H, V;
-  int num_pairs;                 // CTA pairs of the launch
+  int x_rows;                    // rows of x (and dz, split2) that a CTA loads into its half of a unit: 128, or what a short call has
   int row_units;                 // ceil(T / 256)
   int band;                      // row units that are walked together (see unit_of)
   // --- forward ---
@@ -23,6 +23,7 @@ struct LossParams {
   float* target_logit;           // [T]
   const long long* targets;      // [T]
   long long ignore_index;
+  int* zero; int zero_ints;      // memory that the forward kernel clears for the kernels after it
   // --- backward ---
   const float* lse;              // [T] log of the softmax denominator
   const float* row_scale;        // [T] upstream gradient of each token's loss, or null: 1
@@ -37,8 +38,12 @@ struct LossParams {
   int splits;                    // reductions over a piece of the vocabulary into which a dx unit is split
   int split_blocks;              // k-blocks of each but the last
   int h_units;                   // ceil(H / 256)
-  int* claim;                    // next unit; zero on entry
-  int* done;                     // [3][pieces] epilogue warps that have finished dz / dx / dw units; zero on entry
+  int dw_group;                  // column tiles of a dw unit
+  int* claim;                    // next unit; zero on entry.  Null (forward): units are dealt out in turn
+  int claim_lead;                // units that are claimed ahead of the one whose operands are being requested, beyond the next
+  int* done;                     // epilogue warps that have finished units, zero on entry: [3][pieces] of a piece's dz / dx / dw,
+                                 // then [pieces][piece / 256] of the dz of one column tile
+  int dw_first;                  // the dw units of a piece come before its dx units
   StatusBlock* status;
   int rank;
   unsigned long long wait_budget_ns;
@@ -67,7 +72,7 @@ struct LossFinalParams {
   float* lse;                    // [T]
   float* loss;                   // [1] where they are reduced
   float* inv_count;              // [1] 1 / counted tokens (mean; 0 without any)
-  int* ticket;                   // [1], zero on entry
+  int* ticket;                   // [1], zero on entry (cleared by the forward kernel)
   StatusBlock* status;
   int rank;
 };
@@ -75,6 +80,7 @@ cudaError_t launch_loss_final(const LossFinalParams& p, cudaStream_t stream);
 
 struct LossDxParams {
   int T, H, slots;
+  int lanes;                     // threads that share the slots of an element: a power of two (set by the launcher)
   const float* parts;            // [slots][T][H]
   const float* scale;            // as in LossParams
   const float* scale2;

@@ -22,14 +22,15 @@ namespace sep {
 namespace {
 
 constexpr int kBK = 64;                          // bf16 elements of a k-block: one 128-byte swizzle row
-constexpr int kStages = 6;
 constexpr int kOperandBytes = 128 * kBK * 2;     // A or B of one CTA: 128 rows of a k-block
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps + 1) * 32;   // 0 TMA producer, 1 MMA, 2..9 epilogue, 10 scheduler
-constexpr int kStagingBytes = 4096;              // per epilogue warp: 32 rows of 128 bytes
+constexpr int kStagingBytes = 2 * 4096;          // per epilogue warp of the backward: two tiles of 32 rows of 128 bytes
 constexpr int kQueue = 4;
-constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kStagingBytes + 1024;
+// The forward's epilogue stores nothing but statistics, so all shared memory is its operand ring's.
+constexpr int stages_of(bool fwd) { return fwd ? 7 : 5; }
+constexpr int smem_bytes(bool fwd) { return stages_of(fwd) * kStageBytes + (fwd ? 0 : kEpiWarps * kStagingBytes) + 1024; }
 constexpr int kTmemCols = 512;
 constexpr int kDoneWarps = 2 * kEpiWarps;        // reports per unit
 // The scheduler claims the next unit when the producer has this many k-blocks of the one before left: a claimed unit is work that
@@ -48,6 +49,7 @@ struct Unit {
   int kind, piece, m, n;         // unit row and column in its product
   int k0, k_blocks;              // first k-block (dx: of the piece) and how many
   int split;
+  int tiles;                     // column tiles, one after another (dw)
   bool last;                     // of the last, possibly narrower, piece
 };
 
@@ -71,8 +73,9 @@ __host__ __device__ inline Counts loss_counts(const LossParams& p) {
   c.dz = p.row_units * (p.piece / kLossUnit);
   c.dz_last = p.row_units * ((p.last_cols + kLossUnit - 1) / kLossUnit);
   c.dx = p.want_dx ? p.row_units * p.h_units * p.splits : 0;
-  c.dw = p.want_dw ? (p.piece / kLossUnit) * p.h_units : 0;
-  c.dw_last = p.want_dw ? ((p.last_cols + kLossUnit - 1) / kLossUnit) * p.h_units : 0;
+  const int groups = (p.h_units + p.dw_group - 1) / p.dw_group;
+  c.dw = p.want_dw ? (p.piece / kLossUnit) * groups : 0;
+  c.dw_last = p.want_dw ? ((p.last_cols + kLossUnit - 1) / kLossUnit) * groups : 0;
   return c;
 }
 
@@ -80,7 +83,7 @@ __host__ __device__ inline Counts loss_counts(const LossParams& p) {
 __host__ __device__ __forceinline__ Unit unit_of(const LossParams& p, int lin) {
   const Counts c = loss_counts(p);
   Unit u;
-  u.split = 0; u.k0 = 0;
+  u.split = 0; u.k0 = 0; u.tiles = 1;
   const int last = p.pieces - 1;
   int kind = kLossDz, piece = 0, rem = lin;
   const int lead = lesser(p.ahead, p.pieces);                   // pieces of the lead-in
@@ -108,8 +111,9 @@ __host__ __device__ __forceinline__ Unit unit_of(const LossParams& p, int lin) {
       piece = j + p.ahead;
     } else {
       rem -= here;
-      if (rem < c.dx) kind = kLossDx;
-      else { rem -= c.dx; kind = kLossDw; }
+      const int first = p.dw_first ? (j == last ? c.dw_last : c.dw) : c.dx;
+      kind = (rem < first) == (p.dw_first != 0) ? kLossDw : kLossDx;
+      if (rem >= first) rem -= first;
     }
   }
   u.kind = kind; u.piece = piece; u.last = piece == last;
@@ -124,7 +128,9 @@ __host__ __device__ __forceinline__ Unit unit_of(const LossParams& p, int lin) {
     u.k0 = u.split * p.split_blocks;
     u.k_blocks = greater(lesser(p.split_blocks, ceil_div(cols, kBK) - u.k0), 0);
   } else {
-    band_decode(8, rem, ceil_div(cols, kLossUnit), p.h_units, u.m, u.n);
+    band_decode(8, rem, ceil_div(cols, kLossUnit), ceil_div(p.h_units, p.dw_group), u.m, u.n);
+    u.n *= p.dw_group;
+    u.tiles = lesser(p.dw_group, p.h_units - u.n);
     u.k_blocks = ceil_div(p.T, kBK) * (p.split2 ? 2 : 1);
   }
   return u;
@@ -150,6 +156,7 @@ __device__ __forceinline__ void tma_reduce_add_3d(const void* tmap, const void* 
 template <bool FWD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__ LossMaps maps) {
+  constexpr int kStages = stages_of(FWD);
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   unsigned char* stage_base = smem;
@@ -181,6 +188,9 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
   cluster_sync();
   tc_fence_after_sync();
   const uint32_t tmem_base = s_tmem;
+  grid_release();
+  if (FWD && blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.zero_ints; i += kThreads) p.zero[i] = 0;
 
   int total;
   if (FWD) {
@@ -192,7 +202,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
   auto decode = [&](int lin) {
     if constexpr (FWD) {
       Unit u;
-      u.kind = kLossStats; u.piece = 0; u.split = 0; u.k0 = 0; u.last = true;
+      u.kind = kLossStats; u.piece = 0; u.split = 0; u.k0 = 0; u.tiles = 1; u.last = true;
       band_decode(p.band, lin, p.row_units, ceil_div(p.V, kLossUnit), u.m, u.n);
       u.k_blocks = ceil_div(p.H, kBK);
       return u;
@@ -220,8 +230,8 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
       for (int it = 0;; ++it) {
         const int q = it % kQueue;
         if (!mbar_wait<true>(&queue_empty[q], ((it / kQueue) & 1) ^ 1, budget, p.status)) break;
-        if (!spin_until([&] { return *reinterpret_cast<volatile int*>(&s_progress) >= it; }, budget, p.status)) break;
-        const int lin = atomicAdd(p.claim, 1);
+        if (!spin_until([&] { return *reinterpret_cast<volatile int*>(&s_progress) >= it - p.claim_lead; }, budget, p.status)) break;
+        const int lin = FWD && p.claim == nullptr ? static_cast<int>(blockIdx.x / 2 + it * (gridDim.x / 2)) : atomicAdd(p.claim, 1);
         s_queue[q] = lin;
         st_cluster(cluster_map(&s_queue[q], 1), lin);
         mbar_arrive(&queue_full[q]);
@@ -233,43 +243,62 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int stage = 0; uint32_t phase = 0; int issued = 0; bool ok = true;
+      int seen_dz = -1, seen_free = -1, seen_sum = -1;      // pieces whose counters were found complete: not asked for again
       for (int it = 0; ok; ++it) {
         int lin;
         if (!next_unit(it, lin)) { ok = false; break; }
         release_entry(it);
         if (lin >= total) break;
-        const Unit u = decode(lin);
+        Unit u = decode(lin);
         if (!FWD) {
           // what this unit reads, or overwrites, of other units' results (all of lower numbers)
           const Counts c = loss_counts(p);
           auto reached = [&](int list, int piece, int units) {
-            const int* d = p.done + list * p.pieces + piece;
+            const int* d = p.done + list * p.pieces + piece;       // (list 3: by column tile)
             if (spin_until([&] { return ld_acquire_gpu(d) >= units * kDoneWarps; }, budget, p.status)) return true;
             report_failure(p.status, kStatusTimeoutTileGate, kKernelLoss, list, p.rank, piece, units * kDoneWarps, ld_acquire_gpu(d));
             return false;
           };
+          bool asked = false;
+          auto once = [&](int& seen, int piece, auto ask) {
+            if (piece <= seen) return true;
+            if (!ask()) return false;
+            seen = piece; asked = true;
+            return true;
+          };
           if (u.kind == kLossDz) {
-            if (u.piece >= p.buffers)      // the buffer's piece before was never the last one
-              ok = reached(1, u.piece - p.buffers, c.dx) && reached(2, u.piece - p.buffers, c.dw);
-          } else {
-            ok = reached(0, u.piece, u.last ? c.dz_last : c.dz);
+            if (u.piece >= p.buffers)      // (the piece that was in this buffer was not the last one)
+              ok = once(seen_free, u.piece - p.buffers, [&] { return reached(1, u.piece - p.buffers, c.dx) && reached(2, u.piece - p.buffers, c.dw); });
+          } else if (u.kind == kLossDx) {
+            ok = once(seen_dz, u.piece, [&] { return reached(0, u.piece, u.last ? c.dz_last : c.dz); });
             // sums of pieces are added in the order of the pieces, so that a repeated call gives the same bits
-            if (ok && u.kind == kLossDx && u.piece > 0) ok = reached(1, u.piece - 1, c.dx);
+            if (ok && u.piece > 0) ok = once(seen_sum, u.piece - 1, [&] { return reached(1, u.piece - 1, c.dx); });
+          } else if (u.piece > seen_dz) {
+            asked = true;
+            if (ld_acquire_gpu(p.done + u.piece) >= (u.last ? c.dz_last : c.dz) * kDoneWarps) seen_dz = u.piece;
+            else ok = reached(3, u.piece * (p.piece / kLossUnit) + u.m, p.row_units);      // one column tile of dz is enough
           }
           if (!ok) break;
-          fence_proxy_async();
+          if (asked) fence_proxy_async();
         }
         const int n_cols = (u.kind <= kLossDz) ? (FWD ? p.V : (u.last ? p.last_cols : p.piece)) : p.H;
-        const int n0 = u.n * kLossUnit;
-        const int b0 = n0 + half * (tile_cols(n_cols, n0) / 2);
         const int a0 = u.m * kLossUnit + half * 128;
         const int v0 = u.piece * (FWD ? 0 : p.piece);
         const int zbuf = FWD ? 0 : (u.piece % p.buffers) * (p.split2 ? 2 : 1);
         const int t_blocks = ceil_div(p.T, kBK);
+        // Short calls load only the rows that exist (what else the buffer holds ends up in accumulator rows that nobody reads): of one
+        // token at H 4096, V 128000 221 -> 198 us, since rows out of bounds cost the copy unit as much as others.
+        const bool short_rows = p.x_rows < 128 && (FWD || u.kind != kLossDw);
+        const bool load_a = !short_rows || half == 0 || (!FWD && u.kind == kLossDx);
+        const uint32_t pair_bytes = !short_rows ? 2 * kStageBytes
+            : 2 * kOperandBytes + p.x_rows * 128 * (!FWD && u.kind == kLossDx ? 2 : 1);
         const int warn = max(u.k_blocks - kClaimAhead, 0);
         if (u.k_blocks == 0 && leader) st_volatile_shared(&s_progress, it + 1);
+        for (int tile = 0; tile < u.tiles && ok; ++tile, ++u.n) {
+        const int n0 = u.n * kLossUnit;
+        const int b0 = n0 + half * (tile_cols(n_cols, n0) / 2);
         for (int kb = 0; kb < u.k_blocks; ++kb) {
-          if (leader && kb == warn) st_volatile_shared(&s_progress, it + 1);
+          if (leader && kb == warn && tile == u.tiles - 1) st_volatile_shared(&s_progress, it + 1);
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, budget, p.status)) {
             report_failure(p.status, kStatusTimeoutPipeline, kKernelLoss, 0, p.rank, lin, kb, stage);
             ok = false; break;
@@ -277,11 +306,11 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           unsigned char* sa = stage_base + stage * kStageBytes;
           unsigned char* sb = sa + kOperandBytes;
           // Both CTAs' bytes are counted on the first CTA's barrier, which that CTA arms for the sum.
-          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * kStageBytes);
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], pair_bytes);
           const uint32_t bar = cluster_map(&full_bar[stage], 0);
           const int k = (u.k0 + kb) * kBK;
           if (FWD || u.kind == kLossDz) {
-            tma_load_3d_pair(sa, &maps.x_k, bar, k, a0, 0);
+            if (load_a) tma_load_3d_pair(sa, &maps.x_k, bar, k, a0, 0);
             tma_load_3d_pair(sb, &maps.w_k, bar, k, v0 + b0, 0);
           } else if (u.kind == kLossDx) {
             // split2: the first CTA multiplies the leading halves of dz, the second the remainders
@@ -300,6 +329,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           ++issued;
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
+        }
       }
       if (!ok && issued > 0) {       // let the copies in flight land before the CTA may exit (bounded)
         const unsigned long long t0 = globaltimer_ns();
@@ -317,10 +347,11 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         __syncwarp();
         if (lane == 0) release_entry(it);
         if (lin >= total) break;
-        const Unit u = decode(lin);
+        Unit u = decode(lin);
         if (u.k_blocks == 0) continue;
         const bool a_mn = !FWD && u.kind == kLossDw, b_mn = !FWD && u.kind >= kLossDx;
         const int n_cols = (u.kind <= kLossDz) ? (FWD ? p.V : (u.last ? p.last_cols : p.piece)) : p.H;
+        for (int tile = 0; tile < u.tiles && ok; ++tile, ++u.n) {
         const uint32_t idesc = (a_mn ? idesc_mm : b_mn ? idesc_km : idesc_kk) | (static_cast<uint32_t>(tile_cols(n_cols, u.n * kLossUnit) >> 3) << 17);
         // per 16 elements of K: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major box
         const uint32_t step_a = a_mn ? 16 * 128 : 32, step_b = b_mn ? 16 * 128 : 32;
@@ -348,6 +379,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         }
         acc ^= 1; if (acc == 0) acc_phase ^= 1;
         }
+        }
       }
       if (!ok && lane == 0) report_failure(p.status, kStatusTimeoutPipeline, kKernelLoss, 1, p.rank, 0, 0, 0);
     }
@@ -355,17 +387,29 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
     // ------------------------------------------------------------------ epilogue: a warp reads the 32 accumulator lanes of its quarter,
     // warps 2..5 the left 128 columns of the tile and warps 6..9 the right ones.  Warps do not wait for one another.
     const int quarter = warp & 3, side = (warp - 2) >> 2;
+    // A tile of results is written to shared memory and leaves by a bulk store, while the warp fills the other one.
     unsigned char* stage_tile = staging + (warp - 2) * kStagingBytes;
-    const uint32_t stg = smem_u32(stage_tile);
+    auto next_tile = [&] {               // whole warp: the tile that the store before the last one has read
+      stage_tile = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(stage_tile) ^ 4096);
+      if (lane == 0) bulk_wait_read_but_one();
+      __syncwarp();
+      return smem_u32(stage_tile);
+    };
+    uint32_t stg = 0;
+    float scale = 1.f;                   // of dw
+    if (!FWD && p.scale != nullptr) scale = *p.scale;
+    if (!FWD && p.scale2 != nullptr) scale *= *p.scale2;
     int acc = 0; uint32_t acc_phase = 0;
-    for (int it = 0;; ++it) {
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
       int lin = 0;
       if (!__all_sync(0xffffffffu, next_unit(it, lin))) break;
       __syncwarp();
       if (lane == 0) release_entry(it);
       if (lin >= total) break;
-      const Unit u = decode(lin);
+      Unit u = decode(lin);
       const int n_cols = (u.kind <= kLossDz) ? (FWD ? p.V : (u.last ? p.last_cols : p.piece)) : p.H;
+      for (int tile = 0; tile < u.tiles; ++tile, ++u.n) {
       const int n0 = u.n * kLossUnit + side * 128;                 // first column of this warp
       const int chunks = min(4, max(0, (n_cols - n0 + 31) / 32));
       const int row0 = u.m * kLossUnit + half * 128 + quarter * 32;  // first row of this warp
@@ -374,7 +418,6 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
       // fetched while the tensor cores still work on the tile
       int col = -1; float lse2 = 0.f, c_t = 0.f;
       bool dead = true;              // an ignored token (or no token): zeros whatever its logits are
-      float scale = 1.f;
       if (u.kind <= kLossDz) {
         if (row < p.T) {
           const long long y = p.targets[row];
@@ -386,9 +429,6 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
             lse2 = p.lse[row] * kLog2e;
           }
         }
-      } else if (u.kind == kLossDw) {
-        if (p.scale != nullptr) scale = *p.scale;
-        if (p.scale2 != nullptr) scale *= *p.scale2;
       }
       auto accumulated = [&] {
         if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], acc_phase, budget, p.status))) {
@@ -398,7 +438,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         tc_fence_after_sync();
         return true;
       };
-      if (!FWD && !empty && !accumulated()) break;
+      if (!FWD && !empty && !(ok = accumulated())) break;
       const uint32_t lanes = tmem_base + side * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
       const uint32_t taddr = lanes + acc * kLossUnit;
       auto give_back = [&] {
@@ -419,9 +459,9 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         float z[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) z[i] = 0.f;
-        bool ok = true;
         for (int first = 0; first < u.k_blocks; first += kSegmentBlocks) {
           if (!(ok = accumulated())) break;
+          if (row0 < p.T) {
 #pragma unroll
           for (int c = 0; c < 8; ++c) {       // (16 columns at a time: 32 spill)
             uint32_t part[16];
@@ -430,11 +470,14 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
 #pragma unroll
             for (int i = 0; i < 16; ++i) z[c * 16 + i] += __uint_as_float(part[i]);
           }
+          } else {
+            give_back();
+          }
           acc ^= 1; if (acc == 0) acc_phase ^= 1;
         }
         if (!ok) break;
         const int left = n_cols - n0;        // (columns that were not multiplied hold anything)
-        if (left <= 0) continue;
+        if (left <= 0 || row0 >= p.T) continue;
         const float ninf = __int_as_float(0xff800000);
         if (left < 128) {
 #pragma unroll
@@ -461,19 +504,16 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         const int zbuf = (u.piece % p.buffers) * (p.split2 ? 2 : 1);
         const int passes = p.split2 ? 2 : 1;
         const bool rows = row0 < p.T;
+        if (!rows) give_back();
 #pragma unroll 1
-        for (int part = 0; part < passes; ++part) {
+        for (int part = 0; part < passes && rows; ++part) {
 #pragma unroll 1
           for (int c = 0; c < chunks; ++c) {
             fetch(c);
             if (c == chunks - 1 && part == passes - 1) give_back();
-            if (!rows) continue;
             const int left = n_cols - n0 - c * 32;
             const bool target_here = __any_sync(0xffffffffu, (col >> 5) == c);
-            if ((c & 1) == 0) {
-              if (lane == 0) bulk_wait_read();
-              __syncwarp();
-            }
+            if ((c & 1) == 0) stg = next_tile();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               uint32_t o[4];
@@ -504,19 +544,24 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
             }
           }
         }
-        if (chunks == 0) give_back();
+        if (chunks == 0 && rows) give_back();
         __syncwarp();
-        if (lane == 0) { bulk_wait_all(); fence_proxy_async(); red_release_gpu_add(p.done + u.piece, 1); }
+        if (lane == 0) {
+          bulk_wait_all();
+          fence_proxy_async();
+          red_release_gpu_add(p.done + u.piece, 1);
+          red_release_gpu_add(p.done + 3 * p.pieces + u.piece * (p.piece / kLossUnit) + u.n, 1);
+        }
       } else if (u.kind == kLossDx) {
         const int z = p.split2 ? u.split * 2 + half : u.split;
         const int y = p.split2 ? quarter * 32 : row0;
+        const bool rows = y < p.T;
+        if (!rows && !empty) give_back();
 #pragma unroll 1
-        for (int c = 0; c < chunks; ++c) {
+        for (int c = 0; c < chunks && rows; ++c) {
           fetch(c);
           if (c == chunks - 1 && !empty) give_back();
-          if (y >= p.T) continue;
-          if (lane == 0) bulk_wait_read();
-          __syncwarp();
+          stg = next_tile();
 #pragma unroll
           for (int q = 0; q < 8; ++q) st_shared_v4(stg + stage_off<128>(lane, q), r[q * 4], r[q * 4 + 1], r[q * 4 + 2], r[q * 4 + 3]);
           fence_proxy_async_smem();
@@ -527,43 +572,44 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
             bulk_commit();
           }
         }
-        if (chunks == 0 && !empty) give_back();
+        if (chunks == 0 && rows && !empty) give_back();
         __syncwarp();
         if (lane == 0) { bulk_wait_all(); red_release_gpu_add(p.done + p.pieces + u.piece, 1); }
       } else {
         const int v = u.piece * p.piece + row0;
 #pragma unroll 1
-        for (int c = 0; c < chunks; ++c) {
-          fetch(c);
-          if (c == chunks - 1) {
+        for (int c = 0; c < chunks; c += 2) {
+          uint32_t r2[32];             // two chunks on their way at once (columns past the last were not multiplied and are not stored)
+          tmem_ld_32x32(taddr + c * 32, r);
+          tmem_ld_32x32(taddr + c * 32 + 32, r2);
+          tmem_ld_wait();
+          if (c + 2 >= chunks) {
             give_back();
-            if (lane == 0) red_release_gpu_add(p.done + 2 * p.pieces + u.piece, 1);   // the operands have been read
+            if (lane == 0 && tile == u.tiles - 1) red_release_gpu_add(p.done + 2 * p.pieces + u.piece, 1);   // the operands have been read
           }
           if (v >= p.V) continue;
-          if ((c & 1) == 0) {
-            if (lane == 0) bulk_wait_read();
-            __syncwarp();
-          }
+          stg = next_tile();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 8; ++q) {
             uint32_t o[4];
 #pragma unroll
-            for (int h = 0; h < 4; ++h)
-              o[h] = pack_bf16x2(scale * __uint_as_float(r[q * 8 + h * 2]), scale * __uint_as_float(r[q * 8 + h * 2 + 1]));
-            st_shared_v4(stg + stage_off<128>(lane, (c & 1) * 4 + q), o[0], o[1], o[2], o[3]);
+            for (int h = 0; h < 4; ++h) {
+              const int i = (q & 3) * 8 + h * 2;
+              o[h] = pack_bf16x2(scale * __uint_as_float(q < 4 ? r[i] : r2[i]), scale * __uint_as_float(q < 4 ? r[i + 1] : r2[i + 1]));
+            }
+            st_shared_v4(stg + stage_off<128>(lane, q), o[0], o[1], o[2], o[3]);
           }
-          if ((c & 1) == 1 || c == chunks - 1) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) { tma_store_3d(&maps.dw, stage_tile, n0 + (c & ~1) * 32, v, 0); bulk_commit(); }
-          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) { tma_store_3d(&maps.dw, stage_tile, n0 + c * 32, v, 0); bulk_commit(); }
         }
         if (chunks == 0) {
           give_back();
-          if (lane == 0) red_release_gpu_add(p.done + 2 * p.pieces + u.piece, 1);
+          if (lane == 0 && tile == u.tiles - 1) red_release_gpu_add(p.done + 2 * p.pieces + u.piece, 1);
         }
       }
       if (!FWD && !empty) { acc ^= 1; if (acc == 0) acc_phase ^= 1; }
+      }
     }
     if (lane == 0) bulk_wait_all();
   }
@@ -585,55 +631,70 @@ cudaError_t launch_pairs(const LossParams& p, const LossMaps& m, long long units
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(FWD));
     if (e != cudaSuccess) return e;
     configured[dev].store(true, std::memory_order_release);
   }
   const long long pairs = units < sms / 2 ? units : sms / 2;
-  kernel<<<static_cast<unsigned>(pairs * 2), kThreads, kSmemBytes, stream>>>(p, m);
+  kernel<<<static_cast<unsigned>(pairs * 2), kThreads, smem_bytes(FWD), stream>>>(p, m);
   return cudaGetLastError();
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the parts of each row, and the rows' losses.  A block takes 32 rows: lanes are rows, warps take parts in turn.
+// Joins the parts of each row, and the rows' losses.  A block takes 8 rows (64 contiguous bytes of every part) and 64 threads for
+// each: with 32 rows and 16 threads a call of one token waited for 49 loads in a row (V 100003: 16.6 us).
 // ---------------------------------------------------------------------------------------------
-constexpr int kFinalWarps = 16;
+constexpr int kFinalRows = 8, kFinalThreads = 512, kFinalLanes = kFinalThreads / kFinalRows;
 
-__global__ void __launch_bounds__(kFinalWarps * 32) loss_final_kernel(const LossFinalParams p) {
-  __shared__ float2 joined[kFinalWarps][32];
-  __shared__ double sums[kFinalWarps];
-  __shared__ int counts[kFinalWarps];
+__global__ void __launch_bounds__(kFinalThreads) loss_final_kernel(const LossFinalParams p) {
+  __shared__ float2 joined[kFinalLanes][kFinalRows];
+  __shared__ double sums[kFinalThreads / 32];
+  __shared__ int counts[kFinalThreads / 32];
   __shared__ bool last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long row = static_cast<long long>(blockIdx.x) * 32 + lane;
+  const int r = threadIdx.x % kFinalRows, part = threadIdx.x / kFinalRows;
+  const long long row = static_cast<long long>(blockIdx.x) * kFinalRows + r;
   const float ninf = __int_as_float(0xff800000);
   auto join = [&](float2 a, float2 b) {
     const float m = fmaxf(a.x, b.x);
-    if (m == ninf) return make_float2(m, a.y + b.y);
-    return make_float2(m, a.y * exp2f((a.x - m) * kLog2e) + b.y * exp2f((b.x - m) * kLog2e));
+    const float ref = m == ninf ? 0.f : m * kLog2e;
+    return make_float2(m, a.y * ex2(fmaf(a.x, kLog2e, -ref)) + b.y * ex2(fmaf(b.x, kLog2e, -ref)));
   };
+  grid_wait();
   float2 v = make_float2(ninf, 0.f);
   if (row < p.T) {
-#pragma unroll 4
-    for (int i = warp; i < p.num_parts; i += kFinalWarps) v = join(v, p.parts[static_cast<size_t>(i) * p.T + row]);
-  }
-  joined[warp][lane] = v;
-  __syncthreads();
-  if (warp == 0 && row < p.T) {
-    for (int w = 1; w < kFinalWarps; ++w) v = join(v, joined[w][lane]);
-    float lse = v.x + logf(v.y);
-    const long long y = p.targets[row];
-    float loss = 0.f;
-    if (y != p.ignore_index) {
-      if (y < 0 || y >= p.V) {       // the loss and every gradient become NaN, and the caller can ask why
-        report_note(p.status, kStatusBadTarget, kKernelLoss, 0, p.rank, static_cast<int>(row), p.V, static_cast<int>(y));
-        lse = loss = __int_as_float(0x7fc00000);
-      } else {
-        loss = lse - p.target_logit[row];
-      }
+    const float2* q = p.parts + row;
+    int i = part;
+    for (; i + 3 * kFinalLanes < p.num_parts; i += 4 * kFinalLanes) {
+      float2 u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = q[static_cast<size_t>(i + j * kFinalLanes) * p.T];
+      v = join(v, join(join(u[0], u[1]), join(u[2], u[3])));
     }
-    p.lse[row] = lse;
-    p.each[row] = loss;
+    for (; i < p.num_parts; i += kFinalLanes) v = join(v, q[static_cast<size_t>(i) * p.T]);
+  }
+  joined[part][r] = v;
+  __syncthreads();
+  if (warp == 0) {
+    // four lanes for each row
+    v = joined[part][r];
+    for (int w = part + 4; w < kFinalLanes; w += 4) v = join(v, joined[w][r]);
+    for (int d = 8; d < 32; d *= 2) v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, d), __shfl_xor_sync(0xffffffffu, v.y, d)));
+    if (lane < kFinalRows && row < p.T) {
+      float lse = v.x + logf(v.y);
+      const long long y = p.targets[row];
+      float loss = 0.f;
+      if (y != p.ignore_index) {
+        if (y < 0 || y >= p.V) {       // the loss and every gradient become NaN, and the caller can ask why
+          report_note(p.status, kStatusBadTarget, kKernelLoss, 0, p.rank, static_cast<int>(row), p.V, static_cast<int>(y));
+          lse = loss = __int_as_float(0x7fc00000);
+        } else {
+          loss = lse - p.target_logit[row];
+        }
+      }
+      p.lse[row] = lse;
+      p.each[row] = loss;
+    }
   }
   if (!p.mean && !p.sum) return;
   __threadfence();
@@ -643,7 +704,7 @@ __global__ void __launch_bounds__(kFinalWarps * 32) loss_final_kernel(const Loss
   if (!last) return;
   __threadfence();
   double sum = 0.0; int count = 0;
-  for (int t = threadIdx.x; t < p.T; t += blockDim.x) {
+  for (int t = threadIdx.x; t < p.T; t += kFinalThreads) {
     sum += static_cast<double>(__ldcg(p.each + t));
     count += p.targets[t] != p.ignore_index ? 1 : 0;
   }
@@ -654,29 +715,48 @@ __global__ void __launch_bounds__(kFinalWarps * 32) loss_final_kernel(const Loss
   if (lane == 0) { sums[warp] = sum; counts[warp] = count; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kFinalWarps; ++w) { sum += sums[w]; count += counts[w]; }
+    for (int w = 1; w < kFinalThreads / 32; ++w) { sum += sums[w]; count += counts[w]; }
     // without a counted token the mean is 0 / 0, and its gradients are zeros
     *p.loss = static_cast<float>(p.mean ? sum / static_cast<double>(count) : sum);
     if (p.mean) *p.inv_count = count > 0 ? static_cast<float>(1.0 / count) : 0.f;
   }
 }
 
-// dx = scale * sum of its slots, rounded once.
-__global__ void __launch_bounds__(256) loss_dx_kernel(const LossDxParams p) {
-  const size_t n = static_cast<size_t>(p.T) * p.H;
+// dx = scale * sum of its slots, rounded once.  Calls of few elements and many slots share the slots of four elements among several
+// threads (16 tokens, hidden 2048, 60 slots: one thread after another waited for 60 loads in a row, 40 us).
+constexpr int kDxThreads = 256;
+
+__global__ void __launch_bounds__(kDxThreads) loss_dx_kernel(const LossDxParams p) {
+  __shared__ float4 shared[kDxThreads];
+  const size_t n = static_cast<size_t>(p.T) * p.H / 4;            // vectors (H is a multiple of 8)
+  const int per_block = kDxThreads / p.lanes, lane = threadIdx.x / per_block, v = threadIdx.x % per_block;
+  grid_wait();
   float scale = p.scale != nullptr ? *p.scale : 1.f;
   if (p.scale2 != nullptr) scale *= *p.scale2;
-  for (size_t i = (static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8; i < n; i += static_cast<size_t>(gridDim.x) * blockDim.x * 8) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-    for (int s = 0; s < p.slots; ++s) {
-      const float4* q = reinterpret_cast<const float4*>(p.parts + s * n + i);
-      const float4 u = __ldcs(q), w = __ldcs(q + 1);
-      a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
-      b.x += w.x; b.y += w.y; b.z += w.z; b.w += w.w;
+  auto add = [](float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); };
+  for (size_t first = static_cast<size_t>(blockIdx.x) * per_block; first < n; first += static_cast<size_t>(gridDim.x) * per_block) {
+    const size_t i = first + v;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < n) {
+      const float4* q = reinterpret_cast<const float4*>(p.parts) + i;
+      int s = lane;
+      for (; s + 3 * p.lanes < p.slots; s += 4 * p.lanes) {
+        float4 u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = __ldcs(q + (s + j * p.lanes) * n);
+        a = add(a, add(add(u[0], u[1]), add(u[2], u[3])));
+      }
+      for (; s < p.slots; s += p.lanes) a = add(a, __ldcs(q + s * n));
     }
-    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.dx) + i) =
-        make_uint4(pack_bf16x2(scale * a.x, scale * a.y), pack_bf16x2(scale * a.z, scale * a.w),
-                   pack_bf16x2(scale * b.x, scale * b.y), pack_bf16x2(scale * b.z, scale * b.w));
+    if (p.lanes > 1) {
+      shared[threadIdx.x] = a;
+      __syncthreads();
+      if (lane == 0)
+        for (int l = 1; l < p.lanes; ++l) a = add(a, shared[l * per_block + v]);
+      __syncthreads();
+    }
+    if (lane == 0 && i < n)
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.dx) + i * 4) = make_uint2(pack_bf16x2(scale * a.x, scale * a.y), pack_bf16x2(scale * a.z, scale * a.w));
   }
 }
 
@@ -698,15 +778,29 @@ cudaError_t launch_loss_forward(const LossParams& p, const LossMaps& m, int sms,
 cudaError_t launch_loss_backward(const LossParams& p, const LossMaps& m, int sms, cudaStream_t stream) {
   return launch_pairs<false>(p, m, loss_backward_units(p), sms, stream);
 }
-cudaError_t launch_loss_final(const LossFinalParams& p, cudaStream_t stream) {
-  loss_final_kernel<<<static_cast<unsigned>((p.T + 31) / 32), kFinalWarps * 32, 0, stream>>>(p);
-  return cudaGetLastError();
+// Both follow the kernel whose results they read, and may be launched while it drains.
+template <class Params>
+static cudaError_t launch_after(void (*kernel)(const Params), const Params& p, long long blocks, int threads, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
-cudaError_t launch_loss_dx(const LossDxParams& p, cudaStream_t stream) {
-  const long long vectors = static_cast<long long>(p.T) * p.H / 8;
-  const long long blocks = (vectors + 255) / 256;
-  loss_dx_kernel<<<static_cast<unsigned>(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_loss_final(const LossFinalParams& p, cudaStream_t stream) {
+  return launch_after(loss_final_kernel, p, (p.T + kFinalRows - 1) / kFinalRows, kFinalThreads, stream);
+}
+cudaError_t launch_loss_dx(const LossDxParams& p_in, cudaStream_t stream) {
+  LossDxParams p = p_in;
+  const long long vectors = static_cast<long long>(p.T) * p.H / 4;
+  p.lanes = 1;
+  while (p.lanes < 16 && p.lanes * 4 <= p.slots && vectors * p.lanes < 148 * 1024) p.lanes *= 2;
+  const long long per_block = kDxThreads / p.lanes, blocks = (vectors + per_block - 1) / per_block;
+  return launch_after(loss_dx_kernel, p, blocks < 148 * 8 ? blocks : 148 * 8, kDxThreads, stream);
 }
 
 }  // namespace sep

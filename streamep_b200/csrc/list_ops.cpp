@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <deque>
 
 #include "host_common.h"
 #include "list_kernels.h"
@@ -16,9 +17,10 @@ namespace {
 
 bool is_half(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16; }
 
-void check_tensor(const at::Tensor& t, const at::Device& device, const char* what) {
-  SEP_ASSERT(t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.device() == device, what << " must be dense tensors on one CUDA device");
-  SEP_ASSERT(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, what << " must be bf16 or float32");
+constexpr char kListMessage[] = "the tensors of a list must be dense tensors on one CUDA device, bf16 or float32";
+
+bool usable(const at::Tensor& t, const at::Device& device) {
+  return t.defined() && t.layout() == at::kStrided && t.device() == device && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat);
 }
 
 // What is written in place must not lie in two entries: its owner would be undefined.
@@ -47,9 +49,9 @@ int chunk_of(int64_t elements, int64_t blocks) {
 
 // Cuts `tensors` (none of them empty) into lists of at most kNormEntries.
 template <class Launch>
-void for_norm_lists(const std::vector<at::Tensor>& tensors, Launch launch) {
+void for_norm_lists(const TensorList& tensors, Launch launch) {
   int64_t elements = 0;
-  for (const auto& t : tensors) elements += t.numel();
+  for (const at::Tensor* t : tensors) elements += t->numel();
   NormList list;
   const int most = num_sms() * kNormBlocksPerSm;
   list.chunk = chunk_of(elements, most);
@@ -57,7 +59,7 @@ void for_norm_lists(const std::vector<at::Tensor>& tensors, Launch launch) {
     list.count = static_cast<int>(std::min<size_t>(kNormEntries, tensors.size() - at));
     int64_t chunks = 0;
     for (int i = 0; i < list.count; ++i) {
-      const at::Tensor& t = tensors[at + i];
+      const at::Tensor& t = *tensors[at + i];
       list.data[i] = t.data_ptr();
       list.length[i] = static_cast<unsigned long long>(t.numel()) | (static_cast<unsigned long long>(is_half(t) ? kListHalf : 0) << kListTypeShift);
       list.first[i] = static_cast<int>(chunks);
@@ -70,21 +72,25 @@ void for_norm_lists(const std::vector<at::Tensor>& tensors, Launch launch) {
 }
 
 // The tensors to read for a norm: dense ones as they lie (the order of elements does not matter), others as contiguous copies.
-TensorList readable(const TensorList& tensors) {
-  TensorList out;
-  out.reserve(tensors.size());
-  for (const auto& t : tensors) {
-    check_tensor(t, tensors[0].device(), "the tensors of a list");
-    if (t.numel() == 0) continue;
-    out.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());
+struct Readable {
+  TensorList list;
+  std::deque<at::Tensor> copies;
+  Readable(const TensorList& tensors, const at::Device& device) {
+    list.reserve(tensors.size());
+    for (const at::Tensor* t : tensors) {
+      SEP_ASSERT(usable(*t, device), kListMessage);
+      if (t->numel() == 0) continue;
+      if (t->is_non_overlapping_and_dense()) { list.push_back(t); continue; }
+      copies.push_back(t->detach().contiguous());
+      list.push_back(&copies.back());
+    }
   }
-  return out;
-}
+};
 
 // The partial sums of squares of a list, one double per block of every launch.
 at::Tensor squares(const TensorList& tensors, cudaStream_t stream, int& count) {
   const int64_t lists = (static_cast<int64_t>(tensors.size()) + kNormEntries - 1) / kNormEntries;
-  const at::Tensor sums = at::empty({lists * num_sms() * kNormBlocksPerSm}, tensors[0].options().dtype(at::kDouble));
+  const at::Tensor sums = at::empty({lists * num_sms() * kNormBlocksPerSm}, tensors[0]->options().dtype(at::kDouble));
   count = 0;
   for_norm_lists(tensors, [&](const NormList& list, int blocks) {
     SEP_CUDA_CHECK(launch_list_squares(list, sums.data_ptr<double>() + count, blocks, stream));
@@ -106,54 +112,65 @@ void changed(const at::Tensor& t) {
 // Tensors that will be scaled in place: dense ones themselves; others through contiguous copies that go back afterwards.
 struct InPlace {
   TensorList work;
-  std::vector<std::pair<at::Tensor, at::Tensor>> back;     // (tensor, its copy)
-  explicit InPlace(const TensorList& tensors) {
+  std::deque<at::Tensor> copies;
+  std::vector<const at::Tensor*> back;             // whose copies they are
+  InPlace(const TensorList& tensors, const at::Device& device) {
     Ranges ranges;
-    for (const auto& t : tensors) {
-      check_tensor(t, tensors[0].device(), "the tensors of a list");
-      if (t.numel() == 0) continue;
-      if (t.is_non_overlapping_and_dense()) {
-        ranges.add(t);
+    work.reserve(tensors.size());
+    ranges.all.reserve(tensors.size());
+    for (const at::Tensor* t : tensors) {
+      SEP_ASSERT(usable(*t, device), kListMessage);
+      if (t->numel() == 0) continue;
+      if (t->is_non_overlapping_and_dense()) {
+        ranges.add(*t);
         work.push_back(t);
       } else {
-        for (int64_t d = 0; d < t.dim(); ++d)
-          SEP_ASSERT(t.size(d) <= 1 || t.stride(d) != 0, "an expanded tensor cannot be changed in place");
-        back.emplace_back(t.detach(), t.detach().contiguous());
-        work.push_back(back.back().second);
+        for (int64_t d = 0; d < t->dim(); ++d)
+          SEP_ASSERT(t->size(d) <= 1 || t->stride(d) != 0, "an expanded tensor cannot be changed in place");
+        copies.push_back(t->detach().contiguous());
+        back.push_back(t);
+        work.push_back(&copies.back());
       }
     }
     ranges.check();
   }
   void finish(const TensorList& tensors) {
-    for (auto& b : back) b.first.copy_(b.second);
-    for (const auto& t : tensors) changed(t);
+    for (size_t i = 0; i < back.size(); ++i) back[i]->detach().copy_(copies[i]);
+    for (const at::Tensor* t : tensors) changed(*t);
   }
 };
+
+// The device of a list; the current one for an empty list.
+at::Device device_of(const TensorList& tensors) {
+  if (tensors.empty()) return at::Device(at::kCUDA, c10::cuda::current_device());
+  SEP_ASSERT(tensors[0]->defined() && tensors[0]->is_cuda(), kListMessage);
+  return tensors[0]->device();
+}
 
 void check_max_norm(double max_norm) { SEP_ASSERT(max_norm >= 0.0, "max_norm must not be negative"); }
 
 }  // namespace
 
 std::pair<at::Tensor, at::Tensor> list_norm(const TensorList& tensors) {
-  const auto options = at::TensorOptions().device(tensors.empty() ? at::Device(at::kCUDA, c10::cuda::current_device()) : tensors[0].device());
-  if (!tensors.empty()) SEP_ASSERT(tensors[0].defined() && tensors[0].is_cuda(), "the tensors of a list must be dense tensors on one CUDA device");
-  const c10::cuda::CUDAGuard guard(options.device());
-  const TensorList list = readable(tensors);
-  if (list.empty()) return {at::zeros({}, options.dtype(at::kFloat)), at::zeros({}, options.dtype(at::kDouble))};
+  const at::Device device = device_of(tensors);
+  const auto options = at::TensorOptions().device(device);
+  const c10::cuda::CUDAGuard guard(device);
+  const Readable r(tensors, device);
+  if (r.list.empty()) return {at::zeros({}, options.dtype(at::kFloat)), at::zeros({}, options.dtype(at::kDouble))};
   const auto stream = at::cuda::getCurrentCUDAStream();
   const at::Tensor norm = at::empty({}, options.dtype(at::kFloat)), total = at::empty({}, options.dtype(at::kDouble));
   int count = 0;
-  const at::Tensor sums = squares(list, stream, count);
+  const at::Tensor sums = squares(r.list, stream, count);
   SEP_CUDA_CHECK(launch_list_norm(sums.data_ptr<double>(), count, norm.data_ptr<float>(), total.data_ptr<double>(), stream));
   return {norm, total};
 }
 
 at::Tensor list_clip(const TensorList& tensors, double max_norm) {
   check_max_norm(max_norm);
-  const auto options = at::TensorOptions().dtype(at::kFloat).device(tensors.empty() ? at::Device(at::kCUDA, c10::cuda::current_device()) : tensors[0].device());
-  if (!tensors.empty()) SEP_ASSERT(tensors[0].defined() && tensors[0].is_cuda(), "the tensors of a list must be dense tensors on one CUDA device");
-  const c10::cuda::CUDAGuard guard(options.device());
-  InPlace list(tensors);
+  const at::Device device = device_of(tensors);
+  const auto options = at::TensorOptions().device(device).dtype(at::kFloat);
+  const c10::cuda::CUDAGuard guard(device);
+  InPlace list(tensors, device);
   if (list.work.empty()) return at::zeros({}, options);
   const auto stream = at::cuda::getCurrentCUDAStream();
   const at::Tensor norm = at::empty({}, options);
@@ -167,10 +184,10 @@ at::Tensor list_clip(const TensorList& tensors, double max_norm) {
 void list_scale(const TensorList& tensors, const at::Tensor& norm, double max_norm) {
   check_max_norm(max_norm);
   if (tensors.empty()) return;
-  SEP_ASSERT(tensors[0].defined() && tensors[0].is_cuda(), "the tensors of a list must be dense tensors on one CUDA device");
-  SEP_ASSERT(norm.device() == tensors[0].device() && norm.scalar_type() == at::kFloat && norm.numel() == 1, "norm must be one float32 number on the tensors' device");
-  const c10::cuda::CUDAGuard guard(tensors[0].device());
-  InPlace list(tensors);
+  const at::Device device = device_of(tensors);
+  SEP_ASSERT(norm.device() == device && norm.scalar_type() == at::kFloat && norm.numel() == 1, "norm must be one float32 number on the tensors' device");
+  const c10::cuda::CUDAGuard guard(device);
+  InPlace list(tensors, device);
   if (list.work.empty()) return;
   scale_lists(list.work, nullptr, 0, norm.data_ptr<float>(), max_norm, at::cuda::getCurrentCUDAStream());
   list.finish(tensors);
@@ -185,47 +202,40 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
   SEP_ASSERT(o.lr >= 0.0 && o.eps >= 0.0 && o.weight_decay >= 0.0 && o.beta1 >= 0.0 && o.beta1 < 1.0 && o.beta2 >= 0.0 && o.beta2 < 1.0,
              "lr, eps and weight_decay must not be negative, betas within [0, 1)");
   if (n == 0) return;
-  SEP_ASSERT(params[0].defined() && params[0].is_cuda(), "params must be dense tensors on one CUDA device");
-  const at::Device device = params[0].device();
+  const at::Device device = device_of(params);
   if (norm.has_value())
     SEP_ASSERT(norm->device() == device && norm->scalar_type() == at::kFloat && norm->numel() == 1, "norm must be one float32 number on the parameters' device");
   const c10::cuda::CUDAGuard guard(device);
   const bool have_masters = !masters.empty();
-  TensorList held;                                   // gradients that had to be laid out like their parameters
-  std::vector<const at::Tensor*> grad_at(n);
-  held.reserve(n);
-  Ranges ranges;
+  std::deque<at::Tensor> held;                       // gradients that had to be laid out like their parameters
+  TensorList grad_at = grads;
+  Ranges ranges[4];
+  for (Ranges& r : ranges) r.all.reserve(n);
   int64_t elements = 0;
   for (size_t i = 0; i < n; ++i) {
-    const at::Tensor& p = params[i];
-    check_tensor(p, device, "params");
-    check_tensor(grads[i], device, "grads");
-    SEP_ASSERT(grads[i].sizes() == p.sizes(), "a gradient does not have its parameter's shape");
+    const at::Tensor &p = *params[i], &g = *grads[i];
+    SEP_ASSERT(usable(p, device) && usable(g, device), kListMessage);
+    SEP_ASSERT(g.sizes() == p.sizes(), "a gradient does not have its parameter's shape");
     SEP_ASSERT(p.is_non_overlapping_and_dense(), "a parameter with gaps or repeats in memory cannot be updated in place");
-    auto like = [&](const at::Tensor& t, const char* what) {
-      check_tensor(t, device, what);
-      SEP_ASSERT(t.scalar_type() == at::kFloat && t.sizes() == p.sizes() && (t.strides() == p.strides() || (t.is_contiguous() && p.is_contiguous())),
+    const bool plain = p.is_contiguous();
+    auto same_layout = [&](const at::Tensor& t) { return plain ? t.is_contiguous() : t.strides() == p.strides(); };
+    auto state = [&](const at::Tensor& t, const char* what, Ranges& r) {
+      SEP_ASSERT(usable(t, device) && t.scalar_type() == at::kFloat && t.sizes() == p.sizes() && same_layout(t),
                  what << " must be float32 and laid out like their parameters");
+      if (t.numel() > 0) r.add(t);
     };
-    like(exp_avgs[i], "exp_avgs");
-    like(exp_avg_sqs[i], "exp_avg_sqs");
-    if (have_masters) like(masters[i], "masters");
-    grad_at[i] = &grads[i];
-    if (!(grads[i].strides() == p.strides() || (grads[i].is_contiguous() && p.is_contiguous()))) {
-      held.push_back(at::empty_strided(p.sizes(), p.strides(), grads[i].options()));
-      held.back().copy_(grads[i].detach());
+    state(*exp_avgs[i], "exp_avgs", ranges[1]);
+    state(*exp_avg_sqs[i], "exp_avg_sqs", ranges[2]);
+    if (have_masters) state(*masters[i], "masters", ranges[3]);
+    if (!same_layout(g)) {
+      held.push_back(at::empty_strided(p.sizes(), p.strides(), g.options()));
+      held.back().copy_(g.detach());
       grad_at[i] = &held.back();
     }
-    if (p.numel() == 0) continue;
     elements += p.numel();
-    ranges.add(p); 
+    if (p.numel() > 0) ranges[0].add(p);
   }
-  ranges.check();
-  for (const TensorList* l : {&exp_avgs, &exp_avg_sqs, &masters}) {
-    Ranges r;
-    for (const auto& t : *l) if (t.numel() > 0) r.add(t);
-    r.check();
-  }
+  for (Ranges& r : ranges) r.check();
   AdamParams a{};
   const double c1 = 1.0 - std::pow(o.beta1, static_cast<double>(o.step)), c2 = 1.0 - std::pow(o.beta2, static_cast<double>(o.step));
   a.step_size = static_cast<float>(o.lr / c1);
@@ -248,15 +258,15 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
     list.count = 0; chunks = 0;
   };
   for (size_t i = 0; i < n; ++i) {
-    const at::Tensor &p = params[i], &g = *grad_at[i];
+    const at::Tensor &p = *params[i], &g = *grad_at[i];
     if (p.numel() == 0) continue;
     if (list.count == kAdamEntries) flush();
     const int at = list.count++;
     list.param[at] = p.data_ptr();
     list.grad[at] = g.data_ptr();
-    list.exp_avg[at] = exp_avgs[i].data_ptr<float>();
-    list.exp_avg_sq[at] = exp_avg_sqs[i].data_ptr<float>();
-    list.master[at] = have_masters ? masters[i].data_ptr<float>() : nullptr;
+    list.exp_avg[at] = static_cast<float*>(exp_avgs[i]->data_ptr());
+    list.exp_avg_sq[at] = static_cast<float*>(exp_avg_sqs[i]->data_ptr());
+    list.master[at] = have_masters ? static_cast<float*>(masters[i]->data_ptr()) : nullptr;
     // the first element at which all of them stand on a boundary of four elements
     auto place = [](const void* q, int width) { return static_cast<int>(reinterpret_cast<uintptr_t>(q) / width % 4); };
     const int off = place(list.exp_avg[at], 4);
@@ -271,7 +281,7 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
   }
   flush();
   for (const TensorList* l : {&params, &exp_avgs, &exp_avg_sqs, &masters})
-    for (const auto& t : *l) changed(t);
+    for (const at::Tensor* t : *l) changed(*t);
 }
 
 }  // namespace sep

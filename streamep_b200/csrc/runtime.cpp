@@ -2243,12 +2243,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return linear_loss([r](int launches) { return r->launch_context(launches); }, x, weight, targets, ignore_index, reduction);
       });
   m.def("linear_loss_schedule", &linear_loss_schedule);
-  m.def("list_norm", &list_norm);
-  m.def("list_clip", &list_clip);
-  m.def("list_scale", &list_scale);
-  m.def("list_adamw", [](const TensorList& params, const TensorList& grads, const TensorList& exp_avgs, const TensorList& exp_avg_sqs, const TensorList& masters,
-                         const std::optional<at::Tensor>& norm, int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
-                         double max_norm, bool skip_nonfinite) {
-    list_adamw(params, grads, exp_avgs, exp_avg_sqs, masters, norm, AdamOptions{step, lr, beta1, beta2, eps, weight_decay, max_norm, skip_nonfinite});
+  // Lists come as Python lists and their tensors are read in place: the generic conversion to a vector of tensors costs more than the
+  // launch from a hundred tensors up (four lists of 250: 86 -> 41 us a call).
+  auto tensors = [](const py::list& l) {
+    TensorList out;
+    out.reserve(l.size());
+    for (const py::handle h : l) {
+      SEP_ASSERT(THPVariable_Check(h.ptr()), "a list holds something that is not a tensor");
+      out.push_back(&THPVariable_Unpack(h.ptr()));
+    }
+    return out;
+  };
+  m.def("list_norm", [tensors](const py::list& l) { return list_norm(tensors(l)); });
+  m.def("list_clip", [tensors](const py::list& l, double max_norm) { return list_clip(tensors(l), max_norm); });
+  m.def("list_scale", [tensors](const py::list& l, const at::Tensor& norm, double max_norm) { list_scale(tensors(l), norm, max_norm); });
+  m.def("list_adamw", [tensors](const py::list& params, const py::list& grads, const py::list& exp_avgs, const py::list& exp_avg_sqs, const py::list& masters,
+                                const std::optional<at::Tensor>& norm, int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
+                                double max_norm, bool skip_nonfinite) {
+    list_adamw(tensors(params), tensors(grads), tensors(exp_avgs), tensors(exp_avg_sqs), tensors(masters), norm,
+               AdamOptions{step, lr, beta1, beta2, eps, weight_decay, max_norm, skip_nonfinite});
   });
 }

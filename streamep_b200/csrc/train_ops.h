@@ -29,10 +29,11 @@ enum LossReduction : int { kLossNone = 0, kLossMean = 1, kLossSum = 2 };
 at::Tensor linear_loss(const ContextFn& context, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets,
                        int64_t ignore_index, int reduction);
 // The backward's units in order, for the schedule's test: each {kind, piece, unit row, unit column, split, first k-block, k-blocks};
-// first of all {pieces, columns of a piece, splits, ahead, buffers, row units, split2}.
+// first of all {pieces, columns of a piece, splits, ahead, buffers, row units, split2, column tiles of a dw unit}.
 std::vector<std::vector<int>> linear_loss_schedule(int64_t tokens, int64_t hidden, int64_t vocab, int sms, bool want_dx, bool want_dw);
 
-using TensorList = std::vector<at::Tensor>;
+// Tensors that the caller (a Python list) keeps alive during the call.
+using TensorList = std::vector<const at::Tensor*>;
 // {norm (fp32), sum of squares (fp64)}, 0-dim
 std::pair<at::Tensor, at::Tensor> list_norm(const TensorList& tensors);
 at::Tensor list_clip(const TensorList& tensors, double max_norm);

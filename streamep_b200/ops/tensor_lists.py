@@ -69,6 +69,8 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
         raise ValueError(f"max_norm must not be negative (got {max_norm})")
     if skip_nonfinite and norm is None:
         raise ValueError("skip_nonfinite needs the gradients' norm (grad_norm)")
+    if masters is not None and len(masters) != len(params):
+        raise ValueError(f"{len(params)} params and {len(masters)} masters")
     _ext.load().list_adamw(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), list(masters) if masters is not None else [], norm,
                            int(step), float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
                            -1.0 if max_norm is None else float(max_norm), bool(skip_nonfinite))

@@ -17,7 +17,7 @@ def up(a, b):
 @pytest.mark.parametrize("T,H,V", [(1, 8, 1), (1, 64, 300), (64, 256, 1000), (128, 2048, 100003), (129, 520, 4097), (1777, 1000, 50257),
                                    (8192, 2048, 65536), (16384, 72, 131072), (300, 7168, 9000), (5003, 4096, 257)])
 def test_units_and_order(T, H, V, want_dx, want_dw):
-    (pieces, piece, splits, ahead, buffers, row_units, split2), *units = _ext.load().linear_loss_schedule(T, H, V, 148, want_dx, want_dw)
+    (pieces, piece, splits, ahead, buffers, row_units, split2, group), *units = _ext.load().linear_loss_schedule(T, H, V, 148, want_dx, want_dw)
     assert piece % 256 == 0 and (pieces - 1) * piece < V <= pieces * piece
     assert row_units == up(T, 256) and (not split2 or T <= 128) and pieces >= buffers >= min(ahead + 1, pieces)
     cols = [min(piece, V - j * piece) for j in range(pieces)]
@@ -28,7 +28,7 @@ def test_units_and_order(T, H, V, want_dx, want_dw):
         if want_dx:
             want |= {(DX, j, m, n, s) for m, n, s in itertools.product(range(row_units), range(up(H, 256)), range(splits))}
         if want_dw:
-            want |= {(DW, j, m, n, 0) for m, n in itertools.product(range(tiles), range(up(H, 256)))}
+            want |= {(DW, j, m, n, 0) for m, n in itertools.product(range(tiles), range(0, up(H, 256), group))}
     assert len(units) == len(want) and {tuple(u[:5]) for u in units} == want
     place = {}
     for i, u in enumerate(units):
