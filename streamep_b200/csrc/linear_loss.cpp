@@ -19,15 +19,23 @@ int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // One dz buffer holds at most about this much.  Larger pieces mean fewer passes over the fp32 sums of dx.
 constexpr int64_t kPieceBytes = 128ll << 20;
 constexpr int64_t kSplitTokens = 64;             // calls whose dz is kept as a sum of two bf16 numbers: one k-block of tokens
+constexpr int64_t kNarrowTokens = 1024;
 constexpr int64_t kBandBytes = 48ll << 20;       // rows of x that a band of units shares in L2
 
+// Tokens as columns (the narrow form) where that multiplies at least an eighth less, among calls that are short enough for its more
+// numerous softmax parts; always where dz is split.
+void plan_tiles(LossParams& p) {
+  const int64_t T = p.T, units = ceil_of(T, kLossUnit), tokens = ceil_of(ceil_of(T, units), 32) * 32;
+  p.narrow = T <= kSplitTokens || (T <= kNarrowTokens && tokens * units * 8 <= 7 * kLossUnit * units);
+  p.tile_tokens = p.narrow ? static_cast<int>(tokens) : kLossUnit;
+  p.row_units = static_cast<int>(units);
+  loss_narrow_ring(p);
+}
 void plan_backward(LossParams& p, int sms) {
   const int64_t T = p.T, H = p.H, V = p.V, pairs = sms / 2;
-  p.row_units = static_cast<int>(ceil_of(T, kLossUnit));
   p.h_units = static_cast<int>(ceil_of(H, kLossUnit));
   // Short calls keep dz to 16 bits of mantissa, as a sum of two bf16 numbers: rounding errors of many tokens average out in dW,
-  // those of a few do not (one token, target at p = 0.5: dW 0.4 % off where the result's own rounding is 0.2 %).  The remainders sit
-  // where the second CTA's rows of a unit would be empty, so they cost no further products.
+  // those of a few do not (one token, target at p = 0.5: dW 0.4 % off where the result's own rounding is 0.2 %).
   p.split2 = T <= kSplitTokens ? 1 : 0;
   const int64_t row_bytes = T * 2 * (p.split2 ? 2 : 1);
   const int64_t want = ceil_of(V * row_bytes, kPieceBytes);
@@ -36,24 +44,32 @@ void plan_backward(LossParams& p, int sms) {
   p.last_cols = static_cast<int>(V - static_cast<int64_t>(p.pieces - 1) * p.piece);
   p.ahead = std::min(1, p.pieces);
   p.buffers = std::min(p.ahead + 1, p.pieces);
-  // A single piece: nothing but its dz stands before its products, and dw units can begin on the first finished column tiles.
-  p.dw_first = p.pieces == 1 ? 1 : 0;
   const int64_t v_blocks = ceil_of(V, 64), t_blocks = ceil_of(T, 64) * (p.split2 ? 2 : 1), tiles = ceil_of(V, kLossUnit);
   // k-blocks of all the work, for each pair
   const int64_t all = (p.row_units * tiles * ceil_of(H, 64) + (p.want_dx ? p.row_units * p.h_units * v_blocks : 0) +
                        (p.want_dw ? tiles * p.h_units * t_blocks : 0)) / pairs + 1;
   // dx units of one place follow each other piece by piece: a chain of v_blocks / splits k-blocks, which is to stay within half of the
-  // time that the whole takes; and a unit within an eighth of it, so that pairs end together.
-  const int64_t piece_blocks = ceil_of(std::min<int64_t>(V, p.piece), 64);
-  // But no more than keep the traffic of the partial sums (4 bytes, written and read) within an eighth of reading the projection.
-  const int64_t chain = ceil_of(2 * v_blocks, all), even = std::min(ceil_of(8 * piece_blocks, all), V / (32 * T * (p.split2 ? 2 : 1)));
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min({std::max(chain, even), piece_blocks / 4, static_cast<int64_t>(64)})));
+  // time that the whole takes; and a unit within an eighth of it, so that pairs end together.  But no more splits than keep the
+  // traffic of the partial sums (4 bytes, written and read) within an eighth of reading the projection.  Where the dx units of a piece
+  // are few rounds of all pairs, the number whose rounds are fullest is taken.
+  const int64_t piece_blocks = ceil_of(std::min<int64_t>(V, p.piece), 64), places = static_cast<int64_t>(p.row_units) * p.h_units;
+  const int64_t chain = ceil_of(2 * v_blocks, all), even = std::min(ceil_of(8 * piece_blocks, all), V / (32 * T));
+  const int64_t most = std::max<int64_t>(1, std::min({std::max(chain, even), piece_blocks / 4, static_cast<int64_t>(64)}));
+  int64_t best = most, best_time = -1;
+  for (int64_t s = std::max<int64_t>(1, std::max(chain, most / 2)); s <= most; ++s) {
+    const int64_t time = ceil_of(places * s, pairs) * ceil_of(piece_blocks, s);
+    if (best_time < 0 || time < best_time) { best = s; best_time = time; }
+  }
+  p.splits = static_cast<int>(best);
   p.split_blocks = static_cast<int>(ceil_of(piece_blocks, p.splits));
   p.splits = static_cast<int>(ceil_of(piece_blocks, p.split_blocks));
   // dw units of few k-blocks take several column tiles, as long as there are a few units for every pair: claiming one and asking
   // whether its dz is there takes longer than its products.
   const int64_t per_pair = tiles * p.h_units / pairs;
   p.dw_group = static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(p.h_units), 24 / t_blocks, per_pair / 4})));
+  // A single piece has nothing but its own dz ahead of its products.  Some dw units, which can begin on the first finished column
+  // tiles of dz, bridge the wait for the last ones; the others come after the longer dx units.
+  p.dw_lead = p.pieces == 1 ? static_cast<int>(pairs) : 0;
 }
 // Units of few k-blocks are claimed further ahead: a claim takes about as long as the operands of four k-blocks.
 int claim_lead(const LossParams& p, bool backward) {
@@ -62,10 +78,8 @@ int claim_lead(const LossParams& p, bool backward) {
 }
 void plan_band(LossParams& p) {
   const int64_t rows = std::max<int64_t>(kBandBytes / (2 * static_cast<int64_t>(p.H)), kLossUnit);
-  p.row_units = static_cast<int>(ceil_of(p.T, kLossUnit));
-  p.x_rows = static_cast<int>(std::min<int64_t>(128, ceil_of(p.T, 8) * 8));
   // bands of equal height
-  const int64_t bands = ceil_of(p.row_units, std::max<int64_t>(rows / kLossUnit, 1));
+  const int64_t bands = ceil_of(p.row_units, std::max<int64_t>(rows / p.tile_tokens, 1));
   p.band = static_cast<int>(ceil_of(p.row_units, bands));
 }
 
@@ -99,6 +113,7 @@ LossParams plan(int64_t T, int64_t H, int64_t V, bool want_dx, bool want_dw, int
   LossParams p{};
   p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
   p.want_dx = want_dx; p.want_dw = want_dw;
+  plan_tiles(p);
   plan_backward(p, sms);
   plan_band(p);
   p.claim_lead = claim_lead(p, true);
@@ -118,16 +133,16 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   }
   out.loss = reduced ? at::empty({}, f32) : at::empty({T}, f32);
   const LaunchContext ctx = call.context(2);
-  const int64_t parts = ceil_of(V, kLossPart);
+  LossParams p{};
+  p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
+  plan_tiles(p);
+  plan_band(p);
+  p.claim_lead = claim_lead(p, false);
+  const int64_t parts = loss_forward_parts(p, ctx.sms);
   Carver c;
   const int64_t counters = c.take(64), part_at = c.take(parts * T * 8), logit_at = c.take(T * 4), each_at = reduced ? c.take(T * 4) : 0;
   const at::Tensor space = at::empty({c.bytes}, x.options().dtype(at::kByte));
   char* base = static_cast<char*>(space.data_ptr());
-
-  LossParams p{};
-  p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
-  plan_band(p);
-  p.claim_lead = claim_lead(p, false);
   p.parts = reinterpret_cast<float2*>(base + part_at);
   p.target_logit = reinterpret_cast<float*>(base + logit_at);
   p.targets = reinterpret_cast<const long long*>(targets.data_ptr<int64_t>());
@@ -143,7 +158,7 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   }
   p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
   LossMaps m{};
-  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, p.x_rows);
+  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, p.tile_tokens / 2);
   m.w_k = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 128);
   if (static_cast<int64_t>(p.row_units) * ceil_of(V, kLossUnit) > ctx.sms / 2) {      // (else every pair has one unit at most)
     p.claim = reinterpret_cast<int*>(base + counters);
@@ -181,7 +196,7 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
 
   LossParams p = plan(T, H, V, want_dx, want_dw, ctx.sms);
   SEP_ASSERT(loss_backward_units(p) < (1ll << 30), "this loss has too many tiles for one call: split the tokens");
-  const int64_t z_layers = p.split2 ? 2 : 1, slots = static_cast<int64_t>(p.splits) * z_layers;
+  const int64_t z_layers = p.split2 ? 2 : 1, slots = p.splits;
   Carver c;
   const int64_t z_at = c.take(p.buffers * z_layers * T * p.piece * 2), dx_at = want_dx ? c.take(slots * T * H * 4) : 0;
   const at::Tensor space = at::empty({c.bytes}, x.options().dtype(at::kByte));
@@ -197,19 +212,18 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
   p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
 
   LossMaps m{};
-  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, p.x_rows);
+  m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, p.tile_tokens / 2);
   m.w_k = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 128);
   if (want_dw) m.x_mn = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, 64);
   if (want_dx) m.w_mn = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 64);
-  for (int i = p.pieces > 1 ? 0 : 1; i < 2; ++i) {
-    // of the last piece only the columns that exist (up to whole 16 bytes, zeros in between) are stored and read back
-    const int64_t cols = i == 0 ? p.piece : ceil_of(p.last_cols, 8) * 8, layers = p.buffers * z_layers;
-    if (want_dx) m.z_k[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, p.x_rows);
-    if (want_dw) m.z_mn[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, 64);
-    m.z_out[i] = make_tmap(base + z_at, cols, T, layers, p.piece, T * p.piece, 64, 32);
-  }
+  const int64_t panels = p.buffers * z_layers * (p.piece / 64);
+  auto z_map = [&](int cols, int rows, CUtensorMapSwizzle swizzle) { return make_tmap(base + z_at, 64, T, panels, 64, T * 64, cols, rows, swizzle); };
+  if (want_dx) m.z_k = z_map(64, p.split2 ? p.tile_tokens : p.tile_tokens / 2, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (want_dw) m.z_mn = z_map(64, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+  m.z_out = p.narrow ? z_map(32, 32, CU_TENSOR_MAP_SWIZZLE_64B) : z_map(64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
   if (want_dw) m.dw = make_tmap(dw.data_ptr(), H, V, 1, H, H * V, 64, 32);
-  if (want_dx) m.dx = make_tmap(base + dx_at, H, T, slots, H, T * H, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
+  p.dx_parts = reinterpret_cast<float*>(base + dx_at);
+  if (want_dx && !p.narrow) m.dx = make_tmap(base + dx_at, H, T, slots, H, T * H, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
   if (call.counters_used) SEP_CUDA_CHECK(cudaMemsetAsync(p.claim, 0, counter_ints(p) * sizeof(int), ctx.stream));
   call.counters_used = true;
   SEP_CUDA_CHECK(launch_loss_backward(p, m, ctx.sms, ctx.stream));

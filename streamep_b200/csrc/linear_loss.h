@@ -8,18 +8,21 @@
 namespace sep {
 
 constexpr int kLossUnit = 256;        // rows and columns of a unit of work: one tile of a CTA pair
-constexpr int kLossPart = 128;        // columns that one thread reduces: the softmax statistics come in parts of this many
+constexpr int kLossPart = 128;        // columns that one thread reduces: the softmax statistics come in parts of this many (narrow form: one
+                                      // part for each quarter of every CTA)
 
 // Kinds of work.  Forward: kLossStats.  Backward, for each piece of the vocabulary: kLossDz, then kLossDx and kLossDw.
 enum LossKind : int { kLossStats = 0, kLossDz = 1, kLossDx = 2, kLossDw = 3 };
 
 struct LossParams {
   int T, H, V;
-  int x_rows;                    // rows of x (and dz, split2) that a CTA loads into its half of a unit: 128, or what a short call has
-  int row_units;                 // ceil(T / 256)
+  int narrow;                    // 1: tokens are the columns of a unit (see linear_loss_kernels.cu), `tile_tokens` of them
+  int tile_tokens;               // tokens of a unit: 256, narrow: a multiple of 32
+  int row_units;                 // ceil(T / tile_tokens)
+  int stages, stage_bytes;       // narrow forward: the operand ring
   int band;                      // row units that are walked together (see unit_of)
   // --- forward ---
-  float2* parts;                 // [ceil(V / 128)][T] running maximum and sum of exp(z - maximum) of 128 columns
+  float2* parts;                 // [loss_forward_parts][T] maximum and sum of exp(z - maximum)
   float* target_logit;           // [T]
   const long long* targets;      // [T]
   long long ignore_index;
@@ -33,7 +36,8 @@ struct LossParams {
   int pieces, last_cols;         // how many, and the columns of the last
   int ahead;                     // pieces whose dz is computed before the first product is taken from one
   int buffers;                   // dz buffers in rotation, > ahead
-  int split2;                    // 1: dz is kept as the sum of two bf16 numbers (short calls)
+  int split2;                    // 1: dz is kept as the sum of two bf16 numbers (short calls, narrow)
+  float* dx_parts;               // narrow: [splits][T][H]
   int want_dx, want_dw;
   int splits;                    // reductions over a piece of the vocabulary into which a dx unit is split
   int split_blocks;              // k-blocks of each but the last
@@ -43,18 +47,21 @@ struct LossParams {
   int claim_lead;                // units that are claimed ahead of the one whose operands are being requested, beyond the next
   int* done;                     // epilogue warps that have finished units, zero on entry: [3][pieces] of a piece's dz / dx / dw,
                                  // then [pieces][piece / 256] of the dz of one column tile
-  int dw_first;                  // the dw units of a piece come before its dx units
+  int dw_lead;                   // dw units of a piece that come before its dx units
   StatusBlock* status;
   int rank;
   unsigned long long wait_budget_ns;
 };
 
-struct LossMaps {                // CUtensorMap each: loads in boxes of 64 columns by 128 (k: K-major) or 64 (mn) rows
+struct LossMaps {                // CUtensorMap each: loads in boxes of 64 columns by 128 (k: K-major; narrow: x and dz by what a CTA
+                                 // takes of the tokens) or 64 (mn) rows
   CUtensorMap x_k, x_mn, w_k, w_mn;
-  CUtensorMap z_k[2], z_mn[2], z_out[2];    // [0] full pieces, [1] the last one
+  CUtensorMap z_k, z_mn, z_out;
   CUtensorMap dw, dx;
 };
 
+void loss_narrow_ring(LossParams& p);      // stages and stage_bytes of the narrow forward
+long long loss_forward_parts(const LossParams& p, int sms);
 cudaError_t launch_loss_forward(const LossParams& p, const LossMaps& m, int sms, cudaStream_t stream);
 cudaError_t launch_loss_backward(const LossParams& p, const LossMaps& m, int sms, cudaStream_t stream);
 long long loss_backward_units(const LossParams& p);

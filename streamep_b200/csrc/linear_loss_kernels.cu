@@ -10,6 +10,10 @@
 // What bounds it: the tensor cores, 2THV operations forward and 6THV backward (one of the three products is the recomputation, the price
 // of not keeping the logits); below a few hundred tokens the reads of W and the writes of dW.
 //
+// Two forms.  The tensor cores multiply 256 rows at a time however few of them exist, so with the tokens as rows a call of 300 pays for 512
+// and one of 1 for 256.  The narrow form makes the vocabulary (for dx: the hidden dimension) the rows, and 32 to 256 tokens the columns of
+// a unit, which cost what they are; its epilogues turn 32 x 32 pieces around in shared memory, so that a thread has a token again.
+//
 // Order and progress.  Units are claimed one after another from a counter, by CTAs that run, so a unit that waits for others
 // only waits for units that are already being worked on: the kernel needs no number of co-resident CTAs.
 #include <atomic>
@@ -29,8 +33,14 @@ constexpr int kThreads = (2 + kEpiWarps + 1) * 32;   // 0 TMA producer, 1 MMA, 2
 constexpr int kStagingBytes = 2 * 4096;          // per epilogue warp of the backward: two tiles of 32 rows of 128 bytes
 constexpr int kQueue = 4;
 // The forward's epilogue stores nothing but statistics, so all shared memory is its operand ring's.
-constexpr int stages_of(bool fwd) { return fwd ? 7 : 5; }
-constexpr int smem_bytes(bool fwd) { return stages_of(fwd) * kStageBytes + (fwd ? 0 : kEpiWarps * kStagingBytes) + 1024; }
+// The narrow forward needs one tile a warp, keeps each warp's statistics of all its units beside it (a part for every 32 columns made the
+// joining kernel longer than the product: 100 tokens, V 100003 92 -> 108 us), and has as many stages as its few tokens leave room for.
+constexpr int kNarrowStages = 9, kNarrowRing = 5 * kStageBytes;
+constexpr int kNarrowUnits = 4;                  // token tiles of the narrow form, at most
+constexpr int kNarrowStats = kNarrowUnits * 4 * 32 * 8;   // bytes a warp: [token tile][its 32-token pieces][lane] (maximum, sum)
+constexpr int stages_of(bool fwd, bool narrow) { return fwd ? (narrow ? kNarrowStages : 7) : 5; }
+constexpr int ring_bytes(bool fwd, bool narrow) { return fwd && narrow ? kNarrowRing : stages_of(fwd, narrow) * kStageBytes; }
+constexpr int smem_bytes(bool fwd, bool narrow) { return ring_bytes(fwd, narrow) + (fwd ? (narrow ? kEpiWarps * (4096 + kNarrowStats) : 0) : kEpiWarps * kStagingBytes) + 1024; }
 constexpr int kTmemCols = 512;
 constexpr int kDoneWarps = 2 * kEpiWarps;        // reports per unit
 // The scheduler claims the next unit when the producer has this many k-blocks of the one before left: a claimed unit is work that
@@ -79,7 +89,8 @@ __host__ __device__ inline Counts loss_counts(const LossParams& p) {
   return c;
 }
 
-// Backward order: dz of the first `ahead` pieces; then for each piece j: dz of piece j + ahead, dx and dW of piece j.
+// Backward order: dz of the first `ahead` pieces; then for each piece j: dz of piece j + ahead, dx and dW of piece j (`dw_lead` dw units of
+// it before the dx units).
 __host__ __device__ __forceinline__ Unit unit_of(const LossParams& p, int lin) {
   const Counts c = loss_counts(p);
   Unit u;
@@ -111,9 +122,10 @@ __host__ __device__ __forceinline__ Unit unit_of(const LossParams& p, int lin) {
       piece = j + p.ahead;
     } else {
       rem -= here;
-      const int first = p.dw_first ? (j == last ? c.dw_last : c.dw) : c.dx;
-      kind = (rem < first) == (p.dw_first != 0) ? kLossDw : kLossDx;
-      if (rem >= first) rem -= first;
+      const int lead_dw = lesser(p.dw_lead, j == last ? c.dw_last : c.dw);
+      kind = rem >= lead_dw && rem < lead_dw + c.dx ? kLossDx : kLossDw;
+      if (kind == kLossDx) rem -= lead_dw;
+      else if (rem >= lead_dw) rem -= c.dx;
     }
   }
   u.kind = kind; u.piece = piece; u.last = piece == last;
@@ -136,6 +148,12 @@ __host__ __device__ __forceinline__ Unit unit_of(const LossParams& p, int lin) {
   return u;
 }
 
+// dz lies in panels of 64 columns, [panel][T][64]: what a load or a store moves is one contiguous block (with rows of a whole piece,
+// 128 bytes here and the next 200 KB away, PANELNOTE).  The first panel of a piece, of its leading halves or (split2) remainders:
+__device__ __forceinline__ int panel_of(const LossParams& p, int piece, int rest) {
+  return ((piece % p.buffers) * (p.split2 ? 2 : 1) + rest) * (p.piece / 64);
+}
+
 // Columns of a tile that are multiplied (a multiple of 32, at most 256).
 __device__ __forceinline__ int tile_cols(int n, int n0) { return min(kLossUnit, (n - n0 + 31) / 32 * 32); }
 
@@ -153,14 +171,26 @@ __device__ __forceinline__ void tma_reduce_add_3d(const void* tmap, const void* 
                :: "l"(tmap), "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
-template <bool FWD>
+// Lane l has element i of 32 in v[i]; afterwards lane l has in v[j] what lane j had in v[l].  `tile`: 4 KB of the warp's own.
+__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void turn_write(uint32_t tile, int lane, int i, float v) { st_shared_f32(tile + (i * 32 + (lane ^ i)) * 4, v); }
+__device__ __forceinline__ float turn_read(uint32_t tile, int lane, int j) { return ld_shared_f32(tile + (lane * 32 + (j ^ lane)) * 4); }
+
+template <bool FWD, bool NARROW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__ LossMaps maps) {
-  constexpr int kStages = stages_of(FWD);
+  constexpr int kStages = stages_of(FWD, NARROW);
+  const int stages = FWD && NARROW ? p.stages : kStages;
+  const int stage_bytes = FWD && NARROW ? p.stage_bytes : kStageBytes;
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   unsigned char* stage_base = smem;
-  unsigned char* staging = smem + kStages * kStageBytes;
+  unsigned char* staging = smem + ring_bytes(FWD, NARROW);
   __shared__ uint64_t full_bar[kStages], empty_bar[kStages], tmem_full[2], tmem_empty[2], queue_full[kQueue], queue_empty[kQueue];
   __shared__ int s_queue[kQueue];
   __shared__ int s_progress;           // units whose operands the producer has nearly all requested
@@ -284,50 +314,49 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         const int n_cols = (u.kind <= kLossDz) ? (FWD ? p.V : (u.last ? p.last_cols : p.piece)) : p.H;
         const int a0 = u.m * kLossUnit + half * 128;
         const int v0 = u.piece * (FWD ? 0 : p.piece);
-        const int zbuf = FWD ? 0 : (u.piece % p.buffers) * (p.split2 ? 2 : 1);
+        const int z0 = FWD ? 0 : panel_of(p, u.piece, 0);
         const int t_blocks = ceil_div(p.T, kBK);
-        // Short calls load only the rows that exist (what else the buffer holds ends up in accumulator rows that nobody reads): of one
-        // token at H 4096, V 128000 221 -> 198 us, since rows out of bounds cost the copy unit as much as others.
-        const bool short_rows = p.x_rows < 128 && (FWD || u.kind != kLossDw);
-        const bool load_a = !short_rows || half == 0 || (!FWD && u.kind == kLossDx);
-        const uint32_t pair_bytes = !short_rows ? 2 * kStageBytes
-            : 2 * kOperandBytes + p.x_rows * 128 * (!FWD && u.kind == kLossDx ? 2 : 1);
+        // narrow: rows of x / dz that this CTA loads, and which (split2: the leading halves of dz by the first CTA, the remainders by the second)
+        const bool both = NARROW && !FWD && u.kind == kLossDx && p.split2;
+        const int my_tokens = NARROW ? (both ? p.tile_tokens : p.tile_tokens / 2) : 0;
+        const int t0 = NARROW ? u.m * p.tile_tokens + (both ? 0 : half * my_tokens) : 0;
+        const uint32_t pair_bytes = NARROW && (FWD || u.kind != kLossDw) ? 2 * (kOperandBytes + my_tokens * 128) : 2 * kStageBytes;
         const int warn = max(u.k_blocks - kClaimAhead, 0);
         if (u.k_blocks == 0 && leader) st_volatile_shared(&s_progress, it + 1);
         for (int tile = 0; tile < u.tiles && ok; ++tile, ++u.n) {
         const int n0 = u.n * kLossUnit;
-        const int b0 = n0 + half * (tile_cols(n_cols, n0) / 2);
+        const int b0 = n0 + half * (NARROW && (FWD || u.kind != kLossDw) ? 128 : tile_cols(n_cols, n0) / 2);
         for (int kb = 0; kb < u.k_blocks; ++kb) {
           if (leader && kb == warn && tile == u.tiles - 1) st_volatile_shared(&s_progress, it + 1);
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, budget, p.status)) {
             report_failure(p.status, kStatusTimeoutPipeline, kKernelLoss, 0, p.rank, lin, kb, stage);
             ok = false; break;
           }
-          unsigned char* sa = stage_base + stage * kStageBytes;
+          unsigned char* sa = stage_base + stage * stage_bytes;
           unsigned char* sb = sa + kOperandBytes;
           // Both CTAs' bytes are counted on the first CTA's barrier, which that CTA arms for the sum.
           if (leader) mbar_arrive_expect_tx(&full_bar[stage], pair_bytes);
           const uint32_t bar = cluster_map(&full_bar[stage], 0);
           const int k = (u.k0 + kb) * kBK;
           if (FWD || u.kind == kLossDz) {
-            if (load_a) tma_load_3d_pair(sa, &maps.x_k, bar, k, a0, 0);
-            tma_load_3d_pair(sb, &maps.w_k, bar, k, v0 + b0, 0);
+            tma_load_3d_pair(sa, NARROW ? &maps.w_k : &maps.x_k, bar, k, NARROW ? v0 + b0 : a0, 0);
+            tma_load_3d_pair(sb, NARROW ? &maps.x_k : &maps.w_k, bar, k, NARROW ? t0 : v0 + b0, 0);
           } else if (u.kind == kLossDx) {
-            // split2: the first CTA multiplies the leading halves of dz, the second the remainders
-            if (p.split2) tma_load_3d_pair(sa, &maps.z_k[u.last], bar, k, 0, zbuf + half);
-            else tma_load_3d_pair(sa, &maps.z_k[u.last], bar, k, a0, zbuf);
-            tma_load_3d_pair(sb, &maps.w_mn, bar, b0, v0 + k, 0);
-            tma_load_3d_pair(sb + kOperandBytes / 2, &maps.w_mn, bar, b0 + 64, v0 + k, 0);
+            unsigned char* sw = NARROW ? sa : sb;
+            tma_load_3d_pair(NARROW ? sb : sa, &maps.z_k, bar, 0, NARROW ? t0 : a0, (both && half ? panel_of(p, u.piece, 1) : z0) + u.k0 + kb);
+            tma_load_3d_pair(sw, &maps.w_mn, bar, b0, v0 + k, 0);
+            tma_load_3d_pair(sw + kOperandBytes / 2, &maps.w_mn, bar, b0 + 64, v0 + k, 0);
           } else {
             const int rest = kb >= t_blocks ? 1 : 0;         // split2: all leading halves, then all remainders
             const int t = (kb - rest * t_blocks) * kBK;
-            tma_load_3d_pair(sa, &maps.z_mn[u.last], bar, a0, t, zbuf + rest);
-            tma_load_3d_pair(sa + kOperandBytes / 2, &maps.z_mn[u.last], bar, a0 + 64, t, zbuf + rest);
+            const int panel = (rest ? panel_of(p, u.piece, 1) : z0) + a0 / 64;
+            tma_load_3d_pair(sa, &maps.z_mn, bar, 0, t, panel);
+            tma_load_3d_pair(sa + kOperandBytes / 2, &maps.z_mn, bar, 0, t, panel + 1);
             tma_load_3d_pair(sb, &maps.x_mn, bar, b0, t, 0);
             tma_load_3d_pair(sb + kOperandBytes / 2, &maps.x_mn, bar, b0 + 64, t, 0);
           }
           ++issued;
-          if (++stage == kStages) { stage = 0; phase ^= 1; }
+          if (++stage == stages) { stage = 0; phase ^= 1; }
         }
         }
       }
@@ -339,7 +368,6 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (first CTA of a pair)
     if (leader) {
-      constexpr uint32_t idesc_kk = umma_idesc_bf16(256, 0, 0, 0), idesc_km = umma_idesc_bf16(256, 0, 0, 1), idesc_mm = umma_idesc_bf16(256, 0, 1, 1);
       int stage = 0; uint32_t phase = 0; int acc = 0; uint32_t acc_phase = 0; bool ok = true;
       for (int it = 0; ok; ++it) {
         int lin = 0;
@@ -349,10 +377,12 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         if (lin >= total) break;
         Unit u = decode(lin);
         if (u.k_blocks == 0) continue;
-        const bool a_mn = !FWD && u.kind == kLossDw, b_mn = !FWD && u.kind >= kLossDx;
+        const bool a_mn = !FWD && (u.kind == kLossDw || (NARROW && u.kind == kLossDx)), b_mn = !FWD && (u.kind == kLossDw || (!NARROW && u.kind == kLossDx));
+        const bool tokens = NARROW && (FWD || u.kind != kLossDw);      // columns are tokens
         const int n_cols = (u.kind <= kLossDz) ? (FWD ? p.V : (u.last ? p.last_cols : p.piece)) : p.H;
         for (int tile = 0; tile < u.tiles && ok; ++tile, ++u.n) {
-        const uint32_t idesc = (a_mn ? idesc_mm : b_mn ? idesc_km : idesc_kk) | (static_cast<uint32_t>(tile_cols(n_cols, u.n * kLossUnit) >> 3) << 17);
+        const int cols = tokens ? (!FWD && u.kind == kLossDx && p.split2 ? 2 : 1) * p.tile_tokens : tile_cols(n_cols, u.n * kLossUnit);
+        const uint32_t idesc = umma_idesc_bf16(256, 0, 0, 0) | (a_mn ? 1u << 15 : 0) | (b_mn ? 1u << 16 : 0) | (static_cast<uint32_t>(cols >> 3) << 17);
         // per 16 elements of K: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major box
         const uint32_t step_a = a_mn ? 16 * 128 : 32, step_b = b_mn ? 16 * 128 : 32;
         const uint32_t lbo_a = a_mn ? kBK * 128 : 16, lbo_b = b_mn ? kBK * 128 : 16;
@@ -366,7 +396,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           if (!__all_sync(0xffffffffu, mbar_wait<true>(&full_bar[stage], phase, budget, p.status))) { ok = false; break; }
           tc_fence_after_sync();
           if (elect_one()) {
-            const uint32_t a_addr = smem_u32(stage_base + stage * kStageBytes), b_addr = a_addr + kOperandBytes;
+            const uint32_t a_addr = smem_u32(stage_base + stage * stage_bytes), b_addr = a_addr + kOperandBytes;
 #pragma unroll
             for (int j = 0; j < kBK / 16; ++j)
               umma_bf16_ss<2>(tmem_d, umma_smem_desc(a_addr + j * step_a, lbo_a, 1024), umma_smem_desc(b_addr + j * step_b, lbo_b, 1024),
@@ -375,7 +405,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
             if (kb == end - 1) umma_commit<2>(&tmem_full[acc]);
           }
           __syncwarp();
-          if (++stage == kStages) { stage = 0; phase ^= 1; }
+          if (++stage == stages) { stage = 0; phase ^= 1; }
         }
         acc ^= 1; if (acc == 0) acc_phase ^= 1;
         }
@@ -388,7 +418,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
     // warps 2..5 the left 128 columns of the tile and warps 6..9 the right ones.  Warps do not wait for one another.
     const int quarter = warp & 3, side = (warp - 2) >> 2;
     // A tile of results is written to shared memory and leaves by a bulk store, while the warp fills the other one.
-    unsigned char* stage_tile = staging + (warp - 2) * kStagingBytes;
+    unsigned char* stage_tile = staging + (warp - 2) * (FWD ? 4096 : kStagingBytes);
     auto next_tile = [&] {               // whole warp: the tile that the store before the last one has read
       stage_tile = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(stage_tile) ^ 4096);
       if (lane == 0) bulk_wait_read_but_one();
@@ -396,6 +426,15 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
       return smem_u32(stage_tile);
     };
     uint32_t stg = 0;
+    // narrow: this warp's 32-token pieces of a unit
+    const int pieces32 = NARROW ? p.tile_tokens / 32 : 0;
+    const int first32 = side == 0 ? 0 : (pieces32 + 1) / 2, count32 = side == 0 ? (pieces32 + 1) / 2 : pieces32 / 2;
+    const uint32_t turn = smem_u32(stage_tile);                    // narrow: where pieces are turned around ...
+    unsigned char* const narrow_out = stage_tile + 4096;           // ... and where dz waits for its stores
+    int flip = 0;
+    float2* const stats = reinterpret_cast<float2*>(staging + kEpiWarps * 4096 + (warp - 2) * kNarrowStats) + lane;    // (forward) [unit row * 4 + piece] * 32
+    if (FWD && NARROW)
+      for (int i = 0; i < kNarrowUnits * 4; ++i) stats[i * 32] = make_float2(__int_as_float(0xff800000), 0.f);
     float scale = 1.f;                   // of dw
     if (!FWD && p.scale != nullptr) scale = *p.scale;
     if (!FWD && p.scale2 != nullptr) scale *= *p.scale2;
@@ -418,7 +457,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
       // fetched while the tensor cores still work on the tile
       int col = -1; float lse2 = 0.f, c_t = 0.f;
       bool dead = true;              // an ignored token (or no token): zeros whatever its logits are
-      if (u.kind <= kLossDz) {
+      if (!NARROW && u.kind <= kLossDz) {
         if (row < p.T) {
           const long long y = p.targets[row];
           const long long rel = y - (FWD ? 0 : static_cast<long long>(u.piece) * p.piece) - n0;
@@ -439,7 +478,9 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         return true;
       };
       if (!FWD && !empty && !(ok = accumulated())) break;
-      const uint32_t lanes = tmem_base + side * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
+      const bool tokens = NARROW && (FWD || u.kind != kLossDw);      // columns are tokens
+      const uint32_t lanes = tmem_base + (tokens ? first32 * 32 : side * 128) + (static_cast<uint32_t>(quarter * 32) << 16);
+      const int v_first = u.n * kLossUnit + half * 128 + quarter * 32;   // (tokens) first row of this warp: in the vocabulary's piece, or of H
       const uint32_t taddr = lanes + acc * kLossUnit;
       auto give_back = [&] {
         tc_fence_before_sync();
@@ -455,7 +496,149 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           tmem_ld_32x32(taddr + c * 32, r); tmem_ld_wait();
         }
       };
-      if (FWD) {
+      if (FWD && NARROW) {
+        float z[128];
+#pragma unroll
+        for (int i = 0; i < 128; ++i) z[i] = 0.f;
+        for (int first = 0; first < u.k_blocks; first += kSegmentBlocks) {
+          if (!(ok = accumulated())) break;
+          if (count32 == 0) give_back();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            if (c < 2 * count32) {
+              uint32_t part[16];
+              tmem_ld_32x16(lanes + acc * kLossUnit + c * 16, part); tmem_ld_wait();
+              if (c == 2 * count32 - 1) give_back();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) z[c * 16 + i] += __uint_as_float(part[i]);
+            }
+          }
+          acc ^= 1; if (acc == 0) acc_phase ^= 1;
+        }
+        if (!ok) break;
+        if (v_first >= p.V) continue;
+        const float ninf = __int_as_float(0xff800000);
+        const bool exists = v_first + lane < p.V;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c < count32) {
+            const int t = u.m * p.tile_tokens + (first32 + c) * 32 + lane;
+            const long long y = t < p.T ? p.targets[t] : -1;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) turn_write(turn, lane, i, exists ? z[c * 32 + i] : ninf);
+            __syncwarp();
+            float2& so_far = stats[(u.m * 4 + c) * 32];
+            const float2 before = so_far;
+            float v[32], top[4] = {before.x, ninf, ninf, ninf}, s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 32; ++j) { v[j] = turn_read(turn, lane, j); top[j & 3] = fmaxf(top[j & 3], v[j]); }
+            const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const float ref = m == ninf ? 0.f : m * kLog2e;      // (a row of -inf: subtract 0, every term is exp(-inf) = 0)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[j & 3] += ex2(fmaf(v[j], kLog2e, -ref));
+            so_far = make_float2(m, before.y * ex2(fmaf(before.x, kLog2e, -ref)) + ((s[0] + s[1]) + (s[2] + s[3])));
+            if (t < p.T) {
+              if (y >= v_first && y < v_first + 32 && y < p.V) p.target_logit[t] = turn_read(turn, lane, static_cast<int>(y) - v_first);
+            }
+          }
+        }
+      } else if (NARROW && u.kind == kLossDz) {
+        if (count32 == 0) give_back();
+        if (lane == 0) bulk_wait_read();       // (stores of a dw unit before still read both tiles)
+        __syncwarp();
+#pragma unroll 1
+        for (int c = 0; c < count32; ++c) {
+          const int t_first = u.m * p.tile_tokens + (first32 + c) * 32, t = t_first + lane;
+          float lse2 = 0.f, c_t = 0.f;
+          int target = -1;               // among this warp's rows
+          bool dead = true;
+          if (t < p.T) {
+            const long long y = p.targets[t];
+            if (y != p.ignore_index) {
+              dead = false;
+              c_t = p.row_scale != nullptr ? p.row_scale[t] : 1.f;
+              lse2 = p.lse[t] * kLog2e;
+              const long long rel = y - static_cast<long long>(u.piece) * p.piece - v_first;
+              if (rel >= 0 && rel < 32) target = static_cast<int>(rel);
+            }
+          }
+          fetch(c);
+          if (c == count32 - 1) give_back();
+          if (v_first >= (n_cols + 63) / 64 * 64 || t_first >= p.T) continue;     // (the last panel is filled up with zeros)
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) turn_write(turn, lane, i, __uint_as_float(r[i]));
+          // the stores before must have read where this piece will stand (split2: both halves, else the one before the last)
+          if (lane == 0) { if (p.split2) bulk_wait_read(); else bulk_wait_read_but_one(); }
+          __syncwarp();
+          unsigned char* const lead_tile = narrow_out + (p.split2 ? 0 : flip * 2048);
+          flip ^= 1;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t o[4], rest[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              float d[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int j = q * 8 + h * 2 + e;
+                float v = ex2(fmaf(turn_read(turn, lane, j), kLog2e, -lse2));
+                if (j == target) v -= 1.f;
+                v *= c_t;
+                if (dead || v_first + j >= n_cols) v = 0.f;
+                d[e] = v;
+              }
+              o[h] = pack_bf16x2(d[0], d[1]);
+              const float2 lead = unpack_bf16x2(o[h]);
+              rest[h] = pack_bf16x2(d[0] - lead.x, d[1] - lead.y);
+            }
+            st_shared_v4(smem_u32(lead_tile) + stage_off<64>(lane, q), o[0], o[1], o[2], o[3]);
+            if (p.split2) st_shared_v4(smem_u32(lead_tile) + 2048 + stage_off<64>(lane, q), rest[0], rest[1], rest[2], rest[3]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&maps.z_out, lead_tile, v_first % 64, t_first, panel_of(p, u.piece, 0) + v_first / 64);
+            if (p.split2) tma_store_3d(&maps.z_out, lead_tile + 2048, v_first % 64, t_first, panel_of(p, u.piece, 1) + v_first / 64);
+            bulk_commit();
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          bulk_wait_all();
+          fence_proxy_async();
+          red_release_gpu_add(p.done + u.piece, 1);
+          red_release_gpu_add(p.done + 3 * p.pieces + u.piece * (p.piece / kLossUnit) + u.n, 1);
+        }
+      } else if (NARROW && u.kind == kLossDx) {
+        if (count32 == 0 && !empty) give_back();
+        const int h = v_first + lane;
+#pragma unroll 1
+        for (int c = 0; c < count32; ++c) {
+          fetch(c);
+          if (p.split2 && !empty) {          // the products of the remainders
+            uint32_t r2[32];
+            tmem_ld_32x32(taddr + p.tile_tokens + c * 32, r2); tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(r2[i]));
+          }
+          if (c == count32 - 1 && !empty) give_back();
+          const int t_first = u.m * p.tile_tokens + (first32 + c) * 32;
+          float* out = p.dx_parts + (static_cast<size_t>(u.split) * p.T + t_first) * p.H + h;
+          if (h < p.H) {                     // 32 lanes write 128 contiguous bytes of each token
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (t_first + i < p.T) {
+                if (u.piece == 0) out[static_cast<size_t>(i) * p.H] = __uint_as_float(r[i]);
+                else red_add_f32(out + static_cast<size_t>(i) * p.H, __uint_as_float(r[i]));
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) red_release_gpu_add(p.done + p.pieces + u.piece, 1);
+      } else if (FWD) {
         float z[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) z[i] = 0.f;
@@ -500,48 +683,39 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         for (int i = 0; i < 128; ++i) s[i & 3] += ex2(fmaf(z[i], kLog2e, -ref));
         if (row < p.T) p.parts[static_cast<size_t>(u.n * 2 + side) * p.T + row] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
       } else if (u.kind == kLossDz) {
-        const CUtensorMap* out = &maps.z_out[u.last];
-        const int zbuf = (u.piece % p.buffers) * (p.split2 ? 2 : 1);
-        const int passes = p.split2 ? 2 : 1;
+        const int z_chunks = (chunks + 1) / 2 * 2;       // (the last panel is filled up with zeros)
         const bool rows = row0 < p.T;
         if (!rows) give_back();
 #pragma unroll 1
-        for (int part = 0; part < passes && rows; ++part) {
-#pragma unroll 1
-          for (int c = 0; c < chunks; ++c) {
-            fetch(c);
-            if (c == chunks - 1 && part == passes - 1) give_back();
-            const int left = n_cols - n0 - c * 32;
-            const bool target_here = __any_sync(0xffffffffu, (col >> 5) == c);
-            if ((c & 1) == 0) stg = next_tile();
+        for (int c = 0; c < z_chunks && rows; ++c) {
+          fetch(c);
+          if (c == z_chunks - 1) give_back();
+          const int left = n_cols - n0 - c * 32;
+          const bool target_here = __any_sync(0xffffffffu, (col >> 5) == c);
+          if ((c & 1) == 0) stg = next_tile();
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t o[4];
+          for (int q = 0; q < 4; ++q) {
+            uint32_t o[4];
 #pragma unroll
-              for (int h = 0; h < 4; ++h) {
-                float d[2];
+            for (int h = 0; h < 4; ++h) {
+              float d[2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int i = q * 8 + h * 2 + e;
-                  float v = ex2(fmaf(__uint_as_float(r[i]), kLog2e, -lse2));
-                  if (target_here && col == c * 32 + i) v -= 1.f;
-                  v *= c_t;
-                  if (dead || i >= left) v = 0.f;
-                  d[e] = v;
-                }
-                o[h] = pack_bf16x2(d[0], d[1]);
-                if (part == 1) {
-                  const float2 lead = unpack_bf16x2(o[h]);
-                  o[h] = pack_bf16x2(d[0] - lead.x, d[1] - lead.y);
-                }
+              for (int e = 0; e < 2; ++e) {
+                const int i = q * 8 + h * 2 + e;
+                float v = ex2(fmaf(__uint_as_float(r[i]), kLog2e, -lse2));
+                if (target_here && col == c * 32 + i) v -= 1.f;
+                v *= c_t;
+                if (dead || i >= left) v = 0.f;
+                d[e] = v;
               }
-              st_shared_v4(stg + stage_off<128>(lane, (c & 1) * 4 + q), o[0], o[1], o[2], o[3]);
+              o[h] = pack_bf16x2(d[0], d[1]);
             }
-            if ((c & 1) == 1 || c == chunks - 1) {
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) { tma_store_3d(out, stage_tile, n0 + (c & ~1) * 32, row0, zbuf + part); bulk_commit(); }
-            }
+            st_shared_v4(stg + stage_off<128>(lane, (c & 1) * 4 + q), o[0], o[1], o[2], o[3]);
+          }
+          if ((c & 1) == 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) { tma_store_3d(&maps.z_out, stage_tile, 0, row0, panel_of(p, u.piece, 0) + (n0 + c * 32) / 64); bulk_commit(); }
           }
         }
         if (chunks == 0 && rows) give_back();
@@ -553,9 +727,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           red_release_gpu_add(p.done + 3 * p.pieces + u.piece * (p.piece / kLossUnit) + u.n, 1);
         }
       } else if (u.kind == kLossDx) {
-        const int z = p.split2 ? u.split * 2 + half : u.split;
-        const int y = p.split2 ? quarter * 32 : row0;
-        const bool rows = y < p.T;
+        const bool rows = row0 < p.T;
         if (!rows && !empty) give_back();
 #pragma unroll 1
         for (int c = 0; c < chunks && rows; ++c) {
@@ -567,8 +739,8 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            if (u.piece == 0) tma_store_3d(&maps.dx, stage_tile, n0 + c * 32, y, z);
-            else tma_reduce_add_3d(&maps.dx, stage_tile, n0 + c * 32, y, z);
+            if (u.piece == 0) tma_store_3d(&maps.dx, stage_tile, n0 + c * 32, row0, u.split);
+            else tma_reduce_add_3d(&maps.dx, stage_tile, n0 + c * 32, row0, u.split);
             bulk_commit();
           }
         }
@@ -611,6 +783,13 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
       if (!FWD && !empty) { acc ^= 1; if (acc == 0) acc_phase ^= 1; }
       }
     }
+    if (FWD && NARROW) {
+      for (int m = 0; m < p.row_units; ++m)
+        for (int c = 0; c < count32; ++c) {
+          const int t = m * p.tile_tokens + (first32 + c) * 32 + lane;
+          if (t < p.T) p.parts[static_cast<size_t>(blockIdx.x * 4 + quarter) * p.T + t] = stats[(m * 4 + c) * 32];
+        }
+    }
     if (lane == 0) bulk_wait_all();
   }
 
@@ -624,19 +803,19 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
   }
 }
 
-template <bool FWD>
+template <bool FWD, bool NARROW>
 cudaError_t launch_pairs(const LossParams& p, const LossMaps& m, long long units, int sms, cudaStream_t stream) {
-  auto kernel = linear_loss_kernel<FWD>;
+  auto kernel = linear_loss_kernel<FWD, NARROW>;
   static std::atomic<bool> configured[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(FWD));
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(FWD, NARROW));
     if (e != cudaSuccess) return e;
     configured[dev].store(true, std::memory_order_release);
   }
   const long long pairs = units < sms / 2 ? units : sms / 2;
-  kernel<<<static_cast<unsigned>(pairs * 2), kThreads, smem_bytes(FWD), stream>>>(p, m);
+  kernel<<<static_cast<unsigned>(pairs * 2), kThreads, smem_bytes(FWD, NARROW), stream>>>(p, m);
   return cudaGetLastError();
 }
 
@@ -772,11 +951,22 @@ long long loss_backward_units(const LossParams& p) {
   return static_cast<long long>(p.pieces - 1) * (c.dz + c.dw) + c.dz_last + c.dw_last + static_cast<long long>(p.pieces) * c.dx;
 }
 
+void loss_narrow_ring(LossParams& p) {
+  p.stage_bytes = kOperandBytes + (p.tile_tokens / 2 * 128 + 1023) / 1024 * 1024;      // (operands stand on 1024-byte boundaries)
+  p.stages = lesser(kNarrowStages, kNarrowRing / p.stage_bytes);
+}
+static long long forward_units(const LossParams& p) { return static_cast<long long>(p.row_units) * ((p.V + kLossUnit - 1) / kLossUnit); }
+long long loss_forward_parts(const LossParams& p, int sms) {
+  if (!p.narrow) return (static_cast<long long>(p.V) + kLossPart - 1) / kLossPart;
+  const long long units = forward_units(p);
+  return (units < sms / 2 ? units : sms / 2) * 2 * 4;           // one for each warp quarter of every CTA
+}
 cudaError_t launch_loss_forward(const LossParams& p, const LossMaps& m, int sms, cudaStream_t stream) {
-  return launch_pairs<true>(p, m, static_cast<long long>(p.row_units) * ((p.V + kLossUnit - 1) / kLossUnit), sms, stream);
+  const long long units = forward_units(p);
+  return p.narrow ? launch_pairs<true, true>(p, m, units, sms, stream) : launch_pairs<true, false>(p, m, units, sms, stream);
 }
 cudaError_t launch_loss_backward(const LossParams& p, const LossMaps& m, int sms, cudaStream_t stream) {
-  return launch_pairs<false>(p, m, loss_backward_units(p), sms, stream);
+  return p.narrow ? launch_pairs<false, true>(p, m, loss_backward_units(p), sms, stream) : launch_pairs<false, false>(p, m, loss_backward_units(p), sms, stream);
 }
 // Both follow the kernel whose results they read, and may be launched while it drains.
 template <class Params>

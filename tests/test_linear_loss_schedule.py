@@ -19,7 +19,7 @@ def up(a, b):
 def test_units_and_order(T, H, V, want_dx, want_dw):
     (pieces, piece, splits, ahead, buffers, row_units, split2, group), *units = _ext.load().linear_loss_schedule(T, H, V, 148, want_dx, want_dw)
     assert piece % 256 == 0 and (pieces - 1) * piece < V <= pieces * piece
-    assert row_units == up(T, 256) and (not split2 or T <= 128) and pieces >= buffers >= min(ahead + 1, pieces)
+    assert row_units == up(T, 256) and (not split2 or T <= 64) and pieces >= buffers >= min(ahead + 1, pieces)
     cols = [min(piece, V - j * piece) for j in range(pieces)]
     want = set()
     for j in range(pieces):
