@@ -206,63 +206,65 @@ __global__ void __launch_bounds__(kListThreads, 2) list_adamw_kernel(const __gri
     if (p.skip_nonfinite && !isfinite(norm)) return;
     if (p.max_norm >= 0.f) f = clip_factor(norm, p.max_norm);
   }
-  const Run run = run_of(list.chunks, static_cast<int>(gridDim.x - 1 - blockIdx.x), gridDim.x);
-  if (run.begin >= run.end) return;
-  int e = entry_of(list, run.begin);
-  int c = run.begin;
-  while (c < run.end) {
-    while (e + 1 < list.count && list.first[e + 1] <= c) ++e;
-    const int stop = min(run.end, list.first[e + 1]);
-    const unsigned long long word = list.length[e];
-    const int flags = static_cast<int>(word >> kListTypeShift);
-    const bool half = flags & kListHalf, grad_half = flags & kListGradHalf;
-    const long long n = static_cast<long long>(word & kListLength);
-    const long long begin = static_cast<long long>(c - list.first[e]) * list.chunk;
-    const long long end = min(n, static_cast<long long>(stop - list.first[e]) * list.chunk);
-    void* param = list.param[e];
-    const void* grad = list.grad[e];
-    float* m = list.exp_avg[e];
-    float* v = list.exp_avg_sq[e];
-    float* master = list.master[e];
-    auto one = [&](long long i) {
-      const Adam a = adam(p, load_one(grad, i, grad_half) * f, m[i], v[i], master != nullptr ? master[i] : load_one(param, i, half));
-      m[i] = a.m; v[i] = a.v;
-      if (master != nullptr) master[i] = a.w;
-      store_one(param, i, half, a.w);
-    };
-    // Vectors of four start `lead` elements into the tensor, hence into every chunk (chunks are multiples of four); what lies before
-    // the first and after the last goes one by one, and all of it where the entry's tensors have no boundary in common.
-    const int lead = (flags >> kListHeadShift) & 3;
-    long long head = end, tail = end;
-    if (!(flags & kListScalar)) {
-      head = min(end, begin + lead);
-      tail = head + (end - head) / 4 * 4;
+  // from the end of the list: what the norm read last is still in L2
+  for (long long last = list.chunks - static_cast<long long>(blockIdx.x) * list.window; last > 0; last -= static_cast<long long>(gridDim.x) * list.window) {
+    const Run run = {static_cast<int>(max(last - list.window, 0ll)), static_cast<int>(last)};
+    int e = entry_of(list, run.begin);
+    int c = run.begin;
+    while (c < run.end) {
+      while (e + 1 < list.count && list.first[e + 1] <= c) ++e;
+      const int stop = min(run.end, list.first[e + 1]);
+      const unsigned long long word = list.length[e];
+      const int flags = static_cast<int>(word >> kListTypeShift);
+      const bool half = flags & kListHalf, grad_half = flags & kListGradHalf;
+      const long long n = static_cast<long long>(word & kListLength);
+      const long long begin = static_cast<long long>(c - list.first[e]) * list.chunk;
+      const long long end = min(n, static_cast<long long>(stop - list.first[e]) * list.chunk);
+      void* param = list.param[e];
+      const void* grad = list.grad[e];
+      float* m = list.exp_avg[e];
+      float* v = list.exp_avg_sq[e];
+      float* master = list.master[e];
+      auto one = [&](long long i) {
+        const Adam a = adam(p, load_one(grad, i, grad_half) * f, m[i], v[i], master != nullptr ? master[i] : load_one(param, i, half));
+        m[i] = a.m; v[i] = a.v;
+        if (master != nullptr) master[i] = a.w;
+        store_one(param, i, half, a.w);
+      };
+      // Vectors of four start `lead` elements into the tensor, hence into every chunk (chunks are multiples of four); what lies before
+      // the first and after the last goes one by one, and all of it where the entry's tensors have no boundary in common.
+      const int lead = (flags >> kListHeadShift) & 3;
+      long long head = end, tail = end;
+      if (!(flags & kListScalar)) {
+        head = min(end, begin + lead);
+        tail = head + (end - head) / 4 * 4;
+      }
+      for (long long i = begin + threadIdx.x; i < head; i += kListThreads) one(i);
+      for (long long i = tail + threadIdx.x; i < end; i += kListThreads) one(i);
+      const long long step = 4 * kListThreads;
+      long long i = head + 4 * threadIdx.x;
+      auto four = [&](long long at, float4 g, float4 a, float4 b, float4 w) {
+        const Adam r0 = adam(p, g.x * f, a.x, b.x, w.x), r1 = adam(p, g.y * f, a.y, b.y, w.y), r2 = adam(p, g.z * f, a.z, b.z, w.z), r3 = adam(p, g.w * f, a.w, b.w, w.w);
+        *reinterpret_cast<float4*>(m + at) = make_float4(r0.m, r1.m, r2.m, r3.m);
+        *reinterpret_cast<float4*>(v + at) = make_float4(r0.v, r1.v, r2.v, r3.v);
+        const float4 w4 = make_float4(r0.w, r1.w, r2.w, r3.w);
+        if (master != nullptr) *reinterpret_cast<float4*>(master + at) = w4;
+        store_four(param, at, half, w4);
+      };
+      for (; i + step < tail; i += 2 * step) {
+        const float4 g0 = load_four(grad, i, grad_half), a0 = *reinterpret_cast<const float4*>(m + i), b0 = *reinterpret_cast<const float4*>(v + i);
+        const float4 w0 = master != nullptr ? *reinterpret_cast<const float4*>(master + i) : load_four(param, i, half);
+        const long long k = i + step;
+        const float4 g1 = load_four(grad, k, grad_half), a1 = *reinterpret_cast<const float4*>(m + k), b1 = *reinterpret_cast<const float4*>(v + k);
+        const float4 w1 = master != nullptr ? *reinterpret_cast<const float4*>(master + k) : load_four(param, k, half);
+        four(i, g0, a0, b0, w0);
+        four(k, g1, a1, b1, w1);
+      }
+      for (; i < tail; i += step)
+        four(i, load_four(grad, i, grad_half), *reinterpret_cast<const float4*>(m + i), *reinterpret_cast<const float4*>(v + i),
+             master != nullptr ? *reinterpret_cast<const float4*>(master + i) : load_four(param, i, half));
+      c = stop;
     }
-    for (long long i = begin + threadIdx.x; i < head; i += kListThreads) one(i);
-    for (long long i = tail + threadIdx.x; i < end; i += kListThreads) one(i);
-    const long long step = 4 * kListThreads;
-    long long i = head + 4 * threadIdx.x;
-    auto four = [&](long long at, float4 g, float4 a, float4 b, float4 w) {
-      const Adam r0 = adam(p, g.x * f, a.x, b.x, w.x), r1 = adam(p, g.y * f, a.y, b.y, w.y), r2 = adam(p, g.z * f, a.z, b.z, w.z), r3 = adam(p, g.w * f, a.w, b.w, w.w);
-      *reinterpret_cast<float4*>(m + at) = make_float4(r0.m, r1.m, r2.m, r3.m);
-      *reinterpret_cast<float4*>(v + at) = make_float4(r0.v, r1.v, r2.v, r3.v);
-      const float4 w4 = make_float4(r0.w, r1.w, r2.w, r3.w);
-      if (master != nullptr) *reinterpret_cast<float4*>(master + at) = w4;
-      store_four(param, at, half, w4);
-    };
-    for (; i + step < tail; i += 2 * step) {
-      const float4 g0 = load_four(grad, i, grad_half), a0 = *reinterpret_cast<const float4*>(m + i), b0 = *reinterpret_cast<const float4*>(v + i);
-      const float4 w0 = master != nullptr ? *reinterpret_cast<const float4*>(master + i) : load_four(param, i, half);
-      const long long k = i + step;
-      const float4 g1 = load_four(grad, k, grad_half), a1 = *reinterpret_cast<const float4*>(m + k), b1 = *reinterpret_cast<const float4*>(v + k);
-      const float4 w1 = master != nullptr ? *reinterpret_cast<const float4*>(master + k) : load_four(param, k, half);
-      four(i, g0, a0, b0, w0);
-      four(k, g1, a1, b1, w1);
-    }
-    for (; i < tail; i += step)
-      four(i, load_four(grad, i, grad_half), *reinterpret_cast<const float4*>(m + i), *reinterpret_cast<const float4*>(v + i),
-           master != nullptr ? *reinterpret_cast<const float4*>(master + i) : load_four(param, i, half));
-    c = stop;
   }
 }
 

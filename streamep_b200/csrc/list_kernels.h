@@ -35,6 +35,7 @@ struct AdamList {
   unsigned long long length[kAdamEntries];
   int first[kAdamEntries + 1];
   int count, chunks, chunk;
+  int window;                    // chunks that a block takes at a time
 };
 
 // One double per block: the sum of squares of its chunks.

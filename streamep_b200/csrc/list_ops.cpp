@@ -248,12 +248,17 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
   const auto stream = at::cuda::getCurrentCUDAStream();
   const int most = num_sms() * kAdamBlocksPerSm;
   AdamList list;
-  list.chunk = chunk_of(elements, most);
+  // Long lists: chunks of one vector a thread, dealt out in turn, so that the blocks that run together read and write one window of each of
+  // the seven arrays and not 296: 411 M elements with masters 1948 -> 1841 us, 20 M in 400 tensors 108 -> 100 (any larger chunk or
+  // window 1926 to 1948).  Short lists: a run of chunks for every block, one search for each: 250 tensors of 5 M elements in all, 101 -> 90.
+  const bool in_turn = elements >= 8'000'000;
+  list.chunk = in_turn ? 4 * kListThreads : chunk_of(elements, most);
   list.count = 0;
   int64_t chunks = 0;
   auto flush = [&] {
     if (list.count == 0) return;
     list.first[list.count] = list.chunks = static_cast<int>(chunks);
+    list.window = in_turn ? 1 : static_cast<int>((chunks + most - 1) / most);
     SEP_CUDA_CHECK(launch_list_adamw(list, a, static_cast<int>(std::min<int64_t>(most, chunks)), stream));
     list.count = 0; chunks = 0;
   };

@@ -167,7 +167,7 @@ def oracle(p, g, m, v, w, o, f):
     return m2, b1 * m.abs() + (1 - b1) * g.abs(), v2, w * (1 - o["lr"] * o["weight_decay"]) - move, w.abs() + scale
 
 
-ADAM_SIZES = [[1], [0, 5], [4, 3, 1, 4095, 4096, 4097, 30_001], [7] * 700, [2_000_003, 11]]
+ADAM_SIZES = [[1], [0, 5], [4, 3, 1, 4095, 4096, 4097, 30_001], [7] * 700, [2_000_003, 11], [5_000_003, 2, 4_000_001, 2047]]
 
 
 @pytest.mark.parametrize("kind", ["master", "bf16", "fp32", "fp32 bf16 grads"])
