@@ -285,11 +285,14 @@ class Buffer:
     def check_status(self) -> None:
         """Synchronise the device and raise :class:`StreamEPTimeout` if any bounded
         device wait gave up since the last check (:class:`StreamEPOverflow` if a
-        capacity-mode dispatch did not fit its region).  The context stays usable."""
+        capacity-mode dispatch did not fit its region, :class:`StreamEPError` if a loss
+        got a target outside its vocabulary).  The context stays usable."""
         msg = self.runtime.poll_status(True)
         if msg:
             if "capacity overflow" in msg:
                 raise StreamEPOverflow(f"rank {self.rank}: {msg}; {self._overflow_text()}")
+            if "outside the vocabulary" in msg:
+                raise StreamEPError(f"rank {self.rank}: {msg}")
             raise StreamEPTimeout(f"rank {self.rank}: {msg}")
 
     # ------------------------------------------------------------------ capacity mode
@@ -771,6 +774,8 @@ class LocalWorld:
         if msgs:
             if all("capacity overflow" in m for m in msgs):
                 raise StreamEPOverflow("; ".join(msgs))
+            if all("outside the vocabulary" in m for m in msgs):
+                raise StreamEPError("; ".join(msgs))
             raise StreamEPTimeout("; ".join(msgs))
 
     def enable_capacity_mode(self, *args, **kwargs):

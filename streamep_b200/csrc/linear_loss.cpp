@@ -106,7 +106,7 @@ struct LossCall : torch::CustomClassHolder {
   bool counters_used = false;    // a backward has run (with retain_graph another may follow)
 };
 
-// the loss; and [T] log-denominators followed by 1 / counted tokens
+// the loss; and [2][T] softmax statistics followed by 1 / counted tokens
 struct Forward { at::Tensor loss, stats; };
 
 LossParams plan(int64_t T, int64_t H, int64_t V, bool want_dx, bool want_dw, int sms) {
@@ -126,7 +126,7 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   const auto f32 = x.options().dtype(at::kFloat);
   const bool reduced = call.reduction != kLossNone;
   Forward out;
-  out.stats = at::empty({T + 1}, f32);
+  out.stats = at::empty({2 * T + 1}, f32);
   if (T == 0) {
     out.loss = reduced ? at::full({}, call.reduction == kLossMean ? std::numeric_limits<float>::quiet_NaN() : 0.0, f32) : at::empty({0}, f32);
     return out;
@@ -171,9 +171,9 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   f.parts = p.parts; f.target_logit = p.target_logit; f.targets = p.targets; f.ignore_index = p.ignore_index;
   f.mean = call.reduction == kLossMean; f.sum = call.reduction == kLossSum;
   f.each = reduced ? reinterpret_cast<float*>(base + each_at) : out.loss.data_ptr<float>();
-  f.lse = out.stats.data_ptr<float>();
+  f.top = out.stats.data_ptr<float>();
   f.loss = reduced ? out.loss.data_ptr<float>() : nullptr;
-  f.inv_count = f.lse + T;
+  f.inv_count = f.top + 2 * T;
   f.ticket = ticket;
   f.status = ctx.status; f.rank = ctx.rank;
   SEP_CUDA_CHECK(launch_loss_final(f, ctx.stream));
@@ -203,10 +203,10 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
   char* base = static_cast<char*>(space.data_ptr());
   p.targets = reinterpret_cast<const long long*>(targets.data_ptr<int64_t>());
   p.ignore_index = call.ignore_index;
-  p.lse = stats.data_ptr<float>();
+  p.top = stats.data_ptr<float>();
   if (call.reduction == kLossNone) p.row_scale = up.data_ptr<float>();
   else p.scale = up.data_ptr<float>();
-  if (call.reduction == kLossMean) p.scale2 = p.lse + T;
+  if (call.reduction == kLossMean) p.scale2 = p.top + 2 * T;
   p.claim = call.counters.data_ptr<int>();
   p.done = p.claim + 4;
   p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;

@@ -1,5 +1,7 @@
 // Output projection with softmax cross entropy, without logits in memory: z = x W^T, and for each token t with target y
-//   loss_t = log sum_v exp(z_tv) - z_ty,   dz_tv = c_t (exp(z_tv - lse_t) - [v = y]),   dx = dz W,   dW = dz^T x.
+//   loss_t = log sum_v exp(z_tv) - z_ty,   dz_tv = c_t (exp(z_tv) / sum_v exp(z_tv) - [v = y]),   dx = dz W,   dW = dz^T x.
+// Differences with the row's maximum are formed first, (z - max) log2 e and not z log2 e - max log2 e: logits masked with the type's lowest
+// value would overflow in the second form.
 //
 // All four products run in one kernel template over units of 256 x 256 (tcgen05 on CTA pairs, fp32 accumulators in tensor memory,
 // operands by TMA).  Forward: the epilogue reduces each row's 128 columns to a maximum m and the sum of exp(z - m) and drops the
@@ -149,7 +151,7 @@ __host__ __device__ __forceinline__ Unit unit_of(const LossParams& p, int lin) {
 }
 
 // dz lies in panels of 64 columns, [panel][T][64]: what a load or a store moves is one contiguous block (with rows of a whole piece,
-// 128 bytes here and the next 200 KB away, PANELNOTE).  The first panel of a piece, of its leading halves or (split2) remainders:
+// 128 bytes here and the next 200 KB away, calls of 1 to 800 tokens took 2 to 4 % longer).  The first panel of a piece, of its leading halves or (split2) remainders:
 __device__ __forceinline__ int panel_of(const LossParams& p, int piece, int rest) {
   return ((piece % p.buffers) * (p.split2 ? 2 : 1) + rest) * (p.piece / 64);
 }
@@ -455,7 +457,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
       const int row = row0 + lane;
       const bool empty = u.k_blocks == 0;
       // fetched while the tensor cores still work on the tile
-      int col = -1; float lse2 = 0.f, c_t = 0.f;
+      int col = -1; float top = 0.f, log2_sum = 0.f, c_t = 0.f;
       bool dead = true;              // an ignored token (or no token): zeros whatever its logits are
       if (!NARROW && u.kind <= kLossDz) {
         if (row < p.T) {
@@ -465,7 +467,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           if (!FWD && y != p.ignore_index) {
             dead = false;
             c_t = p.row_scale != nullptr ? p.row_scale[row] : 1.f;
-            lse2 = p.lse[row] * kLog2e;
+            top = p.top[row]; log2_sum = p.top[p.T + row];
           }
         }
       }
@@ -530,14 +532,14 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
             __syncwarp();
             float2& so_far = stats[(u.m * 4 + c) * 32];
             const float2 before = so_far;
-            float v[32], top[4] = {before.x, ninf, ninf, ninf}, s[4] = {0.f, 0.f, 0.f, 0.f};
+            float v[32], most[4] = {before.x, ninf, ninf, ninf}, s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) { v[j] = turn_read(turn, lane, j); top[j & 3] = fmaxf(top[j & 3], v[j]); }
-            const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            const float ref = m == ninf ? 0.f : m * kLog2e;      // (a row of -inf: subtract 0, every term is exp(-inf) = 0)
+            for (int j = 0; j < 32; ++j) { v[j] = turn_read(turn, lane, j); most[j & 3] = fmaxf(most[j & 3], v[j]); }
+            const float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+            const float ref = m == ninf ? 0.f : m;         // (a row of -inf: subtract 0, every term is exp(-inf) = 0)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) s[j & 3] += ex2(fmaf(v[j], kLog2e, -ref));
-            so_far = make_float2(m, before.y * ex2(fmaf(before.x, kLog2e, -ref)) + ((s[0] + s[1]) + (s[2] + s[3])));
+            for (int j = 0; j < 32; ++j) s[j & 3] += ex2((v[j] - ref) * kLog2e);
+            so_far = make_float2(m, before.y * ex2((before.x - ref) * kLog2e) + ((s[0] + s[1]) + (s[2] + s[3])));
             if (t < p.T) {
               if (y >= v_first && y < v_first + 32 && y < p.V) p.target_logit[t] = turn_read(turn, lane, static_cast<int>(y) - v_first);
             }
@@ -550,7 +552,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
 #pragma unroll 1
         for (int c = 0; c < count32; ++c) {
           const int t_first = u.m * p.tile_tokens + (first32 + c) * 32, t = t_first + lane;
-          float lse2 = 0.f, c_t = 0.f;
+          float top = 0.f, log2_sum = 0.f, c_t = 0.f;
           int target = -1;               // among this warp's rows
           bool dead = true;
           if (t < p.T) {
@@ -558,7 +560,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
             if (y != p.ignore_index) {
               dead = false;
               c_t = p.row_scale != nullptr ? p.row_scale[t] : 1.f;
-              lse2 = p.lse[t] * kLog2e;
+              top = p.top[t]; log2_sum = p.top[p.T + t];
               const long long rel = y - static_cast<long long>(u.piece) * p.piece - v_first;
               if (rel >= 0 && rel < 32) target = static_cast<int>(rel);
             }
@@ -583,7 +585,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int j = q * 8 + h * 2 + e;
-                float v = ex2(fmaf(turn_read(turn, lane, j), kLog2e, -lse2));
+                float v = ex2(fmaf(turn_read(turn, lane, j) - top, kLog2e, -log2_sum));
                 if (j == target) v -= 1.f;
                 v *= c_t;
                 if (dead || v_first + j >= n_cols) v = 0.f;
@@ -672,15 +674,15 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           for (int i = 0; i < 128; ++i) if (col == i) zt = z[i];
           if (col >= 0) p.target_logit[row] = zt;
         }
-        float top[4] = {ninf, ninf, ninf, ninf};
+        float most[4] = {ninf, ninf, ninf, ninf};
 #pragma unroll
-        for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], z[i]);
-        const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        for (int i = 0; i < 128; ++i) most[i & 3] = fmaxf(most[i & 3], z[i]);
+        const float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
         // (a row of -inf: subtract 0, every term is exp(-inf) = 0)
-        const float ref = m == ninf ? 0.f : m * kLog2e;
+        const float ref = m == ninf ? 0.f : m;
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 128; ++i) s[i & 3] += ex2(fmaf(z[i], kLog2e, -ref));
+        for (int i = 0; i < 128; ++i) s[i & 3] += ex2((z[i] - ref) * kLog2e);
         if (row < p.T) p.parts[static_cast<size_t>(u.n * 2 + side) * p.T + row] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
       } else if (u.kind == kLossDz) {
         const int z_chunks = (chunks + 1) / 2 * 2;       // (the last panel is filled up with zeros)
@@ -702,7 +704,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int i = q * 8 + h * 2 + e;
-                float v = ex2(fmaf(__uint_as_float(r[i]), kLog2e, -lse2));
+                float v = ex2(fmaf(__uint_as_float(r[i]) - top, kLog2e, -log2_sum));
                 if (target_here && col == c * 32 + i) v -= 1.f;
                 v *= c_t;
                 if (dead || i >= left) v = 0.f;
@@ -836,8 +838,8 @@ __global__ void __launch_bounds__(kFinalThreads) loss_final_kernel(const LossFin
   const float ninf = __int_as_float(0xff800000);
   auto join = [&](float2 a, float2 b) {
     const float m = fmaxf(a.x, b.x);
-    const float ref = m == ninf ? 0.f : m * kLog2e;
-    return make_float2(m, a.y * ex2(fmaf(a.x, kLog2e, -ref)) + b.y * ex2(fmaf(b.x, kLog2e, -ref)));
+    const float ref = m == ninf ? 0.f : m;
+    return make_float2(m, a.y * ex2((a.x - ref) * kLog2e) + b.y * ex2((b.x - ref) * kLog2e));
   };
   grid_wait();
   float2 v = make_float2(ninf, 0.f);
@@ -860,18 +862,20 @@ __global__ void __launch_bounds__(kFinalThreads) loss_final_kernel(const LossFin
     for (int w = part + 4; w < kFinalLanes; w += 4) v = join(v, joined[w][r]);
     for (int d = 8; d < 32; d *= 2) v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, d), __shfl_xor_sync(0xffffffffu, v.y, d)));
     if (lane < kFinalRows && row < p.T) {
-      float lse = v.x + logf(v.y);
+      // The maximum and the logarithm of the sum stay apart: next to a maximum of the type's lowest value, or a loss near zero, their sum
+      // would have lost the logarithm.
       const long long y = p.targets[row];
       float loss = 0.f;
       if (y != p.ignore_index) {
         if (y < 0 || y >= p.V) {       // the loss and every gradient become NaN, and the caller can ask why
           report_note(p.status, kStatusBadTarget, kKernelLoss, 0, p.rank, static_cast<int>(row), p.V, static_cast<int>(y));
-          lse = loss = __int_as_float(0x7fc00000);
+          v.x = loss = __int_as_float(0x7fc00000);
         } else {
-          loss = lse - p.target_logit[row];
+          loss = (v.x - p.target_logit[row]) + logf(v.y);
         }
       }
-      p.lse[row] = lse;
+      p.top[row] = v.x;
+      p.top[p.T + row] = log2f(v.y);
       p.each[row] = loss;
     }
   }

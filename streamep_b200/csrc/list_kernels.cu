@@ -217,9 +217,11 @@ __global__ void __launch_bounds__(kListThreads, 2) list_adamw_kernel(const __gri
       const unsigned long long word = list.length[e];
       const int flags = static_cast<int>(word >> kListTypeShift);
       const bool half = flags & kListHalf, grad_half = flags & kListGradHalf;
-      const long long n = static_cast<long long>(word & kListLength);
-      const long long begin = static_cast<long long>(c - list.first[e]) * list.chunk;
-      const long long end = min(n, static_cast<long long>(stop - list.first[e]) * list.chunk);
+      // Vectors of four start `lead` elements into the tensor; these belong to its first chunk in addition, so that all others begin on a
+      // boundary (with heads and tails in every chunk a packed list of 200 M odd elements took 1533 us instead of 1096).
+      const int lead = flags >> kListHeadShift;
+      const long long begin = c == list.first[e] ? 0 : lead + static_cast<long long>(c - list.first[e]) * list.chunk;
+      const long long end = stop == list.first[e + 1] ? static_cast<long long>(word & kListLength) : lead + static_cast<long long>(stop - list.first[e]) * list.chunk;
       void* param = list.param[e];
       const void* grad = list.grad[e];
       float* m = list.exp_avg[e];
@@ -231,12 +233,10 @@ __global__ void __launch_bounds__(kListThreads, 2) list_adamw_kernel(const __gri
         if (master != nullptr) master[i] = a.w;
         store_one(param, i, half, a.w);
       };
-      // Vectors of four start `lead` elements into the tensor, hence into every chunk (chunks are multiples of four); what lies before
-      // the first and after the last goes one by one, and all of it where the entry's tensors have no boundary in common.
-      const int lead = (flags >> kListHeadShift) & 3;
+      // what lies before the first vector and after the last goes one by one, and all of it where the entry's arrays have no boundary in common
       long long head = end, tail = end;
       if (!(flags & kListScalar)) {
-        head = min(end, begin + lead);
+        head = begin == 0 ? min(end, static_cast<long long>(lead)) : begin;
         tail = head + (end - head) / 4 * 4;
       }
       for (long long i = begin + threadIdx.x; i < head; i += kListThreads) one(i);

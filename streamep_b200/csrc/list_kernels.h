@@ -16,7 +16,8 @@ enum ListFlag : int {
   kListGradHalf = 2,             // AdamW: the gradient is bf16
   kListScalar = 4,               // AdamW: the tensors of this entry cannot be brought to 16-byte boundaries together
 };
-constexpr int kListHeadShift = 4;                // AdamW: flags >> 4 = elements before the first common boundary
+constexpr int kListHeadShift = 4;                // AdamW: flags >> 4 = elements before the first common boundary, in addition to those of the
+                                                 // tensor's first chunk
 
 constexpr int kNormEntries = 1024;
 struct NormList {

@@ -248,10 +248,12 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
   const auto stream = at::cuda::getCurrentCUDAStream();
   const int most = num_sms() * kAdamBlocksPerSm;
   AdamList list;
-  // Long lists: chunks of one vector a thread, dealt out in turn, so that the blocks that run together read and write one window of each of
-  // the seven arrays and not 296: 411 M elements with masters 1948 -> 1841 us, 20 M in 400 tensors 108 -> 100 (any larger chunk or
-  // window 1926 to 1948).  Short lists: a run of chunks for every block, one search for each: 250 tensors of 5 M elements in all, 101 -> 90.
-  const bool in_turn = elements >= 8'000'000;
+  // Long lists with master copies: chunks of one vector a thread, dealt out in turn, so that the blocks that run together read and write one
+  // window of each of the seven arrays and not 296: 411 M elements 1948 -> 1841 us, 20 M in 400 tensors 108 -> 100 (any larger
+  // chunk or window 1926 to 1948).  Not without masters, where the arrays are of one width and such windows meet in the same DRAM banks (203 M
+  // elements fp32 1033 -> 1137 us, bf16 812 -> 977).  Short lists: a run of chunks for every block, one search for each: 250 tensors of 5 M
+  // elements in all, 101 -> 90.
+  const bool in_turn = have_masters && elements >= 8'000'000;
   list.chunk = in_turn ? 4 * kListThreads : chunk_of(elements, most);
   list.count = 0;
   int64_t chunks = 0;
@@ -277,11 +279,12 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
     const int off = place(list.exp_avg[at], 4);
     const bool together = place(list.param[at], is_half(p) ? 2 : 4) == off && place(list.grad[at], is_half(g) ? 2 : 4) == off &&
                           place(list.exp_avg_sq[at], 4) == off && (!have_masters || place(list.master[at], 4) == off);
+    const int lead = together ? (4 - off) % 4 : 0;
     const unsigned long long flags = (is_half(p) ? kListHalf : 0) | (is_half(g) ? kListGradHalf : 0) | (together ? 0 : kListScalar) |
-                                     (static_cast<unsigned long long>((4 - off) % 4) << kListHeadShift);
+                                     (static_cast<unsigned long long>(lead) << kListHeadShift);
     list.length[at] = static_cast<unsigned long long>(p.numel()) | (flags << kListTypeShift);
     list.first[at] = static_cast<int>(chunks);
-    chunks += (p.numel() + list.chunk - 1) / list.chunk;
+    chunks += std::max<int64_t>(1, (p.numel() - lead + list.chunk - 1) / list.chunk);
     SEP_ASSERT(chunks < (1ll << 31), "the list is too large");
   }
   flush();

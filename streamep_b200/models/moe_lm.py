@@ -1,0 +1,107 @@
+"""``MoELM`` and ``ExpertAdamW``: a training program around the MoE layer, from token ids to the updated weights.
+
+The reference ends at the layer; what its users write around it (an embedding, the loss over the vocabulary, clipping, the
+optimizer) is here in its smallest form, on the library's own operators: ``linear_cross_entropy`` for the output
+projection and the loss, ``grad_norm`` over replicated and expert weights, ``adamw_step_`` with the clipping in it.
+"""
+from __future__ import annotations
+
+from typing import List, Optional
+
+import torch
+from torch import nn
+
+from ..buffer import Buffer
+from ..ops.linear_loss import linear_cross_entropy
+from ..ops.tensor_lists import adamw_step_, grad_norm
+from .moe_layer import StreamMoE
+
+
+class MoELM(nn.Module):
+    """Embedding, ``num_layers`` residual MoE layers on RMS-normalised rows, output projection.  There is no token mixer:
+    it models the next token from the present one, which is what a training step needs to be exercised."""
+
+    def __init__(self, vocab: int, hidden: int, ffn: int, num_experts: int, top_k: int, num_layers: int, buffer: Buffer, *,
+                 device=None, seed: int = 0):
+        super().__init__()
+        g = torch.Generator(device="cpu").manual_seed(seed)
+        self.embedding = nn.Parameter(torch.randn(vocab, hidden, generator=g).to(torch.bfloat16).to(device))
+        self.head = nn.Parameter((torch.randn(vocab, hidden, generator=g) * 0.02).to(torch.bfloat16).to(device))
+        self.layers = nn.ModuleList(StreamMoE(hidden, ffn, num_experts, top_k, buffer, device=device, seed=seed + i)
+                                    for i in range(num_layers))
+        self.buffer = buffer
+
+    def hidden_states(self, tokens: torch.Tensor) -> torch.Tensor:
+        x = torch.nn.functional.embedding(tokens.reshape(-1), self.embedding)
+        for layer in self.layers:
+            x = x + layer(torch.nn.functional.rms_norm(x, x.shape[-1:]))
+        return torch.nn.functional.rms_norm(x, x.shape[-1:])
+
+    def forward(self, tokens: torch.Tensor, targets: torch.Tensor, reduction: str = "mean") -> torch.Tensor:
+        return linear_cross_entropy(self.hidden_states(tokens), self.head, targets.reshape(-1), reduction=reduction, buffer=self.buffer)
+
+    @torch.no_grad()
+    def log_probs(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        """log P(target) of every token, shaped like ``tokens``."""
+        return -self.forward(tokens, targets, reduction="none").view(tokens.shape)
+
+    def replicated_parameters(self) -> List[nn.Parameter]:
+        return [self.embedding, self.head]
+
+    def expert_parameters(self) -> List[nn.Parameter]:
+        return [p for layer in self.layers for p in (layer.w1, layer.w2)]
+
+
+class ExpertAdamW:
+    """AdamW with float32 master copies for a model whose expert weights are sharded over ``group`` and whose other
+    weights are replicated.  ``step()`` averages the replicated gradients over the group, takes the norm over everything
+    (each expert counted once), clips and updates: one pass over the gradients for the norm, one over all state."""
+
+    def __init__(self, replicated, experts, *, lr: float, betas=(0.9, 0.95), eps: float = 1e-8, weight_decay: float = 0.1,
+                 max_norm: Optional[float] = 1.0, skip_nonfinite: bool = True, group=None):
+        self.replicated, self.experts, self.group = list(replicated), list(experts), group
+        self.params = self.replicated + self.experts
+        self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
+        self.max_norm, self.skip_nonfinite = max_norm, skip_nonfinite
+        self.masters = [p.detach().float() for p in self.params]
+        self.exp_avgs = [torch.zeros_like(m) for m in self.masters]
+        self.exp_avg_sqs = [torch.zeros_like(m) for m in self.masters]
+        self.steps = 0
+
+    def zero_grad(self) -> None:
+        for p in self.params:
+            p.grad = None
+
+    @torch.no_grad()
+    def step(self) -> torch.Tensor:
+        """Returns the norm (0-dim, on the device).  Parameters without a gradient are left out."""
+        ranks = self.group.size() if self.group is not None else 1
+        if ranks > 1:
+            # a mean over the ranks' tokens: experts already hold the sum of what all ranks sent them
+            for p in self.replicated:
+                if p.grad is not None:
+                    torch.distributed.all_reduce(p.grad, group=self.group)
+            for p in self.params:
+                if p.grad is not None:
+                    p.grad.div_(ranks)
+        live = [i for i, p in enumerate(self.params) if p.grad is not None]
+        grads = [self.params[i].grad for i in live]
+        sharded = [self.params[i].grad for i in live if i >= len(self.replicated)] if ranks > 1 else []
+        norm = grad_norm(grads[:len(grads) - len(sharded)], sharded=sharded, group=self.group)
+        self.steps += 1
+        adamw_step_([self.params[i] for i in live], grads, [self.exp_avgs[i] for i in live], [self.exp_avg_sqs[i] for i in live],
+                    masters=[self.masters[i] for i in live], step=self.steps, lr=self.lr, betas=self.betas, eps=self.eps,
+                    weight_decay=self.weight_decay, norm=norm, max_norm=self.max_norm, skip_nonfinite=self.skip_nonfinite)
+        return norm
+
+    def state_dict(self) -> dict:
+        return {"steps": self.steps, "masters": self.masters, "exp_avgs": self.exp_avgs, "exp_avg_sqs": self.exp_avg_sqs}
+
+    @torch.no_grad()
+    def load_state_dict(self, state: dict) -> None:
+        self.steps = int(state["steps"])
+        for name in ("masters", "exp_avgs", "exp_avg_sqs"):
+            for mine, theirs in zip(getattr(self, name), state[name], strict=True):
+                mine.copy_(theirs)
+        for p, m in zip(self.params, self.masters):
+            p.copy_(m)

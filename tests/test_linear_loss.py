@@ -81,3 +81,255 @@ def test_other_reductions(native, T, H, V, reduction):
     torch.testing.assert_close(loss.double(), want[0], rtol=2e-6, atol=2e-5 * (T if reduction == "sum" else 1))
     near(gx, want[1])
     near(gw, want[2])
+
+
+# ------------------------------------------------------------------------------------------------------------------- edges
+def test_gradient_against_differences(native):
+    """(loss(a) - loss(b)) against the gradient half way, along random directions.  Steps of 2 % of each value: the third-order term is
+    below 1 % of the difference, the losses' own errors (2e-6 of about 6) below 1 % of differences of at least 1e-2."""
+    for T, H, V in ((40, 128, 300), (300, 64, 500)):
+        x, w, y = make(T, H, V, seed=T)
+        g = torch.Generator(device=DEV).manual_seed(3)
+        for k in range(4):
+            dx, dw = torch.randn(x.shape, generator=g, device=DEV) * x.abs() * 0.02, torch.randn(w.shape, generator=g, device=DEV) * w.abs() * 0.02
+            if k % 2 == 0:        # along the gradient, where the difference is largest
+                _, gx, gw = run(x, w, y, reduction="sum")
+                dx, dw = gx.float().sign() * dx.abs(), gw.float().sign() * dw.abs()
+            xa, xb, wa, wb = (x + dx).to(x.dtype), (x - dx).to(x.dtype), (w + dw).to(w.dtype), (w - dw).to(w.dtype)
+            mid_x, mid_w = ((xa.float() + xb.float()) / 2).to(x.dtype), ((wa.float() + wb.float()) / 2).to(w.dtype)
+            _, gx, gw = run(mid_x, mid_w, y, reduction="sum")
+            with torch.no_grad():
+                diff = float(linear_cross_entropy(xa, wa, y, reduction="sum").double() - linear_cross_entropy(xb, wb, y, reduction="sum").double())
+            want = float((gx.double() * (xa.double() - xb.double())).sum() + (gw.double() * (wa.double() - wb.double())).sum())
+            size = float((gx.double() * (xa.double() - xb.double())).norm() + (gw.double() * (wa.double() - wb.double())).norm())
+            assert abs(diff - want) <= 0.02 * abs(want) + 0.05 * size + 1e-2, (T, k, diff, want, size)
+
+
+@pytest.mark.parametrize("T", [20, 300])
+def test_a_repeated_call_gives_the_same_bits(native, T):
+    x, w, y = make(T, 512, 9000)
+    a, b = run(x, w, y), run(x, w, y)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    with torch.no_grad():
+        assert torch.equal(linear_cross_entropy(x, w, y), a[0])
+
+
+@pytest.mark.parametrize("T", [48, 500])
+def test_one_gradient_only_and_twice(native, T):
+    x, w, y = make(T, 256, 3000)
+    _, gx, gw = run(x, w, y)
+    for which in (0, 1):
+        ts = [x.detach().requires_grad_(which == 0), w.detach().requires_grad_(which == 1)]
+        loss = linear_cross_entropy(ts[0], ts[1], y)
+        first, = torch.autograd.grad(loss, ts[which], retain_graph=True)
+        second, = torch.autograd.grad(loss, ts[which])
+        assert torch.equal(first, second)
+        near(first, (gx, gw)[which].double(), 1e-5 if which else 1e-2)     # (dx may be split otherwise)
+    xs, ws = x.detach().requires_grad_(True), w.detach().requires_grad_(True)      # both wanted by the graph, one by the caller
+    only, = torch.autograd.grad(linear_cross_entropy(xs, ws, y), ws)
+    assert torch.equal(only, gw)
+
+
+def test_strides_leading_dimensions_and_alignment(native):
+    T, H, V = 6 * 17, 136, 700
+    x, w, y = make(T, H, V)
+    want = run(x, w, y, reduction="none", upstream=torch.ones(T, device=DEV))
+    wide = torch.zeros(T, 3 * H, dtype=torch.bfloat16, device=DEV)
+    wide[:, H:2 * H] = x
+    odd = torch.zeros(T * H + 1, dtype=torch.bfloat16, device=DEV)[1:].view(T, H).copy_(x)
+    turned = w.t().contiguous().t()
+    padded = torch.zeros(V, H + 8, dtype=torch.bfloat16, device=DEV)
+    padded[:, :H] = w
+    y2 = torch.stack([y, y], 1)[:, 0]
+    for xx in (wide[:, H:2 * H], odd, x.view(6, 17, H)):
+        for ww in (w, turned, padded[:, :H]):
+            yy = y2.reshape(6, 17) if xx.dim() == 3 else y2
+            loss, gx, gw = run(xx, ww, yy, reduction="none", upstream=torch.ones(yy.shape, device=DEV))
+            assert loss.shape == yy.shape and gx.shape == xx.shape and gw.shape == ww.shape
+            for got, b in zip((loss.reshape(-1), gx.reshape(T, H), gw), want):
+                assert torch.equal(got, b)
+    xe = x.detach().requires_grad_(True)
+    linear_cross_entropy(xe, w, y, reduction="none").sum().backward()               # an expanded gradient comes back
+    assert torch.equal(xe.grad, run(x, w.detach(), y, reduction="sum", upstream=torch.tensor(1.0, device=DEV))[1])
+
+
+def test_nothing_and_nothing_counted(native):
+    x, w, y = make(5, 64, 100)
+    for reduction in ("mean", "sum", "none"):
+        xe, we = x[:0].detach().requires_grad_(True), w.detach().requires_grad_(True)
+        loss = linear_cross_entropy(xe, we, y[:0], reduction=reduction)
+        gx, gw = torch.autograd.grad(loss, (xe, we), torch.ones_like(loss))
+        assert loss.shape == (torch.Size([0]) if reduction == "none" else torch.Size([])) and gx.shape == (0, 64) and not gw.any()
+        if reduction != "none":
+            assert torch.isnan(loss) if reduction == "mean" else float(loss.detach()) == 0.0
+    for T in (5, 300):
+        x, w, y = make(T, 64, 100)
+        xe, we = x.requires_grad_(True), w.requires_grad_(True)
+        loss = linear_cross_entropy(xe, we, torch.full_like(y, -100))
+        gx, gw = torch.autograd.grad(loss, (xe, we))
+        assert torch.isnan(loss) and not gx.any() and not gw.any()
+
+
+@pytest.mark.parametrize("T", [30, 400, 700])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_non_finite_rows_of_ignored_tokens(native, T, bad):
+    """An ignored token's hidden state may hold anything: the losses and the other tokens' gradients do not see it."""
+    x, w, y = make(T, 128, 1000)
+    clean = run(x, w.detach(), torch.where(torch.arange(T, device=DEV) % 7 == 3, -100, y))
+    dirty = x.detach().clone()
+    dirty[3::7] = bad
+    y[3::7] = -100
+    xe = dirty.requires_grad_(True)
+    loss = linear_cross_entropy(xe, w.detach(), y)
+    gx, = torch.autograd.grad(loss, xe)
+    assert torch.equal(loss, clean[0]) and torch.equal(gx, clean[1]) and not gx[3::7].any()
+
+
+@pytest.mark.parametrize("T", [30, 400, 700])
+def test_columns_that_are_out_of_reach(native, T):
+    """Logits of -inf and of the type's lowest values among the others (masked vocabulary): probability zero, no NaN."""
+    x, w, y = make(T, 64, 1000)
+    x = x.clone()
+    x[:, 0] = 1.0
+    w = w.clone()
+    w[500:700] = 0
+    w[500:600, 0] = -float("inf")
+    w[600:700, 0] = torch.finfo(torch.bfloat16).min
+    y = torch.where((y >= 500) & (y < 700), 0, y)
+    with torch.no_grad():
+        loss = linear_cross_entropy(x, w, y, reduction="none")
+    keep = torch.cat([w[:500], w[700:]])
+    z = x.double() @ keep.double().t()
+    want = torch.logsumexp(z, 1) - (x.double() * w[y].double()).sum(1)
+    torch.testing.assert_close(loss.double(), want, rtol=2e-6, atol=2e-5)
+    w[500:600, 0] = torch.finfo(torch.bfloat16).min
+    xe, we = x.requires_grad_(True), w.requires_grad_(True)
+    gx, gw = torch.autograd.grad(linear_cross_entropy(xe, we, y), (xe, we))
+    assert torch.isfinite(gx).all() and torch.isfinite(gw).all() and not gw[500:700].any()
+
+
+@pytest.mark.parametrize("T", [30, 400, 700])
+def test_rows_at_the_lowest_value(native, T):
+    """Every logit at the type's lowest value: all columns alike, loss ln(V), a gradient of p = 1 / V."""
+    V = 1000
+    x, w = torch.zeros(T, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(V, 64, dtype=torch.bfloat16, device=DEV)
+    x[:, 0] = 1.0
+    w[:, 0] = torch.finfo(torch.bfloat16).min
+    x[:, 1] = 0.5
+    y = torch.randint(0, V, (T,), device=DEV)
+    loss, gx, gw = run(x, w, y, reduction="none", upstream=torch.ones(T, device=DEV))
+    torch.testing.assert_close(loss.double(), torch.full((T,), float(V), dtype=torch.float64, device=DEV).log(), rtol=1e-6, atol=0)
+    want = torch.full((V, T), 1.0 / V, dtype=torch.float64, device=DEV)
+    want[y, torch.arange(T, device=DEV)] -= 1.0
+    near(gw, want @ x.double())
+
+
+@pytest.mark.parametrize("T", [30, 400, 700])
+def test_target_outside_the_vocabulary(native, T):
+    from streamep_b200 import LocalWorld
+    buf = LocalWorld(1, arena_bytes=64 << 20).buffers[0]
+    x, w, y = make(T, 64, 1000)
+    for bad in (1000, -1, 1 << 40):
+        y2 = y.clone()
+        y2[T // 2] = bad
+        xe, we = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        loss = linear_cross_entropy(xe, we, y2, buffer=buf)
+        gx, gw = torch.autograd.grad(loss, (xe, we))
+        assert torch.isnan(loss) and torch.isnan(gx[T // 2]).all() and torch.isfinite(gx[:T // 2]).all()
+        with pytest.raises(StreamEPError, match="outside the vocabulary"):
+            buf.check_status()
+    assert torch.isfinite(linear_cross_entropy(x, w, y, buffer=buf))
+    buf.check_status()
+
+
+def test_streams_and_capture(native):
+    x, w, y = make(200, 256, 5000)
+    want = run(x, w, y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        xe, we = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        loss = linear_cross_entropy(xe, we, y)
+    got = torch.autograd.grad(loss, (xe, we))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[1]) and torch.equal(got[1], want[2])
+    xs, ws = x.detach().clone().requires_grad_(True), w.detach().clone().requires_grad_(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = linear_cross_entropy(xs, ws, y)
+        grads = torch.autograd.grad(loss, (xs, ws))
+    for scale in (1.0, 0.5, 1.0):
+        with torch.no_grad():
+            xs.copy_(x * scale)
+        graph.replay()
+        torch.cuda.synchronize()
+    assert torch.equal(loss, want[0]) and torch.equal(grads[0], want[1]) and torch.equal(grads[1], want[2])
+
+
+def test_two_streams_at_once(native):
+    """Both calls want every SM: neither may wait for the other's blocks."""
+    xs = [make(1500, 512, 20000, seed=s) for s in (1, 2)]
+    want = [run(*a) for a in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    out = []
+    for _ in range(3):
+        out = []
+        for s, (x, w, y) in zip(streams, xs):
+            with torch.cuda.stream(s):
+                xe, we = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+                loss = linear_cross_entropy(xe, we, y)
+                out.append((loss,) + torch.autograd.grad(loss, (xe, we)))
+    torch.cuda.synchronize()
+    assert gg.default_runtime().poll_status(True) == ""
+    for got, b in zip(out, want):
+        assert all(torch.equal(p, q) for p, q in zip(got, b))
+
+
+def test_offsets_beyond_32_bits(native):
+    """A projection of 2.3 G elements, and hidden states of 2.4 G."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    for T, H, V in ((2, 16384, 140_000), (300_000, 8192, 300)):
+        x = torch.empty(T, H, dtype=torch.bfloat16, device=DEV).normal_(0, 0.1, generator=g).requires_grad_(True)
+        w = torch.empty(V, H, dtype=torch.bfloat16, device=DEV).normal_(0, 0.02, generator=g).requires_grad_(True)
+        y = torch.randint(0, V, (T,), generator=g, device=DEV)
+        y[-1] = V - 1
+        loss = linear_cross_entropy(x, w, y, reduction="none")
+        gx, gw = torch.autograd.grad(loss, (x, w), torch.ones_like(loss))
+        rows = torch.tensor([0, T - 1], device=DEV)
+        with torch.no_grad():
+            z = torch.cat([x[rows].double() @ w[a:a + 5000].double().t() for a in range(0, V, 5000)], 1)
+            lse = torch.logsumexp(z, 1, keepdim=True)
+            torch.testing.assert_close(loss[rows].double(), (lse - z.gather(1, y[rows, None])).squeeze(1), rtol=2e-6, atol=2e-5)
+            dz = (z - lse).exp()
+            dz[torch.arange(2, device=DEV), y[rows]] -= 1.0
+            near(gx[rows], sum(dz[:, a:a + 5000] @ w[a:a + 5000].double() for a in range(0, V, 5000)))
+            if T == 2:
+                near(gw[-1000:], dz[:, -1000:].t() @ x.double())
+        del x, w, loss, gx, gw, z
+        torch.cuda.empty_cache()
+
+
+def test_refusals(native):
+    x, w, y = make(8, 64, 100)
+    for args, kw in (((x.float(), w, y), {}), ((x, w.float(), y), {}), ((x, w, y.int()), {}), ((x[:, :60], w[:, :60], y), {}), ((x, w[:, :56], y), {}),
+                     ((x, w, y[:-1]), {}), ((x, w[:0], y), {}), ((x.cpu(), w, y), {}), ((x, w.cpu(), y), {}), ((x, w, y.cpu()), {}),
+                     ((x, w, y), dict(reduction="max")), ((x, w[0], y), {}), ((x, w, y.view(2, 4)), {})):
+        with pytest.raises(ValueError):
+            linear_cross_entropy(*args, **kw)
+    xe = x.detach().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second derivative"):      # (the autograd engine turns every exception into this type)
+        torch.autograd.grad(linear_cross_entropy(xe, w, y), xe, create_graph=True)
+    xe = x.detach().requires_grad_(True)
+    loss = linear_cross_entropy(xe, w, y)
+    w.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(loss, xe)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        linear_cross_entropy(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), w, y)
+    from streamep_b200 import LocalWorld
+    buf = LocalWorld(1, arena_bytes=64 << 20).buffers[0]
+    buf.runtime.destroy()
+    with pytest.raises(ValueError, match="destroyed"):
+        linear_cross_entropy(x, w, y, buffer=buf)
