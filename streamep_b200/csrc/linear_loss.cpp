@@ -19,6 +19,7 @@ int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // One dz buffer holds at most about this much.  Larger pieces mean fewer passes over the fp32 sums of dx.
 constexpr int64_t kPieceBytes = 128ll << 20;
 constexpr int64_t kSplitTokens = 64;             // calls whose dz is kept as a sum of two bf16 numbers: one k-block of tokens
+constexpr int64_t kDirectBlocks = 32;            // k-blocks of dx that are not worth splitting
 constexpr int64_t kNarrowTokens = 1024;
 constexpr int64_t kBandBytes = 48ll << 20;       // rows of x that a band of units shares in L2
 
@@ -63,6 +64,10 @@ void plan_backward(LossParams& p, int sms) {
   p.splits = static_cast<int>(best);
   p.split_blocks = static_cast<int>(ceil_of(piece_blocks, p.splits));
   p.splits = static_cast<int>(ceil_of(piece_blocks, p.split_blocks));
+  // Small vocabularies are not split: such calls are bound by the host, to whom the kernel that joins the splits costs a launch (64 tokens,
+  // hidden 256, V 1000: 87 -> 81 us a training pass).
+  if (v_blocks <= kDirectBlocks) { p.splits = 1; p.split_blocks = static_cast<int>(piece_blocks); }
+  p.dx_direct = p.splits == 1 && p.pieces == 1;
   // dw units of few k-blocks take several column tiles, as long as there are a few units for every pair: claiming one and asking
   // whether its dz is there takes longer than its products.
   const int64_t per_pair = tiles * p.h_units / pairs;
@@ -102,11 +107,11 @@ struct LossCall : torch::CustomClassHolder {
   int64_t ignore_index;
   int reduction;
   bool want_dx = false, want_dw = false;
-  at::Tensor counters;           // of the backward's kernel, cleared by the forward's
   bool counters_used = false;    // a backward has run (with retain_graph another may follow)
 };
 
-// the loss; and [2][T] softmax statistics followed by 1 / counted tokens
+// The loss; and what the backward needs: [2][T] softmax statistics, 1 / counted tokens, and from `counters_at` on the counters of its kernel,
+// which the forward's kernel clears.
 struct Forward { at::Tensor loss, stats; };
 
 LossParams plan(int64_t T, int64_t H, int64_t V, bool want_dx, bool want_dw, int sms) {
@@ -119,6 +124,7 @@ LossParams plan(int64_t T, int64_t H, int64_t V, bool want_dx, bool want_dw, int
   p.claim_lead = claim_lead(p, true);
   return p;
 }
+int64_t counters_at(int64_t T) { return ceil_of(2 * T + 1, 64) * 64; }
 int64_t counter_ints(const LossParams& p) { return 4 + (3 + p.piece / kLossUnit) * static_cast<int64_t>(p.pieces); }
 
 Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets) {
@@ -126,8 +132,8 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   const auto f32 = x.options().dtype(at::kFloat);
   const bool reduced = call.reduction != kLossNone;
   Forward out;
-  out.stats = at::empty({2 * T + 1}, f32);
   if (T == 0) {
+    out.stats = at::empty({1}, f32);
     out.loss = reduced ? at::full({}, call.reduction == kLossMean ? std::numeric_limits<float>::quiet_NaN() : 0.0, f32) : at::empty({0}, f32);
     return out;
   }
@@ -150,11 +156,14 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   int* ticket = reinterpret_cast<int*>(base + counters) + 1;
   p.zero = ticket; p.zero_ints = 1;
   if (call.want_dx || call.want_dw) {
-    // the ticket stands in front of the backward's counters, to be cleared with them
+    // the ticket stands behind the backward's counters, to be cleared with them
     const int64_t ints = counter_ints(plan(T, H, V, call.want_dx, call.want_dw, ctx.sms));
-    call.counters = at::empty({ints + 1}, x.options().dtype(at::kInt));
-    ticket = call.counters.data_ptr<int>() + ints;
-    p.zero = call.counters.data_ptr<int>(); p.zero_ints = static_cast<int>(ints + 1);
+    out.stats = at::empty({counters_at(T) + ints + 1}, f32);
+    p.zero = reinterpret_cast<int*>(out.stats.data_ptr<float>() + counters_at(T));
+    p.zero_ints = static_cast<int>(ints + 1);
+    ticket = p.zero + ints;
+  } else {
+    out.stats = at::empty({2 * T + 1}, f32);
   }
   p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
   LossMaps m{};
@@ -191,14 +200,14 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
   }
   if (want_dx) dx = at::empty({T, H}, x.options());
   if (want_dw) dw = at::empty({V, H}, w.options());
-  const LaunchContext ctx = call.context(want_dx ? 2 : 1);
+  const LaunchContext ctx = call.context(1);
   const at::Tensor up = upstream.to(at::kFloat).contiguous();
 
   LossParams p = plan(T, H, V, want_dx, want_dw, ctx.sms);
   SEP_ASSERT(loss_backward_units(p) < (1ll << 30), "this loss has too many tiles for one call: split the tokens");
   const int64_t z_layers = p.split2 ? 2 : 1, slots = p.splits;
   Carver c;
-  const int64_t z_at = c.take(p.buffers * z_layers * T * p.piece * 2), dx_at = want_dx ? c.take(slots * T * H * 4) : 0;
+  const int64_t z_at = c.take(p.buffers * z_layers * T * p.piece * 2), dx_at = want_dx && !p.dx_direct ? c.take(slots * T * H * 4) : 0;
   const at::Tensor space = at::empty({c.bytes}, x.options().dtype(at::kByte));
   char* base = static_cast<char*>(space.data_ptr());
   p.targets = reinterpret_cast<const long long*>(targets.data_ptr<int64_t>());
@@ -207,7 +216,7 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
   if (call.reduction == kLossNone) p.row_scale = up.data_ptr<float>();
   else p.scale = up.data_ptr<float>();
   if (call.reduction == kLossMean) p.scale2 = p.top + 2 * T;
-  p.claim = call.counters.data_ptr<int>();
+  p.claim = reinterpret_cast<int*>(stats.data_ptr<float>() + counters_at(T));
   p.done = p.claim + 4;
   p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
 
@@ -223,17 +232,19 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
   m.z_out = p.narrow ? z_map(32, 32, CU_TENSOR_MAP_SWIZZLE_64B) : z_map(64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
   if (want_dw) m.dw = make_tmap(dw.data_ptr(), H, V, 1, H, H * V, 64, 32);
   p.dx_parts = reinterpret_cast<float*>(base + dx_at);
-  if (want_dx && !p.narrow) m.dx = make_tmap(base + dx_at, H, T, slots, H, T * H, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
+  p.dx = want_dx ? dx.data_ptr() : nullptr;
+  if (want_dx && p.dx_direct) m.dx = make_tmap(dx.data_ptr(), H, T, 1, H, T * H, 64, 32);
+  else if (want_dx && !p.narrow) m.dx = make_tmap(base + dx_at, H, T, slots, H, T * H, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
   if (call.counters_used) SEP_CUDA_CHECK(cudaMemsetAsync(p.claim, 0, counter_ints(p) * sizeof(int), ctx.stream));
   call.counters_used = true;
   SEP_CUDA_CHECK(launch_loss_backward(p, m, ctx.sms, ctx.stream));
-  if (want_dx) {
+  if (want_dx && !p.dx_direct) {
     LossDxParams d{};
     d.T = p.T; d.H = p.H; d.slots = static_cast<int>(slots);
     d.parts = reinterpret_cast<const float*>(base + dx_at);
     d.scale = p.scale; d.scale2 = p.scale2;
     d.dx = dx.data_ptr();
-    SEP_CUDA_CHECK(launch_loss_dx(d, ctx.stream));
+    SEP_CUDA_CHECK(launch_loss_dx(d, call.context(1).stream));
   }
   return {dx, dw};
 }

@@ -37,7 +37,9 @@ struct LossParams {
   int ahead;                     // pieces whose dz is computed before the first product is taken from one
   int buffers;                   // dz buffers in rotation, > ahead
   int split2;                    // 1: dz is kept as the sum of two bf16 numbers (short calls, narrow)
-  float* dx_parts;               // narrow: [splits][T][H]
+  int dx_direct;                 // 1: a dx unit is all there is of its place (one split, one piece) and stores bf16: no partial sums
+  float* dx_parts;               // narrow: [splits][T][H] ...
+  void* dx;                      // ... or [T, H] bf16
   int want_dx, want_dw;
   int splits;                    // reductions over a piece of the vocabulary into which a dx unit is split
   int split_blocks;              // k-blocks of each but the last

@@ -628,18 +628,19 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           if (c == count32 - 1 && !empty) give_back();
           const int t_first = u.m * p.tile_tokens + (first32 + c) * 32;
           float* out = p.dx_parts + (static_cast<size_t>(u.split) * p.T + t_first) * p.H + h;
-          if (h < p.H) {                     // 32 lanes write 128 contiguous bytes of each token
+          if (h < p.H) {                     // 32 lanes write 128 contiguous bytes of each token (64 of the finished bf16)
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               if (t_first + i < p.T) {
-                if (u.piece == 0) out[static_cast<size_t>(i) * p.H] = __uint_as_float(r[i]);
+                if (p.dx_direct) static_cast<__nv_bfloat16*>(p.dx)[static_cast<size_t>(t_first + i) * p.H + h] = __float2bfloat16_rn(scale * __uint_as_float(r[i]));
+                else if (u.piece == 0) out[static_cast<size_t>(i) * p.H] = __uint_as_float(r[i]);
                 else red_add_f32(out + static_cast<size_t>(i) * p.H, __uint_as_float(r[i]));
               }
             }
           }
         }
         __syncwarp();
-        if (lane == 0) red_release_gpu_add(p.done + p.pieces + u.piece, 1);
+        if (lane == 0 && p.pieces > 1) red_release_gpu_add(p.done + p.pieces + u.piece, 1);
       } else if (FWD) {
         float z[128];
 #pragma unroll
@@ -728,7 +729,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           red_release_gpu_add(p.done + u.piece, 1);
           red_release_gpu_add(p.done + 3 * p.pieces + u.piece * (p.piece / kLossUnit) + u.n, 1);
         }
-      } else if (u.kind == kLossDx) {
+      } else if (u.kind == kLossDx && !p.dx_direct) {
         const bool rows = row0 < p.T;
         if (!rows && !empty) give_back();
 #pragma unroll 1
@@ -748,9 +749,12 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         }
         if (chunks == 0 && rows && !empty) give_back();
         __syncwarp();
-        if (lane == 0) { bulk_wait_all(); red_release_gpu_add(p.done + p.pieces + u.piece, 1); }
+        if (lane == 0 && p.pieces > 1) { bulk_wait_all(); red_release_gpu_add(p.done + p.pieces + u.piece, 1); }
       } else {
-        const int v = u.piece * p.piece + row0;
+        // finished rows of dW, or (the only unit of its place, a single piece) of dx
+        const bool is_dw = u.kind == kLossDw;
+        const int y = is_dw ? u.piece * p.piece + row0 : row0, y_end = is_dw ? p.V : p.T;
+        const bool report = is_dw && p.pieces > 1 && tile == u.tiles - 1;      // the operands have been read
 #pragma unroll 1
         for (int c = 0; c < chunks; c += 2) {
           uint32_t r2[32];             // two chunks on their way at once (columns past the last were not multiplied and are not stored)
@@ -759,9 +763,9 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           tmem_ld_wait();
           if (c + 2 >= chunks) {
             give_back();
-            if (lane == 0 && tile == u.tiles - 1) red_release_gpu_add(p.done + 2 * p.pieces + u.piece, 1);   // the operands have been read
+            if (lane == 0 && report) red_release_gpu_add(p.done + 2 * p.pieces + u.piece, 1);
           }
-          if (v >= p.V) continue;
+          if (y >= y_end) continue;
           stg = next_tile();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
@@ -775,11 +779,11 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) { tma_store_3d(&maps.dw, stage_tile, n0 + c * 32, v, 0); bulk_commit(); }
+          if (lane == 0) { tma_store_3d(is_dw ? &maps.dw : &maps.dx, stage_tile, n0 + c * 32, y, 0); bulk_commit(); }
         }
         if (chunks == 0) {
           give_back();
-          if (lane == 0 && tile == u.tiles - 1) red_release_gpu_add(p.done + 2 * p.pieces + u.piece, 1);
+          if (lane == 0 && report) red_release_gpu_add(p.done + 2 * p.pieces + u.piece, 1);
         }
       }
       if (!FWD && !empty) { acc ^= 1; if (acc == 0) acc_phase ^= 1; }

@@ -12,5 +12,8 @@ def __getattr__(name):
     for module in _MODULES:
         mod = importlib.import_module(f"{__name__}.{module}")
         if hasattr(mod, name):
-            return getattr(mod, name)
+            value = getattr(mod, name)
+            if not name.startswith("_") and callable(value):
+                globals()[name] = value        # found once: an import inside a function does not search again
+            return value
     raise AttributeError(name)
