@@ -40,6 +40,13 @@ KERNELS = {  # kernel function -> logical name
     "router_kernel": "router (SIMT path)",
     "device_barrier_kernel": "barrier / tail handshake",
     "tile_producer_kernel": "tile producer (test stand-in for a dispatch)",
+    "linear_loss_kernel": "output projection and cross entropy (forward, or all of the backward)",
+    "loss_final_kernel": "output projection and cross entropy (joins statistics and losses)",
+    "loss_dx_kernel": "output projection and cross entropy (joins dx)",
+    "list_squares_kernel": "gradients' norm",
+    "list_norm_kernel": "gradients' norm",
+    "list_scale_kernel": "gradients' clipping",
+    "list_adamw_kernel": "AdamW",
 }
 GEMMS = {  # (A is MN-major, B is MN-major, epilogue, fused push) of grouped_gemm_kernel -> logical name
     (0, 0, 1, 1): "dispatch (+) GEMM-A SwiGLU (fused)",
