@@ -25,14 +25,25 @@ bool usable(const at::Tensor& t, const at::Device& device) {
 
 // What is written in place must not lie in two entries: its owner would be undefined.
 struct Ranges {
-  std::vector<std::pair<uintptr_t, uintptr_t>> all;
-  void add(const at::Tensor& t) {
+  using List = std::vector<std::pair<uintptr_t, uintptr_t>>;
+  List all;                      // sorted so far
+  static bool less(const List::value_type& a, const List::value_type& b) { return a.first < b.first; }
+  static List::value_type of(const at::Tensor& t) {
     const auto p = reinterpret_cast<uintptr_t>(t.data_ptr());
-    all.emplace_back(p, p + t.numel() * t.element_size());
+    return {p, p + t.numel() * t.element_size()};
   }
-  void check() {
-    auto less = [](const auto& a, const auto& b) { return a.first < b.first; };
-    if (!std::is_sorted(all.begin(), all.end(), less)) std::sort(all.begin(), all.end(), less);
+  // (lists are mostly in the order of their addresses, and one behind the other: nothing to sort or merge)
+  void add(List&& more) {
+    if (!std::is_sorted(more.begin(), more.end(), less)) std::sort(more.begin(), more.end(), less);
+    if (all.empty()) { all = std::move(more); return; }
+    if (more.empty()) return;
+    if (less(more.back(), all.front())) all.swap(more);
+    const size_t n = all.size();
+    const bool behind = !less(more.front(), all.back());
+    all.insert(all.end(), more.begin(), more.end());
+    if (!behind) std::inplace_merge(all.begin(), all.begin() + n, all.end(), less);
+  }
+  void check() const {
     for (size_t i = 1; i < all.size(); ++i)
       SEP_ASSERT(all[i].first >= all[i - 1].second, "two tensors that are written in place share memory");
   }
@@ -115,14 +126,14 @@ struct InPlace {
   std::deque<at::Tensor> copies;
   std::vector<const at::Tensor*> back;             // whose copies they are
   InPlace(const TensorList& tensors, const at::Device& device) {
-    Ranges ranges;
+    Ranges::List ranges;
     work.reserve(tensors.size());
-    ranges.all.reserve(tensors.size());
+    ranges.reserve(tensors.size());
     for (const at::Tensor* t : tensors) {
       SEP_ASSERT(usable(*t, device), kListMessage);
       if (t->numel() == 0) continue;
       if (t->is_non_overlapping_and_dense()) {
-        ranges.add(*t);
+        ranges.push_back(Ranges::of(*t));
         work.push_back(t);
       } else {
         for (int64_t d = 0; d < t->dim(); ++d)
@@ -132,7 +143,9 @@ struct InPlace {
         work.push_back(&copies.back());
       }
     }
-    ranges.check();
+    Ranges r;
+    r.add(std::move(ranges));
+    r.check();
   }
   void finish(const TensorList& tensors) {
     for (size_t i = 0; i < back.size(); ++i) back[i]->detach().copy_(copies[i]);
@@ -209,8 +222,8 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
   const bool have_masters = !masters.empty();
   std::deque<at::Tensor> held;                       // gradients that had to be laid out like their parameters
   TensorList grad_at = grads;
-  Ranges ranges[4];
-  for (Ranges& r : ranges) r.all.reserve(n);
+  Ranges::List ranges[4];
+  for (Ranges::List& r : ranges) r.reserve(n);
   int64_t elements = 0;
   for (size_t i = 0; i < n; ++i) {
     const at::Tensor &p = *params[i], &g = *grads[i];
@@ -219,10 +232,10 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
     SEP_ASSERT(p.is_non_overlapping_and_dense(), "a parameter with gaps or repeats in memory cannot be updated in place");
     const bool plain = p.is_contiguous();
     auto same_layout = [&](const at::Tensor& t) { return plain ? t.is_contiguous() : t.strides() == p.strides(); };
-    auto state = [&](const at::Tensor& t, const char* what, Ranges& r) {
+    auto state = [&](const at::Tensor& t, const char* what, Ranges::List& r) {
       SEP_ASSERT(usable(t, device) && t.scalar_type() == at::kFloat && t.sizes() == p.sizes() && same_layout(t),
                  what << " must be float32 and laid out like their parameters");
-      if (t.numel() > 0) r.add(t);
+      if (t.numel() > 0) r.push_back(Ranges::of(t));
     };
     state(*exp_avgs[i], "exp_avgs", ranges[1]);
     state(*exp_avg_sqs[i], "exp_avg_sqs", ranges[2]);
@@ -233,9 +246,11 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
       grad_at[i] = &held.back();
     }
     elements += p.numel();
-    if (p.numel() > 0) ranges[0].add(p);
+    if (p.numel() > 0) ranges[0].push_back(Ranges::of(p));
   }
-  for (Ranges& r : ranges) r.check();
+  Ranges written;
+  for (Ranges::List& r : ranges) written.add(std::move(r));
+  written.check();
   AdamParams a{};
   const double c1 = 1.0 - std::pow(o.beta1, static_cast<double>(o.step)), c2 = 1.0 - std::pow(o.beta2, static_cast<double>(o.step));
   a.step_size = static_cast<float>(o.lr / c1);

@@ -11,16 +11,19 @@ import torch
 from .. import _ext
 
 
+def _over_ranks(group) -> bool:
+    return group is not None and group.size() > 1
+
+
 def _total(grads, sharded, group):
-    """``(norm, grads, sharded)`` with the sharded gradients' squares summed over the ranks of ``group``."""
+    """The norm, with the sharded gradients' squares summed over the ranks of ``group`` (every rank takes part, also one
+    that holds no sharded gradient)."""
     C = _ext.load()
-    norm, squares = C.list_norm(grads)
-    if not sharded:
-        return norm
-    parts = C.list_norm(sharded)[1]
-    if group is not None and group.size() > 1:
-        torch.distributed.all_reduce(parts, group=group)
-    return (squares.to(parts.device) + parts).sqrt().float()
+    if not _over_ranks(group):
+        return C.list_norm(grads + sharded)[0]
+    squares, parts = C.list_norm(grads)[1], C.list_norm(sharded)[1]
+    torch.distributed.all_reduce(parts, group=group)
+    return (squares + parts).sqrt().float()
 
 
 def grad_norm(grads: Sequence[torch.Tensor], *, sharded: Sequence[torch.Tensor] = (), group=None) -> torch.Tensor:
@@ -29,7 +32,7 @@ def grad_norm(grads: Sequence[torch.Tensor], *, sharded: Sequence[torch.Tensor] 
 
     ``sharded``: gradients of which every rank of ``group`` holds others (the experts' weights under expert
     parallelism); their squares are summed over the group, those of ``grads`` (the same on all ranks) are counted
-    once.  Squares are formed in 32 bits: elements above 1.8e19 give an infinite norm."""
+    once.  With a ``group`` of several ranks the call is collective.  Squares are formed in 32 bits: elements above 1.8e19 give an infinite norm."""
     return _total(list(grads), list(sharded), group)
 
 
@@ -43,8 +46,8 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, *, sharded: 
     needed for it."""
     grads, sharded = list(grads), list(sharded)
     C = _ext.load()
-    if not sharded:
-        return C.list_clip(grads, float(max_norm))
+    if not _over_ranks(group):
+        return C.list_clip(grads + sharded, float(max_norm))
     norm = _total(grads, sharded, group)
     C.list_scale(grads + sharded, norm, float(max_norm))
     return norm

@@ -39,7 +39,7 @@ def train(model, optimizer, steps: int, tokens: int, vocab: int, device, seed: i
         norm = optimizer.step()
         losses.append(loss.detach())
         if report is not None:
-            report(i, loss, norm)
+            report(i, loss.detach(), norm)
     return torch.stack(losses).tolist()
 
 

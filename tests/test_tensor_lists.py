@@ -152,7 +152,7 @@ def test_refusals(native):
         with pytest.raises(ValueError):
             adamw_step_([p], [t], [m], [v], **{**ok, **change})
     for lists in (([p], [t[:50]], [m], [v]), ([p], [t], [m], []), ([p, p], [t, t], [m, m.clone()], [v, v.clone()]), ([p.double()], [t], [m], [v]),
-                  ([p], [t], [m.to(BF)], [v]), ([p[::2]], [t[::2]], [m[::2]], [v[::2]])):
+                  ([p], [t], [m], [m]), ([p], [t], [p], [v]), ([p], [t], [m.to(BF)], [v]), ([p[::2]], [t[::2]], [m[::2]], [v[::2]])):
         with pytest.raises(ValueError):
             adamw_step_(*lists, **ok)
 

@@ -52,6 +52,11 @@ def _rank(rank, world, store, out):
     dist.init_process_group("gloo", init_method=f"file://{store}", rank=rank, world_size=world)
     _ext.load = lambda: FakeNative
     shared, mine = [torch.full((10,), 2.0), torch.full((3,), -1.0)], [torch.full((7,), float(rank + 1))]
+    if rank == 1:                     # a rank without sharded gradients takes part all the same
+        alone = grad_norm(shared, sharded=[], group=dist.group.WORLD)
+    else:
+        alone = grad_norm(shared, sharded=mine, group=dist.group.WORLD)
+    assert abs(float(alone) - (40.0 + 3.0 + 7.0) ** 0.5) < 1e-5
     norm = grad_norm(shared, sharded=mine, group=dist.group.WORLD)
     clipped = clip_grad_norm_(shared, 3.0, sharded=mine, group=dist.group.WORLD)
     torch.save((norm, clipped, shared, mine), f"{out}.{rank}")
