@@ -27,19 +27,23 @@ constexpr int64_t kBandBytes = 48ll << 20;       // rows of x that a band of uni
 // Tokens as columns (the narrow form) where that multiplies at least an eighth less, among calls of up to as many tokens as its warps keep
 // statistics of; always where dz is split.  300 tokens, hidden 2048, V 100003: 737 us a training pass with rows, 640 with columns; 1 token,
 // hidden 4096, V 128000, forward: 248 and 172.
-void plan_tiles(LossParams& p) {
+void plan_tiles(LossParams& p, bool backward) {
   const int64_t T = p.T, units = ceil_of(T, kLossUnit), tokens = ceil_of(ceil_of(T, units), 32) * 32;
   p.narrow = T <= kSplitTokens || (T <= kNarrowTokens && tokens * units * 8 <= 7 * kLossUnit * units);
   p.tile_tokens = p.narrow ? static_cast<int>(tokens) : kLossUnit;
   p.row_units = static_cast<int>(units);
-  loss_narrow_ring(p);
+  // Short calls keep dz to 16 bits of mantissa, as a sum of two bf16 numbers: rounding errors of many tokens average out in dW,
+  // those of a few do not (one token, target at p = 0.5: dW 0.4 % off where the result's own rounding is 0.2 %).
+  p.split2 = T <= kSplitTokens ? 1 : 0;
+  // Up to 32 tokens dw takes 32 at a time, so that a stage of the ring need not hold more than 128 rows of the projection and those tokens, and more
+  // of the projection is on its way: 1 token, hidden 4096, V 128000 581 -> 547 us, 16 tokens, hidden 2048, V 100003 255 -> 241.  (40
+  // tokens in two such blocks: 259 -> 287.)
+  p.dw_rows = T <= 32 ? 32 : 64;
+  loss_narrow_ring(p, backward);
 }
 void plan_backward(LossParams& p, int sms) {
   const int64_t T = p.T, H = p.H, V = p.V, pairs = sms / 2;
   p.h_units = static_cast<int>(ceil_of(H, kLossUnit));
-  // Short calls keep dz to 16 bits of mantissa, as a sum of two bf16 numbers: rounding errors of many tokens average out in dW,
-  // those of a few do not (one token, target at p = 0.5: dW 0.4 % off where the result's own rounding is 0.2 %).
-  p.split2 = T <= kSplitTokens ? 1 : 0;
   const int64_t row_bytes = T * 2 * (p.split2 ? 2 : 1);
   const int64_t want = ceil_of(V * row_bytes, kPieceBytes);
   p.piece = static_cast<int>(ceil_of(ceil_of(V, want), kLossUnit) * kLossUnit);
@@ -47,7 +51,7 @@ void plan_backward(LossParams& p, int sms) {
   p.last_cols = static_cast<int>(V - static_cast<int64_t>(p.pieces - 1) * p.piece);
   p.ahead = std::min(1, p.pieces);
   p.buffers = std::min(p.ahead + 1, p.pieces);
-  const int64_t v_blocks = ceil_of(V, 64), t_blocks = ceil_of(T, 64) * (p.split2 ? 2 : 1), tiles = ceil_of(V, kLossUnit);
+  const int64_t v_blocks = ceil_of(V, 64), t_blocks = ceil_of(T, p.dw_rows) * (p.split2 ? 2 : 1), tiles = ceil_of(V, kLossUnit);
   // k-blocks of all the work, for each pair
   const int64_t all = (p.row_units * tiles * ceil_of(H, 64) + (p.want_dx ? p.row_units * p.h_units * v_blocks : 0) +
                        (p.want_dw ? tiles * p.h_units * t_blocks : 0)) / pairs + 1;
@@ -120,7 +124,7 @@ LossParams plan(int64_t T, int64_t H, int64_t V, bool want_dx, bool want_dw, int
   LossParams p{};
   p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
   p.want_dx = want_dx; p.want_dw = want_dw;
-  plan_tiles(p);
+  plan_tiles(p, true);
   plan_backward(p, sms);
   plan_band(p);
   p.claim_lead = claim_lead(p, true);
@@ -143,7 +147,7 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   const LaunchContext ctx = call.context(2);
   LossParams p{};
   p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
-  plan_tiles(p);
+  plan_tiles(p, false);
   plan_band(p);
   p.claim_lead = claim_lead(p, false);
   const int64_t parts = loss_forward_parts(p, ctx.sms);
@@ -225,12 +229,12 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
   LossMaps m{};
   m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, p.tile_tokens / 2);
   m.w_k = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 128);
-  if (want_dw) m.x_mn = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, 64);
+  if (want_dw) m.x_mn = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, p.dw_rows);
   if (want_dx) m.w_mn = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 64);
   const int64_t panels = p.buffers * z_layers * (p.piece / 64);
   auto z_map = [&](int cols, int rows, CUtensorMapSwizzle swizzle) { return make_tmap(base + z_at, 64, T, panels, 64, T * 64, cols, rows, swizzle); };
   if (want_dx) m.z_k = z_map(64, p.split2 ? p.tile_tokens : p.tile_tokens / 2, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (want_dw) m.z_mn = z_map(64, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (want_dw) m.z_mn = z_map(64, p.dw_rows, CU_TENSOR_MAP_SWIZZLE_128B);
   m.z_out = p.narrow ? z_map(32, 32, CU_TENSOR_MAP_SWIZZLE_64B) : z_map(64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
   if (want_dw) m.dw = make_tmap(dw.data_ptr(), H, V, 1, H, H * V, 64, 32);
   p.dx_parts = reinterpret_cast<float*>(base + dx_at);

@@ -19,7 +19,8 @@ struct LossParams {
   int narrow;                    // 1: tokens are the columns of a unit (see linear_loss_kernels.cu), `tile_tokens` of them
   int tile_tokens;               // tokens of a unit: 256, narrow: a multiple of 32
   int row_units;                 // ceil(T / tile_tokens)
-  int stages, stage_bytes;       // narrow forward: the operand ring
+  int stages, stage_bytes;       // narrow: the operand ring
+  int dw_rows;                   // tokens of a k-block of dw: 64, or 32 where the ring's stages are too small for that
   int band;                      // row units that are walked together (see unit_of)
   // --- forward ---
   float2* parts;                 // [loss_forward_parts][T] maximum and sum of exp(z - maximum)
@@ -62,7 +63,7 @@ struct LossMaps {                // CUtensorMap each: loads in boxes of 64 colum
   CUtensorMap dw, dx;
 };
 
-void loss_narrow_ring(LossParams& p);      // stages and stage_bytes of the narrow forward
+void loss_narrow_ring(LossParams& p, bool backward);      // stages and stage_bytes of the narrow form (tile_tokens, split2, dw_rows given)
 long long loss_forward_parts(const LossParams& p, int sms);
 cudaError_t launch_loss_forward(const LossParams& p, const LossMaps& m, int sms, cudaStream_t stream);
 cudaError_t launch_loss_backward(const LossParams& p, const LossMaps& m, int sms, cudaStream_t stream);

@@ -40,8 +40,8 @@ constexpr int kQueue = 4;
 constexpr int kNarrowStages = 9, kNarrowRing = 5 * kStageBytes;
 constexpr int kNarrowUnits = 4;                  // token tiles of the narrow form, at most
 constexpr int kNarrowStats = kNarrowUnits * 4 * 32 * 8;   // bytes a warp: [token tile][its 32-token pieces][lane] (maximum, sum)
-constexpr int stages_of(bool fwd, bool narrow) { return fwd ? (narrow ? kNarrowStages : 7) : 5; }
-constexpr int ring_bytes(bool fwd, bool narrow) { return fwd && narrow ? kNarrowRing : stages_of(fwd, narrow) * kStageBytes; }
+constexpr int stages_of(bool fwd, bool narrow) { return narrow ? kNarrowStages : fwd ? 7 : 5; }
+constexpr int ring_bytes(bool fwd, bool narrow) { return narrow ? kNarrowRing : stages_of(fwd, narrow) * kStageBytes; }
 constexpr int smem_bytes(bool fwd, bool narrow) { return ring_bytes(fwd, narrow) + (fwd ? (narrow ? kEpiWarps * (4096 + kNarrowStats) : 0) : kEpiWarps * kStagingBytes) + 1024; }
 constexpr int kTmemCols = 512;
 constexpr int kDoneWarps = 2 * kEpiWarps;        // reports per unit
@@ -145,7 +145,7 @@ __host__ __device__ __forceinline__ Unit unit_of(const LossParams& p, int lin) {
     band_decode(8, rem, ceil_div(cols, kLossUnit), ceil_div(p.h_units, p.dw_group), u.m, u.n);
     u.n *= p.dw_group;
     u.tiles = lesser(p.dw_group, p.h_units - u.n);
-    u.k_blocks = ceil_div(p.T, kBK) * (p.split2 ? 2 : 1);
+    u.k_blocks = ceil_div(p.T, p.dw_rows) * (p.split2 ? 2 : 1);
   }
   return u;
 }
@@ -196,8 +196,9 @@ template <bool FWD, bool NARROW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__ LossMaps maps) {
   constexpr int kStages = stages_of(FWD, NARROW);
-  const int stages = FWD && NARROW ? p.stages : kStages;
-  const int stage_bytes = FWD && NARROW ? p.stage_bytes : kStageBytes;
+  const int stages = NARROW ? p.stages : kStages;
+  const int stage_bytes = NARROW ? p.stage_bytes : kStageBytes;
+  const int dw_rows = NARROW ? p.dw_rows : kBK;
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   unsigned char* stage_base = smem;
@@ -326,12 +327,12 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         const int a0 = u.m * kLossUnit + half * 128;
         const int v0 = u.piece * (FWD ? 0 : p.piece);
         const int z0 = FWD ? 0 : panel_of(p, u.piece, 0);
-        const int t_blocks = ceil_div(p.T, kBK);
+        const int t_blocks = ceil_div(p.T, dw_rows);
         // narrow: rows of x / dz that this CTA loads, and which (split2: the leading halves of dz by the first CTA, the remainders by the second)
         const bool both = NARROW && !FWD && u.kind == kLossDx && p.split2;
         const int my_tokens = NARROW ? (both ? p.tile_tokens : p.tile_tokens / 2) : 0;
         const int t0 = NARROW ? u.m * p.tile_tokens + (both ? 0 : half * my_tokens) : 0;
-        const uint32_t pair_bytes = NARROW && (FWD || u.kind != kLossDw) ? 2 * (kOperandBytes + my_tokens * 128) : 2 * kStageBytes;
+        const uint32_t pair_bytes = NARROW ? 2 * (FWD || u.kind != kLossDw ? kOperandBytes + my_tokens * 128 : 4 * dw_rows * 128) : 2 * kStageBytes;
         const int warn = max(u.k_blocks - kClaimAhead, 0);
         if (u.k_blocks == 0 && leader) st_volatile_shared(&s_progress, it + 1);
         for (int tile = 0; tile < u.tiles && ok; ++tile, ++u.n) {
@@ -359,12 +360,13 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
             tma_load_3d_pair(sw + kOperandBytes / 2, &maps.w_mn, bar, b0 + 64, v0 + k, 0);
           } else {
             const int rest = kb >= t_blocks ? 1 : 0;         // split2: all leading halves, then all remainders
-            const int t = (kb - rest * t_blocks) * kBK;
+            const int t = (kb - rest * t_blocks) * dw_rows, box = dw_rows * 128;
+            unsigned char* const sx = sa + 2 * box;
             const int panel = (rest ? panel_of(p, u.piece, 1) : z0) + a0 / 64;
             tma_load_3d_pair(sa, &maps.z_mn, bar, 0, t, panel);
-            tma_load_3d_pair(sa + kOperandBytes / 2, &maps.z_mn, bar, 0, t, panel + 1);
-            tma_load_3d_pair(sb, &maps.x_mn, bar, b0, t, 0);
-            tma_load_3d_pair(sb + kOperandBytes / 2, &maps.x_mn, bar, b0 + 64, t, 0);
+            tma_load_3d_pair(sa + box, &maps.z_mn, bar, 0, t, panel + 1);
+            tma_load_3d_pair(sx, &maps.x_mn, bar, b0, t, 0);
+            tma_load_3d_pair(sx + box, &maps.x_mn, bar, b0 + 64, t, 0);
           }
           ++issued;
           if (++stage == stages) { stage = 0; phase ^= 1; }
@@ -396,7 +398,9 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         const uint32_t idesc = umma_idesc_bf16(256, 0, 0, 0) | (a_mn ? 1u << 15 : 0) | (b_mn ? 1u << 16 : 0) | (static_cast<uint32_t>(cols >> 3) << 17);
         // per 16 elements of K: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major box
         const uint32_t step_a = a_mn ? 16 * 128 : 32, step_b = b_mn ? 16 * 128 : 32;
-        const uint32_t lbo_a = a_mn ? kBK * 128 : 16, lbo_b = b_mn ? kBK * 128 : 16;
+        const bool half_blocks = NARROW && !FWD && u.kind == kLossDw && dw_rows != kBK;
+        const uint32_t rows = half_blocks ? kBK / 2 : kBK;           // of K in a stage
+        const uint32_t lbo_a = a_mn ? rows * 128 : 16, lbo_b = b_mn ? rows * 128 : 16;
         const int segment = FWD ? kSegmentBlocks : u.k_blocks;
         for (int first = 0; first < u.k_blocks && ok; first += segment) {
         if (!__all_sync(0xffffffffu, mbar_wait<true>(&tmem_empty[acc], acc_phase ^ 1, budget, p.status))) { ok = false; break; }
@@ -407,10 +411,10 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           if (!__all_sync(0xffffffffu, mbar_wait<true>(&full_bar[stage], phase, budget, p.status))) { ok = false; break; }
           tc_fence_after_sync();
           if (elect_one()) {
-            const uint32_t a_addr = smem_u32(stage_base + stage * stage_bytes), b_addr = a_addr + kOperandBytes;
+            const uint32_t a_addr = smem_u32(stage_base + stage * stage_bytes), b_addr = a_addr + kOperandBytes / kBK * rows;
 #pragma unroll
             for (int j = 0; j < kBK / 16; ++j)
-              umma_bf16_ss<2>(tmem_d, umma_smem_desc(a_addr + j * step_a, lbo_a, 1024), umma_smem_desc(b_addr + j * step_b, lbo_b, 1024),
+              if (!NARROW || j < 2 || !half_blocks) umma_bf16_ss<2>(tmem_d, umma_smem_desc(a_addr + j * step_a, lbo_a, 1024), umma_smem_desc(b_addr + j * step_b, lbo_b, 1024),
                               idesc, (kb > first || j > 0) ? 1u : 0u);
             umma_commit<2>(&empty_bar[stage]);
             if (kb == end - 1) umma_commit<2>(&tmem_full[acc]);
@@ -988,8 +992,10 @@ long long loss_backward_units(const LossParams& p) {
   return static_cast<long long>(p.pieces - 1) * (c.dz + c.dw) + c.dz_last + c.dw_last + static_cast<long long>(p.pieces) * c.dx;
 }
 
-void loss_narrow_ring(LossParams& p) {
-  p.stage_bytes = kOperandBytes + (p.tile_tokens / 2 * 128 + 1023) / 1024 * 1024;      // (operands stand on 1024-byte boundaries)
+void loss_narrow_ring(LossParams& p, bool backward) {
+  const int tokens = backward && p.split2 ? p.tile_tokens : p.tile_tokens / 2;      // that a CTA loads
+  p.stage_bytes = kOperandBytes + (tokens * 128 + 1023) / 1024 * 1024;              // (operands stand on 1024-byte boundaries)
+  if (backward) p.stage_bytes = greater(p.stage_bytes, 4 * p.dw_rows * 128);
   p.stages = lesser(kNarrowStages, kNarrowRing / p.stage_bytes);
 }
 static long long forward_units(const LossParams& p) { return static_cast<long long>(p.row_units) * ((p.V + kLossUnit - 1) / kLossUnit); }

@@ -45,7 +45,7 @@ def test_units_and_order(T, H, V, want_dx, want_dw):
                 assert j == 0 or max(place[DX, j - 1]) < i
                 blocks.setdefault((j, m, n), []).append((k0, k))
             else:
-                assert (k0, k) == (0, up(T, 64) * (2 if split2 else 1))
+                assert (k0, k) == (0, up(T, 32 if T <= 32 else 64) * (2 if split2 else 1))
     for (j, m, n), got in blocks.items():      # the splits of a dx tile cover its piece once
         covered = [b for k0, k in got for b in range(k0, k0 + k)]
         assert sorted(covered) == list(range(up(cols[j], 64)))
