@@ -116,7 +116,7 @@ struct LossCall : torch::CustomClassHolder {
   bool counters_used = false;    // a backward has run (with retain_graph another may follow)
 };
 
-// The loss; and what the backward needs: [2][T] softmax statistics, 1 / counted tokens, and from `counters_at` on the counters of its kernel,
+// The loss; and what the backward needs: [3][T] softmax statistics, 1 / counted tokens, and from `counters_at` on the counters of its kernel,
 // which the forward's kernel clears.
 struct Forward { at::Tensor loss, stats; };
 
@@ -130,7 +130,7 @@ LossParams plan(int64_t T, int64_t H, int64_t V, bool want_dx, bool want_dw, int
   p.claim_lead = claim_lead(p, true);
   return p;
 }
-int64_t counters_at(int64_t T) { return ceil_of(2 * T + 1, 64) * 64; }
+int64_t counters_at(int64_t T) { return ceil_of(3 * T + 1, 64) * 64; }
 int64_t counter_ints(const LossParams& p) { return 4 + (3 + p.piece / kLossUnit) * static_cast<int64_t>(p.pieces); }
 
 Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets) {
@@ -169,7 +169,7 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
     p.zero_ints = static_cast<int>(ints + 1);
     ticket = p.zero + ints;
   } else {
-    out.stats = at::empty({2 * T + 1}, f32);
+    out.stats = at::empty({3 * T + 1}, f32);
   }
   p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
   LossMaps m{};
@@ -188,7 +188,7 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   f.each = reduced ? reinterpret_cast<float*>(base + each_at) : out.loss.data_ptr<float>();
   f.top = out.stats.data_ptr<float>();
   f.loss = reduced ? out.loss.data_ptr<float>() : nullptr;
-  f.inv_count = f.top + 2 * T;
+  f.inv_count = f.top + 3 * T;
   f.ticket = ticket;
   f.status = ctx.status; f.rank = ctx.rank;
   SEP_CUDA_CHECK(launch_loss_final(f, ctx.stream));
@@ -221,7 +221,7 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
   p.top = stats.data_ptr<float>();
   if (call.reduction == kLossNone) p.row_scale = up.data_ptr<float>();
   else p.scale = up.data_ptr<float>();
-  if (call.reduction == kLossMean) p.scale2 = p.top + 2 * T;
+  if (call.reduction == kLossMean) p.scale2 = p.top + 3 * T;
   p.claim = reinterpret_cast<int*>(stats.data_ptr<float>() + counters_at(T));
   p.done = p.claim + 4;
   p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;

@@ -29,7 +29,7 @@ struct LossParams {
   long long ignore_index;
   int* zero; int zero_ints;      // memory that the forward kernel clears for the kernels after it
   // --- backward ---
-  const float* top;              // [2][T] each token's largest logit, and log2 of its sum of exp(z - largest)
+  const float* top;              // [3][T] each token's largest logit, log2 of its sum of exp(z - largest), and its target's logit
   const float* row_scale;        // [T] upstream gradient of each token's loss, or null: 1
   const float* scale;            // [1] factor of every gradient, or null: 1 ...
   const float* scale2;           // [1] ... and another (1 / counted tokens)
@@ -79,7 +79,7 @@ struct LossFinalParams {
   long long ignore_index;
   int mean, sum;                 // reduction (neither: per token)
   float* each;                   // [T] losses (scratch where they are reduced)
-  float* top;                    // [2][T], as in LossParams
+  float* top;                    // [3][T], as in LossParams
   float* loss;                   // [1] where they are reduced
   float* inv_count;              // [1] 1 / counted tokens (mean; 0 without any)
   int* ticket;                   // [1], zero on entry (cleared by the forward kernel)

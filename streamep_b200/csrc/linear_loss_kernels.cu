@@ -182,6 +182,14 @@ __device__ __forceinline__ void tma_reduce_add_3d(const void* tmap, const void* 
                :: "l"(tmap), "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
+__device__ __forceinline__ void st_shared_b16(uint32_t addr, uint32_t low_half) {
+  asm volatile("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tst.shared.b16 [%0], h;\n\t}" :: "r"(addr), "r"(low_half) : "memory");
+}
+// p - 1 of the target, from the forward's own logit: the one computed again lacks what kSegmentBlocks is for, 1e-4 of a logit of 12 at H 7168,
+// which is more than 1 - p of a token that the model is sure of.
+__device__ __forceinline__ float target_gradient(float target_z, float top, float log2_sum) {
+  return expm1f(fmaf(-0.693147181f, log2_sum, target_z - top));
+}
 // Lane l has element i of 32 in v[i]; afterwards lane l has in v[j] what lane j had in v[l].  `tile`: 4 KB of the warp's own.
 __device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory"); }
 __device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
@@ -470,7 +478,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
       const int row = row0 + lane;
       const bool empty = u.k_blocks == 0;
       // fetched while the tensor cores still work on the tile
-      int col = -1; float top = 0.f, log2_sum = 0.f, c_t = 0.f;
+      int col = -1; float top = 0.f, log2_sum = 0.f, target_z = 0.f, c_t = 0.f;
       bool dead = true;              // an ignored token (or no token): zeros whatever its logits are
       if (!NARROW && u.kind <= kLossDz) {
         if (row < p.T) {
@@ -480,7 +488,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           if (!FWD && y != p.ignore_index) {
             dead = false;
             c_t = p.row_scale != nullptr ? p.row_scale[row] : 1.f;
-            top = p.top[row]; log2_sum = p.top[p.T + row];
+            top = p.top[row]; log2_sum = p.top[p.T + row]; target_z = p.top[2 * static_cast<size_t>(p.T) + row];
           }
         }
       }
@@ -565,7 +573,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
 #pragma unroll 1
         for (int c = 0; c < count32; ++c) {
           const int t_first = u.m * p.tile_tokens + (first32 + c) * 32, t = t_first + lane;
-          float top = 0.f, log2_sum = 0.f, c_t = 0.f;
+          float top = 0.f, log2_sum = 0.f, target_z = 0.f, c_t = 0.f;
           int target = -1;               // among this warp's rows
           bool dead = true;
           if (t < p.T) {
@@ -573,7 +581,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
             if (y != p.ignore_index) {
               dead = false;
               c_t = p.row_scale != nullptr ? p.row_scale[t] : 1.f;
-              top = p.top[t]; log2_sum = p.top[p.T + t];
+              top = p.top[t]; log2_sum = p.top[p.T + t]; target_z = p.top[2 * static_cast<size_t>(p.T) + t];
               const long long rel = y - static_cast<long long>(u.piece) * p.piece - v_first;
               if (rel >= 0 && rel < 32) target = static_cast<int>(rel);
             }
@@ -594,22 +602,22 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
             uint32_t o[4], rest[4];
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
-              float d[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int j = q * 8 + h * 2 + e;
-                float v = ex2(fmaf(turn_read(turn, lane, j) - top, kLog2e, -log2_sum));
-                if (j == target) v -= 1.f;
-                v *= c_t;
-                if (dead || v_first + j >= n_cols) v = 0.f;
-                d[e] = v;
-              }
-              o[h] = pack_bf16x2(d[0], d[1]);
+              const int j = q * 8 + h * 2;
+              float a = ex2(fmaf(turn_read(turn, lane, j) - top, kLog2e, -log2_sum)) * c_t, b = ex2(fmaf(turn_read(turn, lane, j + 1) - top, kLog2e, -log2_sum)) * c_t;
+              if (dead || v_first + j >= n_cols) a = 0.f;
+              if (dead || v_first + j + 1 >= n_cols) b = 0.f;
+              o[h] = pack_bf16x2(a, b);
               const float2 lead = unpack_bf16x2(o[h]);
-              rest[h] = pack_bf16x2(d[0] - lead.x, d[1] - lead.y);
+              rest[h] = pack_bf16x2(a - lead.x, b - lead.y);
             }
             st_shared_v4(smem_u32(lead_tile) + stage_off<64>(lane, q), o[0], o[1], o[2], o[3]);
             if (p.split2) st_shared_v4(smem_u32(lead_tile) + 2048 + stage_off<64>(lane, q), rest[0], rest[1], rest[2], rest[3]);
+          }
+          if (target >= 0) {                 // (a lane writes over what it wrote itself)
+            const float d = target_gradient(target_z, top, log2_sum) * c_t;
+            const uint32_t at = smem_u32(lead_tile) + stage_off<64>(lane, target / 8) + (target & 7) * 2, lead = pack_bf16x2(d, 0.f);
+            st_shared_b16(at, lead);
+            if (p.split2) st_shared_b16(at + 2048, pack_bf16x2(d - unpack_bf16x2(lead).x, 0.f));
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -717,6 +725,8 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         if (row < p.T) p.parts[static_cast<size_t>(u.n * 2 + side) * p.T + row] = make_float2(m, s0 + s1);
       } else if (u.kind == kLossDz) {
         const int z_chunks = (chunks + 1) / 2 * 2;       // (the last panel is filled up with zeros)
+        const Pair minus_top = pair_of(-top, -top), minus_sum = pair_of(-log2_sum, -log2_sum), log2e = pair_of(kLog2e, kLog2e), scale_t = pair_of(c_t, c_t);
+        const uint32_t target_dz = pack_bf16x2(target_gradient(target_z, top, log2_sum) * c_t, 0.f);
         const bool rows = row0 < p.T;
         if (!rows) give_back();
 #pragma unroll 1
@@ -724,29 +734,26 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
           fetch(c);
           if (c == z_chunks - 1) give_back();
           const int left = n_cols - n0 - c * 32;
-          const bool target_here = __any_sync(0xffffffffu, (col >> 5) == c), masked = left < 32 || __any_sync(0xffffffffu, dead);
+          const bool target_here = __any_sync(0xffffffffu, (col >> 5) == c);
           if ((c & 1) == 0) stg = next_tile();
-          const Pair minus_top = pair_of(-top, -top), minus_sum = pair_of(-log2_sum, -log2_sum), log2e = pair_of(kLog2e, kLog2e), scale_t = pair_of(c_t, c_t);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t o[4];
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
               const int i = q * 8 + h * 2;
-              float d[2];
-              parts_of(ex2(fma2(pair_of(__uint_as_float(r[i]), __uint_as_float(r[i + 1])) + minus_top, log2e, minus_sum)), d[0], d[1]);
-              if (target_here) {
-                if (col == c * 32 + i) d[0] -= 1.f;
-                if (col == c * 32 + i + 1) d[1] -= 1.f;
+              float a, b;
+              parts_of(ex2(fma2(pair_of(__uint_as_float(r[i]), __uint_as_float(r[i + 1])) + minus_top, log2e, minus_sum)) * scale_t, a, b);
+              o[h] = dead ? 0u : pack_bf16x2(a, b);
+              if (left < 32) {                 // (uniform: the piece ends here)
+                if (i >= left) o[h] = 0u;
+                else if (i + 1 >= left) o[h] &= 0xffffu;
               }
-              parts_of(pair_of(d[0], d[1]) * scale_t, d[0], d[1]);
-              if (masked) {
-                if (dead || i >= left) d[0] = 0.f;
-                if (dead || i + 1 >= left) d[1] = 0.f;
-              }
-              o[h] = pack_bf16x2(d[0], d[1]);
             }
             st_shared_v4(stg + stage_off<128>(lane, (c & 1) * 4 + q), o[0], o[1], o[2], o[3]);
+          }
+          if (target_here) {                 // (a lane writes over what it wrote itself)
+            if ((col >> 5) == c) st_shared_b16(stg + stage_off<128>(lane, (c & 1) * 4 + (col & 31) / 8) + (col & 7) * 2, target_dz);
           }
           if ((c & 1) == 1) {
             fence_proxy_async_smem();
@@ -913,6 +920,7 @@ __global__ void __launch_bounds__(kFinalThreads) loss_final_kernel(const LossFin
       }
       p.top[row] = v.x;
       p.top[p.T + row] = log2f(v.y);
+      p.top[2 * static_cast<size_t>(p.T) + row] = p.target_logit[row];
       p.each[row] = loss;
     }
   }

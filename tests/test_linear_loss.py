@@ -84,6 +84,28 @@ def test_other_reductions(native, T, H, V, reduction):
 
 
 # ------------------------------------------------------------------------------------------------------------------- edges
+@pytest.mark.parametrize("T", [20, 200, 500])
+def test_tokens_that_the_model_is_sure_of(native, T):
+    """A target that stands out by 14 (p = 1 - 1e-4 or so): its gradient is the small number 1 - p, and keeps its digits.  p - 1 from the forward's
+    fp32 logit: a few 1e-6 of a logit of 14, relative to 1 - p; then bf16 (2^-9), with the other columns' sum along W."""
+    H, V = 4096, 600
+    g = torch.Generator(device="cpu").manual_seed(T)
+    w = torch.sign(torch.randn(V, H, generator=g)).to(torch.bfloat16).to(DEV) / 64          # |w|^2 = 1
+    y = torch.randint(0, V, (T,), generator=g).to(DEV)
+    x = (14.0 * w[y].float() + 0.01 * torch.randn(T, H, generator=g).to(DEV)).to(torch.bfloat16)
+    loss, gx, _ = run(x, w, y, reduction="none", upstream=torch.ones(T, device=DEV))
+    want = oracle(x, w, y, torch.ones(T, device=DEV), "none")
+    assert float(want[0].max()) < 2e-3
+    torch.testing.assert_close(loss.double(), want[0], rtol=1e-2, atol=3e-7)
+    near(gx, want[1], 1e-2)
+
+
+def test_a_vocabulary_of_one(native):
+    x, w, y = make(50, 64, 1)
+    loss, gx, gw = run(x, w, y)
+    assert float(loss) == 0.0 and not gx.any() and not gw.any()
+
+
 def test_gradient_against_differences(native):
     """(loss(a) - loss(b)) against the gradient half way, along random directions.  Steps of 2 % of each value: the third-order term is
     below 1 % of the difference, the losses' own errors (2e-6 of about 6) below 1 % of differences of at least 1e-2."""
