@@ -113,8 +113,19 @@ struct LossCall : torch::CustomClassHolder {
   int64_t ignore_index;
   int reduction;
   bool want_dx = false, want_dw = false;
-  bool counters_used = false;    // a backward has run (with retain_graph another may follow)
+  // The forward's kernel clears the backward's counters, for one backward after it.  A backward clears them itself when another has run
+  // (retain_graph), and when the two are not of one captured graph (or of none): one may be replayed without the other.
+  bool counters_used = false;
+  unsigned long long capture = 0;
 };
+
+// The capture that the stream takes part in, 0: none.
+unsigned long long capture_of(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  SEP_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
 
 // The loss; and what the backward needs: [3][T] softmax statistics, 1 / counted tokens, and from `counters_at` on the counters of its kernel,
 // which the forward's kernel clears.
@@ -165,6 +176,7 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
     // the ticket stands behind the backward's counters, to be cleared with them
     const int64_t ints = counter_ints(plan(T, H, V, call.want_dx, call.want_dw, ctx.sms));
     out.stats = at::empty({counters_at(T) + ints + 1}, f32);
+    call.capture = capture_of(ctx.stream);
     p.zero = reinterpret_cast<int*>(out.stats.data_ptr<float>() + counters_at(T));
     p.zero_ints = static_cast<int>(ints + 1);
     ticket = p.zero + ints;
@@ -241,7 +253,7 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
   p.dx = want_dx ? dx.data_ptr() : nullptr;
   if (want_dx && p.dx_direct) m.dx = make_tmap(dx.data_ptr(), H, T, 1, H, T * H, 64, 32);
   else if (want_dx && !p.narrow) m.dx = make_tmap(base + dx_at, H, T, slots, H, T * H, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
-  if (call.counters_used) SEP_CUDA_CHECK(cudaMemsetAsync(p.claim, 0, counter_ints(p) * sizeof(int), ctx.stream));
+  if (call.counters_used || call.capture != capture_of(ctx.stream)) SEP_CUDA_CHECK(cudaMemsetAsync(p.claim, 0, counter_ints(p) * sizeof(int), ctx.stream));
   call.counters_used = true;
   SEP_CUDA_CHECK(launch_loss_backward(p, m, ctx.sms, ctx.stream));
   if (want_dx && !p.dx_direct) {

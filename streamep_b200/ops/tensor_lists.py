@@ -40,7 +40,7 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, *, sharded: 
     """Scales all gradients in place by ``min(1, max_norm / (norm + 1e-6))`` and returns their norm before that (see
     :func:`grad_norm`).  Below the limit the gradients are read once and not written.  A norm of NaN makes all
     gradients NaN, an infinite one makes them 0 (and NaN where they are infinite), as ``torch.nn.utils`` has it.
-    Tensors that share memory are refused, and so are expanded ones.
+    Tensors that share memory are refused (strided views, which go through copies, are not compared), and so are expanded ones.
 
     Where an update follows, :func:`adamw_step_` applies the same factor on its way and no pass over the gradients is
     needed for it."""
@@ -64,7 +64,8 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
         w = w * (1 - lr * weight_decay) - lr * (exp_avg / (1 - b1**step)) / (sqrt(exp_avg_sq / (1 - b2**step)) + eps)
 
     Parameters and gradients are bf16 or float32, the moments float32, all arithmetic 32 bits.  With ``masters``
-    (float32) ``w`` is the master copy and the parameter becomes its rounding.  ``step`` counts from 1.
+    (float32) ``w`` is the master copy and the parameter becomes its rounding.  ``step`` counts from 1;
+    like ``lr`` it is a number of the host, which a captured graph repeats.
     ``skip_nonfinite``: leave everything as it is when ``norm`` is not finite, decided on the device."""
     if max_norm is not None and norm is None:
         raise ValueError("max_norm needs the gradients' norm (grad_norm)")

@@ -289,6 +289,45 @@ def test_streams_and_capture(native):
     assert torch.equal(loss, want[0]) and torch.equal(grads[0], want[1]) and torch.equal(grads[1], want[2])
 
 
+@pytest.mark.parametrize("shape", [(48, 256, 5000), (700, 512, 3000)])
+def test_backward_captured_on_its_own(native, shape):
+    """A graph with the backward alone may be replayed more than once after one forward."""
+    x, w, y = make(*shape)
+    want = run(x, w, y)
+    xs, ws = x.detach().clone().requires_grad_(True), w.detach().clone().requires_grad_(True)
+    up = torch.ones((), device=x.device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = linear_cross_entropy(xs, ws, y)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        grads = torch.autograd.grad(loss, (xs, ws), up)
+    for scale in (1.0, 0.5, 1.0):
+        up.fill_(scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, g in zip(grads, want[1:]):
+            assert torch.equal(got, g * scale)       # (a power of two)
+
+
+def test_forward_and_backward_captured_apart(native):
+    x, w, y = make(300, 256, 5000)
+    want = run(x, w, y)
+    xs, ws = x.detach().clone().requires_grad_(True), w.detach().clone().requires_grad_(True)
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    with torch.cuda.graph(first, stream=side):
+        loss = linear_cross_entropy(xs, ws, y)
+    with torch.cuda.graph(second, pool=first.pool(), stream=side):
+        grads = torch.autograd.grad(loss, (xs, ws))
+    for graph in (first, second, second, first, first, second):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(loss, want[0]) and torch.equal(grads[0], want[1]) and torch.equal(grads[1], want[2])
+
+
 def test_two_streams_at_once(native):
     """Both calls want every SM: neither may wait for the other's blocks."""
     xs = [make(1500, 512, 20000, seed=s) for s in (1, 2)]
