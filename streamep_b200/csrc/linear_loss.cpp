@@ -187,7 +187,10 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   LossMaps m{};
   m.x_k = make_tmap(x.data_ptr(), H, T, 1, pitch(x), pitch(x) * T, 64, p.tile_tokens / 2);
   m.w_k = make_tmap(w.data_ptr(), H, V, 1, pitch(w), pitch(w) * V, 64, 128);
-  if (static_cast<int64_t>(p.row_units) * ceil_of(V, kLossUnit) > ctx.sms / 2) {      // (else every pair has one unit at most)
+  // Units of the narrow form are dealt out in turn, since each warp keeps one statistic of all that it gets: claimed by whoever is free
+  // first, a repeated call would add in another order and not give the same bits.  (Of the others each unit has its own part; and with
+  // a unit a pair there is nothing to claim.)
+  if (!p.narrow && static_cast<int64_t>(p.row_units) * ceil_of(V, kLossUnit) > ctx.sms / 2) {
     p.claim = reinterpret_cast<int*>(base + counters);
     SEP_CUDA_CHECK(cudaMemsetAsync(p.claim, 0, sizeof(int), ctx.stream));
   }

@@ -136,6 +136,21 @@ def test_a_repeated_call_gives_the_same_bits(native, T):
         assert torch.equal(linear_cross_entropy(x, w, y), a[0])
 
 
+@pytest.mark.parametrize("T", [1, 33, 300, 1000])
+def test_repeated_calls_of_many_units_give_the_same_bits(native, T):
+    """Several units for every pair of CTAs, whichever is free first."""
+    x, w, y = make(T, 264, 60001)
+    load = torch.empty(64 << 20, device=DEV)
+    a = run(x, w, y, reduction="none", upstream=torch.ones(T, device=DEV))
+    for i in range(8):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):            # other work beside it, begun at other times
+            for _ in range(i):
+                load.add_(1.0)
+        b = run(x, w, y, reduction="none", upstream=torch.ones(T, device=DEV))
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
 @pytest.mark.parametrize("T", [48, 500])
 def test_one_gradient_only_and_twice(native, T):
     x, w, y = make(T, 256, 3000)
