@@ -13,7 +13,7 @@
 // of not keeping the logits); below a few hundred tokens the reads of W and the writes of dW.
 //
 // Two forms.  The tensor cores multiply 256 rows at a time however few of them exist, so with the tokens as rows a call of 300 pays for 512
-// and one of 1 for 256.  The narrow form makes the vocabulary (for dx: the hidden dimension) the rows, and 32 to 256 tokens the columns of
+// and one of 1 for 256.  The narrow form makes the vocabulary (for dx: the hidden dimension) the rows, and 32 to 192 tokens the columns of
 // a unit, which cost what they are; its epilogues turn 32 x 32 pieces around in shared memory, so that a thread has a token again.
 //
 // Order and progress.  Units are claimed one after another from a counter, by CTAs that run, so a unit that waits for others
@@ -38,8 +38,8 @@ constexpr int kQueue = 4;
 // The narrow forward needs one tile a warp, keeps each warp's statistics of all its units beside it (a part for every 32 columns made the
 // joining kernel longer than the product: 100 tokens, V 100003 92 -> 108 us), and has as many stages as its few tokens leave room for.
 constexpr int kNarrowStages = 9, kNarrowRing = 5 * kStageBytes;
-constexpr int kNarrowUnits = 4;                  // token tiles of the narrow form, at most
-constexpr int kNarrowStats = kNarrowUnits * 4 * 32 * 8;   // bytes a warp: [token tile][its 32-token pieces][lane] (maximum, sum)
+constexpr int kNarrowUnits = 3, kNarrowTiles = 3;   // units of tokens of the narrow form, and a warp's 32-token pieces of one, at most
+constexpr int kNarrowStats = kNarrowUnits * kNarrowTiles * 32 * 8;   // bytes a warp: [unit][its 32-token pieces][lane] (maximum, sum)
 constexpr int stages_of(bool fwd, bool narrow) { return narrow ? kNarrowStages : fwd ? 7 : 5; }
 constexpr int ring_bytes(bool fwd, bool narrow) { return narrow ? kNarrowRing : stages_of(fwd, narrow) * kStageBytes; }
 constexpr int smem_bytes(bool fwd, bool narrow) { return ring_bytes(fwd, narrow) + (fwd ? (narrow ? kEpiWarps * (4096 + kNarrowStats) : 0) : kEpiWarps * kStagingBytes) + 1024; }
@@ -455,9 +455,9 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
     const uint32_t turn = smem_u32(stage_tile);                    // narrow: where pieces are turned around ...
     unsigned char* const narrow_out = stage_tile + 4096;           // ... and where dz waits for its stores
     int flip = 0;
-    float2* const stats = reinterpret_cast<float2*>(staging + kEpiWarps * 4096 + (warp - 2) * kNarrowStats) + lane;    // (forward) [unit row * 4 + piece] * 32
+    float2* const stats = reinterpret_cast<float2*>(staging + kEpiWarps * 4096 + (warp - 2) * kNarrowStats) + lane;    // (forward) [unit row * kNarrowTiles + piece] * 32
     if (FWD && NARROW)
-      for (int i = 0; i < kNarrowUnits * 4; ++i) stats[i * 32] = make_float2(__int_as_float(0xff800000), 0.f);
+      for (int i = 0; i < kNarrowUnits * kNarrowTiles; ++i) stats[i * 32] = make_float2(__int_as_float(0xff800000), 0.f);
     float scale = 1.f;                   // of dw
     if (!FWD && p.scale != nullptr) scale = *p.scale;
     if (!FWD && p.scale2 != nullptr) scale *= *p.scale2;
@@ -520,14 +520,14 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         }
       };
       if (FWD && NARROW) {
-        float z[128];
+        float z[kNarrowTiles * 32];
 #pragma unroll
-        for (int i = 0; i < 128; ++i) z[i] = 0.f;
+        for (int i = 0; i < kNarrowTiles * 32; ++i) z[i] = 0.f;
         for (int first = 0; first < u.k_blocks; first += kSegmentBlocks) {
           if (!(ok = accumulated())) break;
           if (count32 == 0) give_back();
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
+          for (int c = 0; c < 2 * kNarrowTiles; ++c) {
             if (c < 2 * count32) {
               uint32_t part[16];
               tmem_ld_32x16(lanes + acc * kLossUnit + c * 16, part); tmem_ld_wait();
@@ -543,7 +543,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
         const float ninf = __int_as_float(0xff800000);
         const bool exists = v_first + lane < p.V;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kNarrowTiles; ++c) {
           if (c < count32) {
             const int t = u.m * p.tile_tokens + (first32 + c) * 32 + lane;
             const long long y = t < p.T ? p.targets[t] : -1;
@@ -551,7 +551,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
 #pragma unroll
             for (int i = 0; i < 32; ++i) turn_write(turn, lane, i, exists ? z[c * 32 + i] : ninf);
             __syncwarp();
-            float2& so_far = stats[(u.m * 4 + c) * 32];
+            float2& so_far = stats[(u.m * kNarrowTiles + c) * 32];
             const float2 before = so_far;
             float v[32], most[4] = {before.x, ninf, ninf, ninf}, s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -833,7 +833,7 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
       for (int m = 0; m < p.row_units; ++m)
         for (int c = 0; c < count32; ++c) {
           const int t = m * p.tile_tokens + (first32 + c) * 32 + lane;
-          if (t < p.T) p.parts[static_cast<size_t>(blockIdx.x * 4 + quarter) * p.T + t] = stats[(m * 4 + c) * 32];
+          if (t < p.T) p.parts[static_cast<size_t>(blockIdx.x * 4 + quarter) * p.T + t] = stats[(m * kNarrowTiles + c) * 32];
         }
     }
     if (lane == 0) bulk_wait_all();

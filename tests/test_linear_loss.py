@@ -53,7 +53,8 @@ def run(x, w, y, upstream=None, **kw):
 
 SIZES = [(1, 8, 1), (1, 64, 2), (1, 256, 1000), (3, 72, 129), (64, 256, 1000), (127, 128, 255), (128, 200, 2049), (129, 64, 300), (255, 520, 513),
          (257, 1000, 5000), (300, 2048, 10007), (1000, 136, 33000), (2049, 264, 2500), (700, 7168, 1500), (33, 640, 4000), (65, 320, 777), (224, 96, 3001), (225, 96, 3001),
-         (448, 512, 1025), (449, 512, 1025), (640, 192, 70000), (1024, 64, 131073), (1025, 72, 2000)]
+         (448, 512, 1025), (449, 512, 1025), (640, 192, 70000), (1024, 64, 131073), (1025, 72, 2000),
+         (192, 72, 30001), (193, 264, 2000), (384, 520, 1500), (385, 96, 3001), (530, 200, 40000), (576, 136, 2049), (577, 72, 2000)]
 
 
 @pytest.mark.parametrize("T,H,V", SIZES)
