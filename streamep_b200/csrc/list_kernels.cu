@@ -180,11 +180,20 @@ __global__ void __launch_bounds__(kListThreads) list_scale_kernel(const __grid_c
   }
 }
 
+struct Corrections { float step_size, inv_sqrt; };
+__device__ __forceinline__ Corrections corrections_of(const AdamParams& p) {
+  if (p.step == nullptr) return {p.step_size, p.inv_sqrt_correction};
+  // 1 - beta^step = -expm1(step log beta): the exponent is rounded once, so the result keeps its digits however near 1 beta is
+  const double t = static_cast<double>(*p.step);
+  const float c1 = -expm1f(static_cast<float>(t * p.log_beta1)), c2 = -expm1f(static_cast<float>(t * p.log_beta2));
+  return {p.lr / c1, 1.f / sqrtf(c2)};
+}
+
 struct Adam { float m, v, w; };
-__device__ __forceinline__ Adam adam(const AdamParams& p, float g, float m, float v, float w) {
+__device__ __forceinline__ Adam adam(const AdamParams& p, const Corrections& c, float g, float m, float v, float w) {
   m = fmaf(p.beta1, m, p.one_minus_beta1 * g);
   v = fmaf(p.beta2, v, p.one_minus_beta2 * g * g);
-  w = w * p.keep - p.step_size * m / (sqrtf(v) * p.inv_sqrt_correction + p.eps);
+  w = w * p.keep - c.step_size * m / (sqrtf(v) * c.inv_sqrt + p.eps);
   return {m, v, w};
 }
 __device__ __forceinline__ float4 load_four(const void* base, long long i, bool half) {
@@ -206,6 +215,7 @@ __global__ void __launch_bounds__(kListThreads, 2) list_adamw_kernel(const __gri
     if (p.skip_nonfinite && !isfinite(norm)) return;
     if (p.max_norm >= 0.f) f = clip_factor(norm, p.max_norm);
   }
+  const Corrections corrections = corrections_of(p);
   // from the end of the list: what the norm read last is still in L2
   for (long long last = list.chunks - static_cast<long long>(blockIdx.x) * list.window; last > 0; last -= static_cast<long long>(gridDim.x) * list.window) {
     const Run run = {static_cast<int>(max(last - list.window, 0ll)), static_cast<int>(last)};
@@ -228,7 +238,7 @@ __global__ void __launch_bounds__(kListThreads, 2) list_adamw_kernel(const __gri
       float* v = list.exp_avg_sq[e];
       float* master = list.master[e];
       auto one = [&](long long i) {
-        const Adam a = adam(p, load_one(grad, i, grad_half) * f, m[i], v[i], master != nullptr ? master[i] : load_one(param, i, half));
+        const Adam a = adam(p, corrections, load_one(grad, i, grad_half) * f, m[i], v[i], master != nullptr ? master[i] : load_one(param, i, half));
         m[i] = a.m; v[i] = a.v;
         if (master != nullptr) master[i] = a.w;
         store_one(param, i, half, a.w);
@@ -244,7 +254,8 @@ __global__ void __launch_bounds__(kListThreads, 2) list_adamw_kernel(const __gri
       const long long step = 4 * kListThreads;
       long long i = head + 4 * threadIdx.x;
       auto four = [&](long long at, float4 g, float4 a, float4 b, float4 w) {
-        const Adam r0 = adam(p, g.x * f, a.x, b.x, w.x), r1 = adam(p, g.y * f, a.y, b.y, w.y), r2 = adam(p, g.z * f, a.z, b.z, w.z), r3 = adam(p, g.w * f, a.w, b.w, w.w);
+        const Adam r0 = adam(p, corrections, g.x * f, a.x, b.x, w.x), r1 = adam(p, corrections, g.y * f, a.y, b.y, w.y),
+                   r2 = adam(p, corrections, g.z * f, a.z, b.z, w.z), r3 = adam(p, corrections, g.w * f, a.w, b.w, w.w);
         *reinterpret_cast<float4*>(m + at) = make_float4(r0.m, r1.m, r2.m, r3.m);
         *reinterpret_cast<float4*>(v + at) = make_float4(r0.v, r1.v, r2.v, r3.v);
         const float4 w4 = make_float4(r0.w, r1.w, r2.w, r3.w);

@@ -49,6 +49,9 @@ cudaError_t launch_list_scale(const NormList& list, const double* sums, int num_
 struct AdamParams {
   float step_size;               // lr / (1 - beta1^step)
   float inv_sqrt_correction;     // 1 / sqrt(1 - beta2^step)
+  const long long* step;         // optional: the step is this number on the device, and the two above are formed from it and these:
+  float lr;
+  double log_beta1, log_beta2;
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, keep;   // keep = 1 - lr * weight_decay
   const float* norm;             // optional: the gradients' norm, and clipping by it (max_norm < 0: none)
   float max_norm;

@@ -211,13 +211,16 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
   const size_t n = params.size();
   SEP_ASSERT(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && (masters.empty() || masters.size() == n),
              "params, grads, exp_avgs, exp_avg_sqs and masters must be lists of one length");
-  SEP_ASSERT(o.step >= 1, "step counts from 1");
+  SEP_ASSERT(o.device_step.has_value() || o.step >= 1, "step counts from 1");
   SEP_ASSERT(o.lr >= 0.0 && o.eps >= 0.0 && o.weight_decay >= 0.0 && o.beta1 >= 0.0 && o.beta1 < 1.0 && o.beta2 >= 0.0 && o.beta2 < 1.0,
              "lr, eps and weight_decay must not be negative, betas within [0, 1)");
   if (n == 0) return;
   const at::Device device = device_of(params);
   if (norm.has_value())
     SEP_ASSERT(norm->device() == device && norm->scalar_type() == at::kFloat && norm->numel() == 1, "norm must be one float32 number on the parameters' device");
+  if (o.device_step.has_value())
+    SEP_ASSERT(o.device_step->device() == device && o.device_step->scalar_type() == at::kLong && o.device_step->numel() == 1,
+               "a step that is a tensor must be one int64 number on the parameters' device");
   const c10::cuda::CUDAGuard guard(device);
   const bool have_masters = !masters.empty();
   std::deque<at::Tensor> held;                       // gradients that had to be laid out like their parameters
@@ -252,9 +255,15 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
   for (Ranges::List& r : ranges) written.add(std::move(r));
   written.check();
   AdamParams a{};
-  const double c1 = 1.0 - std::pow(o.beta1, static_cast<double>(o.step)), c2 = 1.0 - std::pow(o.beta2, static_cast<double>(o.step));
-  a.step_size = static_cast<float>(o.lr / c1);
-  a.inv_sqrt_correction = static_cast<float>(1.0 / std::sqrt(c2));
+  if (o.device_step.has_value()) {
+    a.step = reinterpret_cast<const long long*>(o.device_step->data_ptr<int64_t>());
+    a.lr = static_cast<float>(o.lr);
+    a.log_beta1 = std::log(o.beta1); a.log_beta2 = std::log(o.beta2);
+  } else {
+    const double c1 = 1.0 - std::pow(o.beta1, static_cast<double>(o.step)), c2 = 1.0 - std::pow(o.beta2, static_cast<double>(o.step));
+    a.step_size = static_cast<float>(o.lr / c1);
+    a.inv_sqrt_correction = static_cast<float>(1.0 / std::sqrt(c2));
+  }
   a.beta1 = static_cast<float>(o.beta1); a.one_minus_beta1 = static_cast<float>(1.0 - o.beta1);
   a.beta2 = static_cast<float>(o.beta2); a.one_minus_beta2 = static_cast<float>(1.0 - o.beta2);
   a.eps = static_cast<float>(o.eps); a.keep = static_cast<float>(1.0 - o.lr * o.weight_decay);

@@ -2258,9 +2258,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("list_clip", [tensors](const py::list& l, double max_norm) { return list_clip(tensors(l), max_norm); });
   m.def("list_scale", [tensors](const py::list& l, const at::Tensor& norm, double max_norm) { list_scale(tensors(l), norm, max_norm); });
   m.def("list_adamw", [tensors](const py::list& params, const py::list& grads, const py::list& exp_avgs, const py::list& exp_avg_sqs, const py::list& masters,
-                                const std::optional<at::Tensor>& norm, int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
-                                double max_norm, bool skip_nonfinite) {
+                                const std::optional<at::Tensor>& norm, int64_t step, const std::optional<at::Tensor>& device_step, double lr, double beta1,
+                                double beta2, double eps, double weight_decay, double max_norm, bool skip_nonfinite) {
     list_adamw(tensors(params), tensors(grads), tensors(exp_avgs), tensors(exp_avg_sqs), tensors(masters), norm,
-               AdamOptions{step, lr, beta1, beta2, eps, weight_decay, max_norm, skip_nonfinite});
+               AdamOptions{step, device_step, lr, beta1, beta2, eps, weight_decay, max_norm, skip_nonfinite});
   });
 }

@@ -40,6 +40,7 @@ at::Tensor list_clip(const TensorList& tensors, double max_norm);
 void list_scale(const TensorList& tensors, const at::Tensor& norm, double max_norm);
 struct AdamOptions {
   int64_t step;
+  std::optional<at::Tensor> device_step;           // instead of `step`: one int64 on the device
   double lr, beta1, beta2, eps, weight_decay;
   double max_norm;               // < 0: no clipping
   bool skip_nonfinite;

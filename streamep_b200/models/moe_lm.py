@@ -6,6 +6,7 @@ projection and the loss, ``grad_norm`` over replicated and expert weights, ``ada
 """
 from __future__ import annotations
 
+import math
 from typing import List, Optional
 
 import torch
@@ -66,7 +67,7 @@ class ExpertAdamW:
         self.masters = [p.detach().float() for p in self.params]
         self.exp_avgs = [torch.zeros_like(m) for m in self.masters]
         self.exp_avg_sqs = [torch.zeros_like(m) for m in self.masters]
-        self.steps = 0
+        self.steps = torch.zeros((), dtype=torch.int64, device=self.masters[0].device if self.masters else None)     # updates made: a skipped one is none
 
     def zero_grad(self) -> None:
         for p in self.params:
@@ -88,7 +89,7 @@ class ExpertAdamW:
         grads = [self.params[i].grad for i in live]
         sharded = [self.params[i].grad for i in live if i >= len(self.replicated)] if ranks > 1 else []
         norm = grad_norm(grads[:len(grads) - len(sharded)], sharded=sharded, group=self.group)
-        self.steps += 1
+        self.steps += norm < math.inf if self.skip_nonfinite else 1
         adamw_step_([self.params[i] for i in live], grads, [self.exp_avgs[i] for i in live], [self.exp_avg_sqs[i] for i in live],
                     masters=[self.masters[i] for i in live], step=self.steps, lr=self.lr, betas=self.betas, eps=self.eps,
                     weight_decay=self.weight_decay, norm=norm, max_norm=self.max_norm, skip_nonfinite=self.skip_nonfinite)
@@ -99,7 +100,7 @@ class ExpertAdamW:
 
     @torch.no_grad()
     def load_state_dict(self, state: dict) -> None:
-        self.steps = int(state["steps"])
+        self.steps.copy_(torch.as_tensor(state["steps"]))
         for name in ("masters", "exp_avgs", "exp_avg_sqs"):
             for mine, theirs in zip(getattr(self, name), state[name], strict=True):
                 mine.copy_(theirs)

@@ -4,7 +4,7 @@ No counterpart in the reference, which ends at the MoE layer.
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -54,7 +54,7 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, *, sharded: 
 
 
 def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
-                exp_avg_sqs: Sequence[torch.Tensor], *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.999),
+                exp_avg_sqs: Sequence[torch.Tensor], *, step: Union[int, torch.Tensor], lr: float, betas: Tuple[float, float] = (0.9, 0.999),
                 eps: float = 1e-8, weight_decay: float = 0.0, masters: Optional[Sequence[torch.Tensor]] = None,
                 norm: Optional[torch.Tensor] = None, max_norm: Optional[float] = None, skip_nonfinite: bool = False) -> None:
     """One AdamW step (decoupled weight decay) on all of ``params`` in place, in one launch per 512 tensors::
@@ -64,9 +64,13 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
         w = w * (1 - lr * weight_decay) - lr * (exp_avg / (1 - b1**step)) / (sqrt(exp_avg_sq / (1 - b2**step)) + eps)
 
     Parameters and gradients are bf16 or float32, the moments float32, all arithmetic 32 bits.  With ``masters``
-    (float32) ``w`` is the master copy and the parameter becomes its rounding.  ``step`` counts from 1;
-    like ``lr`` it is a number of the host, which a captured graph repeats.
-    ``skip_nonfinite``: leave everything as it is when ``norm`` is not finite, decided on the device."""
+    (float32) ``w`` is the master copy and the parameter becomes its rounding.
+
+    ``step``, the number of this update, counts from 1.  Like ``lr`` it may be a number of the host, which a captured graph
+    repeats; or one int64 number on the parameters' device, read when the update runs (below 1 the weights become NaN).
+    ``skip_nonfinite``: leave everything as it is when ``norm`` is not finite, decided on the device.  An update that was
+    skipped must not be counted: ``steps += norm < math.inf`` before the call, and ``step=steps``, does that without reading
+    the norm on the host."""
     if max_norm is not None and norm is None:
         raise ValueError("max_norm needs the gradients' norm (grad_norm)")
     if max_norm is not None and not max_norm >= 0:
@@ -75,6 +79,7 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
         raise ValueError("skip_nonfinite needs the gradients' norm (grad_norm)")
     if masters is not None and len(masters) != len(params):
         raise ValueError(f"{len(params)} params and {len(masters)} masters")
+    device_step = step if isinstance(step, torch.Tensor) else None
     _ext.load().list_adamw(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), list(masters) if masters is not None else [], norm,
-                           int(step), float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
+                           0 if device_step is not None else int(step), device_step, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
                            -1.0 if max_norm is None else float(max_norm), bool(skip_nonfinite))
