@@ -64,7 +64,7 @@ class ExpertAdamW:
         self.params = self.replicated + self.experts
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
         self.max_norm, self.skip_nonfinite = max_norm, skip_nonfinite
-        self.masters = [p.detach().float() for p in self.params]
+        self.masters = [p.detach().to(torch.float32, copy=True) for p in self.params]      # (of float32 parameters too: both are written)
         self.exp_avgs = [torch.zeros_like(m) for m in self.masters]
         self.exp_avg_sqs = [torch.zeros_like(m) for m in self.masters]
         self.steps = torch.zeros((), dtype=torch.int64, device=self.masters[0].device if self.masters else None)     # updates made: a skipped one is none

@@ -1,0 +1,67 @@
+"""ExpertAdamW on the host: what it keeps and what it hands on, with the native calls replaced by their definitions on the CPU."""
+import pytest
+import torch
+
+from streamep_b200 import _ext
+from streamep_b200.models import ExpertAdamW
+
+
+class Native:
+    """The native calls by their definitions, in 64 bits."""
+
+    @staticmethod
+    def list_norm(ts):
+        s = sum((t.double().square().sum() for t in ts), torch.zeros((), dtype=torch.float64))
+        return s.sqrt().float(), s
+
+    @staticmethod
+    def list_adamw(params, grads, exp_avgs, exp_avg_sqs, masters, norm, step, device_step, lr, beta1, beta2, eps, decay, max_norm, skip):
+        places = [t.data_ptr() for l in (params, exp_avgs, exp_avg_sqs, masters) for t in l if t.numel()]
+        if len(set(places)) != len(places):
+            raise ValueError("two tensors that are written in place share memory")
+        t = int(device_step) if device_step is not None else step
+        f = min(1.0, max_norm / (float(norm) + 1e-6)) if max_norm >= 0 else 1.0
+        if skip and not torch.isfinite(norm):
+            return
+        for p, g, m, v, w in zip(params, grads, exp_avgs, exp_avg_sqs, masters):
+            g = g.double() * f
+            m.copy_(beta1 * m.double() + (1 - beta1) * g)
+            v.copy_(beta2 * v.double() + (1 - beta2) * g * g)
+            w.copy_(w.double() * (1 - lr * decay) - lr * (m.double() / (1 - beta1 ** t)) / ((v.double() / (1 - beta2 ** t)).sqrt() + eps))
+            p.copy_(w)
+
+
+@pytest.fixture(autouse=True)
+def on_the_cpu(monkeypatch):
+    monkeypatch.setattr(_ext, "load", lambda: Native)
+
+
+def torch_twin(opt):
+    twin = [m.clone().requires_grad_(True) for m in opt.masters]
+    return twin, torch.optim.AdamW(twin, lr=opt.lr, betas=opt.betas, eps=opt.eps, weight_decay=opt.weight_decay)
+
+
+def follow(opt, twin, ref, grads):
+    """One step of both; a gradient of None is none."""
+    for p, t, g in zip(opt.params, twin, grads):
+        p.grad = None if g is None else g.to(p.dtype)
+        t.grad = None if g is None else g.to(p.dtype).to(torch.float32, copy=True)
+    if opt.max_norm is not None:
+        torch.nn.utils.clip_grad_norm_([t for t in twin if t.grad is not None], opt.max_norm)
+    ref.step()
+    opt.step()
+    for got, want in zip(opt.masters, twin):       # 32-bit arithmetic of the reference: a few 1e-7 of the value, and of a step
+        torch.testing.assert_close(got, want.detach(), rtol=1e-6, atol=1e-5 * opt.lr)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_masters_are_copies(dtype):
+    """Parameters of the masters' own type as well: both are written in a step."""
+    params = [torch.randn(50).to(dtype).requires_grad_(True), torch.randn(7).bfloat16().requires_grad_(True)]
+    opt = ExpertAdamW(params[:1], params[1:], lr=1e-2)
+    assert all(m.dtype == torch.float32 and m.data_ptr() != p.data_ptr() for m, p in zip(opt.masters, params))
+    twin, ref = torch_twin(opt)
+    for _ in range(3):
+        follow(opt, twin, ref, [torch.randn(50), torch.randn(7)])
+    for p, m in zip(params, opt.masters):
+        assert torch.equal(p.detach(), m.to(p.dtype))
