@@ -67,7 +67,10 @@ class ExpertAdamW:
         self.masters = [p.detach().to(torch.float32, copy=True) for p in self.params]      # (of float32 parameters too: both are written)
         self.exp_avgs = [torch.zeros_like(m) for m in self.masters]
         self.exp_avg_sqs = [torch.zeros_like(m) for m in self.masters]
-        self.steps = torch.zeros((), dtype=torch.int64, device=self.masters[0].device if self.masters else None)     # updates made: a skipped one is none
+        # updates made, of each parameter: a skipped one is none, nor one without a gradient.  Parameters that have taken part in the same
+        # updates share one number, and an update.
+        start = torch.zeros((), dtype=torch.int64, device=self.masters[0].device if self.masters else None)
+        self.steps = [start] * len(self.params)
 
     def zero_grad(self) -> None:
         for p in self.params:
@@ -75,7 +78,8 @@ class ExpertAdamW:
 
     @torch.no_grad()
     def step(self) -> torch.Tensor:
-        """Returns the norm (0-dim, on the device).  Parameters without a gradient are left out."""
+        """Returns the norm (0-dim, on the device).  Parameters without a gradient are left out: their moments and their count of
+        updates stay."""
         ranks = self.group.size() if self.group is not None else 1
         if ranks > 1:
             # a mean over the ranks' tokens: experts already hold the sum of what all ranks sent them
@@ -89,18 +93,39 @@ class ExpertAdamW:
         grads = [self.params[i].grad for i in live]
         sharded = [self.params[i].grad for i in live if i >= len(self.replicated)] if ranks > 1 else []
         norm = grad_norm(grads[:len(grads) - len(sharded)], sharded=sharded, group=self.group)
-        self.steps += norm < math.inf if self.skip_nonfinite else 1
-        adamw_step_([self.params[i] for i in live], grads, [self.exp_avgs[i] for i in live], [self.exp_avg_sqs[i] for i in live],
-                    masters=[self.masters[i] for i in live], step=self.steps, lr=self.lr, betas=self.betas, eps=self.eps,
-                    weight_decay=self.weight_decay, norm=norm, max_norm=self.max_norm, skip_nonfinite=self.skip_nonfinite)
+        made = norm < math.inf if self.skip_nonfinite else 1
+        for together in self._same_steps(live):
+            step = self.steps[together[0]]
+            step += made
+            pick = lambda tensors: [tensors[i] for i in together]
+            adamw_step_(pick(self.params), [self.params[i].grad for i in together], pick(self.exp_avgs), pick(self.exp_avg_sqs),
+                        masters=pick(self.masters), step=step, lr=self.lr, betas=self.betas, eps=self.eps,
+                        weight_decay=self.weight_decay, norm=norm, max_norm=self.max_norm, skip_nonfinite=self.skip_nonfinite)
         return norm
 
+    def _same_steps(self, live: List[int]) -> List[List[int]]:
+        """``live`` by their counts; one that others hold as well, who are not in ``live``, is copied first."""
+        groups = {}
+        for i in live:
+            groups.setdefault(id(self.steps[i]), []).append(i)
+        if len(live) < len(self.params):
+            left = {id(self.steps[i]) for i in set(range(len(self.params))).difference(live)}
+            for key, members in groups.items():
+                if key in left:
+                    own = self.steps[members[0]].clone()
+                    for i in members:
+                        self.steps[i] = own
+        return list(groups.values())
+
     def state_dict(self) -> dict:
-        return {"steps": self.steps, "masters": self.masters, "exp_avgs": self.exp_avgs, "exp_avg_sqs": self.exp_avg_sqs}
+        steps = torch.stack(self.steps) if self.steps else torch.zeros(0, dtype=torch.int64)
+        return {"steps": steps, "masters": self.masters, "exp_avgs": self.exp_avgs, "exp_avg_sqs": self.exp_avg_sqs}
 
     @torch.no_grad()
     def load_state_dict(self, state: dict) -> None:
-        self.steps.copy_(torch.as_tensor(state["steps"]))
+        numbers = torch.as_tensor(state["steps"]).expand(len(self.params)).tolist()        # (one for all of them will do)
+        shared = {n: torch.tensor(n, dtype=torch.int64, device=self.masters[0].device) for n in set(numbers)}
+        self.steps = [shared[n] for n in numbers]
         for name in ("masters", "exp_avgs", "exp_avg_sqs"):
             for mine, theirs in zip(getattr(self, name), state[name], strict=True):
                 mine.copy_(theirs)

@@ -65,3 +65,27 @@ def test_masters_are_copies(dtype):
         follow(opt, twin, ref, [torch.randn(50), torch.randn(7)])
     for p, m in zip(params, opt.masters):
         assert torch.equal(p.detach(), m.to(p.dtype))
+
+
+def test_parameters_that_join_late_or_pause():
+    """Each parameter's corrections go by its own updates, as the reference optimizer has it."""
+    torch.manual_seed(0)
+    params = [torch.randn(n).bfloat16().requires_grad_(True) for n in (50, 7, 30)]
+    opt = ExpertAdamW(params[:1], params[1:], lr=1e-2)
+    twin, ref = torch_twin(opt)
+    for mask in ((1, 1, 0), (1, 1, 0), (1, 1, 1), (1, 0, 1), (0, 1, 0), (0, 0, 0), (1, 1, 1)):
+        if any(mask):
+            follow(opt, twin, ref, [torch.randn(p.shape) if m else None for p, m in zip(params, mask)])
+        else:
+            opt.zero_grad()
+            assert float(opt.step()) == 0.0
+    assert opt.state_dict()["steps"].tolist() == [5, 5, 3] and len({id(s) for s in opt.steps}) <= 3
+    other = ExpertAdamW([params[0].detach().clone().requires_grad_(True)], [p.detach().clone().requires_grad_(True) for p in params[1:]], lr=1e-2)
+    other.load_state_dict(opt.state_dict())
+    for a, b in zip(params, other.params):
+        a.grad = b.grad = torch.ones_like(b)
+    opt.step()
+    other.step()
+    assert all(torch.equal(a, b) for a, b in zip(opt.masters, other.masters))
+    other.load_state_dict({**opt.state_dict(), "steps": 4})                         # one number for all
+    assert other.state_dict()["steps"].tolist() == [4, 4, 4]
