@@ -55,8 +55,10 @@ class MoELM(nn.Module):
 
 class ExpertAdamW:
     """AdamW with float32 master copies for a model whose expert weights are sharded over ``group`` and whose other
-    weights are replicated.  ``step()`` averages the replicated gradients over the group, takes the norm over everything
-    (each expert counted once), clips and updates: one pass over the gradients for the norm, one over all state."""
+    weights are replicated.  ``step()`` takes the norm over everything (each expert counted once), clips and updates: one pass
+    over the gradients for the norm, one over all state.  With several ranks it first averages the replicated gradients over
+    the group and divides the experts' by its size, in place: an all-reduce and a division a tensor, one more pass over the
+    gradients.  The all-reduces are collective: a replicated parameter has a gradient on every rank or on none."""
 
     def __init__(self, replicated, experts, *, lr: float, betas=(0.9, 0.95), eps: float = 1e-8, weight_decay: float = 0.1,
                  max_norm: Optional[float] = 1.0, skip_nonfinite: bool = True, group=None):

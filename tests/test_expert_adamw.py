@@ -1,6 +1,11 @@
 """ExpertAdamW on the host: what it keeps and what it hands on, with the native calls replaced by their definitions on the CPU."""
+import os
+import tempfile
+
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from streamep_b200 import _ext
 from streamep_b200.models import ExpertAdamW
@@ -89,3 +94,56 @@ def test_parameters_that_join_late_or_pause():
     assert all(torch.equal(a, b) for a, b in zip(opt.masters, other.masters))
     other.load_state_dict({**opt.state_dict(), "steps": 4})                         # one number for all
     assert other.state_dict()["steps"].tolist() == [4, 4, 4]
+
+
+def _rank(rank, world, store, out):
+    dist.init_process_group("gloo", init_method=f"file://{store}", rank=rank, world_size=world)
+    _ext.load = lambda: Native
+    shared, mine = weights(rank)
+    opt = ExpertAdamW(shared, mine, lr=1e-2, max_norm=1.0, group=dist.group.WORLD)
+    norms = []
+    for step in range(3):
+        for p, g in zip(shared + mine, gradients(rank, step)):
+            p.grad = None if g is None else g.clone()
+        norms.append(float(opt.step()))
+    torch.save((norms, opt.masters, opt.state_dict()["steps"]), f"{out}.{rank}")
+    dist.destroy_process_group()
+
+
+def weights(rank):
+    g = torch.Generator().manual_seed(1)
+    shared = [torch.randn(n, generator=g).requires_grad_(True) for n in (40, 3)]
+    g = torch.Generator().manual_seed(10 + rank)
+    return shared, [torch.randn(n, generator=g).requires_grad_(True) for n in (20, 11)]
+
+
+def gradients(rank, step):
+    """The second replicated parameter is without one in the middle step, rank 1's last expert in all."""
+    g = torch.Generator().manual_seed(100 * step + rank)
+    a, b, c, d = (torch.randn(n, generator=g) for n in (40, 3, 20, 11))
+    return a, None if step == 1 else b, c, None if rank == 1 else d
+
+
+def test_step_over_a_group():
+    """Two ranks against one process with all experts: replicated gradients are means, the experts' the sum over all tokens divided by the ranks."""
+    world = 2
+    with tempfile.TemporaryDirectory() as d:
+        out = os.path.join(d, "out")
+        mp.spawn(_rank, args=(world, os.path.join(d, "store"), out), nprocs=world)
+        got = [torch.load(f"{out}.{r}") for r in range(world)]
+    shared = weights(0)[0]
+    params = shared + weights(0)[1] + weights(1)[1]
+    masters = [p.detach().clone().requires_grad_(True) for p in params]
+    ref = torch.optim.AdamW(masters, lr=1e-2, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
+    for step in range(3):
+        a, b = gradients(0, step), gradients(1, step)
+        grads = [None if x is None else (x + y) / 2 for x, y in zip(a[:2], b[:2])] + [None if x is None else x / 2 for x in a[2:] + b[2:]]
+        for m, g in zip(masters, grads):
+            m.grad = g
+        norm = float(torch.nn.utils.clip_grad_norm_([m for m in masters if m.grad is not None], 1.0))
+        ref.step()
+        assert all(abs(norms[step] - norm) <= 1e-5 * norm for norms, _, _ in got)
+    for rank, (_, mine, steps) in enumerate(got):
+        assert steps.tolist() == [3, 2, 3, 0 if rank == 1 else 3]
+        for m, want in zip(mine, masters[:2] + masters[2 + 2 * rank:4 + 2 * rank]):
+            torch.testing.assert_close(m, want.detach(), rtol=1e-6, atol=1e-5 * 1e-2)
