@@ -21,7 +21,11 @@ def _total(grads, sharded, group):
     C = _ext.load()
     if not _over_ranks(group):
         return C.list_norm(grads + sharded)[0]
-    squares, parts = C.list_norm(grads)[1], C.list_norm(sharded)[1]
+    # (an empty list beside one with tensors: on their device, whichever is current)
+    squares = C.list_norm(grads)[1] if grads or not sharded else None
+    parts = C.list_norm(sharded)[1] if sharded or not grads else torch.zeros_like(squares)
+    if squares is None:
+        squares = torch.zeros_like(parts)
     torch.distributed.all_reduce(parts, group=group)
     return (squares + parts).sqrt().float()
 
