@@ -19,30 +19,47 @@ from typing import Optional, Sequence
 import torch
 
 from .. import _ext
+from ..errors import StreamEPError, StreamEPTimeout
 
 VARLEN_M, VARLEN_K = 0, 1
 EPI_STORE, EPI_SWIGLU, EPI_SCATTER, EPI_DSWIGLU = 0, 1, 2, 3
 KIND_GEMM_Y_TAIL, KIND_GEMM_A_BWD_TAIL = 5, 6
 GATE_KERNEL_Y, GATE_KERNEL_A_BWD = 2, 3
 
-_default_runtime = None
+_default_runtimes = {}           # by device index
 
 
-def default_runtime():
-    """A private single-rank runtime for callers that have no ``Buffer`` (kernel
-    tests, micro-benchmarks): it owns the status block and the launch-gate flags
+def default_runtime(device: Optional[torch.device] = None):
+    """A private single-rank runtime of ``device`` (the current one by default) for callers that have no ``Buffer`` (kernel
+    tests, micro-benchmarks, the loss): it owns the status block and the launch-gate flags
     the kernels report into."""
-    global _default_runtime
-    if _default_runtime is None:
+    index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
+    if index not in _default_runtimes:
         C = _ext.load()
-        _default_runtime = C.Runtime(0, 1, 64 << 20, 4, C.MAX_EXPERTS, 2000)
-        _default_runtime.sync_local([_default_runtime.get_local_base_ptr()])
-    return _default_runtime
+        with torch.cuda.device(index):
+            runtime = C.Runtime(0, 1, 64 << 20, 4, C.MAX_EXPERTS, 2000)
+            runtime.sync_local([runtime.get_local_base_ptr()])
+        _default_runtimes[index] = runtime
+    return _default_runtimes[index]
 
 
-def _rt(buffer):
+def check_status(device: Optional[torch.device] = None) -> None:
+    """:meth:`Buffer.check_status` for the calls on ``device`` (the current one by default) that were given no buffer:
+    synchronises it and raises :class:`StreamEPTimeout` if any bounded device wait gave up since the last check,
+    :class:`StreamEPError` if a loss got a target outside its vocabulary."""
+    device = torch.device(device) if device is not None else None
+    index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
+    if index not in _default_runtimes:
+        return
+    with torch.cuda.device(index):
+        msg = _default_runtimes[index].poll_status(True)
+    if msg:
+        raise (StreamEPError if "outside the vocabulary" in msg else StreamEPTimeout)(msg)
+
+
+def _rt(buffer, device: Optional[torch.device] = None):
     if buffer is None:
-        return default_runtime()
+        return default_runtime(device)
     return buffer.runtime if hasattr(buffer, "runtime") else buffer
 
 

@@ -25,7 +25,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     ``targets [...]`` int64; tokens whose target is ``ignore_index`` have no loss, count for nothing in the mean and
     get zero gradients.  ``reduction``: ``"mean"`` over the counted tokens (NaN without any, gradients zero),
     ``"sum"``, or ``"none"`` for a loss per token (float32, shaped like ``targets``).  A target outside the
-    vocabulary makes the loss and the gradients NaN and is reported by ``buffer.check_status()``.
+    vocabulary makes the loss and the gradients NaN and is reported, like a wait on the device that gave up, by
+    ``buffer.check_status()``, or without ``buffer`` by ``streamep_b200.ops.check_status()``.
 
     Under ``torch.no_grad()`` only the forward runs: ``-linear_cross_entropy(..., reduction="none")`` are the
     log-probabilities of given tokens, for one token as for a batch.  There is no second derivative.
@@ -34,6 +35,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)} (got {reduction!r})")
     if x.dim() < 1 or x.shape[:-1] != targets.shape:
         raise ValueError(f"targets must have the shape of x without its last dimension (x {tuple(x.shape)}, targets {tuple(targets.shape)})")
-    loss = _rt(buffer).linear_loss(x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x, weight, targets.reshape(-1),
-                                   int(ignore_index), _REDUCTIONS[reduction])
+    if not x.is_cuda:
+        raise ValueError(f"x must be a [..., H] bf16 CUDA tensor (got one on {x.device})")
+    loss = _rt(buffer, x.device).linear_loss(x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x, weight, targets.reshape(-1),
+                                             int(ignore_index), _REDUCTIONS[reduction])
     return loss.view(targets.shape) if reduction == "none" else loss
