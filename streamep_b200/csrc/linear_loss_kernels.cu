@@ -32,7 +32,16 @@ constexpr int kOperandBytes = 128 * kBK * 2;     // A or B of one CTA: 128 rows 
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps + 1) * 32;   // 0 TMA producer, 1 MMA, 2..9 epilogue, 10 scheduler
-constexpr int kStagingBytes = 2 * 4096;          // per epilogue warp of the backward: two tiles of 32 rows of 128 bytes
+constexpr int kTileBytes = 4096;                 // 32 rows of 128 bytes
+constexpr int kStagingBytes = 2 * kTileBytes;    // per epilogue warp of the backward: two of them
+// Of the two tiles that begin at `own` the one that is not at `tile`, wherever shared memory places them.
+__host__ __device__ constexpr uint32_t other_tile(uint32_t own, uint32_t tile) { return own + kTileBytes - (tile - own); }
+constexpr bool tiles_take_turns() {
+  for (uint32_t own = 0; own < 4 * kStagingBytes; own += 1024)
+    if (other_tile(own, own) != own + kTileBytes || other_tile(own, own + kTileBytes) != own) return false;
+  return true;
+}
+static_assert(tiles_take_turns(), "a warp's two staging tiles take turns at every alignment of shared memory");
 constexpr int kQueue = 4;
 // The forward's epilogue stores nothing but statistics, so all shared memory is its operand ring's.
 // The narrow forward needs one tile a warp, keeps each warp's statistics of all its units beside it (a part for every 32 columns made the
@@ -441,9 +450,10 @@ linear_loss_kernel(const __grid_constant__ LossParams p, const __grid_constant__
     // warps 2..5 the left 128 columns of the tile and warps 6..9 the right ones.  Warps do not wait for one another.
     const int quarter = warp & 3, side = (warp - 2) >> 2;
     // A tile of results is written to shared memory and leaves by a bulk store, while the warp fills the other one.
-    unsigned char* stage_tile = staging + (warp - 2) * (FWD ? 4096 : kStagingBytes);
+    const uint32_t own_tiles = (warp - 2) * (FWD ? kTileBytes : kStagingBytes);          // from `staging` on
+    unsigned char* stage_tile = staging + own_tiles;
     auto next_tile = [&] {               // whole warp: the tile that the store before the last one has read
-      stage_tile = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(stage_tile) ^ 4096);
+      stage_tile = staging + other_tile(own_tiles, static_cast<uint32_t>(stage_tile - staging));
       if (lane == 0) bulk_wait_read_but_one();
       __syncwarp();
       return smem_u32(stage_tile);
