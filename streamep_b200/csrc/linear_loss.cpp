@@ -42,11 +42,11 @@ void plan_tiles(LossParams& p, bool backward) {
   p.dw_rows = T <= 32 ? 32 : 64;
   loss_narrow_ring(p, backward);
 }
-void plan_backward(LossParams& p, int sms) {
+void plan_backward(LossParams& p, int sms, int64_t piece_bytes) {
   const int64_t T = p.T, H = p.H, V = p.V, pairs = sms / 2;
   p.h_units = static_cast<int>(ceil_of(H, kLossUnit));
   const int64_t row_bytes = T * 2 * (p.split2 ? 2 : 1);
-  const int64_t want = ceil_of(V * row_bytes, kPieceBytes);
+  const int64_t want = ceil_of(V * row_bytes, piece_bytes);
   p.piece = static_cast<int>(ceil_of(ceil_of(V, want), kLossUnit) * kLossUnit);
   p.pieces = static_cast<int>(ceil_of(V, p.piece));
   p.last_cols = static_cast<int>(V - static_cast<int64_t>(p.pieces - 1) * p.piece);
@@ -113,6 +113,7 @@ struct LossCall : torch::CustomClassHolder {
   ContextFn context;
   int64_t ignore_index;
   int reduction;
+  int64_t piece_bytes;
   bool want_dx = false, want_dw = false;
   // The forward's kernel clears the backward's counters, for one backward after it.  A backward clears them itself when another has run
   // (retain_graph), and when the two are not of one captured graph (or of none): one may be replayed without the other.
@@ -132,12 +133,12 @@ unsigned long long capture_of(cudaStream_t stream) {
 // which the forward's kernel clears.
 struct Forward { at::Tensor loss, stats; };
 
-LossParams plan(int64_t T, int64_t H, int64_t V, bool want_dx, bool want_dw, int sms) {
+LossParams plan(int64_t T, int64_t H, int64_t V, bool want_dx, bool want_dw, int sms, int64_t piece_bytes) {
   LossParams p{};
   p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.V = static_cast<int>(V);
   p.want_dx = want_dx; p.want_dw = want_dw;
   plan_tiles(p, true);
-  plan_backward(p, sms);
+  plan_backward(p, sms, piece_bytes);
   plan_band(p);
   p.claim_lead = claim_lead(p, true);
   return p;
@@ -175,7 +176,7 @@ Forward loss_forward(LossCall& call, const at::Tensor& x, const at::Tensor& w, c
   p.zero = ticket; p.zero_ints = 1;
   if (call.want_dx || call.want_dw) {
     // the ticket stands behind the backward's counters, to be cleared with them
-    const int64_t ints = counter_ints(plan(T, H, V, call.want_dx, call.want_dw, ctx.sms));
+    const int64_t ints = counter_ints(plan(T, H, V, call.want_dx, call.want_dw, ctx.sms, call.piece_bytes));
     out.stats = at::empty({counters_at(T) + ints + 1}, f32);
     call.capture = capture_of(ctx.stream);
     p.zero = reinterpret_cast<int*>(out.stats.data_ptr<float>() + counters_at(T));
@@ -225,7 +226,7 @@ std::pair<at::Tensor, at::Tensor> loss_backward(LossCall& call, const at::Tensor
   const LaunchContext ctx = call.context(1);
   const at::Tensor up = upstream.to(at::kFloat).contiguous();
 
-  LossParams p = plan(T, H, V, want_dx, want_dw, ctx.sms);
+  LossParams p = plan(T, H, V, want_dx, want_dw, ctx.sms, call.piece_bytes);
   SEP_ASSERT(loss_backward_units(p) < (1ll << 30), "this loss has too many tiles for one call: split the tokens");
   const int64_t z_layers = p.split2 ? 2 : 1, slots = p.splits;
   Carver c;
@@ -299,7 +300,7 @@ class LinearLoss : public torch::autograd::Function<LinearLoss> {
 }  // namespace
 
 at::Tensor linear_loss(const ContextFn& context, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets,
-                       int64_t ignore_index, int reduction) {
+                       int64_t ignore_index, int reduction, int64_t piece_bytes) {
   SEP_ASSERT(x.is_cuda() && x.dim() == 2 && x.scalar_type() == at::kBFloat16, "x must be a [..., H] bf16 CUDA tensor");
   SEP_ASSERT(weight.dim() == 2 && weight.scalar_type() == at::kBFloat16 && weight.device() == x.device() && weight.size(1) == x.size(1),
              "weight must be a [V, H] bf16 tensor on the device of x");
@@ -311,12 +312,14 @@ at::Tensor linear_loss(const ContextFn& context, const at::Tensor& x, const at::
                  ceil_of(x.size(0), kLossUnit) * ceil_of(weight.size(0), kLossUnit) < (1ll << 30),
              "this loss has too many tiles for one call: split the tokens");
   SEP_ASSERT(reduction >= kLossNone && reduction <= kLossSum, "unknown reduction");
+  SEP_ASSERT(piece_bytes >= 0, "piece_bytes must not be negative");
   SEP_ASSERT(!x._fw_grad(0).defined() && !weight._fw_grad(0).defined(), "linear_cross_entropy has no forward-mode derivative");
   const c10::cuda::CUDAGuard guard(x.device());
   auto call = c10::make_intrusive<LossCall>();
   call->context = context;
   call->ignore_index = ignore_index;
   call->reduction = reduction;
+  call->piece_bytes = piece_bytes > 0 ? piece_bytes : kPieceBytes;
   SEP_ASSERT(context(0).device == x.get_device(), "x is not on the device of the buffer that this call reports into");
   if (!(at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad())))
     return loss_forward(*call, readable(x), readable(weight), targets.contiguous()).loss;
@@ -325,8 +328,8 @@ at::Tensor linear_loss(const ContextFn& context, const at::Tensor& x, const at::
   return LinearLoss::apply(x, weight, targets, call);
 }
 
-std::vector<std::vector<int>> linear_loss_schedule(int64_t tokens, int64_t hidden, int64_t vocab, int sms, bool want_dx, bool want_dw) {
-  const LossParams p = plan(tokens, hidden, vocab, want_dx, want_dw, sms);
+std::vector<std::vector<int>> linear_loss_schedule(int64_t tokens, int64_t hidden, int64_t vocab, int sms, bool want_dx, bool want_dw, int64_t piece_bytes) {
+  const LossParams p = plan(tokens, hidden, vocab, want_dx, want_dw, sms, piece_bytes > 0 ? piece_bytes : kPieceBytes);
   std::vector<std::vector<int>> out = {{p.pieces, p.piece, p.splits, p.ahead, p.buffers, p.row_units, p.split2, p.dw_group}};
   const long long units = loss_backward_units(p);
   for (long long i = 0; i < units; ++i) {

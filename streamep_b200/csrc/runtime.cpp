@@ -2239,10 +2239,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("pool_expand", &Runtime::pool_expand)
       .def("router", &Runtime::router)
       .def("linear_loss", [](const std::shared_ptr<Runtime>& r, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets,
-                             int64_t ignore_index, int reduction) {
-        return linear_loss([r](int launches) { return r->launch_context(launches); }, x, weight, targets, ignore_index, reduction);
-      });
-  m.def("linear_loss_schedule", &linear_loss_schedule);
+                             int64_t ignore_index, int reduction, int64_t piece_bytes) {
+        return linear_loss([r](int launches) { return r->launch_context(launches); }, x, weight, targets, ignore_index, reduction, piece_bytes);
+      }, py::arg("x"), py::arg("weight"), py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"), py::arg("piece_bytes") = 0);
+  m.def("linear_loss_schedule", &linear_loss_schedule, py::arg("tokens"), py::arg("hidden"), py::arg("vocab"), py::arg("sms"), py::arg("want_dx"),
+        py::arg("want_dw"), py::arg("piece_bytes") = 0);
   // Lists come as Python lists and their tensors are read in place: the generic conversion to a vector of tensors costs more than the
   // launch from a hundred tensors up (four lists of 250: 86 -> 41 us a call).
   auto tensors = [](const py::list& l) {

@@ -25,12 +25,14 @@ struct LaunchContext {
 using ContextFn = std::function<LaunchContext(int launches)>;   // `launches`: how many kernels the caller is about to launch
 
 enum LossReduction : int { kLossNone = 0, kLossMean = 1, kLossSum = 2 };
-// x [T, H], weight [V, H] bf16, targets [T] int64; differentiable in x and weight
+// x [T, H], weight [V, H] bf16, targets [T] int64; differentiable in x and weight.  `piece_bytes`: what a piece of the backward may take (0: the
+// plan's own limit; tests give less, so that small calls have many pieces)
 at::Tensor linear_loss(const ContextFn& context, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets,
-                       int64_t ignore_index, int reduction);
+                       int64_t ignore_index, int reduction, int64_t piece_bytes);
 // The backward's units in order, for the schedule's test: each {kind, piece, unit row, unit column, split, first k-block, k-blocks};
 // first of all {pieces, columns of a piece, splits, ahead, buffers, row units, split2, column tiles of a dw unit}.
-std::vector<std::vector<int>> linear_loss_schedule(int64_t tokens, int64_t hidden, int64_t vocab, int sms, bool want_dx, bool want_dw);
+std::vector<std::vector<int>> linear_loss_schedule(int64_t tokens, int64_t hidden, int64_t vocab, int sms, bool want_dx, bool want_dw,
+                                                   int64_t piece_bytes);
 
 // Tensors that the caller (a Python list) keeps alive during the call.
 using TensorList = std::vector<const at::Tensor*>;
