@@ -21,13 +21,15 @@ int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int64_t kPieceBytes = 256ll << 20;
 constexpr int64_t kSplitTokens = 64;             // calls whose dz is kept as a sum of two bf16 numbers: one k-block of tokens
 constexpr int64_t kDirectBlocks = 32;            // k-blocks of dx that are not worth splitting
-constexpr int64_t kNarrowTokens = 768;           // (four token tiles would have to have more than three quarters of 256)
+constexpr int64_t kNarrowTokens = 576;           // three token tiles of 192, three quarters of 256
 constexpr int64_t kBandBytes = 48ll << 20;       // rows of x that a band of units shares in L2
 
 // Tokens as columns (the narrow form) where that multiplies at least a quarter less; always where dz is split.  Hidden 2048, V 100003, with rows
 // and with columns, forward alone: 96 tokens 103 and 90 us, 160 107 and 102, 192 109 and 107, 224 111 and 113, 300 175 and 166, 384 178 and
 // 177, 448 183 and 188; with gradients 418 and 382, 467 and 440, 474 and 460, 492 and 494, 702 and 669, 739 and 725, 779 and 777.
-// Hidden 512 and 300 tokens, forward: 31 and 35.  1 token, hidden 4096, V 128000, forward: 248 and 172.
+// 513 243 and 238, with gradients 994 and 968, 576 246 and 240, 1016 and 978.  576 tokens, hidden 4096, V 32000: 167 and 165, with gradients 661 and
+// 643.  Short reductions lose, forward alone: hidden 512 and 300 tokens 31 and 35, 576 (V 50257) 44.1 and 46.4, with gradients 181 and 186.
+// 1 token, hidden 4096, V 128000, forward: 248 and 172.
 void plan_tiles(LossParams& p, bool backward) {
   const int64_t T = p.T, units = ceil_of(T, kLossUnit), tokens = ceil_of(ceil_of(T, units), 32) * 32;
   p.narrow = T <= kSplitTokens || (T <= kNarrowTokens && tokens * 4 <= 3 * kLossUnit);

@@ -42,7 +42,8 @@ def grad_norm(grads: Sequence[torch.Tensor], *, sharded: Sequence[torch.Tensor] 
 
 def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, *, sharded: Sequence[torch.Tensor] = (), group=None) -> torch.Tensor:
     """Scales all gradients in place by ``min(1, max_norm / (norm + 1e-6))`` and returns their norm before that (see
-    :func:`grad_norm`).  Below the limit the gradients are read once and not written.  A norm of NaN makes all
+    :func:`grad_norm`).  Below the limit the gradients are read once and not written (those with gaps in memory, which go through
+    copies, are written back as they were).  A norm of NaN makes all
     gradients NaN, an infinite one makes them 0 (and NaN where they are infinite), as ``torch.nn.utils`` has it.
     Tensors that share memory are refused (strided views, which go through copies, are not compared), and so are expanded ones.
 
