@@ -2255,6 +2255,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     }
     return out;
   };
+  m.def("norm_rows", &norm_rows);
   m.def("list_norm", [tensors](const py::list& l) { return list_norm(tensors(l)); });
   m.def("list_clip", [tensors](const py::list& l, double max_norm) { return list_clip(tensors(l), max_norm); });
   m.def("list_scale", [tensors](const py::list& l, const at::Tensor& norm, double max_norm) { list_scale(tensors(l), norm, max_norm); });

@@ -1,5 +1,5 @@
-// Operators of a training step around the MoE layer, host side: the loss over the vocabulary (linear_loss.cpp), and lists
-// of tensors (list_ops.cpp): gradients' norm and clipping, AdamW.
+// Operators of a training step around the MoE layer, host side: the loss over the vocabulary (linear_loss.cpp), lists
+// of tensors (list_ops.cpp): gradients' norm and clipping, AdamW; and normalisation (norm.cpp).
 #pragma once
 
 #include <functional>
@@ -49,5 +49,9 @@ struct AdamOptions {
 };
 void list_adamw(const TensorList& params, const TensorList& grads, const TensorList& exp_avgs, const TensorList& exp_avg_sqs,
                 const TensorList& masters, const std::optional<at::Tensor>& norm, const AdamOptions& o);
+
+// Rows normalised, after adding `residual` where there is one: {y} or {y, sum}; differentiable in all tensors.  `center`: subtract the mean.
+std::vector<at::Tensor> norm_rows(const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias,
+                                  const std::optional<at::Tensor>& residual, bool center, double eps);
 
 }  // namespace sep
