@@ -21,7 +21,7 @@ from typing import Any, List, Optional, Sequence, Tuple
 import torch
 
 from . import _ext
-from .errors import StreamEPError, StreamEPOverflow, StreamEPTimeout
+from .errors import StreamEPError, StreamEPOverflow, StreamEPTimeout, reports_bad_input
 
 topk_idx_t = torch.int64
 
@@ -286,12 +286,12 @@ class Buffer:
         """Synchronise the device and raise :class:`StreamEPTimeout` if any bounded
         device wait gave up since the last check (:class:`StreamEPOverflow` if a
         capacity-mode dispatch did not fit its region, :class:`StreamEPError` if a loss
-        got a target outside its vocabulary).  The context stays usable."""
+        got a target outside its vocabulary or a recurrence offsets that are none).  The context stays usable."""
         msg = self.runtime.poll_status(True)
         if msg:
             if "capacity overflow" in msg:
                 raise StreamEPOverflow(f"rank {self.rank}: {msg}; {self._overflow_text()}")
-            if "outside the vocabulary" in msg:
+            if reports_bad_input(msg):
                 raise StreamEPError(f"rank {self.rank}: {msg}")
             raise StreamEPTimeout(f"rank {self.rank}: {msg}")
 
@@ -774,7 +774,7 @@ class LocalWorld:
         if msgs:
             if all("capacity overflow" in m for m in msgs):
                 raise StreamEPOverflow("; ".join(msgs))
-            if all("outside the vocabulary" in m for m in msgs):
+            if all(reports_bad_input(m) for m in msgs):
                 raise StreamEPError("; ".join(msgs))
             raise StreamEPTimeout("; ".join(msgs))
 

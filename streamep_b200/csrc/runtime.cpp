@@ -734,9 +734,10 @@ class Runtime : public std::enable_shared_from_this<Runtime> {
                                   "token gate timeout", "GEMM pipeline timeout", "tail wait timeout", "bad index",
                                   "capacity overflow (where = region, expected = tile capacity, observed = tiles needed; the dispatch was run as an empty one)",
                                   "ranks disagree on the capacity-mode region of a dispatch",
-                                  "target outside the vocabulary (where = token, expected = vocabulary, observed = target; its loss and the gradients are NaN)"};
+                                  "target outside the vocabulary (where = token, expected = vocabulary, observed = target; its loss and the gradients are NaN)",
+                                  "offsets of packed sequences decrease or point outside (where = sequence, expected and observed = its two offsets; it is undefined)"};
     std::ostringstream os;
-    os << names[(h.code >= 0 && h.code < 11) ? h.code : 0] << " (code " << h.code << ") in kernel " << h.kernel_id
+    os << names[(h.code >= 0 && h.code < 12) ? h.code : 0] << " (code " << h.code << ") in kernel " << h.kernel_id
        << " role " << h.role << " on rank " << h.rank << ": where=" << h.where << " expected=" << h.expected
        << " observed=" << h.observed;
     return os.str();
@@ -2241,7 +2242,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("linear_loss", [](const std::shared_ptr<Runtime>& r, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets,
                              int64_t ignore_index, int reduction, int64_t piece_bytes) {
         return linear_loss([r](int launches) { return r->launch_context(launches); }, x, weight, targets, ignore_index, reduction, piece_bytes);
-      }, py::arg("x"), py::arg("weight"), py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"), py::arg("piece_bytes") = 0);
+      }, py::arg("x"), py::arg("weight"), py::arg("targets"), py::arg("ignore_index"), py::arg("reduction"), py::arg("piece_bytes") = 0)
+      .def("gated_scan", [](const std::shared_ptr<Runtime>& r, const at::Tensor& x, const at::Tensor& gate, const std::optional<at::Tensor>& initial,
+                            const std::optional<at::Tensor>& offsets, bool want_state) {
+        return gated_scan([r](int launches) { return r->launch_context(launches); }, x, gate, initial, offsets, want_state);
+      });
   m.def("linear_loss_schedule", &linear_loss_schedule, py::arg("tokens"), py::arg("hidden"), py::arg("vocab"), py::arg("sms"), py::arg("want_dx"),
         py::arg("want_dw"), py::arg("piece_bytes") = 0);
   // Lists come as Python lists and their tensors are read in place: the generic conversion to a vector of tensors costs more than the
@@ -2256,6 +2261,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return out;
   };
   m.def("norm_rows", &norm_rows);
+  m.def("gated_scan_step", &gated_scan_step);
   m.def("list_norm", [tensors](const py::list& l) { return list_norm(tensors(l)); });
   m.def("list_clip", [tensors](const py::list& l, double max_norm) { return list_clip(tensors(l), max_norm); });
   m.def("list_scale", [tensors](const py::list& l, const at::Tensor& norm, double max_norm) { list_scale(tensors(l), norm, max_norm); });

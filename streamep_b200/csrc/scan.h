@@ -1,0 +1,51 @@
+// Gated linear recurrence: launches of scan_kernels.cu.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "status.h"
+
+namespace sep {
+
+struct ScanShape {
+  int half;                      // 1: x, gate, h and their gradients are bf16, 0: fp32
+  int rows, channels;            // of all sequences together
+  int sequences;
+  int length;                    // rows of each sequence, where `offsets` is null
+  const void* offsets;           // [sequences + 1] first rows of packed sequences, or null
+  int offsets_wide;              // 1: int64, 0: int32
+  long long x_stride, gate_stride;
+  const void* x;
+  const void* gate;
+  const float* initial;          // [sequences, channels] or null (zeros)
+  StatusBlock* status;
+  int rank;
+  unsigned long long wait_budget_ns;
+};
+struct ScanParams : ScanShape {
+  void* h;                       // [rows, channels]
+  float* final_state;            // [sequences, channels] or null
+};
+struct ScanGradParams : ScanShape {
+  const void* h;
+  const void* dh;                // rows `dh_stride` apart; null: zeros
+  long long dh_stride;
+  const float* dfinal;           // or null
+  void* dx;                      // or null
+  void* dgate;                   // or null
+  float* dinitial;               // or null
+};
+cudaError_t launch_scan_forward(const ScanParams& p, int sms, cudaStream_t stream);
+cudaError_t launch_scan_backward(const ScanGradParams& p, int sms, cudaStream_t stream);
+
+struct ScanStepParams {
+  int half, rows, channels;
+  long long x_stride, gate_stride, state_stride;
+  const void* x;
+  const void* gate;
+  float* state;
+  void* h;                       // [rows, channels]
+};
+cudaError_t launch_scan_step(const ScanStepParams& p, int sms, cudaStream_t stream);
+
+}  // namespace sep

@@ -18,6 +18,7 @@ enum StatusCode : int {
   kStatusOverflow = 8,             // capacity mode: a rank's pool layout does not fit the fixed regions
   kStatusRegionMismatch = 9,       // capacity mode: the ranks did not pick the same region for this dispatch
   kStatusBadTarget = 10,           // linear_cross_entropy: a target outside the vocabulary (where = token)
+  kStatusBadOffsets = 11,          // gated_scan: offsets that decrease or point outside (where = sequence)
 };
 
 struct StatusBlock {
@@ -33,7 +34,7 @@ struct StatusBlock {
 
 enum KernelId : int {
   kKernelMetadata = 1, kKernelFill = 2, kKernelDispatch = 3, kKernelDispatchGrads = 4,
-  kKernelCombine = 5, kKernelGemm = 6, kKernelBarrier = 7, kKernelProducer = 8, kKernelLoss = 9,
+  kKernelCombine = 5, kKernelGemm = 6, kKernelBarrier = 7, kKernelProducer = 8, kKernelLoss = 9, kKernelScan = 10,
 };
 
 }  // namespace sep

@@ -1,5 +1,6 @@
 // Operators of a training step around the MoE layer, host side: the loss over the vocabulary (linear_loss.cpp), lists
-// of tensors (list_ops.cpp): gradients' norm and clipping, AdamW; and normalisation (norm.cpp).
+// of tensors (list_ops.cpp): gradients' norm and clipping, AdamW; normalisation (norm.cpp); and a gated
+// linear recurrence (scan.cpp).
 #pragma once
 
 #include <functional>
@@ -53,5 +54,11 @@ void list_adamw(const TensorList& params, const TensorList& grads, const TensorL
 // Rows normalised, after adding `residual` where there is one: {y} or {y, sum}; differentiable in all tensors.  `center`: subtract the mean.
 std::vector<at::Tensor> norm_rows(const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias,
                                   const std::optional<at::Tensor>& residual, bool center, double eps);
+
+// h (and the final state) of h_t = sigmoid(gate_t) h_{t-1} + (1 - sigmoid(gate_t)) x_t, for x [B, T, D], or [N, D] cut at `offsets`; differentiable
+// in x, gate and initial.
+std::vector<at::Tensor> gated_scan(const ContextFn& context, const at::Tensor& x, const at::Tensor& gate, const std::optional<at::Tensor>& initial,
+                                   const std::optional<at::Tensor>& offsets, bool want_state);
+at::Tensor gated_scan_step(const at::Tensor& state, const at::Tensor& x, const at::Tensor& gate);
 
 }  // namespace sep

@@ -12,6 +12,11 @@ class StreamEPTimeout(StreamEPError):
     csrc/kernels/utils.cuh:643-646)."""
 
 
+def reports_bad_input(message: str) -> bool:
+    """Whether a status message is about what a call was given (a loss's target, a recurrence's offsets) and not about a wait."""
+    return "outside the vocabulary" in message or "offsets of packed sequences" in message
+
+
 class StreamEPOverflow(StreamEPError):
     """A capacity-mode dispatch needed more pool tiles or recv tokens than the fixed regions hold on some rank.
     Every rank ran that dispatch as an empty one (outputs and gradients of that layer are zero); the step is

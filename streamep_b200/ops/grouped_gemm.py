@@ -19,7 +19,7 @@ from typing import Optional, Sequence
 import torch
 
 from .. import _ext
-from ..errors import StreamEPError, StreamEPTimeout
+from ..errors import StreamEPError, StreamEPTimeout, reports_bad_input
 
 VARLEN_M, VARLEN_K = 0, 1
 EPI_STORE, EPI_SWIGLU, EPI_SCATTER, EPI_DSWIGLU = 0, 1, 2, 3
@@ -46,7 +46,8 @@ def default_runtime(device: Optional[torch.device] = None):
 def check_status(device: Optional[torch.device] = None) -> None:
     """:meth:`Buffer.check_status` for the calls on ``device`` (the current one by default) that were given no buffer:
     synchronises it and raises :class:`StreamEPTimeout` if any bounded device wait gave up since the last check,
-    :class:`StreamEPError` if a loss got a target outside its vocabulary."""
+    :class:`StreamEPError` if a loss got a target outside its vocabulary or a recurrence
+    offsets that are none."""
     device = torch.device(device) if device is not None else None
     index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
     if index not in _default_runtimes:
@@ -54,7 +55,7 @@ def check_status(device: Optional[torch.device] = None) -> None:
     with torch.cuda.device(index):
         msg = _default_runtimes[index].poll_status(True)
     if msg:
-        raise (StreamEPError if "outside the vocabulary" in msg else StreamEPTimeout)(msg)
+        raise (StreamEPError if reports_bad_input(msg) else StreamEPTimeout)(msg)
 
 
 def _rt(buffer, device: Optional[torch.device] = None):
