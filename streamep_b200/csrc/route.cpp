@@ -1,0 +1,154 @@
+// Host side of routing that is trained: argument checks, the router's launch with what its losses need, the autograd node.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "api.h"
+#include "host_common.h"
+#include "route.h"
+#include "train_ops.h"
+
+namespace sep {
+
+namespace {
+
+// bf16 rows as the tensor maps read them; a copy where they do not lie so.
+at::Tensor readable(const at::Tensor& t) { return aligned_rows(t.contiguous()); }
+
+struct RouteCall : torch::CustomClassHolder {
+  ContextFn context;
+  int top_k, num_ranks;
+  bool renormalize;
+};
+
+struct Route { at::Tensor idx, weights, in_rank, balance, z, counts, probs, lse, load; };
+
+const unsigned char* mask_of(const at::Tensor& mask) { return mask.defined() ? reinterpret_cast<const unsigned char*>(mask.data_ptr<bool>()) : nullptr; }
+
+Route route_forward(const RouteCall& call, const at::Tensor& x, const at::Tensor& w, const at::Tensor& mask) {
+  const int64_t T = x.size(0), H = x.size(1), E = w.size(0), K = call.top_k;
+  const auto f32 = x.options().dtype(at::kFloat);
+  Route r;
+  r.idx = at::empty({T, K}, x.options().dtype(at::kLong));
+  r.weights = at::empty({T, K}, f32);
+  r.in_rank = at::empty({T, call.num_ranks}, x.options().dtype(at::kBool));
+  r.balance = at::empty({}, f32);
+  r.z = at::empty({}, f32);
+  r.counts = at::empty({E}, x.options().dtype(at::kLong));
+  r.probs = at::empty({T, E}, f32);
+  r.lse = at::empty({T}, f32);
+  r.load = at::empty({E + 1}, f32);
+  const LaunchContext ctx = call.context(T > 0 ? 3 : 1);
+  if (T > 0) {
+    RouterParams p{};
+    p.x = x.data_ptr(); p.w_gate = w.data_ptr();
+    p.num_tokens = static_cast<int>(T); p.hidden = static_cast<int>(H); p.num_experts = static_cast<int>(E); p.num_topk = call.top_k;
+    p.num_ranks = call.num_ranks; p.renormalize = call.renormalize ? 1 : 0;
+    p.topk_idx = reinterpret_cast<long long*>(r.idx.data_ptr<int64_t>());
+    p.topk_weights = r.weights.data_ptr<float>();
+    p.is_token_in_rank = reinterpret_cast<unsigned char*>(r.in_rank.data_ptr<bool>());
+    p.probs = r.probs.data_ptr<float>();
+    p.lse = r.lse.data_ptr<float>();
+    const CUtensorMap mw = make_tmap(w.data_ptr(), H, E, 1, H, E * H, 64, 128);
+    const CUtensorMap mx = make_tmap(x.data_ptr(), H, T, 1, H, T * H, 64, router_tile(p, ctx.sms).tile_tokens);
+    SEP_CUDA_CHECK(launch_router_mma(p, &mw, &mx, ctx.sms, ctx.status, ctx.wait_budget_ns, ctx.stream));
+  }
+  RouteStatsParams s{};
+  s.tokens = static_cast<int>(T); s.experts = static_cast<int>(E); s.top_k = call.top_k;
+  s.probs = r.probs.data_ptr<float>(); s.lse = r.lse.data_ptr<float>();
+  s.idx = reinterpret_cast<const long long*>(r.idx.data_ptr<int64_t>());
+  s.mask = mask_of(mask);
+  s.blocks = route_stats_blocks(s.tokens, ctx.sms);
+  const at::Tensor parts = at::empty({s.blocks * (2 * E + 2) + 1}, f32);
+  s.other_parts = reinterpret_cast<float2*>(parts.data_ptr<float>());
+  s.prob_parts = parts.data_ptr<float>() + 2 * s.blocks;
+  s.count_parts = reinterpret_cast<int*>(s.prob_parts + s.blocks * E);
+  s.balance = r.balance.data_ptr<float>(); s.z = r.z.data_ptr<float>();
+  s.counts = reinterpret_cast<long long*>(r.counts.data_ptr<int64_t>());
+  s.load = r.load.data_ptr<float>();
+  SEP_CUDA_CHECK(launch_route_stats(s, ctx.stream));
+  return r;
+}
+
+class BalancedRoute : public torch::autograd::Function<BalancedRoute> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w_gate,
+                                                const std::optional<at::Tensor>& counted, const c10::intrusive_ptr<RouteCall>& call) {
+    const at::Tensor mask = counted.value_or(at::Tensor());
+    Route r = route_forward(*call, readable(x), readable(w_gate), mask);
+    ctx->save_for_backward({x, w_gate, mask, r.probs, r.lse, r.load, r.idx, r.weights});
+    ctx->saved_data["call"] = c10::IValue::make_capsule(call);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({r.idx, r.in_rank, r.counts});
+    return {r.idx, r.weights, r.in_rank, r.balance, r.z, r.counts};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    SEP_ASSERT(!at::GradMode::is_enabled(), "balanced_router has no second derivative: its backward was asked for a graph");
+    auto call = c10::static_intrusive_pointer_cast<RouteCall>(ctx->saved_data["call"].toCapsule());
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w_gate = saved[1], &mask = saved[2], &probs = saved[3], &lse = saved[4], &load = saved[5], &idx = saved[6], &weights = saved[7];
+    if (!grads[1].defined() && !grads[3].defined() && !grads[4].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
+    const int64_t T = x.size(0), H = x.size(1), E = w_gate.size(0);
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor dx, dw;
+    if (want_dx) dx = at::empty({T, H}, x.options());
+    if (want_dw) dw = T > 0 ? at::empty({E, H}, w_gate.options()) : at::zeros({E, H}, w_gate.options());
+    if (T > 0) {
+      const LaunchContext context = call->context(1 + (want_dx ? 1 : 0) + (want_dw ? 1 : 0));
+      const at::Tensor xr = readable(x), wr = readable(w_gate), dlogits = at::empty({T, E}, probs.options());
+      at::Tensor up[3];
+      for (int i = 0; i < 3; ++i) {
+        const at::Tensor& g = grads[i == 0 ? 1 : i + 2];
+        if (g.defined()) up[i] = g.to(at::kFloat).contiguous();
+      }
+      RouteGradParams p{};
+      p.tokens = static_cast<int>(T); p.experts = static_cast<int>(E); p.top_k = call->top_k; p.hidden = static_cast<int>(H); p.renormalize = call->renormalize;
+      p.probs = probs.data_ptr<float>(); p.lse = lse.data_ptr<float>(); p.load = load.data_ptr<float>();
+      p.idx = reinterpret_cast<const long long*>(idx.data_ptr<int64_t>());
+      p.weights = weights.data_ptr<float>();
+      p.mask = mask_of(mask);
+      p.dweights = up[0].defined() ? up[0].data_ptr<float>() : nullptr;
+      p.dbalance = up[1].defined() ? up[1].data_ptr<float>() : nullptr;
+      p.dz_loss = up[2].defined() ? up[2].data_ptr<float>() : nullptr;
+      p.dlogits = dlogits.data_ptr<float>();
+      p.x = xr.data_ptr(); p.w_gate = wr.data_ptr();
+      p.dx = want_dx ? dx.data_ptr() : nullptr;
+      p.dw = want_dw ? dw.data_ptr() : nullptr;
+      SEP_CUDA_CHECK(launch_route_backward(p, context.stream));
+    }
+    return {dx, dw, at::Tensor(), at::Tensor()};
+  }
+};
+
+}  // namespace
+
+std::vector<at::Tensor> balanced_router(const ContextFn& context, const at::Tensor& x, const at::Tensor& w_gate, int64_t top_k, int64_t num_ranks,
+                                        bool renormalize, const std::optional<at::Tensor>& mask) {
+  auto rows = [](const at::Tensor& t) { return t.is_cuda() && t.layout() == at::kStrided && t.dim() == 2 && t.scalar_type() == at::kBFloat16; };
+  SEP_ASSERT(rows(x), "x must be a [T, H] bf16 CUDA tensor");
+  SEP_ASSERT(rows(w_gate) && w_gate.device() == x.device() && w_gate.size(1) == x.size(1), "w_gate must be an [E, H] bf16 tensor on the device of x");
+  SEP_ASSERT(x.size(1) > 0 && x.size(1) % 8 == 0 && x.size(1) < (1ll << 30), "hidden must be a positive multiple of 8");
+  SEP_ASSERT(x.size(0) < (1ll << 26), "too many tokens for one call");
+  const int64_t E = w_gate.size(0);
+  SEP_ASSERT(E >= 1 && E <= 512, "the router takes 1 to 512 experts");
+  SEP_ASSERT(top_k >= 1 && top_k <= 32 && top_k <= E, "top_k must be between 1 and 32, and no more than there are experts");
+  SEP_ASSERT(num_ranks >= 1 && num_ranks <= 32 && E % num_ranks == 0, "the experts must divide evenly over 1 to 32 ranks");
+  if (mask.has_value())
+    SEP_ASSERT(mask->dim() == 1 && mask->size(0) == x.size(0) && mask->scalar_type() == at::kBool && mask->device() == x.device() && mask->layout() == at::kStrided,
+               "mask must hold one truth value for each token, on the device of x");
+  SEP_ASSERT(!x._fw_grad(0).defined() && !w_gate._fw_grad(0).defined(), "balanced_router has no forward-mode derivative");
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto call = c10::make_intrusive<RouteCall>();
+  call->context = context;
+  call->top_k = static_cast<int>(top_k); call->num_ranks = static_cast<int>(num_ranks);
+  call->renormalize = renormalize;
+  SEP_ASSERT(context(0).device == x.get_device(), "x is not on the device of the buffer that this call reports into");
+  std::optional<at::Tensor> counted;
+  if (mask.has_value()) counted = mask->contiguous();
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w_gate.requires_grad())) return BalancedRoute::apply(x, w_gate, counted, call);
+  const Route r = route_forward(*call, readable(x), readable(w_gate), counted.value_or(at::Tensor()));
+  return {r.idx, r.weights, r.in_rank, r.balance, r.z, r.counts};
+}
+
+}  // namespace sep

@@ -2246,6 +2246,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("gated_scan", [](const std::shared_ptr<Runtime>& r, const at::Tensor& x, const at::Tensor& gate, const std::optional<at::Tensor>& initial,
                             const std::optional<at::Tensor>& offsets, bool want_state) {
         return gated_scan([r](int launches) { return r->launch_context(launches); }, x, gate, initial, offsets, want_state);
+      })
+      .def("balanced_router", [](const std::shared_ptr<Runtime>& r, const at::Tensor& x, const at::Tensor& w_gate, int64_t top_k, int64_t num_ranks,
+                                 bool renormalize, const std::optional<at::Tensor>& mask) {
+        return balanced_router([r](int launches) { return r->launch_context(launches); }, x, w_gate, top_k, num_ranks, renormalize, mask);
       });
   m.def("linear_loss_schedule", &linear_loss_schedule, py::arg("tokens"), py::arg("hidden"), py::arg("vocab"), py::arg("sms"), py::arg("want_dx"),
         py::arg("want_dw"), py::arg("piece_bytes") = 0);

@@ -1,6 +1,6 @@
 // Operators of a training step around the MoE layer, host side: the loss over the vocabulary (linear_loss.cpp), lists
-// of tensors (list_ops.cpp): gradients' norm and clipping, AdamW; normalisation (norm.cpp); and a gated
-// linear recurrence (scan.cpp).
+// of tensors (list_ops.cpp): gradients' norm and clipping, AdamW; normalisation (norm.cpp); a gated
+// linear recurrence (scan.cpp); and routing that is trained (route.cpp).
 #pragma once
 
 #include <functional>
@@ -60,5 +60,9 @@ std::vector<at::Tensor> norm_rows(const at::Tensor& x, const std::optional<at::T
 std::vector<at::Tensor> gated_scan(const ContextFn& context, const at::Tensor& x, const at::Tensor& gate, const std::optional<at::Tensor>& initial,
                                    const std::optional<at::Tensor>& offsets, bool want_state);
 at::Tensor gated_scan_step(const at::Tensor& state, const at::Tensor& x, const at::Tensor& gate);
+
+// {topk_idx, topk_weights, is_token_in_rank, balance loss, z loss, counts} of x [T, H] and w_gate [E, H] bf16; differentiable in both.
+std::vector<at::Tensor> balanced_router(const ContextFn& context, const at::Tensor& x, const at::Tensor& w_gate, int64_t top_k, int64_t num_ranks,
+                                        bool renormalize, const std::optional<at::Tensor>& mask);
 
 }  // namespace sep

@@ -1,7 +1,7 @@
 """Python entry points of the native kernels (lazy: importing the package does not load the extension)."""
 import importlib
 
-_MODULES = ("grouped_gemm", "linear_loss", "tensor_lists", "norm", "recurrence")
+_MODULES = ("grouped_gemm", "linear_loss", "tensor_lists", "norm", "recurrence", "routing")
 
 
 def __getattr__(name):
