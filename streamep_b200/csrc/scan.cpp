@@ -42,6 +42,14 @@ ScanShape shape_of(const at::Tensor& offsets, const at::Tensor& x, const at::Ten
   return p;
 }
 
+template <class Params>
+at::Tensor workspace(const Params& p, const at::Tensor& like) {
+  const ScanPlan plan = scan_plan(p);
+  SEP_ASSERT(static_cast<int64_t>(plan.chunks) * plan.tiles < (1ll << 30), "this recurrence has too many rows and channels for one call");
+  const int64_t bytes = scan_space(plan, p.channels);
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
 ScanResult scan_forward(const ScanCall& call, const at::Tensor& x, const at::Tensor& gate, const at::Tensor& initial, const at::Tensor& offsets,
                         bool want_state) {
   ScanResult out;
@@ -54,7 +62,8 @@ ScanResult scan_forward(const ScanCall& call, const at::Tensor& x, const at::Ten
   if (p.sequences == 0) { out.h.zero_(); return out; }
   p.h = out.h.data_ptr();
   p.final_state = want_state ? out.final_state.data_ptr<float>() : nullptr;
-  SEP_CUDA_CHECK(launch_scan_forward(p, ctx.sms, ctx.stream));
+  const at::Tensor space = workspace(p, x);
+  SEP_CUDA_CHECK(launch_scan_forward(p, space.defined() ? space.data_ptr() : nullptr, ctx.stream));
   return out;
 }
 
@@ -99,7 +108,8 @@ class Scan : public torch::autograd::Function<Scan> {
       p.dx = want_dx ? dx.data_ptr() : nullptr;
       p.dgate = want_dgate ? dgate.data_ptr() : nullptr;
       p.dinitial = want_dinitial ? dinitial.data_ptr<float>() : nullptr;
-      SEP_CUDA_CHECK(launch_scan_backward(p, context.sms, context.stream));
+      const at::Tensor space = workspace(p, x);
+      SEP_CUDA_CHECK(launch_scan_backward(p, space.defined() ? space.data_ptr() : nullptr, context.stream));
     }
     return {dx, dgate, dinitial, at::Tensor(), at::Tensor(), at::Tensor()};
   }

@@ -35,8 +35,13 @@ struct ScanGradParams : ScanShape {
   void* dgate;                   // or null
   float* dinitial;               // or null
 };
-cudaError_t launch_scan_forward(const ScanParams& p, int sms, cudaStream_t stream);
-cudaError_t launch_scan_backward(const ScanGradParams& p, int sms, cudaStream_t stream);
+// Chunks of rows and tiles of channels, and the bytes (from a 16-byte boundary) that blocks hand on to one another in.
+struct ScanPlan { int chunks, tiles; };
+ScanPlan scan_plan(const ScanParams& p);
+ScanPlan scan_plan(const ScanGradParams& p);
+long long scan_space(const ScanPlan& s, int channels);
+cudaError_t launch_scan_forward(const ScanParams& p, void* space, cudaStream_t stream);
+cudaError_t launch_scan_backward(const ScanGradParams& p, void* space, cudaStream_t stream);
 
 struct ScanStepParams {
   int half, rows, channels;
