@@ -63,7 +63,7 @@ ScanResult scan_forward(const ScanCall& call, const at::Tensor& x, const at::Ten
   p.h = out.h.data_ptr();
   p.final_state = want_state ? out.final_state.data_ptr<float>() : nullptr;
   const at::Tensor space = workspace(p, x);
-  SEP_CUDA_CHECK(launch_scan_forward(p, space.defined() ? space.data_ptr() : nullptr, ctx.stream));
+  SEP_CUDA_CHECK(launch_scan_forward(p, ctx.sms, space.defined() ? space.data_ptr() : nullptr, ctx.stream));
   return out;
 }
 
@@ -109,7 +109,7 @@ class Scan : public torch::autograd::Function<Scan> {
       p.dgate = want_dgate ? dgate.data_ptr() : nullptr;
       p.dinitial = want_dinitial ? dinitial.data_ptr<float>() : nullptr;
       const at::Tensor space = workspace(p, x);
-      SEP_CUDA_CHECK(launch_scan_backward(p, space.defined() ? space.data_ptr() : nullptr, context.stream));
+      SEP_CUDA_CHECK(launch_scan_backward(p, context.sms, space.defined() ? space.data_ptr() : nullptr, context.stream));
     }
     return {dx, dgate, dinitial, at::Tensor(), at::Tensor(), at::Tensor()};
   }

@@ -40,8 +40,8 @@ struct ScanPlan { int chunks, tiles; };
 ScanPlan scan_plan(const ScanParams& p);
 ScanPlan scan_plan(const ScanGradParams& p);
 long long scan_space(const ScanPlan& s, int channels);
-cudaError_t launch_scan_forward(const ScanParams& p, void* space, cudaStream_t stream);
-cudaError_t launch_scan_backward(const ScanGradParams& p, void* space, cudaStream_t stream);
+cudaError_t launch_scan_forward(const ScanParams& p, int sms, void* space, cudaStream_t stream);
+cudaError_t launch_scan_backward(const ScanGradParams& p, int sms, void* space, cudaStream_t stream);
 
 struct ScanStepParams {
   int half, rows, channels;

@@ -4,6 +4,8 @@
 //   g_t = dh_t + keep_{t+1} g_{t+1}:   dx_t = take_t g_t,   dgate_t = g_t keep_t take_t (h_{t-1} - x_t),   dh_{-1} = keep_0 g_0
 //
 // The state, and everything that is added up along a sequence, is fp32.
+#include <atomic>
+
 #include "scan.h"
 #include "ptx.cuh"
 
@@ -31,20 +33,72 @@ template <class T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// sigmoid(gate) and sigmoid(-gate), each to its own last digits: the smaller one is computed and kept, with the sign of the gate; the other is
-// its difference to 1.  For bf16 gates the exponent is rounded once (|gate| 2^-24 of the result), for fp32 ones it is not.
-template <class T> __device__ __forceinline__ float smaller(float g);
-template <> __device__ __forceinline__ float smaller<__nv_bfloat16>(float g) {
-  float e, m;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * 1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(m) : "f"(1.f + e));
-  return copysignf(m, g);
+// Two fp32 numbers that one instruction works on.
+struct Pair { unsigned long long v; };
+__device__ __forceinline__ Pair pair_of(float a, float b) { Pair p; asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b)); return p; }
+__device__ __forceinline__ void parts_of(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) { Pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) { Pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+__device__ __forceinline__ Pair fused(Pair a, Pair b, Pair c) { Pair d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return d; }
+// V numbers of a thread, of one row.  (Sums and products are written out, so that the bits do not depend on what else a call computes.)
+template <int V> struct Row {
+  Pair p[V / 2];
+  __device__ __forceinline__ static Row all(float f) { Row r; for (int i = 0; i < V / 2; ++i) r.p[i] = pair_of(f, f); return r; }
+  __device__ __forceinline__ void put(int i, float a, float b) { p[i] = pair_of(a, b); }
+  __device__ __forceinline__ void get(float (&f)[V]) const { _Pragma("unroll") for (int i = 0; i < V / 2; ++i) parts_of(p[i], f[2 * i], f[2 * i + 1]); }
+  __device__ __forceinline__ static Row of(const float (&f)[V]) { Row r; _Pragma("unroll") for (int i = 0; i < V / 2; ++i) r.p[i] = pair_of(f[2 * i], f[2 * i + 1]); return r; }
+};
+template <> struct Row<1> {
+  float f;
+  __device__ __forceinline__ static Row all(float f) { return Row{f}; }
+  __device__ __forceinline__ void get(float (&o)[1]) const { o[0] = f; }
+  __device__ __forceinline__ static Row of(const float (&o)[1]) { return Row{o[0]}; }
+};
+template <int V> __device__ __forceinline__ Row<V> operator+(Row<V> a, const Row<V>& b) {
+  if constexpr (V == 1) a.f = __fadd_rn(a.f, b.f);
+  else { _Pragma("unroll") for (int i = 0; i < V / 2; ++i) a.p[i] = a.p[i] + b.p[i]; }
+  return a;
 }
-template <> __device__ __forceinline__ float smaller<float>(float g) { return copysignf(__frcp_rn(1.f + expf(fabsf(g))), g); }
-struct Gate { float keep, take; };
-__device__ __forceinline__ Gate gate_of(float s) {
-  const float m = fabsf(s), o = 1.f - m;
-  return signbit(s) ? Gate{m, o} : Gate{o, m};
+template <int V> __device__ __forceinline__ Row<V> operator*(Row<V> a, const Row<V>& b) {
+  if constexpr (V == 1) a.f = __fmul_rn(a.f, b.f);
+  else { _Pragma("unroll") for (int i = 0; i < V / 2; ++i) a.p[i] = a.p[i] * b.p[i]; }
+  return a;
+}
+template <int V> __device__ __forceinline__ Row<V> fused(const Row<V>& a, const Row<V>& b, Row<V> c) {
+  if constexpr (V == 1) c.f = fmaf(a.f, b.f, c.f);
+  else { _Pragma("unroll") for (int i = 0; i < V / 2; ++i) c.p[i] = fused(a.p[i], b.p[i], c.p[i]); }
+  return c;
+}
+
+// sigmoid(gate) and sigmoid(-gate), each to its own last digits: 1 / (1 + e) and e / (1 + e) of e = exp(gate), which is held at 2^126 (a gate of
+// 87; NaN stays).  For bf16 gates the exponent is rounded once (|gate| 2^-24 of the result), for fp32 ones it is not.
+__device__ __forceinline__ float at_most(float v, float top) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(top)); return r; }
+__device__ __forceinline__ float ex2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float reciprocal(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+template <class T, int V>
+__device__ __forceinline__ void gates_of(const Row<V>& gate, Row<V>& keep, Row<V>& take) {
+  float e[V];
+  if constexpr (sizeof(T) == 2) {
+    const Row<V> scaled = gate * Row<V>::all(1.4426950408889634f);
+    scaled.get(e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = ex2(at_most(e[i], 126.f));
+  } else {
+    gate.get(e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = expf(at_most(e[i], 87.f));
+  }
+  const Row<V> power = Row<V>::of(e), sum = power + Row<V>::all(1.f);
+  sum.get(e);
+#pragma unroll
+  for (int i = 0; i < V; ++i) e[i] = sizeof(T) == 2 ? reciprocal(e[i]) : __frcp_rn(e[i]);
+  take = Row<V>::of(e);
+  keep = power * take;
+}
+__device__ __forceinline__ void gate_of(float gate, float& keep, float& take, bool half) {
+  Row<1> k, t;
+  if (half) gates_of<__nv_bfloat16, 1>(Row<1>{gate}, k, t); else gates_of<float, 1>(Row<1>{gate}, k, t);
+  keep = k.f; take = t.f;
 }
 
 // What a run of rows does to the state in front of it: h -> a h + b, or h -> b where a sequence starts within (a is then -0, and stays negative
@@ -72,188 +126,221 @@ __device__ __forceinline__ int sequence_of(const ScanShape& p, int t) {
 }
 __device__ __forceinline__ long long first_row(const ScanShape& p, int s) { return p.offsets == nullptr ? static_cast<long long>(s) * p.length : offset_of(p, s); }
 
-template <class T, int VEC> struct Raw;
-template <> struct Raw<__nv_bfloat16, 8> {
-  uint4 v;
-  __device__ __forceinline__ void load(const void* base, long long at) { v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + at); }
-  __device__ __forceinline__ void clear() { v = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ float get(int i) const {
-    const uint32_t u = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
-    return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
-  }
-};
-template <> struct Raw<float, 4> {
-  float4 v;
-  __device__ __forceinline__ void load(const void* base, long long at) { v = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at); }
-  __device__ __forceinline__ void clear() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ float get(int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-};
-template <class T> struct Raw<T, 1> {
-  T v;
-  __device__ __forceinline__ void load(const void* base, long long at) { v = static_cast<const T*>(base)[at]; }
-  __device__ __forceinline__ void clear() { v = from_float<T>(0.f); }
-  __device__ __forceinline__ float get(int) const { return to_float(v); }
-};
-template <class T, int VEC>
-__device__ __forceinline__ void store_row(void* base, long long at, const float (&f)[VEC]) {
-  if constexpr (VEC == 8) {
+template <class T, int V>
+__device__ __forceinline__ void store_row(void* base, long long at, const Row<V>& row) {
+  float f[V];
+  row.get(f);
+  if constexpr (V == 8) {
     *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + at) =
         make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  } else if constexpr (VEC == 4) {
+  } else if constexpr (V == 4) {
     *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = make_float4(f[0], f[1], f[2], f[3]);
   } else {
     static_cast<T*>(base)[at] = from_float<T>(f[0]);
   }
 }
-template <int VEC>
-__device__ __forceinline__ void load_state(const float* base, long long at, float (&f)[VEC]) {
-  if (base == nullptr) {
+template <int V>
+__device__ __forceinline__ Row<V> load_state(const float* base, long long at) {
+  if (base == nullptr) return Row<V>::all(0.f);
+  float f[V];
+  if constexpr (V >= 4) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = 0.f;
-  } else if constexpr (VEC >= 4) {
-#pragma unroll
-    for (int i = 0; i < VEC; i += 4) {
+    for (int i = 0; i < V; i += 4) {
       const float4 v = *reinterpret_cast<const float4*>(base + at + i);
       f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
     }
   } else {
     f[0] = base[at];
   }
+  return Row<V>::of(f);
 }
-template <int VEC>
-__device__ __forceinline__ void store_state(float* base, long long at, const float (&f)[VEC]) {
-  if constexpr (VEC >= 4) {
+template <int V>
+__device__ __forceinline__ void store_state(float* base, long long at, const Row<V>& row) {
+  float f[V];
+  row.get(f);
+  if constexpr (V >= 4) {
 #pragma unroll
-    for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(base + at + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(base + at + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
   } else {
     base[at] = f[0];
   }
 }
 
-// A unit of work: a chunk of rows and a tile of channels.  A thread holds R rows of VEC channels in registers, LANES threads lie side by side
-// across the channels, and the others above one another along time.
-template <class T, int V> struct Tile {
-  static constexpr int VEC = V;
+// A unit of work: a chunk of rows and a tile of channels.  A thread has R rows of V channels; LANES threads lie side by side across the
+// channels, and the piles of R rows above one another along time.
+template <class Type, int Vec> struct Tile {
+  using T = Type;
+  static constexpr int V = Vec;
   static constexpr int LANES = V > 1 ? 8 : 32;
-  static constexpr int R = V == 8 ? 4 : V == 4 ? 8 : 16;
-  static constexpr int PILES = kScanThreads / LANES;           // of R rows
+  static constexpr int R = V > 1 ? 4 : 16;
+  static constexpr int PILES = kScanThreads / LANES;
   static constexpr int ROWS = PILES * R;
   static constexpr int COLS = LANES * V;
-  static constexpr int PARTS = kScanThreads / COLS;            // threads that share the joining of one channel
+  static constexpr int PARTS = kScanThreads / COLS;            // threads that share a channel where runs are joined
+  static constexpr int PART_PILES = PILES / PARTS;
+  // Each thread copies its rows into places of its own in shared memory (nobody has to wait for anybody else's copies): row r of thread i lies at
+  // r * PITCH + i * SLOT.  When the gates have been read, the run of a pile and channel takes the place of two of them; the pitch keeps
+  // the 16 channels that are read together in different banks.
+  static constexpr int SLOT = V > 1 ? 16 : 4;
+  static constexpr int PITCH = kScanThreads * SLOT + (V == 8 ? 32 : V == 4 ? 64 : 0);
+  static constexpr int ARRAY = R * PITCH;
+  static constexpr int RUNS = V > 1 ? 0 : PILES * COLS * 8;     // (with one channel a thread the runs lie by themselves)
+  __device__ __forceinline__ static unsigned char* run_at(unsigned char* gates, unsigned char* runs, int pile_order, int ch) {
+    if constexpr (V > 1) return gates + (ch % V) / 2 * PITCH + (pile_order * LANES + ch / V) * SLOT + (ch & 1) * 8;
+    else return runs + (pile_order * COLS + ch) * 8;
+  }
+};
+template <class Tl>
+__device__ __forceinline__ void fetch(unsigned char* place, const void* base, long long at, bool there) {
+  using T = typename Tl::T;
+  if constexpr (Tl::V > 1) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(smem_u32(place)), "l"(static_cast<const T*>(base) + (there ? at : 0)), "r"(there ? 16 : 0) : "memory");
+  } else if constexpr (sizeof(T) == 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(smem_u32(place)), "l"(static_cast<const T*>(base) + (there ? at : 0)), "r"(there ? 4 : 0) : "memory");
+  } else {
+    *reinterpret_cast<float*>(place) = there ? to_float(static_cast<const T*>(base)[at]) : 0.f;
+  }
+}
+template <class Tl>
+__device__ __forceinline__ Row<Tl::V> fetched(const unsigned char* place) {
+  if constexpr (Tl::V == 8) {
+    const uint4 v = *reinterpret_cast<const uint4*>(place);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    Row<8> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.put(i, __uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    return r;
+  } else if constexpr (Tl::V == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(place);
+    Row<4> r;
+    r.put(0, v.x, v.y); r.put(1, v.z, v.w);
+    return r;
+  } else {
+    return Row<1>{*reinterpret_cast<const float*>(place)};
+  }
+}
+__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(kLeft) : "memory"); }
+
+// The rows of a unit and what is handed on within its block.
+template <class Tl>
+struct ScanShared {
+  int seq[2][Tl::ROWS + 2];      // sequences of the rows from the one before the chunk to the one behind it, of two units
+  Run parts[Tl::PARTS][Tl::COLS], before[Tl::PARTS][Tl::COLS], folds[Tl::PARTS][Tl::COLS];
+  float carry[Tl::PARTS][Tl::COLS];
+  int next;                      // the unit after this one
 };
 
-// Chunks are dealt out in the order in which they depend on one another, by a ticket: a chunk waits only for chunks that were dealt out before it
-// and are running or done, however many blocks are resident.  `order` counts chunks from where the recurrence starts (the first row, or the last
-// one for the backward).  Each leaves what it does to the state (Run) as soon as it knows it; the state in front of a chunk is that of its group of
-// 32 chunks, and the runs of the chunks between, joined in one order: no rounding depends on who was first.  Only the
-// groups' states follow one another.
+// Chunks are dealt out in the order in which they depend on one another, by a ticket: a chunk waits only for chunks that were dealt out before it, and
+// every block works on its chunks in that order, so the first unfinished one never waits, however many blocks are resident.
+// `order` counts chunks from where the recurrence starts (the first row, or the last one for the backward).  Each leaves what it does to the state
+// (its run) as soon as it knows it; the state in front of a chunk is that behind the group of 32 chunks before it, and the runs of the chunks
+// between, joined in one order: no rounding depends on who was first.  Only the groups' states follow one another.
 template <class Tl>
 struct Chain {
   const ScanChain& c;
   const ScanShape& p;
-  int order, tile, col0;
+  ScanShared<Tl>& sh;
+  int order, tile;
+  // thread `i` works on channel `ch` of the tile, for part `part` of what is joined
+  int ch, part, col;
 
-  __device__ __forceinline__ float2* runs_at(int k) const { return c.runs + static_cast<long long>(k) * p.channels + col0; }
-  __device__ __forceinline__ float* state_at(int g) const { return c.states + static_cast<long long>(g) * p.channels + col0; }
+  __device__ __forceinline__ Chain(const ScanChain& c, const ScanShape& p, ScanShared<Tl>& sh, int order, int tile)
+      : c(c), p(p), sh(sh), order(order), tile(tile), ch(threadIdx.x % Tl::COLS), part(threadIdx.x / Tl::COLS), col(tile * Tl::COLS + ch) {}
+
+  __device__ __forceinline__ float2* run_at(int k) const { return c.runs + static_cast<long long>(k) * p.channels + col; }
+  __device__ __forceinline__ float* state_at(int g) const { return c.states + static_cast<long long>(g) * p.channels + col; }
   __device__ __forceinline__ int* flag_at(int k) const { return c.flags + static_cast<long long>(k) * c.tiles + tile; }
   __device__ __forceinline__ int* group_flag_at(int g) const { return c.flags + static_cast<long long>(c.chunks + g) * c.tiles + tile; }
+  // a flag counts the warps that have left their channels
+  static constexpr int kWarps = Tl::COLS / 32;
+  __device__ __forceinline__ void leave(int* flag) const {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) { __threadfence(); red_release_gpu_add(flag, 1); }
+  }
+  __device__ __forceinline__ bool wait(int* flag, int what) const {
+    const bool ok = spin_until([&] { return ld_acquire_gpu(flag) >= kWarps; }, p.wait_budget_ns, p.status);
+    if (!ok) report_failure(p.status, kStatusTimeoutPipeline, kKernelScan, 0, p.rank, order, what, tile);
+    return ok;
+  }
 
-  // Thread i < COLS has the chunk's run for its channel; all threads call.
-  __device__ __forceinline__ void publish(Run run) const {
-    if (threadIdx.x < Tl::COLS && col0 + static_cast<int>(threadIdx.x) < p.channels) __stcg(runs_at(order) + threadIdx.x, make_float2(run.a, run.b));
+  // From the runs of the piles in shared memory (in order): each becomes the run of the piles before it in its part; sh.before: of the parts before.
+  // Leaves the whole chunk's run to the chunks behind, and returns it.
+  template <class RunAt>
+  __device__ __forceinline__ Run join_piles(RunAt run_in_smem) {
     __syncthreads();
-    if (threadIdx.x == 0) { __threadfence(); red_release_gpu_add(flag_at(order), 1); }
-  }
-  __device__ __forceinline__ void publish_state(float state) const {
-    if (threadIdx.x < Tl::COLS && col0 + static_cast<int>(threadIdx.x) < p.channels) __stcg(state_at(order / kScanGroup) + threadIdx.x, state);
+    Run run = nothing();
+#pragma unroll
+    for (int i = 0; i < Tl::PART_PILES; ++i) {
+      float2* at = reinterpret_cast<float2*>(run_in_smem(part * Tl::PART_PILES + i, ch));
+      const float2 v = *at;
+      *at = make_float2(run.a, run.b);
+      run = join(run, Run{v.x, v.y});
+    }
+    sh.parts[part][ch] = run;
     __syncthreads();
-    if (threadIdx.x == 0) { __threadfence(); red_release_gpu_add(group_flag_at(order / kScanGroup), 1); }
+    Run whole = nothing(), mine = nothing();
+#pragma unroll
+    for (int i = 0; i < Tl::PARTS; ++i) {
+      if (i == part) mine = whole;
+      whole = join(whole, sh.parts[i][ch]);
+    }
+    sh.before[part][ch] = mine;                  // (read by this thread alone)
+    if (part == 0 && c.ticket != nullptr) {
+      if (col < p.channels) __stcg(run_at(order), make_float2(whole.a, whole.b));
+      leave(flag_at(order));
+    }
+    return whole;
   }
-  // The state in front of this chunk for threads i < COLS, of a sequence that starts in chunk `from` (in this order).  All threads call; `scratch`
-  // holds PARTS x COLS runs.
-  __device__ __forceinline__ float state_before(int from, Run* scratch) const {
+
+  // The state in front of this chunk, of a sequence that starts in chunk `from` (in this order).
+  __device__ __forceinline__ float state_before(int from) {
     const int group = order / kScanGroup, group_start = group * kScanGroup;
     const bool whole = from < group_start;
-    const int begin = whole ? group_start : from, n = order - begin;
+    const int start = whole ? group_start : from, n = order - start;
+    const int begin = start + n * part / Tl::PARTS, end = start + n * (part + 1) / Tl::PARTS, lane = threadIdx.x & 31;
     bool ok = true;
-    if (threadIdx.x < 64) {
-      const int i = threadIdx.x;
-      int* flag = i < n ? flag_at(begin + i) : i == 63 && whole ? group_flag_at(group - 1) : nullptr;
-      if (flag != nullptr) {
-        ok = spin_until([&] { return ld_acquire_gpu(flag) != 0; }, p.wait_budget_ns, p.status);
-        if (!ok) report_failure(p.status, kStatusTimeoutPipeline, kKernelScan, 0, p.rank, order, begin + i, tile);
-      }
-    }
-    ok = __syncthreads_and(ok) != 0;
-    const int ch = threadIdx.x % Tl::COLS, part = threadIdx.x / Tl::COLS;
-    const bool mine = col0 + ch < p.channels;
-    float state = 0.f;
-    if (whole && mine && part == 0) state = __ldcg(state_at(group - 1) + ch);
+    if (lane < end - begin) ok = wait(flag_at(begin + lane), begin + lane);
+    if (lane == 31 && whole) ok = wait(group_flag_at(group - 1), group) && ok;
+    ok = __all_sync(0xffffffffu, ok);
+    const bool in = col < p.channels;
+    float state = whole && in ? __ldcg(state_at(group - 1)) : 0.f;
     Run run = nothing();
-    if (mine) {
-      const int last = begin + n * (part + 1) / Tl::PARTS;
-#pragma unroll 4
-      for (int k = begin + n * part / Tl::PARTS; k < last; ++k) {
-        const float2 v = __ldcg(runs_at(k) + ch);
+    if (in) {
+#pragma unroll 8
+      for (int k = begin; k < end; ++k) {
+        const float2 v = __ldcg(run_at(k));
         run = join(run, Run{v.x, v.y});
       }
     }
-    scratch[threadIdx.x] = run;
+    if (!ok) run = {-0.f, __int_as_float(0x7fc00000)};
+    sh.folds[part][ch] = run;
     __syncthreads();
-    if (part == 0) {
 #pragma unroll
-      for (int i = 0; i < Tl::PARTS; ++i) state = apply(scratch[i * Tl::COLS + ch], state);
+    for (int i = 0; i < Tl::PARTS; ++i) state = apply(sh.folds[i][ch], state);
+    return state;
+  }
+  // The state behind the chunk goes to the group behind; the state in front of each part to the block's threads.
+  __device__ __forceinline__ void spread(Run whole, float state) {
+    if (part == 0 && c.ticket != nullptr && order % kScanGroup == kScanGroup - 1) {
+      if (col < p.channels) __stcg(state_at(order / kScanGroup), apply(whole, state));
+      leave(group_flag_at(order / kScanGroup));
     }
-    return ok ? state : __int_as_float(0x7fc00000);
+    sh.carry[part][ch] = apply(sh.before[part][ch], state);
+    __syncthreads();
+  }
+  // The state in front of this thread's pile.
+  template <class RunAt>
+  __device__ __forceinline__ Row<Tl::V> state_of_pile(RunAt run_in_smem, int pile_order, int side) const {
+    float f[Tl::V];
+#pragma unroll
+    for (int i = 0; i < Tl::V; ++i) {
+      const float2 r = *reinterpret_cast<const float2*>(run_in_smem(pile_order, side * Tl::V + i));
+      f[i] = apply(Run{r.x, r.y}, sh.carry[pile_order / Tl::PART_PILES][side * Tl::V + i]);
+    }
+    return Row<Tl::V>::of(f);
   }
 };
-
-// Which chunk this block takes; the same for all of its threads.
-__device__ __forceinline__ int claim_unit(const ScanChain& c, int* slot) {
-  if (c.ticket == nullptr) return blockIdx.x;
-  if (threadIdx.x == 0) *slot = atomicAdd(c.ticket, 1);
-  __syncthreads();
-  return *slot;
-}
-
-// Runs of the threads of a block that lie above one another, `mine` in the order of threads: what all threads before this one do, and
-// for threads i < COLS what the whole block does to channel i.
-template <class Tl>
-__device__ __forceinline__ void block_runs(Run (&mine)[Tl::VEC], Run (&before)[Tl::VEC], Run& whole, Run (*scratch)[Tl::COLS]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = threadIdx.x % Tl::LANES;
-  // within the warp
-#pragma unroll
-  for (int d = Tl::LANES; d < 32; d *= 2) {
-#pragma unroll
-    for (int i = 0; i < Tl::VEC; ++i) {
-      const Run prev = {__shfl_up_sync(0xffffffffu, mine[i].a, d), __shfl_up_sync(0xffffffffu, mine[i].b, d)};
-      if (lane >= d) mine[i] = join(prev, mine[i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < Tl::VEC; ++i) {
-    if (lane >= 32 - Tl::LANES) scratch[warp][side * Tl::VEC + i] = mine[i];
-    if constexpr (Tl::LANES < 32) {
-      const Run prev = {__shfl_up_sync(0xffffffffu, mine[i].a, Tl::LANES), __shfl_up_sync(0xffffffffu, mine[i].b, Tl::LANES)};
-      before[i] = lane >= Tl::LANES ? prev : nothing();
-    } else {
-      before[i] = nothing();
-    }
-  }
-  __syncthreads();
-  whole = nothing();
-  if (threadIdx.x < Tl::COLS) {
-#pragma unroll
-    for (int w = 0; w < kScanThreads / 32; ++w) {
-      const Run r = scratch[w][threadIdx.x];
-      scratch[w][threadIdx.x] = whole;
-      whole = join(whole, r);
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < Tl::VEC; ++i) before[i] = join(scratch[warp][side * Tl::VEC + i], before[i]);
-}
 
 // Sequences without rows hand their state on (`from` to `to`); offsets that are none are reported.  A block looks at its share of the sequences.
 template <class Tl>
@@ -274,188 +361,211 @@ __device__ __forceinline__ void empty_sequences(const ScanShape& p, const ScanCh
   }
 }
 
-template <class T, int V>
+// The first unit of a block.
+__device__ __forceinline__ int first_unit(const ScanChain& c, int* next) {
+  if (c.ticket == nullptr) return blockIdx.x;
+  if (threadIdx.x == 0) *next = atomicAdd(c.ticket, 1);
+  __syncthreads();
+  const int unit = *next;
+  __syncthreads();
+  return unit;
+}
+
+// Rows of the unit after this one are on their way while this one's are worked on.
+template <class Tl>
 __global__ void __launch_bounds__(kScanThreads, 2) scan_forward_kernel(const ScanParams p, const ScanChain c) {
-  using Tl = Tile<T, V>;
-  __shared__ int seq[Tl::ROWS + 2];              // of the rows from the one before the chunk to the one behind it
-  __shared__ Run warps[kScanThreads / 32][Tl::COLS];
-  __shared__ Run parts[kScanThreads];
-  __shared__ float carry[Tl::COLS];
-  __shared__ int slot;
-  const int unit = claim_unit(c, &slot), chunk = unit / c.tiles, tile = unit - chunk * c.tiles;
-  const int row0 = chunk * Tl::ROWS, col0 = tile * Tl::COLS;
-  const int side = threadIdx.x % Tl::LANES, pile = threadIdx.x / Tl::LANES;
-  const int col = col0 + side * V, first = row0 + pile * Tl::R;
-  const bool in = col < p.channels;
-  Raw<T, V> x[Tl::R], gate[Tl::R];
+  using T = typename Tl::T;
+  constexpr int V = Tl::V, R = Tl::R;
+  extern __shared__ __align__(16) unsigned char space[];       // [2 units][gate, x], runs
+  __shared__ ScanShared<Tl> sh;
+  const int side = threadIdx.x % Tl::LANES, pile = threadIdx.x / Tl::LANES, units = c.chunks * c.tiles;
+  auto array = [&](int buffer, int which) { return space + (buffer * 2 + which) * Tl::ARRAY; };
+  auto place = [&](int buffer, int which, int r) { return array(buffer, which) + r * Tl::PITCH + threadIdx.x * Tl::SLOT; };
+  auto issue = [&](int unit, int buffer) {
+    if (unit < units) {
+      const int chunk = unit / c.tiles, tile = unit - chunk * c.tiles, row0 = chunk * Tl::ROWS, col = tile * Tl::COLS + side * V;
 #pragma unroll
-  for (int r = 0; r < Tl::R; ++r) {
-    if (in && first + r < p.rows) {
-      gate[r].load(p.gate, (first + r) * p.gate_stride + col);
-      x[r].load(p.x, (first + r) * p.x_stride + col);
-    } else {
-      gate[r].clear(); x[r].clear();
+      for (int r = 0; r < R; ++r) {
+        const int t = row0 + pile * R + r;
+        const bool there = col < p.channels && t < p.rows;
+        fetch<Tl>(place(buffer, 0, r), p.gate, t * p.gate_stride + col, there);
+        fetch<Tl>(place(buffer, 1, r), p.x, t * p.x_stride + col, there);
+      }
+      for (int i = threadIdx.x; i < Tl::ROWS + 2; i += kScanThreads) sh.seq[buffer][i] = sequence_of(p, row0 - 1 + i);
     }
-  }
-  for (int i = threadIdx.x; i < Tl::ROWS + 2; i += kScanThreads) seq[i] = sequence_of(p, row0 - 1 + i);
-  empty_sequences<Tl>(p, c, chunk, tile, p.initial, p.final_state, true);
+    fetch_commit();
+  };
+  int unit = first_unit(c, &sh.next), buffer = 0;
+  issue(unit, 0);
   __syncthreads();
+  for (; unit < units; buffer ^= 1) {
+    const int chunk = unit / c.tiles, tile = unit - chunk * c.tiles;
+    const int first = chunk * Tl::ROWS + pile * R, col = tile * Tl::COLS + side * V;
+    const bool in = col < p.channels;
+    const int* seq = sh.seq[buffer];
+    auto run_at = [&](int pile_order, int ch) { return Tl::run_at(array(buffer, 0), space + 4 * Tl::ARRAY, pile_order, ch); };
+    empty_sequences<Tl>(p, c, chunk, tile, p.initial, p.final_state, true);
+    if (c.ticket != nullptr && threadIdx.x == 0) sh.next = atomicAdd(c.ticket, 1);
+    fetch_wait<0>();
 
-  float small[Tl::R][V];
-  Run mine[V], before[V], whole;
+    Row<V> keep[R], add[R];                      // h -> keep h + add
+    Row<V> a = Row<V>::all(1.f), b = Row<V>::all(0.f);
 #pragma unroll
-  for (int i = 0; i < V; ++i) mine[i] = nothing();
-#pragma unroll
-  for (int r = 0; r < Tl::R; ++r) {
-    const int at = pile * Tl::R + r + 1, s = seq[at];
-    if (s != seq[at - 1] || s < 0) {
-      float start[V];
-      load_state<V>(s >= 0 && in ? p.initial : nullptr, static_cast<long long>(s) * p.channels + col, start);
-#pragma unroll
-      for (int i = 0; i < V; ++i) mine[i] = {-0.f, start[i]};
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      small[r][i] = smaller<T>(gate[r].get(i));
+    for (int r = 0; r < R; ++r) {
+      const int at = pile * R + r + 1, s = seq[at];
+      gates_of<T, V>(fetched<Tl>(place(buffer, 0, r)), keep[r], add[r]);
+      add[r] = add[r] * fetched<Tl>(place(buffer, 1, r));
+      if (s != seq[at - 1] || s < 0) {
+        a = Row<V>::all(-0.f);
+        b = load_state<V>(s >= 0 && in ? p.initial : nullptr, static_cast<long long>(s) * p.channels + col);
+      }
       if (s >= 0) {
-        const Gate g = gate_of(small[r][i]);
-        mine[i] = {mine[i].a * g.keep, fmaf(g.keep, mine[i].b, g.take * x[r].get(i))};
+        a = a * keep[r];
+        b = fused(keep[r], b, add[r]);
       }
     }
-  }
-  block_runs<Tl>(mine, before, whole, warps);
-
-  const Chain<Tl> chain{c, p, chunk, tile, col0};
-  if (c.ticket != nullptr) chain.publish(whole);
-  const bool continues = seq[1] >= 0 && seq[1] == seq[0];
-  float state = 0.f;
-  if (continues) state = chain.state_before(static_cast<int>(max(first_row(p, seq[1]), 0ll) / Tl::ROWS), parts);
-  if (threadIdx.x < Tl::COLS) carry[threadIdx.x] = state;
-  if (c.ticket != nullptr && chunk % kScanGroup == kScanGroup - 1) chain.publish_state(apply(whole, state));
-  __syncthreads();
-  if (!in) return;
-
-  float h[V];
+    {
+      float fa[V], fb[V];
+      a.get(fa); b.get(fb);
 #pragma unroll
-  for (int i = 0; i < V; ++i) h[i] = apply(before[i], carry[side * V + i]);
-#pragma unroll
-  for (int r = 0; r < Tl::R; ++r) {
-    if (first + r >= p.rows) break;
-    const int at = pile * Tl::R + r + 1, s = seq[at];
-    if (s != seq[at - 1] || s < 0) load_state<V>(s >= 0 ? p.initial : nullptr, static_cast<long long>(s) * p.channels + col, h);
-    if (s >= 0) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const Gate g = gate_of(small[r][i]);
-        h[i] = fmaf(g.keep, h[i], g.take * x[r].get(i));
-      }
-      if (p.final_state != nullptr && seq[at + 1] != s) store_state<V>(p.final_state, static_cast<long long>(s) * p.channels + col, h);
+      for (int i = 0; i < V; ++i) *reinterpret_cast<float2*>(run_at(pile, side * V + i)) = make_float2(fa[i], fb[i]);
     }
-    store_row<T, V>(p.h, static_cast<long long>(first + r) * p.channels + col, h);
+    Chain<Tl> chain(c, p, sh, chunk, tile);
+    const Run whole = chain.join_piles(run_at);
+    const int next = c.ticket != nullptr ? sh.next : units;
+    issue(next, buffer ^ 1);
+    float state = 0.f;
+    if (seq[1] >= 0 && seq[1] == seq[0]) state = chain.state_before(static_cast<int>(max(first_row(p, seq[1]), 0ll) / Tl::ROWS));
+    chain.spread(whole, state);
+
+    Row<V> h = chain.state_of_pile(run_at, pile, side);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (!in || first + r >= p.rows) break;
+      const int at = pile * R + r + 1, s = seq[at];
+      if (s != seq[at - 1] || s < 0) h = load_state<V>(s >= 0 ? p.initial : nullptr, static_cast<long long>(s) * p.channels + col);
+      if (s >= 0) {
+        h = fused(keep[r], h, add[r]);
+        if (p.final_state != nullptr && seq[at + 1] != s) store_state<V>(p.final_state, static_cast<long long>(s) * p.channels + col, h);
+      }
+      store_row<T, V>(p.h, static_cast<long long>(first + r) * p.channels + col, h);
+    }
+    unit = next;
   }
 }
 
 // As the forward, from the last row to the first: what runs along is keep_t g_t.
-template <class T, int V>
+template <class Tl>
 __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(const ScanGradParams p, const ScanChain c) {
-  using Tl = Tile<T, V>;
-  __shared__ int seq[Tl::ROWS + 2];
-  __shared__ Run warps[kScanThreads / 32][Tl::COLS];
-  __shared__ Run parts[kScanThreads];
-  __shared__ float carry[Tl::COLS];
-  __shared__ int slot;
-  const int unit = claim_unit(c, &slot), order = unit / c.tiles, tile = unit - order * c.tiles;
-  const int chunk = c.chunks - 1 - order, row0 = chunk * Tl::ROWS, col0 = tile * Tl::COLS;
-  const int side = threadIdx.x % Tl::LANES, pile = Tl::PILES - 1 - static_cast<int>(threadIdx.x) / Tl::LANES;
-  const int col = col0 + side * V, first = row0 + pile * Tl::R;
-  const bool in = col < p.channels;
-  Raw<T, V> x[Tl::R], gate[Tl::R], dh[Tl::R], before_row[Tl::R];
+  using T = typename Tl::T;
+  constexpr int V = Tl::V, R = Tl::R;
+  extern __shared__ __align__(16) unsigned char space[];       // [2 units][gate, dh], x, h of the row before, runs
+  __shared__ ScanShared<Tl> sh;
+  const int side = threadIdx.x % Tl::LANES, pile_order = threadIdx.x / Tl::LANES, pile = Tl::PILES - 1 - pile_order, units = c.chunks * c.tiles;
+  auto array = [&](int buffer, int which) { return space + (buffer * 2 + which) * Tl::ARRAY; };
+  auto place = [&](int buffer, int which, int r) { return array(buffer, which) + r * Tl::PITCH + threadIdx.x * Tl::SLOT; };
+  auto issue = [&](int unit, int buffer) {
+    if (unit < units) {
+      const int order = unit / c.tiles, tile = unit - order * c.tiles, row0 = (c.chunks - 1 - order) * Tl::ROWS, col = tile * Tl::COLS + side * V;
 #pragma unroll
-  for (int r = 0; r < Tl::R; ++r) {
-    const int t = first + r;
-    const bool there = in && t < p.rows;
-    if (there) gate[r].load(p.gate, t * p.gate_stride + col); else gate[r].clear();
-    if (there && p.dh != nullptr) dh[r].load(p.dh, t * p.dh_stride + col); else dh[r].clear();
-    if (there && p.dgate != nullptr) x[r].load(p.x, t * p.x_stride + col); else x[r].clear();
-    if (there && p.dgate != nullptr && t > 0) before_row[r].load(p.h, static_cast<long long>(t - 1) * p.channels + col); else before_row[r].clear();
-  }
-  for (int i = threadIdx.x; i < Tl::ROWS + 2; i += kScanThreads) seq[i] = sequence_of(p, row0 - 1 + i);
-  empty_sequences<Tl>(p, c, order, tile, p.dfinal, p.dinitial, false);
-  __syncthreads();
-
-  float small[Tl::R][V];
-  Run mine[V], before[V], whole;
-#pragma unroll
-  for (int i = 0; i < V; ++i) mine[i] = nothing();
-#pragma unroll
-  for (int r = Tl::R - 1; r >= 0; --r) {
-    const int at = pile * Tl::R + r + 1, s = seq[at];
-    if (s != seq[at + 1] || s < 0) {
-      float end[V];
-      load_state<V>(s >= 0 && in ? p.dfinal : nullptr, static_cast<long long>(s) * p.channels + col, end);
-#pragma unroll
-      for (int i = 0; i < V; ++i) mine[i] = {-0.f, end[i]};
+      for (int r = 0; r < R; ++r) {
+        const int t = row0 + pile * R + r;
+        const bool there = col < p.channels && t < p.rows;
+        fetch<Tl>(place(buffer, 0, r), p.gate, t * p.gate_stride + col, there);
+        fetch<Tl>(place(buffer, 1, r), p.dh, t * p.dh_stride + col, there && p.dh != nullptr);
+      }
+      for (int i = threadIdx.x; i < Tl::ROWS + 2; i += kScanThreads) sh.seq[buffer][i] = sequence_of(p, row0 - 1 + i);
     }
+    fetch_commit();
+  };
+  // what only the gate's gradient needs, later than the rest
+  auto issue_late = [&](int unit) {
+    if (unit < units && p.dgate != nullptr) {
+      const int order = unit / c.tiles, tile = unit - order * c.tiles, row0 = (c.chunks - 1 - order) * Tl::ROWS, col = tile * Tl::COLS + side * V;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      small[r][i] = smaller<T>(gate[r].get(i));
+      for (int r = 0; r < R; ++r) {
+        const int t = row0 + pile * R + r;
+        const bool there = col < p.channels && t < p.rows;
+        fetch<Tl>(place(2, 0, r), p.x, t * p.x_stride + col, there);
+        fetch<Tl>(place(2, 1, r), p.h, static_cast<long long>(t - 1) * p.channels + col, there && t > 0);
+      }
+    }
+    fetch_commit();
+  };
+  int unit = first_unit(c, &sh.next), buffer = 0;
+  issue(unit, 0);
+  issue_late(unit);
+  __syncthreads();
+  for (; unit < units; buffer ^= 1) {
+    const int order = unit / c.tiles, tile = unit - order * c.tiles, chunk = c.chunks - 1 - order;
+    const int first = chunk * Tl::ROWS + pile * R, col = tile * Tl::COLS + side * V;
+    const bool in = col < p.channels;
+    const int* seq = sh.seq[buffer];
+    auto run_at = [&](int order_of_pile, int ch) { return Tl::run_at(array(buffer, 0), space + 6 * Tl::ARRAY, order_of_pile, ch); };
+    empty_sequences<Tl>(p, c, order, tile, p.dfinal, p.dinitial, false);
+    if (c.ticket != nullptr && threadIdx.x == 0) sh.next = atomicAdd(c.ticket, 1);
+    fetch_wait<1>();
+
+    Row<V> keep[R], take[R];
+    Row<V> a = Row<V>::all(1.f), b = Row<V>::all(0.f);
+#pragma unroll
+    for (int r = R - 1; r >= 0; --r) {
+      const int at = pile * R + r + 1, s = seq[at];
+      gates_of<T, V>(fetched<Tl>(place(buffer, 0, r)), keep[r], take[r]);
+      if (s != seq[at + 1] || s < 0) {
+        a = Row<V>::all(-0.f);
+        b = load_state<V>(s >= 0 && in ? p.dfinal : nullptr, static_cast<long long>(s) * p.channels + col);
+      }
       if (s >= 0) {
-        const float keep = gate_of(small[r][i]).keep;
-        mine[i] = {mine[i].a * keep, __fmul_rn(keep, __fadd_rn(mine[i].b, dh[r].get(i)))};
+        a = a * keep[r];
+        b = keep[r] * (b + fetched<Tl>(place(buffer, 1, r)));
       }
     }
-  }
-  block_runs<Tl>(mine, before, whole, warps);
-
-  const Chain<Tl> chain{c, p, order, tile, col0};
-  if (c.ticket != nullptr) chain.publish(whole);
-  const int last = seq[Tl::ROWS];
-  float state = 0.f;
-  if (last >= 0 && last == seq[Tl::ROWS + 1]) {
-    const long long end = min(max(first_row(p, last + 1), 1ll), static_cast<long long>(p.rows)) - 1;      // the sequence's last row
-    state = chain.state_before(max(c.chunks - 1 - static_cast<int>(end / Tl::ROWS), 0), parts);
-  }
-  if (threadIdx.x < Tl::COLS) carry[threadIdx.x] = state;
-  if (c.ticket != nullptr && order % kScanGroup == kScanGroup - 1) chain.publish_state(apply(whole, state));
-  __syncthreads();
-  if (!in) return;
-
-  float back[V];                                 // keep_{t+1} g_{t+1}
+    {
+      float fa[V], fb[V];
+      a.get(fa); b.get(fb);
 #pragma unroll
-  for (int i = 0; i < V; ++i) back[i] = apply(before[i], carry[side * V + i]);
-#pragma unroll
-  for (int r = Tl::R - 1; r >= 0; --r) {
-    const int t = first + r;
-    if (t >= p.rows) continue;
-    const int at = pile * Tl::R + r + 1, s = seq[at];
-    float dx[V], dgate[V];
-    if (s >= 0) {
-      const long long state_at = static_cast<long long>(s) * p.channels + col;
-      if (s != seq[at + 1]) load_state<V>(p.dfinal, state_at, back);
-      const bool start = s != seq[at - 1];
-      float h[V];
-      if (start) {
-        load_state<V>(p.initial, state_at, h);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = before_row[r].get(i);
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const Gate k = gate_of(small[r][i]);
-        const float g = __fadd_rn(back[i], dh[r].get(i));
-        dx[i] = k.take * g;
-        dgate[i] = g * (k.keep * k.take) * (h[i] - x[r].get(i));
-        back[i] = __fmul_rn(k.keep, g);
-      }
-      if (start && p.dinitial != nullptr) store_state<V>(p.dinitial, state_at, back);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) dx[i] = dgate[i] = 0.f;
+      for (int i = 0; i < V; ++i) *reinterpret_cast<float2*>(run_at(pile_order, side * V + i)) = make_float2(fa[i], fb[i]);
     }
-    const long long out = static_cast<long long>(t) * p.channels + col;
-    if (p.dx != nullptr) store_row<T, V>(p.dx, out, dx);
-    if (p.dgate != nullptr) store_row<T, V>(p.dgate, out, dgate);
+    Chain<Tl> chain(c, p, sh, order, tile);
+    const Run whole = chain.join_piles(run_at);
+    const int next = c.ticket != nullptr ? sh.next : units;
+    issue(next, buffer ^ 1);
+    const int last = seq[Tl::ROWS];
+    float state = 0.f;
+    if (last >= 0 && last == seq[Tl::ROWS + 1]) {
+      const long long end = min(max(first_row(p, last + 1), 1ll), static_cast<long long>(p.rows)) - 1;      // the sequence's last row
+      state = chain.state_before(max(c.chunks - 1 - static_cast<int>(end / Tl::ROWS), 0));
+    }
+    chain.spread(whole, state);
+
+    Row<V> back = chain.state_of_pile(run_at, pile_order, side);                   // keep_{t+1} g_{t+1}
+    fetch_wait<1>();
+#pragma unroll
+    for (int r = R - 1; r >= 0; --r) {
+      const int t = first + r;
+      if (!in || t >= p.rows) continue;
+      const int at = pile * R + r + 1, s = seq[at];
+      Row<V> dx = Row<V>::all(0.f), dgate = dx;
+      if (s >= 0) {
+        const long long state_at = static_cast<long long>(s) * p.channels + col;
+        if (s != seq[at + 1]) back = load_state<V>(p.dfinal, state_at);
+        const bool start = s != seq[at - 1];
+        const Row<V> g = back + fetched<Tl>(place(buffer, 1, r));
+        dx = take[r] * g;
+        if (p.dgate != nullptr) {
+          const Row<V> h = start ? load_state<V>(p.initial, state_at) : fetched<Tl>(place(2, 1, r));
+          dgate = g * (keep[r] * take[r]) * fused(Row<V>::all(-1.f), fetched<Tl>(place(2, 0, r)), h);
+        }
+        back = keep[r] * g;
+        if (start && p.dinitial != nullptr) store_state<V>(p.dinitial, state_at, back);
+      }
+      const long long out = static_cast<long long>(t) * p.channels + col;
+      if (p.dx != nullptr) store_row<T, V>(p.dx, out, dx);
+      if (p.dgate != nullptr) store_row<T, V>(p.dgate, out, dgate);
+    }
+    issue_late(next);
+    unit = next;
   }
 }
 
@@ -465,8 +575,9 @@ __global__ void __launch_bounds__(kThreads) scan_step_kernel(const ScanStepParam
   if (d >= p.channels) return;
   for (long long s = blockIdx.y; s < p.rows; s += gridDim.y) {
     float* state = p.state + s * p.state_stride + d;
-    const Gate g = gate_of(smaller<T>(to_float(static_cast<const T*>(p.gate)[s * p.gate_stride + d])));
-    const float h = fmaf(g.keep, *state, g.take * to_float(static_cast<const T*>(p.x)[s * p.x_stride + d]));
+    float keep, take;
+    gate_of(to_float(static_cast<const T*>(p.gate)[s * p.gate_stride + d]), keep, take, sizeof(T) == 2);
+    const float h = fmaf(keep, *state, __fmul_rn(take, to_float(static_cast<const T*>(p.x)[s * p.x_stride + d])));
     *state = h;
     static_cast<T*>(p.h)[s * p.channels + d] = from_float<T>(h);
   }
@@ -493,8 +604,8 @@ ScanPlan plan(const ScanShape& p) {
 }
 template <class F>
 auto by_tile(bool half, bool vectors, F f) {
-  if (half) return vectors ? f(Tile<__nv_bfloat16, 8>{}, __nv_bfloat16{}) : f(Tile<__nv_bfloat16, 1>{}, __nv_bfloat16{});
-  return vectors ? f(Tile<float, 4>{}, float{}) : f(Tile<float, 1>{}, float{});
+  if (half) return vectors ? f(Tile<__nv_bfloat16, 8>{}) : f(Tile<__nv_bfloat16, 1>{});
+  return vectors ? f(Tile<float, 4>{}) : f(Tile<float, 1>{});
 }
 
 // Where the parts of the workspace lie.
@@ -512,34 +623,44 @@ cudaError_t lay_out(ScanChain& c, const ScanPlan& s, int channels, void* space, 
 
 }  // namespace
 
-ScanPlan scan_plan(const ScanParams& p) { return by_tile(p.half, whole_vectors(p), [&](auto tile, auto) { return plan<decltype(tile)>(p); }); }
-ScanPlan scan_plan(const ScanGradParams& p) { return by_tile(p.half, whole_vectors(p), [&](auto tile, auto) { return plan<decltype(tile)>(p); }); }
+ScanPlan scan_plan(const ScanParams& p) { return by_tile(p.half, whole_vectors(p), [&](auto tile) { return plan<decltype(tile)>(p); }); }
+ScanPlan scan_plan(const ScanGradParams& p) { return by_tile(p.half, whole_vectors(p), [&](auto tile) { return plan<decltype(tile)>(p); }); }
 long long scan_space(const ScanPlan& s, int channels) {
   if (s.chunks == 1) return 0;
   const long long groups = (s.chunks + kScanGroup - 1) / kScanGroup;
   return 32 + 4 * (s.chunks + groups) * s.tiles + 8ll * s.chunks * channels + 4ll * groups * channels;
 }
 
-cudaError_t launch_scan_forward(const ScanParams& p, void* space, cudaStream_t stream) {
-  return by_tile(p.half, whole_vectors(p), [&](auto tile, auto type) {
-    const ScanPlan s = plan<decltype(tile)>(p);
-    ScanChain c{};
-    const cudaError_t e = lay_out(c, s, p.channels, space, stream);
-    if (e != cudaSuccess) return e;
-    scan_forward_kernel<decltype(type), decltype(tile)::VEC><<<static_cast<unsigned>(s.chunks) * s.tiles, kScanThreads, 0, stream>>>(p, c);
-    return cudaGetLastError();
-  });
+namespace {
+
+template <class Tl, class Params>
+cudaError_t launch_scan(void (*kernel)(const Params, const ScanChain), const Params& p, int arrays, int sms, void* space, cudaStream_t stream) {
+  const ScanPlan s = plan<Tl>(p);
+  ScanChain c{};
+  cudaError_t e = lay_out(c, s, p.channels, space, stream);
+  if (e != cudaSuccess) return e;
+  const int smem = arrays * Tl::ARRAY + Tl::RUNS;
+  static std::atomic<bool> configured[64];       // the shared-memory limit is an attribute of the function on a device
+  int dev = 0;
+  if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+    configured[dev].store(true, std::memory_order_release);
+  }
+  const long long units = static_cast<long long>(s.chunks) * s.tiles;
+  const unsigned grid = static_cast<unsigned>(s.chunks == 1 || units < 2 * sms ? units : 2 * sms);
+  kernel<<<grid, kScanThreads, smem, stream>>>(p, c);
+  return cudaGetLastError();
 }
 
-cudaError_t launch_scan_backward(const ScanGradParams& p, void* space, cudaStream_t stream) {
-  return by_tile(p.half, whole_vectors(p), [&](auto tile, auto type) {
-    const ScanPlan s = plan<decltype(tile)>(p);
-    ScanChain c{};
-    const cudaError_t e = lay_out(c, s, p.channels, space, stream);
-    if (e != cudaSuccess) return e;
-    scan_backward_kernel<decltype(type), decltype(tile)::VEC><<<static_cast<unsigned>(s.chunks) * s.tiles, kScanThreads, 0, stream>>>(p, c);
-    return cudaGetLastError();
-  });
+}  // namespace
+
+cudaError_t launch_scan_forward(const ScanParams& p, int sms, void* space, cudaStream_t stream) {
+  return by_tile(p.half, whole_vectors(p), [&](auto tile) { return launch_scan<decltype(tile)>(scan_forward_kernel<decltype(tile)>, p, 4, sms, space, stream); });
+}
+cudaError_t launch_scan_backward(const ScanGradParams& p, int sms, void* space, cudaStream_t stream) {
+  return by_tile(p.half, whole_vectors(p), [&](auto tile) { return launch_scan<decltype(tile)>(scan_backward_kernel<decltype(tile)>, p, 6, sms, space, stream); });
 }
 
 cudaError_t launch_scan_step(const ScanStepParams& p, int sms, cudaStream_t stream) {
