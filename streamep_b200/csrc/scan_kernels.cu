@@ -21,7 +21,6 @@ constexpr int kScanGroup = 32;                   // chunks between two states th
 struct ScanChain {
   int chunks, tiles;
   int* ticket;                   // null: one chunk, nothing is handed on
-  int* flags;                    // [chunks + groups][tiles]: the run, the group's state is there
   float2* runs;                  // [chunks][channels]
   float* states;                 // [groups][channels] behind each group
 };
@@ -178,15 +177,17 @@ template <class Type, int Vec> struct Tile {
   static constexpr int COLS = LANES * V;
   static constexpr int PARTS = kScanThreads / COLS;            // threads that share a channel where runs are joined
   static constexpr int PART_PILES = PILES / PARTS;
+  static constexpr int WARP_COLS = COLS / (kScanThreads / 32); // there, a warp has these channels of all parts
   // Each thread copies its rows into places of its own in shared memory (nobody has to wait for anybody else's copies): row r of thread i lies at
-  // r * PITCH + i * SLOT.  When the gates have been read, the run of a pile and channel takes the place of two of them; the pitch keeps
-  // the 16 channels that are read together in different banks.
+  // r * PITCH + slot(i).  When the gates have been read, the run of a pile and channel takes the place of two of them; the pitch, and 16 bytes between
+  // the threads of two parts, keep what half a warp reads together in different banks.
   static constexpr int SLOT = V > 1 ? 16 : 4;
-  static constexpr int PITCH = kScanThreads * SLOT + (V == 8 ? 32 : V == 4 ? 64 : 0);
+  static constexpr int PITCH = kScanThreads * SLOT + (V == 8 ? 160 : V == 4 ? 192 : 0);
+  __device__ __forceinline__ static int slot(int thread) { return thread * SLOT + (V > 1 ? thread / (PART_PILES * LANES) * 16 : 0); }
   static constexpr int ARRAY = R * PITCH;
   static constexpr int RUNS = V > 1 ? 0 : PILES * COLS * 8;     // (with one channel a thread the runs lie by themselves)
   __device__ __forceinline__ static unsigned char* run_at(unsigned char* gates, unsigned char* runs, int pile_order, int ch) {
-    if constexpr (V > 1) return gates + (ch % V) / 2 * PITCH + (pile_order * LANES + ch / V) * SLOT + (ch & 1) * 8;
+    if constexpr (V > 1) return gates + (ch % V) / 2 * PITCH + slot(pile_order * LANES + ch / V) + (ch & 1) * 8;
     else return runs + (pile_order * COLS + ch) * 8;
   }
 };
@@ -226,7 +227,6 @@ template <int kLeft> __device__ __forceinline__ void fetch_wait() { asm volatile
 template <class Tl>
 struct ScanShared {
   int seq[2][Tl::ROWS + 2];      // sequences of the rows from the one before the chunk to the one behind it, of two units
-  Run parts[Tl::PARTS][Tl::COLS], before[Tl::PARTS][Tl::COLS], folds[Tl::PARTS][Tl::COLS];
   float carry[Tl::PARTS][Tl::COLS];
   int next;                      // the unit after this one
 };
@@ -236,39 +236,62 @@ struct ScanShared {
 // `order` counts chunks from where the recurrence starts (the first row, or the last one for the backward).  Each leaves what it does to the state
 // (its run) as soon as it knows it; the state in front of a chunk is that behind the group of 32 chunks before it, and the runs of the chunks
 // between, joined in one order: no rounding depends on who was first.  Only the groups' states follow one another.
+//
+// A number says by itself that it is there: the workspace is filled with ones, which no number that is left has (NaN is left as 0x7fffffff), a run is
+// written and read as one 8-byte word, and nothing else is handed on with it that would have to be in order.  (With a flag beside it, its
+// writer waits for the numbers to arrive before the flag, its reader for the flag before the numbers: 8192 rows of 2048 channels 46.7 us, in
+// four barriers a unit instead of two.)
+constexpr uint32_t kAbsent = 0xffffffffu;
+__device__ __forceinline__ uint32_t present(float f) { const uint32_t u = __float_as_uint(f); return u == kAbsent ? 0x7fffffffu : u; }
+__device__ __forceinline__ void leave(float2* at, Run r) {
+  const unsigned long long v = static_cast<unsigned long long>(present(r.b)) << 32 | present(r.a);
+  asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" :: "l"(at), "l"(v) : "memory");
+}
+__device__ __forceinline__ void leave(float* at, float f) { asm volatile("st.relaxed.gpu.global.b32 [%0], %1;" :: "l"(at), "r"(present(f)) : "memory"); }
+__device__ __forceinline__ uint2 look(const float2* at) {
+  unsigned long long v;
+  asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(v) : "l"(at) : "memory");
+  return make_uint2(static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32));
+}
+__device__ __forceinline__ uint32_t look(const float* at) { uint32_t v; asm volatile("ld.relaxed.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(at) : "memory"); return v; }
+
 template <class Tl>
 struct Chain {
   const ScanChain& c;
   const ScanShape& p;
   ScanShared<Tl>& sh;
   int order, tile;
-  // thread `i` works on channel `ch` of the tile, for part `part` of what is joined
+  // this thread works on channel `ch` of the tile, for part `part` of what is joined; the other parts belong to lanes of its warp
   int ch, part, col;
+  Run before, whole;             // of this chunk: of the parts before, of all
 
-  __device__ __forceinline__ Chain(const ScanChain& c, const ScanShape& p, ScanShared<Tl>& sh, int order, int tile)
-      : c(c), p(p), sh(sh), order(order), tile(tile), ch(threadIdx.x % Tl::COLS), part(threadIdx.x / Tl::COLS), col(tile * Tl::COLS + ch) {}
-
+  __device__ __forceinline__ Chain(const ScanChain& c, const ScanShape& p, ScanShared<Tl>& sh, int order, int tile) : c(c), p(p), sh(sh), order(order), tile(tile) {
+    const int lane = threadIdx.x & 31;
+    ch = (threadIdx.x >> 5) * Tl::WARP_COLS + lane % Tl::WARP_COLS;
+    part = lane / Tl::WARP_COLS;
+    col = tile * Tl::COLS + ch;
+  }
   __device__ __forceinline__ float2* run_at(int k) const { return c.runs + static_cast<long long>(k) * p.channels + col; }
   __device__ __forceinline__ float* state_at(int g) const { return c.states + static_cast<long long>(g) * p.channels + col; }
-  __device__ __forceinline__ int* flag_at(int k) const { return c.flags + static_cast<long long>(k) * c.tiles + tile; }
-  __device__ __forceinline__ int* group_flag_at(int g) const { return c.flags + static_cast<long long>(c.chunks + g) * c.tiles + tile; }
-  // a flag counts the warps that have left their channels
-  static constexpr int kWarps = Tl::COLS / 32;
-  __device__ __forceinline__ void leave(int* flag) const {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) { __threadfence(); red_release_gpu_add(flag, 1); }
+
+  // `run` of each part becomes that of all parts up to it.
+  __device__ __forceinline__ Run join_parts(Run run) const {
+#pragma unroll
+    for (int d = Tl::WARP_COLS; d < 32; d *= 2) {
+      const Run prev = {__shfl_up_sync(0xffffffffu, run.a, d), __shfl_up_sync(0xffffffffu, run.b, d)};
+      if (static_cast<int>(threadIdx.x & 31) >= d) run = join(prev, run);
+    }
+    return run;
   }
-  __device__ __forceinline__ bool wait(int* flag, int what) const {
-    const bool ok = spin_until([&] { return ld_acquire_gpu(flag) >= kWarps; }, p.wait_budget_ns, p.status);
-    if (!ok) report_failure(p.status, kStatusTimeoutPipeline, kKernelScan, 0, p.rank, order, what, tile);
-    return ok;
+  __device__ __forceinline__ static Run of_last_part(Run run) {
+    const int from = 32 - Tl::WARP_COLS + static_cast<int>(threadIdx.x & 31) % Tl::WARP_COLS;
+    return {__shfl_sync(0xffffffffu, run.a, from), __shfl_sync(0xffffffffu, run.b, from)};
   }
 
-  // From the runs of the piles in shared memory (in order): each becomes the run of the piles before it in its part; sh.before: of the parts before.
-  // Leaves the whole chunk's run to the chunks behind, and returns it.
+  // From the runs of the piles in shared memory (in order): each becomes the run of the piles before it in its part.  Leaves the whole chunk's run
+  // to the chunks behind.
   template <class RunAt>
-  __device__ __forceinline__ Run join_piles(RunAt run_in_smem) {
-    __syncthreads();
+  __device__ __forceinline__ void join_piles(RunAt run_in_smem) {
     Run run = nothing();
 #pragma unroll
     for (int i = 0; i < Tl::PART_PILES; ++i) {
@@ -277,56 +300,47 @@ struct Chain {
       *at = make_float2(run.a, run.b);
       run = join(run, Run{v.x, v.y});
     }
-    sh.parts[part][ch] = run;
-    __syncthreads();
-    Run whole = nothing(), mine = nothing();
-#pragma unroll
-    for (int i = 0; i < Tl::PARTS; ++i) {
-      if (i == part) mine = whole;
-      whole = join(whole, sh.parts[i][ch]);
-    }
-    sh.before[part][ch] = mine;                  // (read by this thread alone)
-    if (part == 0 && c.ticket != nullptr) {
-      if (col < p.channels) __stcg(run_at(order), make_float2(whole.a, whole.b));
-      leave(flag_at(order));
-    }
-    return whole;
+    run = join_parts(run);
+    before = {__shfl_up_sync(0xffffffffu, run.a, Tl::WARP_COLS), __shfl_up_sync(0xffffffffu, run.b, Tl::WARP_COLS)};
+    if (part == 0) before = nothing();
+    whole = of_last_part(run);
+    if (part == 0 && col < p.channels && c.ticket != nullptr) leave(run_at(order), whole);
   }
 
   // The state in front of this chunk, of a sequence that starts in chunk `from` (in this order).
   __device__ __forceinline__ float state_before(int from) {
     const int group = order / kScanGroup, group_start = group * kScanGroup;
-    const bool whole = from < group_start;
-    const int start = whole ? group_start : from, n = order - start;
-    const int begin = start + n * part / Tl::PARTS, end = start + n * (part + 1) / Tl::PARTS, lane = threadIdx.x & 31;
+    const bool handed = from < group_start;
+    const int start = handed ? group_start : from, n = max(order - start, 0);
+    const int begin = start + n * part / Tl::PARTS, count = start + n * (part + 1) / Tl::PARTS - begin;
+    constexpr int kMost = kScanGroup / Tl::PARTS;              // (n is less than kScanGroup)
+    uint2 got[kMost];
+    uint32_t state = 0;
     bool ok = true;
-    if (lane < end - begin) ok = wait(flag_at(begin + lane), begin + lane);
-    if (lane == 31 && whole) ok = wait(group_flag_at(group - 1), group) && ok;
-    ok = __all_sync(0xffffffffu, ok);
-    const bool in = col < p.channels;
-    float state = whole && in ? __ldcg(state_at(group - 1)) : 0.f;
+    if (col < p.channels) {
+      ok = spin_until([&] {
+        bool all = true;
+        if (handed) { state = look(state_at(group - 1)); all = state != kAbsent; }
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) if (i < count) got[i] = look(run_at(begin + i));
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) if (i < count) all = all && got[i].x != kAbsent;
+        return all;
+      }, p.wait_budget_ns, p.status);
+      if (!ok) report_failure(p.status, kStatusTimeoutPipeline, kKernelScan, 0, p.rank, order, begin, tile);
+    }
     Run run = nothing();
-    if (in) {
-#pragma unroll 8
-      for (int k = begin; k < end; ++k) {
-        const float2 v = __ldcg(run_at(k));
-        run = join(run, Run{v.x, v.y});
-      }
+    if (col < p.channels) {
+#pragma unroll
+      for (int i = 0; i < kMost; ++i) if (i < count) run = join(run, Run{__uint_as_float(got[i].x), __uint_as_float(got[i].y)});
     }
     if (!ok) run = {-0.f, __int_as_float(0x7fc00000)};
-    sh.folds[part][ch] = run;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < Tl::PARTS; ++i) state = apply(sh.folds[i][ch], state);
-    return state;
+    return apply(of_last_part(join_parts(run)), __uint_as_float(state));
   }
   // The state behind the chunk goes to the group behind; the state in front of each part to the block's threads.
-  __device__ __forceinline__ void spread(Run whole, float state) {
-    if (part == 0 && c.ticket != nullptr && order % kScanGroup == kScanGroup - 1) {
-      if (col < p.channels) __stcg(state_at(order / kScanGroup), apply(whole, state));
-      leave(group_flag_at(order / kScanGroup));
-    }
-    sh.carry[part][ch] = apply(sh.before[part][ch], state);
+  __device__ __forceinline__ void spread(float state) {
+    if (part == 0 && col < p.channels && c.ticket != nullptr && order % kScanGroup == kScanGroup - 1) leave(state_at(order / kScanGroup), apply(whole, state));
+    sh.carry[part][ch] = apply(before, state);
     __syncthreads();
   }
   // The state in front of this thread's pile.
@@ -361,10 +375,14 @@ __device__ __forceinline__ void empty_sequences(const ScanShape& p, const ScanCh
   }
 }
 
-// The first unit of a block.
+// The first unit of a block; thread 0 has the next one in hand, and claims the one after it when it gives that out.  (No block has a second
+// unit where there is one for each.)
+__device__ __forceinline__ int claim(const ScanChain& c, int units) {
+  return c.ticket != nullptr && units > static_cast<int>(gridDim.x) ? atomicAdd(c.ticket, 1) + 1 : units;
+}
 __device__ __forceinline__ int first_unit(const ScanChain& c, int* next) {
   if (c.ticket == nullptr) return blockIdx.x;
-  if (threadIdx.x == 0) *next = atomicAdd(c.ticket, 1);
+  if (threadIdx.x == 0) *next = atomicAdd(c.ticket, 1) + 1;
   __syncthreads();
   const int unit = *next;
   __syncthreads();
@@ -380,7 +398,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_forward_kernel(const Sca
   __shared__ ScanShared<Tl> sh;
   const int side = threadIdx.x % Tl::LANES, pile = threadIdx.x / Tl::LANES, units = c.chunks * c.tiles;
   auto array = [&](int buffer, int which) { return space + (buffer * 2 + which) * Tl::ARRAY; };
-  auto place = [&](int buffer, int which, int r) { return array(buffer, which) + r * Tl::PITCH + threadIdx.x * Tl::SLOT; };
+  auto place = [&](int buffer, int which, int r) { return array(buffer, which) + r * Tl::PITCH + Tl::slot(threadIdx.x); };
   auto issue = [&](int unit, int buffer) {
     if (unit < units) {
       const int chunk = unit / c.tiles, tile = unit - chunk * c.tiles, row0 = chunk * Tl::ROWS, col = tile * Tl::COLS + side * V;
@@ -395,8 +413,9 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_forward_kernel(const Sca
     }
     fetch_commit();
   };
-  int unit = first_unit(c, &sh.next), buffer = 0;
+  int claimed = units, buffer = 0, unit = first_unit(c, &sh.next);
   issue(unit, 0);
+  if (threadIdx.x == 0) claimed = claim(c, units);
   __syncthreads();
   for (; unit < units; buffer ^= 1) {
     const int chunk = unit / c.tiles, tile = unit - chunk * c.tiles;
@@ -405,7 +424,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_forward_kernel(const Sca
     const int* seq = sh.seq[buffer];
     auto run_at = [&](int pile_order, int ch) { return Tl::run_at(array(buffer, 0), space + 4 * Tl::ARRAY, pile_order, ch); };
     empty_sequences<Tl>(p, c, chunk, tile, p.initial, p.final_state, true);
-    if (c.ticket != nullptr && threadIdx.x == 0) sh.next = atomicAdd(c.ticket, 1);
+    if (threadIdx.x == 0) sh.next = claimed;
     fetch_wait<0>();
 
     Row<V> keep[R], add[R];                      // h -> keep h + add
@@ -431,12 +450,14 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_forward_kernel(const Sca
       for (int i = 0; i < V; ++i) *reinterpret_cast<float2*>(run_at(pile, side * V + i)) = make_float2(fa[i], fb[i]);
     }
     Chain<Tl> chain(c, p, sh, chunk, tile);
-    const Run whole = chain.join_piles(run_at);
-    const int next = c.ticket != nullptr ? sh.next : units;
+    __syncthreads();
+    const int next = sh.next;
+    if (threadIdx.x == 0 && next < units) claimed = claim(c, units);
+    chain.join_piles(run_at);
     issue(next, buffer ^ 1);
     float state = 0.f;
     if (seq[1] >= 0 && seq[1] == seq[0]) state = chain.state_before(static_cast<int>(max(first_row(p, seq[1]), 0ll) / Tl::ROWS));
-    chain.spread(whole, state);
+    chain.spread(state);
 
     Row<V> h = chain.state_of_pile(run_at, pile, side);
 #pragma unroll
@@ -463,7 +484,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(const Sc
   __shared__ ScanShared<Tl> sh;
   const int side = threadIdx.x % Tl::LANES, pile_order = threadIdx.x / Tl::LANES, pile = Tl::PILES - 1 - pile_order, units = c.chunks * c.tiles;
   auto array = [&](int buffer, int which) { return space + (buffer * 2 + which) * Tl::ARRAY; };
-  auto place = [&](int buffer, int which, int r) { return array(buffer, which) + r * Tl::PITCH + threadIdx.x * Tl::SLOT; };
+  auto place = [&](int buffer, int which, int r) { return array(buffer, which) + r * Tl::PITCH + Tl::slot(threadIdx.x); };
   auto issue = [&](int unit, int buffer) {
     if (unit < units) {
       const int order = unit / c.tiles, tile = unit - order * c.tiles, row0 = (c.chunks - 1 - order) * Tl::ROWS, col = tile * Tl::COLS + side * V;
@@ -492,9 +513,10 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(const Sc
     }
     fetch_commit();
   };
-  int unit = first_unit(c, &sh.next), buffer = 0;
+  int claimed = units, buffer = 0, unit = first_unit(c, &sh.next);
   issue(unit, 0);
   issue_late(unit);
+  if (threadIdx.x == 0) claimed = claim(c, units);
   __syncthreads();
   for (; unit < units; buffer ^= 1) {
     const int order = unit / c.tiles, tile = unit - order * c.tiles, chunk = c.chunks - 1 - order;
@@ -503,7 +525,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(const Sc
     const int* seq = sh.seq[buffer];
     auto run_at = [&](int order_of_pile, int ch) { return Tl::run_at(array(buffer, 0), space + 6 * Tl::ARRAY, order_of_pile, ch); };
     empty_sequences<Tl>(p, c, order, tile, p.dfinal, p.dinitial, false);
-    if (c.ticket != nullptr && threadIdx.x == 0) sh.next = atomicAdd(c.ticket, 1);
+    if (threadIdx.x == 0) sh.next = claimed;
     fetch_wait<1>();
 
     Row<V> keep[R], take[R];
@@ -528,8 +550,10 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(const Sc
       for (int i = 0; i < V; ++i) *reinterpret_cast<float2*>(run_at(pile_order, side * V + i)) = make_float2(fa[i], fb[i]);
     }
     Chain<Tl> chain(c, p, sh, order, tile);
-    const Run whole = chain.join_piles(run_at);
-    const int next = c.ticket != nullptr ? sh.next : units;
+    __syncthreads();
+    const int next = sh.next;
+    if (threadIdx.x == 0 && next < units) claimed = claim(c, units);
+    chain.join_piles(run_at);
     issue(next, buffer ^ 1);
     const int last = seq[Tl::ROWS];
     float state = 0.f;
@@ -537,7 +561,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_kernel(const Sc
       const long long end = min(max(first_row(p, last + 1), 1ll), static_cast<long long>(p.rows)) - 1;      // the sequence's last row
       state = chain.state_before(max(c.chunks - 1 - static_cast<int>(end / Tl::ROWS), 0));
     }
-    chain.spread(whole, state);
+    chain.spread(state);
 
     Row<V> back = chain.state_of_pile(run_at, pile_order, side);                   // keep_{t+1} g_{t+1}
     fetch_wait<1>();
@@ -608,17 +632,14 @@ auto by_tile(bool half, bool vectors, F f) {
   return vectors ? f(Tile<float, 4>{}) : f(Tile<float, 1>{});
 }
 
-// Where the parts of the workspace lie.
+// Where the parts of the workspace lie.  The ticket counts up from -1, as all of it is filled.
 cudaError_t lay_out(ScanChain& c, const ScanPlan& s, int channels, void* space, cudaStream_t stream) {
   c.chunks = s.chunks; c.tiles = s.tiles;
   if (s.chunks == 1) return cudaSuccess;
-  const int groups = (s.chunks + kScanGroup - 1) / kScanGroup;
   c.ticket = static_cast<int*>(space);
-  c.flags = c.ticket + 4;
-  const size_t ints = 4 + static_cast<size_t>(s.chunks + groups) * s.tiles;
-  c.runs = reinterpret_cast<float2*>(c.ticket + (ints + 3) / 4 * 4);
+  c.runs = reinterpret_cast<float2*>(c.ticket + 4);
   c.states = reinterpret_cast<float*>(c.runs + static_cast<size_t>(s.chunks) * channels);
-  return cudaMemsetAsync(space, 0, ints * sizeof(int), stream);
+  return cudaMemsetAsync(space, 0xff, static_cast<size_t>(scan_space(s, channels)), stream);
 }
 
 }  // namespace
@@ -628,7 +649,7 @@ ScanPlan scan_plan(const ScanGradParams& p) { return by_tile(p.half, whole_vecto
 long long scan_space(const ScanPlan& s, int channels) {
   if (s.chunks == 1) return 0;
   const long long groups = (s.chunks + kScanGroup - 1) / kScanGroup;
-  return 32 + 4 * (s.chunks + groups) * s.tiles + 8ll * s.chunks * channels + 4ll * groups * channels;
+  return 16 + 8ll * s.chunks * channels + 4ll * groups * channels;
 }
 
 namespace {
