@@ -38,17 +38,15 @@ ScanShape shape_of(const at::Tensor& offsets, const at::Tensor& x, const at::Ten
   p.x = xr.data_ptr(); p.x_stride = xr.stride(0);
   p.gate = gr.data_ptr(); p.gate_stride = gr.stride(0);
   p.initial = initial.defined() ? initial.data_ptr<float>() : nullptr;
-  p.status = ctx.status; p.rank = ctx.rank; p.wait_budget_ns = ctx.wait_budget_ns;
+  p.status = ctx.status; p.rank = ctx.rank;
   return p;
 }
 
-template <class Params>
-at::Tensor workspace(const Params& p, const at::Tensor& like) {
-  const ScanPlan plan = scan_plan(p);
-  SEP_ASSERT(static_cast<int64_t>(plan.chunks) * plan.tiles < (1ll << 30), "this recurrence has too many rows and channels for one call");
-  const int64_t bytes = scan_space(plan, p.channels);
+at::Tensor workspace(const ScanSplit& split, int channels, const at::Tensor& like) {
+  const int64_t bytes = scan_space(split, channels);
   return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
 }
+void* pointer(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 ScanResult scan_forward(const ScanCall& call, const at::Tensor& x, const at::Tensor& gate, const at::Tensor& initial, const at::Tensor& offsets,
                         bool want_state) {
@@ -62,8 +60,9 @@ ScanResult scan_forward(const ScanCall& call, const at::Tensor& x, const at::Ten
   if (p.sequences == 0) { out.h.zero_(); return out; }
   p.h = out.h.data_ptr();
   p.final_state = want_state ? out.final_state.data_ptr<float>() : nullptr;
-  const at::Tensor space = workspace(p, x);
-  SEP_CUDA_CHECK(launch_scan_forward(p, ctx.sms, space.defined() ? space.data_ptr() : nullptr, ctx.stream));
+  const ScanSplit split = scan_split(p, ctx.sms);
+  const at::Tensor space = workspace(split, p.channels, x);
+  SEP_CUDA_CHECK(launch_scan_forward(p, split, pointer(space), ctx.stream));
   return out;
 }
 
@@ -108,8 +107,9 @@ class Scan : public torch::autograd::Function<Scan> {
       p.dx = want_dx ? dx.data_ptr() : nullptr;
       p.dgate = want_dgate ? dgate.data_ptr() : nullptr;
       p.dinitial = want_dinitial ? dinitial.data_ptr<float>() : nullptr;
-      const at::Tensor space = workspace(p, x);
-      SEP_CUDA_CHECK(launch_scan_backward(p, context.sms, space.defined() ? space.data_ptr() : nullptr, context.stream));
+      const ScanSplit split = scan_split(p, context.sms);
+      const at::Tensor space = workspace(split, p.channels, x);
+      SEP_CUDA_CHECK(launch_scan_backward(p, split, pointer(space), context.stream));
     }
     return {dx, dgate, dinitial, at::Tensor(), at::Tensor(), at::Tensor()};
   }
@@ -171,7 +171,7 @@ at::Tensor gated_scan_step(const at::Tensor& state, const at::Tensor& x, const a
   p.gate = gr.data_ptr(); p.gate_stride = gr.stride(0);
   p.state = state.data_ptr<float>(); p.state_stride = state.stride(0);
   p.h = h.data_ptr();
-  SEP_CUDA_CHECK(launch_scan_step(p, at::cuda::getCurrentDeviceProperties()->multiProcessorCount, at::cuda::getCurrentCUDAStream()));
+  SEP_CUDA_CHECK(launch_scan_step(p, at::cuda::getCurrentCUDAStream()));
   if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
   return h;
 }

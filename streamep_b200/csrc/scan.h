@@ -20,7 +20,6 @@ struct ScanShape {
   const float* initial;          // [sequences, channels] or null (zeros)
   StatusBlock* status;
   int rank;
-  unsigned long long wait_budget_ns;
 };
 struct ScanParams : ScanShape {
   void* h;                       // [rows, channels]
@@ -35,13 +34,18 @@ struct ScanGradParams : ScanShape {
   void* dgate;                   // or null
   float* dinitial;               // or null
 };
-// Chunks of rows and tiles of channels, and the bytes (from a 16-byte boundary) that blocks hand on to one another in.
-struct ScanPlan { int chunks, tiles; };
-ScanPlan scan_plan(const ScanParams& p);
-ScanPlan scan_plan(const ScanGradParams& p);
-long long scan_space(const ScanPlan& s, int channels);
-cudaError_t launch_scan_forward(const ScanParams& p, int sms, void* space, cudaStream_t stream);
-cudaError_t launch_scan_backward(const ScanGradParams& p, int sms, void* space, cudaStream_t stream);
+// How time is split: each sequence (packed ones: all rows) into `parts` segments of `rows` rows, and where more than one, the workspace of their runs.
+struct ScanSplit {
+  long long segments;            // of all sequences
+  int parts, rows;
+  float* factors;                // [segments][channels]
+  float* states;                 // [segments][channels]: sums, then the states in front of the segments
+};
+ScanSplit scan_split(const ScanParams& p, int sms);
+ScanSplit scan_split(const ScanGradParams& p, int sms);
+long long scan_space(const ScanSplit& s, int channels);        // bytes, from a 16-byte boundary on
+cudaError_t launch_scan_forward(const ScanParams& p, ScanSplit s, void* space, cudaStream_t stream);
+cudaError_t launch_scan_backward(const ScanGradParams& p, ScanSplit s, void* space, cudaStream_t stream);
 
 struct ScanStepParams {
   int half, rows, channels;
@@ -51,6 +55,6 @@ struct ScanStepParams {
   float* state;
   void* h;                       // [rows, channels]
 };
-cudaError_t launch_scan_step(const ScanStepParams& p, int sms, cudaStream_t stream);
+cudaError_t launch_scan_step(const ScanStepParams& p, cudaStream_t stream);
 
 }  // namespace sep
