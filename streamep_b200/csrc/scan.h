@@ -34,12 +34,14 @@ struct ScanGradParams : ScanShape {
   void* dgate;                   // or null
   float* dinitial;               // or null
 };
-// How time is split: each sequence (packed ones: all rows) into `parts` segments of `rows` rows, and where more than one, the workspace of their runs.
+// How time is split: each sequence (packed ones: all rows) into `parts` segments of `rows` rows, of which a block takes a number side by side; and
+// the workspace of their runs, where a sequence goes on in another block.
 struct ScanSplit {
-  long long segments;            // of all sequences
-  int parts, rows;
-  float* factors;                // [segments][channels]
-  float* states;                 // [segments][channels]: sums, then the states in front of the segments
+  int segments, parts, rows;
+  int blocks, tiles;             // of segments, of channels
+  int within;                    // 1: the segments of a sequence lie in one block
+  float *factors, *sums;         // [segments][channels]
+  float *block_factors, *block_sums;             // [blocks][channels]
 };
 ScanSplit scan_split(const ScanParams& p, int sms);
 ScanSplit scan_split(const ScanGradParams& p, int sms);

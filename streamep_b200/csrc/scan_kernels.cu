@@ -7,10 +7,12 @@
 //
 // What bounds it: memory (two arrays read and one written, four and two in the backward), and two special-function results an element.  A thread
 // walks one vector of channels through a segment of rows.  Where sequences and channels alone are threads enough, a segment is a whole
-// sequence, and one kernel does it all.  Else time is split: a first kernel forms what each segment does to the state in front of it (its run, h ->
-// a h + b), a small one joins the runs of a sequence, and the last walks the segments again from their states.  The second reading comes from L2
-// as far as that reaches.  No thread waits for another, and all is added in one order: a repeated call gives the same bits.
+// sequence, and that is all.  Else time is split: what each segment does to the state in front of it (its run, h -> a h + b) is formed first, the
+// runs of a block's segments are joined, and a second walk begins from each segment's state.  Where the segments of a sequence lie in one block, one
+// kernel does both; else a first kernel leaves the runs, and the second one's blocks join those of the blocks before.  The second reading comes
+// from L2 as far as that reaches.  No block waits for another, and all is added in one order: a repeated call gives the same bits.
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 #include <utility>
@@ -23,7 +25,6 @@ namespace sep {
 namespace {
 
 constexpr int kScanThreads = 256;
-constexpr int kJoinThreads = 512, kJoinCols = 16, kJoinParts = kJoinThreads / kJoinCols;
 
 template <class T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
@@ -208,24 +209,36 @@ __device__ __forceinline__ void store_state(float* at, const Row<V>& row) {
   }
 }
 
-// What a thread works on: V channels from `col` on, and rows [first, last) of a segment.
-template <int V>
+// A block's threads: LANES side by side across the channels, V channels each, and SEGS segments above one another.  Where runs are joined, PARTS
+// threads share a channel.
+template <int V> struct Tile {
+  static constexpr int LANES = V >= 4 ? 8 : 32;
+  static constexpr int COLS = LANES * V;
+  static constexpr int SEGS = kScanThreads / LANES;
+  static constexpr int PARTS = kScanThreads / COLS;
+  static_assert(SEGS % PARTS == 0, "parts of equal length");
+};
+
+// What a thread works on: V channels from `col` on, and rows [first, last) of a segment.  `order` counts segments from where the recurrence starts:
+// the first one, or with kBack the last one.
+template <int V, bool kBack>
 struct Segment {
-  long long index;               // of the segment
-  int sequence, part, col, first, last;
+  int order, index, sequence, part, col, first, last;
   bool there;
-  __device__ __forceinline__ Segment(const ScanShape& p, const ScanSplit& s, long long thread) {
-    const int vectors = p.channels / V;
-    index = thread / vectors;
-    col = static_cast<int>(thread - index * vectors) * V;
-    there = index < s.segments;
-    sequence = static_cast<int>(index / s.parts);
-    part = static_cast<int>(index - static_cast<long long>(sequence) * s.parts);
+  __device__ __forceinline__ Segment(const ScanShape& p, const ScanSplit& s, int block, int tile) {
+    order = block * Tile<V>::SEGS + static_cast<int>(threadIdx.x) / Tile<V>::LANES;
+    col = tile * Tile<V>::COLS + static_cast<int>(threadIdx.x) % Tile<V>::LANES * V;
+    there = order < s.segments && col < p.channels;
+    index = kBack ? s.segments - 1 - order : order;
+    sequence = index / s.parts;
+    part = index - sequence * s.parts;
+    if (order >= s.segments) { first = last = 0; return; }
     const int base = p.offsets == nullptr ? sequence * p.length : 0, end = p.offsets == nullptr ? base + p.length : p.rows;
     first = min(base + part * s.rows, end);
     last = min(first + s.rows, end);
   }
 };
+
 // Rows that are on their way while one is worked on: in places of the thread's own in shared memory, filled by asynchronous copies (nobody waits for
 // anybody else's), as many as 48 KB a block hold.  bf16 channels taken one by one, 2 bytes, come through registers.
 template <class T, int V> constexpr bool by_copies() { return V * sizeof(T) >= 4; }
@@ -302,95 +315,167 @@ __device__ __forceinline__ void walk_rows(int first, int last, const T* (&base)[
   }
 }
 
-// The runs of all segments but each sequence's last one (first one, in the backward), whose run nobody asks for.
+// What the rows of a segment do to the state in front of them.  `rows`: x, or the rows' own gradients (which may be left out).
 template <class T, int V, bool kBack>
-__global__ void __launch_bounds__(kScanThreads) scan_runs_kernel(const ScanShape p, const ScanSplit s, const void* rows, long long rows_stride, const float* edge) {
-  grid_release();
-  const Segment<V> seg(p, s, static_cast<long long>(blockIdx.x) * kScanThreads + threadIdx.x);
-  if (!seg.there || seg.part == (kBack ? 0 : s.parts - 1)) return;
-  Row<V> a = Row<V>::all(1.f), b = Row<V>::all(0.f);
+__device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSplit& s, const Segment<V, kBack>& seg, const void* rows, long long rows_stride, const float* edge,
+                                               Row<V>& a, Row<V>& b) {
+  a = Row<V>::all(1.f); b = Row<V>::all(0.f);
   auto begin = [&](int sequence) {
     a = Row<V>::all(-0.f);
     b = edge != nullptr && sequence >= 0 ? load_state<V>(edge + static_cast<long long>(sequence) * p.channels + seg.col) : Row<V>::all(0.f);
   };
+  const bool none = kBack && rows == nullptr;
   auto take_row = [&](const Raw<T, V> (&row)[2]) {
     Row<V> keep, take;
     gates_of<T, V>(row[0].get(), keep, take);
     a = a * keep;
-    b = kBack ? keep * (b + row[1].get()) : fused(keep, b, take * row[1].get());
+    if constexpr (kBack) b = keep * (none ? b : b + row[1].get()); else b = fused(keep, b, take * row[1].get());
   };
-  const T* base[2] = {static_cast<const T*>(p.gate) + seg.col, static_cast<const T*>(rows != nullptr ? rows : p.gate) + seg.col};
-  const long long stride[2] = {p.gate_stride, rows != nullptr ? rows_stride : p.gate_stride};
-  const bool none = rows == nullptr;             // (a backward without the rows' own gradients)
+  const T* base[2] = {static_cast<const T*>(p.gate) + seg.col, static_cast<const T*>(none ? p.gate : rows) + seg.col};
+  const long long stride[2] = {p.gate_stride, none ? p.gate_stride : rows_stride};
   const bool dense = p.offsets == nullptr;
   if (dense || within_one(p, kBack ? seg.first : seg.first - 1, kBack ? seg.last + 1 : seg.last)) {
     if (dense && seg.part == (kBack ? s.parts - 1 : 0)) begin(seg.sequence);
-    if (none) {
-      walk_rows<T, V, kBack, 2>(seg.first, seg.last, base, stride, [&](int, Raw<T, V> (&row)[2]) {
-        Row<V> keep, take;
-        gates_of<T, V>(row[0].get(), keep, take);
-        a = a * keep;
-        b = keep * b;
-      });
-    } else {
-      walk_rows<T, V, kBack, 2>(seg.first, seg.last, base, stride, [&](int, Raw<T, V> (&row)[2]) { take_row(row); });
-    }
+    walk_rows<T, V, kBack, 2>(seg.first, seg.last, base, stride, [&](int, Raw<T, V> (&row)[2]) { take_row(row); });
   } else {
     SequenceWalk walk(p, kBack ? seg.last : seg.first - 1);
     int previous = walk.at(p, kBack ? seg.last : seg.first - 1);
     walk_rows<T, V, kBack, 2>(seg.first, seg.last, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
       const int sequence = walk.at(p, t);
       if (sequence != previous || sequence < 0) begin(sequence);
-      if (sequence >= 0) {
-        if (none) {
-          Row<V> keep, take;
-          gates_of<T, V>(row[0].get(), keep, take);
-          a = a * keep;
-          b = keep * b;
-        } else {
-          take_row(row);
-        }
-      }
+      if (sequence >= 0) take_row(row);
       previous = sequence;
     });
   }
-  const long long at = seg.index * p.channels + seg.col;
-  store_state<V>(s.factors + at, a);
-  store_state<V>(s.states + at, b);
 }
 
-// The states in front of the segments of a sequence (of all rows, for packed ones) from their runs, in place of the runs' sums.  Each of the parts of a
-// block joins a stretch of segments of 16 channels.
-template <bool kBack>
-__global__ void __launch_bounds__(kJoinThreads) scan_join_kernel(const ScanSplit s, int channels) {
-  __shared__ Run stretch[kJoinParts][kJoinCols];
-  grid_release();
-  grid_wait();
-  const int ch = threadIdx.x % kJoinCols, part = threadIdx.x / kJoinCols, col = blockIdx.x * kJoinCols + ch;
-  const bool in = col < channels;
-  const int n = s.parts - 1;                     // the state in front of the last is what all runs before it come to
-  const int begin = static_cast<int>(static_cast<long long>(n) * part / kJoinParts), end = static_cast<int>(static_cast<long long>(n) * (part + 1) / kJoinParts);
-  for (long long q = blockIdx.y; q < s.segments / s.parts; q += gridDim.y) {
-    auto at = [&](int i) { return (q * s.parts + (kBack ? s.parts - 1 - i : i)) * channels + col; };
-    Run run = nothing();
-    if (in) {
-#pragma unroll 8
-      for (int i = begin; i < end; ++i) run = join(run, Run{s.factors[at(i)], s.states[at(i)]});
-    }
-    __syncthreads();             // (the stretches of the sequence before have been read)
-    stretch[part][ch] = run;
-    __syncthreads();
-    if (!in) continue;
-    float state = 0.f;
-    for (int i = 0; i < part; ++i) state = apply(stretch[i][ch], state);
-#pragma unroll 4
-    for (int i = begin; i < end; ++i) {
-      const Run r = {s.factors[at(i)], s.states[at(i)]};
-      s.states[at(i)] = state;
-      state = apply(r, state);
-    }
-    if (part == kJoinParts - 1) s.states[at(n)] = state;
+// From the runs of a block's segments: of those before each thread's own.  All threads call; the ring is not in use.
+template <int V>
+__device__ __forceinline__ void runs_before(Row<V> a, Row<V> b, Run (&before)[V]) {
+  using Tl = Tile<V>;
+  extern __shared__ __align__(16) unsigned char ring[];
+  Run* runs = reinterpret_cast<Run*>(ring);                    // [SEGS][COLS]
+  __shared__ Run parts[Tl::PARTS][Tl::COLS];
+  const int seg = threadIdx.x / Tl::LANES, side = threadIdx.x % Tl::LANES;
+  float fa[V], fb[V];
+  a.get(fa); b.get(fb);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < V; ++i) runs[seg * Tl::COLS + side * V + i] = Run{fa[i], fb[i]};
+  __syncthreads();
+  const int ch = threadIdx.x % Tl::COLS, part = threadIdx.x / Tl::COLS;
+  constexpr int kEach = Tl::SEGS / Tl::PARTS;
+  Run run = nothing();
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    Run* at = runs + (part * kEach + i) * Tl::COLS + ch;
+    const Run r = *at;
+    *at = run;
+    run = join(run, r);
   }
+  parts[part][ch] = run;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    run = nothing();
+#pragma unroll
+    for (int q = 0; q < Tl::PARTS; ++q)
+      if (q < seg / kEach) run = join(run, parts[q][side * V + i]);
+    before[i] = join(run, runs[seg * Tl::COLS + side * V + i]);
+  }
+  __syncthreads();               // the ring may be filled again
+}
+
+// Leaves, of every segment, the run of the segments before it in its block; and of every block the run of all.
+template <class T, int V, bool kBack>
+__global__ void __launch_bounds__(kScanThreads, 3) scan_runs_kernel(const ScanShape p, const ScanSplit s, const void* rows, long long rows_stride, const float* edge) {
+  using Tl = Tile<V>;
+  grid_release();
+  const int block = blockIdx.x / s.tiles, tile = blockIdx.x - block * s.tiles;
+  const Segment<V, kBack> seg(p, s, block, tile);
+  Row<V> a = Row<V>::all(1.f), b = Row<V>::all(0.f);
+  if (seg.there) run_of_segment<T, V, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
+  Run before[V];
+  runs_before<V>(a, b, before);
+  if (!seg.there) return;
+  float fa[V], fb[V];
+  const long long at = static_cast<long long>(seg.order) * p.channels + seg.col;
+#pragma unroll
+  for (int i = 0; i < V; ++i) { fa[i] = before[i].a; fb[i] = before[i].b; }
+  store_state<V>(s.factors + at, Row<V>::of(fa));
+  store_state<V>(s.sums + at, Row<V>::of(fb));
+  if (seg.order % Tl::SEGS != Tl::SEGS - 1) return;            // (nobody follows a block that is not full)
+  float ga[V], gb[V];
+  a.get(ga); b.get(gb);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const Run r = join(before[i], Run{ga[i], gb[i]});
+    ga[i] = r.a; gb[i] = r.b;
+  }
+  const long long block_at = static_cast<long long>(block) * p.channels + seg.col;
+  store_state<V>(s.block_factors + block_at, Row<V>::of(ga));
+  store_state<V>(s.block_sums + block_at, Row<V>::of(gb));
+}
+
+// The state in front of each thread's segment.  All threads call.
+template <class T, int V, bool kBack>
+__device__ __forceinline__ Row<V> state_before(const ScanShape& p, const ScanSplit& s, const Segment<V, kBack>& seg, int block, int tile, const void* rows, long long rows_stride,
+                                               const float* edge) {
+  using Tl = Tile<V>;
+  if (s.parts == 1) return Row<V>::all(0.f);
+  if (s.within) {                                // no sequence goes on in another block
+    Row<V> a = Row<V>::all(1.f), b = Row<V>::all(0.f);
+    if (seg.there) run_of_segment<T, V, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
+    Run before[V];
+    runs_before<V>(a, b, before);
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = before[i].b;
+    return Row<V>::of(f);
+  }
+  __shared__ Run parts[Tl::PARTS][Tl::COLS];
+  const int ch = threadIdx.x % Tl::COLS, part = threadIdx.x / Tl::COLS, col = tile * Tl::COLS + ch;
+  // the first block that the sequence of this block's first segment has a part in
+  const int order0 = block * Tl::SEGS, index0 = kBack ? s.segments - 1 - order0 : order0;
+  int from = block;
+  if (p.offsets == nullptr) {
+    const int sequence = index0 / s.parts;
+    from = (kBack ? s.segments - (sequence + 1) * s.parts : sequence * s.parts) / Tl::SEGS;
+  } else {
+    const int edge_row = kBack ? min(index0 * s.rows + s.rows, p.rows) : index0 * s.rows;      // the rows on both sides of it: of one sequence?
+    SequenceWalk walk(p, edge_row - 1);
+    const int i = walk.at(p, edge_row - 1);
+    if (i >= 0 && walk.all_within(p, edge_row + 1)) {
+      const long long far = kBack ? min(max(walk.behind, 1ll), static_cast<long long>(p.rows)) - 1 : max(walk.first, 0ll);
+      const int segment = static_cast<int>(far / s.rows);
+      from = (kBack ? s.segments - 1 - segment : segment) / Tl::SEGS;
+    }
+  }
+  const int n = max(block - from, 0), begin = from + n * part / Tl::PARTS, end = from + n * (part + 1) / Tl::PARTS;
+  Run run = nothing();
+  if (col < p.channels) {
+#pragma unroll 8
+    for (int k = begin; k < end; ++k) {
+      const long long at = static_cast<long long>(k) * p.channels + col;
+      run = join(run, Run{s.block_factors[at], s.block_sums[at]});
+    }
+  }
+  parts[part][ch] = run;
+  __syncthreads();
+  if (!seg.there) return Row<V>::all(0.f);
+  const int side = threadIdx.x % Tl::LANES;
+  const long long at = static_cast<long long>(seg.order) * p.channels + seg.col;
+  float fa[V], fb[V], f[V];
+  load_state<V>(s.factors + at).get(fa);
+  load_state<V>(s.sums + at).get(fb);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float state = 0.f;
+#pragma unroll
+    for (int q = 0; q < Tl::PARTS; ++q) state = apply(parts[q][side * V + i], state);
+    f[i] = apply(Run{fa[i], fb[i]}, state);
+  }
+  return Row<V>::of(f);
 }
 
 // Sequences without rows hand their state on (`from` to `to`); offsets that are none are reported.
@@ -415,13 +500,14 @@ __device__ __forceinline__ void empty_sequences(const ScanShape& p, const float*
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(const ScanParams p, const ScanSplit s) {
+__global__ void __launch_bounds__(kScanThreads, 3) scan_forward_kernel(const ScanParams p, const ScanSplit s) {
   grid_wait();
   empty_sequences<V>(p, p.initial, p.final_state, true);
-  // (from the last segment: what was read last is still in L2)
-  const Segment<V> seg(p, s, static_cast<long long>(gridDim.x - 1 - blockIdx.x) * kScanThreads + threadIdx.x);
+  // (from the last block: what was read last is still in L2)
+  const int unit = gridDim.x - 1 - blockIdx.x, block = unit / s.tiles, tile = unit - block * s.tiles;
+  const Segment<V, false> seg(p, s, block, tile);
+  Row<V> h = state_before<T, V, false>(p, s, seg, block, tile, p.x, p.x_stride, p.initial);
   if (!seg.there) return;
-  Row<V> h = Row<V>::all(0.f);
   auto state_at = [&](int sequence) { return static_cast<long long>(sequence) * p.channels + seg.col; };
   auto begin = [&](int sequence) { h = p.initial != nullptr ? load_state<V>(p.initial + state_at(sequence)) : Row<V>::all(0.f); };
   auto step = [&](const Raw<T, V> (&row)[2]) {
@@ -432,7 +518,6 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(const ScanPa
   const T* base[2] = {static_cast<const T*>(p.gate) + seg.col, static_cast<const T*>(p.x) + seg.col};
   const long long stride[2] = {p.gate_stride, p.x_stride};
   T* out = static_cast<T*>(p.h) + seg.col;
-  if (s.parts > 1 && seg.part > 0) h = load_state<V>(s.states + seg.index * p.channels + seg.col);
   const bool dense = p.offsets == nullptr;
   if (dense || within_one(p, seg.first - 1, seg.last + 1)) {
     if (dense && seg.part == 0) begin(seg.sequence);
@@ -462,12 +547,13 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(const ScanPa
 
 // kGate: with the gate's gradient, for which x and h of the row before are read too.
 template <class T, int V, bool kGate>
-__global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(const ScanGradParams p, const ScanSplit s) {
+__global__ void __launch_bounds__(kScanThreads, 3) scan_backward_kernel(const ScanGradParams p, const ScanSplit s) {
   grid_wait();
   empty_sequences<V>(p, p.dfinal, p.dinitial, false);
-  const Segment<V> seg(p, s, static_cast<long long>(gridDim.x - 1 - blockIdx.x) * kScanThreads + threadIdx.x);
+  const int unit = gridDim.x - 1 - blockIdx.x, block = unit / s.tiles, tile = unit - block * s.tiles;
+  const Segment<V, true> seg(p, s, block, tile);
+  Row<V> back = state_before<T, V, true>(p, s, seg, block, tile, p.dh, p.dh_stride, p.dfinal);     // keep_{t+1} g_{t+1}
   if (!seg.there) return;
-  Row<V> back = Row<V>::all(0.f);                // keep_{t+1} g_{t+1}
   auto state_at = [&](int sequence) { return static_cast<long long>(sequence) * p.channels + seg.col; };
   const bool none = p.dh == nullptr;
   // one row, whose state before is h
@@ -488,7 +574,6 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(const ScanG
   };
   auto begin = [&](int sequence) { back = p.dfinal != nullptr ? load_state<V>(p.dfinal + state_at(sequence)) : Row<V>::all(0.f); };
   auto initial = [&](int sequence) { return p.initial != nullptr ? load_state<V>(p.initial + state_at(sequence)) : Row<V>::all(0.f); };
-  if (s.parts > 1 && seg.part < s.parts - 1) back = load_state<V>(s.states + seg.index * p.channels + seg.col);
 
   constexpr int kArrays = kGate ? 4 : 2;
   const T* gate = static_cast<const T*>(p.gate) + seg.col;
@@ -595,6 +680,7 @@ ScanSplit split_of(const ScanShape& p, int vec, int sms) {
   ScanSplit s{};
   const long long sequences = p.offsets == nullptr ? p.sequences : 1, length = p.offsets == nullptr ? p.length : p.rows;
   const long long vectors = p.channels / vec;
+  const int lanes = vec >= 4 ? 8 : 32, segs = kScanThreads / lanes;
   // Threads that are enough to keep memory busy; and rows of a segment.
   const long long enough = static_cast<long long>(sms) * (vec >= 4 ? 384 : 1536);
   long long parts = 1;
@@ -602,15 +688,27 @@ ScanSplit split_of(const ScanShape& p, int vec, int sms) {
   s.rows = static_cast<int>((length + parts - 1) / parts);
   if (s.rows < 1) s.rows = 1;
   s.parts = static_cast<int>(length > 0 ? (length + s.rows - 1) / s.rows : 1);
-  s.segments = sequences * s.parts;
+  s.segments = static_cast<int>(sequences * s.parts);
+  s.tiles = static_cast<int>((vectors + lanes - 1) / lanes);
+  s.blocks = (s.segments + segs - 1) / segs;
+  s.within = s.blocks <= 1 || segs % s.parts == 0;
   return s;
 }
 
-template <class... Params, class... Args>
-cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, bool early, cudaStream_t stream, Args... args) {
+template <auto kKernel, class... Args>
+cudaError_t launch(dim3 grid, int smem, bool early, cudaStream_t stream, const Args&... args) {
+  static std::atomic<bool> configured[64];       // the shared-memory limit is an attribute of the function on a device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (smem > 0 && !configured[dev].load(std::memory_order_acquire)) {
+    if ((e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+    configured[dev].store(true, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = dim3(kScanThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -618,58 +716,51 @@ cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = early ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
-}
-unsigned blocks_of(const ScanShape& p, const ScanSplit& s, int vec) {
-  const long long threads = s.segments * (p.channels / vec);
-  return static_cast<unsigned>(std::max<long long>(1, (threads + kScanThreads - 1) / kScanThreads));
-}
-template <bool kBack>
-cudaError_t launch_join(const ScanSplit& s, int channels, cudaStream_t stream) {
-  const dim3 grid((channels + kJoinCols - 1) / kJoinCols, static_cast<unsigned>(std::min<long long>(s.segments / s.parts, 65535)));
-  return launch(scan_join_kernel<kBack>, grid, kJoinThreads, 0, true, stream, s, channels);
+  return cudaLaunchKernelEx(&cfg, kKernel, args...);
 }
 void lay_out(ScanSplit& s, int channels, void* space) {
   s.factors = static_cast<float*>(space);
-  s.states = s.factors + s.segments * channels;
+  s.sums = s.factors + static_cast<long long>(s.segments) * channels;
+  s.block_factors = s.sums + static_cast<long long>(s.segments) * channels;
+  s.block_sums = s.block_factors + static_cast<long long>(s.blocks) * channels;
+}
+// Blocks of the walks: their ring, or the runs in its place.
+template <class T, int V, int kArrays> constexpr int walk_bytes() {
+  return std::max(ring_bytes<T, V, kArrays>(), Tile<V>::SEGS * Tile<V>::COLS * static_cast<int>(sizeof(Run)));
 }
 
 }  // namespace
 
 ScanSplit scan_split(const ScanParams& p, int sms) { return split_of(p, vector_of(p), sms); }
 ScanSplit scan_split(const ScanGradParams& p, int sms) { return split_of(p, vector_of(p), sms); }
-long long scan_space(const ScanSplit& s, int channels) { return s.parts > 1 ? 8 * s.segments * channels : 0; }
+long long scan_space(const ScanSplit& s, int channels) { return s.within ? 0 : 8ll * (static_cast<long long>(s.segments) + s.blocks) * channels; }
 
 cudaError_t launch_scan_forward(const ScanParams& p, ScanSplit s, void* space, cudaStream_t stream) {
-  const int vec = vector_of(p);
-  return by_vector(p.half, vec, [&](auto type, auto v) {
+  return by_vector(p.half, vector_of(p), [&](auto type, auto v) {
     using T = decltype(type);
-    constexpr int V = decltype(v)::value;
-    const unsigned blocks = blocks_of(p, s, vec);
-    if (s.parts > 1) {
+    constexpr int V = decltype(v)::value, smem = walk_bytes<T, V, 2>();
+    const dim3 grid(static_cast<unsigned>(std::max(1, s.blocks * s.tiles)));
+    if (!s.within) {
       lay_out(s, p.channels, space);
-      cudaError_t e = launch(scan_runs_kernel<T, V, false>, dim3(blocks), kScanThreads, ring_bytes<T, V, 2>(), false, stream, static_cast<const ScanShape&>(p), s, p.x, p.x_stride, p.initial);
-      if (e == cudaSuccess) e = launch_join<false>(s, p.channels, stream);
+      const cudaError_t e = launch<scan_runs_kernel<T, V, false>>(grid, smem, false, stream, static_cast<const ScanShape&>(p), s, p.x, p.x_stride, p.initial);
       if (e != cudaSuccess) return e;
     }
-    return launch(scan_forward_kernel<T, V>, dim3(blocks), kScanThreads, ring_bytes<T, V, 2>(), s.parts > 1, stream, p, s);
+    return launch<scan_forward_kernel<T, V>>(grid, smem, !s.within, stream, p, s);
   });
 }
 
 cudaError_t launch_scan_backward(const ScanGradParams& p, ScanSplit s, void* space, cudaStream_t stream) {
-  const int vec = vector_of(p);
-  return by_vector(p.half, vec, [&](auto type, auto v) {
+  return by_vector(p.half, vector_of(p), [&](auto type, auto v) {
     using T = decltype(type);
-    constexpr int V = decltype(v)::value;
-    const unsigned blocks = blocks_of(p, s, vec);
-    if (s.parts > 1) {
+    constexpr int V = decltype(v)::value, smem = walk_bytes<T, V, 2>();
+    const dim3 grid(static_cast<unsigned>(std::max(1, s.blocks * s.tiles)));
+    if (!s.within) {
       lay_out(s, p.channels, space);
-      cudaError_t e = launch(scan_runs_kernel<T, V, true>, dim3(blocks), kScanThreads, ring_bytes<T, V, 2>(), false, stream, static_cast<const ScanShape&>(p), s, p.dh, p.dh_stride, p.dfinal);
-      if (e == cudaSuccess) e = launch_join<true>(s, p.channels, stream);
+      const cudaError_t e = launch<scan_runs_kernel<T, V, true>>(grid, smem, false, stream, static_cast<const ScanShape&>(p), s, p.dh, p.dh_stride, p.dfinal);
       if (e != cudaSuccess) return e;
     }
-    if (p.dgate == nullptr) return launch(scan_backward_kernel<T, V, false>, dim3(blocks), kScanThreads, ring_bytes<T, V, 2>(), s.parts > 1, stream, p, s);
-    return launch(scan_backward_kernel<T, V, true>, dim3(blocks), kScanThreads, ring_bytes<T, V, 4>(), s.parts > 1, stream, p, s);
+    if (p.dgate == nullptr) return launch<scan_backward_kernel<T, V, false>>(grid, smem, !s.within, stream, p, s);
+    return launch<scan_backward_kernel<T, V, true>>(grid, walk_bytes<T, V, 4>(), !s.within, stream, p, s);
   });
 }
 
@@ -677,7 +768,7 @@ cudaError_t launch_scan_step(const ScanStepParams& p, cudaStream_t stream) {
   const int vec = vector_of(p.half, p.channels, {{p.gate, p.gate_stride}, {p.x, p.x_stride}, {nullptr, 0}}, {p.state, reinterpret_cast<const void*>(p.state_stride * 4)});
   return by_vector(p.half, vec, [&](auto type, auto v) {
     const long long threads = static_cast<long long>(p.rows) * (p.channels / vec);
-    return launch(scan_step_kernel<decltype(type), decltype(v)::value>, dim3(static_cast<unsigned>((threads + kScanThreads - 1) / kScanThreads)), kScanThreads, 0, false, stream, p);
+    return launch<scan_step_kernel<decltype(type), decltype(v)::value>>(dim3(static_cast<unsigned>((threads + kScanThreads - 1) / kScanThreads)), 0, false, stream, p);
   });
 }
 
