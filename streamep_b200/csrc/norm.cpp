@@ -58,10 +58,9 @@ class Norm : public torch::autograd::Function<Norm> {
                                                 const std::optional<at::Tensor>& b, const std::optional<at::Tensor>& res, const c10::intrusive_ptr<NormCall>& call) {
     const at::Tensor weight = w.value_or(at::Tensor()), bias = b.value_or(at::Tensor()), residual = res.value_or(at::Tensor());
     NormResult r = norm_forward(*call, x, weight, bias, residual, true);
-    ctx->save_for_backward({residual.defined() ? r.sum : x, weight, r.stats});
+    ctx->save_for_backward({x, weight, r.stats, residual});
     ctx->saved_data["center"] = call->center;
     ctx->saved_data["bias"] = bias.defined() ? static_cast<int64_t>(type_of(bias)) : static_cast<int64_t>(kNormNone);
-    ctx->saved_data["residual"] = residual.defined();
     ctx->set_materialize_grads(false);
     if (residual.defined()) return {r.y, r.sum};
     return {r.y};
@@ -69,9 +68,9 @@ class Norm : public torch::autograd::Function<Norm> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     SEP_ASSERT(!at::GradMode::is_enabled(), "the normalisation has no second derivative: its backward was asked for a graph");
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+    const at::Tensor &x = saved[0], &weight = saved[1], &stats = saved[2], &added = saved[3];
     const int bias_type = static_cast<int>(ctx->saved_data["bias"].toInt());
-    const bool residual = ctx->saved_data["residual"].toBool();
+    const bool residual = added.defined();
     const at::Tensor dy = grads[0], dsum = residual ? grads[1] : at::Tensor();
     // (tensors that were left out have no edge in the graph)
     int edge = 1;
@@ -96,6 +95,8 @@ class Norm : public torch::autograd::Function<Norm> {
       p.center = ctx->saved_data["center"].toBool(); p.rows = rows; p.hidden = static_cast<int>(H);
       p.x = xr.data_ptr(); p.x_stride = xr.stride(0);
       p.dy = dyr.data_ptr(); p.dy_stride = dyr.stride(0);
+      at::Tensor rr;
+      if (residual) { rr = as_rows(added); p.residual = rr.data_ptr(); p.residual_stride = rr.stride(0); }
       if (sr.defined()) { p.dsum = sr.data_ptr(); p.dsum_stride = sr.stride(0); }
       p.weight = w.defined() ? w.data_ptr() : nullptr;
       p.stats = reinterpret_cast<const float2*>(stats.data_ptr<float>());
@@ -104,7 +105,7 @@ class Norm : public torch::autograd::Function<Norm> {
       p.dbias = want_db ? db.data_ptr() : nullptr;
       at::Tensor parts;
       if (want_dw || want_db) {
-        parts = at::empty({2 * static_cast<int64_t>(norm_parts(rows, p.hidden, sms)) * H}, x.options().dtype(at::kFloat));
+        parts = at::empty({2 * static_cast<int64_t>(norm_parts(p, sms)) * H}, x.options().dtype(at::kFloat));
         p.parts = parts.data_ptr<float>();
       }
       SEP_CUDA_CHECK(launch_norm_backward(p, sms, at::cuda::getCurrentCUDAStream()));

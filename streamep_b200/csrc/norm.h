@@ -29,10 +29,11 @@ struct NormGradParams {
   int type, weight_type, center;
   long long rows;
   int hidden;
-  const void* x;                 // what was normalised: x, or the sum
+  const void* x;
+  const void* residual;          // or null
   const void* dy;
   const void* dsum;              // the sum's own gradient, or null
-  long long x_stride, dy_stride, dsum_stride;
+  long long x_stride, residual_stride, dy_stride, dsum_stride;
   const void* weight;
   const float2* stats;
   void* dx;                      // [rows, hidden] contiguous
@@ -41,7 +42,7 @@ struct NormGradParams {
   float* parts;                  // [2][norm_parts][hidden] sums of the blocks' rows
 };
 // How many blocks leave sums of their own for the gradients of weight and bias.
-int norm_parts(long long rows, int hidden, int sms);
+int norm_parts(const NormGradParams& p, int sms);
 cudaError_t launch_norm_backward(const NormGradParams& p, int sms, cudaStream_t stream);
 
 }  // namespace sep

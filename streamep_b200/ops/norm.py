@@ -22,8 +22,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     ``y`` comes from the sum before its rounding.
 
     Differentiable in all four tensors; there is no second derivative.  Mean and variance (of centred values), and all sums, are
-    formed in 32 bits; the gradients are those of the formula, with the sum as it was returned in the place of the unrounded one.  A repeated
-    call gives the same bits.  A row with an infinity or NaN becomes NaN, and so do weight and bias' gradients that it has a part in."""
+    formed in 32 bits, the gradients of ``x + residual`` before its rounding too (so both are kept for the backward, not the sum).  A
+    repeated call gives the same bits.  A row with an infinity or NaN becomes NaN, and so do weight and bias' gradients that it has a part in."""
     out = _ext.load().norm_rows(x, weight, bias, residual, True, float(eps))
     return (out[0], out[1]) if residual is not None else out[0]
 

@@ -71,9 +71,6 @@ def check(t, center, dy=None, dsum=None, eps=1e-5, grads=True):
     if total is not None and dsum is not None:
         outs, ups = [y, total], [dy, dsum]
     got = dict(zip(t, torch.autograd.grad(outs, list(t.values()), ups)))
-    if total is not None:                                # the gradient's formula on the sum as it was returned
-        s = total.detach().double()
-        u = (s - mean) * rstd
     d = dy.double() * w
     mean_d = d.mean(-1, keepdim=True) if center else 0.0
     dx = rstd * (d - mean_d - u * (d * u).mean(-1, keepdim=True))
@@ -276,10 +273,15 @@ def test_refusals(native):
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(ValueError, match="forward-mode"):
             layer_norm(torch.autograd.forward_ad.make_dual(x, x))
-    # what was saved must not have changed
-    y, s = layer_norm(x, w, residual=x.detach())
+    # what was saved must not have changed; the sum, which a program may go on in, was not
+    r = x.detach().clone()
+    y, s = layer_norm(x, w, residual=r)
     with torch.no_grad():
         s.add_(1.0)
+    torch.autograd.grad(y.sum(), x)
+    y, s = layer_norm(x, w, residual=r)
+    with torch.no_grad():
+        r.add_(1.0)
     with pytest.raises(RuntimeError, match="inplace"):
         torch.autograd.grad(y.sum(), x)
 
