@@ -13,6 +13,7 @@
 
 #include "norm.h"
 #include "ptx.cuh"
+#include "rows.cuh"
 
 namespace sep {
 
@@ -20,13 +21,6 @@ namespace {
 
 constexpr int kRowThreads = 256;                 // of a block that takes one row at a time
 constexpr int kColumnThreads = 32, kColumnRows = 8;
-
-template <class T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 __device__ __forceinline__ float load_weight(const void* w, int type, int i) {
   return type == kNormHalf ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]) : static_cast<const float*>(w)[i];
@@ -54,100 +48,82 @@ __device__ __forceinline__ float2 block_sum(float2 v, float2* scratch) {
   return s;
 }
 
-// V elements of a row, as they lie in memory.
-template <class T, int V> __device__ __forceinline__ void unpack(const void* from, float (&f)[V]) {
-  if constexpr (sizeof(T) * V == 16 && sizeof(T) == 2) {
-    const uint4 v = *static_cast<const uint4*>(from);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { const float2 p = unpack_bf16x2(w[i]); f[2 * i] = p.x; f[2 * i + 1] = p.y; }
-  } else if constexpr (sizeof(T) * V == 16) {
-    const float4 v = *static_cast<const float4*>(from);
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-  } else if constexpr (sizeof(T) == 2 && V == 2) {
-    const float2 p = unpack_bf16x2(*static_cast<const uint32_t*>(from));
-    f[0] = p.x; f[1] = p.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = to_float(static_cast<const T*>(from)[i]);
-  }
-}
-template <class T, int V> __device__ __forceinline__ void store(T* at, const float (&f)[V]) {
-  if constexpr (sizeof(T) * V == 16 && sizeof(T) == 2)
-    *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  else if constexpr (sizeof(T) * V == 16) *reinterpret_cast<float4*>(at) = make_float4(f[0], f[1], f[2], f[3]);
-  else if constexpr (sizeof(T) == 2 && V == 2) *reinterpret_cast<uint32_t*>(at) = pack_bf16x2(f[0], f[1]);
-  else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) at[i] = from_float<T>(f[i]);
-  }
-}
-// V numbers of weight or bias (which lie on boundaries of 4 numbers where V >= 4).
-template <int V> __device__ __forceinline__ void load_weights(const void* w, int type, int at, float (&f)[V]) {
-  if constexpr (V == 8) {
-    if (type == kNormHalf) { unpack<__nv_bfloat16, 8>(static_cast<const __nv_bfloat16*>(w) + at, f); return; }
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + at + i);
-      f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
-    }
-  } else if constexpr (V == 4) {
-    if (type == kNormFloat) { unpack<float, 4>(static_cast<const float*>(w) + at, f); return; }
-    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + at);
-    const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y);
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = load_weight(w, type, at + i);
-  }
-}
-
 constexpr int kMostColumns = 8192;               // of rows that stay in registers: 512 threads of 16
 constexpr int kGroupThreads = 256;               // of a block, where a row takes no more
 
-// A block's threads in groups of `threads` (32 to 512) for a row each; a thread takes vectors lane, lane + threads, ... of it.
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// A block's threads in groups of `threads` (a multiple of 32, up to 512) for a row each; a thread takes vectors lane, lane + threads, ... of it.
 struct Group {
   int threads, lane, index, count;
   __device__ __forceinline__ explicit Group(int t) : threads(t), lane(threadIdx.x % t), index(threadIdx.x / t), count(blockDim.x / t) {}
   // Every thread of a group gets its sums.  All of the block call, each time with the next of three buffers.
-  __device__ __forceinline__ float2 sum(float2 v, float2 (*scratch)[16], int& turn) const {
+  template <class Sum>
+  __device__ __forceinline__ Sum sum(Sum v, float2 (*scratch)[16], int& turn) const {
     v = warp_sum(v);
     if (threads == 32) return v;
-    float2* mine = scratch[turn];
+    Sum* mine = reinterpret_cast<Sum*>(scratch[turn]);
     turn = turn == 2 ? 0 : turn + 1;
     if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5] = v;
     __syncthreads();
-    float2 s = make_float2(0.f, 0.f);
-    const int first = index * (threads >> 5);
-    for (int w = 0; w < (threads >> 5); ++w) { s.x += mine[first + w].x; s.y += mine[first + w].y; }
-    return s;
+    // (the warps' sums like a warp's: one after another they took 500 cycles a row of 14 warps)
+    const int warps = threads >> 5, w = threadIdx.x & 31;
+    v = Sum{};
+    if (w < warps) v = mine[index * warps + w];
+    return warp_sum(v);
   }
 };
+template <int V> __device__ __forceinline__ float across(const Row<V>& r) {
+  float f[V], s = 0.f;
+  r.get(f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) s = i == 0 ? f[0] : s + f[i];
+  return s;
+}
 
-// Arrays of a row ahead: `kArrays` of them, some of which may be left out (null).
+// Rows that are on their way, kArrays arrays of each, some of which may be left out (null).  bf16 taken one by one, 2 bytes, come through registers.
 template <class T, int V, int K, int kArrays>
 struct RowsAhead {
   static constexpr bool kCopies = sizeof(T) * V >= 4;
-  static constexpr int kBytes = sizeof(T) * V >= 4 ? sizeof(T) * V : 4;
+  static constexpr int kBytes = kCopies ? sizeof(T) * V : 4;
   int ahead;                     // rows that the ring holds: 2, or 1 where two do not fit
-  unsigned char* ring;
-  const T* base[kArrays];
-  long long stride[kArrays];
-  __device__ __forceinline__ unsigned char* place(int slot, int a, int k) const { return ring + (((slot * kArrays + a) * K + k) * blockDim.x + threadIdx.x) * kBytes; }
-  __device__ __forceinline__ void fetch(int slot, long long row, bool there, const Group& g, int vectors) const {
+  unsigned char* mine;           // this thread's place in the ring
+  int plane;                     // bytes of a vector of all threads
+  bool in[K];                    // whether this thread has a vector there
+  int columns;                   // between a thread's vectors
+  const T* next[kArrays];        // this thread's first vector of the next row to fetch
+  long long step[kArrays];
+
+  __device__ __forceinline__ RowsAhead(int ahead, unsigned char* ring, const Group& g, int vectors) : ahead(ahead) {
+    mine = ring + threadIdx.x * kBytes;
+    plane = blockDim.x * kBytes;
+    columns = g.threads * V;
+#pragma unroll
+    for (int k = 0; k < K; ++k) in[k] = g.lane + k * g.threads < vectors;
+  }
+  __device__ __forceinline__ void array(int a, const void* base, long long stride, long long first, long long rows, int column) {
+    next[a] = base != nullptr ? static_cast<const T*>(base) + first * stride + column : nullptr;
+    step[a] = rows * stride;
+  }
+  __device__ __forceinline__ unsigned char* place(int slot, int a, int k) const { return mine + ((slot * kArrays + a) * K + k) * plane; }
+  __device__ __forceinline__ void fetch(int slot, bool there) {
     if (there) {
 #pragma unroll
       for (int a = 0; a < kArrays; ++a) {
-        if (base[a] == nullptr) continue;
-        const T* from = base[a] + row * stride[a];
+        if (next[a] == nullptr) continue;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          const int v = g.lane + k * g.threads;
-          if (v >= vectors) continue;
-          if constexpr (!kCopies) *reinterpret_cast<float*>(place(slot, a, k)) = to_float(from[v]);
-          else if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(place(slot, a, k))), "l"(from + v * V) : "memory");
-          else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(place(slot, a, k))), "l"(from + v * V) : "memory");
+          if (!in[k]) continue;
+          const T* from = next[a] + k * columns;
+          if constexpr (!kCopies) *reinterpret_cast<float*>(place(slot, a, k)) = to_float(*from);
+          else if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(place(slot, a, k))), "l"(from) : "memory");
+          else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(place(slot, a, k))), "l"(from) : "memory");
         }
+        next[a] += step[a];
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -156,191 +132,153 @@ struct RowsAhead {
     if (ahead == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  __device__ __forceinline__ void get(int slot, int a, int k, float (&f)[V]) const {
-    if constexpr (!kCopies) f[0] = *reinterpret_cast<const float*>(place(slot, a, k));
-    else unpack<T, V>(place(slot, a, k), f);
+  __device__ __forceinline__ Row<V> get(int slot, int a, int k) const {
+    if constexpr (!kCopies) return Row<V>::all(*reinterpret_cast<const float*>(place(slot, a, k)));
+    else { Raw<T, V> raw; raw.load(reinterpret_cast<const T*>(place(slot, a, k))); return raw.get(); }
   }
 };
 
-template <class T, int V, int K>
-__global__ void __launch_bounds__(512) norm_forward_kernel(const NormParams p, int group_threads, int ahead) {
+// V numbers of weight or bias, from L1 for every row but the first: in registers they would cost half of the threads that an SM holds.
+template <int V>
+__device__ __forceinline__ Row<V> load_weights(const void* w, int type, int at) {
+  if (type == kNormHalf) {
+    Raw<__nv_bfloat16, V> raw;
+    raw.load(static_cast<const __nv_bfloat16*>(w) + at);
+    return raw.get();
+  }
+  return load_state<V>(static_cast<const float*>(w) + at);
+}
+
+template <class T, int V, int K, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) norm_forward_kernel(const NormParams p, int group_threads, int ahead) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float2 scratch[3][16];
   const Group g(group_threads);
-  RowsAhead<T, V, K, 2> rows{ahead, ring, {static_cast<const T*>(p.x), static_cast<const T*>(p.residual)}, {p.x_stride, p.residual_stride}};
-  const int vectors = p.hidden / V;
   const float inv = 1.f / static_cast<float>(p.hidden);
   const long long step = static_cast<long long>(gridDim.x) * g.count, first = static_cast<long long>(blockIdx.x) * g.count + g.index;
-  int turn = 0;
-  for (int i = 0; i < ahead; ++i) rows.fetch(i, first + i * step, first + i * step < p.rows, g, vectors);
+  RowsAhead<T, V, K, 2> rows(ahead, ring, g, p.hidden / V);
+  rows.array(0, p.x, p.x_stride, first, step, g.lane * V);
+  rows.array(1, p.residual, p.residual_stride, first, step, g.lane * V);
+  for (int i = 0; i < ahead; ++i) rows.fetch(i, first + i * step < p.rows);
+  T* y = static_cast<T*>(p.y) + first * p.hidden + g.lane * V;
+  T* sum = p.sum != nullptr ? static_cast<T*>(p.sum) + first * p.hidden + g.lane * V : nullptr;
+  int turn = 0, slot = 0;
   // (all groups of a block take as many turns as its first one, for the barriers)
-  const long long turns = (p.rows - static_cast<long long>(blockIdx.x) * g.count + step - 1) / step;
-  for (long long t = 0; t < turns; ++t) {
-    const long long row = first + t * step;
+  for (long long row = first, lead = first - g.index; lead < p.rows; row += step, lead += step, y += step * p.hidden, slot = ahead == 2 ? slot ^ 1 : 0) {
     const bool there = row < p.rows;
-    const int slot = ahead == 2 ? static_cast<int>(t & 1) : 0;
     rows.wait();
-    float s[K][V];
-    float2 sums = make_float2(0.f, 0.f);
+    Row<V> s[K], total = Row<V>::all(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[k][i] = 0.f;
-      if (there && g.lane + k * g.threads < vectors) {
-        rows.get(slot, 0, k, s[k]);
+      s[k] = Row<V>::all(0.f);
+      if (there && rows.in[k]) {
+        s[k] = rows.get(slot, 0, k);
         if (p.residual != nullptr) {
-          float r[V];
-          rows.get(slot, 1, k, r);
-#pragma unroll
-          for (int i = 0; i < V; ++i) s[k][i] += r[i];
+          s[k] = s[k] + rows.get(slot, 1, k);
+          store_row<T, V>(sum + k * rows.columns, s[k]);
         }
-#pragma unroll
-        for (int i = 0; i < V; ++i) sums.x += s[k][i];
+        total = total + s[k];
       }
     }
-    rows.fetch(slot, row + ahead * step, row + ahead * step < p.rows, g, vectors);
+    if (sum != nullptr) sum += step * p.hidden;
+    rows.fetch(slot, row + ahead * step < p.rows);
     float mean = 0.f;
-    if (p.center) mean = g.sum(sums, scratch, turn).x * inv;
-    sums.x = 0.f;
+    if (p.center) mean = g.sum(across(total), scratch, turn) * inv;
+    const Row<V> minus = Row<V>::all(-mean);
+    total = Row<V>::all(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (g.lane + k * g.threads < vectors) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) { const float d = s[k][i] - mean; sums.x = fmaf(d, d, sums.x); }
+      if (rows.in[k]) {
+        s[k] = s[k] + minus;
+        total = fused(s[k], s[k], total);
       }
-    const float rstd = rsqrtf(g.sum(sums, scratch, turn).x * inv + p.eps);
+    const float rstd = rsqrtf(g.sum(across(total), scratch, turn) * inv + p.eps);
     if (!there) continue;
     if (p.stats != nullptr && g.lane == 0) p.stats[row] = make_float2(mean, rstd);
-    T* y = static_cast<T*>(p.y) + row * p.hidden;
-    T* sum = static_cast<T*>(p.sum) + row * p.hidden;
+    const Row<V> scale = Row<V>::all(rstd);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int at = (g.lane + k * g.threads) * V;
-      if (at >= p.hidden) continue;
-      if (p.sum != nullptr) store<T, V>(sum + at, s[k]);
-      float w[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[k][i] = (s[k][i] - mean) * rstd;
-      if (p.weight != nullptr) {
-        load_weights<V>(p.weight, p.weight_type, at, w);
-#pragma unroll
-        for (int i = 0; i < V; ++i) s[k][i] *= w[i];
-      }
-      if (p.bias != nullptr) {
-        load_weights<V>(p.bias, p.weight_type, at, w);
-#pragma unroll
-        for (int i = 0; i < V; ++i) s[k][i] += w[i];
-      }
-      store<T, V>(y + at, s[k]);
+      if (!rows.in[k]) continue;
+      Row<V> u = s[k] * scale;
+      const int at = g.lane * V + k * rows.columns;
+      if (p.weight != nullptr && p.bias != nullptr) u = fused(u, load_weights<V>(p.weight, p.weight_type, at), load_weights<V>(p.bias, p.weight_type, at));
+      else if (p.weight != nullptr) u = u * load_weights<V>(p.weight, p.weight_type, at);
+      else if (p.bias != nullptr) u = u + load_weights<V>(p.bias, p.weight_type, at);
+      store_row<T, V>(y + k * rows.columns, u);
     }
   }
 }
 
-template <class T, int V, int K>
-__global__ void __launch_bounds__(512) norm_backward_kernel(const NormGradParams p, int group_threads, int ahead) {
+template <class T, int V, int K, int kThreads>
+__global__ void __launch_bounds__(kThreads, 512 / kThreads) norm_backward_kernel(const NormGradParams p, int group_threads, int ahead) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float2 scratch[3][16];
   const Group g(group_threads);
-  RowsAhead<T, V, K, 4> rows{ahead, ring,
-                                     {static_cast<const T*>(p.x), static_cast<const T*>(p.dy), static_cast<const T*>(p.residual), static_cast<const T*>(p.dsum)},
-                                     {p.x_stride, p.dy_stride, p.residual_stride, p.dsum_stride}};
-  const int vectors = p.hidden / V;
   const float inv = 1.f / static_cast<float>(p.hidden);
   const long long step = static_cast<long long>(gridDim.x) * g.count, first = static_cast<long long>(blockIdx.x) * g.count + g.index;
-  int turn = 0;
-  float dw[K][V], db[K][V];
+  RowsAhead<T, V, K, 4> rows(ahead, ring, g, p.hidden / V);
+  rows.array(0, p.x, p.x_stride, first, step, g.lane * V);
+  rows.array(1, p.dy, p.dy_stride, first, step, g.lane * V);
+  rows.array(2, p.residual, p.residual_stride, first, step, g.lane * V);
+  rows.array(3, p.dsum, p.dsum_stride, first, step, g.lane * V);
+  for (int i = 0; i < ahead; ++i) rows.fetch(i, first + i * step < p.rows);
+  Row<V> dw[K], db[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
-  for (int i = 0; i < ahead; ++i) rows.fetch(i, first + i * step, first + i * step < p.rows, g, vectors);
-  const long long turns = (p.rows - static_cast<long long>(blockIdx.x) * g.count + step - 1) / step;
+  for (int k = 0; k < K; ++k) dw[k] = db[k] = Row<V>::all(0.f);
+  T* dx = p.dx != nullptr ? static_cast<T*>(p.dx) + first * p.hidden + g.lane * V : nullptr;
   float2 next_stats = first < p.rows ? p.stats[first] : make_float2(0.f, 0.f);
-  for (long long t = 0; t < turns; ++t) {
-    const long long row = first + t * step;
+  int turn = 0, slot = 0;
+  for (long long row = first, lead = first - g.index; lead < p.rows; row += step, lead += step, slot = ahead == 2 ? slot ^ 1 : 0) {
     const bool there = row < p.rows;
-    const int slot = ahead == 2 ? static_cast<int>(t & 1) : 0;
     const float2 st = next_stats;
     if (row + step < p.rows) next_stats = p.stats[row + step];
     rows.wait();
-    float u[K][V], d[K][V];
-    float2 sums = make_float2(0.f, 0.f);
+    const Row<V> minus = Row<V>::all(-st.x), scale = Row<V>::all(st.y);
+    Row<V> u[K], d[K], sum_d = Row<V>::all(0.f), sum_du = Row<V>::all(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (!there || g.lane + k * g.threads >= vectors) continue;
-      rows.get(slot, 0, k, u[k]);
-      rows.get(slot, 1, k, d[k]);
-      float w[V];
-      if (p.residual != nullptr) {
-        rows.get(slot, 2, k, w);
-#pragma unroll
-        for (int i = 0; i < V; ++i) u[k][i] += w[i];
-      }
-      if (p.weight != nullptr) load_weights<V>(p.weight, p.weight_type, (g.lane + k * g.threads) * V, w);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        u[k][i] = (u[k][i] - st.x) * st.y;
-        dw[k][i] = fmaf(d[k][i], u[k][i], dw[k][i]);
-        db[k][i] += d[k][i];
-        if (p.weight != nullptr) d[k][i] *= w[i];
-        sums.x += d[k][i];
-        sums.y = fmaf(d[k][i], u[k][i], sums.y);
-      }
+      if (!there || !rows.in[k]) continue;
+      u[k] = rows.get(slot, 0, k);
+      if (p.residual != nullptr) u[k] = u[k] + rows.get(slot, 2, k);
+      u[k] = (u[k] + minus) * scale;
+      d[k] = rows.get(slot, 1, k);
+      dw[k] = fused(d[k], u[k], dw[k]);
+      db[k] = db[k] + d[k];
+      if (p.weight != nullptr) d[k] = d[k] * load_weights<V>(p.weight, p.weight_type, g.lane * V + k * rows.columns);
+      sum_d = sum_d + d[k];
+      sum_du = fused(d[k], u[k], sum_du);
     }
-    if (p.dx != nullptr) {
-      sums = g.sum(sums, scratch, turn);
-      const float mean_d = p.center ? sums.x * inv : 0.f, mean_du = sums.y * inv;
-      T* dx = static_cast<T*>(p.dx) + row * p.hidden;
+    if (dx != nullptr) {
+      const float2 sums = g.sum(make_float2(across(sum_d), across(sum_du)), scratch, turn);
+      const Row<V> minus_d = Row<V>::all(p.center ? -sums.x * inv : 0.f), minus_du = Row<V>::all(-sums.y * inv);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int at = (g.lane + k * g.threads) * V;
-        if (!there || at >= p.hidden) continue;
-#pragma unroll
-        for (int i = 0; i < V; ++i) d[k][i] = st.y * (d[k][i] - mean_d - u[k][i] * mean_du);
-        if (p.dsum != nullptr) {
-          float add[V];
-          rows.get(slot, 3, k, add);
-#pragma unroll
-          for (int i = 0; i < V; ++i) d[k][i] += add[i];
-        }
-        store<T, V>(dx + at, d[k]);
+        if (!there || !rows.in[k]) continue;
+        const Row<V> v = fused(u[k], minus_du, d[k] + minus_d);
+        store_row<T, V>(dx + k * rows.columns, p.dsum != nullptr ? fused(v, scale, rows.get(slot, 3, k)) : v * scale);
       }
+      dx += step * p.hidden;
     }
-    rows.fetch(slot, row + ahead * step, row + ahead * step < p.rows, g, vectors);
+    rows.fetch(slot, row + ahead * step < p.rows);
   }
   if (p.parts == nullptr) return;
   // the groups' sums, one after another, in place of the ring
   asm volatile("cp.async.wait_group 0;" ::: "memory");
-  float2* all = reinterpret_cast<float2*>(ring);
+  float* all = reinterpret_cast<float*>(ring);
   for (int q = g.count - 1; q >= 0; --q) {
     __syncthreads();
     if (g.index != q) continue;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int at = (g.lane + k * g.threads) * V + i;
-        if (at >= p.hidden) continue;
-        if (q < g.count - 1) { const float2 v = all[at]; dw[k][i] += v.x; db[k][i] += v.y; }
-        if (q > 0) all[at] = make_float2(dw[k][i], db[k][i]);
-      }
-    if (q > 0) continue;
-    float* out_w = p.parts + static_cast<long long>(blockIdx.x) * p.hidden;
-    float* out_b = p.parts + static_cast<long long>(gridDim.x + blockIdx.x) * p.hidden;
-#pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int at = (g.lane + k * g.threads) * V;
-      if (at >= p.hidden) continue;
-      if constexpr (V == 8) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-          *reinterpret_cast<float4*>(out_w + at + i) = make_float4(dw[k][i], dw[k][i + 1], dw[k][i + 2], dw[k][i + 3]);
-          *reinterpret_cast<float4*>(out_b + at + i) = make_float4(db[k][i], db[k][i + 1], db[k][i + 2], db[k][i + 3]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) { out_w[at + i] = dw[k][i]; out_b[at + i] = db[k][i]; }
+      if (!rows.in[k]) continue;
+      const int at = g.lane * V + k * rows.columns;
+      if (q < g.count - 1) {
+        dw[k] = dw[k] + load_state<V>(all + at);
+        db[k] = db[k] + load_state<V>(all + p.hidden + at);
       }
+      float* to = q > 0 ? all : p.parts + static_cast<long long>(blockIdx.x) * p.hidden;
+      store_state<V>(to + at, dw[k]);
+      store_state<V>(to + (q > 0 ? static_cast<long long>(p.hidden) : static_cast<long long>(gridDim.x) * p.hidden) + at, db[k]);
     }
   }
 }
@@ -462,8 +400,8 @@ Form form_of(int half, int hidden, bool sixteen, bool four) {
   f.vec = sixteen ? (half ? 8 : 4) : half && four ? 2 : 1;
   const int vectors = hidden / f.vec;
   f.each = vectors <= 32 ? 1 : 16 / f.vec;
-  f.threads = 32;
-  while (f.threads * f.each < vectors) f.threads *= 2;
+  f.threads = (vectors + f.each - 1) / f.each;                 // whole warps; more than half of them, a block that is not full
+  f.threads = (f.threads + 31) / 32 * 32;
   return f;
 }
 // Whether all rows and the weights begin on boundaries of 16 bytes (and of 4).
@@ -475,7 +413,8 @@ struct Boundaries {
     const auto at = reinterpret_cast<uintptr_t>(base) | static_cast<uintptr_t>(stride * (half ? 2 : 4));
     sixteen = sixteen && at % 16 == 0; four = four && at % 4 == 0;
   }
-  void weights(const void* w) { sixteen = sixteen && reinterpret_cast<uintptr_t>(w) % 16 == 0; }
+  // (fp32 weights beside pairs of bf16 rows are read 8 bytes at a time)
+  void weights(const void* w) { sixteen = sixteen && reinterpret_cast<uintptr_t>(w) % 16 == 0; four = four && reinterpret_cast<uintptr_t>(w) % 8 == 0; }
 };
 Form form_of(const NormParams& p) {
   const int half = p.type == kNormHalf;
@@ -490,14 +429,14 @@ Form form_of(const NormGradParams& p) {
   b.weights(p.weight);
   return form_of(half, p.hidden, b.sixteen, b.four);
 }
-int threads_of(const Form& f) { return f.threads > kGroupThreads ? f.threads : kGroupThreads; }
+int threads_of(const Form& f) { return f.threads > kGroupThreads ? f.threads : kGroupThreads / f.threads * f.threads; }
 int blocks_of(const Form& f, long long rows, int sms, int resident) {
   const long long groups = threads_of(f) / f.threads, most = (rows + groups - 1) / groups, all = static_cast<long long>(sms) * resident;
   return static_cast<int>(most < all ? most : all);
 }
 // Blocks that share an SM: as many as its registers (128 a thread in the backward, 64 in the forward) and shared memory hold.
 int resident_backward(const Form& f) { return threads_of(f) > kGroupThreads ? 1 : 2; }
-int resident_forward(const Form& f) { return (threads_of(f) > kGroupThreads ? 1 : 2) * (f.vec == 8 || f.each == 1 ? 2 : 1); }
+int resident_forward(const Form& f) { return threads_of(f) > kGroupThreads ? 2 : 4; }
 
 template <class F>
 cudaError_t by_form(int half, const Form& f, F run) {
@@ -545,7 +484,11 @@ cudaError_t launch_norm_forward(const NormParams& p, int sms, cudaStream_t strea
   const int half = p.type == kNormHalf;
   if (f.threads > 0)
     return by_form(half, f, [&](auto type, auto vec, auto each) {
-      return launch_rows<norm_forward_kernel<decltype(type), decltype(vec)::value, decltype(each)::value>>(p, f, blocks_of(f, p.rows, sms, resident_forward(f)), 2 * ring_of(f, half, 2), 2, stream);
+      using T = decltype(type);
+      constexpr int V = decltype(vec)::value, K = decltype(each)::value;
+      const int blocks = blocks_of(f, p.rows, sms, resident_forward(f)), ring = 2 * ring_of(f, half, 2);
+      return f.threads > kGroupThreads ? launch_rows<norm_forward_kernel<T, V, K, 512>>(p, f, blocks, ring, 2, stream)
+                                       : launch_rows<norm_forward_kernel<T, V, K, 256>>(p, f, blocks, ring, 2, stream);
     });
   const int blocks = row_blocks(p.rows, sms);
   if (half) norm_forward_any_kernel<__nv_bfloat16><<<blocks, kRowThreads, 0, stream>>>(p);
@@ -560,7 +503,11 @@ cudaError_t launch_norm_backward(const NormGradParams& p, int sms, cudaStream_t 
   if (f.threads > 0) {
     const int row = ring_of(f, half, 4), ahead = 2 * row <= kMostRing ? 2 : 1, ring = ahead * row, sums = p.hidden * 8;
     e = by_form(half, f, [&](auto type, auto vec, auto each) {
-      return launch_rows<norm_backward_kernel<decltype(type), decltype(vec)::value, decltype(each)::value>>(p, f, parts, ring > sums ? ring : sums, ahead, stream);
+      using T = decltype(type);
+      constexpr int V = decltype(vec)::value, K = decltype(each)::value;
+      const int smem = ring > sums ? ring : sums;
+      return f.threads > kGroupThreads ? launch_rows<norm_backward_kernel<T, V, K, 512>>(p, f, parts, smem, ahead, stream)
+                                       : launch_rows<norm_backward_kernel<T, V, K, 256>>(p, f, parts, smem, ahead, stream);
     });
   } else {
     const int blocks = row_blocks(p.rows, sms);

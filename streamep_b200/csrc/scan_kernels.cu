@@ -19,56 +19,13 @@
 
 #include "scan.h"
 #include "ptx.cuh"
+#include "rows.cuh"
 
 namespace sep {
 
 namespace {
 
 constexpr int kScanThreads = 256;
-
-template <class T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// Two fp32 numbers that one instruction works on.
-struct Pair { unsigned long long v; };
-__device__ __forceinline__ Pair pair_of(float a, float b) { Pair p; asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b)); return p; }
-__device__ __forceinline__ void parts_of(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) { Pair d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) { Pair d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
-__device__ __forceinline__ Pair fused(Pair a, Pair b, Pair c) { Pair d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return d; }
-// V numbers of a thread, of one row.  (Sums and products are written out, so that the bits do not depend on what else a call computes.)
-template <int V> struct Row {
-  Pair p[V / 2];
-  __device__ __forceinline__ static Row all(float f) { Row r; for (int i = 0; i < V / 2; ++i) r.p[i] = pair_of(f, f); return r; }
-  __device__ __forceinline__ void put(int i, float a, float b) { p[i] = pair_of(a, b); }
-  __device__ __forceinline__ void get(float (&f)[V]) const { _Pragma("unroll") for (int i = 0; i < V / 2; ++i) parts_of(p[i], f[2 * i], f[2 * i + 1]); }
-  __device__ __forceinline__ static Row of(const float (&f)[V]) { Row r; _Pragma("unroll") for (int i = 0; i < V / 2; ++i) r.p[i] = pair_of(f[2 * i], f[2 * i + 1]); return r; }
-};
-template <> struct Row<1> {
-  float f;
-  __device__ __forceinline__ static Row all(float f) { return Row{f}; }
-  __device__ __forceinline__ void get(float (&o)[1]) const { o[0] = f; }
-  __device__ __forceinline__ static Row of(const float (&o)[1]) { return Row{o[0]}; }
-};
-template <int V> __device__ __forceinline__ Row<V> operator+(Row<V> a, const Row<V>& b) {
-  if constexpr (V == 1) a.f = __fadd_rn(a.f, b.f);
-  else { _Pragma("unroll") for (int i = 0; i < V / 2; ++i) a.p[i] = a.p[i] + b.p[i]; }
-  return a;
-}
-template <int V> __device__ __forceinline__ Row<V> operator*(Row<V> a, const Row<V>& b) {
-  if constexpr (V == 1) a.f = __fmul_rn(a.f, b.f);
-  else { _Pragma("unroll") for (int i = 0; i < V / 2; ++i) a.p[i] = a.p[i] * b.p[i]; }
-  return a;
-}
-template <int V> __device__ __forceinline__ Row<V> fused(const Row<V>& a, const Row<V>& b, Row<V> c) {
-  if constexpr (V == 1) c.f = fmaf(a.f, b.f, c.f);
-  else { _Pragma("unroll") for (int i = 0; i < V / 2; ++i) c.p[i] = fused(a.p[i], b.p[i], c.p[i]); }
-  return c;
-}
 
 // sigmoid(gate) and sigmoid(-gate), each to its own last digits: 1 / (1 + e) and e / (1 + e) of e = exp(gate), which is held at 2^126 (a gate of
 // 87; NaN stays).  For bf16 gates the exponent is rounded once (|gate| 2^-24 of the result), for fp32 ones it is not.
@@ -139,74 +96,6 @@ __device__ __forceinline__ bool within_one(const ScanShape& p, int before, int e
   if (before < 0) return false;
   SequenceWalk walk(p, before);
   return walk.at(p, before) >= 0 && walk.all_within(p, end);
-}
-
-// V channels of a row, as they lie in memory.
-template <class T, int V> struct Raw;
-template <> struct Raw<__nv_bfloat16, 8> {
-  uint4 v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ Row<8> get() const {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    Row<8> r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.put(i, __uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-    return r;
-  }
-};
-template <> struct Raw<__nv_bfloat16, 2> {
-  uint32_t v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint32_t*>(p); }
-  __device__ __forceinline__ Row<2> get() const { Row<2> r; r.put(0, __uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); return r; }
-};
-template <> struct Raw<float, 4> {
-  float4 v;
-  __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
-  __device__ __forceinline__ Row<4> get() const { Row<4> r; r.put(0, v.x, v.y); r.put(1, v.z, v.w); return r; }
-};
-template <class T> struct Raw<T, 1> {
-  T v;
-  __device__ __forceinline__ void load(const T* p) { v = *p; }
-  __device__ __forceinline__ Row<1> get() const { return Row<1>{to_float(v)}; }
-};
-template <class T, int V>
-__device__ __forceinline__ void store_row(T* at, const Row<V>& row) {
-  float f[V];
-  row.get(f);
-  if constexpr (V == 8) *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  else if constexpr (V == 2) *reinterpret_cast<uint32_t*>(at) = pack_bf16x2(f[0], f[1]);
-  else if constexpr (V == 4) *reinterpret_cast<float4*>(at) = make_float4(f[0], f[1], f[2], f[3]);
-  else *at = from_float<T>(f[0]);
-}
-template <int V>
-__device__ __forceinline__ Row<V> load_state(const float* at) {
-  float f[V];
-  if constexpr (V >= 4) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(at + i);
-      f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
-    }
-  } else if constexpr (V == 2) {
-    const float2 v = *reinterpret_cast<const float2*>(at);
-    f[0] = v.x; f[1] = v.y;
-  } else {
-    f[0] = *at;
-  }
-  return Row<V>::of(f);
-}
-template <int V>
-__device__ __forceinline__ void store_state(float* at, const Row<V>& row) {
-  float f[V];
-  row.get(f);
-  if constexpr (V >= 4) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(at + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-  } else if constexpr (V == 2) {
-    *reinterpret_cast<float2*>(at) = make_float2(f[0], f[1]);
-  } else {
-    *at = f[0];
-  }
 }
 
 // A block's threads: LANES side by side across the channels, V channels each, and SEGS segments above one another.  Where runs are joined, PARTS
