@@ -86,42 +86,45 @@ template <int V> __device__ __forceinline__ float across(const Row<V>& r) {
 }
 
 // Rows that are on their way, kArrays arrays of each, some of which may be left out (null).  bf16 taken one by one, 2 bytes, come through registers.
-template <class T, int V, int K, int kArrays>
+template <class T, int V, int K, int kThreads, bool kFull, int kArrays>
 struct RowsAhead {
   static constexpr bool kCopies = sizeof(T) * V >= 4;
   static constexpr int kBytes = kCopies ? sizeof(T) * V : 4;
   int ahead;                     // rows that the ring holds: 2, or 1 where two do not fit
-  unsigned char* mine;           // this thread's place in the ring
-  int plane;                     // bytes of a vector of all threads
-  bool in[K];                    // whether this thread has a vector there
+  static constexpr int kPlane = kThreads * kBytes, kRow = kArrays * K * kPlane;        // bytes of a vector of all threads, of a row of the ring
+  unsigned char *mine, *other;   // this thread's place in the row that is worked on, and in the one behind it
+  int left;                      // this thread's vectors
   int columns;                   // between a thread's vectors
   const T* next[kArrays];        // this thread's first vector of the next row to fetch
   long long step[kArrays];
 
   __device__ __forceinline__ RowsAhead(int ahead, unsigned char* ring, const Group& g, int vectors) : ahead(ahead) {
     mine = ring + threadIdx.x * kBytes;
-    plane = blockDim.x * kBytes;
+    other = ahead == 2 ? mine + kRow : mine;
     columns = g.threads * V;
-#pragma unroll
-    for (int k = 0; k < K; ++k) in[k] = g.lane + k * g.threads < vectors;
+    left = (vectors - g.lane + g.threads - 1) / g.threads;
   }
+  __device__ __forceinline__ bool in(int k) const { return kFull || k < left; }
+  __device__ __forceinline__ void turn() { unsigned char* t = mine; mine = other; other = t; }
   __device__ __forceinline__ void array(int a, const void* base, long long stride, long long first, long long rows, int column) {
     next[a] = base != nullptr ? static_cast<const T*>(base) + first * stride + column : nullptr;
     step[a] = rows * stride;
   }
-  __device__ __forceinline__ unsigned char* place(int slot, int a, int k) const { return mine + ((slot * kArrays + a) * K + k) * plane; }
-  __device__ __forceinline__ void fetch(int slot, bool there) {
+  // into the row that has been worked on
+  __device__ __forceinline__ void fetch(bool there) { fetch(mine, there); }
+  __device__ __forceinline__ void fetch(unsigned char* to, bool there) {
     if (there) {
 #pragma unroll
       for (int a = 0; a < kArrays; ++a) {
         if (next[a] == nullptr) continue;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          if (!in[k]) continue;
+          if (!in(k)) continue;
+          unsigned char* place = to + (a * K + k) * kPlane;
           const T* from = next[a] + k * columns;
-          if constexpr (!kCopies) *reinterpret_cast<float*>(place(slot, a, k)) = to_float(*from);
-          else if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(place(slot, a, k))), "l"(from) : "memory");
-          else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(place(slot, a, k))), "l"(from) : "memory");
+          if constexpr (!kCopies) *reinterpret_cast<float*>(place) = to_float(*from);
+          else if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(place)), "l"(from) : "memory");
+          else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(place)), "l"(from) : "memory");
         }
         next[a] += step[a];
       }
@@ -132,9 +135,10 @@ struct RowsAhead {
     if (ahead == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  __device__ __forceinline__ Row<V> get(int slot, int a, int k) const {
-    if constexpr (!kCopies) return Row<V>::all(*reinterpret_cast<const float*>(place(slot, a, k)));
-    else { Raw<T, V> raw; raw.load(reinterpret_cast<const T*>(place(slot, a, k))); return raw.get(); }
+  __device__ __forceinline__ Row<V> get(int a, int k) const {
+    const unsigned char* place = mine + (a * K + k) * kPlane;
+    if constexpr (!kCopies) return Row<V>::all(*reinterpret_cast<const float*>(place));
+    else { Raw<T, V> raw; raw.load(reinterpret_cast<const T*>(place)); return raw.get(); }
   }
 };
 
@@ -149,46 +153,47 @@ __device__ __forceinline__ Row<V> load_weights(const void* w, int type, int at) 
   return load_state<V>(static_cast<const float*>(w) + at);
 }
 
-template <class T, int V, int K, int kThreads>
+template <class T, int V, int K, int kThreads, bool kFull>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) norm_forward_kernel(const NormParams p, int group_threads, int ahead) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float2 scratch[3][16];
   const Group g(group_threads);
   const float inv = 1.f / static_cast<float>(p.hidden);
   const long long step = static_cast<long long>(gridDim.x) * g.count, first = static_cast<long long>(blockIdx.x) * g.count + g.index;
-  RowsAhead<T, V, K, 2> rows(ahead, ring, g, p.hidden / V);
+  RowsAhead<T, V, K, kThreads, kFull, 2> rows(ahead, ring, g, p.hidden / V);
   rows.array(0, p.x, p.x_stride, first, step, g.lane * V);
   rows.array(1, p.residual, p.residual_stride, first, step, g.lane * V);
-  for (int i = 0; i < ahead; ++i) rows.fetch(i, first + i * step < p.rows);
+  rows.fetch(rows.mine, first < p.rows);
+  if (ahead == 2) rows.fetch(rows.other, first + step < p.rows);
   T* y = static_cast<T*>(p.y) + first * p.hidden + g.lane * V;
   T* sum = p.sum != nullptr ? static_cast<T*>(p.sum) + first * p.hidden + g.lane * V : nullptr;
-  int turn = 0, slot = 0;
+  int turn = 0;
   // (all groups of a block take as many turns as its first one, for the barriers)
-  for (long long row = first, lead = first - g.index; lead < p.rows; row += step, lead += step, y += step * p.hidden, slot = ahead == 2 ? slot ^ 1 : 0) {
+  for (long long row = first, lead = first - g.index; lead < p.rows; row += step, lead += step, y += step * p.hidden, rows.turn()) {
     const bool there = row < p.rows;
     rows.wait();
     Row<V> s[K], total = Row<V>::all(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       s[k] = Row<V>::all(0.f);
-      if (there && rows.in[k]) {
-        s[k] = rows.get(slot, 0, k);
+      if (there && rows.in(k)) {
+        s[k] = rows.get(0, k);
         if (p.residual != nullptr) {
-          s[k] = s[k] + rows.get(slot, 1, k);
+          s[k] = s[k] + rows.get(1, k);
           store_row<T, V>(sum + k * rows.columns, s[k]);
         }
         total = total + s[k];
       }
     }
     if (sum != nullptr) sum += step * p.hidden;
-    rows.fetch(slot, row + ahead * step < p.rows);
+    rows.fetch(row + ahead * step < p.rows);
     float mean = 0.f;
     if (p.center) mean = g.sum(across(total), scratch, turn) * inv;
     const Row<V> minus = Row<V>::all(-mean);
     total = Row<V>::all(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (rows.in[k]) {
+      if (rows.in(k)) {
         s[k] = s[k] + minus;
         total = fused(s[k], s[k], total);
       }
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) norm_forward_kernel
     const Row<V> scale = Row<V>::all(rstd);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (!rows.in[k]) continue;
+      if (!rows.in(k)) continue;
       Row<V> u = s[k] * scale;
       const int at = g.lane * V + k * rows.columns;
       if (p.weight != nullptr && p.bias != nullptr) u = fused(u, load_weights<V>(p.weight, p.weight_type, at), load_weights<V>(p.bias, p.weight_type, at));
@@ -209,26 +214,27 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) norm_forward_kernel
   }
 }
 
-template <class T, int V, int K, int kThreads>
+template <class T, int V, int K, int kThreads, bool kFull>
 __global__ void __launch_bounds__(kThreads, 512 / kThreads) norm_backward_kernel(const NormGradParams p, int group_threads, int ahead) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float2 scratch[3][16];
   const Group g(group_threads);
   const float inv = 1.f / static_cast<float>(p.hidden);
   const long long step = static_cast<long long>(gridDim.x) * g.count, first = static_cast<long long>(blockIdx.x) * g.count + g.index;
-  RowsAhead<T, V, K, 4> rows(ahead, ring, g, p.hidden / V);
+  RowsAhead<T, V, K, kThreads, kFull, 4> rows(ahead, ring, g, p.hidden / V);
   rows.array(0, p.x, p.x_stride, first, step, g.lane * V);
   rows.array(1, p.dy, p.dy_stride, first, step, g.lane * V);
   rows.array(2, p.residual, p.residual_stride, first, step, g.lane * V);
   rows.array(3, p.dsum, p.dsum_stride, first, step, g.lane * V);
-  for (int i = 0; i < ahead; ++i) rows.fetch(i, first + i * step < p.rows);
+  rows.fetch(rows.mine, first < p.rows);
+  if (ahead == 2) rows.fetch(rows.other, first + step < p.rows);
   Row<V> dw[K], db[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) dw[k] = db[k] = Row<V>::all(0.f);
   T* dx = p.dx != nullptr ? static_cast<T*>(p.dx) + first * p.hidden + g.lane * V : nullptr;
   float2 next_stats = first < p.rows ? p.stats[first] : make_float2(0.f, 0.f);
-  int turn = 0, slot = 0;
-  for (long long row = first, lead = first - g.index; lead < p.rows; row += step, lead += step, slot = ahead == 2 ? slot ^ 1 : 0) {
+  int turn = 0;
+  for (long long row = first, lead = first - g.index; lead < p.rows; row += step, lead += step, rows.turn()) {
     const bool there = row < p.rows;
     const float2 st = next_stats;
     if (row + step < p.rows) next_stats = p.stats[row + step];
@@ -237,11 +243,11 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) norm_backward_kernel
     Row<V> u[K], d[K], sum_d = Row<V>::all(0.f), sum_du = Row<V>::all(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (!there || !rows.in[k]) continue;
-      u[k] = rows.get(slot, 0, k);
-      if (p.residual != nullptr) u[k] = u[k] + rows.get(slot, 2, k);
+      if (!there || !rows.in(k)) continue;
+      u[k] = rows.get(0, k);
+      if (p.residual != nullptr) u[k] = u[k] + rows.get(2, k);
       u[k] = (u[k] + minus) * scale;
-      d[k] = rows.get(slot, 1, k);
+      d[k] = rows.get(1, k);
       dw[k] = fused(d[k], u[k], dw[k]);
       db[k] = db[k] + d[k];
       if (p.weight != nullptr) d[k] = d[k] * load_weights<V>(p.weight, p.weight_type, g.lane * V + k * rows.columns);
@@ -253,13 +259,13 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) norm_backward_kernel
       const Row<V> minus_d = Row<V>::all(p.center ? -sums.x * inv : 0.f), minus_du = Row<V>::all(-sums.y * inv);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        if (!there || !rows.in[k]) continue;
+        if (!there || !rows.in(k)) continue;
         const Row<V> v = fused(u[k], minus_du, d[k] + minus_d);
-        store_row<T, V>(dx + k * rows.columns, p.dsum != nullptr ? fused(v, scale, rows.get(slot, 3, k)) : v * scale);
+        store_row<T, V>(dx + k * rows.columns, p.dsum != nullptr ? fused(v, scale, rows.get(3, k)) : v * scale);
       }
       dx += step * p.hidden;
     }
-    rows.fetch(slot, row + ahead * step < p.rows);
+    rows.fetch(row + ahead * step < p.rows);
   }
   if (p.parts == nullptr) return;
   // the groups' sums, one after another, in place of the ring
@@ -270,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) norm_backward_kernel
     if (g.index != q) continue;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (!rows.in[k]) continue;
+      if (!rows.in(k)) continue;
       const int at = g.lane * V + k * rows.columns;
       if (q < g.count - 1) {
         dw[k] = dw[k] + load_state<V>(all + at);
@@ -399,7 +405,9 @@ Form form_of(int half, int hidden, bool sixteen, bool four) {
   if (hidden > kMostColumns) return f;
   f.vec = sixteen ? (half ? 8 : 4) : half && four ? 2 : 1;
   const int vectors = hidden / f.vec;
-  f.each = vectors <= 32 ? 1 : 16 / f.vec;
+  // Few vectors a thread keep short rows of single numbers and pairs from waiting for one another's loads: 1777 rows of 1001 fp32 columns with 16 a
+  // thread 19.5 us, with 4 XXX.  (Whole vectors the other way: 8192 rows of 2048 with one a thread 32.9, with two 27.9.)
+  f.each = vectors <= 32 ? 1 : f.vec == 1 && vectors <= 1024 ? 4 : f.vec == 2 && vectors <= 512 ? 2 : 16 / f.vec;
   f.threads = (vectors + f.each - 1) / f.each;                 // whole warps; more than half of them, a block that is not full
   f.threads = (f.threads + 31) / 32 * 32;
   return f;
@@ -442,18 +450,19 @@ template <class F>
 cudaError_t by_form(int half, const Form& f, F run) {
   using H = __nv_bfloat16;
   using std::integral_constant;
-  if (half) {
-    if (f.vec == 8) return f.each == 1 ? run(H{}, integral_constant<int, 8>{}, integral_constant<int, 1>{}) : run(H{}, integral_constant<int, 8>{}, integral_constant<int, 2>{});
-    if (f.vec == 2) return f.each == 1 ? run(H{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}) : run(H{}, integral_constant<int, 2>{}, integral_constant<int, 8>{});
-    return f.each == 1 ? run(H{}, integral_constant<int, 1>{}, integral_constant<int, 1>{}) : run(H{}, integral_constant<int, 1>{}, integral_constant<int, 16>{});
-  }
-  if (f.vec == 4) return f.each == 1 ? run(float{}, integral_constant<int, 4>{}, integral_constant<int, 1>{}) : run(float{}, integral_constant<int, 4>{}, integral_constant<int, 4>{});
-  return f.each == 1 ? run(float{}, integral_constant<int, 1>{}, integral_constant<int, 1>{}) : run(float{}, integral_constant<int, 1>{}, integral_constant<int, 16>{});
+  auto with = [&](auto type, auto vec) {
+    constexpr int V = decltype(vec)::value;
+    if (f.each == 1) return run(type, vec, integral_constant<int, 1>{});
+    if constexpr (V <= 2) { if (f.each == 4 / V) return run(type, vec, integral_constant<int, 4 / V>{}); }
+    return run(type, vec, integral_constant<int, 16 / V>{});
+  };
+  if (!half) return f.vec == 4 ? with(float{}, integral_constant<int, 4>{}) : with(float{}, integral_constant<int, 1>{});
+  return f.vec == 8 ? with(H{}, integral_constant<int, 8>{}) : f.vec == 2 ? with(H{}, integral_constant<int, 2>{}) : with(H{}, integral_constant<int, 1>{});
 }
 // Bytes of a ring of one row.
 int ring_of(const Form& f, int half, int arrays) {
   const int bytes = f.vec * (half ? 2 : 4);
-  return arrays * f.each * threads_of(f) * (bytes < 4 ? 4 : bytes);
+  return arrays * f.each * (f.threads > kGroupThreads ? 512 : kGroupThreads) * (bytes < 4 ? 4 : bytes);
 }
 constexpr int kMostRing = 160 * 1024;
 
@@ -487,8 +496,13 @@ cudaError_t launch_norm_forward(const NormParams& p, int sms, cudaStream_t strea
       using T = decltype(type);
       constexpr int V = decltype(vec)::value, K = decltype(each)::value;
       const int blocks = blocks_of(f, p.rows, sms, resident_forward(f)), ring = 2 * ring_of(f, half, 2);
-      return f.threads > kGroupThreads ? launch_rows<norm_forward_kernel<T, V, K, 512>>(p, f, blocks, ring, 2, stream)
-                                       : launch_rows<norm_forward_kernel<T, V, K, 256>>(p, f, blocks, ring, 2, stream);
+      // (rows that all threads have K vectors of, such as those of 2048 and 7168 columns, without a look whether they do)
+      constexpr bool kCan = V == 8 && K == 2;
+      if (kCan && f.threads * K * V == p.hidden)
+        return f.threads > kGroupThreads ? launch_rows<norm_forward_kernel<T, V, K, 512, kCan>>(p, f, blocks, ring, 2, stream)
+                                         : launch_rows<norm_forward_kernel<T, V, K, 256, kCan>>(p, f, blocks, ring, 2, stream);
+      return f.threads > kGroupThreads ? launch_rows<norm_forward_kernel<T, V, K, 512, false>>(p, f, blocks, ring, 2, stream)
+                                       : launch_rows<norm_forward_kernel<T, V, K, 256, false>>(p, f, blocks, ring, 2, stream);
     });
   const int blocks = row_blocks(p.rows, sms);
   if (half) norm_forward_any_kernel<__nv_bfloat16><<<blocks, kRowThreads, 0, stream>>>(p);
@@ -506,8 +520,12 @@ cudaError_t launch_norm_backward(const NormGradParams& p, int sms, cudaStream_t 
       using T = decltype(type);
       constexpr int V = decltype(vec)::value, K = decltype(each)::value;
       const int smem = ring > sums ? ring : sums;
-      return f.threads > kGroupThreads ? launch_rows<norm_backward_kernel<T, V, K, 512>>(p, f, parts, smem, ahead, stream)
-                                       : launch_rows<norm_backward_kernel<T, V, K, 256>>(p, f, parts, smem, ahead, stream);
+      constexpr bool kCan = V == 8 && K == 2;
+      if (kCan && f.threads * K * V == p.hidden)
+        return f.threads > kGroupThreads ? launch_rows<norm_backward_kernel<T, V, K, 512, kCan>>(p, f, parts, smem, ahead, stream)
+                                         : launch_rows<norm_backward_kernel<T, V, K, 256, kCan>>(p, f, parts, smem, ahead, stream);
+      return f.threads > kGroupThreads ? launch_rows<norm_backward_kernel<T, V, K, 512, false>>(p, f, parts, smem, ahead, stream)
+                                       : launch_rows<norm_backward_kernel<T, V, K, 256, false>>(p, f, parts, smem, ahead, stream);
     });
   } else {
     const int blocks = row_blocks(p.rows, sms);
