@@ -28,7 +28,7 @@ _module = None
 
 SOURCES = ["runtime.cpp", "comm_kernels.cu", "local_kernels.cu", "router_kernels.cu", "gemm_kernels.cu", "gemm_inst_swiglu.cu", "gemm_inst_dswiglu.cu",
            "gemm_inst_scatter.cu", "gemm_inst_store.cu", "gemm_inst_dw.cu", "linear_loss_kernels.cu", "linear_loss.cpp", "list_kernels.cu", "list_ops.cpp",
-           "norm_kernels.cu", "norm.cpp", "scan_kernels.cu", "scan.cpp", "route_kernels.cu", "route.cpp"]
+           "norm_kernels.cu", "norm.cpp", "scan_kernels.cu", "scan.cpp", "route_kernels.cu", "route_grad_kernels.cu", "route.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

@@ -91,12 +91,16 @@ class BalancedRoute : public torch::autograd::Function<BalancedRoute> {
     const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
     const int64_t T = x.size(0), H = x.size(1), E = w_gate.size(0);
     const c10::cuda::CUDAGuard guard(x.device());
+    // A thread of the autograd engine may not have made a call of the CUDA runtime yet, and the driver encodes tensor maps only
+    // with a context bound to the thread.
+    SEP_CUDA_CHECK(cudaSetDevice(x.get_device()));
     at::Tensor dx, dw;
     if (want_dx) dx = at::empty({T, H}, x.options());
     if (want_dw) dw = T > 0 ? at::empty({E, H}, w_gate.options()) : at::zeros({E, H}, w_gate.options());
     if (T > 0) {
-      const LaunchContext context = call->context(1 + (want_dx ? 1 : 0) + (want_dw ? 1 : 0));
-      const at::Tensor xr = readable(x), wr = readable(w_gate), dlogits = at::empty({T, E}, probs.options());
+      const LaunchContext context = call->context(want_dw ? 3 : 1);
+      const at::Tensor xr = readable(x), wr = readable(w_gate);
+      const RouteGradPlan plan = route_grad_plan(static_cast<int>(T), static_cast<int>(H), static_cast<int>(E), context.sms);
       at::Tensor up[3];
       for (int i = 0; i < 3; ++i) {
         const at::Tensor& g = grads[i == 0 ? 1 : i + 2];
@@ -111,11 +115,28 @@ class BalancedRoute : public torch::autograd::Function<BalancedRoute> {
       p.dweights = up[0].defined() ? up[0].data_ptr<float>() : nullptr;
       p.dbalance = up[1].defined() ? up[1].data_ptr<float>() : nullptr;
       p.dz_loss = up[2].defined() ? up[2].data_ptr<float>() : nullptr;
-      p.dlogits = dlogits.data_ptr<float>();
-      p.x = xr.data_ptr(); p.w_gate = wr.data_ptr();
       p.dx = want_dx ? dx.data_ptr() : nullptr;
       p.dw = want_dw ? dw.data_ptr() : nullptr;
-      SEP_CUDA_CHECK(launch_route_backward(p, context.stream));
+      p.status = context.status; p.rank = context.rank; p.wait_budget_ns = context.wait_budget_ns;
+      at::Tensor space;                          // dz, and the parts of dw
+      const int64_t dz_bytes = (T * plan.padded * 2 + 255) / 256 * 256, parts = plan.dw_splits > 1 ? plan.dw_splits : 0;
+      if (want_dw) {
+        space = at::empty({dz_bytes + parts * E * H * 4}, x.options().dtype(at::kByte));
+        p.dz = space.data_ptr();
+      }
+      CUtensorMap map_w{}, map_dx{};
+      if (want_dx) {
+        map_w = make_tmap(wr.data_ptr(), H, E, 1, H, E * H, 64, 64);
+        map_dx = make_tmap(p.dx, H, T, 1, H, T * H, 64, 32);
+      }
+      SEP_CUDA_CHECK(launch_route_dx(p, plan, &map_w, &map_dx, context.stream));
+      if (want_dw) {
+        float* sums = reinterpret_cast<float*>(static_cast<char*>(space.data_ptr()) + dz_bytes);
+        const CUtensorMap map_dz = make_tmap(p.dz, plan.padded, T, 1, plan.padded, T * plan.padded, 64, 64), map_x = make_tmap(xr.data_ptr(), H, T, 1, H, T * H, 64, 64),
+                          map_out = parts > 0 ? make_tmap(sums, H, E, parts, H, E * H, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT32)
+                                              : make_tmap(p.dw, H, E, 1, H, E * H, 64, 32);
+        SEP_CUDA_CHECK(launch_route_dw(p, plan, &map_dz, &map_x, &map_out, sums, context.stream));
+      }
     }
     return {dx, dw, at::Tensor(), at::Tensor()};
   }

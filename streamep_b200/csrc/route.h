@@ -1,7 +1,9 @@
-// Routing that is trained: statistics of the router's probabilities, and its gradients (route_kernels.cu).
+// Routing that is trained: statistics of the router's probabilities, and its gradients (route_kernels.cu, route_grad_kernels.cu).
 #pragma once
 
 #include <cuda_runtime.h>
+
+#include "status.h"
 
 namespace sep {
 
@@ -34,12 +36,24 @@ struct RouteGradParams {
   const float* dweights;         // [tokens, top_k] or null
   const float* dbalance;         // one number or null
   const float* dz_loss;          // one number or null
-  float* dlogits;                // [tokens, experts]
-  const void* x;                 // [tokens, hidden] bf16
-  const void* w_gate;            // [experts, hidden] bf16
-  void* dx;                      // or null
-  void* dw;                      // or null
+  void* dz;                      // [tokens, padded] bf16: the logits' gradients, or null (no dw)
+  void* dx;                      // [tokens, hidden] bf16, or null
+  void* dw;                      // [experts, hidden] bf16, or null
+  StatusBlock* status;
+  int rank;
+  unsigned long long wait_budget_ns;
 };
-cudaError_t launch_route_backward(const RouteGradParams& p, cudaStream_t stream);
+// How the products are cut up: `padded` experts (a multiple of 64); blocks that share the columns of 128 tokens' dx; experts (in blocks of 128) and parts of
+// the tokens of a unit of dW.
+struct RouteGradPlan {
+  int padded;
+  int dx_splits, dx_stages, dx_staging, dx_smem;
+  int dw_blocks, dw_splits, dw_units, dw_stages, dw_smem;
+};
+RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms);
+// Maps: `map_w` [E, H] boxes of 64 x 64, `map_dx` [T, H] boxes of 32 rows x 64; `map_dz` [T, padded] and `map_x` [T, H] boxes of 64 x 64; `map_out` dW boxes of
+// 32 x 64 (bf16), or with several parts [splits, E, H] fp32 boxes of 32 x 32 over `parts`.  All with 128-byte swizzle.
+cudaError_t launch_route_dx(const RouteGradParams& p, const RouteGradPlan& g, const void* map_w, const void* map_dx, cudaStream_t stream);
+cudaError_t launch_route_dw(const RouteGradParams& p, const RouteGradPlan& g, const void* map_dz, const void* map_x, const void* map_out, float* parts, cudaStream_t stream);
 
 }  // namespace sep

@@ -1,0 +1,424 @@
+// Gradients of routing on the tensor cores: from the gradients of weights, balance and z loss that of the logits, dz [T, E], and from it
+//
+//   dx = dz W  [T, H]      a block takes 128 tokens: their dz is formed in shared memory, where it stays as the left operand, and W's columns go by
+//   dW = dz^T x  [E, H]    a block takes up to 256 experts, 256 columns and a part of the tokens; the parts are added up by a small kernel
+//
+// dz is rounded to bf16 for both products, 2^-9 of each term at most, as bf16 training code rounds the gradient of its logits; all sums are fp32.
+// What bounds them: x is read and dx written once (HBM), and for many experts the tensor cores.  All operands lie in memory as TMA brings them in, dz as
+// [T, experts rounded up to 64]; nothing is transposed.  Parts and sums have a fixed order: a repeated call gives the same bits.
+#include <atomic>
+#include <cuda.h>
+
+#include "ptx.cuh"
+#include "route.h"
+
+namespace sep {
+
+namespace {
+
+constexpr int kThreads = 320;                    // TMA, MMA, 8 warps of epilogue
+constexpr int kEpiWarps = 8;
+constexpr int kTokens = 128, kCols = 256, kBK = 64;
+constexpr int kChunk = 64 * 128;                 // a box of 64 x 64 bf16
+constexpr int kStaging = 4096;
+constexpr int kMostSmem = 226 * 1024;
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The gradient of one token's logits, by one warp: lane l has experts l, l + 32, ...
+template <int EPL>
+__device__ __forceinline__ void token_gradient(const RouteGradParams& p, int t, int lane, float share, float db, float dzl, float (&v)[EPL]) {
+  const float* probs = p.probs + static_cast<long long>(t) * p.experts;
+  float prob[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) prob[j] = j * 32 + lane < p.experts ? probs[j * 32 + lane] : 0.f;
+  int mine = -1;
+  float up = 0.f, w = 0.f;
+  if (lane < p.top_k && p.dweights != nullptr) {
+    const long long at = static_cast<long long>(t) * p.top_k + lane;
+    mine = static_cast<int>(p.idx[at]);
+    w = p.weights[at];
+    up = p.dweights[at];
+  }
+  const bool counts = p.mask == nullptr || p.mask[t] != 0;
+  const float cb = counts ? db * share : 0.f, cz = counts && dzl != 0.f ? 2.f * dzl * share * p.lse[t] : 0.f;
+  float load[EPL], mean_load = 0.f;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    load[j] = cb != 0.f && j * 32 + lane < p.experts ? p.load[j * 32 + lane] : 0.f;
+    mean_load = fmaf(prob[j], load[j], mean_load);
+  }
+  if (cb != 0.f) mean_load = warp_sum(mean_load);
+  // (where the weights are not normalised again, w is the probability itself)
+  const float mean_up = p.dweights != nullptr ? warp_sum(w * up) : 0.f;
+  const float at_chosen = p.renormalize ? w * (up - mean_up) : w * up;
+  const float all = p.renormalize ? 0.f : mean_up;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    v[j] = cb != 0.f ? cb * prob[j] * (load[j] - mean_load) : 0.f;
+    if (cz != 0.f) v[j] = fmaf(cz, prob[j], v[j]);
+    v[j] = fmaf(-all, prob[j], v[j]);
+  }
+  if (p.dweights != nullptr) {
+    for (int k = 0; k < p.top_k; ++k) {
+      const int chosen = __shfl_sync(0xffffffffu, mine, k);
+      const float add = __shfl_sync(0xffffffffu, at_chosen, k);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j)
+        if (chosen == j * 32 + lane) v[j] += add;
+    }
+  }
+}
+
+// A failed wait: the copies that this thread may have in flight land before the block leaves (bounded).
+__device__ __forceinline__ void give_up(StatusBlock* status, int role, int rank, int where) {
+  report_failure(status, kStatusTimeoutPipeline, kKernelRoute, role, rank, where, 0, 0);
+  const unsigned long long t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 2000000ull) {}
+}
+
+// 32 rows and 64 columns of an accumulator leave as bf16.
+__device__ __forceinline__ void store_half_tile(uint32_t taddr, unsigned char* tile, const CUtensorMap* map, int x, int y, int lane) {
+  uint32_t a[32], b[32];
+  tmem_ld_32x32(taddr, a);
+  tmem_ld_32x32(taddr + 32, b);
+  tmem_ld_wait();
+  const uint32_t stg = smem_u32(tile);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    uint32_t o[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int i = (q & 3) * 8 + h * 2;
+      o[h] = pack_bf16x2(__uint_as_float(q < 4 ? a[i] : b[i]), __uint_as_float(q < 4 ? a[i + 1] : b[i + 1]));
+    }
+    st_shared_v4(stg + stage_off<128>(lane, q), o[0], o[1], o[2], o[3]);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) { tma_store_3d(map, tile, x, y, 0); bulk_commit(); }
+}
+
+template <int EPL>
+__global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_dx, const RouteGradParams p,
+                                                               const RouteGradPlan g) {
+  extern __shared__ unsigned char smem_dyn[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full_bar[4], empty_bar[4], tmem_full[2], tmem_empty[2], dz_bar;
+  __shared__ uint32_t s_tmem;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = static_cast<int>(blockIdx.x) / g.dx_splits, split = static_cast<int>(blockIdx.x) % g.dx_splits;
+  const int k_blocks = g.padded / kBK, n_tiles = p.dx != nullptr ? (p.hidden + kCols - 1) / kCols : 0;
+  const int n0 = n_tiles * split / g.dx_splits, n1 = n_tiles * (split + 1) / g.dx_splits;
+  unsigned char* dz = smem;                      // [k_blocks][128 rows][128 bytes]
+  unsigned char* stages = dz + k_blocks * kTokens * 128;
+  unsigned char* staging = stages + g.dx_stages * 4 * kChunk;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_w);
+    for (int s = 0; s < g.dx_stages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&tmem_full[b], 1); mbar_init(&tmem_empty[b], kEpiWarps); }
+    mbar_init(&dz_bar, kEpiWarps);
+    mbar_fence_init();
+  }
+  if (warp == 1) { tmem_alloc<1>(&s_tmem, 512); tmem_relinquish<1>(); }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0; uint32_t phase = 0; bool ok = true;
+      for (int n = n0; n < n1 && ok; ++n) {
+        const int chunks = (min(kCols, p.hidden - n * kCols) + 63) / 64;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, p.wait_budget_ns, p.status)) { ok = false; break; }
+          mbar_arrive_expect_tx(&full_bar[stage], chunks * kChunk);
+          for (int c = 0; c < chunks; ++c) tma_load_3d(stages + (stage * 4 + c) * kChunk, &map_w, &full_bar[stage], n * kCols + c * 64, kb * kBK, 0);
+          if (++stage == g.dx_stages) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) give_up(p.status, 0, p.rank, tile);
+    }
+  } else if (warp == 1) {
+    bool ok = __all_sync(0xffffffffu, mbar_wait(&dz_bar, 0, p.wait_budget_ns, p.status));
+    int stage = 0, acc = 0; uint32_t phase = 0, acc_phase = 0;
+    for (int n = n0; n < n1 && ok; ++n) {
+      const int cols = min(kCols, (p.hidden - n * kCols + 31) / 32 * 32);
+      const uint32_t idesc = umma_idesc_bf16(kTokens, 0, 0, 1) | (static_cast<uint32_t>(cols >> 3) << 17);
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[acc], acc_phase ^ 1, p.wait_budget_ns, p.status))) { ok = false; break; }
+      tc_fence_after_sync();
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, p.wait_budget_ns, p.status))) { ok = false; break; }
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t a = smem_u32(dz + kb * kTokens * 128), b = smem_u32(stages + stage * 4 * kChunk);
+#pragma unroll
+          for (int j = 0; j < kBK / 16; ++j)
+            umma_bf16_ss<1>(tmem + acc * kCols, umma_smem_desc(a + j * 32, 16, 1024), umma_smem_desc(b + j * 16 * 128, kChunk, 1024), idesc, (kb > 0 || j > 0) ? 1u : 0u);
+          umma_commit<1>(&empty_bar[stage]);
+          if (kb == k_blocks - 1) umma_commit<1>(&tmem_full[acc]);
+        }
+        __syncwarp();
+        if (++stage == g.dx_stages) { stage = 0; phase ^= 1; }
+      }
+      acc ^= 1; if (acc == 0) acc_phase ^= 1;
+    }
+    if (!ok && lane == 0) report_failure(p.status, kStatusTimeoutPipeline, kKernelRoute, 1, p.rank, tile, 0, 0);
+  } else {
+    const int w = warp - 2, quarter = warp & 3, side = w >> 2;
+    const float share = p.load[p.experts], db = p.dbalance != nullptr ? *p.dbalance : 0.f, dzl = p.dz_loss != nullptr ? *p.dz_loss : 0.f;
+    for (int r = w; r < kTokens; r += kEpiWarps) {
+      const int t = tile * kTokens + r;
+      float v[EPL];
+      if (t < p.tokens) token_gradient<EPL>(p, t, lane, share, db, dzl, v);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        const int e = j * 32 + lane;
+        if (e >= g.padded) continue;
+        const __nv_bfloat16 b = __float2bfloat16_rn(t < p.tokens && e < p.experts ? v[j] : 0.f);
+        *reinterpret_cast<__nv_bfloat16*>(dz + e / 64 * kTokens * 128 + stage_off<128>(r, e % 64 / 8) + e % 8 * 2) = b;
+        if (split == 0 && t < p.tokens && p.dz != nullptr) static_cast<__nv_bfloat16*>(p.dz)[static_cast<long long>(t) * g.padded + e] = b;
+      }
+      if (EPL == 1 && g.padded > 32) {           // (the second half of a block of 64)
+        *reinterpret_cast<__nv_bfloat16*>(dz + stage_off<128>(r, (32 + lane) / 8) + lane % 8 * 2) = __float2bfloat16_rn(0.f);
+        if (split == 0 && t < p.tokens && p.dz != nullptr) static_cast<__nv_bfloat16*>(p.dz)[static_cast<long long>(t) * g.padded + 32 + lane] = __float2bfloat16_rn(0.f);
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&dz_bar);
+    int acc = 0, flip = 0; uint32_t acc_phase = 0;
+    unsigned char* const mine = staging + w * g.dx_staging * kStaging;
+    const int row0 = tile * kTokens + quarter * 32;
+    for (int n = n0; n < n1; ++n) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], acc_phase, p.wait_budget_ns, p.status))) {
+        if (lane == 0) report_failure(p.status, kStatusTimeoutPipeline, kKernelRoute, 2, p.rank, tile, n, 0);
+        break;
+      }
+      tc_fence_after_sync();
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 64) {
+        const int col = side * 128 + c;
+        if (n * kCols + col >= p.hidden || row0 >= p.tokens) continue;
+        if (lane == 0) { if (g.dx_staging == 2) bulk_wait_read_but_one(); else bulk_wait_read(); }
+        __syncwarp();
+        store_half_tile(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kCols + col, mine + flip * kStaging, &map_dx, n * kCols + col, row0, lane);
+        if (g.dx_staging == 2) flip ^= 1;
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+      acc ^= 1; if (acc == 0) acc_phase ^= 1;
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<1>(tmem, 512); }
+}
+
+// A unit: `g.dw_blocks` blocks of 128 experts, 256 columns, a part of the tokens.
+__global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_constant__ CUtensorMap map_dz, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out,
+                                                               const RouteGradParams p, const RouteGradPlan g) {
+  extern __shared__ unsigned char smem_dyn[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full_bar[4], empty_bar[4], done_bar;
+  __shared__ uint32_t s_tmem;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_tiles = (p.hidden + kCols - 1) / kCols;
+  const int n = static_cast<int>(blockIdx.x) % n_tiles, rest = static_cast<int>(blockIdx.x) / n_tiles, split = rest % g.dw_splits, group = rest / g.dw_splits;
+  const int all_blocks = (p.experts + 127) / 128, m0 = group * g.dw_blocks, blocks = min(g.dw_blocks, all_blocks - m0);
+  const int k_blocks = (p.tokens + kBK - 1) / kBK, kb0 = static_cast<int>(static_cast<long long>(k_blocks) * split / g.dw_splits),
+            kb1 = static_cast<int>(static_cast<long long>(k_blocks) * (split + 1) / g.dw_splits);
+  const int chunks = (min(kCols, p.hidden - n * kCols) + 63) / 64, cols = min(kCols, (p.hidden - n * kCols + 31) / 32 * 32);
+  const int stage_bytes = (g.dw_blocks * 2 + 4) * kChunk, tmem_cols = g.dw_blocks * kCols;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_dz);
+    tma_prefetch_desc(&map_x);
+    for (int s = 0; s < g.dw_stages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    mbar_init(&done_bar, 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) { tmem_alloc<1>(&s_tmem, tmem_cols); tmem_relinquish<1>(); }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0; uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1, p.wait_budget_ns, p.status)) { give_up(p.status, 3, p.rank, static_cast<int>(blockIdx.x)); break; }
+        unsigned char* s = smem + stage * stage_bytes;
+        // (experts beyond the padded ones: chunks outside are not fetched, and their rows of the result not stored)
+        const int left = min(blocks * 2, g.padded / 64 - m0 * 2);
+        mbar_arrive_expect_tx(&full_bar[stage], (left + chunks) * kChunk);
+        for (int c = 0; c < left; ++c) tma_load_3d(s + c * kChunk, &map_dz, &full_bar[stage], (m0 * 2 + c) * 64, kb * kBK, 0);
+        for (int c = 0; c < chunks; ++c) tma_load_3d(s + (g.dw_blocks * 2 + c) * kChunk, &map_x, &full_bar[stage], n * kCols + c * 64, kb * kBK, 0);
+        if (++stage == g.dw_stages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = umma_idesc_bf16(128, 0, 1, 1) | (static_cast<uint32_t>(cols >> 3) << 17);
+    int stage = 0; uint32_t phase = 0; bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, p.wait_budget_ns, p.status))) { ok = false; break; }
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + g.dw_blocks * 2 * kChunk;
+        for (int m = 0; m < blocks; ++m)
+#pragma unroll
+          for (int j = 0; j < kBK / 16; ++j)
+            umma_bf16_ss<1>(tmem + m * kCols, umma_smem_desc(a + m * 2 * kChunk + j * 16 * 128, kChunk, 1024), umma_smem_desc(b + j * 16 * 128, kChunk, 1024), idesc,
+                            (kb > kb0 || j > 0) ? 1u : 0u);
+        umma_commit<1>(&empty_bar[stage]);
+        if (kb == kb1 - 1) umma_commit<1>(&done_bar);
+      }
+      __syncwarp();
+      if (++stage == g.dw_stages) { stage = 0; phase ^= 1; }
+    }
+    if (!ok && lane == 0) report_failure(p.status, kStatusTimeoutPipeline, kKernelRoute, 4, p.rank, static_cast<int>(blockIdx.x), 0, 0);
+  } else {
+    // (the operands' place is free once the products are done)
+    const bool have = kb1 > kb0;
+    const bool ok = !have || __all_sync(0xffffffffu, mbar_wait(&done_bar, 0, p.wait_budget_ns, p.status));
+    if (!ok && lane == 0) report_failure(p.status, kStatusTimeoutPipeline, kKernelRoute, 5, p.rank, static_cast<int>(blockIdx.x), 0, 0);
+    if (ok) {
+      tc_fence_after_sync();
+      const int w = warp - 2, quarter = warp & 3, side = w >> 2;
+      unsigned char* const mine = smem + w * 2 * kStaging;
+      int flip = 0;
+      for (int m = 0; m < blocks; ++m) {
+        const int row0 = (m0 + m) * 128 + quarter * 32;
+        if (row0 >= p.experts) continue;
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + m * kCols;
+        for (int c = side * 128; c < side * 128 + 128; c += g.dw_splits > 1 ? 32 : 64) {
+          if (n * kCols + c >= p.hidden) break;
+          if (lane == 0) bulk_wait_read_but_one();
+          __syncwarp();
+          unsigned char* tile = mine + flip * kStaging;
+          flip ^= 1;
+          if (g.dw_splits == 1) {
+            store_half_tile(taddr + c, tile, &map_out, n * kCols + c, row0, lane);
+            continue;
+          }
+          uint32_t r[32];
+          tmem_ld_32x32(taddr + c, r);
+          tmem_ld_wait();
+          const uint32_t stg = smem_u32(tile);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) st_shared_v4(stg + stage_off<128>(lane, q), r[q * 4], r[q * 4 + 1], r[q * 4 + 2], r[q * 4 + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) { tma_store_3d(&map_out, tile, n * kCols + c, row0, split); bulk_commit(); }
+        }
+      }
+      if (lane == 0) bulk_wait_all();
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<1>(tmem, tmem_cols); }
+}
+
+// The sum of the parts of dW, 8 elements a thread.
+__global__ void __launch_bounds__(256) route_dw_join_kernel(const float* parts, void* dw, long long elements, int splits) {
+  grid_wait();
+  const long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 8;
+  if (i >= elements) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float4* at = reinterpret_cast<const float4*>(parts + s * elements + i);
+    const float4 u = at[0], v = at[1];
+    a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+    b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+  }
+  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(dw) + i) = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+}
+
+template <auto kKernel, class... Args>
+cudaError_t launch(unsigned grid, int smem, cudaStream_t stream, const Args&... args) {
+  static std::atomic<bool> configured[64];       // the shared-memory limit is an attribute of the function on a device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    if ((e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)) != cudaSuccess) return e;
+    configured[dev].store(true, std::memory_order_release);
+  }
+  kKernel<<<grid, kThreads, smem, stream>>>(args...);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
+  RouteGradPlan g{};
+  g.padded = (experts + 63) / 64 * 64;
+  const int tiles = (tokens + kTokens - 1) / kTokens, n_tiles = (hidden + kCols - 1) / kCols;
+  // dx: a block forms the gradient of its tokens' logits, so several for the same tokens only where there are few
+  g.dx_splits = tiles > 0 ? sms / tiles : 1;
+  if (g.dx_splits > n_tiles) g.dx_splits = n_tiles;
+  if (g.dx_splits < 1) g.dx_splits = 1;
+  g.dx_staging = g.padded <= 256 ? 2 : 1;
+  const int fixed = 1024 + g.padded * kTokens * 2 + kEpiWarps * g.dx_staging * kStaging;
+  g.dx_stages = (kMostSmem - fixed) / (4 * kChunk);
+  if (g.dx_stages > 4) g.dx_stages = 4;
+  g.dx_smem = fixed + g.dx_stages * 4 * kChunk;
+  // dW: tokens are split to fill the GPU, into no shorter parts than 4 blocks of 64, and rather into whole rounds of all SMs
+  const int blocks = (experts + 127) / 128;
+  g.dw_blocks = blocks > 1 ? 2 : 1;
+  const int units = (blocks + g.dw_blocks - 1) / g.dw_blocks * n_tiles, most = (tokens + 4 * kBK - 1) / (4 * kBK);
+  int best = 1;
+  double best_time = 0.0;
+  for (int s = 1; s <= most && s <= 64; ++s) {
+    const int rounds = (units * s + sms - 1) / sms;
+    // a round's blocks of tokens, and what an output tile costs: about as much as 6 blocks
+    const double time = rounds * (static_cast<double>((tokens + kBK - 1) / kBK) / s + 6.0);
+    if (s == 1 || time < best_time) { best = s; best_time = time; }
+  }
+  g.dw_splits = best;
+  g.dw_stages = g.dw_blocks == 2 ? 3 : 4;
+  g.dw_smem = 1024 + g.dw_stages * (g.dw_blocks * 2 + 4) * kChunk;
+  g.dw_units = units * best;
+  return g;
+}
+
+cudaError_t launch_route_dx(const RouteGradParams& p, const RouteGradPlan& g, const void* map_w, const void* map_dx, cudaStream_t stream) {
+  const CUtensorMap &mw = *static_cast<const CUtensorMap*>(map_w), &mdx = *static_cast<const CUtensorMap*>(map_dx);
+  const unsigned grid = static_cast<unsigned>((p.tokens + kTokens - 1) / kTokens * (p.dx != nullptr ? g.dx_splits : 1));
+  RouteGradPlan q = g;
+  if (p.dx == nullptr) q.dx_splits = 1;
+  if (p.experts <= 32) return launch<route_dx_kernel<1>>(grid, g.dx_smem, stream, mw, mdx, p, q);
+  if (p.experts <= 64) return launch<route_dx_kernel<2>>(grid, g.dx_smem, stream, mw, mdx, p, q);
+  if (p.experts <= 128) return launch<route_dx_kernel<4>>(grid, g.dx_smem, stream, mw, mdx, p, q);
+  if (p.experts <= 256) return launch<route_dx_kernel<8>>(grid, g.dx_smem, stream, mw, mdx, p, q);
+  return launch<route_dx_kernel<16>>(grid, g.dx_smem, stream, mw, mdx, p, q);
+}
+
+cudaError_t launch_route_dw(const RouteGradParams& p, const RouteGradPlan& g, const void* map_dz, const void* map_x, const void* map_out, float* parts, cudaStream_t stream) {
+  const CUtensorMap &mz = *static_cast<const CUtensorMap*>(map_dz), &mx = *static_cast<const CUtensorMap*>(map_x), &mo = *static_cast<const CUtensorMap*>(map_out);
+  const cudaError_t e = launch<route_dw_kernel>(static_cast<unsigned>(g.dw_units), g.dw_smem, stream, mz, mx, mo, p, g);
+  if (e != cudaSuccess || g.dw_splits == 1) return e;
+  const long long elements = static_cast<long long>(p.experts) * p.hidden;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((elements / 8 + 255) / 256));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, route_dw_join_kernel, static_cast<const float*>(parts), p.dw, elements, g.dw_splits);
+}
+
+}  // namespace sep

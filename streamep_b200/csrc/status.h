@@ -34,7 +34,7 @@ struct StatusBlock {
 
 enum KernelId : int {
   kKernelMetadata = 1, kKernelFill = 2, kKernelDispatch = 3, kKernelDispatchGrads = 4,
-  kKernelCombine = 5, kKernelGemm = 6, kKernelBarrier = 7, kKernelProducer = 8, kKernelLoss = 9, kKernelScan = 10,
+  kKernelCombine = 5, kKernelGemm = 6, kKernelBarrier = 7, kKernelProducer = 8, kKernelLoss = 9, kKernelScan = 10, kKernelRoute = 11,
 };
 
 }  // namespace sep
