@@ -308,7 +308,7 @@ struct RouterParams {
   float* topk_weights;  // [T, K]
   unsigned char* is_token_in_rank;  // [T, R]
   float* probs;         // optional [T, E] softmax output (for the backward), may be null
-  float* lse;           // optional [T] log of the sum of exponentials, may be null
+  float* lse;           // [T] log of the sum of exponentials (of routing that is trained)
 };
 void launch_router(const RouterParams& p, cudaStream_t stream);
 // The tensor-core router in one launch: `map_w` [E, H] with boxes of 128 x 64 and `map_x` [T, H] with boxes of

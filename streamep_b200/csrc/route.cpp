@@ -38,35 +38,32 @@ Route route_forward(const RouteCall& call, const at::Tensor& x, const at::Tensor
   r.probs = at::empty({T, E}, f32);
   r.lse = at::empty({T}, f32);
   r.load = at::empty({E + 1}, f32);
-  const LaunchContext ctx = call.context(T > 0 ? 3 : 1);
-  if (T > 0) {
-    RouterParams p{};
-    p.x = x.data_ptr(); p.w_gate = w.data_ptr();
-    p.num_tokens = static_cast<int>(T); p.hidden = static_cast<int>(H); p.num_experts = static_cast<int>(E); p.num_topk = call.top_k;
-    p.num_ranks = call.num_ranks; p.renormalize = call.renormalize ? 1 : 0;
-    p.topk_idx = reinterpret_cast<long long*>(r.idx.data_ptr<int64_t>());
-    p.topk_weights = r.weights.data_ptr<float>();
-    p.is_token_in_rank = reinterpret_cast<unsigned char*>(r.in_rank.data_ptr<bool>());
-    p.probs = r.probs.data_ptr<float>();
-    p.lse = r.lse.data_ptr<float>();
-    const CUtensorMap mw = make_tmap(w.data_ptr(), H, E, 1, H, E * H, 64, 128);
-    const CUtensorMap mx = make_tmap(x.data_ptr(), H, T, 1, H, T * H, 64, router_tile(p, ctx.sms).tile_tokens);
-    SEP_CUDA_CHECK(launch_router_mma(p, &mw, &mx, ctx.sms, ctx.status, ctx.wait_budget_ns, ctx.stream));
-  }
+  const LaunchContext ctx = call.context(T > 0 ? 2 : 1);
+  RouterParams p{};
+  p.x = x.data_ptr(); p.w_gate = w.data_ptr();
+  p.num_tokens = static_cast<int>(T); p.hidden = static_cast<int>(H); p.num_experts = static_cast<int>(E); p.num_topk = call.top_k;
+  p.num_ranks = call.num_ranks; p.renormalize = call.renormalize ? 1 : 0;
+  p.topk_idx = reinterpret_cast<long long*>(r.idx.data_ptr<int64_t>());
+  p.topk_weights = r.weights.data_ptr<float>();
+  p.is_token_in_rank = reinterpret_cast<unsigned char*>(r.in_rank.data_ptr<bool>());
+  p.probs = r.probs.data_ptr<float>();
+  p.lse = r.lse.data_ptr<float>();
   RouteStatsParams s{};
-  s.tokens = static_cast<int>(T); s.experts = static_cast<int>(E); s.top_k = call.top_k;
-  s.probs = r.probs.data_ptr<float>(); s.lse = r.lse.data_ptr<float>();
-  s.idx = reinterpret_cast<const long long*>(r.idx.data_ptr<int64_t>());
+  s.experts = static_cast<int>(E); s.top_k = call.top_k;
   s.mask = mask_of(mask);
-  s.blocks = route_stats_blocks(s.tokens, ctx.sms);
-  const at::Tensor parts = at::empty({s.blocks * (2 * E + 2) + 1}, f32);
+  s.blocks = route_blocks(p, ctx.sms);
+  const at::Tensor parts = at::empty({s.blocks * (2 * E + 2) + 2}, f32);
   s.other_parts = reinterpret_cast<float2*>(parts.data_ptr<float>());
-  s.prob_parts = parts.data_ptr<float>() + 2 * s.blocks;
-  s.count_parts = reinterpret_cast<int*>(s.prob_parts + s.blocks * E);
+  s.parts = s.other_parts + s.blocks;
   s.balance = r.balance.data_ptr<float>(); s.z = r.z.data_ptr<float>();
   s.counts = reinterpret_cast<long long*>(r.counts.data_ptr<int64_t>());
   s.load = r.load.data_ptr<float>();
-  SEP_CUDA_CHECK(launch_route_stats(s, ctx.stream));
+  CUtensorMap mw{}, mx{};
+  if (T > 0) {
+    mw = make_tmap(w.data_ptr(), H, E, 1, H, E * H, 64, 128);
+    mx = make_tmap(x.data_ptr(), H, T, 1, H, T * H, 64, router_tile(p, ctx.sms).tile_tokens);
+  }
+  SEP_CUDA_CHECK(launch_route_forward(p, s, &mw, &mx, ctx.sms, ctx.status, ctx.wait_budget_ns, ctx.stream));
   return r;
 }
 

@@ -3,27 +3,26 @@
 
 #include <cuda_runtime.h>
 
+#include "api.h"
 #include "status.h"
 
 namespace sep {
 
 struct RouteStatsParams {
-  int tokens, experts, top_k;
-  const float* probs;            // [tokens, experts]
-  const float* lse;              // [tokens]
-  const long long* idx;          // [tokens, top_k]
+  int experts, top_k;
   const unsigned char* mask;     // [tokens] or null: tokens that count
-  int blocks;                    // route_stats_blocks()
-  float* prob_parts;             // [blocks][experts] sums over a block's tokens
-  int* count_parts;              // [blocks][experts]
+  int blocks;                    // route_blocks()
+  float2* parts;                 // [blocks][experts] (sum of probabilities, bits of the count)
   float2* other_parts;           // [blocks] (sum of lse^2, bits of the number of tokens that count)
   float* balance;                // one number each
   float* z;
   long long* counts;             // [experts]
   float* load;                   // [experts + 1]: experts * counts / (top_k * n); behind them 1 / n (0 without any that count)
 };
-int route_stats_blocks(int tokens, int sms);
-cudaError_t launch_route_stats(const RouteStatsParams& p, cudaStream_t stream);
+int route_blocks(const RouterParams& p, int sms);
+// Maps as for the router (api.h); all outputs of `p`, probs and lse too.
+cudaError_t launch_route_forward(const RouterParams& p, const RouteStatsParams& s, const void* map_w, const void* map_x, int sms, StatusBlock* status, unsigned long long wait_budget_ns,
+                                 cudaStream_t stream);
 
 struct RouteGradParams {
   int tokens, experts, top_k, hidden, renormalize;

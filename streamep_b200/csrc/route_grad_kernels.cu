@@ -29,47 +29,63 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The gradient of one token's logits, by one warp: lane l has experts l, l + 32, ...
-template <int EPL>
-__device__ __forceinline__ void token_gradient(const RouteGradParams& p, int t, int lane, float share, float db, float dzl, float (&v)[EPL]) {
-  const float* probs = p.probs + static_cast<long long>(t) * p.experts;
-  float prob[EPL];
+// The gradients of N tokens' logits, by one warp: lane l has experts l, l + 32, ...  All loads first: a warp has 16 tokens to form before the first
+// product, and one after another they took 15 us.
+template <int EPL, int N>
+__device__ __forceinline__ void token_gradients(const RouteGradParams& p, int t0, int step, int lane, float share, float db, float dzl, float (&v)[N][EPL]) {
+  float prob[N][EPL], up[N], w[N], lse[N];
+  int mine[N];
+  bool counts[N];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) prob[j] = j * 32 + lane < p.experts ? probs[j * 32 + lane] : 0.f;
-  int mine = -1;
-  float up = 0.f, w = 0.f;
-  if (lane < p.top_k && p.dweights != nullptr) {
-    const long long at = static_cast<long long>(t) * p.top_k + lane;
-    mine = static_cast<int>(p.idx[at]);
-    w = p.weights[at];
-    up = p.dweights[at];
+  for (int i = 0; i < N; ++i) {
+    const int t = t0 + i * step;
+    const bool there = t < p.tokens;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) prob[i][j] = there && j * 32 + lane < p.experts ? p.probs[static_cast<long long>(t) * p.experts + j * 32 + lane] : 0.f;
+    mine[i] = -1; up[i] = w[i] = 0.f;
+    if (there && lane < p.top_k && p.dweights != nullptr) {
+      const long long at = static_cast<long long>(t) * p.top_k + lane;
+      mine[i] = static_cast<int>(p.idx[at]);
+      w[i] = p.weights[at];
+      up[i] = p.dweights[at];
+    }
+    counts[i] = there && (p.mask == nullptr || p.mask[t] != 0);
+    lse[i] = there && dzl != 0.f ? p.lse[t] : 0.f;
   }
-  const bool counts = p.mask == nullptr || p.mask[t] != 0;
-  const float cb = counts ? db * share : 0.f, cz = counts && dzl != 0.f ? 2.f * dzl * share * p.lse[t] : 0.f;
-  float load[EPL], mean_load = 0.f;
+  float load[EPL], mean_load[N], mean_up[N];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    load[j] = cb != 0.f && j * 32 + lane < p.experts ? p.load[j * 32 + lane] : 0.f;
-    mean_load = fmaf(prob[j], load[j], mean_load);
+  for (int j = 0; j < EPL; ++j) load[j] = db != 0.f && j * 32 + lane < p.experts ? p.load[j * 32 + lane] : 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    mean_load[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) mean_load[i] = fmaf(prob[i][j], load[j], mean_load[i]);
+    // (where the weights are not normalised again, w is the probability itself)
+    mean_up[i] = w[i] * up[i];
   }
-  if (cb != 0.f) mean_load = warp_sum(mean_load);
-  // (where the weights are not normalised again, w is the probability itself)
-  const float mean_up = p.dweights != nullptr ? warp_sum(w * up) : 0.f;
-  const float at_chosen = p.renormalize ? w * (up - mean_up) : w * up;
-  const float all = p.renormalize ? 0.f : mean_up;
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    v[j] = cb != 0.f ? cb * prob[j] * (load[j] - mean_load) : 0.f;
-    if (cz != 0.f) v[j] = fmaf(cz, prob[j], v[j]);
-    v[j] = fmaf(-all, prob[j], v[j]);
+  for (int i = 0; i < N; ++i) {
+    if (db != 0.f) mean_load[i] = warp_sum(mean_load[i]);
+    if (p.dweights != nullptr) mean_up[i] = warp_sum(mean_up[i]);
   }
-  if (p.dweights != nullptr) {
-    for (int k = 0; k < p.top_k; ++k) {
-      const int chosen = __shfl_sync(0xffffffffu, mine, k);
-      const float add = __shfl_sync(0xffffffffu, at_chosen, k);
 #pragma unroll
-      for (int j = 0; j < EPL; ++j)
-        if (chosen == j * 32 + lane) v[j] += add;
+  for (int i = 0; i < N; ++i) {
+    const float cb = counts[i] ? db * share : 0.f, cz = counts[i] ? 2.f * dzl * share * lse[i] : 0.f;
+    const float all = p.renormalize ? 0.f : mean_up[i], at_chosen = p.renormalize ? w[i] * (up[i] - mean_up[i]) : w[i] * up[i];
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      // (a token that does not count is not multiplied with: it may hold anything)
+      v[i][j] = counts[i] ? fmaf(cz, prob[i][j], cb * prob[i][j] * (load[j] - mean_load[i])) : 0.f;
+      if (p.dweights != nullptr) v[i][j] = fmaf(-all, prob[i][j], v[i][j]);
+    }
+    if (p.dweights != nullptr) {
+      for (int k = 0; k < p.top_k; ++k) {
+        const int chosen = __shfl_sync(0xffffffffu, mine[i], k);
+        const float add = __shfl_sync(0xffffffffu, at_chosen, k);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j)
+          if (chosen == j * 32 + lane) v[i][j] += add;
+      }
     }
   }
 }
@@ -171,21 +187,22 @@ __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_cons
   } else {
     const int w = warp - 2, quarter = warp & 3, side = w >> 2;
     const float share = p.load[p.experts], db = p.dbalance != nullptr ? *p.dbalance : 0.f, dzl = p.dz_loss != nullptr ? *p.dz_loss : 0.f;
-    for (int r = w; r < kTokens; r += kEpiWarps) {
-      const int t = tile * kTokens + r;
-      float v[EPL];
-      if (t < p.tokens) token_gradient<EPL>(p, t, lane, share, db, dzl, v);
+    constexpr int kAtOnce = EPL <= 4 ? 8 : EPL <= 8 ? 4 : 2;
+    constexpr int kHalves = EPL == 1 ? 2 : EPL;  // (32 experts: the other half of a block of 64 is zero)
+    for (int r0 = w; r0 < kTokens; r0 += kEpiWarps * kAtOnce) {
+      float v[kAtOnce][EPL];
+      token_gradients<EPL, kAtOnce>(p, tile * kTokens + r0, kEpiWarps, lane, share, db, dzl, v);
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) {
-        const int e = j * 32 + lane;
-        if (e >= g.padded) continue;
-        const __nv_bfloat16 b = __float2bfloat16_rn(t < p.tokens && e < p.experts ? v[j] : 0.f);
-        *reinterpret_cast<__nv_bfloat16*>(dz + e / 64 * kTokens * 128 + stage_off<128>(r, e % 64 / 8) + e % 8 * 2) = b;
-        if (split == 0 && t < p.tokens && p.dz != nullptr) static_cast<__nv_bfloat16*>(p.dz)[static_cast<long long>(t) * g.padded + e] = b;
-      }
-      if (EPL == 1 && g.padded > 32) {           // (the second half of a block of 64)
-        *reinterpret_cast<__nv_bfloat16*>(dz + stage_off<128>(r, (32 + lane) / 8) + lane % 8 * 2) = __float2bfloat16_rn(0.f);
-        if (split == 0 && t < p.tokens && p.dz != nullptr) static_cast<__nv_bfloat16*>(p.dz)[static_cast<long long>(t) * g.padded + 32 + lane] = __float2bfloat16_rn(0.f);
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int r = r0 + i * kEpiWarps, t = tile * kTokens + r;
+#pragma unroll
+        for (int j = 0; j < kHalves; ++j) {
+          const int e = j * 32 + lane;
+          if (e >= g.padded) continue;
+          const __nv_bfloat16 b = __float2bfloat16_rn(j < EPL && t < p.tokens && e < p.experts ? v[i][j < EPL ? j : 0] : 0.f);
+          *reinterpret_cast<__nv_bfloat16*>(dz + e / 64 * kTokens * 128 + stage_off<128>(r, e % 64 / 8) + e % 8 * 2) = b;
+          if (split == 0 && t < p.tokens && p.dz != nullptr) static_cast<__nv_bfloat16*>(p.dz)[static_cast<long long>(t) * g.padded + e] = b;
+        }
       }
     }
     fence_proxy_async_smem();

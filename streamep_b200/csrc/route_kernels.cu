@@ -1,88 +1,383 @@
-// Routing that is trained: from the router's probabilities p = softmax(z), z = x W^T, and its choice of top_k experts a token
+// Routing that is trained: the router's product and choice with what its losses need.
 //
+//   z = x W^T,  p = softmax(z),  the top_k experts of each token and their weights
 //   counts_e = tokens (that count: n) that chose e,   load_e = E counts_e / (top_k n)
 //   balance = sum_e load_e mean_t p_te,   z_loss = mean_t logsumexp(z_t)^2
 //
-// and the gradients of both and of the weights w:
+// One kernel multiplies, chooses, leaves p and the logsumexp for the backward and adds up its tokens' probabilities, counts and squares; a small one adds
+// up the blocks' sums, in one order (a repeated call gives the same bits).
 //
-//   dz_t = [counts] (db p_t (load - <p_t, load>) + 2 dz_loss lse_t p_t) / n
-//          + w (dw - <w, dw>) at the chosen experts where w is the softmax over them, or p (dp - <p, dp>) with dp = dw there
-//   dx = dz W,   dW = dz^T x
-#include "route.h"
+// What bounds it: reading x once (HBM), for many experts the tensor cores too, and the finishing of tokens one by one in each warp.
+#include <atomic>
+#include <cuda.h>
 
+#include "api.h"
 #include "ptx.cuh"
+#include "route.h"
 
 namespace sep {
 
 namespace {
 
-constexpr int kStatThreads = 512;                // one expert a thread
-constexpr int kMaxExperts = 512;
+constexpr int kThreads = 512;
+constexpr int kBK = 64;
+// The tensor cores cut off what an accumulator cannot hold instead of rounding, so it starts anew every 512 elements of the reduction and the
+// segments are added up in registers: with one accumulator over 7168 elements the z loss came out 6e-6 too small, with segments XXX.
+constexpr int kSegment = 8;                      // k-blocks
+constexpr int kDrainFirst = 4, kDrainers = 12;   // warps that take the segments' sums: three for each quarter of the accumulator's lanes
+constexpr int kMostChunks = 6;                   // of 16 columns, of up to 256, for one of the three
+constexpr int kMaxStages = 8, kMaxSplits = 8, kMostExperts = 512;
+__host__ __device__ constexpr int e_pad_of(int experts) { return (experts + 127) / 128 * 128 + 1; }
 
-__global__ void __launch_bounds__(kStatThreads) route_stats_kernel(const RouteStatsParams p) {
-  __shared__ int hist[kMaxExperts];
-  const int e = threadIdx.x;
-  hist[e] = 0;
-  __syncthreads();
-  const int begin = static_cast<int>(static_cast<long long>(p.tokens) * blockIdx.x / p.blocks), end = static_cast<int>(static_cast<long long>(p.tokens) * (blockIdx.x + 1) / p.blocks);
-  float sum = 0.f, squares = 0.f;
-  int live = 0;
-  for (int t = begin; t < end; ++t) {
-    if (p.mask != nullptr && p.mask[t] == 0) continue;
-    if (e < p.experts) sum += p.probs[static_cast<long long>(t) * p.experts + e];
-    if (e < p.top_k) atomicAdd(&hist[p.idx[static_cast<long long>(t) * p.top_k + e]], 1);
-    const float lse = p.lse[t];
-    squares = fmaf(lse, lse, squares);
-    ++live;
-  }
-  __syncthreads();
-  if (e < p.experts) {
-    p.prob_parts[blockIdx.x * p.experts + e] = sum;
-    p.count_parts[blockIdx.x * p.experts + e] = hist[e];
-  }
-  if (e == 0) p.other_parts[blockIdx.x] = make_float2(squares, __int_as_float(live));
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-__global__ void __launch_bounds__(kStatThreads) route_join_kernel(const RouteStatsParams p) {
-  __shared__ float scratch[kStatThreads / 32];
+// What a warp adds up over its tokens.
+template <int EPL> struct Sums { float probs[EPL], squares; int live; };
+
+// One warp finishes one token from its fp32 logits: softmax, the top_k by repeated arg-max (ties: lowest expert), weights, ranks, sums.
+template <int EPL, class Row>
+__device__ __forceinline__ void finish_token(const RouterParams& p, const RouteStatsParams& s, Row row, int t, int lane, int* hist, Sums<EPL>& sums) {
+  const int E = p.num_experts, K = p.num_topk;
+  float v[EPL], top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const int e = j * 32 + lane;
+    v[j] = e < E ? row(e) : -INFINITY;
+    top = fmaxf(top, v[j]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    v[j] = j * 32 + lane < E ? expf(v[j] - top) : 0.f;
+    sum += v[j];
+  }
+  sum = warp_sum(sum);
+  const float inv = 1.f / sum, lse = top + logf(sum);
+  const bool counts = s.mask == nullptr || s.mask[t] != 0;
+  unsigned key[EPL];             // probability bits + 1, which order like the values (0: taken, or no such expert)
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const int e = j * 32 + lane;
+    const float prob = v[j] * inv;
+    if (e < E) p.probs[static_cast<size_t>(t) * E + e] = prob;
+    if (counts) sums.probs[j] += prob;
+    key[j] = e < E ? __float_as_uint(prob) + 1u : 0u;
+  }
+  if (counts) { sums.squares = fmaf(lse, lse, sums.squares); ++sums.live; }
+  if (lane == 0) p.lse[t] = lse;
+  float wsum = 0.f, my_w = 0.f;
+  int my_e = -1;
+  unsigned rank_mask = 0;
+  const int e_local = E / p.num_ranks;
+  for (int k = 0; k < K; ++k) {
+    unsigned best = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) best = max(best, key[j]);
+    const unsigned most = __reduce_max_sync(0xffffffffu, best);
+    unsigned mine = 0x7fffffffu;
+#pragma unroll
+    for (int j = EPL - 1; j >= 0; --j)
+      if (key[j] == most) mine = j * 32 + lane;
+    const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, mine));
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (j * 32 + lane == e) key[j] = 0;
+    const float w = __uint_as_float(most - 1u);
+    if (lane == k) { my_w = w; my_e = e; }
+    wsum += w;
+    rank_mask |= 1u << (e / e_local);
+  }
+  if (lane < K) {
+    p.topk_idx[static_cast<size_t>(t) * K + lane] = my_e;
+    p.topk_weights[static_cast<size_t>(t) * K + lane] = p.renormalize ? my_w / wsum : my_w;
+    if (counts) atomicAdd(&hist[my_e], 1);       // (whole numbers: the order does not matter)
+  }
+  if (lane < p.num_ranks) p.is_token_in_rank[static_cast<size_t>(t) * p.num_ranks + lane] = (rank_mask >> lane) & 1u;
+}
+
+// A unit of `g.tile_tokens` tokens belongs to a cluster of `splits` blocks; each multiplies its share of the hidden dimension, W (experts, 128 per
+// accumulator) times the tokens (16 to 128 columns), and leaves its partial logits in shared memory; then every block of the cluster finishes its
+// share of the tokens, adding the partial sums over distributed shared memory.
+template <int EPL>
+__global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const RouterParams p,
+                                                                    const RouteStatsParams s, const RouterTile g, StatusBlock* status, unsigned long long budget) {
+  extern __shared__ unsigned char smem_dyn[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tmem_full[2], tmem_empty[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ int hist[kMostExperts];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = static_cast<int>(blockIdx.x) % g.splits, tile = static_cast<int>(blockIdx.x) / g.splits;
+  const int n = g.tile_tokens, nb = g.blocks, set = nb * n;
+  const int k_blocks = (p.hidden + kBK - 1) / kBK;
+  const int kb0 = k_blocks * split / g.splits, kb1 = k_blocks * (split + 1) / g.splits;
+  const int segments = (kb1 - kb0 + kSegment - 1) / kSegment;
+  const int stage_bytes = nb * 128 * 128 + n * 128;
+  int tmem_cols = 32;
+  while (tmem_cols < 2 * set) tmem_cols *= 2;
+  grid_release();
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&map_x);
+    for (int i = 0; i < g.stages; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&tmem_full[i], 1); mbar_init(&tmem_empty[i], kDrainers); }
+    mbar_fence_init();
+  }
+  if (warp == 1) { tmem_alloc<1>(&s_tmem, tmem_cols); tmem_relinquish<1>(); }
+  hist[threadIdx.x] = 0;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  bool ok = true;
+  float acc[kMostChunks][16];
+#pragma unroll
+  for (int i = 0; i < kMostChunks; ++i)
+#pragma unroll
+    for (int c = 0; c < 16; ++c) acc[i][c] = 0.f;
+  const int quarter = warp & 3, third = (warp - kDrainFirst) >> 2, chunks = set / 16;
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0; uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1, budget, status)) { ok = false; break; }
+        unsigned char* at = smem + stage * stage_bytes;
+        mbar_arrive_expect_tx(&full_bar[stage], stage_bytes);
+        for (int b = 0; b < nb; ++b) tma_load_3d(at + b * 128 * 128, &map_w, &full_bar[stage], kb * kBK, b * 128, 0);
+        tma_load_3d(at + nb * 128 * 128, &map_x, &full_bar[stage], kb * kBK, tile * n, 0);
+        if (++stage == g.stages) { stage = 0; phase ^= 1; }
+      }
+      if (!ok) {
+        report_failure(status, kStatusTimeoutPipeline, kKernelRoute, 6, 0, tile, split, 0);
+        const unsigned long long t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 2000000ull) {}          // copies in flight land before the block leaves (bounded)
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = umma_idesc_bf16(128, 0, 0, 0) | (static_cast<uint32_t>(n >> 3) << 17);
+    int stage = 0; uint32_t phase = 0;
+    for (int q = 0; q < segments && ok; ++q) {
+      const int first = kb0 + q * kSegment, last = min(first + kSegment, kb1);
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[q & 1], ((q >> 1) & 1) ^ 1, budget, status))) { ok = false; break; }
+      tc_fence_after_sync();
+      for (int kb = first; kb < last; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, budget, status))) { ok = false; break; }
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + nb * 128 * 128;
+          for (int m = 0; m < nb; ++m)
+#pragma unroll
+            for (int j = 0; j < kBK / 16; ++j)
+              umma_bf16_ss<1>(tmem + (q & 1) * set + m * n, umma_smem_desc(a + m * 128 * 128 + j * 32, 16, 1024), umma_smem_desc(b + j * 32, 16, 1024), idesc,
+                              (kb > first || j > 0) ? 1u : 0u);
+          umma_commit<1>(&empty_bar[stage]);
+          if (kb == last - 1) umma_commit<1>(&tmem_full[q & 1]);
+        }
+        __syncwarp();
+        if (++stage == g.stages) { stage = 0; phase ^= 1; }
+      }
+    }
+    if (!ok && lane == 0) report_failure(status, kStatusTimeoutPipeline, kKernelRoute, 7, 0, tile, split, 0);
+  } else if (warp >= kDrainFirst) {
+    // accumulator lane = expert within its block of 128, column = token
+    for (int q = 0; q < segments; ++q) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[q & 1], (q >> 1) & 1, budget, status))) { ok = false; break; }
+      tc_fence_after_sync();
+#pragma unroll
+      for (int i = 0; i < kMostChunks; ++i) {
+        const int c = third + i * 3;
+        if (c >= chunks) break;
+        uint32_t r[16];
+        tmem_ld_32x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (q & 1) * set + c * 16, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) acc[i][k] += __uint_as_float(r[k]);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tmem_empty[q & 1]);
+    }
+    if (!ok && lane == 0) report_failure(status, kStatusTimeoutPipeline, kKernelRoute, 8, 0, tile, split, 0);
+  }
+  __syncwarp();
+  const int e_pad = e_pad_of(p.num_experts);
+  float* logits = reinterpret_cast<float*>(smem);              // the operand ring is free once the products are done
+  ok = __syncthreads_and(ok ? 1 : 0) != 0;
+  if (ok && warp >= kDrainFirst) {
+#pragma unroll
+    for (int i = 0; i < kMostChunks; ++i) {
+      const int c = third + i * 3;
+      if (c >= chunks) break;
+      const int block = c * 16 / n, token = c * 16 - block * n;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) logits[(token + k) * e_pad + block * 128 + quarter * 32 + lane] = acc[i][k];
+    }
+  }
+  __syncthreads();
+  if (g.splits > 1) cluster_sync();
+  Sums<EPL> sums;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) sums.probs[j] = 0.f;
+  sums.squares = 0.f; sums.live = 0;
+  if (ok) {
+    for (int tt = split + warp * g.splits; tt < n; tt += g.splits * (kThreads / 32)) {
+      const int t = tile * n + tt;
+      if (t >= p.num_tokens) break;
+      if (g.splits == 1) {
+        finish_token<EPL>(p, s, [&](int e) { return logits[tt * e_pad + e]; }, t, lane, hist, sums);
+      } else {
+        finish_token<EPL>(p, s, [&](int e) {
+          float v[kMaxSplits];
+#pragma unroll
+          for (int q = 0; q < kMaxSplits; ++q) v[q] = q < g.splits ? ld_cluster_f32(cluster_map(&logits[tt * e_pad + e], q)) : 0.f;
+          float sum = 0.f;
+#pragma unroll
+          for (int q = 0; q < kMaxSplits; ++q) sum += v[q];
+          return sum;
+        }, t, lane, hist, sums);
+      }
+    }
+  }
+  if (g.splits > 1) cluster_sync();              // the peers have read this block's logits
+  __syncthreads();
+  // the warps' sums, in place of the logits
+  float* all = logits;                           // [16 warps][experts]
+  __shared__ float2 others[kThreads / 32];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j)
+    if (j * 32 + lane < p.num_experts) all[warp * p.num_experts + j * 32 + lane] = sums.probs[j];
+  if (lane == 0) others[warp] = make_float2(sums.squares, __int_as_float(sums.live));
+  __syncthreads();
   const int e = threadIdx.x;
-  float squares = 0.f;
-  int n = 0;
-  for (int b = 0; b < p.blocks; ++b) { const float2 o = p.other_parts[b]; squares += o.x; n += __float_as_int(o.y); }
+  if (e < p.num_experts) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) sum += all[w * p.num_experts + e];
+    s.parts[static_cast<size_t>(blockIdx.x) * p.num_experts + e] = make_float2(sum, __int_as_float(hist[e]));
+  }
+  if (e == 0) {
+    float squares = 0.f;
+    int live = 0;
+    for (int w = 0; w < kThreads / 32; ++w) { squares += others[w].x; live += __float_as_int(others[w].y); }
+    s.other_parts[blockIdx.x] = make_float2(squares, __int_as_float(live));
+  }
+  if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<1>(tmem, tmem_cols); }
+}
+
+// One block adds up the blocks' sums: `rows` threads for each expert.
+constexpr int kJoinThreads = 1024;
+__global__ void __launch_bounds__(kJoinThreads) route_join_kernel(const RouteStatsParams p) {
+  __shared__ float sums[kJoinThreads];
+  __shared__ int counts[kJoinThreads];
+  __shared__ float other[32];
+  __shared__ int live[32];
+  const int E = p.experts, rows = kJoinThreads / E, e = threadIdx.x % E, row = threadIdx.x / E, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_wait();
+  float sum = 0.f, squares = 0.f;
+  int count = 0, n = 0;
+  if (row < rows) {
+#pragma unroll 8
+    for (int b = row; b < p.blocks; b += rows) {
+      const float2 v = p.parts[static_cast<size_t>(b) * E + e];
+      sum += v.x; count += __float_as_int(v.y);
+    }
+  }
+  for (int b = threadIdx.x; b < p.blocks; b += kJoinThreads) { const float2 v = p.other_parts[b]; squares += v.x; n += __float_as_int(v.y); }
+  squares = warp_sum(squares);
+  n = __reduce_add_sync(0xffffffffu, n);
+  sums[threadIdx.x] = sum;
+  counts[threadIdx.x] = count;
+  if (lane == 0) { other[warp] = squares; live[warp] = n; }
+  __syncthreads();
+  squares = warp_sum(other[lane]);
+  n = __reduce_add_sync(0xffffffffu, live[lane]);
   const float share = n > 0 ? 1.f / static_cast<float>(n) : 0.f;
   float term = 0.f;
-  if (e < p.experts) {
-    float sum = 0.f;
-    long long count = 0;
-    for (int b = 0; b < p.blocks; ++b) { sum += p.prob_parts[b * p.experts + e]; count += p.count_parts[b * p.experts + e]; }
-    const float load = static_cast<float>(static_cast<double>(count) * p.experts / p.top_k) * share;
-    p.counts[e] = count;
+  if (threadIdx.x < E) {
+    long long total = 0;
+    sum = 0.f;
+    for (int r = 0; r < rows; ++r) { sum += sums[r * E + e]; total += counts[r * E + e]; }
+    const float load = static_cast<float>(static_cast<double>(total) * E / p.top_k) * share;
+    p.counts[e] = total;
     p.load[e] = load;
     term = load * (sum * share);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
-  if ((e & 31) == 0) scratch[e >> 5] = term;
   __syncthreads();
-  if (e != 0) return;
-  float balance = 0.f;
-  for (int w = 0; w < kStatThreads / 32; ++w) balance += scratch[w];
-  *p.balance = balance;
+  term = warp_sum(term);
+  if (lane == 0) other[warp] = term;
+  __syncthreads();
+  if (warp != 0) return;
+  term = warp_sum(other[lane]);
+  if (lane != 0) return;
+  *p.balance = term;
   *p.z = squares * share;
-  p.load[p.experts] = share;
+  p.load[E] = share;
+}
+
+template <int EPL>
+cudaError_t launch_width(const RouterParams& p, const RouteStatsParams& s, const RouterTile& g, const CUtensorMap& map_w, const CUtensorMap& map_x, StatusBlock* status,
+                         unsigned long long budget, cudaStream_t stream) {
+  auto kernel = route_forward_kernel<EPL>;
+  static std::atomic<bool> configured[64];       // the shared-memory limit is an attribute of the function on a device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    if (e != cudaSuccess) return e;
+    configured[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(s.blocks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = g.smem_bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = g.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, p, s, g, status, budget);
 }
 
 }  // namespace
 
-int route_stats_blocks(int tokens, int sms) {
-  const int most = (tokens + 15) / 16;
-  return most < sms ? most : sms;
+int route_blocks(const RouterParams& p, int sms) {
+  if (p.num_tokens == 0) return 0;
+  const RouterTile g = router_tile(p, sms);
+  return (p.num_tokens + g.tile_tokens - 1) / g.tile_tokens * g.splits;
 }
 
-cudaError_t launch_route_stats(const RouteStatsParams& p, cudaStream_t stream) {
-  if (p.blocks > 0) route_stats_kernel<<<p.blocks, kStatThreads, 0, stream>>>(p);
-  route_join_kernel<<<1, kStatThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_route_forward(const RouterParams& p, const RouteStatsParams& s, const void* map_w, const void* map_x, int sms, StatusBlock* status, unsigned long long wait_budget_ns,
+                                 cudaStream_t stream) {
+  cudaError_t e = cudaSuccess;
+  if (s.blocks > 0) {
+    const RouterTile g = router_tile(p, sms);
+    const CUtensorMap &mw = *static_cast<const CUtensorMap*>(map_w), &mx = *static_cast<const CUtensorMap*>(map_x);
+    if (p.num_experts <= 32) e = launch_width<1>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    else if (p.num_experts <= 64) e = launch_width<2>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    else if (p.num_experts <= 128) e = launch_width<4>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    else if (p.num_experts <= 256) e = launch_width<8>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    else e = launch_width<16>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = s.blocks > 0 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, route_join_kernel, s);
 }
 
 }  // namespace sep

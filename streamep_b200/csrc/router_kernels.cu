@@ -40,7 +40,6 @@ __device__ __forceinline__ void route_token(const RouterParams& p, Row row, int 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const float inv = 1.f / sum;
-  if (p.lse != nullptr && lane == 0) p.lse[t] = mx + logf(sum);
   unsigned key[EPL];            // probability bits + 1 (0: taken, or no such expert)
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {

@@ -163,7 +163,8 @@ def test_masks(native):
     full, plain = balanced_router(x, w, 4, mask=torch.ones(700, dtype=torch.bool, device=DEV)), balanced_router(x, w, 4)
     assert all(torch.equal(a, b) for a, b in zip(full, plain))
     idx, weights, in_rank = router_topk(x, w, 4)
-    assert torch.equal(idx, plain.topk_idx) and torch.equal(weights, plain.topk_weights) and torch.equal(in_rank, plain.is_token_in_rank)
+    assert torch.equal(idx, plain.topk_idx) and torch.equal(in_rank, plain.is_token_in_rank)
+    torch.testing.assert_close(weights, plain.topk_weights, rtol=1e-5, atol=0.0)           # (its exponentials are coarser: 2^-20 here)
     # padding holds anything at all
     mask = torch.ones(700, dtype=torch.bool, device=DEV)
     mask[600:] = False
