@@ -15,6 +15,7 @@ from torch import nn
 
 from ..buffer import Buffer
 from ..ops.grouped_gemm import router_topk
+from ..ops.routing import BalancedRoute, balanced_router
 from ..stream_moe import StreamHolder, TileConfig, make_streams, stream_moe_func
 
 
@@ -48,11 +49,17 @@ def make_buffer(group, num_tokens: int, hidden: int, num_topk: int, num_experts:
 
 
 class StreamMoE(nn.Module):
+    """Router and experts.  ``train_router``: the gate's weight is trained (it is a plain parameter then, replicated over the ranks); a forward
+    with gradients leaves its :class:`BalancedRoute` in ``last_route``, whose ``balance_loss`` and ``z_loss`` the program adds to
+    its loss and whose ``expert_counts`` it may watch.  Without gradients the tokens are routed by :func:`router_topk`."""
+
     def __init__(self, hidden: int, ffn: int, num_experts: int, top_k: int, buffer: Buffer, *,
                  streams: Optional[StreamHolder] = None, tile_config: Optional[TileConfig] = None,
                  activation_checkpoint_level: int = 0, fused: Optional[bool] = None, renormalize: bool = True,
-                 device=None, seed: int = 0, init_std: float = 0.02):
+                 device=None, seed: int = 0, init_std: float = 0.02, train_router: bool = False):
         super().__init__()
+        self.train_router = train_router
+        self.last_route: Optional[BalancedRoute] = None
         self.hidden, self.ffn, self.num_experts, self.top_k = hidden, ffn, num_experts, top_k
         self.buffer = buffer
         self.ep_size, self.ep_rank = buffer.group_size, buffer.rank
@@ -69,7 +76,7 @@ class StreamMoE(nn.Module):
         g_local = torch.Generator(device="cpu").manual_seed(seed * 1000003 + self.ep_rank + 1)
         w1 = torch.randn(self.num_local_experts, 2 * ffn, hidden, generator=g_local) * init_std
         w2 = torch.randn(self.num_local_experts, hidden, ffn, generator=g_local) * init_std
-        self.w_gate = nn.Parameter(w_gate.to(torch.bfloat16).to(device), requires_grad=False)
+        self.w_gate = nn.Parameter(w_gate.to(torch.bfloat16).to(device), requires_grad=train_router)
         self.w1 = nn.Parameter(w1.to(torch.bfloat16).to(device))
         self.w2 = nn.Parameter(w2.to(torch.bfloat16).to(device))
 
@@ -79,8 +86,13 @@ class StreamMoE(nn.Module):
             self._streams = make_streams(self.w1.device)
         return self._streams
 
-    def route(self, x: torch.Tensor):
-        """``(topk_idx, topk_weights, is_token_in_rank)`` from the fused router kernel."""
+    def route(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None):
+        """``(topk_idx, topk_weights, is_token_in_rank)`` from the fused router kernel.  ``mask``: tokens that count in the losses of a trained
+        router."""
+        if self.train_router and torch.is_grad_enabled():
+            self.last_route = balanced_router(x, self.w_gate, self.top_k, num_ranks=self.ep_size, renormalize=self.renormalize, mask=mask,
+                                              buffer=self.buffer)
+            return self.last_route[:3]
         return router_topk(x.detach(), self.w_gate, self.top_k, num_ranks=self.ep_size,
                            renormalize=self.renormalize, buffer=self.buffer)
 
@@ -89,6 +101,6 @@ class StreamMoE(nn.Module):
                                streams=self.streams, num_experts=self.num_experts, tile_config=self.tile_config,
                                activation_checkpoint_level=self.level, fused=self.fused)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        idx, w, in_rank = self.route(x)
+    def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        idx, w, in_rank = self.route(x, mask)
         return self.experts(x, idx, w, in_rank)

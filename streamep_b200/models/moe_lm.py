@@ -2,7 +2,9 @@
 
 The reference ends at the layer; what its users write around it (an embedding, the loss over the vocabulary, clipping, the
 optimizer) is here in its smallest form, on the library's own operators: ``linear_cross_entropy`` for the output
-projection and the loss, ``grad_norm`` over replicated and expert weights, ``adamw_step_`` with the clipping in it.
+projection and the loss, ``grad_norm`` over replicated and expert weights, ``adamw_step_`` with the clipping in it; and with ``mixer``
+and ``train_router`` a block around the experts: ``layer_norm`` with the residual stream, ``gated_scan`` along the sequences,
+``balanced_router``.
 """
 from __future__ import annotations
 
@@ -14,40 +16,106 @@ from torch import nn
 
 from ..buffer import Buffer
 from ..ops.linear_loss import linear_cross_entropy
+from ..ops.norm import layer_norm
+from ..ops.recurrence import gated_scan, gated_scan_step_
 from ..ops.tensor_lists import adamw_step_, grad_norm
 from .moe_layer import StreamMoE
 
 
+class Mixer(nn.Module):
+    """Mixes the tokens of a sequence: a projection to values and gates, :func:`gated_scan`, a projection back; with the norms in front of it and
+    behind it (in front of the experts)."""
+
+    def __init__(self, hidden: int, generator: torch.Generator, device=None):
+        super().__init__()
+        weight = lambda *shape: nn.Parameter((torch.randn(*shape, generator=generator) / math.sqrt(hidden)).to(torch.bfloat16).to(device))
+        plain = lambda value: nn.Parameter(torch.full((hidden,), value, dtype=torch.bfloat16, device=device))
+        self.w_in, self.w_out = weight(2 * hidden, hidden), weight(hidden, hidden)
+        # channels that forget soon beside channels that remember for hundreds of tokens
+        self.gate_bias = nn.Parameter(torch.linspace(0.0, 6.0, hidden).to(torch.bfloat16).to(device))
+        self.norm_weight, self.norm_bias = plain(1.0), plain(0.0)
+        self.expert_norm_weight, self.expert_norm_bias = plain(1.0), plain(0.0)
+
+    def values_and_gates(self, x: torch.Tensor):
+        values, gates = torch.nn.functional.linear(x, self.w_in).chunk(2, dim=-1)
+        return values, gates + self.gate_bias
+
+
 class MoELM(nn.Module):
-    """Embedding, ``num_layers`` residual MoE layers on RMS-normalised rows, output projection.  There is no token mixer:
-    it models the next token from the present one, which is what a training step needs to be exercised."""
+    """Embedding, ``num_layers`` residual MoE layers on normalised rows, output projection.
+
+    Without ``mixer`` there is no token mixer: it models the next token from the present one, which is what a training step needs to be
+    exercised.  With it each layer is a :class:`Mixer` and the experts, ``tokens`` are ``[B, T]``, or packed sequences ``[N]`` with
+    ``offsets`` (see :func:`gated_scan`), and :meth:`step` goes on token by token.
+
+    ``train_router``: the gates are trained; ``forward`` adds their balance and z losses, times ``balance_coef`` and ``z_coef``, to a mean
+    loss that is differentiated."""
 
     def __init__(self, vocab: int, hidden: int, ffn: int, num_experts: int, top_k: int, num_layers: int, buffer: Buffer, *,
-                 device=None, seed: int = 0):
+                 device=None, seed: int = 0, mixer: bool = False, train_router: bool = False, balance_coef: float = 0.01, z_coef: float = 0.001):
         super().__init__()
         g = torch.Generator(device="cpu").manual_seed(seed)
         self.embedding = nn.Parameter(torch.randn(vocab, hidden, generator=g).to(torch.bfloat16).to(device))
         self.head = nn.Parameter((torch.randn(vocab, hidden, generator=g) * 0.02).to(torch.bfloat16).to(device))
-        self.layers = nn.ModuleList(StreamMoE(hidden, ffn, num_experts, top_k, buffer, device=device, seed=seed + i)
+        self.layers = nn.ModuleList(StreamMoE(hidden, ffn, num_experts, top_k, buffer, device=device, seed=seed + i, train_router=train_router)
                                     for i in range(num_layers))
+        self.mixers = nn.ModuleList(Mixer(hidden, g, device) for _ in range(num_layers if mixer else 0))
+        self.hidden, self.train_router, self.balance_coef, self.z_coef = hidden, train_router, balance_coef, z_coef
         self.buffer = buffer
 
-    def hidden_states(self, tokens: torch.Tensor) -> torch.Tensor:
+    def hidden_states(self, tokens: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
         x = torch.nn.functional.embedding(tokens.reshape(-1), self.embedding)
-        for layer in self.layers:
-            x = x + layer(torch.nn.functional.rms_norm(x, x.shape[-1:]))
-        return torch.nn.functional.rms_norm(x, x.shape[-1:])
+        if not self.mixers:
+            for layer in self.layers:
+                x = x + layer(torch.nn.functional.rms_norm(x, x.shape[-1:]))
+            return torch.nn.functional.rms_norm(x, x.shape[-1:])
+        shape = x.shape if offsets is not None else (*tokens.shape, self.hidden)
+        mix = lambda i, values, gates: gated_scan(values.view(shape), gates.view(shape), offsets=offsets, buffer=self.buffer).view(x.shape)
+        return self._blocks(x, mix)
 
-    def forward(self, tokens: torch.Tensor, targets: torch.Tensor, reduction: str = "mean") -> torch.Tensor:
-        return linear_cross_entropy(self.hidden_states(tokens), self.head, targets.reshape(-1), reduction=reduction, buffer=self.buffer)
+    def _blocks(self, x: torch.Tensor, mix) -> torch.Tensor:
+        """The layers with their mixers; ``mix(i, values, gates)`` is what runs along the sequences."""
+        added = None
+        for i, (mixer, layer) in enumerate(zip(self.mixers, self.layers)):
+            if added is None:
+                y = layer_norm(x, mixer.norm_weight, mixer.norm_bias)
+            else:
+                y, x = layer_norm(added, mixer.norm_weight, mixer.norm_bias, residual=x)
+            mixed = torch.nn.functional.linear(mix(i, *mixer.values_and_gates(y)), mixer.w_out)
+            y, x = layer_norm(mixed, mixer.expert_norm_weight, mixer.expert_norm_bias, residual=x)
+            added = layer(y)
+        return layer_norm(added, residual=x)[0]
+
+    def router_losses(self) -> torch.Tensor:
+        """The gates' losses of the last forward, with their coefficients, averaged over the layers."""
+        routes = [layer.last_route for layer in self.layers]
+        return sum(self.balance_coef * r.balance_loss + self.z_coef * r.z_loss for r in routes) / len(routes)
+
+    def forward(self, tokens: torch.Tensor, targets: torch.Tensor, reduction: str = "mean", offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        loss = linear_cross_entropy(self.hidden_states(tokens, offsets), self.head, targets.reshape(-1), reduction=reduction, buffer=self.buffer)
+        if self.train_router and reduction == "mean" and torch.is_grad_enabled():
+            loss = loss + self.router_losses()
+        return loss
 
     @torch.no_grad()
-    def log_probs(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    def log_probs(self, tokens: torch.Tensor, targets: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
         """log P(target) of every token, shaped like ``tokens``."""
-        return -self.forward(tokens, targets, reduction="none").view(tokens.shape)
+        return -self.forward(tokens, targets, reduction="none", offsets=offsets).view(tokens.shape)
+
+    def states(self, sequences: int) -> List[torch.Tensor]:
+        """What :meth:`step` keeps of ``sequences`` sequences, before their first token."""
+        return [torch.zeros(sequences, self.hidden, device=self.head.device) for _ in self.mixers]
+
+    @torch.no_grad()
+    def step(self, tokens: torch.Tensor, states: List[torch.Tensor]) -> torch.Tensor:
+        """One more token ``[S]`` of every sequence: the next token's logits ``[S, V]``; ``states`` go on in place."""
+        x = torch.nn.functional.embedding(tokens, self.embedding)
+        x = self._blocks(x, lambda i, values, gates: gated_scan_step_(states[i], values, gates))
+        return torch.nn.functional.linear(x, self.head)
 
     def replicated_parameters(self) -> List[nn.Parameter]:
-        return [self.embedding, self.head]
+        gates = [layer.w_gate for layer in self.layers] if self.train_router else []
+        return [self.embedding, self.head] + gates + [p for mixer in self.mixers for p in mixer.parameters()]
 
     def expert_parameters(self) -> List[nn.Parameter]:
         return [p for layer in self.layers for p in (layer.w1, layer.w2)]

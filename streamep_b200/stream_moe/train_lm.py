@@ -2,6 +2,7 @@
 vocabulary, backward, norm, clipping and update (``streamep_b200.models.moe_lm``).
 
     python -m streamep_b200.stream_moe.train_lm --steps 50
+    python -m streamep_b200.stream_moe.train_lm --steps 50 --mixer --train-router
     python -m torch.distributed.run --nnodes=1 --nproc-per-node 2 --master-addr 127.0.0.1 \
         --master-port 29552 -m streamep_b200.stream_moe.train_lm
 
@@ -21,7 +22,7 @@ from ._harness_common import init_distributed, rank_zero_print
 
 
 def batch(gen, vocab: int, tokens: int, device):
-    x = torch.randint(0, vocab, (tokens,), generator=gen, device=device)
+    x = torch.randint(0, vocab, (tokens,), generator=gen, device=device)        # (with a mixer: as sequences of 128)
     follow = (x * 31 + 7) % vocab
     noise = torch.rand(tokens, generator=gen, device=device) < 0.125
     return x, torch.where(noise, torch.randint(0, vocab, (tokens,), generator=gen, device=device), follow)
@@ -34,6 +35,9 @@ def train(model, optimizer, steps: int, tokens: int, vocab: int, device, seed: i
     for i in range(steps):
         x, y = batch(gen, vocab, tokens, device)
         optimizer.zero_grad()
+        if model.mixers:
+            length = 128 if tokens % 128 == 0 else tokens
+            x, y = x.view(-1, length), y.view(-1, length)
         loss = model(x, y)
         loss.backward()
         norm = optimizer.step()
@@ -54,12 +58,15 @@ def main():
     ap.add_argument("--vocab", type=int, default=8192)
     ap.add_argument("--steps", type=int, default=50)
     ap.add_argument("--lr", type=float, default=3e-3)
+    ap.add_argument("--mixer", action="store_true", help="a gated recurrence along sequences of 128 tokens in front of each layer's experts")
+    ap.add_argument("--train-router", action="store_true", help="train the gates, with balance and z loss")
     ap.add_argument("--every", type=int, default=10, help="print every so many steps")
     args = ap.parse_args()
     rank, world, local, dev, group = init_distributed()
     experts = args.experts * world
     buf = make_buffer(group, args.tokens, args.hidden, args.topk, experts, layers_in_flight=args.layers, world_size=world)
-    model = MoELM(args.vocab, args.hidden, args.ffn, experts, args.topk, args.layers, buf, device=dev)
+    model = MoELM(args.vocab, args.hidden, args.ffn, experts, args.topk, args.layers, buf, device=dev,
+                  mixer=args.mixer, train_router=args.train_router)
     opt = ExpertAdamW(model.replicated_parameters(), model.expert_parameters(), lr=args.lr, group=group)
     start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
 
