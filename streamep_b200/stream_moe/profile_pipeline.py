@@ -47,6 +47,21 @@ KERNELS = {  # kernel function -> logical name
     "list_norm_kernel": "gradients' norm",
     "list_scale_kernel": "gradients' clipping",
     "list_adamw_kernel": "AdamW",
+    "norm_forward_kernel": "normalisation",
+    "norm_forward_any_kernel": "normalisation",
+    "norm_backward_kernel": "normalisation, gradients",
+    "norm_dx_any_kernel": "normalisation, gradients",
+    "norm_dw_any_kernel": "normalisation, gradients",
+    "norm_join_kernel": "normalisation, gradients",
+    "scan_runs_kernel": "gated recurrence (runs of segments)",
+    "scan_forward_kernel": "gated recurrence",
+    "scan_backward_kernel": "gated recurrence, gradients",
+    "scan_step_kernel": "gated recurrence, one more token",
+    "route_forward_kernel": "trained router",
+    "route_join_kernel": "trained router (joins its sums)",
+    "route_dx_kernel": "trained router, gradients (dx)",
+    "route_dw_kernel": "trained router, gradients (dW)",
+    "route_dw_join_kernel": "trained router, gradients (dW)",
 }
 GEMMS = {  # (A is MN-major, B is MN-major, epilogue, fused push) of grouped_gemm_kernel -> logical name
     (0, 0, 1, 1): "dispatch (+) GEMM-A SwiGLU (fused)",
