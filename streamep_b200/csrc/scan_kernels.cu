@@ -25,7 +25,7 @@ namespace sep {
 
 namespace {
 
-constexpr int kScanThreads = 256;
+constexpr int kScanThreads = 128;               // (256: 8192 rows of 2048 channels forward 40.8 -> 48 us, backward 58.6 -> 61)
 
 // sigmoid(gate) and sigmoid(-gate), each to its own last digits: 1 / (1 + e) and e / (1 + e) of e = exp(gate), which is held at 2^126 (a gate of
 // 87; NaN stays).  For bf16 gates the exponent is rounded once (|gate| 2^-24 of the result), for fp32 ones it is not.
@@ -129,10 +129,11 @@ struct Segment {
 };
 
 // Rows that are on their way while one is worked on: in places of the thread's own in shared memory, filled by asynchronous copies (nobody waits for
-// anybody else's), as many as 48 KB a block hold.  bf16 channels taken one by one, 2 bytes, come through registers.
+// anybody else's).  Five of two arrays, three of four: more rows leave fewer blocks (8 and 5: 40.8 -> 45 us, 58.6 -> 64 for 8192 rows of 2048
+// channels).  bf16 channels taken one by one, 2 bytes, come through registers.
 template <class T, int V> constexpr bool by_copies() { return V * sizeof(T) >= 4; }
 template <class T, int V, int kArrays> constexpr int rows_ahead() {
-  return !by_copies<T, V>() ? 8 : V * sizeof(T) == 16 ? (kArrays == 2 ? 6 : 3) : 8;
+  return !by_copies<T, V>() ? 8 : V * sizeof(T) == 16 ? (kArrays == 2 ? 5 : 3) : 8;
 }
 template <class T, int V, int kArrays> constexpr int ring_bytes() {
   return by_copies<T, V>() ? rows_ahead<T, V, kArrays>() * kArrays * kScanThreads * V * static_cast<int>(sizeof(T)) : 0;
@@ -156,28 +157,29 @@ __device__ __forceinline__ void walk_rows(int first, int last, const T* (&base)[
   };
   if constexpr (by_copies<T, V>()) {
     extern __shared__ __align__(16) unsigned char ring[];
-    auto place = [&](int u, int a) { return ring + ((u * kArrays + a) * kScanThreads + threadIdx.x) * kBytes; };
-    auto fetch = [&](int u, bool there) {
+    // (a loop over single rows: unrolled over the ring, its code no longer fits the SM's nearest instruction cache)
+    constexpr int kRow = kArrays * kScanThreads * kBytes;
+    unsigned char* const mine = ring + threadIdx.x * kBytes;
+    auto fetch = [&](unsigned char* to, bool there) {
       if (there) {
 #pragma unroll
-        for (int a = 0; a < kArrays; ++a) copy_ahead<kBytes>(smem_u32(place(u, a)), next[a]);
+        for (int a = 0; a < kArrays; ++a) copy_ahead<kBytes>(smem_u32(to + a * kScanThreads * kBytes), next[a]);
         advance();
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    for (int u = 0; u < U; ++u) fetch(mine + u * kRow, u < n);
+    int slot = 0;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      unsigned char* const at = mine + slot;
+      slot = slot == (U - 1) * kRow ? 0 : slot + kRow;
+      asm volatile("cp.async.wait_group %0;" :: "n"(U - 1) : "memory");
+      Raw<T, V> row[kArrays];
 #pragma unroll
-    for (int u = 0; u < U; ++u) fetch(u, u < n);
-    for (int i0 = 0; i0 < n; i0 += U) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i0 + u < n) {
-          asm volatile("cp.async.wait_group %0;" :: "n"(U - 1) : "memory");
-          Raw<T, V> row[kArrays];
-#pragma unroll
-          for (int a = 0; a < kArrays; ++a) row[a].load(reinterpret_cast<const T*>(place(u, a)));
-          fetch(u, i0 + u + U < n);
-          f(kBack ? last - 1 - (i0 + u) : first + i0 + u, row);
-        }
+      for (int a = 0; a < kArrays; ++a) row[a].load(reinterpret_cast<const T*>(at + a * kScanThreads * kBytes));
+      fetch(at, i + U < n);
+      f(kBack ? last - 1 - i : first + i, row);
     }
   } else {
     Raw<T, V> now[U][kArrays], ahead[U][kArrays];
@@ -277,7 +279,7 @@ __device__ __forceinline__ void runs_before(Row<V> a, Row<V> b, Run (&before)[V]
 
 // Leaves, of every segment, the run of the segments before it in its block; and of every block the run of all.
 template <class T, int V, bool kBack>
-__global__ void __launch_bounds__(kScanThreads, 3) scan_runs_kernel(const ScanShape p, const ScanSplit s, const void* rows, long long rows_stride, const float* edge) {
+__global__ void __launch_bounds__(kScanThreads, 6) scan_runs_kernel(const ScanShape p, const ScanSplit s, const void* rows, long long rows_stride, const float* edge) {
   using Tl = Tile<V>;
   grid_release();
   const int block = blockIdx.x / s.tiles, tile = blockIdx.x - block * s.tiles;
@@ -389,7 +391,7 @@ __device__ __forceinline__ void empty_sequences(const ScanShape& p, const float*
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(kScanThreads, 3) scan_forward_kernel(const ScanParams p, const ScanSplit s) {
+__global__ void __launch_bounds__(kScanThreads, 6) scan_forward_kernel(const ScanParams p, const ScanSplit s) {
   grid_wait();
   empty_sequences<V>(p, p.initial, p.final_state, true);
   // (from the last block: what was read last is still in L2)
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_forward_kernel(const Sca
 
 // kGate: with the gate's gradient, for which x and h of the row before are read too.
 template <class T, int V, bool kGate>
-__global__ void __launch_bounds__(kScanThreads, 3) scan_backward_kernel(const ScanGradParams p, const ScanSplit s) {
+__global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const ScanGradParams p, const ScanSplit s) {
   grid_wait();
   empty_sequences<V>(p, p.dfinal, p.dinitial, false);
   const int unit = gridDim.x - 1 - blockIdx.x, block = unit / s.tiles, tile = unit - block * s.tiles;
@@ -565,13 +567,14 @@ cudaError_t by_vector(int half, int vec, F f) {
   return f(float{}, std::integral_constant<int, 1>{});
 }
 
-ScanSplit split_of(const ScanShape& p, int vec, int sms) {
+ScanSplit split_of(const ScanShape& p, int vec, int sms, bool back) {
   ScanSplit s{};
   const long long sequences = p.offsets == nullptr ? p.sequences : 1, length = p.offsets == nullptr ? p.length : p.rows;
   const long long vectors = p.channels / vec;
   const int lanes = vec >= 4 ? 8 : 32, segs = kScanThreads / lanes;
-  // Threads that are enough to keep memory busy; and rows of a segment.
-  const long long enough = static_cast<long long>(sms) * (vec >= 4 ? 384 : 1536);
+  // Threads that are enough to keep memory busy, and at least 16 rows a segment.  One sequence of 131072 rows of 1024 channels, with 384 and 1200 vectors of 16
+  // bytes an SM: forward 232 and 260 us, backward 470 and 396.
+  const long long enough = static_cast<long long>(sms) * (vec < 4 ? 1536 : back ? 1200 : 384);
   long long parts = 1;
   while (sequences * vectors * parts < enough && length > 32 * parts) parts *= 2;
   s.rows = static_cast<int>((length + parts - 1) / parts);
@@ -593,6 +596,9 @@ cudaError_t launch(dim3 grid, int smem, bool early, cudaStream_t stream, const A
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (smem > 0 && !configured[dev].load(std::memory_order_acquire)) {
     if ((e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+    // Kernels that follow each other should not want another split of the SM's memory each: changing it cost 16 us a call (4096 rows of 1024
+    // channels forward 38 -> 21.5 us).
+    if ((e = cudaFuncSetAttribute(kKernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)) != cudaSuccess) return e;
     configured[dev].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
@@ -620,8 +626,8 @@ template <class T, int V, int kArrays> constexpr int walk_bytes() {
 
 }  // namespace
 
-ScanSplit scan_split(const ScanParams& p, int sms) { return split_of(p, vector_of(p), sms); }
-ScanSplit scan_split(const ScanGradParams& p, int sms) { return split_of(p, vector_of(p), sms); }
+ScanSplit scan_split(const ScanParams& p, int sms) { return split_of(p, vector_of(p), sms, false); }
+ScanSplit scan_split(const ScanGradParams& p, int sms) { return split_of(p, vector_of(p), sms, true); }
 long long scan_space(const ScanSplit& s, int channels) { return s.within ? 0 : 8ll * (static_cast<long long>(s.segments) + s.blocks) * channels; }
 
 cudaError_t launch_scan_forward(const ScanParams& p, ScanSplit s, void* space, cudaStream_t stream) {
