@@ -72,6 +72,13 @@ template <> struct Raw<__nv_bfloat16, 2> {
 };
 template <> struct Raw<__nv_bfloat16, 4> {
   uint2 v;
+  // `count` numbers, `step` apart; zeros behind them
+  __device__ __forceinline__ void gather(const __nv_bfloat16* p, int step, int count) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = i < count ? *reinterpret_cast<const unsigned short*>(p + i * step) : 0u;
+    v = make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16);
+  }
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint2*>(p); }
   __device__ __forceinline__ Row<4> get() const {
     return Row<4>{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
@@ -79,6 +86,13 @@ template <> struct Raw<__nv_bfloat16, 4> {
 };
 template <> struct Raw<float, 4> {
   float4 v;
+  __device__ __forceinline__ void gather(const float* p, int step, int count) {
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (count > 0) v.x = p[0];
+    if (count > 1) v.y = p[step];
+    if (count > 2) v.z = p[2 * step];
+    if (count > 3) v.w = p[3 * step];
+  }
   __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
   __device__ __forceinline__ Row<4> get() const { return Row<4>{v.x, v.y, v.z, v.w}; }
 };

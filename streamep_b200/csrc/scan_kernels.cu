@@ -48,7 +48,7 @@ __device__ __forceinline__ void gates_of(const Row<V>& gate, Row<V>& keep, Row<V
   const Row<V> power = Row<V>::of(e), sum = power + Row<V>::all(1.f);
   sum.get(e);
 #pragma unroll
-  for (int i = 0; i < V; ++i) e[i] = sizeof(T) == 2 ? reciprocal(e[i]) : __frcp_rn(e[i]);
+  for (int i = 0; i < V; ++i) e[i] = reciprocal(e[i]);
   take = Row<V>::of(e);
   keep = power * take;
 }
@@ -99,24 +99,59 @@ __device__ __forceinline__ bool within_one(const ScanShape& p, int before, int e
 }
 
 // A block's threads: LANES side by side across the channels, V channels each, and SEGS segments above one another.  Where runs are joined, PARTS
-// threads share a channel.
-template <int V> struct Tile {
-  static constexpr int LANES = V >= 4 ? 8 : 32;
+// threads share a channel.  A thread's channels are one vector; or with kApart, where rows do not begin on boundaries of vectors, every 32nd: a warp then
+// reads and writes neighbouring numbers, and still has V of them for each row that it counts off (7488 rows of 1001 fp32 channels with gradients 131 us
+// one by one, XXX so).
+template <int Vec, bool kApart> struct Tile {
+  static constexpr int V = Vec;
+  static constexpr bool kStrided = kApart;
+  static constexpr int LANES = !kApart && V >= 4 ? 8 : 32;
   static constexpr int COLS = LANES * V;
   static constexpr int SEGS = kScanThreads / LANES;
   static constexpr int PARTS = kScanThreads / COLS;
   static_assert(SEGS % PARTS == 0, "parts of equal length");
+  // of channel i of the thread `side`: its place in the tile, and its distance to the thread's first one
+  __device__ __forceinline__ static constexpr int place(int side, int i) { return kApart ? side + i * 32 : side * V + i; }
+  __device__ __forceinline__ static constexpr int apart(int i) { return kApart ? i * 32 : i; }
+  // V numbers from a thread's first one on, of which `count` are there
+  __device__ __forceinline__ static Row<V> load(const float* at, int count) {
+    if constexpr (!kApart) {
+      return load_state<V>(at);
+    } else {
+      Row<V> r;
+#pragma unroll
+      for (int i = 0; i < V; ++i) r.f[i] = i < count ? at[apart(i)] : 0.f;
+      return r;
+    }
+  }
+  __device__ __forceinline__ static void store(float* at, const Row<V>& r, int count) {
+    if constexpr (!kApart) {
+      store_state<V>(at, r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) if (i < count) at[apart(i)] = r.f[i];
+    }
+  }
+  template <class T> __device__ __forceinline__ static void store_rounded(T* at, const Row<V>& r, int count) {
+    if constexpr (!kApart) {
+      store_row<T, V>(at, r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) if (i < count) at[apart(i)] = from_float<T>(r.f[i]);
+    }
+  }
 };
 
 // What a thread works on: V channels from `col` on, and rows [first, last) of a segment.  `order` counts segments from where the recurrence starts:
 // the first one, or with kBack the last one.
-template <int V, bool kBack>
+template <class Tl, bool kBack>
 struct Segment {
-  int order, index, sequence, part, col, first, last;
+  int order, index, sequence, part, col, count, first, last;
   bool there;
   __device__ __forceinline__ Segment(const ScanShape& p, const ScanSplit& s, int block, int tile) {
-    order = block * Tile<V>::SEGS + static_cast<int>(threadIdx.x) / Tile<V>::LANES;
-    col = tile * Tile<V>::COLS + static_cast<int>(threadIdx.x) % Tile<V>::LANES * V;
+    order = block * Tl::SEGS + static_cast<int>(threadIdx.x) / Tl::LANES;
+    col = tile * Tl::COLS + Tl::place(static_cast<int>(threadIdx.x) % Tl::LANES, 0);
+    count = Tl::kStrided ? min(Tl::V, (p.channels - col + 31) / 32) : Tl::V;     // of the V channels, those that there are
     there = order < s.segments && col < p.channels;
     index = kBack ? s.segments - 1 - order : order;
     sequence = index / s.parts;
@@ -131,12 +166,12 @@ struct Segment {
 // Rows that are on their way while one is worked on: in places of the thread's own in shared memory, filled by asynchronous copies (nobody waits for
 // anybody else's).  Five of two arrays, three of four: more rows leave fewer blocks (8 and 5: 40.8 -> 45 us, 58.6 -> 64 for 8192 rows of 2048
 // channels).  bf16 channels taken one by one, 2 bytes, come through registers.
-template <class T, int V> constexpr bool by_copies() { return V * sizeof(T) >= 4; }
-template <class T, int V, int kArrays> constexpr int rows_ahead() {
-  return !by_copies<T, V>() ? 8 : V * sizeof(T) == 16 ? (kArrays == 2 ? 5 : 3) : 8;
+template <class T, class Tl> constexpr bool by_copies() { return Tl::kStrided ? sizeof(T) == 4 : Tl::V * sizeof(T) >= 4; }
+template <class T, class Tl, int kArrays> constexpr int rows_ahead() {
+  return !by_copies<T, Tl>() ? 8 / kArrays : Tl::V * sizeof(T) == 16 ? (kArrays == 2 ? 5 : 3) : 8;
 }
-template <class T, int V, int kArrays> constexpr int ring_bytes() {
-  return by_copies<T, V>() ? rows_ahead<T, V, kArrays>() * kArrays * kScanThreads * V * static_cast<int>(sizeof(T)) : 0;
+template <class T, class Tl, int kArrays> constexpr int ring_bytes() {
+  return by_copies<T, Tl>() ? rows_ahead<T, Tl, kArrays>() * kArrays * kScanThreads * Tl::V * static_cast<int>(sizeof(T)) : 0;
 }
 template <int kBytes> __device__ __forceinline__ void copy_ahead(uint32_t to, const void* from) {
   if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(from) : "memory");
@@ -144,10 +179,10 @@ template <int kBytes> __device__ __forceinline__ void copy_ahead(uint32_t to, co
 }
 
 // Walks the rows of a segment, backwards from its last one with kBack: f(t, row t of the arrays).
-template <class T, int V, bool kBack, int kArrays, class F>
-__device__ __forceinline__ void walk_rows(int first, int last, const T* (&base)[kArrays], const long long (&stride)[kArrays], F f) {
-  constexpr int U = rows_ahead<T, V, kArrays>(), kBytes = V * sizeof(T);
-  const int n = last - first;
+template <class T, class Tl, bool kBack, int kArrays, class F>
+__device__ __forceinline__ void walk_rows(const Segment<Tl, kBack>& seg, int first, const T* (&base)[kArrays], const long long (&stride)[kArrays], F f) {
+  constexpr int V = Tl::V, U = rows_ahead<T, Tl, kArrays>(), kBytes = V * sizeof(T);
+  const int last = seg.last, n = last - first;
   const T* next[kArrays];
 #pragma unroll
   for (int a = 0; a < kArrays; ++a) next[a] = base[a] + (kBack ? last - 1 : first) * stride[a];
@@ -155,7 +190,7 @@ __device__ __forceinline__ void walk_rows(int first, int last, const T* (&base)[
 #pragma unroll
     for (int a = 0; a < kArrays; ++a) next[a] += kBack ? -stride[a] : stride[a];
   };
-  if constexpr (by_copies<T, V>()) {
+  if constexpr (by_copies<T, Tl>()) {
     extern __shared__ __align__(16) unsigned char ring[];
     // (a loop over single rows: unrolled over the ring, its code no longer fits the SM's nearest instruction cache)
     constexpr int kRow = kArrays * kScanThreads * kBytes;
@@ -163,7 +198,15 @@ __device__ __forceinline__ void walk_rows(int first, int last, const T* (&base)[
     auto fetch = [&](unsigned char* to, bool there) {
       if (there) {
 #pragma unroll
-        for (int a = 0; a < kArrays; ++a) copy_ahead<kBytes>(smem_u32(to + a * kScanThreads * kBytes), next[a]);
+        for (int a = 0; a < kArrays; ++a) {
+          const uint32_t place = smem_u32(to + a * kScanThreads * kBytes);
+          if constexpr (Tl::kStrided) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) if (i < seg.count) copy_ahead<4>(place + i * 4, next[a] + Tl::apart(i));
+          } else {
+            copy_ahead<kBytes>(place, next[a]);
+          }
+        }
         advance();
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -188,7 +231,7 @@ __device__ __forceinline__ void walk_rows(int first, int last, const T* (&base)[
       for (int u = 0; u < U; ++u)
         if (i0 + u < n) {
 #pragma unroll
-          for (int a = 0; a < kArrays; ++a) to[u][a].load(next[a]);
+          for (int a = 0; a < kArrays; ++a) to[u][a].gather(next[a], Tl::apart(1), seg.count);
           advance();
         }
     };
@@ -207,13 +250,14 @@ __device__ __forceinline__ void walk_rows(int first, int last, const T* (&base)[
 }
 
 // What the rows of a segment do to the state in front of them.  `rows`: x, or the rows' own gradients (which may be left out).
-template <class T, int V, bool kBack>
-__device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSplit& s, const Segment<V, kBack>& seg, const void* rows, long long rows_stride, const float* edge,
-                                               Row<V>& a, Row<V>& b) {
+template <class T, class Tl, bool kBack>
+__device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSplit& s, const Segment<Tl, kBack>& seg, const void* rows, long long rows_stride, const float* edge,
+                                               Row<Tl::V>& a, Row<Tl::V>& b) {
+  constexpr int V = Tl::V;
   a = Row<V>::all(1.f); b = Row<V>::all(0.f);
   auto begin = [&](int sequence) {
     a = Row<V>::all(-0.f);
-    b = edge != nullptr && sequence >= 0 ? load_state<V>(edge + static_cast<long long>(sequence) * p.channels + seg.col) : Row<V>::all(0.f);
+    b = edge != nullptr && sequence >= 0 ? Tl::load(edge + static_cast<long long>(sequence) * p.channels + seg.col, seg.count) : Row<V>::all(0.f);
   };
   const bool none = kBack && rows == nullptr;
   auto take_row = [&](const Raw<T, V> (&row)[2]) {
@@ -227,11 +271,11 @@ __device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSpl
   const bool dense = p.offsets == nullptr;
   if (dense || within_one(p, kBack ? seg.first : seg.first - 1, kBack ? seg.last + 1 : seg.last)) {
     if (dense && seg.part == (kBack ? s.parts - 1 : 0)) begin(seg.sequence);
-    walk_rows<T, V, kBack, 2>(seg.first, seg.last, base, stride, [&](int, Raw<T, V> (&row)[2]) { take_row(row); });
+    walk_rows<T, Tl, kBack, 2>(seg, seg.first, base, stride, [&](int, Raw<T, V> (&row)[2]) { take_row(row); });
   } else {
     SequenceWalk walk(p, kBack ? seg.last : seg.first - 1);
     int previous = walk.at(p, kBack ? seg.last : seg.first - 1);
-    walk_rows<T, V, kBack, 2>(seg.first, seg.last, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
+    walk_rows<T, Tl, kBack, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
       const int sequence = walk.at(p, t);
       if (sequence != previous || sequence < 0) begin(sequence);
       if (sequence >= 0) take_row(row);
@@ -241,9 +285,9 @@ __device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSpl
 }
 
 // From the runs of a block's segments: of those before each thread's own.  All threads call; the ring is not in use.
-template <int V>
-__device__ __forceinline__ void runs_before(Row<V> a, Row<V> b, Run (&before)[V]) {
-  using Tl = Tile<V>;
+template <class Tl>
+__device__ __forceinline__ void runs_before(Row<Tl::V> a, Row<Tl::V> b, Run (&before)[Tl::V]) {
+  constexpr int V = Tl::V;
   extern __shared__ __align__(16) unsigned char ring[];
   Run* runs = reinterpret_cast<Run*>(ring);                    // [SEGS][COLS]
   __shared__ Run parts[Tl::PARTS][Tl::COLS];
@@ -252,7 +296,7 @@ __device__ __forceinline__ void runs_before(Row<V> a, Row<V> b, Run (&before)[V]
   a.get(fa); b.get(fb);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < V; ++i) runs[seg * Tl::COLS + side * V + i] = Run{fa[i], fb[i]};
+  for (int i = 0; i < V; ++i) runs[seg * Tl::COLS + Tl::place(side, i)] = Run{fa[i], fb[i]};
   __syncthreads();
   const int ch = threadIdx.x % Tl::COLS, part = threadIdx.x / Tl::COLS;
   constexpr int kEach = Tl::SEGS / Tl::PARTS;
@@ -271,30 +315,30 @@ __device__ __forceinline__ void runs_before(Row<V> a, Row<V> b, Run (&before)[V]
     run = nothing();
 #pragma unroll
     for (int q = 0; q < Tl::PARTS; ++q)
-      if (q < seg / kEach) run = join(run, parts[q][side * V + i]);
-    before[i] = join(run, runs[seg * Tl::COLS + side * V + i]);
+      if (q < seg / kEach) run = join(run, parts[q][Tl::place(side, i)]);
+    before[i] = join(run, runs[seg * Tl::COLS + Tl::place(side, i)]);
   }
   __syncthreads();               // the ring may be filled again
 }
 
 // Leaves, of every segment, the run of the segments before it in its block; and of every block the run of all.
-template <class T, int V, bool kBack>
+template <class T, class Tl, bool kBack>
 __global__ void __launch_bounds__(kScanThreads, 6) scan_runs_kernel(const ScanShape p, const ScanSplit s, const void* rows, long long rows_stride, const float* edge) {
-  using Tl = Tile<V>;
+  constexpr int V = Tl::V;
   grid_release();
   const int block = blockIdx.x / s.tiles, tile = blockIdx.x - block * s.tiles;
-  const Segment<V, kBack> seg(p, s, block, tile);
+  const Segment<Tl, kBack> seg(p, s, block, tile);
   Row<V> a = Row<V>::all(1.f), b = Row<V>::all(0.f);
-  if (seg.there) run_of_segment<T, V, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
+  if (seg.there) run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
   Run before[V];
-  runs_before<V>(a, b, before);
+  runs_before<Tl>(a, b, before);
   if (!seg.there) return;
   float fa[V], fb[V];
   const long long at = static_cast<long long>(seg.order) * p.channels + seg.col;
 #pragma unroll
   for (int i = 0; i < V; ++i) { fa[i] = before[i].a; fb[i] = before[i].b; }
-  store_state<V>(s.factors + at, Row<V>::of(fa));
-  store_state<V>(s.sums + at, Row<V>::of(fb));
+  Tl::store(s.factors + at, Row<V>::of(fa), seg.count);
+  Tl::store(s.sums + at, Row<V>::of(fb), seg.count);
   if (seg.order % Tl::SEGS != Tl::SEGS - 1) return;            // (nobody follows a block that is not full)
   float ga[V], gb[V];
   a.get(ga); b.get(gb);
@@ -304,21 +348,21 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_runs_kernel(const ScanSh
     ga[i] = r.a; gb[i] = r.b;
   }
   const long long block_at = static_cast<long long>(block) * p.channels + seg.col;
-  store_state<V>(s.block_factors + block_at, Row<V>::of(ga));
-  store_state<V>(s.block_sums + block_at, Row<V>::of(gb));
+  Tl::store(s.block_factors + block_at, Row<V>::of(ga), seg.count);
+  Tl::store(s.block_sums + block_at, Row<V>::of(gb), seg.count);
 }
 
 // The state in front of each thread's segment.  All threads call.
-template <class T, int V, bool kBack>
-__device__ __forceinline__ Row<V> state_before(const ScanShape& p, const ScanSplit& s, const Segment<V, kBack>& seg, int block, int tile, const void* rows, long long rows_stride,
+template <class T, class Tl, bool kBack>
+__device__ __forceinline__ Row<Tl::V> state_before(const ScanShape& p, const ScanSplit& s, const Segment<Tl, kBack>& seg, int block, int tile, const void* rows, long long rows_stride,
                                                const float* edge) {
-  using Tl = Tile<V>;
+  constexpr int V = Tl::V;
   if (s.parts == 1) return Row<V>::all(0.f);
   if (s.within) {                                // no sequence goes on in another block
     Row<V> a = Row<V>::all(1.f), b = Row<V>::all(0.f);
-    if (seg.there) run_of_segment<T, V, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
+    if (seg.there) run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
     Run before[V];
-    runs_before<V>(a, b, before);
+    runs_before<Tl>(a, b, before);
     float f[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = before[i].b;
@@ -357,22 +401,23 @@ __device__ __forceinline__ Row<V> state_before(const ScanShape& p, const ScanSpl
   const int side = threadIdx.x % Tl::LANES;
   const long long at = static_cast<long long>(seg.order) * p.channels + seg.col;
   float fa[V], fb[V], f[V];
-  load_state<V>(s.factors + at).get(fa);
-  load_state<V>(s.sums + at).get(fb);
+  Tl::load(s.factors + at, seg.count).get(fa);
+  Tl::load(s.sums + at, seg.count).get(fb);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float state = 0.f;
 #pragma unroll
-    for (int q = 0; q < Tl::PARTS; ++q) state = apply(parts[q][side * V + i], state);
+    for (int q = 0; q < Tl::PARTS; ++q) state = apply(parts[q][Tl::place(side, i)], state);
     f[i] = apply(Run{fa[i], fb[i]}, state);
   }
   return Row<V>::of(f);
 }
 
 // Sequences without rows hand their state on (`from` to `to`); offsets that are none are reported.
-template <int V>
+template <class Tl>
 __device__ __forceinline__ void empty_sequences(const ScanShape& p, const float* from, float* to, bool report) {
   if (p.offsets == nullptr && p.length > 0) return;
+  constexpr int V = Tl::kStrided ? 1 : Tl::V;
   const int vectors = p.channels / V;
   const long long all = static_cast<long long>(p.sequences) * vectors;
   for (long long i = static_cast<long long>(blockIdx.x) * kScanThreads + threadIdx.x; i < all; i += static_cast<long long>(gridDim.x) * kScanThreads) {
@@ -390,17 +435,18 @@ __device__ __forceinline__ void empty_sequences(const ScanShape& p, const float*
   }
 }
 
-template <class T, int V>
+template <class T, class Tl>
 __global__ void __launch_bounds__(kScanThreads, 6) scan_forward_kernel(const ScanParams p, const ScanSplit s) {
+  constexpr int V = Tl::V;
   grid_wait();
-  empty_sequences<V>(p, p.initial, p.final_state, true);
+  empty_sequences<Tl>(p, p.initial, p.final_state, true);
   // (from the last block: what was read last is still in L2)
   const int unit = gridDim.x - 1 - blockIdx.x, block = unit / s.tiles, tile = unit - block * s.tiles;
-  const Segment<V, false> seg(p, s, block, tile);
-  Row<V> h = state_before<T, V, false>(p, s, seg, block, tile, p.x, p.x_stride, p.initial);
+  const Segment<Tl, false> seg(p, s, block, tile);
+  Row<V> h = state_before<T, Tl, false>(p, s, seg, block, tile, p.x, p.x_stride, p.initial);
   if (!seg.there) return;
   auto state_at = [&](int sequence) { return static_cast<long long>(sequence) * p.channels + seg.col; };
-  auto begin = [&](int sequence) { h = p.initial != nullptr ? load_state<V>(p.initial + state_at(sequence)) : Row<V>::all(0.f); };
+  auto begin = [&](int sequence) { h = p.initial != nullptr ? Tl::load(p.initial + state_at(sequence), seg.count) : Row<V>::all(0.f); };
   auto step = [&](const Raw<T, V> (&row)[2]) {
     Row<V> keep, take;
     gates_of<T, V>(row[0].get(), keep, take);
@@ -412,24 +458,24 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_forward_kernel(const Sca
   const bool dense = p.offsets == nullptr;
   if (dense || within_one(p, seg.first - 1, seg.last + 1)) {
     if (dense && seg.part == 0) begin(seg.sequence);
-    walk_rows<T, V, false, 2>(seg.first, seg.last, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
+    walk_rows<T, Tl, false, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
       step(row);
-      store_row<T, V>(out + static_cast<long long>(t) * p.channels, h);
+      Tl::template store_rounded<T>(out + static_cast<long long>(t) * p.channels, h, seg.count);
     });
-    if (dense && p.final_state != nullptr && seg.last == (seg.sequence + 1) * p.length && seg.first < seg.last) store_state<V>(p.final_state + state_at(seg.sequence), h);
+    if (dense && p.final_state != nullptr && seg.last == (seg.sequence + 1) * p.length && seg.first < seg.last) Tl::store(p.final_state + state_at(seg.sequence), h, seg.count);
   } else {
     SequenceWalk walk(p, seg.first - 1);
     int previous = walk.at(p, seg.first - 1), sequence = walk.at(p, seg.first);
-    walk_rows<T, V, false, 2>(seg.first, seg.last, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
+    walk_rows<T, Tl, false, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
       const int behind = walk.at(p, t + 1);
       if (sequence >= 0) {
         if (sequence != previous) begin(sequence);
         step(row);
-        if (p.final_state != nullptr && behind != sequence) store_state<V>(p.final_state + state_at(sequence), h);
+        if (p.final_state != nullptr && behind != sequence) Tl::store(p.final_state + state_at(sequence), h, seg.count);
       } else {
         h = Row<V>::all(0.f);
       }
-      store_row<T, V>(out + static_cast<long long>(t) * p.channels, h);
+      Tl::template store_rounded<T>(out + static_cast<long long>(t) * p.channels, h, seg.count);
       previous = sequence;
       sequence = behind;
     });
@@ -437,13 +483,14 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_forward_kernel(const Sca
 }
 
 // kGate: with the gate's gradient, for which x and h of the row before are read too.
-template <class T, int V, bool kGate>
+template <class T, class Tl, bool kGate>
 __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const ScanGradParams p, const ScanSplit s) {
+  constexpr int V = Tl::V;
   grid_wait();
-  empty_sequences<V>(p, p.dfinal, p.dinitial, false);
+  empty_sequences<Tl>(p, p.dfinal, p.dinitial, false);
   const int unit = gridDim.x - 1 - blockIdx.x, block = unit / s.tiles, tile = unit - block * s.tiles;
-  const Segment<V, true> seg(p, s, block, tile);
-  Row<V> back = state_before<T, V, true>(p, s, seg, block, tile, p.dh, p.dh_stride, p.dfinal);     // keep_{t+1} g_{t+1}
+  const Segment<Tl, true> seg(p, s, block, tile);
+  Row<V> back = state_before<T, Tl, true>(p, s, seg, block, tile, p.dh, p.dh_stride, p.dfinal);     // keep_{t+1} g_{t+1}
   if (!seg.there) return;
   auto state_at = [&](int sequence) { return static_cast<long long>(sequence) * p.channels + seg.col; };
   const bool none = p.dh == nullptr;
@@ -453,18 +500,18 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
     gates_of<T, V>(gate, keep, take);
     const Row<V> g = none ? back : back + dh;
     const long long at = static_cast<long long>(t) * p.channels + seg.col;
-    if (p.dx != nullptr) store_row<T, V>(static_cast<T*>(p.dx) + at, take * g);
-    if constexpr (kGate) store_row<T, V>(static_cast<T*>(p.dgate) + at, g * (keep * take) * fused(Row<V>::all(-1.f), x, h));
+    if (p.dx != nullptr) Tl::template store_rounded<T>(static_cast<T*>(p.dx) + at, take * g, seg.count);
+    if constexpr (kGate) Tl::template store_rounded<T>(static_cast<T*>(p.dgate) + at, g * (keep * take) * fused(Row<V>::all(-1.f), x, h), seg.count);
     back = keep * g;
   };
   auto outside = [&](int t) {
     const long long at = static_cast<long long>(t) * p.channels + seg.col;
-    if (p.dx != nullptr) store_row<T, V>(static_cast<T*>(p.dx) + at, Row<V>::all(0.f));
-    if constexpr (kGate) store_row<T, V>(static_cast<T*>(p.dgate) + at, Row<V>::all(0.f));
+    if (p.dx != nullptr) Tl::template store_rounded<T>(static_cast<T*>(p.dx) + at, Row<V>::all(0.f), seg.count);
+    if constexpr (kGate) Tl::template store_rounded<T>(static_cast<T*>(p.dgate) + at, Row<V>::all(0.f), seg.count);
     back = Row<V>::all(0.f);
   };
-  auto begin = [&](int sequence) { back = p.dfinal != nullptr ? load_state<V>(p.dfinal + state_at(sequence)) : Row<V>::all(0.f); };
-  auto initial = [&](int sequence) { return p.initial != nullptr ? load_state<V>(p.initial + state_at(sequence)) : Row<V>::all(0.f); };
+  auto begin = [&](int sequence) { back = p.dfinal != nullptr ? Tl::load(p.dfinal + state_at(sequence), seg.count) : Row<V>::all(0.f); };
+  auto initial = [&](int sequence) { return p.initial != nullptr ? Tl::load(p.initial + state_at(sequence), seg.count) : Row<V>::all(0.f); };
 
   constexpr int kArrays = kGate ? 4 : 2;
   const T* gate = static_cast<const T*>(p.gate) + seg.col;
@@ -482,20 +529,23 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
   const Row<V> zero = Row<V>::all(0.f);
   auto zeroth = [&](const Row<V>& h) {           // row 0, where it was left out of the walk
     Raw<T, V> g, d, x;
-    g.load(base[0]); d.load(base[1]);
-    if constexpr (kGate) x.load(base[2]); else x = g;
+    auto load = [&](Raw<T, V>& to, const T* from) {
+      if constexpr (Tl::kStrided) to.gather(from, Tl::apart(1), seg.count); else to.load(from);
+    };
+    load(g, base[0]); load(d, base[1]);
+    if constexpr (kGate) load(x, base[2]); else x = g;
     step(0, g.get(), d.get(), x.get(), h);
   };
   const bool dense = p.offsets == nullptr;
   if (dense || within_one(p, seg.first - 1, seg.last + 1)) {
     if (dense && seg.part == s.parts - 1) begin(seg.sequence);
     const int start = dense ? seg.sequence * p.length : -1;
-    walk_rows<T, V, true, kArrays>(first, seg.last, base, stride, [&](int t, Raw<T, V> (&row)[kArrays]) {
+    walk_rows<T, Tl, true, kArrays>(seg, first, base, stride, [&](int t, Raw<T, V> (&row)[kArrays]) {
       if constexpr (kGate) step(t, row[0].get(), row[1].get(), row[2].get(), t == start ? initial(seg.sequence) : row[3].get());
       else step(t, row[0].get(), row[1].get(), zero, zero);
     });
     if (first > seg.first && seg.first < seg.last) zeroth(initial(0));
-    if (dense && seg.first == start && seg.first < seg.last && p.dinitial != nullptr) store_state<V>(p.dinitial + state_at(seg.sequence), back);
+    if (dense && seg.first == start && seg.first < seg.last && p.dinitial != nullptr) Tl::store(p.dinitial + state_at(seg.sequence), back, seg.count);
   } else {
     SequenceWalk walk(p, seg.last);
     int behind = walk.at(p, seg.last), sequence = walk.at(p, seg.last - 1);
@@ -504,14 +554,14 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
       if (sequence >= 0) {
         if (sequence != behind) begin(sequence);
         calculate(sequence != previous);
-        if (sequence != previous && p.dinitial != nullptr) store_state<V>(p.dinitial + state_at(sequence), back);
+        if (sequence != previous && p.dinitial != nullptr) Tl::store(p.dinitial + state_at(sequence), back, seg.count);
       } else {
         outside(t);
       }
       behind = sequence;
       sequence = previous;
     };
-    walk_rows<T, V, true, kArrays>(first, seg.last, base, stride, [&](int t, Raw<T, V> (&row)[kArrays]) {
+    walk_rows<T, Tl, true, kArrays>(seg, first, base, stride, [&](int t, Raw<T, V> (&row)[kArrays]) {
       packed(t, [&](bool start) {
         if constexpr (kGate) step(t, row[0].get(), row[1].get(), row[2].get(), start ? initial(sequence) : row[3].get());
         else step(t, row[0].get(), row[1].get(), zero, zero);
@@ -557,31 +607,31 @@ int vector_of(const ScanGradParams& p) {
   return vector_of(p.half, p.channels, {{p.gate, p.gate_stride}, {p.x, p.x_stride}, {p.dh, p.dh_stride}}, {p.initial, p.dfinal});
 }
 template <class F>
-cudaError_t by_vector(int half, int vec, F f) {
+cudaError_t by_tile(int half, int vec, F f) {
   if (half) {
-    if (vec == 8) return f(__nv_bfloat16{}, std::integral_constant<int, 8>{});
-    if (vec == 2) return f(__nv_bfloat16{}, std::integral_constant<int, 2>{});
-    return f(__nv_bfloat16{}, std::integral_constant<int, 1>{});
+    if (vec == 8) return f(__nv_bfloat16{}, Tile<8, false>{});
+    if (vec == 2) return f(__nv_bfloat16{}, Tile<2, false>{});
+    return f(__nv_bfloat16{}, Tile<4, true>{});
   }
-  if (vec == 4) return f(float{}, std::integral_constant<int, 4>{});
-  return f(float{}, std::integral_constant<int, 1>{});
+  if (vec == 4) return f(float{}, Tile<4, false>{});
+  return f(float{}, Tile<4, true>{});
 }
 
 ScanSplit split_of(const ScanShape& p, int vec, int sms, bool back) {
   ScanSplit s{};
   const long long sequences = p.offsets == nullptr ? p.sequences : 1, length = p.offsets == nullptr ? p.length : p.rows;
-  const long long vectors = p.channels / vec;
-  const int lanes = vec >= 4 ? 8 : 32, segs = kScanThreads / lanes;
+  const int lanes = vec >= 4 ? 8 : 32, segs = kScanThreads / lanes, cols = lanes * (vec == 1 ? 4 : vec);
+  s.tiles = (p.channels + cols - 1) / cols;
+  const long long vectors = static_cast<long long>(s.tiles) * lanes;
   // Threads that are enough to keep memory busy, and at least 16 rows a segment.  One sequence of 131072 rows of 1024 channels, with 384 and 1200 vectors of 16
   // bytes an SM: forward 232 and 260 us, backward 470 and 396.
-  const long long enough = static_cast<long long>(sms) * (vec < 4 ? 1536 : back ? 1200 : 384);
+  const long long enough = static_cast<long long>(sms) * (vec == 2 ? 1536 : vec == 1 ? 768 : back ? 1200 : 384);
   long long parts = 1;
   while (sequences * vectors * parts < enough && length > 32 * parts) parts *= 2;
   s.rows = static_cast<int>((length + parts - 1) / parts);
   if (s.rows < 1) s.rows = 1;
   s.parts = static_cast<int>(length > 0 ? (length + s.rows - 1) / s.rows : 1);
   s.segments = static_cast<int>(sequences * s.parts);
-  s.tiles = static_cast<int>((vectors + lanes - 1) / lanes);
   s.blocks = (s.segments + segs - 1) / segs;
   s.within = s.blocks <= 1 || segs % s.parts == 0;
   return s;
@@ -620,8 +670,8 @@ void lay_out(ScanSplit& s, int channels, void* space) {
   s.block_sums = s.block_factors + static_cast<long long>(s.blocks) * channels;
 }
 // Blocks of the walks: their ring, or the runs in its place.
-template <class T, int V, int kArrays> constexpr int walk_bytes() {
-  return std::max(ring_bytes<T, V, kArrays>(), Tile<V>::SEGS * Tile<V>::COLS * static_cast<int>(sizeof(Run)));
+template <class T, class Tl, int kArrays> constexpr int walk_bytes() {
+  return std::max(ring_bytes<T, Tl, kArrays>(), Tl::SEGS * Tl::COLS * static_cast<int>(sizeof(Run)));
 }
 
 }  // namespace
@@ -631,40 +681,43 @@ ScanSplit scan_split(const ScanGradParams& p, int sms) { return split_of(p, vect
 long long scan_space(const ScanSplit& s, int channels) { return s.within ? 0 : 8ll * (static_cast<long long>(s.segments) + s.blocks) * channels; }
 
 cudaError_t launch_scan_forward(const ScanParams& p, ScanSplit s, void* space, cudaStream_t stream) {
-  return by_vector(p.half, vector_of(p), [&](auto type, auto v) {
+  return by_tile(p.half, vector_of(p), [&](auto type, auto tile) {
     using T = decltype(type);
-    constexpr int V = decltype(v)::value, smem = walk_bytes<T, V, 2>();
+    using Tl = decltype(tile);
+    constexpr int smem = walk_bytes<T, Tl, 2>();
     const dim3 grid(static_cast<unsigned>(std::max(1, s.blocks * s.tiles)));
     if (!s.within) {
       lay_out(s, p.channels, space);
-      const cudaError_t e = launch<scan_runs_kernel<T, V, false>>(grid, smem, false, stream, static_cast<const ScanShape&>(p), s, p.x, p.x_stride, p.initial);
+      const cudaError_t e = launch<scan_runs_kernel<T, Tl, false>>(grid, smem, false, stream, static_cast<const ScanShape&>(p), s, p.x, p.x_stride, p.initial);
       if (e != cudaSuccess) return e;
     }
-    return launch<scan_forward_kernel<T, V>>(grid, smem, !s.within, stream, p, s);
+    return launch<scan_forward_kernel<T, Tl>>(grid, smem, !s.within, stream, p, s);
   });
 }
 
 cudaError_t launch_scan_backward(const ScanGradParams& p, ScanSplit s, void* space, cudaStream_t stream) {
-  return by_vector(p.half, vector_of(p), [&](auto type, auto v) {
+  return by_tile(p.half, vector_of(p), [&](auto type, auto tile) {
     using T = decltype(type);
-    constexpr int V = decltype(v)::value, smem = walk_bytes<T, V, 2>();
+    using Tl = decltype(tile);
+    constexpr int smem = walk_bytes<T, Tl, 2>();
     const dim3 grid(static_cast<unsigned>(std::max(1, s.blocks * s.tiles)));
     if (!s.within) {
       lay_out(s, p.channels, space);
-      const cudaError_t e = launch<scan_runs_kernel<T, V, true>>(grid, smem, false, stream, static_cast<const ScanShape&>(p), s, p.dh, p.dh_stride, p.dfinal);
+      const cudaError_t e = launch<scan_runs_kernel<T, Tl, true>>(grid, smem, false, stream, static_cast<const ScanShape&>(p), s, p.dh, p.dh_stride, p.dfinal);
       if (e != cudaSuccess) return e;
     }
-    if (p.dgate == nullptr) return launch<scan_backward_kernel<T, V, false>>(grid, smem, !s.within, stream, p, s);
-    return launch<scan_backward_kernel<T, V, true>>(grid, walk_bytes<T, V, 4>(), !s.within, stream, p, s);
+    if (p.dgate == nullptr) return launch<scan_backward_kernel<T, Tl, false>>(grid, smem, !s.within, stream, p, s);
+    return launch<scan_backward_kernel<T, Tl, true>>(grid, walk_bytes<T, Tl, 4>(), !s.within, stream, p, s);
   });
 }
 
 cudaError_t launch_scan_step(const ScanStepParams& p, cudaStream_t stream) {
   const int vec = vector_of(p.half, p.channels, {{p.gate, p.gate_stride}, {p.x, p.x_stride}, {nullptr, 0}}, {p.state, reinterpret_cast<const void*>(p.state_stride * 4)});
-  return by_vector(p.half, vec, [&](auto type, auto v) {
-    const long long threads = static_cast<long long>(p.rows) * (p.channels / vec);
-    return launch<scan_step_kernel<decltype(type), decltype(v)::value>>(dim3(static_cast<unsigned>((threads + kScanThreads - 1) / kScanThreads)), 0, false, stream, p);
-  });
+  const long long threads = static_cast<long long>(p.rows) * (p.channels / vec);
+  const dim3 grid(static_cast<unsigned>((threads + kScanThreads - 1) / kScanThreads));
+  if (!p.half) return vec == 4 ? launch<scan_step_kernel<float, 4>>(grid, 0, false, stream, p) : launch<scan_step_kernel<float, 1>>(grid, 0, false, stream, p);
+  if (vec == 8) return launch<scan_step_kernel<__nv_bfloat16, 8>>(grid, 0, false, stream, p);
+  return vec == 2 ? launch<scan_step_kernel<__nv_bfloat16, 2>>(grid, 0, false, stream, p) : launch<scan_step_kernel<__nv_bfloat16, 1>>(grid, 0, false, stream, p);
 }
 
 }  // namespace sep
