@@ -21,7 +21,19 @@ struct RouteCall : torch::CustomClassHolder {
   bool renormalize;
 };
 
-struct Route { at::Tensor idx, weights, in_rank, balance, z, counts, probs, lse, load; };
+// `kept`, for the backward: probabilities [T, E], logsumexp [T], load [E] and 1 / n; behind them what the blocks leave to be added up.
+struct Route { at::Tensor idx, weights, in_rank, balance, z, counts, kept; };
+struct Kept {
+  float *probs, *lse, *load;
+  float2 *other_parts, *parts;
+  int64_t floats;
+  Kept(float* base, int64_t T, int64_t E, int64_t blocks) {
+    const int64_t at_lse = T * E, at_load = at_lse + T, at_other = (at_load + E + 1 + 1) / 2 * 2, at_parts = at_other + 2 * blocks;
+    floats = at_parts + 2 * blocks * E;
+    probs = base; lse = base + at_lse; load = base + at_load;
+    other_parts = reinterpret_cast<float2*>(base + at_other); parts = reinterpret_cast<float2*>(base + at_parts);
+  }
+};
 
 const unsigned char* mask_of(const at::Tensor& mask) { return mask.defined() ? reinterpret_cast<const unsigned char*>(mask.data_ptr<bool>()) : nullptr; }
 
@@ -35,9 +47,6 @@ Route route_forward(const RouteCall& call, const at::Tensor& x, const at::Tensor
   r.balance = at::empty({}, f32);
   r.z = at::empty({}, f32);
   r.counts = at::empty({E}, x.options().dtype(at::kLong));
-  r.probs = at::empty({T, E}, f32);
-  r.lse = at::empty({T}, f32);
-  r.load = at::empty({E + 1}, f32);
   const LaunchContext ctx = call.context(T > 0 ? 2 : 1);
   RouterParams p{};
   p.x = x.data_ptr(); p.w_gate = w.data_ptr();
@@ -46,18 +55,16 @@ Route route_forward(const RouteCall& call, const at::Tensor& x, const at::Tensor
   p.topk_idx = reinterpret_cast<long long*>(r.idx.data_ptr<int64_t>());
   p.topk_weights = r.weights.data_ptr<float>();
   p.is_token_in_rank = reinterpret_cast<unsigned char*>(r.in_rank.data_ptr<bool>());
-  p.probs = r.probs.data_ptr<float>();
-  p.lse = r.lse.data_ptr<float>();
   RouteStatsParams s{};
   s.experts = static_cast<int>(E); s.top_k = call.top_k;
   s.mask = mask_of(mask);
   s.blocks = route_blocks(p, ctx.sms);
-  const at::Tensor parts = at::empty({s.blocks * (2 * E + 2) + 2}, f32);
-  s.other_parts = reinterpret_cast<float2*>(parts.data_ptr<float>());
-  s.parts = s.other_parts + s.blocks;
+  r.kept = at::empty({Kept(nullptr, T, E, s.blocks).floats}, f32);
+  const Kept kept(r.kept.data_ptr<float>(), T, E, s.blocks);
+  p.probs = kept.probs; p.lse = kept.lse;
+  s.other_parts = kept.other_parts; s.parts = kept.parts; s.load = kept.load;
   s.balance = r.balance.data_ptr<float>(); s.z = r.z.data_ptr<float>();
   s.counts = reinterpret_cast<long long*>(r.counts.data_ptr<int64_t>());
-  s.load = r.load.data_ptr<float>();
   CUtensorMap mw{}, mx{};
   if (T > 0) {
     mw = make_tmap(w.data_ptr(), H, E, 1, H, E * H, 64, 128);
@@ -73,7 +80,7 @@ class BalancedRoute : public torch::autograd::Function<BalancedRoute> {
                                                 const std::optional<at::Tensor>& counted, const c10::intrusive_ptr<RouteCall>& call) {
     const at::Tensor mask = counted.value_or(at::Tensor());
     Route r = route_forward(*call, readable(x), readable(w_gate), mask);
-    ctx->save_for_backward({x, w_gate, mask, r.probs, r.lse, r.load, r.idx, r.weights});
+    ctx->save_for_backward({x, w_gate, mask, r.kept, r.idx, r.weights});
     ctx->saved_data["call"] = c10::IValue::make_capsule(call);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({r.idx, r.in_rank, r.counts});
@@ -83,10 +90,11 @@ class BalancedRoute : public torch::autograd::Function<BalancedRoute> {
     SEP_ASSERT(!at::GradMode::is_enabled(), "balanced_router has no second derivative: its backward was asked for a graph");
     auto call = c10::static_intrusive_pointer_cast<RouteCall>(ctx->saved_data["call"].toCapsule());
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &w_gate = saved[1], &mask = saved[2], &probs = saved[3], &lse = saved[4], &load = saved[5], &idx = saved[6], &weights = saved[7];
+    const at::Tensor &x = saved[0], &w_gate = saved[1], &mask = saved[2], &idx = saved[4], &weights = saved[5];
     if (!grads[1].defined() && !grads[3].defined() && !grads[4].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
     const int64_t T = x.size(0), H = x.size(1), E = w_gate.size(0);
+    const Kept kept(saved[3].data_ptr<float>(), T, E, 0);
     const c10::cuda::CUDAGuard guard(x.device());
     // A thread of the autograd engine may not have made a call of the CUDA runtime yet, and the driver encodes tensor maps only
     // with a context bound to the thread.
@@ -101,11 +109,11 @@ class BalancedRoute : public torch::autograd::Function<BalancedRoute> {
       at::Tensor up[3];
       for (int i = 0; i < 3; ++i) {
         const at::Tensor& g = grads[i == 0 ? 1 : i + 2];
-        if (g.defined()) up[i] = g.to(at::kFloat).contiguous();
+        if (g.defined()) up[i] = g.scalar_type() == at::kFloat && g.is_contiguous() ? g : g.to(at::kFloat).contiguous();
       }
       RouteGradParams p{};
       p.tokens = static_cast<int>(T); p.experts = static_cast<int>(E); p.top_k = call->top_k; p.hidden = static_cast<int>(H); p.renormalize = call->renormalize;
-      p.probs = probs.data_ptr<float>(); p.lse = lse.data_ptr<float>(); p.load = load.data_ptr<float>();
+      p.probs = kept.probs; p.lse = kept.lse; p.load = kept.load;
       p.idx = reinterpret_cast<const long long*>(idx.data_ptr<int64_t>());
       p.weights = weights.data_ptr<float>();
       p.mask = mask_of(mask);

@@ -385,7 +385,8 @@ RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
   g.dx_splits = tiles > 0 ? sms / tiles : 1;
   if (g.dx_splits > n_tiles) g.dx_splits = n_tiles;
   if (g.dx_splits < 1) g.dx_splits = 1;
-  g.dx_staging = g.padded <= 256 ? 2 : 1;
+  // (a fourth stage of W is worth more than a second tile of results a warp)
+  g.dx_staging = g.padded <= 128 ? 2 : 1;
   const int fixed = 1024 + g.padded * kTokens * 2 + kEpiWarps * g.dx_staging * kStaging;
   g.dx_stages = (kMostSmem - fixed) / (4 * kChunk);
   if (g.dx_stages > 4) g.dx_stages = 4;
