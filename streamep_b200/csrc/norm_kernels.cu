@@ -406,7 +406,7 @@ Form form_of(int half, int hidden, bool sixteen, bool four) {
   f.vec = sixteen ? (half ? 8 : 4) : half && four ? 2 : 1;
   const int vectors = hidden / f.vec;
   // Few vectors a thread keep short rows of single numbers and pairs from waiting for one another's loads: 1777 rows of 1001 fp32 columns with 16 a
-  // thread 19.5 us, with 4 XXX.  (Whole vectors the other way: 8192 rows of 2048 with one a thread 32.9, with two 27.9.)
+  // thread 19.5 us forward, with 4 8.8.  (Whole vectors the other way: 8192 rows of 2048 with one a thread 32.9, with two 27.9.)
   f.each = vectors <= 32 ? 1 : f.vec == 1 && vectors <= 1024 ? 4 : f.vec == 2 && vectors <= 512 ? 2 : 16 / f.vec;
   f.threads = (vectors + f.each - 1) / f.each;                 // whole warps; more than half of them, a block that is not full
   f.threads = (f.threads + 31) / 32 * 32;

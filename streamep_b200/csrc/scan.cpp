@@ -157,6 +157,7 @@ at::Tensor gated_scan_step(const at::Tensor& state, const at::Tensor& x, const a
              "state must be float32 and have the shape and device of x");
   SEP_ASSERT((state.size(1) == 1 || state.stride(1) == 1) && (state.size(0) <= 1 || state.stride(0) >= state.size(1)),
              "state is changed in place: its rows must be contiguous and must not overlap");
+  SEP_ASSERT(!state.is_alias_of(x) && !state.is_alias_of(gate), "state is changed in place: it must not share memory with x or gate");
   SEP_ASSERT(!(at::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || state.requires_grad())),
              "gated_scan_step_ has no gradient: call it under torch.no_grad(), or gated_scan");
   SEP_ASSERT(!x._fw_grad(0).defined() && !gate._fw_grad(0).defined() && !state._fw_grad(0).defined(), "gated_scan_step_ has no forward-mode derivative");

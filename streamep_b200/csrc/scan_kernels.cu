@@ -91,7 +91,7 @@ struct SequenceWalk {
   __device__ __forceinline__ bool all_within(const ScanShape& p, int end) const { return i >= 0 && i < p.sequences && end <= behind && end <= p.rows; }
 };
 // Of a packed batch: whether all rows from `before` to `end` are of one sequence.  Then nothing starts or ends among them, which saves the rows' own
-// looks (in 32 bits without vectors 7488 rows of 1001 channels 252 -> XXX us with gradients).
+// looks (7488 rows of 1001 fp32 channels in 9 sequences, forward and backward, 252 -> 131 us).
 __device__ __forceinline__ bool within_one(const ScanShape& p, int before, int end) {
   if (before < 0) return false;
   SequenceWalk walk(p, before);
@@ -101,7 +101,7 @@ __device__ __forceinline__ bool within_one(const ScanShape& p, int before, int e
 // A block's threads: LANES side by side across the channels, V channels each, and SEGS segments above one another.  Where runs are joined, PARTS
 // threads share a channel.  A thread's channels are one vector; or with kApart, where rows do not begin on boundaries of vectors, every 32nd: a warp then
 // reads and writes neighbouring numbers, and still has V of them for each row that it counts off (7488 rows of 1001 fp32 channels with gradients 131 us
-// one by one, XXX so).
+// one by one, 115 so).
 template <int Vec, bool kApart> struct Tile {
   static constexpr int V = Vec;
   static constexpr bool kStrided = kApart;
@@ -623,11 +623,13 @@ ScanSplit split_of(const ScanShape& p, int vec, int sms, bool back) {
   const int lanes = vec >= 4 ? 8 : 32, segs = kScanThreads / lanes, cols = lanes * (vec == 1 ? 4 : vec);
   s.tiles = (p.channels + cols - 1) / cols;
   const long long vectors = static_cast<long long>(s.tiles) * lanes;
-  // Threads that are enough to keep memory busy, and at least 16 rows a segment.  One sequence of 131072 rows of 1024 channels, with 384 and 1200 vectors of 16
+  // Threads that are enough to keep memory busy, and 16 to 32 rows a segment at least.  One sequence of 131072 rows of 1024 channels, with 384 and 1200 vectors of 16
   // bytes an SM: forward 232 and 260 us, backward 470 and 396.
   const long long enough = static_cast<long long>(sms) * (vec == 2 ? 1536 : vec == 1 ? 768 : back ? 1200 : 384);
   long long parts = 1;
   while (sequences * vectors * parts < enough && length > 32 * parts) parts *= 2;
+  // (short calls: 4096 rows of 1024 channels in segments of 32 and 16 rows forward 21.5 and 19.5 us, backward 29.7 and 25.7; 8192 rows of 2048 backward 58.6 and 65.6)
+  while (sequences * vectors * parts < sms * 256ll && length > 16 * parts) parts *= 2;
   s.rows = static_cast<int>((length + parts - 1) / parts);
   if (s.rows < 1) s.rows = 1;
   s.parts = static_cast<int>(length > 0 ? (length + s.rows - 1) / s.rows : 1);

@@ -50,8 +50,8 @@ def make_buffer(group, num_tokens: int, hidden: int, num_topk: int, num_experts:
 
 class StreamMoE(nn.Module):
     """Router and experts.  ``train_router``: the gate's weight is trained (it is a plain parameter then, replicated over the ranks); a forward
-    with gradients leaves its :class:`BalancedRoute` in ``last_route``, whose ``balance_loss`` and ``z_loss`` the program adds to
-    its loss and whose ``expert_counts`` it may watch.  Without gradients the tokens are routed by :func:`router_topk`."""
+    with gradients leaves its :class:`BalancedRoute` in ``last_route``, whose ``expert_counts`` the program may watch and whose losses it adds to its
+    own by :meth:`router_losses`.  Without gradients the tokens are routed by :func:`router_topk`."""
 
     def __init__(self, hidden: int, ffn: int, num_experts: int, top_k: int, buffer: Buffer, *,
                  streams: Optional[StreamHolder] = None, tile_config: Optional[TileConfig] = None,
@@ -89,12 +89,22 @@ class StreamMoE(nn.Module):
     def route(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None):
         """``(topk_idx, topk_weights, is_token_in_rank)`` from the fused router kernel.  ``mask``: tokens that count in the losses of a trained
         router."""
+        self.last_route = None           # (the graph of the forward before must not outlive it)
         if self.train_router and torch.is_grad_enabled():
             self.last_route = balanced_router(x, self.w_gate, self.top_k, num_ranks=self.ep_size, renormalize=self.renormalize, mask=mask,
                                               buffer=self.buffer)
             return self.last_route[:3]
         return router_topk(x.detach(), self.w_gate, self.top_k, num_ranks=self.ep_size,
                            renormalize=self.renormalize, buffer=self.buffer)
+
+    def router_losses(self):
+        """``(balance_loss, z_loss)`` of the last forward with gradients, once: the module keeps their values but not their graph, which would otherwise
+        live on until the next forward."""
+        if self.last_route is None or not self.last_route.balance_loss.requires_grad:
+            raise RuntimeError("router_losses() belongs to one forward with gradients of a layer whose router is trained")
+        losses = self.last_route.balance_loss, self.last_route.z_loss
+        self.last_route = BalancedRoute(*(t.detach() for t in self.last_route))
+        return losses
 
     def experts(self, x, topk_idx, topk_weights, is_token_in_rank):
         return stream_moe_func(self.buffer, x, topk_idx, topk_weights, is_token_in_rank, self.w1, self.w2,

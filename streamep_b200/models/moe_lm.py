@@ -87,9 +87,9 @@ class MoELM(nn.Module):
         return layer_norm(added, residual=x)[0]
 
     def router_losses(self) -> torch.Tensor:
-        """The gates' losses of the last forward, with their coefficients, averaged over the layers."""
-        routes = [layer.last_route for layer in self.layers]
-        return sum(self.balance_coef * r.balance_loss + self.z_coef * r.z_loss for r in routes) / len(routes)
+        """The gates' losses of the last forward, with their coefficients, averaged over the layers; once, as :meth:`StreamMoE.router_losses`."""
+        losses = [layer.router_losses() for layer in self.layers]
+        return sum(self.balance_coef * balance + self.z_coef * z for balance, z in losses) / len(losses)
 
     def forward(self, tokens: torch.Tensor, targets: torch.Tensor, reduction: str = "mean", offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
         loss = linear_cross_entropy(self.hidden_states(tokens, offsets), self.head, targets.reshape(-1), reduction=reduction, buffer=self.buffer)

@@ -23,7 +23,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     Differentiable in all four tensors; there is no second derivative.  Mean and variance (of centred values), and all sums, are
     formed in 32 bits, the gradients of ``x + residual`` before its rounding too (so both are kept for the backward, not the sum).  A
-    repeated call gives the same bits.  A row with an infinity or NaN becomes NaN, and so do weight and bias' gradients that it has a part in."""
+    repeated call gives the same bits.  A row with an infinity or NaN becomes NaN, and so do weight and bias' gradients that it has a part in; squares above the
+    range of 32 bits (values 1.8e19 from the mean) make a row's outputs 0."""
     out = _ext.load().norm_rows(x, weight, bias, residual, True, float(eps))
     return (out[0], out[1]) if residual is not None else out[0]
 

@@ -103,6 +103,12 @@ def test_steps_of_a_run(native):
     assert all(not torch.equal(a, p) for a, p in zip(before, opt.params))
     for layer in model.layers:
         assert int(layer.last_route.expert_counts.sum()) == 2 * 256
+        assert not layer.last_route.balance_loss.requires_grad and not layer.last_route.topk_weights.requires_grad      # no graph is kept
+        with pytest.raises(RuntimeError, match="one forward"):
+            layer.router_losses()
+    with torch.no_grad():
+        model(*batch(2, 128))
+    assert all(layer.last_route is None for layer in model.layers)
 
 
 def test_packed_is_dense(native):

@@ -390,7 +390,7 @@ def test_refusals(native):
               lambda: gated_scan(x[..., :0], gate[..., :0]), lambda: gated_scan(x, gate.cpu()),
               lambda: gated_scan_step_(state, x[:, 0], gate[:, 0].to(BF)), lambda: gated_scan_step_(state.to(BF), x[:, 0], gate[:, 0]),
               lambda: gated_scan_step_(state[:1].expand(2, 16), x[:, 0], gate[:, 0]), lambda: gated_scan_step_(torch.zeros(16, 2, device=DEV).t(), x[:, 0], gate[:, 0]),
-              lambda: gated_scan_step_(state, x, gate)):
+              lambda: gated_scan_step_(state, x, gate), lambda: gated_scan_step_(state, state, gate[:, 0]), lambda: gated_scan_step_(state, x[:, 0], state)):
         with pytest.raises(ValueError):
             f()
     leaf = x.clone().requires_grad_(True)
