@@ -124,7 +124,7 @@ class BalancedRoute : public torch::autograd::Function<BalancedRoute> {
       p.dw = want_dw ? dw.data_ptr() : nullptr;
       p.status = context.status; p.rank = context.rank; p.wait_budget_ns = context.wait_budget_ns;
       at::Tensor space;                          // dz, and the parts of dw
-      const int64_t dz_bytes = (T * plan.padded * 2 + 255) / 256 * 256, parts = plan.dw_splits > 1 ? plan.dw_splits : 0;
+      const int64_t dz_bytes = (plan.layers * T * plan.padded * 2 + 255) / 256 * 256, parts = plan.dw_splits > 1 ? plan.dw_splits : 0;
       if (want_dw) {
         space = at::empty({dz_bytes + parts * E * H * 4}, x.options().dtype(at::kByte));
         p.dz = space.data_ptr();
@@ -137,7 +137,7 @@ class BalancedRoute : public torch::autograd::Function<BalancedRoute> {
       SEP_CUDA_CHECK(launch_route_dx(p, plan, &map_w, &map_dx, context.stream));
       if (want_dw) {
         float* sums = reinterpret_cast<float*>(static_cast<char*>(space.data_ptr()) + dz_bytes);
-        const CUtensorMap map_dz = make_tmap(p.dz, plan.padded, T, 1, plan.padded, T * plan.padded, 64, 64), map_x = make_tmap(xr.data_ptr(), H, T, 1, H, T * H, 64, 64),
+        const CUtensorMap map_dz = make_tmap(p.dz, plan.padded, T, plan.layers, plan.padded, T * plan.padded, 64, 64), map_x = make_tmap(xr.data_ptr(), H, T, 1, H, T * H, 64, 64),
                           map_out = parts > 0 ? make_tmap(sums, H, E, parts, H, E * H, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT32)
                                               : make_tmap(p.dw, H, E, 1, H, E * H, 64, 32);
         SEP_CUDA_CHECK(launch_route_dw(p, plan, &map_dz, &map_x, &map_out, sums, context.stream));

@@ -35,22 +35,22 @@ struct RouteGradParams {
   const float* dweights;         // [tokens, top_k] or null
   const float* dbalance;         // one number or null
   const float* dz_loss;          // one number or null
-  void* dz;                      // [tokens, padded] bf16: the logits' gradients, or null (no dw)
+  void* dz;                      // [layers, tokens, padded] bf16: the logits' gradients, or null (no dw)
   void* dx;                      // [tokens, hidden] bf16, or null
   void* dw;                      // [experts, hidden] bf16, or null
   StatusBlock* status;
   int rank;
   unsigned long long wait_budget_ns;
 };
-// How the products are cut up: `padded` experts (a multiple of 64); blocks that share the columns of 128 tokens' dx; experts (in blocks of 128) and parts of
+// How the products are cut up: `padded` experts (a multiple of 64), in `layers` matrices; blocks that share the columns of 128 tokens' dx; experts (in blocks of 128) and parts of
 // the tokens of a unit of dW.
 struct RouteGradPlan {
-  int padded;
+  int padded, layers;            // of dz: bf16 numbers that add up to it
   int dx_splits, dx_stages, dx_staging, dx_smem;
   int dw_blocks, dw_splits, dw_units, dw_stages, dw_smem;
 };
 RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms);
-// Maps: `map_w` [E, H] boxes of 64 x 64, `map_dx` [T, H] boxes of 32 rows x 64; `map_dz` [T, padded] and `map_x` [T, H] boxes of 64 x 64; `map_out` dW boxes of
+// Maps: `map_w` [E, H] boxes of 64 x 64, `map_dx` [T, H] boxes of 32 rows x 64; `map_dz` [layers, T, padded] and `map_x` [T, H] boxes of 64 x 64; `map_out` dW boxes of
 // 32 x 64 (bf16), or with several parts [splits, E, H] fp32 boxes of 32 x 32 over `parts`.  All with 128-byte swizzle.
 cudaError_t launch_route_dx(const RouteGradParams& p, const RouteGradPlan& g, const void* map_w, const void* map_dx, cudaStream_t stream);
 cudaError_t launch_route_dw(const RouteGradParams& p, const RouteGradPlan& g, const void* map_dz, const void* map_x, const void* map_out, float* parts, cudaStream_t stream);

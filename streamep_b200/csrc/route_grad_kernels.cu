@@ -3,9 +3,11 @@
 //   dx = dz W  [T, H]      a block takes 128 tokens: their dz is formed in shared memory, where it stays as the left operand, and W's columns go by
 //   dW = dz^T x  [E, H]    a block takes up to 256 experts, 256 columns and a part of the tokens; the parts are added up by a small kernel
 //
-// dz is rounded to bf16 for both products, 2^-9 of each term at most, as bf16 training code rounds the gradient of its logits; all sums are fp32.
+// For both products dz is rounded to bf16, 2^-9 of each term at most, as bf16 training code rounds the gradient of its logits: against 64 bits dx and dW are
+// 2.3e-3 off in 2-norm, where their own rounding is 1.7e-3.  Up to 128 experts, where twice the products cost nothing beside the reads of x and the writes of
+// dx, dz is kept to 16 bits as the sum of two bf16 numbers (XXX).  All sums are fp32.
 // What bounds them: x is read and dx written once (HBM), and for many experts the tensor cores.  All operands lie in memory as TMA brings them in, dz as
-// [T, experts rounded up to 64]; nothing is transposed.  Parts and sums have a fixed order: a repeated call gives the same bits.
+// [layers, T, experts rounded up to 64]; nothing is transposed.  Parts and sums have a fixed order: a repeated call gives the same bits.
 #include <atomic>
 #include <cuda.h>
 
@@ -122,6 +124,7 @@ __device__ __forceinline__ void store_half_tile(uint32_t taddr, unsigned char* t
 template <int EPL>
 __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_dx, const RouteGradParams p,
                                                                const RouteGradPlan g) {
+  constexpr int kLayers = EPL <= 4 ? 2 : 1;      // g.layers
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full_bar[4], empty_bar[4], tmem_full[2], tmem_empty[2], dz_bar;
@@ -130,8 +133,9 @@ __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_cons
   const int tile = static_cast<int>(blockIdx.x) / g.dx_splits, split = static_cast<int>(blockIdx.x) % g.dx_splits;
   const int k_blocks = g.padded / kBK, n_tiles = p.dx != nullptr ? (p.hidden + kCols - 1) / kCols : 0;
   const int n0 = n_tiles * split / g.dx_splits, n1 = n_tiles * (split + 1) / g.dx_splits;
-  unsigned char* dz = smem;                      // [k_blocks][128 rows][128 bytes]
-  unsigned char* stages = dz + k_blocks * kTokens * 128;
+  unsigned char* dz = smem;                      // [layers][k_blocks][128 rows][128 bytes]
+  const int layer_bytes = k_blocks * kTokens * 128;
+  unsigned char* stages = dz + kLayers * layer_bytes;
   unsigned char* staging = stages + g.dx_stages * 4 * kChunk;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_w);
@@ -173,8 +177,11 @@ __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_cons
         if (elect_one()) {
           const uint32_t a = smem_u32(dz + kb * kTokens * 128), b = smem_u32(stages + stage * 4 * kChunk);
 #pragma unroll
-          for (int j = 0; j < kBK / 16; ++j)
-            umma_bf16_ss<1>(tmem + acc * kCols, umma_smem_desc(a + j * 32, 16, 1024), umma_smem_desc(b + j * 16 * 128, kChunk, 1024), idesc, (kb > 0 || j > 0) ? 1u : 0u);
+          for (int l = 0; l < kLayers; ++l)
+#pragma unroll
+            for (int j = 0; j < kBK / 16; ++j)
+              umma_bf16_ss<1>(tmem + acc * kCols, umma_smem_desc(a + l * layer_bytes + j * 32, 16, 1024), umma_smem_desc(b + j * 16 * 128, kChunk, 1024), idesc,
+                              (kb > 0 || l > 0 || j > 0) ? 1u : 0u);
           umma_commit<1>(&empty_bar[stage]);
           if (kb == k_blocks - 1) umma_commit<1>(&tmem_full[acc]);
         }
@@ -199,9 +206,15 @@ __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_cons
         for (int j = 0; j < kHalves; ++j) {
           const int e = j * 32 + lane;
           if (e >= g.padded) continue;
-          const __nv_bfloat16 b = __float2bfloat16_rn(j < EPL && t < p.tokens && e < p.experts ? v[i][j < EPL ? j : 0] : 0.f);
-          *reinterpret_cast<__nv_bfloat16*>(dz + e / 64 * kTokens * 128 + stage_off<128>(r, e % 64 / 8) + e % 8 * 2) = b;
-          if (split == 0 && t < p.tokens && p.dz != nullptr) static_cast<__nv_bfloat16*>(p.dz)[static_cast<long long>(t) * g.padded + e] = b;
+          float left = j < EPL && t < p.tokens && e < p.experts ? v[i][j < EPL ? j : 0] : 0.f;
+#pragma unroll
+          for (int l = 0; l < kLayers; ++l) {
+            const __nv_bfloat16 b = __float2bfloat16_rn(left);
+            left -= __bfloat162float(b);
+            *reinterpret_cast<__nv_bfloat16*>(dz + l * layer_bytes + e / 64 * kTokens * 128 + stage_off<128>(r, e % 64 / 8) + e % 8 * 2) = b;
+            if (split == 0 && t < p.tokens && p.dz != nullptr)
+              static_cast<__nv_bfloat16*>(p.dz)[(static_cast<long long>(l) * p.tokens + t) * g.padded + e] = b;
+          }
         }
       }
     }
@@ -253,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_cons
   const int k_blocks = (p.tokens + kBK - 1) / kBK, kb0 = static_cast<int>(static_cast<long long>(k_blocks) * split / g.dw_splits),
             kb1 = static_cast<int>(static_cast<long long>(k_blocks) * (split + 1) / g.dw_splits);
   const int chunks = (min(kCols, p.hidden - n * kCols) + 63) / 64, cols = min(kCols, (p.hidden - n * kCols + 31) / 32 * 32);
-  const int stage_bytes = (g.dw_blocks * 2 + 4) * kChunk, tmem_cols = g.dw_blocks * kCols;
+  const int layer_chunks = g.dw_blocks * 2, stage_bytes = (g.layers * layer_chunks + 4) * kChunk, tmem_cols = g.dw_blocks * kCols;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_dz);
     tma_prefetch_desc(&map_x);
@@ -274,9 +287,10 @@ __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_cons
         unsigned char* s = smem + stage * stage_bytes;
         // (experts beyond the padded ones: chunks outside are not fetched, and their rows of the result not stored)
         const int left = min(blocks * 2, g.padded / 64 - m0 * 2);
-        mbar_arrive_expect_tx(&full_bar[stage], (left + chunks) * kChunk);
-        for (int c = 0; c < left; ++c) tma_load_3d(s + c * kChunk, &map_dz, &full_bar[stage], (m0 * 2 + c) * 64, kb * kBK, 0);
-        for (int c = 0; c < chunks; ++c) tma_load_3d(s + (g.dw_blocks * 2 + c) * kChunk, &map_x, &full_bar[stage], n * kCols + c * 64, kb * kBK, 0);
+        mbar_arrive_expect_tx(&full_bar[stage], (g.layers * left + chunks) * kChunk);
+        for (int l = 0; l < g.layers; ++l)
+          for (int c = 0; c < left; ++c) tma_load_3d(s + (l * layer_chunks + c) * kChunk, &map_dz, &full_bar[stage], (m0 * 2 + c) * 64, kb * kBK, l);
+        for (int c = 0; c < chunks; ++c) tma_load_3d(s + (g.layers * layer_chunks + c) * kChunk, &map_x, &full_bar[stage], n * kCols + c * 64, kb * kBK, 0);
         if (++stage == g.dw_stages) { stage = 0; phase ^= 1; }
       }
     }
@@ -287,12 +301,13 @@ __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_cons
       if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, p.wait_budget_ns, p.status))) { ok = false; break; }
       tc_fence_after_sync();
       if (elect_one()) {
-        const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + g.dw_blocks * 2 * kChunk;
-        for (int m = 0; m < blocks; ++m)
+        const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + g.layers * layer_chunks * kChunk;
+        for (int l = 0; l < g.layers; ++l)
+          for (int m = 0; m < blocks; ++m)
 #pragma unroll
-          for (int j = 0; j < kBK / 16; ++j)
-            umma_bf16_ss<1>(tmem + m * kCols, umma_smem_desc(a + m * 2 * kChunk + j * 16 * 128, kChunk, 1024), umma_smem_desc(b + j * 16 * 128, kChunk, 1024), idesc,
-                            (kb > kb0 || j > 0) ? 1u : 0u);
+            for (int j = 0; j < kBK / 16; ++j)
+              umma_bf16_ss<1>(tmem + m * kCols, umma_smem_desc(a + (l * layer_chunks + m * 2) * kChunk + j * 16 * 128, kChunk, 1024),
+                              umma_smem_desc(b + j * 16 * 128, kChunk, 1024), idesc, (kb > kb0 || l > 0 || j > 0) ? 1u : 0u);
         umma_commit<1>(&empty_bar[stage]);
         if (kb == kb1 - 1) umma_commit<1>(&done_bar);
       }
@@ -380,6 +395,7 @@ cudaError_t launch(unsigned grid, int smem, cudaStream_t stream, const Args&... 
 RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
   RouteGradPlan g{};
   g.padded = (experts + 63) / 64 * 64;
+  g.layers = experts <= 128 ? 2 : 1;
   const int tiles = (tokens + kTokens - 1) / kTokens, n_tiles = (hidden + kCols - 1) / kCols;
   // dx: a block forms the gradient of its tokens' logits, so several for the same tokens only where there are few
   g.dx_splits = tiles > 0 ? sms / tiles : 1;
@@ -387,7 +403,7 @@ RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
   if (g.dx_splits < 1) g.dx_splits = 1;
   // (a fourth stage of W is worth more than a second tile of results a warp)
   g.dx_staging = g.padded <= 128 ? 2 : 1;
-  const int fixed = 1024 + g.padded * kTokens * 2 + kEpiWarps * g.dx_staging * kStaging;
+  const int fixed = 1024 + g.layers * g.padded * kTokens * 2 + kEpiWarps * g.dx_staging * kStaging;
   g.dx_stages = (kMostSmem - fixed) / (4 * kChunk);
   if (g.dx_stages > 4) g.dx_stages = 4;
   g.dx_smem = fixed + g.dx_stages * 4 * kChunk;
@@ -404,8 +420,8 @@ RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
     if (s == 1 || time < best_time) { best = s; best_time = time; }
   }
   g.dw_splits = best;
-  g.dw_stages = g.dw_blocks == 2 ? 3 : 4;
-  g.dw_smem = 1024 + g.dw_stages * (g.dw_blocks * 2 + 4) * kChunk;
+  g.dw_stages = 3;               // of 64 KB: two blocks, or two layers of one
+  g.dw_smem = 1024 + g.dw_stages * (g.layers * g.dw_blocks * 2 + 4) * kChunk;
   g.dw_units = units * best;
   return g;
 }

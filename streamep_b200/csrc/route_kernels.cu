@@ -21,9 +21,9 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kBK = 64;
-// The tensor cores cut off what an accumulator cannot hold instead of rounding, so it starts anew every 512 elements of the reduction and the
+// The tensor cores cut off what an accumulator cannot hold instead of rounding, so it starts anew every 256 elements of the reduction and the
 // segments are added up in registers: with one accumulator over 7168 elements the z loss came out 6e-6 too small, with segments 2e-7 off.
-constexpr int kSegment = 8;                      // k-blocks
+constexpr int kSegment = 4;                      // k-blocks
 constexpr int kDrainFirst = 4, kDrainers = 12;   // warps that take the segments' sums: three for each quarter of the accumulator's lanes
 constexpr int kMostChunks = 6;                   // of 16 columns, of up to 256, for one of the three
 constexpr int kMaxStages = 8, kMaxSplits = 8, kMostExperts = 512;
