@@ -51,6 +51,9 @@ __device__ __forceinline__ void gates_of(const Row<V>& gate, Row<V>& keep, Row<V
   for (int i = 0; i < V; ++i) e[i] = reciprocal(e[i]);
   take = Row<V>::of(e);
   keep = power * take;
+  // near 1 the difference is better by far: a relative error of `keep` that has one sign adds up over the rows that a state lasts
+#pragma unroll
+  for (int i = 0; i < V; ++i) keep.f[i] = take.f[i] < 0.5f ? 1.f - take.f[i] : keep.f[i];
 }
 // What a run of rows does to the state in front of it: h -> a h + b, or h -> b where a sequence starts within (a is then -0, and stays negative
 // in products: a state of the sequence before, infinite or NaN as it may be, is not multiplied with).
