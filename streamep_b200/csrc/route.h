@@ -46,7 +46,7 @@ struct RouteGradParams {
 // the tokens of a unit of dW.
 struct RouteGradPlan {
   int padded, layers;            // of dz: bf16 numbers that add up to it
-  int dx_splits, dx_stages, dx_staging, dx_smem;
+  int dx_pairs, dx_splits, dx_stages, dx_staging, dx_smem;
   int dw_blocks, dw_splits, dw_units, dw_stages, dw_smem;
 };
 RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms);

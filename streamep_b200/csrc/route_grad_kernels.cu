@@ -5,11 +5,12 @@
 //
 // For both products dz is rounded to bf16, 2^-9 of each term at most, as bf16 training code rounds the gradient of its logits: against 64 bits dx and dW are
 // 2.3e-3 off in 2-norm, where their own rounding is 1.7e-3.  Up to 128 experts, where twice the products cost nothing beside the reads of x and the writes of
-// dx, dz is kept to 16 bits as the sum of two bf16 numbers (XXX).  All sums are fp32.
+// dx, dz is kept to 16 bits as the sum of two bf16 numbers, and they are 1.7e-3 off.  All sums are fp32.
 // What bounds them: x is read and dx written once (HBM), and for many experts the tensor cores.  All operands lie in memory as TMA brings them in, dz as
 // [layers, T, experts rounded up to 64]; nothing is transposed.  Parts and sums have a fixed order: a repeated call gives the same bits.
 #include <atomic>
 #include <cuda.h>
+#include <type_traits>
 
 #include "ptx.cuh"
 #include "route.h"
@@ -24,6 +25,11 @@ constexpr int kTokens = 128, kCols = 256, kBK = 64;
 constexpr int kChunk = 64 * 128;                 // a box of 64 x 64 bf16
 constexpr int kStaging = 4096;
 constexpr int kMostSmem = 226 * 1024;
+constexpr int kMostStages = 8;
+
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -121,69 +127,81 @@ __device__ __forceinline__ void store_half_tile(uint32_t taddr, unsigned char* t
   if (lane == 0) { tma_store_3d(map, tile, x, y, 0); bulk_commit(); }
 }
 
-template <int EPL>
+// CG = 2: the blocks of a pair multiply their 256 tokens together, each with half of W's columns in its shared memory.  The three kernels of
+// 16384 tokens, hidden 7168 and 256 experts are bound by what the SMs read from L2 (8 TB/s): the whole of W for every 128 tokens took 92 to 97 us, for every 256 77 to 83.
+template <int EPL, int CG>
 __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_dx, const RouteGradParams p,
                                                                const RouteGradPlan g) {
   constexpr int kLayers = EPL <= 4 ? 2 : 1;      // g.layers
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full_bar[4], empty_bar[4], tmem_full[2], tmem_empty[2], dz_bar;
+  constexpr int kHalf = 4 / CG;                  // chunks of W in a stage
+  __shared__ uint64_t full_bar[kMostStages], empty_bar[kMostStages], tmem_full[2], tmem_empty[2], dz_bar;
   __shared__ uint32_t s_tmem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = static_cast<int>(blockIdx.x) / g.dx_splits, split = static_cast<int>(blockIdx.x) % g.dx_splits;
+  const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0, unit = static_cast<int>(blockIdx.x) / CG;
+  const int tile = unit / g.dx_splits * CG + rank, split = unit % g.dx_splits;
+  const bool leader = rank == 0;
   const int k_blocks = g.padded / kBK, n_tiles = p.dx != nullptr ? (p.hidden + kCols - 1) / kCols : 0;
   const int n0 = n_tiles * split / g.dx_splits, n1 = n_tiles * (split + 1) / g.dx_splits;
   unsigned char* dz = smem;                      // [layers][k_blocks][128 rows][128 bytes]
   const int layer_bytes = k_blocks * kTokens * 128;
   unsigned char* stages = dz + kLayers * layer_bytes;
-  unsigned char* staging = stages + g.dx_stages * 4 * kChunk;
+  unsigned char* staging = stages + g.dx_stages * kHalf * kChunk;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_w);
     for (int s = 0; s < g.dx_stages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&tmem_full[b], 1); mbar_init(&tmem_empty[b], kEpiWarps); }
-    mbar_init(&dz_bar, kEpiWarps);
+    for (int b = 0; b < 2; ++b) { mbar_init(&tmem_full[b], 1); mbar_init(&tmem_empty[b], kEpiWarps * CG); }
+    mbar_init(&dz_bar, kEpiWarps * CG);
     mbar_fence_init();
   }
-  if (warp == 1) { tmem_alloc<1>(&s_tmem, 512); tmem_relinquish<1>(); }
+  if (warp == 1) { tmem_alloc<CG>(&s_tmem, 512); tmem_relinquish<CG>(); }
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (CG == 2) cluster_sync(); else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s_tmem;
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0; uint32_t phase = 0; bool ok = true;
       for (int n = n0; n < n1 && ok; ++n) {
-        const int chunks = (min(kCols, p.hidden - n * kCols) + 63) / 64;
+        // (of a pair, each has half of the columns that are multiplied)
+        const int half = CG == 2 ? min(kCols, (p.hidden - n * kCols + 31) / 32 * 32) / 2 : min(kCols, p.hidden - n * kCols), chunks = (half + 63) / 64;
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, p.wait_budget_ns, p.status)) { ok = false; break; }
-          mbar_arrive_expect_tx(&full_bar[stage], chunks * kChunk);
-          for (int c = 0; c < chunks; ++c) tma_load_3d(stages + (stage * 4 + c) * kChunk, &map_w, &full_bar[stage], n * kCols + c * 64, kb * kBK, 0);
+          // (both blocks' bytes are counted on the first one's barrier, which that one arms for the sum)
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * chunks * kChunk);
+          for (int c = 0; c < chunks; ++c) {
+            unsigned char* to = stages + (stage * kHalf + c) * kChunk;
+            if constexpr (CG == 2) tma_load_3d_pair(to, &map_w, cluster_map(&full_bar[stage], 0), n * kCols + rank * half + c * 64, kb * kBK, 0);
+            else tma_load_3d(to, &map_w, &full_bar[stage], n * kCols + c * 64, kb * kBK, 0);
+          }
           if (++stage == g.dx_stages) { stage = 0; phase ^= 1; }
         }
       }
       if (!ok) give_up(p.status, 0, p.rank, tile);
     }
   } else if (warp == 1) {
-    bool ok = __all_sync(0xffffffffu, mbar_wait(&dz_bar, 0, p.wait_budget_ns, p.status));
+    if (leader) {
+    bool ok = __all_sync(0xffffffffu, mbar_wait<CG == 2>(&dz_bar, 0, p.wait_budget_ns, p.status));
     int stage = 0, acc = 0; uint32_t phase = 0, acc_phase = 0;
     for (int n = n0; n < n1 && ok; ++n) {
       const int cols = min(kCols, (p.hidden - n * kCols + 31) / 32 * 32);
-      const uint32_t idesc = umma_idesc_bf16(kTokens, 0, 0, 1) | (static_cast<uint32_t>(cols >> 3) << 17);
-      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[acc], acc_phase ^ 1, p.wait_budget_ns, p.status))) { ok = false; break; }
+      const uint32_t idesc = umma_idesc_bf16(kTokens * CG, 0, 0, 1) | (static_cast<uint32_t>(cols >> 3) << 17);
+      if (!__all_sync(0xffffffffu, mbar_wait<CG == 2>(&tmem_empty[acc], acc_phase ^ 1, p.wait_budget_ns, p.status))) { ok = false; break; }
       tc_fence_after_sync();
       for (int kb = 0; kb < k_blocks; ++kb) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, p.wait_budget_ns, p.status))) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait<CG == 2>(&full_bar[stage], phase, p.wait_budget_ns, p.status))) { ok = false; break; }
         tc_fence_after_sync();
         if (elect_one()) {
-          const uint32_t a = smem_u32(dz + kb * kTokens * 128), b = smem_u32(stages + stage * 4 * kChunk);
+          const uint32_t a = smem_u32(dz + kb * kTokens * 128), b = smem_u32(stages + stage * kHalf * kChunk);
 #pragma unroll
           for (int l = 0; l < kLayers; ++l)
 #pragma unroll
             for (int j = 0; j < kBK / 16; ++j)
-              umma_bf16_ss<1>(tmem + acc * kCols, umma_smem_desc(a + l * layer_bytes + j * 32, 16, 1024), umma_smem_desc(b + j * 16 * 128, kChunk, 1024), idesc,
+              umma_bf16_ss<CG>(tmem + acc * kCols, umma_smem_desc(a + l * layer_bytes + j * 32, 16, 1024), umma_smem_desc(b + j * 16 * 128, kChunk, 1024), idesc,
                               (kb > 0 || l > 0 || j > 0) ? 1u : 0u);
-          umma_commit<1>(&empty_bar[stage]);
-          if (kb == k_blocks - 1) umma_commit<1>(&tmem_full[acc]);
+          umma_commit<CG>(&empty_bar[stage]);
+          if (kb == k_blocks - 1) umma_commit<CG>(&tmem_full[acc]);
         }
         __syncwarp();
         if (++stage == g.dx_stages) { stage = 0; phase ^= 1; }
@@ -191,6 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_cons
       acc ^= 1; if (acc == 0) acc_phase ^= 1;
     }
     if (!ok && lane == 0) report_failure(p.status, kStatusTimeoutPipeline, kKernelRoute, 1, p.rank, tile, 0, 0);
+    }
   } else {
     const int w = warp - 2, quarter = warp & 3, side = w >> 2;
     const float share = p.load[p.experts], db = p.dbalance != nullptr ? *p.dbalance : 0.f, dzl = p.dz_loss != nullptr ? *p.dz_loss : 0.f;
@@ -220,7 +239,9 @@ __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_cons
     }
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&dz_bar);
+    if (lane == 0) {             // (the first block's tensor cores read this block's dz: a release that reaches it)
+      if constexpr (CG == 2) mbar_arrive_release_cluster(cluster_map(&dz_bar, 0)); else mbar_arrive(&dz_bar);
+    }
     int acc = 0, flip = 0; uint32_t acc_phase = 0;
     unsigned char* const mine = staging + w * g.dx_staging * kStaging;
     const int row0 = tile * kTokens + quarter * 32;
@@ -241,7 +262,9 @@ __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_cons
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+      if (lane == 0) {
+        if constexpr (CG == 2) mbar_arrive_cluster(cluster_map(&tmem_empty[acc], 0)); else mbar_arrive(&tmem_empty[acc]);
+      }
       acc ^= 1; if (acc == 0) acc_phase ^= 1;
     }
     if (lane == 0) bulk_wait_all();
@@ -249,7 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_cons
   __syncwarp();
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<1>(tmem, 512); }
+  if constexpr (CG == 2) cluster_sync();         // (the pair's operands, accumulators and barriers are no longer in use)
+  if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<CG>(tmem, 512); }
 }
 
 // A unit: `g.dw_blocks` blocks of 128 experts, 256 columns, a part of the tokens.
@@ -376,7 +400,7 @@ __global__ void __launch_bounds__(256) route_dw_join_kernel(const float* parts, 
 }
 
 template <auto kKernel, class... Args>
-cudaError_t launch(unsigned grid, int smem, cudaStream_t stream, const Args&... args) {
+cudaError_t launch(unsigned grid, int cluster, int smem, cudaStream_t stream, const Args&... args) {
   static std::atomic<bool> configured[64];       // the shared-memory limit is an attribute of the function on a device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -386,8 +410,17 @@ cudaError_t launch(unsigned grid, int smem, cudaStream_t stream, const Args&... 
     if ((e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)) != cudaSuccess) return e;
     configured[dev].store(true, std::memory_order_release);
   }
-  kKernel<<<grid, kThreads, smem, stream>>>(args...);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kKernel, args...);
 }
 
 }  // namespace
@@ -398,15 +431,19 @@ RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
   g.layers = experts <= 128 ? 2 : 1;
   const int tiles = (tokens + kTokens - 1) / kTokens, n_tiles = (hidden + kCols - 1) / kCols;
   // dx: a block forms the gradient of its tokens' logits, so several for the same tokens only where there are few
-  g.dx_splits = tiles > 0 ? sms / tiles : 1;
+  // (blocks in pairs cost 1.4 us and halve what is read of W: even at 48 MB of it, without and with pairs 20.9 and 21.8 us for 2048 tokens,
+  // hidden 4096 and 128 experts, 33.4 and 31.9 for 8192, 50.3 and 44.9 for 16384; at 64 experts the writes hide it: 48.2 and 49.5 for 32768, hidden 2048)
+  g.dx_pairs = g.padded > 64 && static_cast<long long>(tiles) * g.padded * hidden * 2 >= 48ll << 20 ? 1 : 0;
+  const int group = g.dx_pairs ? 2 : 1, groups = (tiles + group - 1) / group;
+  g.dx_splits = groups > 0 ? sms / group / groups : 1;
   if (g.dx_splits > n_tiles) g.dx_splits = n_tiles;
   if (g.dx_splits < 1) g.dx_splits = 1;
   // (a fourth stage of W is worth more than a second tile of results a warp)
   g.dx_staging = g.padded <= 128 ? 2 : 1;
-  const int fixed = 1024 + g.layers * g.padded * kTokens * 2 + kEpiWarps * g.dx_staging * kStaging;
-  g.dx_stages = (kMostSmem - fixed) / (4 * kChunk);
-  if (g.dx_stages > 4) g.dx_stages = 4;
-  g.dx_smem = fixed + g.dx_stages * 4 * kChunk;
+  const int fixed = 1024 + g.layers * g.padded * kTokens * 2 + kEpiWarps * g.dx_staging * kStaging, stage = 4 / group * kChunk;
+  g.dx_stages = (kMostSmem - fixed) / stage;
+  if (g.dx_stages > kMostStages) g.dx_stages = kMostStages;
+  g.dx_smem = fixed + g.dx_stages * stage;
   // dW: tokens are split to fill the GPU, into no shorter parts than 4 blocks of 64, and rather into whole rounds of all SMs
   const int blocks = (experts + 127) / 128;
   g.dw_blocks = blocks > 1 ? 2 : 1;
@@ -428,19 +465,25 @@ RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
 
 cudaError_t launch_route_dx(const RouteGradParams& p, const RouteGradPlan& g, const void* map_w, const void* map_dx, cudaStream_t stream) {
   const CUtensorMap &mw = *static_cast<const CUtensorMap*>(map_w), &mdx = *static_cast<const CUtensorMap*>(map_dx);
-  const unsigned grid = static_cast<unsigned>((p.tokens + kTokens - 1) / kTokens * (p.dx != nullptr ? g.dx_splits : 1));
   RouteGradPlan q = g;
   if (p.dx == nullptr) q.dx_splits = 1;
-  if (p.experts <= 32) return launch<route_dx_kernel<1>>(grid, g.dx_smem, stream, mw, mdx, p, q);
-  if (p.experts <= 64) return launch<route_dx_kernel<2>>(grid, g.dx_smem, stream, mw, mdx, p, q);
-  if (p.experts <= 128) return launch<route_dx_kernel<4>>(grid, g.dx_smem, stream, mw, mdx, p, q);
-  if (p.experts <= 256) return launch<route_dx_kernel<8>>(grid, g.dx_smem, stream, mw, mdx, p, q);
-  return launch<route_dx_kernel<16>>(grid, g.dx_smem, stream, mw, mdx, p, q);
+  const int group = g.dx_pairs ? 2 : 1, tiles = (p.tokens + kTokens - 1) / kTokens;
+  const unsigned grid = static_cast<unsigned>((tiles + group - 1) / group * group * q.dx_splits);
+  auto with = [&](auto experts) {
+    constexpr int EPL = decltype(experts)::value;
+    if constexpr (EPL >= 4) if (g.dx_pairs) return launch<route_dx_kernel<EPL, 2>>(grid, 2, g.dx_smem, stream, mw, mdx, p, q);
+    return launch<route_dx_kernel<EPL, 1>>(grid, 1, g.dx_smem, stream, mw, mdx, p, q);
+  };
+  if (p.experts <= 32) return with(std::integral_constant<int, 1>{});
+  if (p.experts <= 64) return with(std::integral_constant<int, 2>{});
+  if (p.experts <= 128) return with(std::integral_constant<int, 4>{});
+  if (p.experts <= 256) return with(std::integral_constant<int, 8>{});
+  return with(std::integral_constant<int, 16>{});
 }
 
 cudaError_t launch_route_dw(const RouteGradParams& p, const RouteGradPlan& g, const void* map_dz, const void* map_x, const void* map_out, float* parts, cudaStream_t stream) {
   const CUtensorMap &mz = *static_cast<const CUtensorMap*>(map_dz), &mx = *static_cast<const CUtensorMap*>(map_x), &mo = *static_cast<const CUtensorMap*>(map_out);
-  const cudaError_t e = launch<route_dw_kernel>(static_cast<unsigned>(g.dw_units), g.dw_smem, stream, mz, mx, mo, p, g);
+  const cudaError_t e = launch<route_dw_kernel>(static_cast<unsigned>(g.dw_units), 1, g.dw_smem, stream, mz, mx, mo, p, g);
   if (e != cudaSuccess || g.dw_splits == 1) return e;
   const long long elements = static_cast<long long>(p.experts) * p.hidden;
   cudaLaunchConfig_t cfg{};

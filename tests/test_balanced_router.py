@@ -133,6 +133,13 @@ def test_hidden(native, H):
 
 
 @gpu
+@pytest.mark.parametrize("T,H,E", [(3329, 7176, 100), (3457, 7160, 128), (3400, 4104, 200), (1537, 4128, 512), (2049, 8000, 257)])
+def test_many_weights(native, T, H, E):
+    """Products of which two blocks share the work: an odd count of blocks, tokens and columns that end inside."""
+    check(T, H, E, 4, masked=0.1, seed=E)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("which", range(1, 8))
 def test_subsets_of_upstream_gradients(native, which):
     for renormalize in (True, False):
