@@ -101,6 +101,12 @@ __device__ __forceinline__ bool within_one(const ScanShape& p, int before, int e
   return walk.at(p, before) >= 0 && walk.all_within(p, end);
 }
 
+// The same for all segments of a warp: one that looks at each row makes the others wait for it, so that then all do (7488 rows of 1000 fp32 channels in 9
+// sequences, forward and backward, 129 -> 103 us).
+template <class Seg> __device__ __forceinline__ bool all_plain(const ScanShape& p, const Seg& seg, int before, int end) {
+  return p.offsets == nullptr || __all_sync(0xffffffffu, !seg.there || within_one(p, before, end));
+}
+
 // A block's threads: LANES side by side across the channels, V channels each, and SEGS segments above one another.  Where runs are joined, PARTS
 // threads share a channel.  A thread's channels are one vector; or with kApart, where rows do not begin on boundaries of vectors, every 32nd: a warp then
 // reads and writes neighbouring numbers, and still has V of them for each row that it counts off (7488 rows of 1001 fp32 channels with gradients 131 us
@@ -252,12 +258,14 @@ __device__ __forceinline__ void walk_rows(const Segment<Tl, kBack>& seg, int fir
   }
 }
 
-// What the rows of a segment do to the state in front of them.  `rows`: x, or the rows' own gradients (which may be left out).
+// What the rows of a segment do to the state in front of them.  All threads call.  `rows`: x, or the rows' own gradients (which may be left out).
 template <class T, class Tl, bool kBack>
 __device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSplit& s, const Segment<Tl, kBack>& seg, const void* rows, long long rows_stride, const float* edge,
                                                Row<Tl::V>& a, Row<Tl::V>& b) {
   constexpr int V = Tl::V;
   a = Row<V>::all(1.f); b = Row<V>::all(0.f);
+  const bool plain = all_plain(p, seg, kBack ? seg.first : seg.first - 1, kBack ? seg.last + 1 : seg.last);
+  if (!seg.there) return;
   auto begin = [&](int sequence) {
     a = Row<V>::all(-0.f);
     b = edge != nullptr && sequence >= 0 ? Tl::load(edge + static_cast<long long>(sequence) * p.channels + seg.col, seg.count) : Row<V>::all(0.f);
@@ -272,7 +280,7 @@ __device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSpl
   const T* base[2] = {static_cast<const T*>(p.gate) + seg.col, static_cast<const T*>(none ? p.gate : rows) + seg.col};
   const long long stride[2] = {p.gate_stride, none ? p.gate_stride : rows_stride};
   const bool dense = p.offsets == nullptr;
-  if (dense || within_one(p, kBack ? seg.first : seg.first - 1, kBack ? seg.last + 1 : seg.last)) {
+  if (plain) {
     if (dense && seg.part == (kBack ? s.parts - 1 : 0)) begin(seg.sequence);
     walk_rows<T, Tl, kBack, 2>(seg, seg.first, base, stride, [&](int, Raw<T, V> (&row)[2]) { take_row(row); });
   } else {
@@ -331,8 +339,8 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_runs_kernel(const ScanSh
   grid_release();
   const int block = blockIdx.x / s.tiles, tile = blockIdx.x - block * s.tiles;
   const Segment<Tl, kBack> seg(p, s, block, tile);
-  Row<V> a = Row<V>::all(1.f), b = Row<V>::all(0.f);
-  if (seg.there) run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
+  Row<V> a, b;
+  run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
   Run before[V];
   runs_before<Tl>(a, b, before);
   if (!seg.there) return;
@@ -362,8 +370,8 @@ __device__ __forceinline__ Row<Tl::V> state_before(const ScanShape& p, const Sca
   constexpr int V = Tl::V;
   if (s.parts == 1) return Row<V>::all(0.f);
   if (s.within) {                                // no sequence goes on in another block
-    Row<V> a = Row<V>::all(1.f), b = Row<V>::all(0.f);
-    if (seg.there) run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
+    Row<V> a, b;
+    run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
     Run before[V];
     runs_before<Tl>(a, b, before);
     float f[V];
@@ -447,6 +455,7 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_forward_kernel(const Sca
   const int unit = gridDim.x - 1 - blockIdx.x, block = unit / s.tiles, tile = unit - block * s.tiles;
   const Segment<Tl, false> seg(p, s, block, tile);
   Row<V> h = state_before<T, Tl, false>(p, s, seg, block, tile, p.x, p.x_stride, p.initial);
+  const bool plain = all_plain(p, seg, seg.first - 1, seg.last + 1);
   if (!seg.there) return;
   auto state_at = [&](int sequence) { return static_cast<long long>(sequence) * p.channels + seg.col; };
   auto begin = [&](int sequence) { h = p.initial != nullptr ? Tl::load(p.initial + state_at(sequence), seg.count) : Row<V>::all(0.f); };
@@ -459,7 +468,7 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_forward_kernel(const Sca
   const long long stride[2] = {p.gate_stride, p.x_stride};
   T* out = static_cast<T*>(p.h) + seg.col;
   const bool dense = p.offsets == nullptr;
-  if (dense || within_one(p, seg.first - 1, seg.last + 1)) {
+  if (plain) {
     if (dense && seg.part == 0) begin(seg.sequence);
     walk_rows<T, Tl, false, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
       step(row);
@@ -494,6 +503,7 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
   const int unit = gridDim.x - 1 - blockIdx.x, block = unit / s.tiles, tile = unit - block * s.tiles;
   const Segment<Tl, true> seg(p, s, block, tile);
   Row<V> back = state_before<T, Tl, true>(p, s, seg, block, tile, p.dh, p.dh_stride, p.dfinal);     // keep_{t+1} g_{t+1}
+  const bool plain = all_plain(p, seg, seg.first - 1, seg.last + 1);
   if (!seg.there) return;
   auto state_at = [&](int sequence) { return static_cast<long long>(sequence) * p.channels + seg.col; };
   const bool none = p.dh == nullptr;
@@ -540,7 +550,7 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
     step(0, g.get(), d.get(), x.get(), h);
   };
   const bool dense = p.offsets == nullptr;
-  if (dense || within_one(p, seg.first - 1, seg.last + 1)) {
+  if (plain) {
     if (dense && seg.part == s.parts - 1) begin(seg.sequence);
     const int start = dense ? seg.sequence * p.length : -1;
     walk_rows<T, Tl, true, kArrays>(seg, first, base, stride, [&](int t, Raw<T, V> (&row)[kArrays]) {
