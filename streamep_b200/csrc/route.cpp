@@ -58,7 +58,8 @@ Route route_forward(const RouteCall& call, const at::Tensor& x, const at::Tensor
   RouteStatsParams s{};
   s.experts = static_cast<int>(E); s.top_k = call.top_k;
   s.mask = mask_of(mask);
-  s.blocks = route_blocks(p, ctx.sms);
+  const RouteTile tile = route_tile(p, ctx.sms);
+  s.blocks = tile.grid;
   r.kept = at::empty({Kept(nullptr, T, E, s.blocks).floats}, f32);
   const Kept kept(r.kept.data_ptr<float>(), T, E, s.blocks);
   p.probs = kept.probs; p.lse = kept.lse;
@@ -68,7 +69,7 @@ Route route_forward(const RouteCall& call, const at::Tensor& x, const at::Tensor
   CUtensorMap mw{}, mx{};
   if (T > 0) {
     mw = make_tmap(w.data_ptr(), H, E, 1, H, E * H, 64, 128);
-    mx = make_tmap(x.data_ptr(), H, T, 1, H, T * H, 64, router_tile(p, ctx.sms).tile_tokens);
+    mx = make_tmap(x.data_ptr(), H, T, 1, H, T * H, 64, tile.tile_tokens);
   }
   SEP_CUDA_CHECK(launch_route_forward(p, s, &mw, &mx, ctx.sms, ctx.status, ctx.wait_budget_ns, ctx.stream));
   return r;

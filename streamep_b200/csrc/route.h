@@ -11,7 +11,7 @@ namespace sep {
 struct RouteStatsParams {
   int experts, top_k;
   const unsigned char* mask;     // [tokens] or null: tokens that count
-  int blocks;                    // route_blocks()
+  int blocks;                    // RouteTile::grid (0 without tokens)
   float2* parts;                 // [blocks][experts] (sum of probabilities, bits of the count)
   float2* other_parts;           // [blocks] (sum of lse^2, bits of the number of tokens that count)
   float* balance;                // one number each
@@ -19,7 +19,11 @@ struct RouteStatsParams {
   long long* counts;             // [experts]
   float* load;                   // [experts + 1]: experts * counts / (top_k * n); behind them 1 / n (0 without any that count)
 };
-int route_blocks(const RouterParams& p, int sms);
+struct RouteTile : RouterTile {
+  int pairs;                     // 1: blocks multiply in pairs
+  int grid;
+};
+RouteTile route_tile(const RouterParams& p, int sms);
 // Maps as for the router (api.h); all outputs of `p`, probs and lse too.
 cudaError_t launch_route_forward(const RouterParams& p, const RouteStatsParams& s, const void* map_w, const void* map_x, int sms, StatusBlock* status, unsigned long long wait_budget_ns,
                                  cudaStream_t stream);

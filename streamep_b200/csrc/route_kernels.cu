@@ -8,6 +8,7 @@
 // up the blocks' sums, in one order (a repeated call gives the same bits).
 //
 // What bounds it: reading x once (HBM), for many experts the tensor cores too, and the finishing of tokens one by one in each warp.
+#include <algorithm>
 #include <atomic>
 #include <cuda.h>
 
@@ -104,9 +105,12 @@ __device__ __forceinline__ void finish_token(const RouterParams& p, const RouteS
 // A unit of `g.tile_tokens` tokens belongs to a cluster of `splits` blocks; each multiplies its share of the hidden dimension, W (experts, 128 per
 // accumulator) times the tokens (16 to 128 columns), and leaves its partial logits in shared memory; then every block of the cluster finishes its
 // share of the tokens, adding the partial sums over distributed shared memory.
-template <int EPL>
+// CG = 2: no splits; the blocks of a pair multiply their 2 x 128 tokens with 256 experts together, each with half of W in its shared memory, and each then has the logits of half
+// of the experts for the tokens of both, of which it hands the other's over.  What the SMs
+// read from L2 bounds long rows: x once and W for every 128 tokens, or 256 (16384 tokens, hidden 7168, 256 experts: 92.4 -> 78.5 us).
+template <int EPL, int CG>
 __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const RouterParams p,
-                                                                    const RouteStatsParams s, const RouterTile g, StatusBlock* status, unsigned long long budget) {
+                                                                    const RouteStatsParams s, const RouteTile g, StatusBlock* status, unsigned long long budget) {
   extern __shared__ unsigned char smem_dyn[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tmem_full[2], tmem_empty[2];
@@ -114,11 +118,14 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
   __shared__ int hist[kMostExperts];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = static_cast<int>(blockIdx.x) % g.splits, tile = static_cast<int>(blockIdx.x) / g.splits;
-  const int n = g.tile_tokens, nb = g.blocks, set = nb * n;
+  const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0;
+  const bool leader = rank == 0;
+  const int n = g.tile_tokens, nb = g.blocks, set = nb * n;    // (of a pair: one block of experts and twice the tokens)
+  const int own_blocks = nb / CG;                // of experts, in this block's shared memory
   const int k_blocks = (p.hidden + kBK - 1) / kBK;
   const int kb0 = k_blocks * split / g.splits, kb1 = k_blocks * (split + 1) / g.splits;
   const int segments = (kb1 - kb0 + kSegment - 1) / kSegment;
-  const int stage_bytes = nb * 128 * 128 + n * 128;
+  const int stage_bytes = own_blocks * 128 * 128 + n * 128;
   int tmem_cols = 32;
   while (tmem_cols < 2 * set) tmem_cols *= 2;
   grid_release();
@@ -126,13 +133,13 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
     tma_prefetch_desc(&map_w);
     tma_prefetch_desc(&map_x);
     for (int i = 0; i < g.stages; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&tmem_full[i], 1); mbar_init(&tmem_empty[i], kDrainers); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&tmem_full[i], 1); mbar_init(&tmem_empty[i], kDrainers * CG); }
     mbar_fence_init();
   }
-  if (warp == 1) { tmem_alloc<1>(&s_tmem, tmem_cols); tmem_relinquish<1>(); }
+  if (warp == 1) { tmem_alloc<CG>(&s_tmem, tmem_cols); tmem_relinquish<CG>(); }
   hist[threadIdx.x] = 0;
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (CG == 2) cluster_sync(); else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s_tmem;
   bool ok = true;
@@ -148,9 +155,16 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(&empty_bar[stage], phase ^ 1, budget, status)) { ok = false; break; }
         unsigned char* at = smem + stage * stage_bytes;
-        mbar_arrive_expect_tx(&full_bar[stage], stage_bytes);
-        for (int b = 0; b < nb; ++b) tma_load_3d(at + b * 128 * 128, &map_w, &full_bar[stage], kb * kBK, b * 128, 0);
-        tma_load_3d(at + nb * 128 * 128, &map_x, &full_bar[stage], kb * kBK, tile * n, 0);
+        if constexpr (CG == 2) {                 // (the bytes of both are counted on the first one's barrier)
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * stage_bytes);
+          const uint32_t bar = cluster_map(&full_bar[stage], 0);
+          tma_load_3d_pair(at, &map_w, bar, kb * kBK, rank * 128, 0);
+          tma_load_3d_pair(at + 128 * 128, &map_x, bar, kb * kBK, tile * n, 0);
+        } else {
+          mbar_arrive_expect_tx(&full_bar[stage], stage_bytes);
+          for (int b = 0; b < nb; ++b) tma_load_3d(at + b * 128 * 128, &map_w, &full_bar[stage], kb * kBK, b * 128, 0);
+          tma_load_3d(at + nb * 128 * 128, &map_x, &full_bar[stage], kb * kBK, tile * n, 0);
+        }
         if (++stage == g.stages) { stage = 0; phase ^= 1; }
       }
       if (!ok) {
@@ -159,25 +173,25 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
         while (globaltimer_ns() - t0 < 2000000ull) {}          // copies in flight land before the block leaves (bounded)
       }
     }
-  } else if (warp == 1) {
-    const uint32_t idesc = umma_idesc_bf16(128, 0, 0, 0) | (static_cast<uint32_t>(n >> 3) << 17);
+  } else if (warp == 1 && leader) {
+    const uint32_t idesc = umma_idesc_bf16(128 * CG, 0, 0, 0) | (static_cast<uint32_t>(n * CG >> 3) << 17);
     int stage = 0; uint32_t phase = 0;
     for (int q = 0; q < segments && ok; ++q) {
       const int first = kb0 + q * kSegment, last = min(first + kSegment, kb1);
-      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[q & 1], ((q >> 1) & 1) ^ 1, budget, status))) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_wait<CG == 2>(&tmem_empty[q & 1], ((q >> 1) & 1) ^ 1, budget, status))) { ok = false; break; }
       tc_fence_after_sync();
       for (int kb = first; kb < last; ++kb) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, budget, status))) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait<CG == 2>(&full_bar[stage], phase, budget, status))) { ok = false; break; }
         tc_fence_after_sync();
         if (elect_one()) {
-          const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + nb * 128 * 128;
-          for (int m = 0; m < nb; ++m)
+          const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + own_blocks * 128 * 128;
+          for (int m = 0; m < own_blocks; ++m)
 #pragma unroll
             for (int j = 0; j < kBK / 16; ++j)
-              umma_bf16_ss<1>(tmem + (q & 1) * set + m * n, umma_smem_desc(a + m * 128 * 128 + j * 32, 16, 1024), umma_smem_desc(b + j * 32, 16, 1024), idesc,
+              umma_bf16_ss<CG>(tmem + (q & 1) * set + m * n, umma_smem_desc(a + m * 128 * 128 + j * 32, 16, 1024), umma_smem_desc(b + j * 32, 16, 1024), idesc,
                               (kb > first || j > 0) ? 1u : 0u);
-          umma_commit<1>(&empty_bar[stage]);
-          if (kb == last - 1) umma_commit<1>(&tmem_full[q & 1]);
+          umma_commit<CG>(&empty_bar[stage]);
+          if (kb == last - 1) umma_commit<CG>(&tmem_full[q & 1]);
         }
         __syncwarp();
         if (++stage == g.stages) { stage = 0; phase ^= 1; }
@@ -185,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
     }
     if (!ok && lane == 0) report_failure(status, kStatusTimeoutPipeline, kKernelRoute, 7, 0, tile, split, 0);
   } else if (warp >= kDrainFirst) {
-    // accumulator lane = expert within its block of 128, column = token
+    // accumulator lane = expert within its block of 128, column = token (of a pair: of 256)
     for (int q = 0; q < segments; ++q) {
       if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[q & 1], (q >> 1) & 1, budget, status))) { ok = false; break; }
       tc_fence_after_sync();
@@ -201,7 +215,9 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tmem_empty[q & 1]);
+      if (lane == 0) {
+        if constexpr (CG == 2) mbar_arrive_cluster(cluster_map(&tmem_empty[q & 1], 0)); else mbar_arrive(&tmem_empty[q & 1]);
+      }
     }
     if (!ok && lane == 0) report_failure(status, kStatusTimeoutPipeline, kKernelRoute, 8, 0, tile, split, 0);
   }
@@ -215,12 +231,20 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
       const int c = third + i * 3;
       if (c >= chunks) break;
       const int block = c * 16 / n, token = c * 16 - block * n;
+      if constexpr (CG == 2) {                   // (the products, and with them the other's ring, are done: so said the last accumulator)
+        const uint32_t at = cluster_map(&logits[token * e_pad + rank * 128 + quarter * 32 + lane], block);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) logits[(token + k) * e_pad + block * 128 + quarter * 32 + lane] = acc[i][k];
+        for (int k = 0; k < 16; ++k) st_cluster(at + k * e_pad * 4, __float_as_int(acc[i][k]));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) logits[(token + k) * e_pad + block * 128 + quarter * 32 + lane] = acc[i][k];
+      }
     }
   }
+  tc_fence_before_sync();
   __syncthreads();
-  if (g.splits > 1) cluster_sync();
+  if (CG == 2 || g.splits > 1) cluster_sync();
+  if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<CG>(tmem, tmem_cols); }
   Sums<EPL> sums;
 #pragma unroll
   for (int j = 0; j < EPL; ++j) sums.probs[j] = 0.f;
@@ -267,7 +291,6 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
     for (int w = 0; w < kThreads / 32; ++w) { squares += others[w].x; live += __float_as_int(others[w].y); }
     s.other_parts[blockIdx.x] = make_float2(squares, __int_as_float(live));
   }
-  if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<1>(tmem, tmem_cols); }
 }
 
 // One block adds up the blocks' sums: `rows` threads for each expert.
@@ -320,10 +343,10 @@ __global__ void __launch_bounds__(kJoinThreads) route_join_kernel(const RouteSta
   p.load[E] = share;
 }
 
-template <int EPL>
-cudaError_t launch_width(const RouterParams& p, const RouteStatsParams& s, const RouterTile& g, const CUtensorMap& map_w, const CUtensorMap& map_x, StatusBlock* status,
+template <int EPL, int CG>
+cudaError_t launch_width(const RouterParams& p, const RouteStatsParams& s, const RouteTile& g, const CUtensorMap& map_w, const CUtensorMap& map_x, StatusBlock* status,
                          unsigned long long budget, cudaStream_t stream) {
-  auto kernel = route_forward_kernel<EPL>;
+  auto kernel = route_forward_kernel<EPL, CG>;
   static std::atomic<bool> configured[64];       // the shared-memory limit is an attribute of the function on a device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -341,7 +364,7 @@ cudaError_t launch_width(const RouterParams& p, const RouteStatsParams& s, const
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = g.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.x = g.splits * CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, p, s, g, status, budget);
@@ -349,23 +372,32 @@ cudaError_t launch_width(const RouterParams& p, const RouteStatsParams& s, const
 
 }  // namespace
 
-int route_blocks(const RouterParams& p, int sms) {
-  if (p.num_tokens == 0) return 0;
-  const RouterTile g = router_tile(p, sms);
-  return (p.num_tokens + g.tile_tokens - 1) / g.tile_tokens * g.splits;
+RouteTile route_tile(const RouterParams& p, int sms) {
+  RouteTile g{router_tile(p, sms), 0};
+  const int tiles = (p.num_tokens + g.tile_tokens - 1) / g.tile_tokens;
+  // (16384 tokens, 256 experts, without and with pairs: hidden 512 29.8 and 31.2 us, 2048 44.5 and 42.4, 4096 64.2 and 57.5)
+  g.pairs = g.blocks == 2 && g.splits == 1 && g.tile_tokens == 128 && p.hidden > 1024 ? 1 : 0;
+  if (g.pairs) {
+    const int stage = 2 * 128 * 128, logits = 128 * e_pad_of(p.num_experts) * 4;
+    g.stages = kMaxStages - 2;
+    g.smem_bytes = std::max(g.stages * stage, logits) + 1024;
+  }
+  g.grid = g.pairs ? (tiles + 1) / 2 * 2 : tiles * g.splits;
+  return g;
 }
 
 cudaError_t launch_route_forward(const RouterParams& p, const RouteStatsParams& s, const void* map_w, const void* map_x, int sms, StatusBlock* status, unsigned long long wait_budget_ns,
                                  cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   if (s.blocks > 0) {
-    const RouterTile g = router_tile(p, sms);
+    const RouteTile g = route_tile(p, sms);
     const CUtensorMap &mw = *static_cast<const CUtensorMap*>(map_w), &mx = *static_cast<const CUtensorMap*>(map_x);
-    if (p.num_experts <= 32) e = launch_width<1>(p, s, g, mw, mx, status, wait_budget_ns, stream);
-    else if (p.num_experts <= 64) e = launch_width<2>(p, s, g, mw, mx, status, wait_budget_ns, stream);
-    else if (p.num_experts <= 128) e = launch_width<4>(p, s, g, mw, mx, status, wait_budget_ns, stream);
-    else if (p.num_experts <= 256) e = launch_width<8>(p, s, g, mw, mx, status, wait_budget_ns, stream);
-    else e = launch_width<16>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    if (g.pairs) e = launch_width<8, 2>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    else if (p.num_experts <= 32) e = launch_width<1, 1>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    else if (p.num_experts <= 64) e = launch_width<2, 1>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    else if (p.num_experts <= 128) e = launch_width<4, 1>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    else if (p.num_experts <= 256) e = launch_width<8, 1>(p, s, g, mw, mx, status, wait_budget_ns, stream);
+    else e = launch_width<16, 1>(p, s, g, mw, mx, status, wait_budget_ns, stream);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg{};
