@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cuda.h>
+#include <type_traits>
 
 #include "api.h"
 #include "ptx.cuh"
@@ -39,67 +40,101 @@ __device__ __forceinline__ float warp_sum(float v) {
 // What a warp adds up over its tokens.
 template <int EPL> struct Sums { float probs[EPL], squares; int live; };
 
-// One warp finishes one token from its fp32 logits: softmax, the top_k by repeated arg-max (ties: lowest expert), weights, ranks, sums.
-template <int EPL, class Row>
-__device__ __forceinline__ void finish_token(const RouterParams& p, const RouteStatsParams& s, Row row, int t, int lane, int* hist, Sums<EPL>& sums) {
+// One warp finishes N tokens side by side (t[i]; those that `there` are) from their fp32 logits: softmax, the top_k by repeated arg-max (ties: lowest expert), weights,
+// ranks, sums.
+template <int EPL, int N, class Row>
+__device__ __forceinline__ void finish_tokens(const RouterParams& p, const RouteStatsParams& s, Row row, const int (&t)[N], const bool (&there)[N], int lane, int* hist, Sums<EPL>& sums) {
   const int E = p.num_experts, K = p.num_topk;
-  float v[EPL], top = -INFINITY;
+  float v[N][EPL], top[N], sum[N], inv[N];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = j * 32 + lane;
-    v[j] = e < E ? row(e) : -INFINITY;
-    top = fmaxf(top, v[j]);
+  for (int i = 0; i < N; ++i) {
+    top[i] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      const int e = j * 32 + lane;
+      v[i][j] = e < E ? (there[i] ? row(i, e) : 0.f) : -INFINITY;
+      top[i] = fmaxf(top[i], v[i][j]);
+    }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.f;
+  for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    v[j] = j * 32 + lane < E ? expf(v[j] - top) : 0.f;
-    sum += v[j];
-  }
-  sum = warp_sum(sum);
-  const float inv = 1.f / sum, lse = top + logf(sum);
-  const bool counts = s.mask == nullptr || s.mask[t] != 0;
-  unsigned key[EPL];             // probability bits + 1, which order like the values (0: taken, or no such expert)
+    for (int i = 0; i < N; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = j * 32 + lane;
-    const float prob = v[j] * inv;
-    if (e < E) p.probs[static_cast<size_t>(t) * E + e] = prob;
-    if (counts) sums.probs[j] += prob;
-    key[j] = e < E ? __float_as_uint(prob) + 1u : 0u;
+  for (int i = 0; i < N; ++i) {
+    sum[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      v[i][j] = j * 32 + lane < E ? expf(v[i][j] - top[i]) : 0.f;
+      sum[i] += v[i][j];
+    }
   }
-  if (counts) { sums.squares = fmaf(lse, lse, sums.squares); ++sums.live; }
-  if (lane == 0) p.lse[t] = lse;
-  float wsum = 0.f, my_w = 0.f;
-  int my_e = -1;
-  unsigned rank_mask = 0;
-  const int e_local = E / p.num_ranks;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+  bool counts[N];
+  unsigned key[N][EPL];          // probability bits + 1, which order like the values (0: taken, or no such expert)
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    inv[i] = 1.f / sum[i];
+    const float lse = top[i] + logf(sum[i]);
+    counts[i] = there[i] && (s.mask == nullptr || s.mask[t[i]] != 0);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      const int e = j * 32 + lane;
+      const float prob = v[i][j] * inv[i];
+      if (e < E && there[i]) p.probs[static_cast<size_t>(t[i]) * E + e] = prob;
+      if (counts[i]) sums.probs[j] += prob;
+      key[i][j] = e < E ? __float_as_uint(prob) + 1u : 0u;
+    }
+    if (counts[i]) { sums.squares = fmaf(lse, lse, sums.squares); ++sums.live; }
+    if (lane == 0 && there[i]) p.lse[t[i]] = lse;
+  }
+  float wsum[N], my_w[N];
+  int my_e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) { wsum[i] = my_w[i] = 0.f; my_e[i] = 0; }
   for (int k = 0; k < K; ++k) {
-    unsigned best = 0;
+    unsigned most[N];
+    int e[N];
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) best = max(best, key[j]);
-    const unsigned most = __reduce_max_sync(0xffffffffu, best);
-    unsigned mine = 0x7fffffffu;
+    for (int i = 0; i < N; ++i) {
+      unsigned best = 0;
 #pragma unroll
-    for (int j = EPL - 1; j >= 0; --j)
-      if (key[j] == most) mine = j * 32 + lane;
-    const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, mine));
+      for (int j = 0; j < EPL; ++j) best = max(best, key[i][j]);
+      most[i] = __reduce_max_sync(0xffffffffu, best);
+    }
 #pragma unroll
-    for (int j = 0; j < EPL; ++j)
-      if (j * 32 + lane == e) key[j] = 0;
-    const float w = __uint_as_float(most - 1u);
-    if (lane == k) { my_w = w; my_e = e; }
-    wsum += w;
-    rank_mask |= 1u << (e / e_local);
+    for (int i = 0; i < N; ++i) {
+      unsigned mine = 0x7fffffffu;
+#pragma unroll
+      for (int j = EPL - 1; j >= 0; --j)
+        if (key[i][j] == most[i]) mine = j * 32 + lane;
+      e[i] = static_cast<int>(__reduce_min_sync(0xffffffffu, mine));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j)
+        if (j * 32 + lane == e[i]) key[i][j] = 0;
+      const float w = __uint_as_float(most[i] - 1u);
+      if (lane == k) { my_w[i] = w; my_e[i] = e[i]; }
+      wsum[i] += w;
+    }
   }
-  if (lane < K) {
-    p.topk_idx[static_cast<size_t>(t) * K + lane] = my_e;
-    p.topk_weights[static_cast<size_t>(t) * K + lane] = p.renormalize ? my_w / wsum : my_w;
-    if (counts) atomicAdd(&hist[my_e], 1);       // (whole numbers: the order does not matter)
+  const int e_local = E / p.num_ranks;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const unsigned ranks = __reduce_or_sync(0xffffffffu, lane < K ? 1u << my_e[i] / e_local : 0u);
+    if (!there[i]) continue;
+    if (lane < K) {
+      p.topk_idx[static_cast<size_t>(t[i]) * K + lane] = my_e[i];
+      p.topk_weights[static_cast<size_t>(t[i]) * K + lane] = p.renormalize ? my_w[i] / wsum[i] : my_w[i];
+      if (counts[i]) atomicAdd(&hist[my_e[i]], 1);             // (whole numbers: the order does not matter)
+    }
+    if (lane < p.num_ranks) p.is_token_in_rank[static_cast<size_t>(t[i]) * p.num_ranks + lane] = (ranks >> lane) & 1u;
   }
-  if (lane < p.num_ranks) p.is_token_in_rank[static_cast<size_t>(t) * p.num_ranks + lane] = (rank_mask >> lane) & 1u;
 }
 
 // A unit of `g.tile_tokens` tokens belongs to a cluster of `splits` blocks; each multiplies its share of the hidden dimension, W (experts, 128 per
@@ -250,23 +285,36 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
   for (int j = 0; j < EPL; ++j) sums.probs[j] = 0.f;
   sums.squares = 0.f; sums.live = 0;
   if (ok) {
-    for (int tt = split + warp * g.splits; tt < n; tt += g.splits * (kThreads / 32)) {
-      const int t = tile * n + tt;
-      if (t >= p.num_tokens) break;
-      if (g.splits == 1) {
-        finish_token<EPL>(p, s, [&](int e) { return logits[tt * e_pad + e]; }, t, lane, hist, sums);
-      } else {
-        finish_token<EPL>(p, s, [&](int e) {
-          float v[kMaxSplits];
+    constexpr int kWarps = kThreads / 32;
+    auto finish = [&](auto at_once) {
+      constexpr int kAtOnce = decltype(at_once)::value;
+      for (int tt = split + warp * g.splits; tt < n && tile * n + tt < p.num_tokens; tt += g.splits * kWarps * kAtOnce) {
+        int at[kAtOnce], t[kAtOnce];
+        bool there[kAtOnce];
 #pragma unroll
-          for (int q = 0; q < kMaxSplits; ++q) v[q] = q < g.splits ? ld_cluster_f32(cluster_map(&logits[tt * e_pad + e], q)) : 0.f;
-          float sum = 0.f;
+        for (int i = 0; i < kAtOnce; ++i) {
+          at[i] = tt + i * g.splits * kWarps;
+          t[i] = tile * n + at[i];
+          there[i] = at[i] < n && t[i] < p.num_tokens;
+        }
+        if (g.splits == 1) {
+          finish_tokens<EPL, kAtOnce>(p, s, [&](int i, int e) { return logits[at[i] * e_pad + e]; }, t, there, lane, hist, sums);
+        } else {
+          finish_tokens<EPL, kAtOnce>(p, s, [&](int i, int e) {
+            float v[kMaxSplits];
 #pragma unroll
-          for (int q = 0; q < kMaxSplits; ++q) sum += v[q];
-          return sum;
-        }, t, lane, hist, sums);
+            for (int q = 0; q < kMaxSplits; ++q) v[q] = q < g.splits ? ld_cluster_f32(cluster_map(&logits[at[i] * e_pad + e], q)) : 0.f;
+            float sum = 0.f;
+#pragma unroll
+            for (int q = 0; q < kMaxSplits; ++q) sum += v[q];
+            return sum;
+          }, t, there, lane, hist, sums);
+        }
       }
-    }
+    };
+    // Two tokens at once hide each other's latency (16384 tokens, hidden 7168, 256 experts, top-8: 87.4 -> 82.4 us; four no less); a warp with one works for nobody (64 tokens, hidden
+    // 4096, 256 experts: 14.5 -> 15.7).
+    if (n > kWarps * g.splits) finish(std::integral_constant<int, 2>{}); else finish(std::integral_constant<int, 1>{});
   }
   if (g.splits > 1) cluster_sync();              // the peers have read this block's logits
   __syncthreads();
