@@ -51,7 +51,7 @@ struct RouteGradParams {
 struct RouteGradPlan {
   int padded, layers;            // of dz: bf16 numbers that add up to it
   int dx_pairs, dx_splits, dx_stages, dx_staging, dx_smem;
-  int dw_blocks, dw_splits, dw_units, dw_stages, dw_smem;
+  int dw_pairs, dw_blocks, dw_splits, dw_units, dw_stages, dw_smem;             // (units: as blocks of the grid)
 };
 RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms);
 // Maps: `map_w` [E, H] boxes of 64 x 64, `map_dx` [T, H] boxes of 32 rows x 64; `map_dz` [layers, T, padded] and `map_x` [T, H] boxes of 64 x 64; `map_out` dW boxes of

@@ -149,8 +149,8 @@ __device__ __forceinline__ void store_half_tile(uint32_t taddr, unsigned char* t
   if (lane == 0) { tma_store_3d(map, tile, x, y, 0); bulk_commit(); }
 }
 
-// CG = 2: the blocks of a pair multiply their 256 tokens together, each with half of W's columns in its shared memory.  The three kernels of
-// 16384 tokens, hidden 7168 and 256 experts are bound by what the SMs read from L2 (8 TB/s): the whole of W for every 128 tokens took 92 to 97 us, for every 256 77 to 83.
+// CG = 2: the blocks of a pair multiply their 256 tokens together, each with half of W's columns in its shared memory.  The kernels of
+// 16384 tokens, hidden 7168 and 256 experts are bound by what the SMs read from L2 (8 TB/s): with the whole of W for every 128 tokens this one took 82 us, for every 256 67.
 template <int EPL, int CG>
 __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_dx, const RouteGradParams p,
                                                                const RouteGradPlan g) {
@@ -307,7 +307,9 @@ __global__ void __launch_bounds__(kThreads, 1) route_dx_kernel(const __grid_cons
   if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<CG>(tmem, 512); }
 }
 
-// A unit: `g.dw_blocks` blocks of 128 experts, 256 columns, a part of the tokens.
+// A unit: `g.dw_blocks` blocks of 128 experts, 256 columns, a part of the tokens.  CG = 2: a pair of blocks, each with 128 experts, and 512 columns, of which each has half in its
+// shared memory; dz is then read half as often (16384 tokens, hidden 7168, 256 experts 61.4 -> 56.7 us).
+template <int CG>
 __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_constant__ CUtensorMap map_dz, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out,
                                                                const RouteGradParams p, const RouteGradPlan g) {
   extern __shared__ unsigned char smem_dyn[];
@@ -315,13 +317,20 @@ __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_cons
   __shared__ uint64_t full_bar[4], empty_bar[4], done_bar;
   __shared__ uint32_t s_tmem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_tiles = (p.hidden + kCols - 1) / kCols;
-  const int n = static_cast<int>(blockIdx.x) % n_tiles, rest = static_cast<int>(blockIdx.x) / n_tiles, split = rest % g.dw_splits, group = rest / g.dw_splits;
-  const int all_blocks = (p.experts + 127) / 128, m0 = group * g.dw_blocks, blocks = min(g.dw_blocks, all_blocks - m0);
+  constexpr int kUnit = kCols * CG;
+  const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0, unit = static_cast<int>(blockIdx.x) / CG;
+  const bool leader = rank == 0;
+  const int n_tiles = (p.hidden + kUnit - 1) / kUnit;
+  const int n = unit % n_tiles, rest = unit / n_tiles, split = rest % g.dw_splits, group = rest / g.dw_splits;
+  // this block's experts: m0, ... in blocks of 128
+  const int all_blocks = (p.experts + 127) / 128, m0 = group * g.dw_blocks + rank, blocks = CG == 2 ? 1 : min(g.dw_blocks, all_blocks - m0);
   const int k_blocks = (p.tokens + kBK - 1) / kBK, kb0 = static_cast<int>(static_cast<long long>(k_blocks) * split / g.dw_splits),
             kb1 = static_cast<int>(static_cast<long long>(k_blocks) * (split + 1) / g.dw_splits);
-  const int chunks = (min(kCols, p.hidden - n * kCols) + 63) / 64, cols = min(kCols, (p.hidden - n * kCols + 31) / 32 * 32);
-  const int layer_chunks = g.dw_blocks * 2, stage_bytes = (g.layers * layer_chunks + 4) * kChunk, tmem_cols = g.dw_blocks * kCols;
+  // of the h-th 256 columns: those that are multiplied, and the 64-wide pieces of them in this block's shared memory
+  auto cols_of = [&](int h) { return max(0, min(kCols, (p.hidden - n * kUnit - h * kCols + 31) / 32 * 32)); };
+  auto chunks_of = [&](int h) { return CG == 2 ? (cols_of(h) / 2 + 63) / 64 : (min(kCols, p.hidden - n * kUnit) + 63) / 64; };
+  auto experts_of = [&](int block) { return max(0, min((CG == 2 ? 1 : blocks) * 2, g.padded / 64 - block * 2)); };      // (chunks)
+  const int layer_chunks = g.dw_blocks * 2 / CG, stage_bytes = (g.layers * layer_chunks + 4) * kChunk, tmem_cols = g.dw_blocks * kCols;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_dz);
     tma_prefetch_desc(&map_x);
@@ -329,9 +338,9 @@ __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_cons
     mbar_init(&done_bar, 1);
     mbar_fence_init();
   }
-  if (warp == 1) { tmem_alloc<1>(&s_tmem, tmem_cols); tmem_relinquish<1>(); }
+  if (warp == 1) { tmem_alloc<CG>(&s_tmem, tmem_cols); tmem_relinquish<CG>(); }
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (CG == 2) cluster_sync(); else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s_tmem;
   if (warp == 0) {
@@ -341,35 +350,51 @@ __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_cons
         if (!mbar_wait(&empty_bar[stage], phase ^ 1, p.wait_budget_ns, p.status)) { give_up(p.status, 3, p.rank, static_cast<int>(blockIdx.x)); break; }
         unsigned char* s = smem + stage * stage_bytes;
         // (experts beyond the padded ones: chunks outside are not fetched, and their rows of the result not stored)
-        const int left = min(blocks * 2, g.padded / 64 - m0 * 2);
-        mbar_arrive_expect_tx(&full_bar[stage], (g.layers * left + chunks) * kChunk);
-        for (int l = 0; l < g.layers; ++l)
-          for (int c = 0; c < left; ++c) tma_load_3d(s + (l * layer_chunks + c) * kChunk, &map_dz, &full_bar[stage], (m0 * 2 + c) * 64, kb * kBK, l);
-        for (int c = 0; c < chunks; ++c) tma_load_3d(s + (g.layers * layer_chunks + c) * kChunk, &map_x, &full_bar[stage], n * kCols + c * 64, kb * kBK, 0);
+        const int left = experts_of(m0);
+        if constexpr (CG == 2) {                 // (the bytes of both are counted on the first one's barrier)
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], (left + experts_of(m0 + 1) + 2 * (chunks_of(0) + chunks_of(1))) * kChunk);
+          const uint32_t bar = cluster_map(&full_bar[stage], 0);
+          for (int c = 0; c < left; ++c) tma_load_3d_pair(s + c * kChunk, &map_dz, bar, (m0 * 2 + c) * 64, kb * kBK, 0);
+          for (int h = 0; h < 2; ++h)
+            for (int c = 0; c < chunks_of(h); ++c)
+              tma_load_3d_pair(s + (2 + h * 2 + c) * kChunk, &map_x, bar, n * kUnit + h * kCols + rank * (cols_of(h) / 2) + c * 64, kb * kBK, 0);
+        } else {
+          const int chunks = chunks_of(0);
+          mbar_arrive_expect_tx(&full_bar[stage], (g.layers * left + chunks) * kChunk);
+          for (int l = 0; l < g.layers; ++l)
+            for (int c = 0; c < left; ++c) tma_load_3d(s + (l * layer_chunks + c) * kChunk, &map_dz, &full_bar[stage], (m0 * 2 + c) * 64, kb * kBK, l);
+          for (int c = 0; c < chunks; ++c) tma_load_3d(s + (g.layers * layer_chunks + c) * kChunk, &map_x, &full_bar[stage], n * kCols + c * 64, kb * kBK, 0);
+        }
         if (++stage == g.dw_stages) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
-    const uint32_t idesc = umma_idesc_bf16(128, 0, 1, 1) | (static_cast<uint32_t>(cols >> 3) << 17);
+    if (leader) {
+    const uint32_t idesc = umma_idesc_bf16(128 * CG, 0, 1, 1);
     int stage = 0; uint32_t phase = 0; bool ok = true;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, p.wait_budget_ns, p.status))) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_wait<CG == 2>(&full_bar[stage], phase, p.wait_budget_ns, p.status))) { ok = false; break; }
       tc_fence_after_sync();
       if (elect_one()) {
         const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + g.layers * layer_chunks * kChunk;
         for (int l = 0; l < g.layers; ++l)
-          for (int m = 0; m < blocks; ++m)
+          for (int m = 0; m < (CG == 2 ? 2 : blocks); ++m) {           // accumulators: of experts, or of a pair's columns
+            const int cols = cols_of(CG == 2 ? m : 0);
+            if (cols == 0) break;
+            const uint32_t am = a + (l * layer_chunks + (CG == 2 ? 0 : m * 2)) * kChunk, bm = b + (CG == 2 ? m * 2 : 0) * kChunk;
 #pragma unroll
             for (int j = 0; j < kBK / 16; ++j)
-              umma_bf16_ss<1>(tmem + m * kCols, umma_smem_desc(a + (l * layer_chunks + m * 2) * kChunk + j * 16 * 128, kChunk, 1024),
-                              umma_smem_desc(b + j * 16 * 128, kChunk, 1024), idesc, (kb > kb0 || l > 0 || j > 0) ? 1u : 0u);
-        umma_commit<1>(&empty_bar[stage]);
-        if (kb == kb1 - 1) umma_commit<1>(&done_bar);
+              umma_bf16_ss<CG>(tmem + m * kCols, umma_smem_desc(am + j * 16 * 128, kChunk, 1024), umma_smem_desc(bm + j * 16 * 128, kChunk, 1024),
+                               idesc | (static_cast<uint32_t>(cols >> 3) << 17), (kb > kb0 || l > 0 || j > 0) ? 1u : 0u);
+          }
+        umma_commit<CG>(&empty_bar[stage]);
+        if (kb == kb1 - 1) umma_commit<CG>(&done_bar);
       }
       __syncwarp();
       if (++stage == g.dw_stages) { stage = 0; phase ^= 1; }
     }
     if (!ok && lane == 0) report_failure(p.status, kStatusTimeoutPipeline, kKernelRoute, 4, p.rank, static_cast<int>(blockIdx.x), 0, 0);
+    }
   } else {
     // (the operands' place is free once the products are done)
     const bool have = kb1 > kb0;
@@ -380,18 +405,18 @@ __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_cons
       const int w = warp - 2, quarter = warp & 3, side = w >> 2;
       unsigned char* const mine = smem + w * 2 * kStaging;
       int flip = 0;
-      for (int m = 0; m < blocks; ++m) {
-        const int row0 = (m0 + m) * 128 + quarter * 32;
+      for (int m = 0; m < (CG == 2 ? 2 : blocks); ++m) {
+        const int row0 = (CG == 2 ? m0 : m0 + m) * 128 + quarter * 32, col0 = n * kUnit + (CG == 2 ? m * kCols : 0);
         if (row0 >= p.experts) continue;
         const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + m * kCols;
         for (int c = side * 128; c < side * 128 + 128; c += g.dw_splits > 1 ? 32 : 64) {
-          if (n * kCols + c >= p.hidden) break;
+          if (col0 + c >= p.hidden) break;
           if (lane == 0) bulk_wait_read_but_one();
           __syncwarp();
           unsigned char* tile = mine + flip * kStaging;
           flip ^= 1;
           if (g.dw_splits == 1) {
-            store_half_tile(taddr + c, tile, &map_out, n * kCols + c, row0, lane);
+            store_half_tile(taddr + c, tile, &map_out, col0 + c, row0, lane);
             continue;
           }
           uint32_t r[32];
@@ -402,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_cons
           for (int q = 0; q < 8; ++q) st_shared_v4(stg + stage_off<128>(lane, q), r[q * 4], r[q * 4 + 1], r[q * 4 + 2], r[q * 4 + 3]);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) { tma_store_3d(&map_out, tile, n * kCols + c, row0, split); bulk_commit(); }
+          if (lane == 0) { tma_store_3d(&map_out, tile, col0 + c, row0, split); bulk_commit(); }
         }
       }
       if (lane == 0) bulk_wait_all();
@@ -411,7 +436,8 @@ __global__ void __launch_bounds__(kThreads, 1) route_dw_kernel(const __grid_cons
   __syncwarp();
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<1>(tmem, tmem_cols); }
+  if constexpr (CG == 2) cluster_sync();         // (the pair's operands, accumulators and barriers are no longer in use)
+  if (warp == 1) { tc_fence_after_sync(); tmem_dealloc<CG>(tmem, tmem_cols); }
 }
 
 // The sum of the parts of dW, 8 elements a thread.
@@ -462,8 +488,8 @@ RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
   g.layers = experts <= 128 ? 2 : 1;
   const int tiles = (tokens + kTokens - 1) / kTokens, n_tiles = (hidden + kCols - 1) / kCols;
   // dx: a block forms the gradient of its tokens' logits, so several for the same tokens only where there are few
-  // (blocks in pairs cost 1.4 us and halve what is read of W: even at 48 MB of it, without and with pairs 20.9 and 21.8 us for 2048 tokens,
-  // hidden 4096 and 128 experts, 33.4 and 31.9 for 8192, 50.3 and 44.9 for 16384; at 64 experts the writes hide it: 48.2 and 49.5 for 32768, hidden 2048)
+  // (blocks in pairs cost 1.4 us and halve what is read of W: even at 48 MB of it, without and with pairs 15.0 and 16.0 us for 2048 tokens,
+  // hidden 4096 and 128 experts, 27.5 and 26.0 for 8192, 43.8 and 38.8 for 16384; at 64 experts the writes hide it: 1 us lost up to 32768 tokens, hidden 2048)
   g.dx_pairs = g.padded > 64 && static_cast<long long>(tiles) * g.padded * hidden * 2 >= 48ll << 20 ? 1 : 0;
   const int group = g.dx_pairs ? 2 : 1, groups = (tiles + group - 1) / group;
   g.dx_splits = groups > 0 ? sms / group / groups : 1;
@@ -478,19 +504,24 @@ RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
   // dW: tokens are split to fill the GPU, into no shorter parts than 4 blocks of 64, and rather into whole rounds of all SMs
   const int blocks = (experts + 127) / 128;
   g.dw_blocks = blocks > 1 ? 2 : 1;
-  const int units = (blocks + g.dw_blocks - 1) / g.dw_blocks * n_tiles, most = (tokens + 4 * kBK - 1) / (4 * kBK);
+  const int groups_of_experts = (blocks + g.dw_blocks - 1) / g.dw_blocks;
+  // (256 experts, without and with pairs: 1000 tokens of hidden 7168 12.2 and 12.8 us, 4096 23.5 and 22.3, 32768 of hidden 1000 27.8 and 29.4, of 2048 41.4 and 40.1)
+  g.dw_pairs = g.dw_blocks == 2 && hidden >= 2048 && static_cast<long long>(tokens) * hidden * groups_of_experts >= 1 << 24 ? 1 : 0;
+  const int of = g.dw_pairs ? 2 : 1, unit_cols = kCols * of;
+  const int units = groups_of_experts * ((hidden + unit_cols - 1) / unit_cols), most = (tokens + 4 * kBK - 1) / (4 * kBK);
   int best = 1;
   double best_time = 0.0;
   for (int s = 1; s <= most && s <= 64; ++s) {
-    const int rounds = (units * s + sms - 1) / sms;
+    const int rounds = (units * s + sms / of - 1) / (sms / of);
     // a round's blocks of tokens, and what an output tile costs: about as much as 6 blocks
     const double time = rounds * (static_cast<double>((tokens + kBK - 1) / kBK) / s + 6.0);
     if (s == 1 || time < best_time) { best = s; best_time = time; }
   }
   g.dw_splits = best;
-  g.dw_stages = 3;               // of 64 KB: two blocks, or two layers of one
-  g.dw_smem = 1024 + g.dw_stages * (g.layers * g.dw_blocks * 2 + 4) * kChunk;
-  g.dw_units = units * best;
+  // stages of 64 KB: two blocks, or two layers of one; of a pair of 48
+  g.dw_stages = g.dw_pairs ? 4 : 3;
+  g.dw_smem = 1024 + g.dw_stages * (g.layers * g.dw_blocks * 2 / of + 4) * kChunk;
+  g.dw_units = units * best * of;
   return g;
 }
 
@@ -513,7 +544,8 @@ cudaError_t launch_route_dx(const RouteGradParams& p, const RouteGradPlan& g, co
 
 cudaError_t launch_route_dw(const RouteGradParams& p, const RouteGradPlan& g, const void* map_dz, const void* map_x, const void* map_out, float* parts, cudaStream_t stream) {
   const CUtensorMap &mz = *static_cast<const CUtensorMap*>(map_dz), &mx = *static_cast<const CUtensorMap*>(map_x), &mo = *static_cast<const CUtensorMap*>(map_out);
-  const cudaError_t e = launch<route_dw_kernel>(static_cast<unsigned>(g.dw_units), 1, g.dw_smem, stream, mz, mx, mo, p, g);
+  const cudaError_t e = g.dw_pairs ? launch<route_dw_kernel<2>>(static_cast<unsigned>(g.dw_units), 2, g.dw_smem, stream, mz, mx, mo, p, g)
+                                   : launch<route_dw_kernel<1>>(static_cast<unsigned>(g.dw_units), 1, g.dw_smem, stream, mz, mx, mo, p, g);
   if (e != cudaSuccess || g.dw_splits == 1) return e;
   const long long elements = static_cast<long long>(p.experts) * p.hidden;
   cudaLaunchConfig_t cfg{};

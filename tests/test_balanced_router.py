@@ -134,7 +134,7 @@ def test_hidden(native, H):
 
 @gpu
 @pytest.mark.parametrize("T,H,E", [(3329, 7176, 100), (3457, 7160, 128), (3400, 4104, 200), (1537, 4128, 512), (2049, 8000, 257), (9473, 1032, 256),
-                                   (9729, 1304, 130), (19000, 1096, 160), (9500, 1024, 200)])
+                                   (9729, 1304, 130), (19000, 1096, 160), (9500, 1024, 200), (2400, 7176, 200), (4100, 4360, 512), (8200, 2056, 129)])
 def test_many_weights(native, T, H, E):
     """Products of which two blocks share the work: an odd count of blocks, tokens and columns that end inside."""
     check(T, H, E, 4, masked=0.1, seed=E)
