@@ -65,16 +65,20 @@ class MoELM(nn.Module):
 
     def hidden_states(self, tokens: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
         x = torch.nn.functional.embedding(tokens.reshape(-1), self.embedding)
+        counts = None            # (rows of a packed batch that belong to no sequence are padding, and none of the gates' business)
+        if offsets is not None and self.train_router and torch.is_grad_enabled():
+            row = torch.arange(x.shape[0], device=x.device)
+            counts = (row >= offsets[0]) & (row < offsets[-1])
         if not self.mixers:
             for layer in self.layers:
-                x = x + layer(torch.nn.functional.rms_norm(x, x.shape[-1:]))
+                x = x + layer(torch.nn.functional.rms_norm(x, x.shape[-1:]), counts)
             return torch.nn.functional.rms_norm(x, x.shape[-1:])
         shape = x.shape if offsets is not None else (*tokens.shape, self.hidden)
         mix = lambda i, values, gates: gated_scan(values.view(shape), gates.view(shape), offsets=offsets, buffer=self.buffer).view(x.shape)
-        return self._blocks(x, mix)
+        return self._blocks(x, mix, counts)
 
-    def _blocks(self, x: torch.Tensor, mix) -> torch.Tensor:
-        """The layers with their mixers; ``mix(i, values, gates)`` is what runs along the sequences."""
+    def _blocks(self, x: torch.Tensor, mix, counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The layers with their mixers; ``mix(i, values, gates)`` is what runs along the sequences, ``counts`` the tokens that the gates' losses take."""
         added = None
         for i, (mixer, layer) in enumerate(zip(self.mixers, self.layers)):
             if added is None:
@@ -83,7 +87,7 @@ class MoELM(nn.Module):
                 y, x = layer_norm(added, mixer.norm_weight, mixer.norm_bias, residual=x)
             mixed = torch.nn.functional.linear(mix(i, *mixer.values_and_gates(y)), mixer.w_out)
             y, x = layer_norm(mixed, mixer.expert_norm_weight, mixer.expert_norm_bias, residual=x)
-            added = layer(y)
+            added = layer(y, counts)
         return layer_norm(added, residual=x)[0]
 
     def router_losses(self) -> torch.Tensor:

@@ -127,6 +127,24 @@ def test_packed_is_dense(native):
     buf.check_status()
 
 
+def test_padding_of_a_packed_batch_is_not_counted(native):
+    """Rows in front of the first sequence and behind the last one: counts are whole numbers, the losses those of the batch without them but for
+    activations that the recurrence rounds elsewhere (2^-8 of values of size one, a few times over)."""
+    model, buf = build()
+    tokens, targets = batch(1, 150)
+    tokens, targets = tokens.reshape(-1), targets.reshape(-1)
+    model(tokens, targets, offsets=torch.tensor([0, 60, 150], device=DEV))
+    routes = [layer.last_route for layer in model.layers]
+    pad = lambda t, n, m, fill: torch.cat([t.new_full((n,), fill), t, t.new_full((m,), fill)])
+    model(pad(tokens, 7, 43, 3), pad(targets, 7, 43, -100), offsets=torch.tensor([7, 67, 157], device=DEV))
+    for layer, want in zip(model.layers, routes):
+        got = layer.last_route
+        assert int(got.expert_counts.sum()) == 150 * layer.top_k
+        torch.testing.assert_close(got.z_loss, want.z_loss, rtol=0.02, atol=0.0)
+        torch.testing.assert_close(got.balance_loss, want.balance_loss, rtol=0.02, atol=0.0)
+    buf.check_status()
+
+
 def test_decoding_continues(native):
     model, buf = build()
     tokens, _ = batch(3, 40)
