@@ -3,10 +3,10 @@
 //   dx = dz W  [T, H]      a block takes 128 tokens: their dz is formed in shared memory, where it stays as the left operand, and W's columns go by
 //   dW = dz^T x  [E, H]    a block takes up to 256 experts, 256 columns and a part of the tokens; the parts are added up by a small kernel
 //
-// For both products dz is rounded to bf16, 2^-9 of each term at most, as bf16 training code rounds the gradient of its logits: against 64 bits dx and dW are
+// For both products dz is rounded to bf16, 2^-8 of each term at most, as bf16 training code rounds the gradient of its logits: against 64 bits dx and dW are
 // 2.3e-3 off in 2-norm, where their own rounding is 1.7e-3.  Up to 128 experts, where twice the products cost nothing beside the reads of x and the writes of
 // dx, dz is kept to 16 bits as the sum of two bf16 numbers, and they are 1.7e-3 off.  All sums are fp32.
-// What bounds them: x is read and dx written once (HBM), and for many experts the tensor cores.  All operands lie in memory as TMA brings them in, dz as
+// What bounds them: x is read and dx written once (HBM), for many experts what the SMs read from L2; and for short calls the forming of dz.  All operands lie in memory as TMA brings them in, dz as
 // [layers, T, experts rounded up to 64]; nothing is transposed.  Parts and sums have a fixed order: a repeated call gives the same bits.
 #include <atomic>
 #include <cuda.h>

@@ -7,7 +7,7 @@
 // One kernel multiplies, chooses, leaves p and the logsumexp for the backward and adds up its tokens' probabilities, counts and squares; a small one adds
 // up the blocks' sums, in one order (a repeated call gives the same bits).
 //
-// What bounds it: reading x once (HBM), for many experts the tensor cores too, and the finishing of tokens one by one in each warp.
+// What bounds it: reading x once (HBM), for many experts what the SMs read from L2, and the choice (16384 tokens of 256 experts: 1.1 us for each one chosen).
 #include <algorithm>
 #include <atomic>
 #include <cuda.h>
