@@ -33,7 +33,8 @@ def balanced_router(x: torch.Tensor, w_gate: torch.Tensor, top_k: int, num_ranks
         z_loss = mean_t logsumexp(x @ w_gate.T)[t] ** 2
 
     ``mask [T]`` (bool): tokens that count; the others (padding) are routed all the same, but are left out of counts, means and
-    ``n`` (both losses are 0 without any that counts).  Every rank's losses are those of its own tokens.
+    ``n`` (both losses are 0 without any that counts).  Whatever they hold, losses and the losses' gradient of ``x`` are the same; but the gradient of
+    ``w_gate`` multiplies their ``x`` with zero, which an infinity or NaN survives.  Every rank's losses are those of its own tokens.
 
     The choice itself and the counts have no gradient; weights and losses do, for ``x`` and ``w_gate`` (bf16), by ``dz @ w_gate`` and
     ``dz.T @ x`` with the gradient ``dz`` of the logits and all sums in 32 bits.  There is no second derivative.  A repeated call

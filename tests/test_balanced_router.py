@@ -236,10 +236,30 @@ def test_against_differences(native):
 
 
 @gpu
-def test_repeats_streams_and_graphs(native):
-    x, w = inputs(3000, 512, 64, 9)
+def test_gradients_of_losses_where_padding_holds_anything(native):
+    """At sizes whose products are shared by blocks, and below."""
+    for T, H, E in ((700, 128, 64), (9601, 2056, 200)):
+        x, w = inputs(T, H, E, 5)
+        mask = torch.ones(T, dtype=torch.bool, device=DEV)
+        mask[T // 2 + 50:T // 2 + 150] = False
+        bad = x.clone()
+        bad[T // 2 + 50:T // 2 + 100] = float("nan")
+        bad[T // 2 + 100:T // 2 + 150] = float("inf")
+        grads = []
+        for rows in (x, bad):
+            xl, wl = rows.clone().requires_grad_(True), w.clone().requires_grad_(True)
+            r = balanced_router(xl, wl, 4, mask=mask)
+            grads.append(torch.autograd.grad([r.balance_loss, r.z_loss], [xl, wl], [torch.tensor(3.0 * T, device=DEV)] * 2))
+        # (a row of x that is infinite or NaN times a gradient of zero is NaN, for the experts of dW that it meets: only dx is the same)
+        assert torch.equal(grads[0][0], grads[1][0]) and bool((grads[0][0][~mask] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("T,H,E", [(3000, 512, 64), (9601, 2056, 200)])
+def test_repeats_streams_and_graphs(native, T, H, E):
+    x, w = inputs(T, H, E, 9)
     xl, wl = x.requires_grad_(True), w.requires_grad_(True)
-    up = torch.randn(3000, 6, device=DEV)
+    up = torch.randn(T, 6, device=DEV)
 
     def run():
         r = balanced_router(xl, wl, 6, 8)

@@ -367,6 +367,21 @@ def test_repeats_streams_and_graphs(native, T, D):
 
 
 @gpu
+def test_offsets_are_reported_into_the_buffer_of_the_call(native):
+    from streamep_b200.models.moe_layer import make_buffer
+    buf = make_buffer(None, 64, 64, 2, 4)
+    x, gate, dh = inputs(300, 16, BF, seed=1)
+    good = torch.tensor([0, 100, 300], device=DEV)
+    assert torch.equal(gated_scan(x, gate, offsets=good, buffer=buf), gated_scan(x, gate, offsets=good))
+    buf.check_status()
+    gated_scan(x, gate, offsets=torch.tensor([0, 301], device=DEV), buffer=buf)
+    ops.check_status()
+    with pytest.raises(StreamEPError, match="offsets"):
+        buf.check_status()
+    buf.check_status()
+
+
+@gpu
 def test_bad_offsets_are_reported(native):
     x, gate, dh = inputs(300, 16, BF, seed=1)
     for at in ([0, 200, 100, 300], [0, 301], [-1, 5], [5, 2], [0, 2 ** 31 - 1]):
