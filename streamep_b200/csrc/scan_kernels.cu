@@ -640,7 +640,10 @@ ScanSplit split_of(const ScanShape& p, int vec, int sms, bool back) {
   // bytes an SM: forward 232 and 260 us, backward 470 and 396.
   const long long enough = static_cast<long long>(sms) * (vec == 2 ? 1536 : vec == 1 ? 768 : back ? 1200 : 384);
   long long parts = 1;
-  while (sequences * vectors * parts < enough && length > 32 * parts) parts *= 2;
+  // (bf16 channels off the boundaries, which come through registers: 7488 rows of 1001 in 9 sequences with gradients in segments of 32 and 16 rows 174 and 136 us of kernels;
+  // fp32 ones 151 and 149, as one sequence 133 and 142)
+  const long long least = vec == 1 && p.half ? 16 : 32;
+  while (sequences * vectors * parts < enough && length > least * parts) parts *= 2;
   // (short calls: 4096 rows of 1024 channels in segments of 32 and 16 rows forward 21.5 and 19.5 us, backward 29.7 and 25.7; 8192 rows of 2048 backward 58.6 and 65.6)
   while (sequences * vectors * parts < sms * 256ll && length > 16 * parts) parts *= 2;
   s.rows = static_cast<int>((length + parts - 1) / parts);
