@@ -1,6 +1,6 @@
 // Gated linear recurrence along sequences, and its gradients.
 //
-//   keep_t = sigmoid(gate_t), take_t = 1 - keep_t:   h_t = keep_t h_{t-1} + take_t x_t
+//   keep_t = sigmoid(gate_t), take_t = 1 - keep_t:   h_t = keep_t h_{t-1} + take_t x_t = h_{t-1} + take_t (x_t - h_{t-1})
 //   g_t = dh_t + keep_{t+1} g_{t+1}:   dx_t = take_t g_t,   dgate_t = g_t keep_t take_t (h_{t-1} - x_t),   dh_{-1} = keep_0 g_0
 //
 // The state, and everything that is added up along a sequence, is fp32.
@@ -26,14 +26,16 @@ namespace sep {
 namespace {
 
 constexpr int kScanThreads = 128;               // (256: 8192 rows of 2048 channels forward 40.8 -> 48 us, backward 58.6 -> 61)
+// Blocks an SM: 72 registers a thread.  With 80 and 6 blocks 8192 rows of 2048 bf16 channels forward took 42.9 us instead of 37.5, 7488 of 1001 61.6 instead of 45.5.
+constexpr int kScanBlocks = 7;
 
-// sigmoid(gate) and sigmoid(-gate), each to its own last digits: 1 / (1 + e) and e / (1 + e) of e = exp(gate), which is held at 2^126 (a gate of
-// 87; NaN stays).  For bf16 gates the exponent is rounded once (|gate| 2^-24 of the result), for fp32 ones it is not.
+// e = exp(gate), held at 2^126 (a gate of 87; NaN stays), and sigmoid(-gate) = 1 / (1 + e), what a row takes; it keeps e / (1 + e), to that one's own last
+// digits too.  For bf16 gates the exponent is rounded once (|gate| 2^-24 of the result), for fp32 ones it is not.
 __device__ __forceinline__ float at_most(float v, float top) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(top)); return r; }
 __device__ __forceinline__ float ex2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float reciprocal(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 template <class T, int V>
-__device__ __forceinline__ void gates_of(const Row<V>& gate, Row<V>& keep, Row<V>& take) {
+__device__ __forceinline__ void gates_of(const Row<V>& gate, Row<V>& power, Row<V>& take) {
   float e[V];
   if constexpr (sizeof(T) == 2) {
     const Row<V> scaled = gate * Row<V>::all(1.4426950408889634f);
@@ -45,30 +47,78 @@ __device__ __forceinline__ void gates_of(const Row<V>& gate, Row<V>& keep, Row<V
 #pragma unroll
     for (int i = 0; i < V; ++i) e[i] = expf(at_most(e[i], 87.f));
   }
-  const Row<V> power = Row<V>::of(e), sum = power + Row<V>::all(1.f);
+  power = Row<V>::of(e);
+  const Row<V> sum = power + Row<V>::all(1.f);
   sum.get(e);
 #pragma unroll
   for (int i = 0; i < V; ++i) e[i] = reciprocal(e[i]);
   take = Row<V>::of(e);
-  keep = power * take;
-  // near 1 the difference is better by far: a relative error of `keep` that has one sign adds up over the rows that a state lasts
+}
+// keep h + take x, and keep h alone.  Where less than half is taken, as h + take (x - h) and h - take h: 32 bits cannot hold a `keep` near 1 and 1 - keep
+// alike, and what `keep` is off by, at every row to one side, makes a state that lasts e^gate rows drift away from its inputs (300000 rows whose inputs
+// equal the state, gates of 12 to 18: by up to 0.9 %; in these forms by 2e-6).  Else as x - keep (x - h).  Written with predicates, which leave the selections that a
+// compiler makes of it out (131072 rows of 1024 bf16 channels forward 250 -> 242 us).
+// kAny: also where the state, or the difference, is infinite; else that makes a NaN, which stays in the state and is seen at its end.
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+template <bool kAny> __device__ __forceinline__ float follow(float h, float x, float power, float take) {
+  const float d = x - h, keep = power * take;
+  if (kAny && !finite(d)) return fmaf(keep, h, take * x);
+  float r;
+  asm("{\n .reg .pred near;\n setp.gt.f32 near, %1, 0f3F800000;\n @near fma.rn.f32 %0, %2, %4, %5;\n @!near fma.rn.f32 %0, %3, %4, %6;\n}"
+      : "=f"(r) : "f"(power), "f"(take), "f"(-keep), "f"(d), "f"(h), "f"(x));
+  return r;
+}
+template <bool kAny> __device__ __forceinline__ float fade(float g, float power, float take) {
+  const float keep = power * take;
+  if (kAny && !finite(g)) return keep * g;
+  float r;
+  asm("{\n .reg .pred near;\n setp.gt.f32 near, %1, 0f3F800000;\n @near fma.rn.f32 %0, %2, %4, %4;\n @!near mul.rn.f32 %0, %3, %4;\n}"
+      : "=f"(r) : "f"(power), "f"(-take), "f"(keep), "f"(g));
+  return r;
+}
+template <bool kAny, int V> __device__ __forceinline__ Row<V> follow(const Row<V>& h, const Row<V>& x, const Row<V>& power, const Row<V>& take) {
+  Row<V> r;
 #pragma unroll
-  for (int i = 0; i < V; ++i) keep.f[i] = take.f[i] < 0.5f ? 1.f - take.f[i] : keep.f[i];
+  for (int i = 0; i < V; ++i) r.f[i] = follow<kAny>(h.f[i], x.f[i], power.f[i], take.f[i]);
+  return r;
 }
-// What a run of rows does to the state in front of it: h -> a h + b, or h -> b where a sequence starts within (a is then -0, and stays negative
-// in products: a state of the sequence before, infinite or NaN as it may be, is not multiplied with).
-struct Run { float a, b; };
-__device__ __forceinline__ float apply(Run r, float h) { return signbit(r.a) ? r.b : fmaf(r.a, h, r.b); }
+template <bool kAny, int V> __device__ __forceinline__ Row<V> fade(const Row<V>& g, const Row<V>& power, const Row<V>& take) {
+  Row<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.f[i] = fade<kAny>(g.f[i], power.f[i], take.f[i]);
+  return r;
+}
+template <int V> __device__ __forceinline__ bool finite(const Row<V>& r) {
+  bool all = true;
+#pragma unroll
+  for (int i = 0; i < V; ++i) all = all && finite(r.f[i]);
+  return all;
+}
+// What a run of rows does to the state in front of it: h -> a h + b, or h -> b where a sequence starts within (a is then -0: a state of the sequence
+// before, infinite or NaN as it may be, is not multiplied with).  For the same reason as above it knows 1 - a too, and for an a of a half or more goes by that.
+struct Run { float a, lost, b; };                // lost: 1 - a
+__device__ __forceinline__ float apply(Run r, float h) {
+  if (signbit(r.a)) h = 0.f;
+  const bool near = r.lost <= 0.5f && finite(h);
+  return fmaf(near ? -r.lost : r.a, h, r.b) + (near ? h : 0.f);
+}
 __device__ __forceinline__ Run join(Run first, Run then) {
-  return signbit(then.a) ? then : Run{then.a * first.a, fmaf(then.a, first.b, then.b)};
+  return {signbit(then.a) ? then.a : then.a * first.a, fmaf(then.lost, 1.f - first.lost, first.lost), apply(then, first.b)};
 }
-__device__ __forceinline__ Run nothing() { return {1.f, 0.f}; }
-
+__device__ __forceinline__ Run nothing() { return {1.f, 0.f, 0.f}; }
+// a and 1 - a in one number: a start, -(1 - a), or a
+constexpr float kStarts = 2.f;
+__device__ __forceinline__ float factor_of(Run r) { return signbit(r.a) ? kStarts : r.lost <= 0.5f ? -r.lost : r.a; }
+__device__ __forceinline__ Run run_of(float factor, float b) {
+  if (factor == kStarts) return {-0.f, 1.f, b};
+  return signbit(factor) ? Run{1.f + factor, -factor, b} : Run{factor, 1.f - factor, b};
+}
 
 __device__ __forceinline__ long long offset_of(const ScanShape& p, int i) {
+  if (p.offsets == nullptr) return static_cast<long long>(i) * p.length;
   return p.offsets_wide ? static_cast<const long long*>(p.offsets)[i] : static_cast<const int*>(p.offsets)[i];
 }
-// The sequences of neighbouring rows of a packed batch; -1 where a row belongs to none.  Whatever the offsets are, it is one that exists.
+// The sequences of neighbouring rows; -1 where a row belongs to none.  Whatever the offsets are, it is one that exists.
 struct SequenceWalk {
   int i;                         // offsets[i] <= row < offsets[i + 1]
   long long first, behind;
@@ -261,53 +311,66 @@ __device__ __forceinline__ void walk_rows(const Segment<Tl, kBack>& seg, int fir
 // What the rows of a segment do to the state in front of them.  All threads call.  `rows`: x, or the rows' own gradients (which may be left out).
 template <class T, class Tl, bool kBack>
 __device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSplit& s, const Segment<Tl, kBack>& seg, const void* rows, long long rows_stride, const float* edge,
-                                               Row<Tl::V>& a, Row<Tl::V>& b) {
+                                               Run (&run)[Tl::V]) {
   constexpr int V = Tl::V;
-  a = Row<V>::all(1.f); b = Row<V>::all(0.f);
+  Row<V> a = Row<V>::all(1.f), lost = Row<V>::all(0.f), b = Row<V>::all(0.f);    // lost: 1 - a
+  bool starts = false;
+#pragma unroll
+  for (int i = 0; i < V; ++i) run[i] = nothing();
   const bool plain = all_plain(p, seg, kBack ? seg.first : seg.first - 1, kBack ? seg.last + 1 : seg.last);
-  if (!seg.there) return;
+  if (!seg.there || seg.first >= seg.last) return;
   auto begin = [&](int sequence) {
-    a = Row<V>::all(-0.f);
+    starts = true;
     b = edge != nullptr && sequence >= 0 ? Tl::load(edge + static_cast<long long>(sequence) * p.channels + seg.col, seg.count) : Row<V>::all(0.f);
   };
   const bool none = kBack && rows == nullptr;
-  auto take_row = [&](const Raw<T, V> (&row)[2]) {
-    Row<V> keep, take;
-    gates_of<T, V>(row[0].get(), keep, take);
-    a = a * keep;
-    if constexpr (kBack) b = keep * (none ? b : b + row[1].get()); else b = fused(keep, b, take * row[1].get());
+  auto take_row = [&](const Raw<T, V> (&row)[2], auto any) {
+    constexpr bool kAny = decltype(any)::value;
+    Row<V> power, take;
+    gates_of<T, V>(row[0].get(), power, take);
+    lost = fused(take, a, lost);
+    a = fade<false>(a, power, take);
+    if constexpr (kBack) b = fade<kAny>(none ? b : b + row[1].get(), power, take); else b = follow<kAny>(b, row[1].get(), power, take);
   };
   const T* base[2] = {static_cast<const T*>(p.gate) + seg.col, static_cast<const T*>(none ? p.gate : rows) + seg.col};
   const long long stride[2] = {p.gate_stride, none ? p.gate_stride : rows_stride};
-  const bool dense = p.offsets == nullptr;
-  if (plain) {
-    if (dense && seg.part == (kBack ? s.parts - 1 : 0)) begin(seg.sequence);
-    walk_rows<T, Tl, kBack, 2>(seg, seg.first, base, stride, [&](int, Raw<T, V> (&row)[2]) { take_row(row); });
-  } else {
+  bool bad = false;              // a number that is not finite was met
+  auto sequences = [&](auto any) {
     SequenceWalk walk(p, kBack ? seg.last : seg.first - 1);
     int previous = walk.at(p, kBack ? seg.last : seg.first - 1);
     walk_rows<T, Tl, kBack, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
       const int sequence = walk.at(p, t);
-      if (sequence != previous || sequence < 0) begin(sequence);
-      if (sequence >= 0) take_row(row);
+      if (sequence != previous || sequence < 0) { bad = bad || !finite(b); begin(sequence); }
+      if (sequence >= 0) take_row(row, any);
       previous = sequence;
     });
+  };
+  if (plain) {
+    if (p.offsets == nullptr && seg.part == (kBack ? s.parts - 1 : 0)) begin(seg.sequence);
+    walk_rows<T, Tl, kBack, 2>(seg, seg.first, base, stride, [&](int, Raw<T, V> (&row)[2]) { take_row(row, std::false_type{}); });
+  } else {
+    sequences(std::false_type{});
   }
+  if (bad || !finite(b)) {
+    a = Row<V>::all(1.f); lost = b = Row<V>::all(0.f);
+    starts = false;
+    sequences(std::true_type{});
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) run[i] = starts ? Run{-0.f, 1.f, b.f[i]} : Run{a.f[i], lost.f[i], b.f[i]};
 }
 
 // From the runs of a block's segments: of those before each thread's own.  All threads call; the ring is not in use.
 template <class Tl>
-__device__ __forceinline__ void runs_before(Row<Tl::V> a, Row<Tl::V> b, Run (&before)[Tl::V]) {
+__device__ __forceinline__ void runs_before(const Run (&own)[Tl::V], Run (&before)[Tl::V]) {
   constexpr int V = Tl::V;
   extern __shared__ __align__(16) unsigned char ring[];
   Run* runs = reinterpret_cast<Run*>(ring);                    // [SEGS][COLS]
   __shared__ Run parts[Tl::PARTS][Tl::COLS];
   const int seg = threadIdx.x / Tl::LANES, side = threadIdx.x % Tl::LANES;
-  float fa[V], fb[V];
-  a.get(fa); b.get(fb);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < V; ++i) runs[seg * Tl::COLS + Tl::place(side, i)] = Run{fa[i], fb[i]};
+  for (int i = 0; i < V; ++i) runs[seg * Tl::COLS + Tl::place(side, i)] = own[i];
   __syncthreads();
   const int ch = threadIdx.x % Tl::COLS, part = threadIdx.x / Tl::COLS;
   constexpr int kEach = Tl::SEGS / Tl::PARTS;
@@ -317,7 +380,7 @@ __device__ __forceinline__ void runs_before(Row<Tl::V> a, Row<Tl::V> b, Run (&be
     Run* at = runs + (part * kEach + i) * Tl::COLS + ch;
     const Run r = *at;
     *at = run;
-    run = join(run, r);
+    run = i == 0 ? r : join(run, r);
   }
   parts[part][ch] = run;
   __syncthreads();
@@ -325,8 +388,8 @@ __device__ __forceinline__ void runs_before(Row<Tl::V> a, Row<Tl::V> b, Run (&be
   for (int i = 0; i < V; ++i) {
     run = nothing();
 #pragma unroll
-    for (int q = 0; q < Tl::PARTS; ++q)
-      if (q < seg / kEach) run = join(run, parts[q][Tl::place(side, i)]);
+    for (int q = 0; q < Tl::PARTS - 1; ++q)
+      if (q < seg / kEach) run = q == 0 ? parts[q][Tl::place(side, i)] : join(run, parts[q][Tl::place(side, i)]);
     before[i] = join(run, runs[seg * Tl::COLS + Tl::place(side, i)]);
   }
   __syncthreads();               // the ring may be filled again
@@ -334,33 +397,30 @@ __device__ __forceinline__ void runs_before(Row<Tl::V> a, Row<Tl::V> b, Run (&be
 
 // Leaves, of every segment, the run of the segments before it in its block; and of every block the run of all.
 template <class T, class Tl, bool kBack>
-__global__ void __launch_bounds__(kScanThreads, 6) scan_runs_kernel(const ScanShape p, const ScanSplit s, const void* rows, long long rows_stride, const float* edge) {
+__global__ void __launch_bounds__(kScanThreads, kScanBlocks) scan_runs_kernel(const ScanShape p, const ScanSplit s, const void* rows, long long rows_stride, const float* edge) {
   constexpr int V = Tl::V;
   grid_release();
   const int block = blockIdx.x / s.tiles, tile = blockIdx.x - block * s.tiles;
   const Segment<Tl, kBack> seg(p, s, block, tile);
-  Row<V> a, b;
-  run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
-  Run before[V];
-  runs_before<Tl>(a, b, before);
+  Run run[V], before[V];
+  run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, run);
+  runs_before<Tl>(run, before);
   if (!seg.there) return;
   float fa[V], fb[V];
   const long long at = static_cast<long long>(seg.order) * p.channels + seg.col;
 #pragma unroll
-  for (int i = 0; i < V; ++i) { fa[i] = before[i].a; fb[i] = before[i].b; }
+  for (int i = 0; i < V; ++i) { fa[i] = factor_of(before[i]); fb[i] = before[i].b; }
   Tl::store(s.factors + at, Row<V>::of(fa), seg.count);
   Tl::store(s.sums + at, Row<V>::of(fb), seg.count);
   if (seg.order % Tl::SEGS != Tl::SEGS - 1) return;            // (nobody follows a block that is not full)
-  float ga[V], gb[V];
-  a.get(ga); b.get(gb);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const Run r = join(before[i], Run{ga[i], gb[i]});
-    ga[i] = r.a; gb[i] = r.b;
+    const Run r = join(before[i], run[i]);
+    fa[i] = factor_of(r); fb[i] = r.b;
   }
   const long long block_at = static_cast<long long>(block) * p.channels + seg.col;
-  Tl::store(s.block_factors + block_at, Row<V>::of(ga), seg.count);
-  Tl::store(s.block_sums + block_at, Row<V>::of(gb), seg.count);
+  Tl::store(s.block_factors + block_at, Row<V>::of(fa), seg.count);
+  Tl::store(s.block_sums + block_at, Row<V>::of(fb), seg.count);
 }
 
 // The state in front of each thread's segment.  All threads call.
@@ -370,10 +430,9 @@ __device__ __forceinline__ Row<Tl::V> state_before(const ScanShape& p, const Sca
   constexpr int V = Tl::V;
   if (s.parts == 1) return Row<V>::all(0.f);
   if (s.within) {                                // no sequence goes on in another block
-    Row<V> a, b;
-    run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, a, b);
-    Run before[V];
-    runs_before<Tl>(a, b, before);
+    Run run[V], before[V];
+    run_of_segment<T, Tl, kBack>(p, s, seg, rows, rows_stride, edge, run);
+    runs_before<Tl>(run, before);
     float f[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = before[i].b;
@@ -403,7 +462,7 @@ __device__ __forceinline__ Row<Tl::V> state_before(const ScanShape& p, const Sca
 #pragma unroll 8
     for (int k = begin; k < end; ++k) {
       const long long at = static_cast<long long>(k) * p.channels + col;
-      run = join(run, Run{s.block_factors[at], s.block_sums[at]});
+      run = join(run, run_of(s.block_factors[at], s.block_sums[at]));
     }
   }
   parts[part][ch] = run;
@@ -416,10 +475,10 @@ __device__ __forceinline__ Row<Tl::V> state_before(const ScanShape& p, const Sca
   Tl::load(s.sums + at, seg.count).get(fb);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    float state = 0.f;
+    float state = parts[0][Tl::place(side, i)].b;
 #pragma unroll
-    for (int q = 0; q < Tl::PARTS; ++q) state = apply(parts[q][Tl::place(side, i)], state);
-    f[i] = apply(Run{fa[i], fb[i]}, state);
+    for (int q = 1; q < Tl::PARTS; ++q) state = apply(parts[q][Tl::place(side, i)], state);
+    f[i] = apply(run_of(fa[i], fb[i]), state);
   }
   return Row<V>::of(f);
 }
@@ -447,7 +506,7 @@ __device__ __forceinline__ void empty_sequences(const ScanShape& p, const float*
 }
 
 template <class T, class Tl>
-__global__ void __launch_bounds__(kScanThreads, 6) scan_forward_kernel(const ScanParams p, const ScanSplit s) {
+__global__ void __launch_bounds__(kScanThreads, kScanBlocks) scan_forward_kernel(const ScanParams p, const ScanSplit s) {
   constexpr int V = Tl::V;
   grid_wait();
   empty_sequences<Tl>(p, p.initial, p.final_state, true);
@@ -456,41 +515,49 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_forward_kernel(const Sca
   const Segment<Tl, false> seg(p, s, block, tile);
   Row<V> h = state_before<T, Tl, false>(p, s, seg, block, tile, p.x, p.x_stride, p.initial);
   const bool plain = all_plain(p, seg, seg.first - 1, seg.last + 1);
-  if (!seg.there) return;
+  if (!seg.there || seg.first >= seg.last) return;
   auto state_at = [&](int sequence) { return static_cast<long long>(sequence) * p.channels + seg.col; };
   auto begin = [&](int sequence) { h = p.initial != nullptr ? Tl::load(p.initial + state_at(sequence), seg.count) : Row<V>::all(0.f); };
-  auto step = [&](const Raw<T, V> (&row)[2]) {
-    Row<V> keep, take;
-    gates_of<T, V>(row[0].get(), keep, take);
-    h = fused(keep, h, take * row[1].get());
+  auto step = [&](const Raw<T, V> (&row)[2], auto any) {
+    Row<V> power, take;
+    gates_of<T, V>(row[0].get(), power, take);
+    h = follow<decltype(any)::value>(h, row[1].get(), power, take);
   };
   const T* base[2] = {static_cast<const T*>(p.gate) + seg.col, static_cast<const T*>(p.x) + seg.col};
   const long long stride[2] = {p.gate_stride, p.x_stride};
   T* out = static_cast<T*>(p.h) + seg.col;
-  const bool dense = p.offsets == nullptr;
-  if (plain) {
-    if (dense && seg.part == 0) begin(seg.sequence);
-    walk_rows<T, Tl, false, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
-      step(row);
-      Tl::template store_rounded<T>(out + static_cast<long long>(t) * p.channels, h, seg.count);
-    });
-    if (dense && p.final_state != nullptr && seg.last == (seg.sequence + 1) * p.length && seg.first < seg.last) Tl::store(p.final_state + state_at(seg.sequence), h, seg.count);
-  } else {
+  const Row<V> before = h;
+  bool bad = false;              // a number that is not finite was met
+  auto sequences = [&](auto any) {
     SequenceWalk walk(p, seg.first - 1);
     int previous = walk.at(p, seg.first - 1), sequence = walk.at(p, seg.first);
     walk_rows<T, Tl, false, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
       const int behind = walk.at(p, t + 1);
+      if (sequence != previous || sequence < 0) { bad = bad || !finite(h); h = Row<V>::all(0.f); }
       if (sequence >= 0) {
         if (sequence != previous) begin(sequence);
-        step(row);
+        step(row, any);
         if (p.final_state != nullptr && behind != sequence) Tl::store(p.final_state + state_at(sequence), h, seg.count);
-      } else {
-        h = Row<V>::all(0.f);
       }
       Tl::template store_rounded<T>(out + static_cast<long long>(t) * p.channels, h, seg.count);
       previous = sequence;
       sequence = behind;
     });
+  };
+  if (plain) {
+    const bool dense = p.offsets == nullptr;
+    if (dense && seg.part == 0) begin(seg.sequence);
+    walk_rows<T, Tl, false, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
+      step(row, std::false_type{});
+      Tl::template store_rounded<T>(out + static_cast<long long>(t) * p.channels, h, seg.count);
+    });
+    if (dense && p.final_state != nullptr && seg.last == (seg.sequence + 1) * p.length) Tl::store(p.final_state + state_at(seg.sequence), h, seg.count);
+  } else {
+    sequences(std::false_type{});
+  }
+  if (bad || !finite(h)) {       // again, all of it
+    h = before;
+    sequences(std::true_type{});
   }
 }
 
@@ -504,18 +571,18 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
   const Segment<Tl, true> seg(p, s, block, tile);
   Row<V> back = state_before<T, Tl, true>(p, s, seg, block, tile, p.dh, p.dh_stride, p.dfinal);     // keep_{t+1} g_{t+1}
   const bool plain = all_plain(p, seg, seg.first - 1, seg.last + 1);
-  if (!seg.there) return;
+  if (!seg.there || seg.first >= seg.last) return;
   auto state_at = [&](int sequence) { return static_cast<long long>(sequence) * p.channels + seg.col; };
   const bool none = p.dh == nullptr;
   // one row, whose state before is h
-  auto step = [&](int t, const Row<V>& gate, const Row<V>& dh, const Row<V>& x, const Row<V>& h) {
-    Row<V> keep, take;
-    gates_of<T, V>(gate, keep, take);
+  auto step = [&](auto any, int t, const Row<V>& gate, const Row<V>& dh, const Row<V>& x, const Row<V>& h) {
+    Row<V> power, take;
+    gates_of<T, V>(gate, power, take);
     const Row<V> g = none ? back : back + dh;
     const long long at = static_cast<long long>(t) * p.channels + seg.col;
     if (p.dx != nullptr) Tl::template store_rounded<T>(static_cast<T*>(p.dx) + at, take * g, seg.count);
-    if constexpr (kGate) Tl::template store_rounded<T>(static_cast<T*>(p.dgate) + at, g * (keep * take) * fused(Row<V>::all(-1.f), x, h), seg.count);
-    back = keep * g;
+    if constexpr (kGate) Tl::template store_rounded<T>(static_cast<T*>(p.dgate) + at, g * (power * take * take) * fused(Row<V>::all(-1.f), x, h), seg.count);
+    back = fade<decltype(any)::value>(g, power, take);
   };
   auto outside = [&](int t) {
     const long long at = static_cast<long long>(t) * p.channels + seg.col;
@@ -540,30 +607,23 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
     if (first == 0) first = 1;
   }
   const Row<V> zero = Row<V>::all(0.f);
-  auto zeroth = [&](const Row<V>& h) {           // row 0, where it was left out of the walk
+  auto zeroth = [&](auto any, const Row<V>& h) {           // row 0, where it was left out of the walk
     Raw<T, V> g, d, x;
     auto load = [&](Raw<T, V>& to, const T* from) {
       if constexpr (Tl::kStrided) to.gather(from, Tl::apart(1), seg.count); else to.load(from);
     };
     load(g, base[0]); load(d, base[1]);
     if constexpr (kGate) load(x, base[2]); else x = g;
-    step(0, g.get(), d.get(), x.get(), h);
+    step(any, 0, g.get(), d.get(), x.get(), h);
   };
-  const bool dense = p.offsets == nullptr;
-  if (plain) {
-    if (dense && seg.part == s.parts - 1) begin(seg.sequence);
-    const int start = dense ? seg.sequence * p.length : -1;
-    walk_rows<T, Tl, true, kArrays>(seg, first, base, stride, [&](int t, Raw<T, V> (&row)[kArrays]) {
-      if constexpr (kGate) step(t, row[0].get(), row[1].get(), row[2].get(), t == start ? initial(seg.sequence) : row[3].get());
-      else step(t, row[0].get(), row[1].get(), zero, zero);
-    });
-    if (first > seg.first && seg.first < seg.last) zeroth(initial(0));
-    if (dense && seg.first == start && seg.first < seg.last && p.dinitial != nullptr) Tl::store(p.dinitial + state_at(seg.sequence), back, seg.count);
-  } else {
+  const Row<V> beyond = back;
+  bool bad = false;              // a number that is not finite was met
+  auto sequences = [&](auto any) {
     SequenceWalk walk(p, seg.last);
     int behind = walk.at(p, seg.last), sequence = walk.at(p, seg.last - 1);
-    auto packed = [&](int t, auto calculate) {
+    auto row_of = [&](int t, auto calculate) {
       const int previous = walk.at(p, t - 1);
+      if (sequence != behind || sequence < 0) bad = bad || !finite(back);
       if (sequence >= 0) {
         if (sequence != behind) begin(sequence);
         calculate(sequence != previous);
@@ -575,12 +635,30 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
       sequence = previous;
     };
     walk_rows<T, Tl, true, kArrays>(seg, first, base, stride, [&](int t, Raw<T, V> (&row)[kArrays]) {
-      packed(t, [&](bool start) {
-        if constexpr (kGate) step(t, row[0].get(), row[1].get(), row[2].get(), start ? initial(sequence) : row[3].get());
-        else step(t, row[0].get(), row[1].get(), zero, zero);
+      row_of(t, [&](bool start) {
+        if constexpr (kGate) step(any, t, row[0].get(), row[1].get(), row[2].get(), start ? initial(sequence) : row[3].get());
+        else step(any, t, row[0].get(), row[1].get(), zero, zero);
       });
     });
-    if (first > seg.first && seg.first < seg.last) packed(0, [&](bool) { zeroth(initial(sequence)); });
+    if (first > seg.first) row_of(0, [&](bool) { zeroth(any, initial(sequence)); });
+  };
+  if (plain) {
+    constexpr std::false_type kAny{};
+    const bool dense = p.offsets == nullptr;
+    if (dense && seg.part == s.parts - 1) begin(seg.sequence);
+    const int start = dense ? seg.sequence * p.length : -1;
+    walk_rows<T, Tl, true, kArrays>(seg, first, base, stride, [&](int t, Raw<T, V> (&row)[kArrays]) {
+      if constexpr (kGate) step(kAny, t, row[0].get(), row[1].get(), row[2].get(), t == start ? initial(seg.sequence) : row[3].get());
+      else step(kAny, t, row[0].get(), row[1].get(), zero, zero);
+    });
+    if (first > seg.first) zeroth(kAny, initial(0));
+    if (dense && seg.first == start && p.dinitial != nullptr) Tl::store(p.dinitial + state_at(seg.sequence), back, seg.count);
+  } else {
+    sequences(std::false_type{});
+  }
+  if (bad || !finite(back)) {    // again, all of it
+    back = beyond;
+    sequences(std::true_type{});
   }
 }
 
@@ -594,9 +672,9 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(const ScanStepP
   gate.load(static_cast<const T*>(p.gate) + row * p.gate_stride + col);
   x.load(static_cast<const T*>(p.x) + row * p.x_stride + col);
   float* state = p.state + row * p.state_stride + col;
-  Row<V> keep, take;
-  gates_of<T, V>(gate.get(), keep, take);
-  const Row<V> h = fused(keep, load_state<V>(state), take * x.get());
+  Row<V> power, take;
+  gates_of<T, V>(gate.get(), power, take);
+  const Row<V> h = follow<true>(load_state<V>(state), x.get(), power, take);
   store_state<V>(state, h);
   store_row<T, V>(static_cast<T*>(p.h) + row * p.channels + col, h);
 }

@@ -24,9 +24,10 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, *, initial_state: Optional[t
     Returns ``h`` like ``x``; with ``return_state`` ``(h, final_state)``, float32 ``[S, D]``: the unrounded state behind each sequence's last
     row, which continues it as another call's ``initial_state`` (float32, zeros without one).  An empty sequence hands its state on.
 
-    Differentiable in ``x``, ``gate`` and ``initial_state``; there is no second derivative.  The state and its gradient are carried in 32 bits; the
-    gate's gradient ``g_t * s (1 - s) * (h_{t-1} - x_t)`` takes ``h_{t-1}`` as it was returned, rounded to the type of ``x``.  A repeated call gives
-    the same bits.  An infinity or NaN stays within its sequence and channel.
+    Differentiable in ``x``, ``gate`` and ``initial_state``; there is no second derivative.  The state and its gradient are carried in 32 bits (a state
+    that lasts for many rows follows its inputs without drift: what a row keeps and takes adds up to 1).  The gate's gradient
+    ``g_t * s (1 - s) * (h_{t-1} - x_t)`` takes ``h_{t-1}`` as it was returned, rounded to the type of ``x``.  A repeated call gives the
+    same bits.  An infinity or NaN stays within its sequence and channel.
 
     Offsets that decrease or point outside leave the sequences that they belong to undefined, and are reported, like a wait on the device that gave
     up, by ``buffer.check_status()``, or without ``buffer`` by ``streamep_b200.ops.check_status()``."""
