@@ -52,7 +52,7 @@ ScanResult scan_forward(const ScanCall& call, const at::Tensor& x, const at::Ten
                         bool want_state) {
   ScanResult out;
   out.h = at::empty(x.sizes(), x.options());
-  const LaunchContext ctx = call.context(1);
+  const LaunchContext ctx = call.context(0);
   const at::Tensor xr = as_rows(x), gr = as_rows(gate), start = initial.defined() ? initial.contiguous() : initial;
   ScanParams p{};
   static_cast<ScanShape&>(p) = shape_of(offsets, x, xr, gr, start, ctx);
@@ -62,7 +62,7 @@ ScanResult scan_forward(const ScanCall& call, const at::Tensor& x, const at::Ten
   p.final_state = want_state ? out.final_state.data_ptr<float>() : nullptr;
   const ScanSplit split = scan_split(p, ctx.sms);
   const at::Tensor space = workspace(split, p.channels, x);
-  SEP_CUDA_CHECK(launch_scan_forward(p, split, pointer(space), ctx.stream));
+  SEP_CUDA_CHECK(launch_scan_forward(p, split, pointer(space), call.context(split.within ? 1 : 2).stream));
   return out;
 }
 
@@ -88,7 +88,7 @@ class Scan : public torch::autograd::Function<Scan> {
     if (!dh.defined() && !dfinal.defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     const bool want_dx = ctx->needs_input_grad(0), want_dgate = ctx->needs_input_grad(1), want_dinitial = initial.defined() && ctx->needs_input_grad(2);
     const c10::cuda::CUDAGuard guard(x.device());
-    const LaunchContext context = call->context(1);
+    const LaunchContext context = call->context(0);
     const at::Tensor xr = as_rows(x), gr = as_rows(gate), start = initial.defined() ? initial.contiguous() : initial, hr = as_rows(h);
     const at::Tensor dhr = dh.defined() ? as_rows(dh) : dh, dfr = dfinal.defined() ? dfinal.contiguous() : dfinal;
     ScanGradParams p{};
@@ -109,7 +109,7 @@ class Scan : public torch::autograd::Function<Scan> {
       p.dinitial = want_dinitial ? dinitial.data_ptr<float>() : nullptr;
       const ScanSplit split = scan_split(p, context.sms);
       const at::Tensor space = workspace(split, p.channels, x);
-      SEP_CUDA_CHECK(launch_scan_backward(p, split, pointer(space), context.stream));
+      SEP_CUDA_CHECK(launch_scan_backward(p, split, pointer(space), call->context(split.within ? 1 : 2).stream));
     }
     return {dx, dgate, dinitial, at::Tensor(), at::Tensor(), at::Tensor()};
   }
