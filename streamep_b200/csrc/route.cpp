@@ -104,9 +104,10 @@ class BalancedRoute : public torch::autograd::Function<BalancedRoute> {
     if (want_dx) dx = at::empty({T, H}, x.options());
     if (want_dw) dw = T > 0 ? at::empty({E, H}, w_gate.options()) : at::zeros({E, H}, w_gate.options());
     if (T > 0) {
-      const LaunchContext context = call->context(want_dw ? 3 : 1);
+      const LaunchContext context = call->context(0);
       const at::Tensor xr = readable(x), wr = readable(w_gate);
       const RouteGradPlan plan = route_grad_plan(static_cast<int>(T), static_cast<int>(H), static_cast<int>(E), context.sms);
+      call->context(want_dw ? plan.dw_splits > 1 ? 3 : 2 : 1);
       at::Tensor up[3];
       for (int i = 0; i < 3; ++i) {
         const at::Tensor& g = grads[i == 0 ? 1 : i + 2];

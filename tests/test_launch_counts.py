@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from streamep_b200.models.moe_layer import make_buffer
-from streamep_b200.ops import gated_scan
+from streamep_b200.ops import balanced_router, gated_scan
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -43,3 +43,20 @@ def test_recurrence(native, shape):
     both = kernels_of(lambda: torch.autograd.grad(gated_scan(*leaves, buffer=buf), leaves, dh), buf)
     assert forward["counted"] == forward["launched"] and both["counted"] == both["launched"], (forward, both)
     assert forward["launched"] == (2 if shape[1] >= 3000 else 1) and both["launched"] == 2 * forward["launched"]
+
+
+# tokens in one part of dW and in several; gradients of x alone, of w alone
+@pytest.mark.parametrize("T,H,E", [(100, 256, 8), (8192, 512, 64), (3000, 1024, 200)])
+def test_routing(native, T, H, E):
+    buf = make_buffer(None, 64, 64, 2, 4)
+    x, w = torch.randn(T, H, device=DEV).to(BF), (torch.randn(E, H, device=DEV) * 0.02).to(BF)
+    up = torch.randn(T, 2, device=DEV)
+    with torch.no_grad():
+        got = kernels_of(lambda: balanced_router(x, w, 2, buffer=buf), buf)
+        assert got == {"counted": 2, "launched": 2}
+    for wants in ((True, True), (True, False), (False, True)):
+        leaves = [t.detach().requires_grad_(g) for t, g in zip((x, w), wants)]
+        picked = [t for t in leaves if t.requires_grad]
+        got = kernels_of(lambda: torch.autograd.grad(balanced_router(*leaves, 2, buffer=buf).topk_weights, picked, up), buf)
+        assert got["counted"] == got["launched"], (wants, got)
+        assert got["launched"] == 3 + (0 if not wants[1] else 1 if T == 100 else 2)
