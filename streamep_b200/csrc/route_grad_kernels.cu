@@ -5,9 +5,10 @@
 //
 // For both products dz is rounded to bf16, 2^-8 of each term at most, as bf16 training code rounds the gradient of its logits: against 64 bits dx and dW are
 // 2.3e-3 off in 2-norm, where their own rounding is 1.7e-3.  Up to 128 experts, where twice the products cost nothing beside the reads of x and the writes of
-// dx, dz is kept to 16 bits as the sum of two bf16 numbers, and they are 1.7e-3 off.  All sums are fp32.
+// dx, dz is kept to 16 bits as the sum of two bf16 numbers, and they are 1.7e-3 off.  All sums are fp32; of dx over up to 512 experts in one accumulator, of dW over up to 4096 tokens.
 // What bounds them: x is read and dx written once (HBM), for many experts what the SMs read from L2; and for short calls the forming of dz.  All operands lie in memory as TMA brings them in, dz as
 // [layers, T, experts rounded up to 64]; nothing is transposed.  Parts and sums have a fixed order: a repeated call gives the same bits.
+#include <algorithm>
 #include <atomic>
 #include <cuda.h>
 #include <type_traits>
@@ -26,6 +27,10 @@ constexpr int kChunk = 64 * 128;                 // a box of 64 x 64 bf16
 constexpr int kStaging = 4096;
 constexpr int kMostSmem = 226 * 1024;
 constexpr int kMostStages = 8;
+// Tokens of a part of dW.  The tensor cores cut off what an accumulator cannot hold instead of rounding, at every 16 tokens and each layer of dz: 17 numbers of which
+// each may lose 2^-23 of the largest, so that at most 512 steps make 17 2^-15 = 5e-4 of the sum, a quarter of the result's own rounding.  Measured: 2e-5; parts of 65536
+// tokens came out 3.6e-4 too small, of 2^20 6e-3.
+constexpr int kMostPart = 4096;
 
 __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
@@ -509,13 +514,14 @@ RouteGradPlan route_grad_plan(int tokens, int hidden, int experts, int sms) {
   g.dw_pairs = g.dw_blocks == 2 && hidden >= 2048 && static_cast<long long>(tokens) * hidden * groups_of_experts >= 1 << 24 ? 1 : 0;
   const int of = g.dw_pairs ? 2 : 1, unit_cols = kCols * of;
   const int units = groups_of_experts * ((hidden + unit_cols - 1) / unit_cols), most = (tokens + 4 * kBK - 1) / (4 * kBK);
-  int best = 1;
+  const int least = (tokens + kMostPart - 1) / kMostPart;
+  int best = least;
   double best_time = 0.0;
-  for (int s = 1; s <= most && s <= 64; ++s) {
+  for (int s = least; s <= most && s <= std::max(64, least + 32); ++s) {
     const int rounds = (units * s + sms / of - 1) / (sms / of);
     // a round's blocks of tokens, and what an output tile costs: about as much as 6 blocks
     const double time = rounds * (static_cast<double>((tokens + kBK - 1) / kBK) / s + 6.0);
-    if (s == 1 || time < best_time) { best = s; best_time = time; }
+    if (s == least || time < best_time) { best = s; best_time = time; }
   }
   g.dw_splits = best;
   // stages of 64 KB: two blocks, or two layers of one; of a pair of 48
