@@ -341,6 +341,18 @@ __global__ void __launch_bounds__(kThreads, 1) route_forward_kernel(const __grid
   }
 }
 
+// A sum of numbers of one sign with what its roundings lose beside it: of tens of thousands of blocks that are alike (the same token over and over) a plain one came
+// out 2e-4 off.
+struct LongSum {
+  float sum = 0.f, lost = 0.f;
+  __device__ __forceinline__ void add(float v) {
+    const float s = __fadd_rn(sum, v);
+    lost = __fadd_rn(lost, __fsub_rn(v, __fsub_rn(s, sum)));
+    sum = s;
+  }
+  __device__ __forceinline__ float get() const { return sum + lost; }
+};
+
 // One block adds up the blocks' sums: `rows` threads for each expert.
 constexpr int kJoinThreads = 1024;
 __global__ void __launch_bounds__(kJoinThreads) route_join_kernel(const RouteStatsParams p) {
@@ -350,19 +362,19 @@ __global__ void __launch_bounds__(kJoinThreads) route_join_kernel(const RouteSta
   __shared__ int live[32];
   const int E = p.experts, rows = kJoinThreads / E, e = threadIdx.x % E, row = threadIdx.x / E, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_wait();
-  float sum = 0.f, squares = 0.f;
+  LongSum probs, lse2;
   int count = 0, n = 0;
   if (row < rows) {
 #pragma unroll 8
     for (int b = row; b < p.blocks; b += rows) {
       const float2 v = p.parts[static_cast<size_t>(b) * E + e];
-      sum += v.x; count += __float_as_int(v.y);
+      probs.add(v.x); count += __float_as_int(v.y);
     }
   }
-  for (int b = threadIdx.x; b < p.blocks; b += kJoinThreads) { const float2 v = p.other_parts[b]; squares += v.x; n += __float_as_int(v.y); }
-  squares = warp_sum(squares);
+  for (int b = threadIdx.x; b < p.blocks; b += kJoinThreads) { const float2 v = p.other_parts[b]; lse2.add(v.x); n += __float_as_int(v.y); }
+  float squares = warp_sum(lse2.get());
   n = __reduce_add_sync(0xffffffffu, n);
-  sums[threadIdx.x] = sum;
+  sums[threadIdx.x] = probs.get();
   counts[threadIdx.x] = count;
   if (lane == 0) { other[warp] = squares; live[warp] = n; }
   __syncthreads();
@@ -372,12 +384,12 @@ __global__ void __launch_bounds__(kJoinThreads) route_join_kernel(const RouteSta
   float term = 0.f;
   if (threadIdx.x < E) {
     long long total = 0;
-    sum = 0.f;
-    for (int r = 0; r < rows; ++r) { sum += sums[r * E + e]; total += counts[r * E + e]; }
+    LongSum all;
+    for (int r = 0; r < rows; ++r) { all.add(sums[r * E + e]); total += counts[r * E + e]; }
     const float load = static_cast<float>(static_cast<double>(total) * E / p.top_k) * share;
     p.counts[e] = total;
     p.load[e] = load;
-    term = load * (sum * share);
+    term = load * (all.get() * share);
   }
   __syncthreads();
   term = warp_sum(term);

@@ -37,3 +37,22 @@ def test_dw_of_many_tokens_is_not_too_small(native, H):
         least, most = ((want * (1 + sign * slack)).to(torch.bfloat16) for sign in (-1, 1))
         assert bool((got >= least).all()) and bool((got <= most).all()), (i, int((got < least).sum()), int((got > most).sum()))
     ops.check_status()
+
+
+@gpu
+def test_losses_of_many_tokens(native):
+    """All tokens alike, so that the sums of all blocks are, and a plain sum of them would round to one side for long stretches.  In units of 2^-24: a
+    probability is off by 4 (exponential), 15 (its sum: 10 of a lane, 5 steps over the warp) and 3; a block's sum by 4 tokens of a warp and 16 warps; the sum of
+    all blocks keeps what it loses, and 3 rows and 5 steps join it; the load and products 6.  The squared logsumexp: twice 20, and its sums the same way."""
+    T, H, E = 1 << 21, 8, 300
+    slack = 64 * 2.0 ** -24
+    for i in range(6):
+        x = torch.zeros(T, H, device=DEV, dtype=torch.bfloat16)
+        w = torch.zeros(E, H, device=DEV, dtype=torch.bfloat16)
+        x[:, 0], w[0, 0] = 1.0, 5.0 + i * 0.375
+        route = balanced_router(x, w, 1)
+        z = x[0].double() @ w.double().t()
+        assert int(route.expert_counts[0]) == T
+        assert abs(float(route.balance_loss) / float(E * torch.softmax(z, 0)[0]) - 1) <= slack
+        assert abs(float(route.z_loss) / float(torch.logsumexp(z, 0) ** 2) - 1) <= slack
+    ops.check_status()
