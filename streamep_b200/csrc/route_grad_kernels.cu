@@ -28,7 +28,7 @@ constexpr int kStaging = 4096;
 constexpr int kMostSmem = 226 * 1024;
 constexpr int kMostStages = 8;
 // Tokens of a part of dW.  The tensor cores cut off what an accumulator cannot hold instead of rounding, at every 16 tokens and each layer of dz: 17 numbers of which
-// each may lose 2^-23 of the largest, so that at most 512 steps make 17 2^-15 = 5e-4 of the sum, a quarter of the result's own rounding.  Measured: 2e-5; parts of 65536
+// each may lose 2^-23 of the largest, so that at most 512 steps make 17 2^-15 = 5e-4 of the sum, an eighth of the result's own rounding.  Measured: 2e-5; parts of 65536
 // tokens came out 3.6e-4 too small, of 2^20 6e-3.
 constexpr int kMostPart = 4096;
 

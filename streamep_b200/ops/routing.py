@@ -37,8 +37,9 @@ def balanced_router(x: torch.Tensor, w_gate: torch.Tensor, top_k: int, num_ranks
     ``w_gate`` multiplies their ``x`` with zero, which an infinity or NaN survives.  Every rank's losses are those of its own tokens.
 
     The choice itself and the counts have no gradient; weights and losses do, for ``x`` and ``w_gate`` (bf16), by ``dz @ w_gate`` and
-    ``dz.T @ x`` with the gradient ``dz`` of the logits and all sums in 32 bits.  There is no second derivative.  A repeated call
-    gives the same bits.  Ties go to the lowest expert.  1 to 512 experts, up to 32 of them a token, ``H`` a multiple of 8.
+    ``dz.T @ x``.  The gradient ``dz`` of the logits is formed in 32 bits; the products take it as the sum of two bf16 numbers (2^-16 of it) up
+    to 128 experts, and above as one (2^-8 of it, as a bf16 logit's gradient would be): in 2-norm the gradients are then 2.3e-3 off instead of the 1.7e-3 that is the
+    rounding of the results.  Sums are in 32 bits.  There is no second derivative.  A repeated call gives the same bits.  Ties go to the lowest expert.  1 to 512 experts, up to 32 of them a token, ``H`` a multiple of 8.
 
     A wait on the device that gave up is reported by ``buffer.check_status()``, or without ``buffer`` by
     ``streamep_b200.ops.check_status()``."""

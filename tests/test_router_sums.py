@@ -15,10 +15,10 @@ def test_dw_of_many_tokens_is_not_too_small(native, H):
     """All tokens alike, so that every term of an element of dW has one sign, and what an accumulator cuts off adds up.  A part has 4096 tokens at most:
     256 steps of 16, twice for the two numbers of dz.  A step adds 16 products and what was there, aligned to the largest of them; in 24 bits each loses up to
     2^-23 of that one, 17 2^-23 of the sum so far, 17 2^-24 of the final one on average.  Parts are joined by up to 40 sums; dz itself is
-    off by 2^-17 (two bf16 numbers) and 2^-20 (exponentials, products).  The result is that sum rounded, and rounding keeps order: it lies between
-    the rounded ends of the sum's range.  (A result's own rounding is 2^-9 of it, and hides a smaller error in all but the elements next to a border.)"""
+    off by 2^-16 (two bf16 numbers) and 2^-20 (exponentials, products).  The result is that sum rounded, and rounding keeps order: it lies between
+    the rounded ends of the sum's range.  (A result's own rounding is up to 2^-8 of it, and hides a smaller error in all but the elements next to a border.)"""
     T, E = 1 << 17, 2
-    slack = (512 * 17 + 40) * 2.0 ** -24 + 2.0 ** -17 + 2.0 ** -20
+    slack = (512 * 17 + 40) * 2.0 ** -24 + 2.0 ** -16 + 2.0 ** -20
     g = torch.Generator(device=DEV).manual_seed(1)
     row = (0.5 + torch.rand(H, generator=g, device=DEV)).to(torch.bfloat16)
     x = row.expand(T, H).contiguous()
