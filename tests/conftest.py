@@ -1,5 +1,6 @@
 import os
 import sys
+import time
 
 import pytest
 
@@ -13,6 +14,8 @@ def pytest_configure(config):
 def pytest_collection_modifyitems(config, items):
     import torch
 
+    # (a profile that lost an event should not keep other tests from running where the first failure ends the run)
+    items.sort(key=lambda item: "nvtx" in item.nodeid)
     if torch.cuda.is_available():
         return
     skip = pytest.mark.skip(reason="no CUDA device")
@@ -27,3 +30,19 @@ def native():
     from streamep_b200 import _ext
 
     return _ext.load()
+
+
+@pytest.fixture(autouse=True)
+def profiles_begin_before_their_first_kernel(request, monkeypatch):
+    """The profiler leaves out what its clock places before its own start.  A window's first kernel begins 0.4 ms to 2 ms after it, by a clock that is
+    converted from the GPU's; once in some dozen runs it was missing.  With 20 ms in between it is far from the border."""
+    if "gpu" not in request.keywords:
+        return
+    from torch.profiler import profile
+
+    start = profile.start
+
+    def start_and_wait(self):
+        start(self)
+        time.sleep(0.02)
+    monkeypatch.setattr(profile, "start", start_and_wait)
