@@ -442,7 +442,8 @@ int blocks_of(const Form& f, long long rows, int sms, int resident) {
   const long long groups = threads_of(f) / f.threads, most = (rows + groups - 1) / groups, all = static_cast<long long>(sms) * resident;
   return static_cast<int>(most < all ? most : all);
 }
-// Blocks that share an SM: as many as its registers (128 a thread in the backward, 64 in the forward) and shared memory hold.
+// Blocks that share an SM: as many as its registers (128 a thread in the backward, 64 in the forward) hold.  (Shared memory holds as many of bf16 rows in whole vectors; of fp32 rows, and of
+// single numbers in rows above 1024 columns, 3 of 4 forward, 1 of 2 above 4096 columns, and 1 of 2 backward up to 4096: such a grid runs in two rounds.)
 int resident_backward(const Form& f) { return threads_of(f) > kGroupThreads ? 1 : 2; }
 int resident_forward(const Form& f) { return threads_of(f) > kGroupThreads ? 2 : 4; }
 
@@ -498,11 +499,13 @@ cudaError_t launch_norm_forward(const NormParams& p, int sms, cudaStream_t strea
       const int blocks = blocks_of(f, p.rows, sms, resident_forward(f)), ring = 2 * ring_of(f, half, 2);
       // (rows that all threads have K vectors of, such as those of 2048 and 7168 columns, without a look whether they do)
       constexpr bool kCan = V == 8 && K == 2;
-      if (kCan && f.threads * K * V == p.hidden)
-        return f.threads > kGroupThreads ? launch_rows<norm_forward_kernel<T, V, K, 512, kCan>>(p, f, blocks, ring, 2, stream)
-                                         : launch_rows<norm_forward_kernel<T, V, K, 256, kCan>>(p, f, blocks, ring, 2, stream);
-      return f.threads > kGroupThreads ? launch_rows<norm_forward_kernel<T, V, K, 512, false>>(p, f, blocks, ring, 2, stream)
-                                       : launch_rows<norm_forward_kernel<T, V, K, 256, false>>(p, f, blocks, ring, 2, stream);
+      const bool full = kCan && f.threads * K * V == p.hidden;
+      if constexpr (K * V == 16)                 // (with fewer numbers a thread a row takes no more than 256)
+        if (f.threads > kGroupThreads)
+          return full ? launch_rows<norm_forward_kernel<T, V, K, 512, kCan>>(p, f, blocks, ring, 2, stream)
+                      : launch_rows<norm_forward_kernel<T, V, K, 512, false>>(p, f, blocks, ring, 2, stream);
+      return full ? launch_rows<norm_forward_kernel<T, V, K, 256, kCan>>(p, f, blocks, ring, 2, stream)
+                  : launch_rows<norm_forward_kernel<T, V, K, 256, false>>(p, f, blocks, ring, 2, stream);
     });
   const int blocks = row_blocks(p.rows, sms);
   if (half) norm_forward_any_kernel<__nv_bfloat16><<<blocks, kRowThreads, 0, stream>>>(p);
@@ -521,11 +524,13 @@ cudaError_t launch_norm_backward(const NormGradParams& p, int sms, cudaStream_t 
       constexpr int V = decltype(vec)::value, K = decltype(each)::value;
       const int smem = ring > sums ? ring : sums;
       constexpr bool kCan = V == 8 && K == 2;
-      if (kCan && f.threads * K * V == p.hidden)
-        return f.threads > kGroupThreads ? launch_rows<norm_backward_kernel<T, V, K, 512, kCan>>(p, f, parts, smem, ahead, stream)
-                                         : launch_rows<norm_backward_kernel<T, V, K, 256, kCan>>(p, f, parts, smem, ahead, stream);
-      return f.threads > kGroupThreads ? launch_rows<norm_backward_kernel<T, V, K, 512, false>>(p, f, parts, smem, ahead, stream)
-                                       : launch_rows<norm_backward_kernel<T, V, K, 256, false>>(p, f, parts, smem, ahead, stream);
+      const bool full = kCan && f.threads * K * V == p.hidden;
+      if constexpr (K * V == 16)
+        if (f.threads > kGroupThreads)
+          return full ? launch_rows<norm_backward_kernel<T, V, K, 512, kCan>>(p, f, parts, smem, ahead, stream)
+                      : launch_rows<norm_backward_kernel<T, V, K, 512, false>>(p, f, parts, smem, ahead, stream);
+      return full ? launch_rows<norm_backward_kernel<T, V, K, 256, kCan>>(p, f, parts, smem, ahead, stream)
+                  : launch_rows<norm_backward_kernel<T, V, K, 256, false>>(p, f, parts, smem, ahead, stream);
     });
   } else {
     const int blocks = row_blocks(p.rows, sms);
