@@ -112,7 +112,9 @@ class MoELM(nn.Module):
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor, states: List[torch.Tensor]) -> torch.Tensor:
-        """One more token ``[S]`` of every sequence: the next token's logits ``[S, V]``; ``states`` go on in place."""
+        """One more token ``[S]`` of every sequence: the next token's logits ``[S, V]``; ``states`` go on in place.  For a model with mixers."""
+        if not self.mixers:
+            raise RuntimeError("step() continues the states of a model with mixers: MoELM(mixer=True)")
         x = torch.nn.functional.embedding(tokens, self.embedding)
         x = self._blocks(x, lambda i, values, gates: gated_scan_step_(states[i], values, gates))
         return torch.nn.functional.linear(x, self.head)

@@ -47,3 +47,10 @@ def test_every_token_is_decoded_where_all_experts_are_chosen(native):
     rows = torch.stack([model.step(tokens[:, t], states) for t in range(60)], 1).float()
     buf.check_status()
     assert float((rows - whole).abs().max()) <= 0.1
+
+
+def test_steps_are_refused_without_mixers(native):
+    buf = make_buffer(None, 64, 128, 2, 4, layers_in_flight=1, world_size=1)
+    model = MoELM(100, 128, 64, 4, 2, 1, buf, device=DEV)
+    with pytest.raises(RuntimeError, match="mixers"):
+        model.step(torch.zeros(3, dtype=torch.int64, device=DEV), model.states(3))
