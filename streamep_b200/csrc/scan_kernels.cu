@@ -88,10 +88,11 @@ template <bool kAny, int V> __device__ __forceinline__ Row<V> fade(const Row<V>&
   for (int i = 0; i < V; ++i) r.f[i] = fade<kAny>(g.f[i], power.f[i], take.f[i]);
   return r;
 }
-template <int V> __device__ __forceinline__ bool finite(const Row<V>& r) {
+// of the first `count` channels (the ring holds anything for those that are not there)
+template <int V> __device__ __forceinline__ bool finite(const Row<V>& r, int count) {
   bool all = true;
 #pragma unroll
-  for (int i = 0; i < V; ++i) all = all && finite(r.f[i]);
+  for (int i = 0; i < V; ++i) all = all && (i >= count || finite(r.f[i]));
   return all;
 }
 // What a run of rows does to the state in front of it: h -> a h + b, or h -> b where a sequence starts within (a is then -0: a state of the sequence
@@ -340,7 +341,7 @@ __device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSpl
     int previous = walk.at(p, kBack ? seg.last : seg.first - 1);
     walk_rows<T, Tl, kBack, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
       const int sequence = walk.at(p, t);
-      if (sequence != previous || sequence < 0) { bad = bad || !finite(b); begin(sequence); }
+      if (sequence != previous || sequence < 0) { bad = bad || !finite(b, seg.count); begin(sequence); }
       if (sequence >= 0) take_row(row, any);
       previous = sequence;
     });
@@ -351,7 +352,7 @@ __device__ __forceinline__ void run_of_segment(const ScanShape& p, const ScanSpl
   } else {
     sequences(std::false_type{});
   }
-  if (bad || !finite(b)) {
+  if (bad || !finite(b, seg.count)) {
     a = Row<V>::all(1.f); lost = b = Row<V>::all(0.f);
     starts = false;
     sequences(std::true_type{});
@@ -533,7 +534,7 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) scan_forward_kernel
     int previous = walk.at(p, seg.first - 1), sequence = walk.at(p, seg.first);
     walk_rows<T, Tl, false, 2>(seg, seg.first, base, stride, [&](int t, Raw<T, V> (&row)[2]) {
       const int behind = walk.at(p, t + 1);
-      if (sequence != previous || sequence < 0) { bad = bad || !finite(h); h = Row<V>::all(0.f); }
+      if (sequence != previous || sequence < 0) { bad = bad || !finite(h, seg.count); h = Row<V>::all(0.f); }
       if (sequence >= 0) {
         if (sequence != previous) begin(sequence);
         step(row, any);
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) scan_forward_kernel
   } else {
     sequences(std::false_type{});
   }
-  if (bad || !finite(h)) {       // again, all of it
+  if (bad || !finite(h, seg.count)) {       // again, all of it
     h = before;
     sequences(std::true_type{});
   }
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
     int behind = walk.at(p, seg.last), sequence = walk.at(p, seg.last - 1);
     auto row_of = [&](int t, auto calculate) {
       const int previous = walk.at(p, t - 1);
-      if (sequence != behind || sequence < 0) bad = bad || !finite(back);
+      if (sequence != behind || sequence < 0) bad = bad || !finite(back, seg.count);
       if (sequence >= 0) {
         if (sequence != behind) begin(sequence);
         calculate(sequence != previous);
@@ -656,7 +657,7 @@ __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const Sc
   } else {
     sequences(std::false_type{});
   }
-  if (bad || !finite(back)) {    // again, all of it
+  if (bad || !finite(back, seg.count)) {    // again, all of it
     back = beyond;
     sequences(std::true_type{});
   }
