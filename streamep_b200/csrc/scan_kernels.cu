@@ -562,7 +562,9 @@ __global__ void __launch_bounds__(kScanThreads, kScanBlocks) scan_forward_kernel
   }
 }
 
-// kGate: with the gate's gradient, for which x and h of the row before are read too.
+// kGate: with the gate's gradient, for which x and h of the row before are read too: h as it was returned, for bf16 rounded by up to 2^-8 of itself (against 64 bits
+// dgate of 8192 rows of 2048 is 1.8e-3 off in 2-norm, where its own rounding is 1.7e-3).  Its fp32 values would be a third array more to write and read; the state that is
+// carried on, and the gradient that is carried back, are fp32.
 template <class T, class Tl, bool kGate>
 __global__ void __launch_bounds__(kScanThreads, 6) scan_backward_kernel(const ScanGradParams p, const ScanSplit s) {
   constexpr int V = Tl::V;
