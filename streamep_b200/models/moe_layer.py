@@ -51,7 +51,8 @@ def make_buffer(group, num_tokens: int, hidden: int, num_topk: int, num_experts:
 class StreamMoE(nn.Module):
     """Router and experts.  ``train_router``: the gate's weight is trained (it is a plain parameter then, replicated over the ranks); a forward
     with gradients leaves its :class:`BalancedRoute` in ``last_route``, whose ``expert_counts`` the program may watch and whose losses it adds to its
-    own by :meth:`router_losses`.  Without gradients the tokens are routed by :func:`router_topk`."""
+    own by :meth:`router_losses`.  Until that is called, or the next forward, it holds the forward's graph; set it to ``None`` before a CUDA graph of the
+    same parameters is captured.  Without gradients the tokens are routed by :func:`router_topk`."""
 
     def __init__(self, hidden: int, ffn: int, num_experts: int, top_k: int, buffer: Buffer, *,
                  streams: Optional[StreamHolder] = None, tile_config: Optional[TileConfig] = None,

@@ -64,6 +64,8 @@ class MoELM(nn.Module):
         self.buffer = buffer
 
     def hidden_states(self, tokens: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        for layer in self.layers:        # (a forward whose losses nobody took has left its graph with them: it must be gone before this one meets the same
+            layer.last_route = None      # parameters, which a captured forward could not share with it)
         x = torch.nn.functional.embedding(tokens.reshape(-1), self.embedding)
         counts = None            # (rows of a packed batch that belong to no sequence are padding, and none of the gates' business)
         if offsets is not None and self.train_router and torch.is_grad_enabled():

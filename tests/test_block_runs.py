@@ -54,3 +54,36 @@ def test_steps_are_refused_without_mixers(native):
     model = MoELM(100, 128, 64, 4, 2, 1, buf, device=DEV)
     with pytest.raises(RuntimeError, match="mixers"):
         model.step(torch.zeros(3, dtype=torch.int64, device=DEV), model.states(3))
+
+
+@pytest.mark.parametrize("before", ["differentiated", "not differentiated", "taken"])
+def test_a_step_is_captured_behind_forwards_whose_losses_nobody_took(native, before):
+    """A sum or per-token losses leave the routers' losses to the program; what they hold of the graph must not meet the captured one."""
+    buf = make_buffer(None, 256, 128, 2, 8, layers_in_flight=2, world_size=1)
+    model = MoELM(500, 128, 64, 8, 2, 2, buf, device=DEV, mixer=True, train_router=True)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x, y = (torch.randint(0, 500, (2, 128), generator=g, device=DEV) for _ in range(2))
+    for _ in range(2):
+        loss = model(x, y, reduction="sum")
+        if before != "not differentiated":
+            (loss + model.router_losses() if before == "taken" else loss).backward()
+        model.zero_grad(set_to_none=True)
+        del loss
+    want = model(x, y)
+    want.backward()
+    eager = [want.detach()] + [p.grad for p in model.parameters()]
+    model.zero_grad(set_to_none=True)
+    del want
+    model(x, y, reduction="sum")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = model(x, y)
+        loss.backward()
+    graph.replay()
+    buf.check_status()
+    # (the layer adds its experts' rows in bf16, in an order of its own)
+    torch.testing.assert_close(loss.detach(), eager[0], rtol=0.01, atol=0.0)
+    for (n, p), e in zip(model.named_parameters(), eager[1:]):
+        a, b = p.grad.float(), e.float()
+        assert float((a - b).norm()) <= 0.05 * float(b.norm()) + 1e-7, n
